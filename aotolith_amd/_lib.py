@@ -119,12 +119,31 @@ SIGNATURES: dict[str, tuple] = {
     "aoto_hip_generic_fill": (_p, ctypes.c_double, ctypes.c_double, _p),
     "aoto_hip_generic_rms_norm": (_p, _p, _p, _c_float, _c_int, _p),
     "aoto_hip_generic_attention": (_p, _p, _p, _p, _p, _c_int, _c_float, _p),
+    "aoto_hip_paged_tables": (
+        _p, _p, _p, _i64, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _c_int, _p, _p, _p, _p, _p, _p, _p, _p,
+    ),
+    "aoto_hip_paged_rope_append": (
+        _p, _i64, _p, _p, _p, _p, _c_int, _p, _p, _i64, _i64, _i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+        _p, _p, _p,
+    ),
+    "aoto_hip_paged_attention_workspace": (
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+    ),
+    "aoto_hip_paged_attention": (
+        _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _c_int, _c_int, _p, _i64, _c_int, _p, _p, _c_int, _c_int, _c_int,
+        _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _p, _p, _p,
+    ),
+    "aoto_hip_verify_draft_workspace": (_c_int, _c_int, _c_int),
+    "aoto_hip_verify_draft": (
+        _p, _c_int, _i64, _c_int, _c_int, _p, _p, _i64, _i64, _p, _p, _p, _c_int, _c_int, _p, _p, _p, _p,
+    ),
 }
 
 #: Entry points returning a size rather than a status.
 SIZE_RETURNING = {"aoto_hip_last_error", "aoto_hip_take_launches", "aoto_hip_decode_attention_workspace",
                   "aoto_hip_w4_gemm_workspace", "aoto_hip_w4_gemm_gate_up_workspace", "aoto_hip_w4_gemm_qkv_rope_workspace",
-                  "aoto_hip_w4_gemv_argmax_keys", "aoto_hip_w4_gemv_finish_max_keys"}
+                  "aoto_hip_w4_gemv_argmax_keys", "aoto_hip_w4_gemv_finish_max_keys",
+                  "aoto_hip_paged_attention_workspace", "aoto_hip_verify_draft_workspace"}
 
 
 class HipBackendUnavailable(RuntimeError):

@@ -155,20 +155,24 @@ void trace_launch(const char* name) {
   }
 }
 
-template <typename... Args>
-int launch(const char* name, dim3 grid, dim3 block, unsigned shared, void* stream, Args... args) {
+int launch_params(const char* name, dim3 grid, dim3 block, unsigned shared, void* stream, void** params) {
   hipFunction_t fn = nullptr;
   if (int s = lookup(name, &fn)) return s;
   if (g_trace == kTraceOnly) {
     trace_launch(name);
     return AOTO_OK;
   }
-  void* params[] = {static_cast<void*>(&args)...};
   hipError_t err = hipModuleLaunchKernel(fn, grid.x, grid.y, grid.z, block.x, block.y, block.z, shared,
                                          static_cast<hipStream_t>(stream), params, nullptr);
   if (err != hipSuccess) return fail(AOTO_ERR_HIP, "launch %s: %s", name, hipGetErrorString(err));
   trace_launch(name);
   return AOTO_OK;
+}
+
+template <typename... Args>
+int launch(const char* name, dim3 grid, dim3 block, unsigned shared, void* stream, Args... args) {
+  void* params[] = {static_cast<void*>(&args)...};
+  return launch_params(name, grid, block, shared, stream, params);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -189,6 +193,16 @@ int cu_count() {
   counts[device] = n;
   return n;
 }
+
+}  // namespace
+
+int aoto::launch_kernel(const char* name, const unsigned grid[3], unsigned block, void* stream, void** params) {
+  return launch_params(name, dim3(grid[0], grid[1], grid[2]), dim3(block), 0, stream, params);
+}
+
+int aoto::device_cu_count() { return cu_count(); }
+
+namespace {
 
 // Persistent GEMV blocks per CU: the shape's own default unless
 // AOTO_GEMV_BLOCKS_PER_CU overrides it (read once).

@@ -16,4 +16,11 @@ void noalloc_prepare_device(int device);
 // (aoto_hip.cpp); other codes pass unchanged.
 void resolve_gemm_codes(int M, int N, int K, int group, bool gate, bool scale_pairs, int* tile, int* splits);
 
+// Look the kernel up in the current device's code object and enqueue it (params: the addresses of its arguments),
+// with the launch trace of aoto_hip_trace_launches.
+int launch_kernel(const char* name, const unsigned grid[3], unsigned block, void* stream, void** params);
+
+// Compute units of the current device (256 where there is none).
+int device_cu_count();
+
 }  // namespace aoto

@@ -16,6 +16,9 @@
 #include "prefill.h"
 #include "flash_attention.h"
 #include "generic_attention.h"
+#include "paged_cache.h"
+#include "paged_attention.h"
+#include "verify.h"
 
 // Marks the code objects whose build chose plans by the present rules (present_rules in aoto_hip.cpp).
 extern "C" __global__ void aoto_plan_rules_3() {}
@@ -222,3 +225,7 @@ AOTO_GENERIC_ATTENTION(f32, true, 64, v, true)
 AOTO_GENERIC_ATTENTION(f32, true, 64, a, false)
 AOTO_GENERIC_ATTENTION(f32, true, 128, v, true)
 AOTO_GENERIC_ATTENTION(f32, true, 128, a, false)
+
+// Verification of drafted tokens: {logits' type} x {statistics, masses, pick}.
+AOTO_VERIFY_INSTANCE(bf16, false)
+AOTO_VERIFY_INSTANCE(f32, true)

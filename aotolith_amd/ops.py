@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -1197,3 +1198,350 @@ def step_advance(step_state: torch.Tensor, capacity: int) -> None:
     _expect(step_state, "step_state", torch.int32, (4,))
     _ready(step_state)
     _lib.check(_lib.library().aoto_hip_step_advance(_ptr(step_state), int(capacity), _stream()))
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# Requests of different lengths over one paged key/value cache: a step's bookkeeping, the cache write, the attention
+# and the verification of drafted tokens. A layer's cache is a pair ``keys, values`` of bf16 ``[pages, Hkv, page, D]``
+# tensors (views with rows of ``D`` contiguous elements will do, a ``[pages, page, Hkv, D]`` cache transposed for one);
+# slot ``s`` is row ``s % page`` of page ``s // page``.
+
+#: Bits raised in the ``error`` tensor of the paged operators (``AOTO_PAGED_*`` in ``include/aoto_hip.h``).
+PAGED_TOKENS_CUT, PAGED_NO_PAGES, PAGED_TABLE_FULL, PAGED_BAD_SLOT, PAGED_BAD_POSITION = 1, 2, 4, 8, 16
+
+
+class PagedStep(NamedTuple):
+    """What :func:`paged_tables` says of a step (``block_tables`` are extended in place)."""
+
+    query_start: torch.Tensor   # int32 [R + 1]: the rows of request r are query_start[r] .. query_start[r + 1]
+    kv_lens: torch.Tensor       # int32 [R]: cached tokens with the step's own
+    positions: torch.Tensor     # int64 [max_tokens]
+    slots: torch.Tensor         # int64 [max_tokens], -1 behind the last token
+    page_counts: torch.Tensor   # int32 [R]
+    free_start: torch.Tensor    # int32 [1]
+
+
+def _on_current(name: str, tensor: torch.Tensor) -> None:
+    """The launch goes to the current device's stream: a tensor of another device would be read across the link, or
+    not at all."""
+
+    if tensor.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {tensor.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _expect_all(device: int, tensors) -> None:
+    """:func:`_expect` for ``(tensor, name, dtype, shape)`` of one call, all of them on ``device``."""
+
+    for tensor, name, dtype, shape in tensors:
+        _expect(tensor, name, dtype, shape)
+        if tensor.get_device() != device:
+            raise ValueError(f"{name} is on {tensor.device}, the call's other tensors on cuda:{device}")
+
+
+def _expect_rows(tensor: torch.Tensor, name: str, dtype: torch.dtype, dims: int, device: int) -> None:
+    """A ``dims``-dimensional operand whose rows (last dimension) are contiguous, at any other strides."""
+
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(tensor).__name__}")
+    if tensor.device.type != "cuda":
+        raise ValueError(f"{name} must be on the GPU, got {tensor.device}")
+    if tensor.get_device() != device:
+        raise ValueError(f"{name} is on {tensor.device}, the call's other tensors on cuda:{device}")
+    if tensor.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {tensor.dtype}")
+    if tensor.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dimensions, got {tuple(tensor.shape)}")
+    if tensor.shape[-1] != 1 and tensor.stride(-1) != 1 and tensor.numel():
+        raise ValueError(f"{name}'s rows must be contiguous")
+
+
+def _expect_pages(keys: torch.Tensor, values: torch.Tensor, device: int) -> tuple[int, int, int, int]:
+    """``(pages, Hkv, page, D)`` of a layer's cache."""
+
+    _expect_rows(keys, "keys", BF16, 4, device)
+    _expect_rows(values, "values", BF16, 4, device)
+    if keys.shape != values.shape or keys.stride() != values.stride():
+        raise ValueError("keys and values must have one shape and the same strides")
+    return tuple(keys.shape)
+
+
+def paged_tables(
+    context_lens: torch.Tensor,
+    new_lens: torch.Tensor,
+    block_tables: torch.Tensor,
+    page_counts: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_start: torch.Tensor,
+    *,
+    page_size: int,
+    max_tokens: int,
+    step: PagedStep | None = None,
+    error: torch.Tensor | None = None,
+) -> PagedStep:
+    """A step's pages, block tables and token maps, built on the GPU from the requests' lengths.
+
+    Request ``r`` has ``context_lens[r]`` cached tokens and gets ``new_lens[r]`` (int32 ``[R]``). Where the
+    ``page_counts[r]`` pages of its row of ``block_tables`` (int32 ``[R, max_blocks]``) do not hold them all, the next
+    pages of ``free_pages[free_start:]`` (int32) are entered there, requests in order; a request keeps pages that it
+    does not need yet (drafted tokens that did not stand leave some). Token ``i`` of request ``r`` is row
+    ``query_start[r] + i`` of the step, at position ``context_lens[r] + i``, in slot
+    ``block_tables[r][position // page_size] * page_size + position % page_size``; rows from the last token to
+    ``max_tokens`` have position 0 and slot -1.
+
+    ``step`` gives the tensors to write (a captured step replays into them); its ``page_counts`` and ``free_start``
+    may be the ones passed in. ``error`` (int32 ``[1]``) collects ``PAGED_TOKENS_CUT`` (more tokens than
+    ``max_tokens``: the last are left out), ``PAGED_NO_PAGES`` (the free list ran out: table entries and slots of -1)
+    and ``PAGED_TABLE_FULL`` (a request longer than its row: slots of -1).
+    """
+
+    _expect(context_lens, "context_lens", torch.int32)
+    device = context_lens.get_device()
+    _on_current("context_lens", context_lens)
+    requests = context_lens.numel()
+    max_tokens = int(max_tokens)
+    _expect_all(device, (
+        (context_lens, "context_lens", torch.int32, (requests,)), (new_lens, "new_lens", torch.int32, (requests,)),
+        (page_counts, "page_counts", torch.int32, (requests,)), (free_pages, "free_pages", torch.int32, None),
+        (free_start, "free_start", torch.int32, (1,)),
+    ))
+    _expect_rows(block_tables, "block_tables", torch.int32, 2, device)
+    if block_tables.shape[0] != requests:
+        raise ValueError(f"block_tables must have {requests} rows, got {block_tables.shape[0]}")
+    if error is not None:
+        _expect_all(device, ((error, "error", torch.int32, (1,)),))
+    if max_tokens < 0:
+        raise ValueError(f"max_tokens must not be negative, got {max_tokens}")
+    if step is None:
+        where = context_lens.device
+        lens = torch.empty((3 * requests + 2,), dtype=torch.int32, device=where)
+        maps = torch.empty((2, max_tokens), dtype=torch.int64, device=where)
+        start, kv, counts, first = lens.split((requests + 1, requests, requests, 1))
+        step = PagedStep(start, kv, maps[0], maps[1], counts, first)
+    else:
+        _expect_all(device, (
+            (step.query_start, "step.query_start", torch.int32, (requests + 1,)),
+            (step.kv_lens, "step.kv_lens", torch.int32, (requests,)),
+            (step.positions, "step.positions", torch.int64, (max_tokens,)),
+            (step.slots, "step.slots", torch.int64, (max_tokens,)),
+            (step.page_counts, "step.page_counts", torch.int32, (requests,)),
+            (step.free_start, "step.free_start", torch.int32, (1,)),
+        ))
+    _ready(context_lens)
+    _lib.check(
+        _lib.library().aoto_hip_paged_tables(
+            _ptr(context_lens), _ptr(new_lens), _ptr(block_tables), block_tables.stride(0), _ptr(page_counts),
+            _ptr(free_pages), _ptr(free_start), requests, block_tables.shape[1], free_pages.numel(), int(page_size),
+            max_tokens, _ptr(step.query_start), _ptr(step.kv_lens), _ptr(step.positions), _ptr(step.slots),
+            _ptr(step.page_counts), _ptr(step.free_start), _ptr(error), _stream(),
+        )
+    )
+    return step
+
+
+def paged_rope_append(
+    qkv: torch.Tensor,
+    positions: torch.Tensor,
+    slots: torch.Tensor,
+    cos_table: torch.Tensor,
+    sin_table: torch.Tensor,
+    keys: torch.Tensor,
+    values: torch.Tensor,
+    *,
+    query_heads: int,
+    q_out: torch.Tensor | None = None,
+    error: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """RoPE of a step's ``qkv [T, (Hq + 2 Hkv) D]`` rows and the write of one layer's cache: returns ``q [T, Hq, D]``.
+
+    Row ``t`` is rotated by row ``positions[t]`` of the tables (bf16 ``[P, D]``), its key and value go to slot
+    ``slots[t]`` of ``keys``, ``values`` (int64 ``[T]`` both). A row of slot -1 (behind the step's last token) writes
+    nothing, its query included; so does one whose slot or position is out of range, which raises ``PAGED_BAD_SLOT``
+    or ``PAGED_BAD_POSITION`` in ``error`` (int32 ``[1]``). Slots other than -1 must not repeat within a call.
+    """
+
+    _expect(positions, "positions", torch.int64)
+    _on_current("positions", positions)
+    device = positions.get_device()
+    _expect_rows(qkv, "qkv", BF16, 2, device)
+    pages, kv_heads, page, dim = _expect_pages(keys, values, device)
+    tokens, width = qkv.shape
+    query_heads = int(query_heads)
+    if query_heads <= 0 or width != (query_heads + 2 * kv_heads) * dim:
+        raise ValueError(f"qkv rows of {width} do not hold {query_heads} + 2 x {kv_heads} heads of {dim}")
+    _expect(cos_table, "cos_table", BF16)
+    if cos_table.dim() != 2 or cos_table.shape[1] != dim:
+        raise ValueError(f"cos_table must be [P, {dim}], got {tuple(cos_table.shape)}")
+    _expect_all(device, (
+        (positions, "positions", torch.int64, (tokens,)), (slots, "slots", torch.int64, (tokens,)),
+        (cos_table, "cos_table", BF16, None), (sin_table, "sin_table", BF16, tuple(cos_table.shape)),
+    ))
+    if error is not None:
+        _expect_all(device, ((error, "error", torch.int32, (1,)),))
+    if q_out is None:
+        q_out = torch.empty((tokens, query_heads, dim), dtype=BF16, device=qkv.device)
+    else:
+        _expect_all(device, ((q_out, "q_out", BF16, (tokens, query_heads, dim)),))
+    _ready(qkv)
+    _lib.check(
+        _lib.library().aoto_hip_paged_rope_append(
+            _ptr(qkv), qkv.stride(0), _ptr(positions), _ptr(slots), _ptr(cos_table), _ptr(sin_table),
+            cos_table.shape[0], _ptr(keys), _ptr(values), keys.stride(0), keys.stride(1), keys.stride(2), pages, page,
+            tokens, query_heads, kv_heads, dim, _ptr(q_out), _ptr(error), _stream(),
+        )
+    )
+    return q_out
+
+
+def paged_attention_workspace(tokens: int, requests: int, max_blocks: int, page_size: int, query_heads: int,
+                              kv_heads: int, head_dim: int, *, max_query_len: int = 0, max_kv_len: int = 0,
+                              device=None) -> torch.Tensor:
+    """A workspace for :func:`paged_attention` with these shapes and bounds (on ``device``; a GPU's, and torch's
+    default device is the host unless a program sets it)."""
+
+    size = _lib.library().aoto_hip_paged_attention_workspace(
+        int(tokens), int(requests), int(max_blocks), int(page_size), int(query_heads), int(kv_heads), int(head_dim),
+        int(max_query_len), int(max_kv_len))
+    return torch.empty((max(size, 16),), dtype=torch.uint8, device=device)
+
+
+def paged_attention(
+    q: torch.Tensor,
+    keys: torch.Tensor,
+    values: torch.Tensor,
+    block_tables: torch.Tensor,
+    query_start: torch.Tensor,
+    kv_lens: torch.Tensor,
+    *,
+    causal: bool = True,
+    scale: float | None = None,
+    max_query_len: int = 0,
+    max_kv_len: int = 0,
+    workspace: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """GQA attention of the requests' new tokens ``q [T, Hq, D]`` over their pages -> ``[T, Hq * D]``.
+
+    Request ``r`` has the rows ``query_start[r] .. query_start[r + 1]`` (int32 ``[R + 1]``) and ``kv_lens[r]`` keys
+    (int32 ``[R]``), its own new ones among them, in the pages that ``block_tables[r]`` (int32 ``[R, max_blocks]``)
+    names: one token, a few drafted ones or a chunk of a prompt, side by side. Row ``i`` of ``n`` sees the keys up to
+    its own, ``j <= kv_lens[r] - n + i`` (all of them with ``causal=False``); keys past the block table row or in
+    entries that name no page are not there, and a row that sees none gives 0. Rows from ``query_start[R]`` on keep
+    what ``out`` held. The lengths are read on the GPU; ``max_query_len`` and ``max_kv_len`` (0: not known) are the
+    caller's bounds on a request's rows and keys, which choose the launch and never the result.
+    """
+
+    _expect_rows(q, "q", BF16, 3, q.get_device() if isinstance(q, torch.Tensor) else 0)
+    _on_current("q", q)
+    device = q.get_device()
+    tokens, query_heads, dim = q.shape
+    pages, kv_heads, page, key_dim = _expect_pages(keys, values, device)
+    if key_dim != dim:
+        raise ValueError(f"q heads have {dim} elements, the cache's {key_dim}")
+    _expect_rows(block_tables, "block_tables", torch.int32, 2, device)
+    requests, max_blocks = block_tables.shape
+    _expect_all(device, ((query_start, "query_start", torch.int32, (requests + 1,)),
+                         (kv_lens, "kv_lens", torch.int32, (requests,))))
+    if scale is None:
+        scale = ctypes.c_float(dim ** -0.5).value
+    if out is None:
+        out = torch.empty((tokens, query_heads * dim), dtype=BF16, device=q.device)
+    else:
+        _expect_all(device, ((out, "out", BF16, (tokens, query_heads * dim)),))
+    _ready(q)
+    lib = _lib.library()
+    max_query_len, max_kv_len = int(max_query_len), int(max_kv_len)
+    need = lib.aoto_hip_paged_attention_workspace(tokens, requests, max_blocks, page, query_heads, kv_heads, dim,
+                                                  max_query_len, max_kv_len)
+    if workspace is not None:
+        _on_device(workspace)
+        if workspace.get_device() != device:
+            raise ValueError(f"the workspace is on {workspace.device}, the call's other tensors on cuda:{device}")
+        if not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+            workspace = None
+    if need and workspace is None:
+        workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
+    _lib.check(
+        lib.aoto_hip_paged_attention(
+            _ptr(q), q.stride(0), q.stride(1), _ptr(keys), _ptr(values), keys.stride(0), keys.stride(1),
+            keys.stride(2), pages, page, _ptr(block_tables), block_tables.stride(0), max_blocks, _ptr(query_start),
+            _ptr(kv_lens), tokens, requests, query_heads, kv_heads, dim, int(bool(causal)), float(scale),
+            max_query_len, max_kv_len, _ptr(workspace if need else None), _ptr(out), _stream(),
+        )
+    )
+    return out
+
+
+def verify_draft(
+    logits: torch.Tensor,
+    draft_tokens: torch.Tensor,
+    query_start: torch.Tensor,
+    uniforms: torch.Tensor,
+    *,
+    draft_logits: torch.Tensor | None = None,
+    temperature: torch.Tensor | None = None,
+    tokens: torch.Tensor | None = None,
+    accepted: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Drafted tokens against the target's logits: ``(tokens [R, K + 1] int64, accepted [R] int32)``.
+
+    Rows ``query_start[r] .. query_start[r + 1]`` of ``logits [T, V]`` (bf16 or f32) judge the first drafts of
+    ``draft_tokens[r]`` (int64 ``[R, K]``, ``K <= 62``) one row each; the last row follows them all (no drafts: plain
+    sampling). With ``p`` the softmax of a row at ``temperature[r]`` (f32 ``[R]``), ``q`` that of its draft's
+    ``draft_logits[r, i]`` (``[R, K, V]`` of the logits' type; None: the draft is certain) and ``u = uniforms[r]``
+    (f32 ``[R, K + 1]`` in [0, 1)), draft ``x`` stands while ``u[i] * q[x] < p[x]``. The token after those that stand
+    is drawn with ``u[K]`` from ``max(p - q, 0)`` of the first that fell, or from the last row's ``p``: the first one
+    at which the running sum of weights is above ``u[K]`` times their total. At a temperature of 0 (and everywhere
+    with ``temperature=None``) a draft stands where it is the row's first maximum, which is also the token that
+    follows. ``tokens`` holds the drafts that stand, the token that follows them and -1 behind it; ``accepted`` counts
+    the former. A request without rows gets -1 throughout. Everything is summed in 64 bits.
+    """
+
+    dtype = logits.dtype if isinstance(logits, torch.Tensor) else BF16
+    if dtype not in (BF16, torch.float32):
+        raise TypeError(f"logits must be bf16 or f32, got {dtype}")
+    _expect_rows(logits, "logits", dtype, 2, logits.get_device() if isinstance(logits, torch.Tensor) else 0)
+    _on_current("logits", logits)
+    device = logits.get_device()
+    rows, vocab = logits.shape
+    _expect(draft_tokens, "draft_tokens", torch.int64)
+    if draft_tokens.dim() != 2:
+        raise ValueError(f"draft_tokens must be [R, K], got {tuple(draft_tokens.shape)}")
+    requests, drafts = draft_tokens.shape
+    _expect_all(device, ((draft_tokens, "draft_tokens", torch.int64, (requests, drafts)),
+                         (query_start, "query_start", torch.int32, (requests + 1,)),
+                         (uniforms, "uniforms", torch.float32, (requests, drafts + 1))))
+    if temperature is not None:
+        _expect_all(device, ((temperature, "temperature", torch.float32, (requests,)),))
+    if draft_logits is not None:
+        _expect_rows(draft_logits, "draft_logits", dtype, 3, device)
+        if tuple(draft_logits.shape) != (requests, drafts, vocab):
+            raise ValueError(f"draft_logits must be {(requests, drafts, vocab)}, got {tuple(draft_logits.shape)}")
+    if tokens is None:
+        tokens = torch.empty((requests, drafts + 1), dtype=torch.int64, device=logits.device)
+    else:
+        _expect_all(device, ((tokens, "tokens", torch.int64, (requests, drafts + 1)),))
+    if accepted is None:
+        accepted = torch.empty((requests,), dtype=torch.int32, device=logits.device)
+    else:
+        _expect_all(device, ((accepted, "accepted", torch.int32, (requests,)),))
+    _ready(logits)
+    lib = _lib.library()
+    need = lib.aoto_hip_verify_draft_workspace(requests, drafts, vocab)
+    if workspace is not None:
+        _on_device(workspace)
+        if workspace.get_device() != device:
+            raise ValueError(f"the workspace is on {workspace.device}, the call's other tensors on cuda:{device}")
+        if not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+            workspace = None
+    if workspace is None:
+        workspace = torch.empty((need,), dtype=torch.uint8, device=logits.device)
+    _lib.check(
+        lib.aoto_hip_verify_draft(
+            _ptr(logits), int(dtype is torch.float32), logits.stride(0), rows, vocab, _ptr(draft_tokens),
+            _ptr(draft_logits), 0 if draft_logits is None else draft_logits.stride(0),
+            0 if draft_logits is None else draft_logits.stride(1), _ptr(query_start), _ptr(uniforms),
+            _ptr(temperature), requests, drafts, _ptr(workspace), _ptr(tokens), _ptr(accepted), _stream(),
+        )
+    )
+    return tokens, accepted

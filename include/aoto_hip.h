@@ -588,6 +588,85 @@ int aoto_hip_generic_attention(const aoto_tensor* out, const aoto_tensor* q, con
                                const aoto_tensor* v, const aoto_tensor* mask, int causal, float scale,
                                void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Requests of different lengths over one paged key/value cache. No counterpart in the reference, whose cache is one
+ * static window per sequence (models/decoder.py:554-561); these four serve a step of many requests.
+ *
+ * Cache of a layer: keys and values bf16, element (page p, head h, slot s, dim d) at
+ * p * page_stride + h * head_stride + s * slot_stride + d (elements; the strides multiples of 8, the bases 16-byte
+ * aligned). Slot number s names row s % page of page s / page. Lengths, tables and maps are device memory: a captured
+ * step replays with whatever lengths they hold by then. Calls that share a workspace must be ordered on one stream. */
+
+/* Bits that the paged entry points raise in their `error` (an int32 in device memory, or NULL). */
+#define AOTO_PAGED_TOKENS_CUT 1   /* more new tokens than max_tokens: those past it were left out */
+#define AOTO_PAGED_NO_PAGES 2     /* the free list ran out: entries of -1, slots of -1 */
+#define AOTO_PAGED_TABLE_FULL 4   /* a request longer than its block table row: slots of -1 past it */
+#define AOTO_PAGED_BAD_SLOT 8     /* a slot outside the cache and not -1: nothing written for that row */
+#define AOTO_PAGED_BAD_POSITION 16 /* a position outside the RoPE tables: nothing written for that row */
+
+/* A step's pages, block tables and token maps from the requests' lengths. Request r has context_lens[r] cached tokens
+ * (negative ones count as 0, ones past 2^30 as 2^30) and gets new_lens[r] more (negative: 0); its row of block_tables
+ * ([requests, max_blocks] int32, rows table_stride apart) holds page_counts[r] pages.
+ *   query_start[r]   sum of the new tokens before r (requests + 1 entries), none past max_tokens
+ *   kv_lens[r]       context_lens[r] + its new tokens
+ *   page_counts_out  max(page_counts[r], ceil(kv_lens[r] / page)); the pages added are the next ones of
+ *                    free_pages[free_start ..), requests in order, and are entered in block_tables in place
+ *   free_start_out   free_start + the pages taken
+ *   positions, slots int64 [max_tokens]: token i of request r has position context_lens[r] + i and the slot
+ *                    block_tables[r][position / page] * page + position % page; 0 and -1 behind the last token
+ * page_counts_out and free_start_out may be the arrays they are computed from. */
+int aoto_hip_paged_tables(const int32_t* context_lens, const int32_t* new_lens, int32_t* block_tables,
+                          int64_t table_stride, const int32_t* page_counts, const int32_t* free_pages,
+                          const int32_t* free_start, int requests, int max_blocks, int free_count, int page,
+                          int max_tokens, int32_t* query_start, int32_t* kv_lens, int64_t* positions, int64_t* slots,
+                          int32_t* page_counts_out, int32_t* free_start_out, int32_t* error, void* stream);
+
+/* RoPE and cache write of one layer's projection rows qkv (rows row_stride apart: Hq query heads, Hkv key heads, Hkv
+ * value heads of head_dim): q_out [tokens, Hq, head_dim] and the keys rotated by row positions[t] of the tables
+ * ([table_rows, head_dim] bf16) as aoto_hip_rope_qkv_prefill does, keys and values into slot slots[t] of the cache.
+ * A row whose slot or position is out of range (slot -1 without an error) writes nothing, its query included. The
+ * slots of a call are distinct, -1 apart. head_dim a multiple of 16. */
+int aoto_hip_paged_rope_append(const void* qkv, int64_t row_stride, const int64_t* positions, const int64_t* slots,
+                               const void* cos_table, const void* sin_table, int table_rows, void* keys, void* values,
+                               int64_t page_stride, int64_t head_stride, int64_t slot_stride, int pages, int page,
+                               int tokens, int query_heads, int kv_heads, int head_dim, void* q_out, int32_t* error,
+                               void* stream);
+
+/* Attention of the requests' new tokens over their pages: request r's rows are query_start[r] .. query_start[r + 1]
+ * of q (strides in elements, multiples of 8) and of out [tokens, Hq * head_dim]; row i of n sees the keys
+ * j < kv_lens[r] - n + i + 1 (causal) or j < kv_lens[r], as far as its block table reaches and names pages of the
+ * cache. A row that sees none gives 0; rows from query_start[requests] on keep what they held. head_dim 64 or 128.
+ * max_query_len and max_kv_len (0: not known) are the caller's bounds on a request's rows and keys; they choose the
+ * launch and never the result. workspace: aoto_hip_paged_attention_workspace() bytes for the same arguments. */
+size_t aoto_hip_paged_attention_workspace(int tokens, int requests, int max_blocks, int page, int query_heads,
+                                          int kv_heads, int head_dim, int max_query_len, int max_kv_len);
+int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* keys,
+                             const void* values, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                             int pages, int page, const int32_t* block_tables, int64_t table_stride, int max_blocks,
+                             const int32_t* query_start, const int32_t* kv_lens, int tokens, int requests,
+                             int query_heads, int kv_heads, int head_dim, int causal, float scale, int max_query_len,
+                             int max_kv_len, void* workspace, void* out, void* stream);
+
+/* Drafted tokens against the target: request r's rows query_start[r] .. query_start[r + 1] of logits [rows, vocab]
+ * (bf16, or f32 with logits_f32; row_stride in elements) judge its drafts draft_tokens[r][i] one row each, the last
+ * row following them all (n rows: n - 1 drafts, at most `drafts`, at most 62). With p = softmax(logits / T) of the
+ * row, q the softmax of its draft logits at the same T (element (r, i, v) at r * draft_request_stride +
+ * i * draft_row_stride + v, the logits' type) or, where draft_logits is NULL, a point mass on the draft, and
+ * u = uniforms[r] (f32 [drafts + 1] in [0, 1)): draft i stands while u_i q(x_i) < p(x_i); the token after the last
+ * that stands is drawn with u_drafts from max(p - q, 0) where a draft fell (from p where that is 0 throughout), else
+ * from the last row's p: the first token whose running sum of weights is above u times their total. T =
+ * temperature[r]; where it is not above 0, and everywhere with temperature NULL, a draft stands where it is the row's
+ * first maximum, which is also the token that follows. NaN logits count as -inf; a row of nothing else judges no
+ * draft true and is followed by token 0; the logits equal to an infinite maximum share its law. Sums and exponentials in f64.
+ * tokens_out int64 [requests, drafts + 1]: the drafts that stand, the token that follows, -1 behind it (-1 throughout
+ * for a request without rows); accepted int32 [requests]: how many stand. */
+size_t aoto_hip_verify_draft_workspace(int requests, int drafts, int vocab);
+int aoto_hip_verify_draft(const void* logits, int logits_f32, int64_t row_stride, int rows, int vocab,
+                          const int64_t* draft_tokens, const void* draft_logits, int64_t draft_request_stride,
+                          int64_t draft_row_stride, const int32_t* query_start, const float* uniforms,
+                          const float* temperature, int requests, int drafts, void* workspace, int64_t* tokens_out,
+                          int32_t* accepted, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
