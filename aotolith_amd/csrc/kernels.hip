@@ -226,6 +226,10 @@ AOTO_GENERIC_ATTENTION(f32, true, 64, a, false)
 AOTO_GENERIC_ATTENTION(f32, true, 128, v, true)
 AOTO_GENERIC_ATTENTION(f32, true, 128, a, false)
 
+// Attention over a paged cache: head dim x {narrow tiles of 16 and 32 rows, wide tiles beside narrow ones, join}.
+AOTO_PAGED_ATTENTION(64)
+AOTO_PAGED_ATTENTION(128)
+
 // Verification of drafted tokens: {logits' type} x {statistics, masses, pick}.
 AOTO_VERIFY_INSTANCE(bf16, false)
 AOTO_VERIFY_INSTANCE(f32, true)

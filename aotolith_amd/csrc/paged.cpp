@@ -1,6 +1,8 @@
 // Host side of the C ABI's paged-cache entry points (include/aoto_hip.h): checks, launch choices, launches.
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
+#include <cstdio>
 
 #include "aoto_hip.h"
 #include "internal.h"
@@ -28,6 +30,40 @@ int check_pages(const char* what, const void* keys, const void* values, int64_t 
   if (!aligned(keys, 16) || !aligned(values, 16) || page_stride % 8 || head_stride % 8 || slot_stride % 8)
     return set_error(AOTO_ERR_ARGUMENT, "%s: keys/values 16-byte aligned with strides of multiples of 8", what);
   return AOTO_OK;
+}
+
+// Rows of a wide tile of the attention, and keys (in 128) below which a request's keys are not split.
+constexpr int kWideRows = 256;
+constexpr int kLeastChunk = 2;
+
+struct AttentionPlan {
+  bool wide;          // chunks of prompts may be among the requests: the instance with wide tiles
+  int narrow_rows;    // rows of a narrow tile (16 or 32)
+  int target;         // units a kv head that the keys are split to make, 0 where they are not
+  long long units;    // at most, a kv head
+  size_t workspace;
+};
+
+// From what the host knows: shapes and the caller's bounds. The lengths are on the GPU.
+AttentionPlan attention_plan(int tokens, int requests, int max_blocks, int page, int query_heads, int kv_heads,
+                             int head_dim, int max_query_len, int max_kv_len) {
+  const int group = query_heads / kv_heads;
+  const long long rows = (long long)(max_query_len ? std::min(max_query_len, tokens) : tokens) * group;
+  AttentionPlan p{};
+  p.wide = rows > 32;
+  p.narrow_rows = p.wide || rows <= 16 ? 16 : 32;
+  const int tile = (p.wide ? kWideRows : p.narrow_rows) / group;
+  const long long some = std::min(requests, tokens);
+  p.units = some + (tokens - some) / std::max(tile, 1);
+  long long keys = std::min<long long>((long long)max_blocks * page, 1 << 30);
+  if (max_kv_len) keys = std::min<long long>(keys, max_kv_len);
+  const long long blocks = p.units * kv_heads, full = (long long)aoto::device_cu_count() * (p.wide ? 2 : 4);
+  if (keys > kLeastChunk * 128 && blocks < full) p.target = (int)((full + kv_heads - 1) / kv_heads);
+  p.units += p.target;
+  if (p.target)
+    p.workspace = (size_t)tokens * 16 + (size_t)p.units * kv_heads * (p.wide ? kWideRows : p.narrow_rows) *
+                                            (head_dim + 2) * sizeof(float);
+  return p;
 }
 
 // Tokens up to which the tables' one block writes the maps itself: a second launch costs more than it saves.
@@ -92,7 +128,11 @@ int aoto_hip_paged_rope_append(const void* qkv, int64_t row_stride, const int64_
 
 size_t aoto_hip_paged_attention_workspace(int tokens, int requests, int max_blocks, int page, int query_heads,
                                           int kv_heads, int head_dim, int max_query_len, int max_kv_len) {
-  return 0;
+  if (tokens <= 0 || requests <= 0 || max_blocks <= 0 || page <= 0 || query_heads <= 0 || kv_heads <= 0 ||
+      query_heads % kv_heads || head_dim <= 0 || max_query_len < 0 || max_kv_len < 0)
+    return 0;
+  return attention_plan(tokens, requests, max_blocks, page, query_heads, kv_heads, head_dim, max_query_len, max_kv_len)
+      .workspace;
 }
 
 int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* keys,
@@ -111,16 +151,39 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention: head_dim %d (64 or 128)", head_dim);
   if (!aligned(q, 16) || q_token_stride % 8 || q_head_stride % 8 || !aligned(out, 16))
     return set_error(AOTO_ERR_ARGUMENT, "paged_attention: q and out 16-byte aligned, strides of multiples of 8");
+  if (!(scale > 0.f) || !std::isfinite(scale))
+    return set_error(AOTO_ERR_ARGUMENT, "paged_attention: scale %g is not a positive number", (double)scale);
+  if (query_heads / kv_heads > kWideRows)
+    return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention: %d query heads a kv head (at most %d)",
+                     query_heads / kv_heads, kWideRows);
+  const AttentionPlan plan = attention_plan(tokens, requests, max_blocks, page, query_heads, kv_heads, head_dim,
+                                            max_query_len, max_kv_len);
+  if (plan.workspace && (!workspace || !aligned(workspace, 16)))
+    return set_error(AOTO_ERR_ARGUMENT, "paged_attention: needs a 16-byte aligned workspace of %zu bytes", plan.workspace);
   PagedAttentionArgs a{};
   a.q = static_cast<const uint16_t*>(q), a.keys = static_cast<const uint16_t*>(keys);
   a.values = static_cast<const uint16_t*>(values), a.block_tables = block_tables, a.query_start = query_start;
   a.kv_lens = kv_lens, a.out = static_cast<uint16_t*>(out), a.q_token_stride = q_token_stride;
   a.q_head_stride = q_head_stride, a.page_stride = page_stride, a.head_stride = head_stride;
   a.slot_stride = slot_stride, a.table_stride = table_stride, a.tokens = tokens, a.requests = requests;
-  a.pages = pages, a.page = page, a.max_blocks = max_blocks, a.query_heads = query_heads, a.kv_heads = kv_heads;
-  a.causal = causal, a.scale = scale;
-  return launch(head_dim == 64 ? "aoto_paged_attention_d64" : "aoto_paged_attention_d128",
-                (long long)tokens * query_heads, 1, 64, stream, a);
+  a.pages = pages, a.page = page, a.query_heads = query_heads, a.kv_heads = kv_heads;
+  a.causal = causal != 0, a.scale = scale;
+  a.table_keys = (int)std::min<long long>((long long)max_blocks * page, 1 << 30);
+  unsigned log2 = 0;
+  while ((1u << log2) < (unsigned)page) ++log2;
+  a.page_magic = (unsigned)(((1ull << (31 + log2)) + page - 1) / page), a.page_shift = log2 ? log2 - 1 : 0;
+  a.narrow_tokens = plan.narrow_rows / (query_heads / kv_heads);
+  a.wide_tokens = kWideRows / (query_heads / kv_heads);
+  a.target = plan.target, a.least_chunk = kLeastChunk, a.record_rows = plan.wide ? kWideRows : plan.narrow_rows;
+  a.joins = static_cast<int*>(workspace);
+  a.records = reinterpret_cast<float*>(static_cast<char*>(workspace) + (size_t)tokens * 16);
+  char name[64];
+  snprintf(name, sizeof(name), "aoto_paged_attention_d%d_%s", head_dim,
+           plan.wide ? "w" : plan.narrow_rows == 16 ? "n1" : "n2");
+  if (int s = launch(name, plan.units * kv_heads, 1, 256, stream, a)) return s;
+  if (!plan.target) return AOTO_OK;
+  return launch(head_dim == 64 ? "aoto_paged_attention_join_d64" : "aoto_paged_attention_join_d128",
+                ((long long)tokens * query_heads + 3) / 4, 1, 256, stream, a);
 }
 
 size_t aoto_hip_verify_draft_workspace(int requests, int drafts, int vocab) {

@@ -51,7 +51,13 @@ struct PagedAttentionArgs {
   float* records;   // partial results of requests whose keys are split over blocks
   int* joins;       // per token: where its records begin and how many there are
   long long q_token_stride, q_head_stride, page_stride, head_stride, slot_stride, table_stride;
-  int tokens, requests, pages, page, max_blocks, query_heads, kv_heads, causal;
+  int tokens, requests, pages, page, query_heads, kv_heads, causal;
+  int table_keys;      // max_blocks * page, at most 2^30
+  unsigned page_magic, page_shift;  // key / page = (key * page_magic) >> 32 >> page_shift for keys below 2^31
+  int narrow_tokens, wide_tokens;   // of a request, that a tile of 16 NT / 256 rows holds
+  int target;          // units a kv head that the keys are split to make; 0: not split
+  int least_chunk;     // in 128 keys
+  int record_rows;     // rows of a unit's record
   float scale;
 };
 

@@ -4,90 +4,710 @@
 // over the keys j of token t's request r that it may see: with n_r = query_start[r + 1] - query_start[r] rows and
 // kv_r keys, row i sees j < kv_r - n_r + i + 1 (causal) or j < kv_r, as far as the block table row goes and where its
 // entry names a page of the cache; a row that sees none gives 0. Key j of head h / (Hq / Hkv) is row j % page of page
-// block_tables[r][j / page]. Scores, maxima and sums in f32.
+// block_tables[r][j / page]. Scores, maxima and sums in f32, one pass over the keys with a running maximum; P is
+// rounded to bf16 for its product (as the prefill attention does: the matrix instructions take two operands of one
+// type), its sum is not.
+//
+// Work is cut on the GPU, from the lengths as they are there: a unit is one tile of a request's rows (all query heads
+// of a kv head that share its keys, token after token) against one chunk of its keys. Every block finds its unit by
+// two sums over the requests; the chunk is the size at which the units of the whole call make about `target` blocks a
+// kv head, so that requests of very different lengths still end together. A tile whose keys make several chunks
+// leaves records (maximum, sum, unnormalized row) that aoto_paged_attention_join_* combines.
+//   narrow tiles (16 NT rows, decodes and drafted tokens): the four waves take 32 keys each of every 128; K goes
+//     straight from the pages to operand registers, V through the wave's own LDS; no barrier in the loop
+//   wide tiles (256 rows, chunks of prompts): the four waves take 64 rows each, 64-key tiles of K and V staged once
+//     for all of them
 #pragma once
 
 #include "common.h"
+#include "flash_attention.h"
 #include "paged_args.h"
 
 namespace aoto {
 
-// The request that owns token t (t < query_start[requests]): the last r with query_start[r] <= t, found 64 ways a
-// step. All lanes of the wave call it with the same t.
-AOTO_DEVICE int paged_request(const int* __restrict__ query_start, int requests, int t) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, hi = requests;  // the answer is in [lo, hi)
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 63) / 64;
-    const int at = lo + lane * step;
-    const unsigned long long below = __ballot(at < hi && query_start[min(at, requests)] <= t);
-    const int last = below ? 63 - __clzll((long long)below) : 0;
-    lo += last * step;
-    hi = min(hi, lo + step);
+typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
+typedef short pa_s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) pa_s16x4 pa_lds_s16x4;
+
+constexpr int kPagedUnitKeys = 128;  // keys that chunks are counted in
+constexpr int kPagedWideRows = 256;
+
+struct PagedUnit {
+  int request, begin, rows;  // its first row and how many
+  int keys;                  // its keys, as far as the block table reaches
+  int first;                 // key index of the first row's own key, plus one (causal), of all rows otherwise
+  int token, tokens;         // of the request: the tile's first and count
+  int chunk, split, splits;  // in kPagedUnitKeys
+  int record;                // index of the tile's first unit
+  bool narrow;
+};
+
+struct PagedRequest {
+  int begin, rows, keys, tiles, tokens, blocks;  // tokens a tile; blocks of kPagedUnitKeys keys
+  bool narrow;
+};
+
+template <bool MIXED>
+AOTO_DEVICE PagedRequest paged_request(const PagedAttentionArgs& a, int r) {
+  PagedRequest q;
+  q.begin = min(max(a.query_start[r], 0), a.tokens);
+  q.rows = min(max(a.query_start[r + 1], q.begin), a.tokens) - q.begin;
+  q.keys = min(max(a.kv_lens[r], 0), a.table_keys);
+  q.narrow = !MIXED || q.rows <= a.narrow_tokens;
+  q.tokens = max(1, q.narrow ? a.narrow_tokens : a.wide_tokens);  // more than 16 heads: only rowless ones are narrow
+  q.tiles = (q.rows + q.tokens - 1) / q.tokens;
+  q.blocks = max(1, (q.keys + kPagedUnitKeys - 1) / kPagedUnitKeys);
+  return q;
+}
+
+// The block's unit; false where there is none left. 256 threads, all of them.
+template <bool MIXED>
+AOTO_DEVICE bool paged_unit(const PagedAttentionArgs& a, int u, PagedUnit& unit) {
+  __shared__ double s_work[4];
+  __shared__ int s_units[4];
+  __shared__ PagedUnit s_unit;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = (a.requests + 255) / 256;
+  const int lo = min(tid * per, a.requests), hi = min(lo + per, a.requests);
+  int chunk = 1 << 23;  // whole: at most 2^30 keys
+  PagedRequest q{};
+  if (a.target > 0) {
+    double work = 0.0;
+    for (int r = lo; r < hi; ++r) {
+      q = paged_request<MIXED>(a, r);
+      work += (double)q.tiles * q.blocks;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) work += __shfl_xor(work, d);
+    if (lane == 0) s_work[wave] = work;
+    __syncthreads();
+    work = s_work[0] + s_work[1] + s_work[2] + s_work[3];
+    chunk = max(a.least_chunk, (int)ceil(work / a.target));
   }
-  return lo;
+  int units = 0;
+  for (int r = lo; r < hi; ++r) {
+    if (per > 1 || a.target <= 0) q = paged_request<MIXED>(a, r);
+    units += q.tiles * ((q.blocks + chunk - 1) / chunk);
+  }
+  int upto = units;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(upto, d);
+    if (lane >= d) upto += up;
+  }
+  if (lane == 63) s_units[wave] = upto;
+  if (tid == 0) s_unit.request = -1;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) upto += s_units[w];
+  if (u < upto && u >= upto - units) {
+    int before = upto - units;
+    for (int r = lo; r < hi; ++r) {
+      if (per > 1) q = paged_request<MIXED>(a, r);
+      const int splits = (q.blocks + chunk - 1) / chunk;
+      if (u < before + q.tiles * splits) {
+        const int tile = q.tiles - 1 - (u - before) / splits;  // the longest rows of a causal chunk first
+        PagedUnit one;
+        one.request = r;
+        one.begin = q.begin;
+        one.rows = q.rows;
+        one.keys = q.keys;
+        one.token = tile * q.tokens;
+        one.tokens = min(q.tokens, q.rows - one.token);
+        one.first = a.causal ? max(a.kv_lens[r], 0) - q.rows + 1 : 0x3FFFFFFF;
+        one.chunk = chunk;
+        one.split = (u - before) % splits;
+        one.record = u - one.split;
+        one.narrow = q.narrow;
+        // chunks of this tile: its last row's keys
+        const int end = a.causal ? min(q.keys, max(0, one.first + one.token + one.tokens - 1)) : q.keys;
+        one.keys = end;
+        one.splits = max(1, ((end + kPagedUnitKeys - 1) / kPagedUnitKeys + chunk - 1) / chunk);
+        s_unit = one;
+        break;
+      }
+      before += q.tiles * splits;
+    }
+  }
+  __syncthreads();
+  unit = s_unit;
+  return unit.request >= 0 && unit.split < unit.splits;
+}
+
+// Element offset of a key's row in the pages of kv head 0, -1 where its entry names no page.
+AOTO_DEVICE long long paged_row(const PagedAttentionArgs& a, const int* __restrict__ table, int key) {
+  const unsigned block = a.page == 1 ? key : __umulhi((unsigned)key, a.page_magic) >> a.page_shift;
+  const int page = table[block];
+  const int row = key - (int)block * a.page;
+  return (unsigned)page < (unsigned)a.pages ? page * a.page_stride + row * a.slot_stride : -1;
+}
+
+AOTO_DEVICE bool bf16_pair_special(uint32_t w) {
+  return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+}
+AOTO_DEVICE uint32_t bf16_pair_finite(uint32_t w) {
+  if ((w & 0x7F80u) == 0x7F80u) w &= 0xFFFF0000u;
+  if ((w & 0x7F800000u) == 0x7F800000u) w &= 0xFFFFu;
+  return w;
+}
+// Whether a 16-byte chunk of V holds an infinity or a NaN; the chunk without them.
+AOTO_DEVICE bool chunk_special(const uint4& v) {
+  return bf16_pair_special(v.x) || bf16_pair_special(v.y) || bf16_pair_special(v.z) || bf16_pair_special(v.w);
+}
+AOTO_DEVICE uint4 chunk_finite(const uint4& v) {
+  return make_uint4(bf16_pair_finite(v.x), bf16_pair_finite(v.y), bf16_pair_finite(v.z), bf16_pair_finite(v.w));
+}
+// The infinity or NaN in the upper or lower half of w, else 0.
+AOTO_DEVICE float special_lo(uint32_t w) { return (w & 0x7F80u) == 0x7F80u ? bf16_lo(w) : 0.f; }
+AOTO_DEVICE float special_hi(uint32_t w) { return (w & 0x7F800000u) == 0x7F800000u ? bf16_hi(w) : 0.f; }
+
+AOTO_DEVICE float* paged_record(const PagedAttentionArgs& a, int unit, int kvh, int row, int head_dim) {
+  return a.records + (((size_t)unit * a.kv_heads + kvh) * a.record_rows + row) * (head_dim + 2);
+}
+
+// What a joined token needs: its tile's first unit, how many there are, its first row in their records.
+AOTO_DEVICE void paged_note(const PagedAttentionArgs& a, const PagedUnit& unit, int kvh) {
+  if (a.target <= 0 || kvh != 0 || unit.split != 0) return;
+  const int group = a.query_heads / a.kv_heads;
+  for (int i = threadIdx.x; i < unit.tokens; i += 256)
+    reinterpret_cast<int4*>(a.joins)[unit.begin + unit.token + i] = make_int4(unit.record, unit.splits, i * group, 0);
+}
+
+// ---------------------------------------------------------------------------------------------------- narrow tiles
+template <int D, int NT>
+struct PagedNarrowShared {
+  static constexpr int STR = D + 16;  // bf16 of a staged V row: the transposing reads' four rows start 8 banks apart
+  union {
+    uint16_t v[4][32 * STR];
+    float o[4][16 * NT][D];
+  };
+  float m[4][16 * NT], l[4][16 * NT];
+};
+
+// v_mfma_f32_16x16x32_bf16: S^T [16 keys x 16 rows] = K . Q^T, O^T [16 d x 16 rows] += V^T . P^T. Lane l owns row
+// l % 16 of a tile in both; the k slots of the second product hold the keys in the order S^T leaves them in a lane:
+// slot 8 q + j is key 4 q + j of the first 16 (j < 4), 4 q + j - 4 of the second.
+template <int D, int NT>
+AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit, int kvh, PagedNarrowShared<D, NT>& s) {
+  constexpr int DC = D / 32, DT = D / 16, STR = PagedNarrowShared<D, NT>::STR, ROWS = 16 * NT;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, quad = lane >> 4;
+  const int group = a.query_heads / a.kv_heads;
+  const int live = unit.tokens * group;  // rows in use; the others repeat the last
+  const int* table = a.block_tables + unit.request * a.table_stride;
+  const uint16_t* keys = a.keys + kvh * a.head_stride + 8 * quad;
+  const uint16_t* values = a.values + kvh * a.head_stride + 8 * quad;
+  uint16_t* vs = s.v[wave];
+
+  const int k0 = unit.split * unit.chunk * kPagedUnitKeys;
+  const int k1 = min(unit.keys, k0 + unit.chunk * kPagedUnitKeys);
+  // this wave's 32-key tiles: k0 + 32 wave + 128 i
+  const int mine = k0 + 32 * wave;
+  const int trips = k1 > mine ? (k1 - mine + 127) / 128 : 0;
+
+  fa_bf16x8 qf[NT][DC];
+  int limit[NT];  // keys that this lane's row sees
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int row = min(16 * t + col, live - 1), i = unit.token + row / group, g = row % group;
+    const uint16_t* q = a.q + (unit.begin + i) * a.q_token_stride + (kvh * group + g) * a.q_head_stride + 8 * quad;
+#pragma unroll
+    for (int c = 0; c < DC; ++c) qf[t][c] = *reinterpret_cast<const fa_bf16x8*>(q + 32 * c);
+    limit[t] = min(k1, unit.first + i);
+  }
+  const int least = min(k1, unit.first + unit.token);  // keys that every row sees
+
+  float run_max[NT], run_sum[NT];
+  f32x4_t o[NT][DT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    run_max[t] = -INFINITY, run_sum[t] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{};
+  }
+  const float c2 = a.scale * 1.4426950408889634f;
+
+  // rows of the 32 keys at `base` that this lane loads: keys col and 16 + col (clamped into the chunk)
+  long long at[2];
+  auto rows = [&](int base, long long (&to)[2]) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) to[g] = paged_row(a, table, min(base + 16 * g + col, k1 - 1));
+  };
+  uint4 kq[2][DC], vq[2][DC];
+  if (trips > 0) {
+    rows(mine, at);
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int c = 0; c < DC; ++c) kq[g][c] = *reinterpret_cast<const uint4*>(keys + max(at[g], 0LL) + 32 * c);
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int c = 0; c < DC; ++c) vq[g][c] = *reinterpret_cast<const uint4*>(values + max(at[g], 0LL) + 32 * c);
+  }
+  for (int trip = 0; trip < trips; ++trip) {
+    const int base = mine + 128 * trip;
+    long long next[2];
+    rows(min(base + 128, k1 - 1), next);
+    f32x4_t sc[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        sc[t][g] = f32x4_t{};
+#pragma unroll
+        for (int c = 0; c < DC; ++c)
+          sc[t][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(fa_bf16x8, kq[g][c]), qf[t][c],
+                                                             sc[t][g], 0, 0, 0);
+      }
+    // the keys of this tile that exist, one bit each; their values to LDS, zeros for the others
+    bool there[2];
+    uint32_t exist = 0;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      there[g] = at[g] >= 0 && base + 16 * g + col < k1;
+      exist |= (uint32_t)(__ballot(there[g]) & 0xFFFFu) << (16 * g);
+    }
+    const bool whole = exist == 0xFFFFFFFFu && base + 32 <= least;
+    uint32_t special = 0;  // keys, not seen by every row, whose values are not finite: added row by row below
+    if (!whole && least < k1 && base + 32 > least) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        bool odd = false;
+#pragma unroll
+        for (int c = 0; c < DC; ++c) odd |= chunk_special(vq[g][c]);
+        unsigned long long lanes = __ballot(odd && there[g]);
+        lanes |= lanes >> 32;
+        special |= (uint32_t)((lanes | lanes >> 16) & 0xFFFFu) << (16 * g);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int c = 0; c < DC; ++c) {
+        uint4 v = there[g] ? vq[g][c] : make_uint4(0, 0, 0, 0);
+        if (special) v = chunk_finite(v);
+        *reinterpret_cast<uint4*>(vs + (16 * g + col) * STR + 32 * c + 8 * quad) = v;
+      }
+    // the next tile's loads, K first
+    const long long old[2] = {at[0], at[1]};
+#pragma unroll
+    for (int g = 0; g < 2; ++g) at[g] = next[g];
+    if (trip + 1 < trips) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int c = 0; c < DC; ++c) kq[g][c] = *reinterpret_cast<const uint4*>(keys + max(at[g], 0LL) + 32 * c);
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int c = 0; c < DC; ++c) vq[g][c] = *reinterpret_cast<const uint4*>(values + max(at[g], 0LL) + 32 * c);
+    }
+    fa_bf16x8 pb[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (!whole) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = 16 * g + 4 * quad + e;
+            if (!(exist >> k & 1) || base + k >= limit[t]) sc[t][g][e] = -INFINITY;
+          }
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[t][g][e]);
+      top = xor32_max(xor16_max(top)) * c2;
+      // the exponentials' reference moves only where a score passes it by more than 2^8
+      const float moved = top > run_max[t] + 8.f ? top : run_max[t];
+      const float keep = moved == run_max[t] ? 1.f : __builtin_amdgcn_exp2f(run_max[t] - moved);
+      run_max[t] = moved;
+      const float ref = moved == -INFINITY ? 0.f : moved;
+      if (__any(keep != 1.f)) {
+        run_sum[t] *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[t][d] *= keep;
+      }
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j >> 2][j & 3], c2, -ref));
+        run_sum[t] += p[j];
+      }
+      const uint32_t packed[4] = {cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
+                                  cvt_pk_bf16(p[6], p[7])};
+      pb[t] = __builtin_bit_cast(fa_bf16x8, packed);
+    }
+    const uint16_t* vp = vs + (4 * quad + (col >> 2)) * STR + 4 * (col & 3);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const pa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4*)(vp + 16 * d));
+      const pa_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4*)(vp + 16 * STR + 16 * d));
+      const pa_s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(fa_bf16x8, both), pb[t], o[t][d], 0, 0, 0);
+    }
+    while (special) {
+      const int k = __ffs(special) - 1;
+      special &= special - 1;
+      const long long row = __shfl(k < 16 ? old[0] : old[1], k & 15);
+      const uint16_t* v = a.values + kvh * a.head_stride + row + 4 * quad;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const uint2 w = *reinterpret_cast<const uint2*>(v + 16 * d);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          if (base + k < limit[t]) {
+            o[t][d][0] += special_lo(w.x), o[t][d][1] += special_hi(w.x);
+            o[t][d][2] += special_lo(w.y), o[t][d][3] += special_hi(w.y);
+          }
+      }
+    }
+  }
+
+  // the waves' shares of each row, combined as the join combines chunks
+#pragma unroll
+  for (int t = 0; t < NT; ++t) run_sum[t] = xor32_sum(xor16_sum(run_sum[t]));
+  __syncthreads();  // every wave is through with its V
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      *reinterpret_cast<f32x4_t*>(&s.o[wave][16 * t + col][16 * d + 4 * quad]) = o[t][d];
+    if (quad == 0) s.m[wave][16 * t + col] = run_max[t], s.l[wave][16 * t + col] = run_sum[t];
+  }
+  __syncthreads();
+  constexpr int PER_ROW = D / 4;
+  for (int c = threadIdx.x; c < live * PER_ROW; c += 256) {
+    const int row = c / PER_ROW, d = 4 * (c % PER_ROW);
+    float big = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) big = fmaxf(big, s.m[w][row]);
+    float sum = 0.f;
+    f32x4_t v{};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = s.m[w][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s.m[w][row] - big);
+      sum += f * s.l[w][row];
+      // a wave without keys holds zeros: 0 * 0
+      v += f * *reinterpret_cast<const f32x4_t*>(&s.o[w][row][d]);
+    }
+    if (unit.splits > 1) {
+      float* rec = paged_record(a, unit.record + unit.split, kvh, row, D);
+      if (d == 0) rec[0] = big, rec[1] = sum;
+      *reinterpret_cast<float2*>(rec + 2 + d) = make_float2(v[0], v[1]);
+      *reinterpret_cast<float2*>(rec + 4 + d) = make_float2(v[2], v[3]);
+    } else {
+      const float inv = big == -INFINITY ? 0.f : 1.f / sum;
+      const size_t token = unit.begin + unit.token + row / group;
+      *reinterpret_cast<uint2*>(a.out + (token * a.query_heads + kvh * group + row % group) * D + d) =
+          make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------ wide tiles
+template <int D>
+struct PagedWideShared {
+  static constexpr int STRK = D + 8, STRV = D + 32;  // strides of staged rows, as in the prefill attention
+  uint16_t k[2][64 * STRK];
+  uint16_t v[2][64 * STRV];
+  uint32_t exist[2][4];    // by K buffer and staging wave: which of its 16 rows exist
+  uint32_t special[2][4];  // by V buffer: which hold a value that is not finite and not seen by every row
+};
+
+template <int D>
+AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, int kvh, PagedWideShared<D>& s) {
+  constexpr int STRK = PagedWideShared<D>::STRK, STRV = PagedWideShared<D>::STRV;
+  constexpr int DS = D / 16, DT = D / 32, LPR = D / 8;  // lanes a row
+  constexpr int RPL = 64 / LPR;                         // rows a wave's load covers
+  constexpr int LOADS = 16 / RPL;                       // loads of K (and V) a thread does for a 64-key tile
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int group = a.query_heads / a.kv_heads;
+  const int live = unit.tokens * group;
+  const int* table = a.block_tables + unit.request * a.table_stride;
+  const int k0 = unit.split * unit.chunk * kPagedUnitKeys;
+  const int k1 = min(unit.keys, k0 + unit.chunk * kPagedUnitKeys);
+  const int tiles = k1 > k0 ? (k1 - k0 + 63) / 64 : 0;
+  const bool active = 64 * wave < live;  // a wave of none of the rows only stages
+
+  fa_bf16x8 qf[2][DS];
+  int limit[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int row = min(64 * wave + 32 * c + col, live - 1), i = unit.token + row / group, g = row % group;
+    const uint16_t* q = a.q + (unit.begin + i) * a.q_token_stride + (kvh * group + g) * a.q_head_stride + 8 * half;
+#pragma unroll
+    for (int d = 0; d < DS; ++d) qf[c][d] = *reinterpret_cast<const fa_bf16x8*>(q + 16 * d);
+    limit[c] = min(k1, unit.first + i);
+  }
+  const int least = min(k1, unit.first + unit.token);  // keys that every row of the block sees
+  const float c2 = a.scale * 1.4426950408889634f;
+
+  // Staging: load i of a tile takes row (4 i + wave) RPL + lane / LPR, dims 8 (lane % LPR) .. + 7.
+  const uint16_t* keys = a.keys + kvh * a.head_stride + 8 * (lane % LPR);
+  const uint16_t* values = a.values + kvh * a.head_stride + 8 * (lane % LPR);
+  const int stage_row = wave * RPL + lane / LPR;
+  auto rows = [&](int tile, long long (&to)[LOADS]) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      to[i] = paged_row(a, table, min(k0 + 64 * tile + 4 * RPL * i + stage_row, k1 - 1));
+  };
+  auto load = [&](const uint16_t* from, const long long (&at)[LOADS], uint4 (&to)[LOADS]) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) to[i] = *reinterpret_cast<const uint4*>(from + max(at[i], 0LL));
+  };
+  auto store_k = [&](int tile, const long long (&at)[LOADS], const uint4 (&from)[LOADS]) {
+    uint32_t exist = 0;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = 4 * RPL * i + stage_row;
+      *reinterpret_cast<uint4*>(s.k[tile & 1] + row * STRK + 8 * (lane % LPR)) = from[i];
+      const unsigned long long lanes = __ballot(at[i] >= 0 && k0 + 64 * tile + row < k1);
+#pragma unroll
+      for (int j = 0; j < RPL; ++j) exist |= (uint32_t)(lanes >> (j * LPR) & 1) << (i * RPL + j);
+    }
+    if (lane == 0) s.exist[tile & 1][wave] = exist;
+  };
+  auto store_v = [&](int tile, const long long (&at)[LOADS], const uint4 (&from)[LOADS]) {
+    uint32_t special = 0;
+    const bool partial = least < k1 && k0 + 64 * tile + 64 > least;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = 4 * RPL * i + stage_row;
+      uint4 v = at[i] >= 0 && k0 + 64 * tile + row < k1 ? from[i] : make_uint4(0, 0, 0, 0);
+      if (partial) {
+        const unsigned long long lanes = __ballot(chunk_special(v));
+        if (lanes) v = chunk_finite(v);
+#pragma unroll
+        for (int j = 0; j < RPL; ++j)
+          special |= (uint32_t)((lanes >> (j * LPR) & ((1ull << LPR) - 1)) != 0) << (i * RPL + j);
+      }
+      *reinterpret_cast<uint4*>(s.v[tile & 1] + row * STRV + 8 * (lane % LPR)) = v;
+    }
+    if (lane == 0) s.special[tile & 1][wave] = special;
+  };
+  // the bit of a tile's key (a constant, plus 4 in the upper half of the wave) in what the four waves staged
+  auto bit = [&](const uint32_t (&words)[4], int k) {
+    const uint32_t low = words[k / RPL % 4] >> (k / (4 * RPL) * RPL + k % RPL);
+    const uint32_t high = words[(k + 4) / RPL % 4] >> ((k + 4) / (4 * RPL) * RPL + (k + 4) % RPL);
+    return ((half ? high : low) & 1) != 0;
+  };
+
+  float run_max[2] = {-INFINITY, -INFINITY}, run_sum[2] = {0.f, 0.f};
+  fa_f32x16 o[2][DT];
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[c][d] = fa_f32x16{};
+
+  uint4 kr[LOADS], vr[LOADS];
+  long long at[LOADS];
+  for (int t = 0; t < tiles; ++t) {
+    rows(t, at);
+    load(keys, at, kr);
+    load(values, at, vr);
+    store_k(t, at, kr);
+    store_v(t, at, vr);
+    __syncthreads();
+    if (active) {
+      const int j0 = k0 + 64 * t;
+      const uint16_t* ks = s.k[t & 1];
+      const uint16_t* vs = s.v[t & 1];
+      fa_f32x16 sc[2][2];
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        sc[0][sub] = fa_f32x16{}, sc[1][sub] = fa_f32x16{};
+#pragma unroll
+        for (int d = 0; d < DS; ++d) {
+          const fa_bf16x8 k = *reinterpret_cast<const fa_bf16x8*>(ks + (sub * 32 + col) * STRK + 16 * d + 8 * half);
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            sc[c][sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[c][d], sc[c][sub], 0, 0, 0);
+        }
+      }
+      const uint32_t exist[4] = {s.exist[t & 1][0], s.exist[t & 1][1], s.exist[t & 1][2], s.exist[t & 1][3]};
+      const bool all = (exist[0] & exist[1] & exist[2] & exist[3]) == 0xFFFFu;
+      if (!all || j0 + 64 > least) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int k = 32 * sub + 8 * (e >> 2) + (e & 3);
+              if (j0 + k + 4 * half >= limit[c] || !bit(exist, k)) sc[c][sub][e] = -INFINITY;
+            }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[c][sub][e]);
+        top = xor32_max(top) * c2;
+        const float moved = top > run_max[c] + 8.f ? top : run_max[c];
+        const float keep = moved == run_max[c] ? 1.f : __builtin_amdgcn_exp2f(run_max[c] - moved);
+        run_max[c] = moved;
+        const float ref = moved == -INFINITY ? 0.f : moved;
+        if (__any(keep != 1.f)) {
+          run_sum[c] *= keep;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[c][d] *= keep;
+        }
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          float p[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][kt >> 1][8 * (kt & 1) + j], c2, -ref));
+            run_sum[c] += p[j];
+          }
+          const uint32_t packed[4] = {cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
+                                      cvt_pk_bf16(p[6], p[7])};
+          const fa_bf16x8 pb = __builtin_bit_cast(fa_bf16x8, packed);
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+            o[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(flash_v_operand<STRV>(vs, kt, 32 * d, lane), pb, o[c][d],
+                                                              0, 0, 0);
+        }
+      }
+      for (int w = 0; w < 4; ++w) {
+        uint32_t special = __builtin_amdgcn_readfirstlane(s.special[t & 1][w]);
+        while (special) {
+          const int b = __ffs(special) - 1;
+          special &= special - 1;
+          const int k = (4 * (b / RPL) + w) * RPL + b % RPL;
+          const uint16_t* v = a.values + kvh * a.head_stride + paged_row(a, table, j0 + k) + 4 * half;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const uint2 x = *reinterpret_cast<const uint2*>(v + 32 * d + 8 * g);
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+                if (j0 + k < limit[c]) {
+                  o[c][d][4 * g] += special_lo(x.x), o[c][d][4 * g + 1] += special_hi(x.x);
+                  o[c][d][4 * g + 2] += special_lo(x.y), o[c][d][4 * g + 3] += special_hi(x.y);
+                }
+            }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  if (!active) return;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const float sum = xor32_sum(run_sum[c]);
+    const int row = 64 * wave + 32 * c + col;
+    if (row >= live) continue;
+    if (unit.splits > 1) {
+      float* rec = paged_record(a, unit.record + unit.split, kvh, row, D);
+      if (half == 0) rec[0] = run_max[c], rec[1] = sum;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float2* to = reinterpret_cast<float2*>(rec + 2 + 32 * d + 8 * g + 4 * half);
+          to[0] = make_float2(o[c][d][4 * g], o[c][d][4 * g + 1]);
+          to[1] = make_float2(o[c][d][4 * g + 2], o[c][d][4 * g + 3]);
+        }
+    } else {
+      const float inv = run_max[c] == -INFINITY ? 0.f : 1.f / sum;
+      const size_t token = unit.begin + unit.token + row / group;
+      uint16_t* to = a.out + (token * a.query_heads + kvh * group + row % group) * D + 4 * half;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<uint2*>(to + 32 * d + 8 * g) =
+              make_uint2(pack_bf16x2(o[c][d][4 * g] * inv, o[c][d][4 * g + 1] * inv),
+                         pack_bf16x2(o[c][d][4 * g + 2] * inv, o[c][d][4 * g + 3] * inv));
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------- the blocks
+template <int D, int NT>
+__device__ void paged_attention_narrow(const PagedAttentionArgs& a) {
+  __shared__ __attribute__((aligned(16))) PagedNarrowShared<D, NT> s;
+  PagedUnit unit;
+  const int kvh = blockIdx.x % a.kv_heads;
+  if (!paged_unit<false>(a, blockIdx.x / a.kv_heads, unit)) return;
+  paged_note(a, unit, kvh);
+  paged_narrow<D, NT>(a, unit, kvh, s);
 }
 
 template <int D>
-__device__ void paged_attention_simple(const PagedAttentionArgs& a) {
-  constexpr int LPK = D / 8, KPI = 64 / LPK;
-  const int t = blockIdx.x / a.query_heads, h = blockIdx.x % a.query_heads;
-  const int lane = threadIdx.x, sub = lane % LPK, kin = lane / LPK;
-  if (t >= a.query_start[a.requests]) return;
-  const int r = paged_request(a.query_start, a.requests, t);
-  const int begin = a.query_start[r], n = a.query_start[r + 1] - begin;
-  int keys = a.kv_lens[r];
-  if (a.causal) keys = min(keys, keys - n + (t - begin) + 1);
-  keys = min(keys, (int)min((long long)a.max_blocks * a.page, 0x7FFFFFFFLL));
-  const int kvh = h / (a.query_heads / a.kv_heads);
-  const uint4 qc = *reinterpret_cast<const uint4*>(a.q + t * a.q_token_stride + h * a.q_head_stride + 8 * sub);
-  float m = -INFINITY, l = 0.f, acc[8] = {};
-  for (int j0 = 0; j0 < keys; j0 += KPI) {
-    const int j = j0 + kin;
-    const int page = j < keys ? a.block_tables[r * a.table_stride + j / a.page] : -1;
-    const bool there = page >= 0 && page < a.pages;
-    const long long at = there ? page * a.page_stride + kvh * a.head_stride + (j % a.page) * a.slot_stride : 0;
-    const uint4 k = *reinterpret_cast<const uint4*>(a.keys + at + 8 * sub);
-    const uint4 v = *reinterpret_cast<const uint4*>(a.values + at + 8 * sub);
-    float dot = dot2_bf16(k.x, qc.x, 0.f);
-    dot = dot2_bf16(k.y, qc.y, dot);
-    dot = dot2_bf16(k.z, qc.z, dot);
-    dot = dot2_bf16(k.w, qc.w, dot);
-    const float score = there ? group_sum<LPK>(dot) * a.scale : -INFINITY;
-    const float big = fmaxf(m, score);
-    const float ref = big == -INFINITY ? 0.f : big;
-    const float p = expf(score - ref), keep = expf(m - ref);
-    m = big;
-    l = l * keep + p;
-    const uint32_t va[4] = {v.x, v.y, v.z, v.w};
+__device__ void paged_attention_mixed(const PagedAttentionArgs& a) {
+  __shared__ __attribute__((aligned(16))) union {
+    PagedNarrowShared<D, 1> narrow;
+    PagedWideShared<D> wide;
+  } s;
+  PagedUnit unit;
+  const int kvh = blockIdx.x % a.kv_heads;
+  if (!paged_unit<true>(a, blockIdx.x / a.kv_heads, unit)) return;
+  paged_note(a, unit, kvh);
+  if (unit.narrow) paged_narrow<D, 1>(a, unit, kvh, s.narrow);
+  else paged_wide<D>(a, unit, kvh, s.wide);
+}
+
+// A wave joins the chunks of one row: with m the largest maximum, out = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.
+template <int D>
+__device__ void paged_attention_join(const PagedAttentionArgs& a) {
+  constexpr int PER = D / 64;
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int t = row / a.query_heads, h = row % a.query_heads;
+  if (t >= min(a.tokens, a.query_start[a.requests])) return;
+  const int4 note = reinterpret_cast<const int4*>(a.joins)[t];
+  if (note.y <= 1) return;
+  const int group = a.query_heads / a.kv_heads, kvh = h / group, at = note.z + h % group;
+  const size_t step = (size_t)a.kv_heads * a.record_rows * (D + 2);
+  const float* rec = paged_record(a, note.x, kvh, at, D);
+  float big = -INFINITY;
+  for (int s = lane; s < note.y; s += 64) big = fmaxf(big, rec[s * step]);
+  big = wave_max(big);
+  float sum = 0.f, acc[PER] = {};
+  for (int s0 = 0; s0 < note.y; s0 += 64) {
+    const int s = s0 + lane;
+    const float m = s < note.y ? rec[s * step] : -INFINITY;
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - big);
+    sum += s < note.y ? f * rec[s * step + 1] : 0.f;
+    const int here = min(64, note.y - s0);
+#pragma unroll 4
+    for (int i = 0; i < here; ++i) {
+      const float w = __shfl(f, i);
+      const float* o = rec + (s0 + i) * step + 2 + PER * lane;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      acc[2 * i] = acc[2 * i] * keep + (there ? p * bf16_lo(va[i]) : 0.f);
-      acc[2 * i + 1] = acc[2 * i + 1] * keep + (there ? p * bf16_hi(va[i]) : 0.f);
+      for (int e = 0; e < PER; ++e) acc[e] += w * o[e];
     }
   }
-  const float big = wave_max(m);
-  const float f = m == -INFINITY ? 0.f : expf(m - big);
-  const float sum = wave_sum(sub == 0 ? l * f : 0.f);
-  float o[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float v = acc[e] * f;
-    for (int d = LPK; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    o[e] = sum > 0.f ? v / sum : 0.f;
-  }
-  if (kin == 0) {
-    uint4 w = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]),
-                         pack_bf16x2(o[6], o[7]));
-    *reinterpret_cast<uint4*>(a.out + ((size_t)t * a.query_heads + h) * D + 8 * sub) = w;
-  }
+  sum = wave_sum(sum);
+  const float inv = big == -INFINITY ? 0.f : 1.f / sum;
+  uint16_t* out = a.out + ((size_t)t * a.query_heads + h) * D + PER * lane;
+  if constexpr (PER == 2) *reinterpret_cast<uint32_t*>(out) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  else out[0] = (uint16_t)f32_to_bf16(acc[0] * inv);
 }
 
 }  // namespace aoto
 
-extern "C" __global__ __launch_bounds__(64) void aoto_paged_attention_d64(PagedAttentionArgs a) {
-  aoto::paged_attention_simple<64>(a);
-}
-extern "C" __global__ __launch_bounds__(64) void aoto_paged_attention_d128(PagedAttentionArgs a) {
-  aoto::paged_attention_simple<128>(a);
-}
+#define AOTO_PAGED_ATTENTION(D)                                                                                    \
+  extern "C" __global__ __launch_bounds__(256, 3) void aoto_paged_attention_d##D##_n1(PagedAttentionArgs a) {      \
+    aoto::paged_attention_narrow<D, 1>(a);                                                                         \
+  }                                                                                                                \
+  extern "C" __global__ __launch_bounds__(256, 2) void aoto_paged_attention_d##D##_n2(PagedAttentionArgs a) {      \
+    aoto::paged_attention_narrow<D, 2>(a);                                                                         \
+  }                                                                                                                \
+  extern "C" __global__ __launch_bounds__(256, 1) void aoto_paged_attention_d##D##_w(PagedAttentionArgs a) {       \
+    aoto::paged_attention_mixed<D>(a);                                                                             \
+  }                                                                                                                \
+  extern "C" __global__ __launch_bounds__(256) void aoto_paged_attention_join_d##D(PagedAttentionArgs a) {         \
+    aoto::paged_attention_join<D>(a);                                                                              \
+  }
