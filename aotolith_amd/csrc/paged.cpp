@@ -3,6 +3,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
+#include <cstdlib>
 
 #include "aoto_hip.h"
 #include "internal.h"
@@ -57,7 +58,11 @@ AttentionPlan attention_plan(int tokens, int requests, int max_blocks, int page,
   p.units = some + (tokens - some) / std::max(tile, 1);
   long long keys = std::min<long long>((long long)max_blocks * page, 1 << 30);
   if (max_kv_len) keys = std::min<long long>(keys, max_kv_len);
-  const long long blocks = p.units * kv_heads, full = (long long)aoto::device_cu_count() * (p.wide ? 2 : 4);
+  const long long blocks = p.units * kv_heads, full = (long long)aoto::device_cu_count() * (p.wide ? 1 : 4);
+#ifdef PA_TUNE
+  if (getenv("PA_T") && !p.wide) { const long long f = atoi(getenv("PA_T")); if (keys > kLeastChunk * 128) p.target = (int)((f + kv_heads - 1) / kv_heads); }
+  else
+#endif
   if (keys > kLeastChunk * 128 && blocks < full) p.target = (int)((full + kv_heads - 1) / kv_heads);
   p.units += p.target;
   if (p.target)
@@ -151,6 +156,8 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention: head_dim %d (64 or 128)", head_dim);
   if (!aligned(q, 16) || q_token_stride % 8 || q_head_stride % 8 || !aligned(out, 16))
     return set_error(AOTO_ERR_ARGUMENT, "paged_attention: q and out 16-byte aligned, strides of multiples of 8");
+  if (page_stride < 0 || page_stride > 0xFFFFFFFFLL || slot_stride < 0 || slot_stride * page > 0x3FFFFFFFLL)
+    return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention: pages of more than 2^32 elements, or rows 2^30 apart");
   if (!(scale > 0.f) || !std::isfinite(scale))
     return set_error(AOTO_ERR_ARGUMENT, "paged_attention: scale %g is not a positive number", (double)scale);
   if (query_heads / kv_heads > kWideRows)

@@ -29,6 +29,12 @@ typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 typedef short pa_s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) pa_s16x4 pa_lds_s16x4;
 
+typedef __attribute__((address_space(3))) fa_bf16x8 paged_lds_bf16x8;
+
+AOTO_DEVICE uint32_t paged_lds(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
 constexpr int kPagedUnitKeys = 128;  // keys that chunks are counted in
 constexpr int kPagedWideRows = 256;
 
@@ -133,11 +139,16 @@ AOTO_DEVICE bool paged_unit(const PagedAttentionArgs& a, int u, PagedUnit& unit)
   return unit.request >= 0 && unit.split < unit.splits;
 }
 
+// The block table entry of a key.
+AOTO_DEVICE int paged_block(const PagedAttentionArgs& a, int key) {
+  return a.page == 1 ? key : (int)(__umulhi((unsigned)key, a.page_magic) >> a.page_shift);
+}
+
 // Element offset of a key's row in the pages of kv head 0, -1 where its entry names no page.
 AOTO_DEVICE long long paged_row(const PagedAttentionArgs& a, const int* __restrict__ table, int key) {
-  const unsigned block = a.page == 1 ? key : __umulhi((unsigned)key, a.page_magic) >> a.page_shift;
+  const int block = paged_block(a, key);
   const int page = table[block];
-  const int row = key - (int)block * a.page;
+  const int row = key - block * a.page;
   return (unsigned)page < (unsigned)a.pages ? page * a.page_stride + row * a.slot_stride : -1;
 }
 
@@ -412,19 +423,61 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
 // ------------------------------------------------------------------------------------------------------ wide tiles
 template <int D>
 struct PagedWideShared {
-  static constexpr int STRK = D + 8, STRV = D + 32;  // strides of staged rows, as in the prefill attention
-  uint16_t k[2][64 * STRK];
-  uint16_t v[2][64 * STRV];
-  uint32_t exist[2][4];    // by K buffer and staging wave: which of its 16 rows exist
-  uint32_t special[2][4];  // by V buffer: which hold a value that is not finite and not seen by every row
+  uint16_t k[3][64 * D];
+  uint16_t v[2][64 * D];
+  uint32_t exist[4][4];  // by tile (mod 4) and staging wave: which of its 16 rows exist
+  uint32_t special[4];   // which of the V tile's rows hold a value that is not finite and not seen by every row
 };
 
+// 16 bytes a lane from global memory to 1 KB of LDS. Not the builtin: the compiler's wait counts lose track of which
+// buffer such a load writes; the loop below waits for all of them before its barrier.
+AOTO_DEVICE void paged_dma(const uint16_t* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
+}
+
+// Waits for all loads in flight, those to LDS among them: the builtin, so that the compiler knows it too and does not
+// wait, inside the loop, for loads it thinks are still out.
+AOTO_DEVICE void paged_landed() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0) alone
+  asm volatile("" ::: "memory");
+}
+
+// Changes of an accumulator that the tile loop makes seldom, in place: as plain arithmetic they make the compiler hold O
+// in the ordinary registers and move all of it (128 registers) to the accumulation registers and back in every tile.
+// It does not see that these read what products wrote, so acc_settle() stands before the first and after the last: the
+// 64 cycles that a product's result takes, with room.
+AOTO_DEVICE void acc_scale(float& x, float by) {
+  float y;
+  asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
+               : "+a"(x), "=&v"(y) : "v"(by));
+}
+AOTO_DEVICE void acc_add(float& x, float by) {
+  float y;
+  asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_add_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
+               : "+a"(x), "=&v"(y) : "v"(by));
+}
+AOTO_DEVICE void acc_settle() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// v_mfma_f32_32x32x16_bf16: S^T [32 keys x 32 rows] = K . Q^T, O^T [32 d x 32 rows] += V^T . P^T (layouts and slot
+// order as in the prefill attention). A wave has 64 rows: each K and V operand read from LDS serves two products, which
+// halves the traffic that otherwise (32 rows a wave) asks for all of the LDS's 128 bytes a cycle at the products' full
+// rate. One wave runs on a SIMD, with 512 registers, and what it issues between two products is free as long as it
+// takes no longer than they do; so a step holds, in this order and spread out between its products, the scores of the
+// next 32 keys (16 products; 24 of the present keys' 32 exponentials a lane) and the present keys' weights with V (16;
+// the other exponentials, the next scores out of their accumulators, their maximum). Operands are read from LDS two
+// products ahead. K and V go from memory to LDS without registers, K two tiles ahead and V one; the 16-byte pieces of a
+// row are permuted by a function of the row (the lanes fetch them so) that spreads each phase of the reads over all
+// banks. Rows' addresses advance by 64 keys a tile without a division or a product but the page's.
 template <int D>
 AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, int kvh, PagedWideShared<D>& s) {
-  constexpr int STRK = PagedWideShared<D>::STRK, STRV = PagedWideShared<D>::STRV;
-  constexpr int DS = D / 16, DT = D / 32, LPR = D / 8;  // lanes a row
+  constexpr int DS = D / 16, DT = D / 32, LPR = D / 8;  // lanes (16-byte pieces) a row
   constexpr int RPL = 64 / LPR;                         // rows a wave's load covers
   constexpr int LOADS = 16 / RPL;                       // loads of K (and V) a thread does for a 64-key tile
+  constexpr int ROWB = 2 * D, TILEB = 64 * ROWB;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int group = a.query_heads / a.kv_heads;
@@ -448,48 +501,66 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   const int least = min(k1, unit.first + unit.token);  // keys that every row of the block sees
   const float c2 = a.scale * 1.4426950408889634f;
 
-  // Staging: load i of a tile takes row (4 i + wave) RPL + lane / LPR, dims 8 (lane % LPR) .. + 7.
-  const uint16_t* keys = a.keys + kvh * a.head_stride + 8 * (lane % LPR);
-  const uint16_t* values = a.values + kvh * a.head_stride + 8 * (lane % LPR);
+  // The permutation of a row's pieces: piece c of row r lies at c ^ swizzle(r).
+  auto swizzle = [](int r) { return D == 128 ? (r & 3) << 2 | (r >> 2 & 3) : (r >> 1 & 1) << 2 | (r >> 2 & 3); };
+  // Staging: load i of a tile takes row 4 RPL i + stage_row, its piece lane % LPR.
   const int stage_row = wave * RPL + lane / LPR;
-  auto rows = [&](int tile, long long (&to)[LOADS]) {
+  const int piece = 8 * ((lane % LPR) ^ swizzle(stage_row));
+  const uint16_t* keys = a.keys + kvh * a.head_stride + piece;
+  const uint16_t* values = a.values + kvh * a.head_stride + piece;
+  const int last_block = paged_block(a, max(k1 - 1, 0));
+  const int page_span = a.page * (int)a.slot_stride;
+  const int step_blocks = paged_block(a, 64), step_off = (64 - step_blocks * a.page) * (int)a.slot_stride;
+  // of the tile looked up next: the rows' table entries and offsets in their pages; of the one before, page and offset
+  int block[LOADS], off[LOADS], page[LOADS], off_page[LOADS];
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i)
-      to[i] = paged_row(a, table, min(k0 + 64 * tile + 4 * RPL * i + stage_row, k1 - 1));
+  for (int i = 0; i < LOADS; ++i) {
+    const int key = k0 + 4 * RPL * i + stage_row;
+    block[i] = paged_block(a, key);
+    off[i] = (key - block[i] * a.page) * (int)a.slot_stride;
+  }
+  auto look_row = [&](int i) __attribute__((always_inline)) {
+    page[i] = table[min(block[i], last_block)];
+    off_page[i] = off[i];
+    off[i] += step_off;
+    const bool over = off[i] >= page_span;
+    off[i] -= over ? page_span : 0;
+    block[i] += step_blocks + (over ? 1 : 0);
   };
-  auto load = [&](const uint16_t* from, const long long (&at)[LOADS], uint4 (&to)[LOADS]) {
+  auto look = [&] {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) to[i] = *reinterpret_cast<const uint4*>(from + max(at[i], 0LL));
+    for (int i = 0; i < LOADS; ++i) look_row(i);
   };
-  auto store_k = [&](int tile, const long long (&at)[LOADS], const uint4 (&from)[LOADS]) {
-    uint32_t exist = 0;
+  auto place = [&](int tile, long long (&at)[LOADS]) {
+    bool fine = true;
+    bool there[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int row = 4 * RPL * i + stage_row;
-      *reinterpret_cast<uint4*>(s.k[tile & 1] + row * STRK + 8 * (lane % LPR)) = from[i];
-      const unsigned long long lanes = __ballot(at[i] >= 0 && k0 + 64 * tile + row < k1);
-#pragma unroll
-      for (int j = 0; j < RPL; ++j) exist |= (uint32_t)(lanes >> (j * LPR) & 1) << (i * RPL + j);
+      const bool known = (unsigned)page[i] < (unsigned)a.pages;
+      at[i] = (long long)((unsigned long long)(unsigned)(known ? page[i] : 0) * (unsigned)a.page_stride) + off_page[i];
+      there[i] = known && k0 + 64 * tile + 4 * RPL * i + stage_row < k1;
+      fine = fine && there[i];
     }
-    if (lane == 0) s.exist[tile & 1][wave] = exist;
-  };
-  auto store_v = [&](int tile, const long long (&at)[LOADS], const uint4 (&from)[LOADS]) {
-    uint32_t special = 0;
-    const bool partial = least < k1 && k0 + 64 * tile + 64 > least;
+    uint32_t exist = 0xFFFFu;
+    if (!__all(fine)) {
+      exist = 0;
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int row = 4 * RPL * i + stage_row;
-      uint4 v = at[i] >= 0 && k0 + 64 * tile + row < k1 ? from[i] : make_uint4(0, 0, 0, 0);
-      if (partial) {
-        const unsigned long long lanes = __ballot(chunk_special(v));
-        if (lanes) v = chunk_finite(v);
+      for (int i = 0; i < LOADS; ++i) {
+        const unsigned long long lanes = __ballot(there[i]);
 #pragma unroll
-        for (int j = 0; j < RPL; ++j)
-          special |= (uint32_t)((lanes >> (j * LPR) & ((1ull << LPR) - 1)) != 0) << (i * RPL + j);
+        for (int j = 0; j < RPL; ++j) exist |= (uint32_t)(lanes >> (j * LPR) & 1) << (i * RPL + j);
       }
-      *reinterpret_cast<uint4*>(s.v[tile & 1] + row * STRV + 8 * (lane % LPR)) = v;
     }
-    if (lane == 0) s.special[tile & 1][wave] = special;
+    if (lane == 0) s.exist[tile & 3][wave] = exist;
+  };
+  const uint32_t lds_k0 = paged_lds(s.k[0]), lds_v0 = paged_lds(s.v[0]);
+  auto fetch_row = [&](const uint16_t* from, const long long (&at)[LOADS], uint32_t to, int i)
+      __attribute__((always_inline)) {
+    paged_dma(from + at[i], __builtin_amdgcn_readfirstlane(to + (4 * i + wave) * 1024));
+  };
+  auto fetch = [&](const uint16_t* from, const long long (&at)[LOADS], uint32_t to) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) fetch_row(from, at, to, i);
   };
   // the bit of a tile's key (a constant, plus 4 in the upper half of the wave) in what the four waves staged
   auto bit = [&](const uint32_t (&words)[4], int k) {
@@ -498,111 +569,305 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
     return ((half ? high : low) & 1) != 0;
   };
 
-  float run_max[2] = {-INFINITY, -INFINITY}, run_sum[2] = {0.f, 0.f};
+  // Operands: byte addresses in a tile, XORed with a constant per 16 (K) or 32 (V) dims.
+  const uint32_t lds_k = lds_k0 + col * ROWB + ((half ^ swizzle(col)) << 4);
+  const int r = lane & 15, v_row = 4 * half + (r >> 2);
+  const uint32_t lds_v = lds_v0 + v_row * ROWB + (((2 * (lane >> 4 & 1) + (r & 3) / 2) ^ swizzle(v_row)) << 4) + (r & 1) * 8;
+  auto read_k = [&](uint32_t base, int sub, int d) {
+    return *(const paged_lds_bf16x8*)((base ^ (d << 5)) + sub * (32 * ROWB));
+  };
+  auto read_v = [&](uint32_t base, int kt, int d) {  // keys 16 kt .. of the tile
+    const pa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4*)((base ^ (d << 6)) + kt * (16 * ROWB)));
+    const pa_s16x4 hi =
+        __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4*)((base ^ (32 | d << 6)) + kt * (16 * ROWB) + 8 * ROWB));
+    const pa_s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(fa_bf16x8, both);
+  };
+
+  float run_max[2] = {-INFINITY, -INFINITY}, run_sum[2] = {0.f, 0.f}, ref[2] = {0.f, 0.f};
   fa_f32x16 o[2][DT];
 #pragma unroll
   for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[c][d] = fa_f32x16{};
+    for (int d = 0; d < DT; ++d) {
+      o[c][d] = fa_f32x16{};
+      asm("" : "+a"(o[c][d]));  // in the accumulation registers, here and wherever else than a product changes it
+    }
+  fa_f32x16 sc[2];        // scores of the present 32 keys
+  float top[2];           // their maximum, over this lane's
+  constexpr int AHEAD = 2;                 // products (pairs of them) that operands are read ahead; 3 measured the same
+  fa_bf16x8 kf[AHEAD + 1], vf[AHEAD + 1];  // operands on their way
 
-  uint4 kr[LOADS], vr[LOADS];
-  long long at[LOADS];
-  for (int t = 0; t < tiles; ++t) {
-    rows(t, at);
-    load(keys, at, kr);
-    load(values, at, vr);
-    store_k(t, at, kr);
-    store_v(t, at, vr);
-    __syncthreads();
-    if (active) {
-      const int j0 = k0 + 64 * t;
-      const uint16_t* ks = s.k[t & 1];
-      const uint16_t* vs = s.v[t & 1];
-      fa_f32x16 sc[2][2];
+  auto top_of = [&] {
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        sc[0][sub] = fa_f32x16{}, sc[1][sub] = fa_f32x16{};
+    for (int c = 0; c < 2; ++c) {
+      top[c] = sc[c][0];
 #pragma unroll
-        for (int d = 0; d < DS; ++d) {
-          const fa_bf16x8 k = *reinterpret_cast<const fa_bf16x8*>(ks + (sub * 32 + col) * STRK + 16 * d + 8 * half);
+      for (int e = 1; e < 16; ++e) top[c] = fmaxf(top[c], sc[c][e]);
+    }
+  };
+  // Whether every row sees every key of tile t.
+  auto whole = [&](int t) {
+    const uint32_t exist = s.exist[t & 3][0] & s.exist[t & 3][1] & s.exist[t & 3][2] & s.exist[t & 3][3];
+    return __builtin_amdgcn_readfirstlane(exist == 0xFFFFu && k0 + 64 * t + 64 <= least) != 0;
+  };
+  // The scores that a row may not see, or that are of no key, leave; then the maximum.
+  auto mask = [&](int t, int sub) {
+    if (whole(t)) return;
+    const int j0 = k0 + 64 * t;
+    const uint32_t exist[4] = {s.exist[t & 3][0], s.exist[t & 3][1], s.exist[t & 3][2], s.exist[t & 3][3]};
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-            sc[c][sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[c][d], sc[c][sub], 0, 0, 0);
-        }
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int k = 32 * sub + 8 * (e >> 2) + (e & 3);
+        if (j0 + k + 4 * half >= limit[c] || !bit(exist, k)) sc[c][e] = -INFINITY;
       }
-      const uint32_t exist[4] = {s.exist[t & 1][0], s.exist[t & 1][1], s.exist[t & 1][2], s.exist[t & 1][3]};
-      const bool all = (exist[0] & exist[1] & exist[2] & exist[3]) == 0xFFFFu;
-      if (!all || j0 + 64 > least) {
+    top_of();
+  };
+  // the exponentials' reference moves only where a score passes it by more than 2^8; O and the sum follow
+  auto move = [&] {
+    float keep[2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int k = 32 * sub + 8 * (e >> 2) + (e & 3);
-              if (j0 + k + 4 * half >= limit[c] || !bit(exist, k)) sc[c][sub][e] = -INFINITY;
-            }
-      }
+    for (int c = 0; c < 2; ++c) {
+      const float most = xor32_max(top[c]) * c2;
+      const float moved = most > run_max[c] + 8.f ? most : run_max[c];
+      keep[c] = moved == run_max[c] ? 1.f : __builtin_amdgcn_exp2f(run_max[c] - moved);
+      run_max[c] = moved;
+      ref[c] = moved == -INFINITY ? 0.f : moved;
+    }
+    if (__any(keep[0] != 1.f || keep[1] != 1.f)) {
+      acc_settle();
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float top = -INFINITY;
+        run_sum[c] *= keep[c];
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[c][sub][e]);
-        top = xor32_max(top) * c2;
-        const float moved = top > run_max[c] + 8.f ? top : run_max[c];
-        const float keep = moved == run_max[c] ? 1.f : __builtin_amdgcn_exp2f(run_max[c] - moved);
-        run_max[c] = moved;
-        const float ref = moved == -INFINITY ? 0.f : moved;
-        if (__any(keep != 1.f)) {
-          run_sum[c] *= keep;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[c][d] *= keep;
-        }
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          float p[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][kt >> 1][8 * (kt & 1) + j], c2, -ref));
-            run_sum[c] += p[j];
+          for (int e = 0; e < 16; ++e) {
+            float x = o[c][d][e];
+            acc_scale(x, keep[c]);
+            o[c][d][e] = x;
           }
-          const uint32_t packed[4] = {cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
-                                      cvt_pk_bf16(p[6], p[7])};
-          const fa_bf16x8 pb = __builtin_bit_cast(fa_bf16x8, packed);
+      }
+      acc_settle();
+    }
+  };
+  // Keys 32 sub .. of tile t (their scores in sc); then, with K of 32 keys at k_base (operands 0 and 1 in kf), the
+  // scores of those; the first operands at kn_base follow into kf.
+  // `beside(i)`: what else goes among the products, i of DS + 2 DT times.
+  auto step = [&](uint32_t v_base, int sub, uint32_t k_base, int k_sub, uint32_t kn_base, int kn_sub, auto beside)
+      __attribute__((always_inline)) {
+    constexpr int START = DS == 8 ? 2 : 1;           // products after which the reference is settled
+    constexpr int PER = 12 / (DS - START);           // pairs of exponentials after each of the others
+    uint32_t pk[2][2][4];
+    auto pair = [&](int u) {  // pair u of 16: k-step u / 8, rows' half u / 4 % 2
+      const int kt = u >> 3, c = u >> 2 & 1, j = u & 3, e = 8 * kt + 2 * j;
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][e], c2, -ref[c]));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][e + 1], c2, -ref[c]));
+      pk[c][kt][j] = cvt_pk_bf16(p0, p1);
+      run_sum[c] = dot2_bf16(pk[c][kt][j], 0x3F803F80u, run_sum[c]);  // the rounded weights' sum
+    };
+    fa_f32x16 next[2] = {fa_f32x16{}, fa_f32x16{}};
 #pragma unroll
-          for (int d = 0; d < DT; ++d)
-            o[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(flash_v_operand<STRV>(vs, kt, 32 * d, lane), pb, o[c][d],
-                                                              0, 0, 0);
+    for (int d = 0; d < DS; ++d) {
+      constexpr int RING = AHEAD + 1;
+      if (d + AHEAD < DS) kf[(d + AHEAD) % RING] = read_k(k_base, k_sub, d + AHEAD);
+      else vf[d + AHEAD - DS] = read_v(v_base, 2 * sub + (d + AHEAD - DS) / DT, (d + AHEAD - DS) % DT);
+      next[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[d % RING], qf[0][d], next[0], 0, 0, 0);
+      if (d >= START)
+#pragma unroll
+        for (int u = 0; u < PER / 2; ++u) pair((d - START) * PER + u);
+      next[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[d % RING], qf[1][d], next[1], 0, 0, 0);
+      if (d >= START)
+#pragma unroll
+        for (int u = PER / 2; u < PER; ++u) pair((d - START) * PER + u);
+      beside(d);
+      if (d == START - 1) move();
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int m = 0; m < 2 * DT; ++m) {
+      const int kt = m / DT, d = m % DT;
+      constexpr int RING = AHEAD + 1;
+      if (m + AHEAD < 2 * DT) vf[(m + AHEAD) % RING] = read_v(v_base, 2 * sub + (m + AHEAD) / DT, (m + AHEAD) % DT);
+      else kf[m + AHEAD - 2 * DT] = read_k(kn_base, kn_sub, m + AHEAD - 2 * DT);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t w[4] = {pk[c][kt][0], pk[c][kt][1], pk[c][kt][2], pk[c][kt][3]};
+        o[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[m % RING], __builtin_bit_cast(fa_bf16x8, w), o[c][d], 0, 0, 0);
+        if (kt == 0)
+#pragma unroll
+          for (int u = 12 + 4 * d / DT; u < 12 + 4 * (d + 1) / DT; ++u)
+            if (c == u % 2) pair(u);
+        // the next scores of rows' half c: 8 / DT of the first (second) eight
+#pragma unroll
+        for (int i = 0; i < 8 / DT; ++i) {
+          const int e = 8 * kt + d * (8 / DT) + i;
+          float x = next[c][e];
+          asm("" : "+v"(x));  // out of its accumulator once, here
+          sc[c][e] = x;
+          most[c] = fmaxf(most[c], x);
         }
       }
-      for (int w = 0; w < 4; ++w) {
-        uint32_t special = __builtin_amdgcn_readfirstlane(s.special[t & 1][w]);
-        while (special) {
-          const int b = __ffs(special) - 1;
-          special &= special - 1;
-          const int k = (4 * (b / RPL) + w) * RPL + b % RPL;
-          const uint16_t* v = a.values + kvh * a.head_stride + paged_row(a, table, j0 + k) + 4 * half;
+      beside(DS + m);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    top[0] = most[0], top[1] = most[1];
+    // what the next step needs is done in this one, among its products
+    asm volatile("" : "+v"(run_sum[0]), "+v"(run_sum[1]), "+v"(top[0]), "+v"(top[1]));
+  };
+  // V of tile t in LDS, where some of its rows do not exist or are not seen by every row: zeros for the former; for the
+  // latter what is not finite goes (0 * inf) and is added at the end of the tile, row by row
+  auto tidy = [&](int t) {
+    const uint32_t exist = s.exist[t & 3][wave];
+    const bool partial = least < k1 && k0 + 64 * t + 64 > least;
+    uint32_t special = 0;
 #pragma unroll
-          for (int d = 0; d < DT; ++d)
+    for (int i = 0; i < LOADS; ++i) {
+      uint4* at = reinterpret_cast<uint4*>(s.v[t & 1] + (4 * i + wave) * 512 + 8 * lane);
+      uint4 v = *at;
+      if (!(exist >> (i * RPL + lane / LPR) & 1)) v = make_uint4(0, 0, 0, 0);
+      if (partial) {
+        const unsigned long long lanes = __ballot(chunk_special(v));
+        v = chunk_finite(v);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const uint2 x = *reinterpret_cast<const uint2*>(v + 32 * d + 8 * g);
+        for (int j = 0; j < RPL; ++j)
+          special |= (uint32_t)((lanes >> (j * LPR) & ((1ull << LPR) - 1)) != 0) << (i * RPL + j);
+      }
+      *at = v;
+    }
+    if (lane == 0) s.special[wave] = special;
+  };
+  auto add_special = [&](int t) {
+    acc_settle();
+    for (int w = 0; w < 4; ++w) {
+      uint32_t special = __builtin_amdgcn_readfirstlane(s.special[w]);
+      while (special) {
+        const int b = __ffs(special) - 1;
+        special &= special - 1;
+        const int k = k0 + 64 * t + (4 * (b / RPL) + w) * RPL + b % RPL;
+        const uint16_t* v = a.values + kvh * a.head_stride + paged_row(a, table, k) + 4 * half;
 #pragma unroll
-              for (int c = 0; c < 2; ++c)
-                if (j0 + k < limit[c]) {
-                  o[c][d][4 * g] += special_lo(x.x), o[c][d][4 * g + 1] += special_hi(x.x);
-                  o[c][d][4 * g + 2] += special_lo(x.y), o[c][d][4 * g + 3] += special_hi(x.y);
-                }
-            }
-        }
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const uint2 x = *reinterpret_cast<const uint2*>(v + 32 * d + 8 * g);
+            const float add[4] = {special_lo(x.x), special_hi(x.x), special_lo(x.y), special_hi(x.y)};
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float y = o[c][d][4 * g + i];
+                acc_add(y, k < limit[c] ? add[i] : 0.f);
+                o[c][d][4 * g + i] = y;
+              }
+          }
       }
     }
+    acc_settle();
+  };
+
+  // At tile t: K of tiles t and t + 1 and V of tile t are in LDS, the scores of tile t's first 32 keys in sc; K of tile
+  // t + 2 goes to the buffer of tile t - 1 and V of tile t + 1 to that of tile t - 1 while it runs, and the rows of
+  // tile t + 3 are looked up.
+  long long at_k[LOADS], at_v[LOADS];
+  if (tiles > 0) {
+    look();
+    place(0, at_v);
+    fetch(keys, at_v, lds_k0);
+    fetch(values, at_v, lds_v0);
+    look();
+    place(1, at_v);
+    fetch(keys, at_v, lds_k0 + TILEB);
+    look();
+    place(2, at_k);
+    paged_landed();
     __syncthreads();
+    if (active) {
+      sc[0] = fa_f32x16{}, sc[1] = fa_f32x16{};
+#pragma unroll
+      for (int d = 0; d < DS; ++d) {
+        const fa_bf16x8 k = read_k(lds_k, 0, d);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) sc[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[c][d], sc[c], 0, 0, 0);
+      }
+      top_of();
+      mask(0, 0);
+#pragma unroll
+      for (int d = 0; d < AHEAD; ++d) kf[d] = read_k(lds_k, 1, d);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float x = sc[c][e];
+          asm("" : "+v"(x));
+          sc[c][e] = x;
+        }
+    }
+  }
+  auto stage = [&](int t, int kb) {
+    fetch(keys, at_k, lds_k0 + (kb == 0 ? 2 : kb - 1) * TILEB);
+    fetch(values, at_v, lds_v0 + ((t + 1) & 1) * TILEB);
+    look();
+  };
+  auto staged = [&](int t) {
+    paged_landed();
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) at_v[i] = at_k[i];
+    place(t + 3, at_k);
+    __syncthreads();
+  };
+  // The two steps of a tile. `edge` (a compile-time bool): keys that a row may not see or that are of no page may be
+  // among those of this tile and the next one's; without it there is no branch but the reference's move.
+  auto tile = [&](int t, int kb, auto edge) __attribute__((always_inline)) {
+    const uint32_t vb = lds_v + (t & 1) * TILEB, kn = lds_k + (kb == 2 ? 0 : kb + 1) * TILEB;
+    const uint32_t to_k = lds_k0 + (kb == 0 ? 2 : kb - 1) * TILEB, to_v = lds_v0 + ((t + 1) & 1) * TILEB;
+    step(vb, 0, lds_k + kb * TILEB, 1, kn, 0, [&](int i) __attribute__((always_inline)) {
+      if (i < LOADS) fetch_row(keys, at_k, to_k, i);
+      else if (i < 2 * LOADS) fetch_row(values, at_v, to_v, i - LOADS);
+      else if (i < 3 * LOADS) look_row(i - 2 * LOADS);
+    });
+    if constexpr (decltype(edge)::value) mask(t, 1);
+    step(vb, 1, kn, 0, kn, 1, [](int) {});
+    if constexpr (decltype(edge)::value)
+      if (t + 1 < tiles) mask(t + 1, 0);
+  };
+  auto after = [](int kb) { return kb == 2 ? 0 : kb + 1; };
+  paged_landed();     // on the way past the block above too
+  int t = 0, kb = 0;  // kb = t % 3
+  if (!active) {
+    for (; t < tiles; ++t, kb = after(kb)) {
+      stage(t, kb);
+      if (!whole(t)) {
+        tidy(t);
+        __syncthreads();
+      }
+      staged(t);
+    }
+    return;
+  }
+  for (bool easy = tiles > 1 && whole(0) && whole(1); easy; ++t, kb = after(kb)) {
+    // written before the last barrier, for the next tile
+    const uint4 one = *reinterpret_cast<const uint4*>(s.exist[(t + 1) & 3]);
+    const uint4 two = *reinterpret_cast<const uint4*>(s.exist[(t + 2) & 3]);
+    tile(t, kb, std::false_type{});
+    const uint32_t exist = one.x & one.y & one.z & one.w & two.x & two.y & two.z & two.w;
+    easy = t + 2 < tiles && k0 + 64 * t + 192 <= least && __builtin_amdgcn_readfirstlane(exist) == 0xFFFFu;
+    staged(t);
+  }
+  for (; t < tiles; ++t, kb = after(kb)) {  // the last tiles, and all from one on that has a row without a page
+    const bool care = !whole(t);
+    if (care) {
+      tidy(t);
+      __syncthreads();
+    }
+    tile(t, kb, std::true_type{});
+    if (care) add_special(t);
+    staged(t);
   }
 
-  if (!active) return;
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const float sum = xor32_sum(run_sum[c]);
@@ -618,6 +883,7 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
           float2* to = reinterpret_cast<float2*>(rec + 2 + 32 * d + 8 * g + 4 * half);
           to[0] = make_float2(o[c][d][4 * g], o[c][d][4 * g + 1]);
           to[1] = make_float2(o[c][d][4 * g + 2], o[c][d][4 * g + 3]);
+          __builtin_amdgcn_sched_barrier(0);
         }
     } else {
       const float inv = run_max[c] == -INFINITY ? 0.f : 1.f / sum;
@@ -626,10 +892,12 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+        for (int g = 0; g < 4; ++g) {
           *reinterpret_cast<uint2*>(to + 32 * d + 8 * g) =
-              make_uint2(pack_bf16x2(o[c][d][4 * g] * inv, o[c][d][4 * g + 1] * inv),
-                         pack_bf16x2(o[c][d][4 * g + 2] * inv, o[c][d][4 * g + 3] * inv));
+              make_uint2(cvt_pk_bf16(o[c][d][4 * g] * inv, o[c][d][4 * g + 1] * inv),
+                         cvt_pk_bf16(o[c][d][4 * g + 2] * inv, o[c][d][4 * g + 3] * inv));
+          __builtin_amdgcn_sched_barrier(0);
+        }
     }
   }
 }
@@ -647,7 +915,7 @@ __device__ void paged_attention_narrow(const PagedAttentionArgs& a) {
 
 template <int D>
 __device__ void paged_attention_mixed(const PagedAttentionArgs& a) {
-  __shared__ __attribute__((aligned(16))) union {
+  __shared__ __attribute__((aligned(256))) union {  // the wide form's addresses are XORed within a row
     PagedNarrowShared<D, 1> narrow;
     PagedWideShared<D> wide;
   } s;
