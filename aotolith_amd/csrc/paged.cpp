@@ -33,15 +33,15 @@ int check_pages(const char* what, const void* keys, const void* values, int64_t 
   return AOTO_OK;
 }
 
-// Rows of a wide tile of the attention, and keys (in 128) below which a request's keys are not split.
+// Rows of a wide tile of the attention, and the blocks of 128 keys that a GPU block takes at least.
 constexpr int kWideRows = 256;
-constexpr int kLeastChunk = 2;
+constexpr int kLeastBlocks = 2;
 
 struct AttentionPlan {
   bool wide;          // chunks of prompts may be among the requests: the instance with wide tiles
   int narrow_rows;    // rows of a narrow tile (16 or 32)
-  int target;         // units a kv head that the keys are split to make, 0 where they are not
-  long long units;    // at most, a kv head
+  int target;         // GPU blocks a kv head among which the keys are dealt, 0 where each takes one tile
+  long long units;    // tiles and cuts of them, a kv head, at most
   size_t workspace;
 };
 
@@ -55,19 +55,22 @@ AttentionPlan attention_plan(int tokens, int requests, int max_blocks, int page,
   p.narrow_rows = p.wide || rows <= 16 ? 16 : 32;
   const int tile = (p.wide ? kWideRows : p.narrow_rows) / group;
   const long long some = std::min(requests, tokens);
-  p.units = some + (tokens - some) / std::max(tile, 1);
-  long long keys = std::min<long long>((long long)max_blocks * page, 1 << 30);
+  const long long tiles = some + (tokens - some) / std::max(tile, 1);
+  long long keys = std::min<long long>((long long)max_blocks * page, 1 << 28);
   if (max_kv_len) keys = std::min<long long>(keys, max_kv_len);
-  const long long blocks = p.units * kv_heads, full = (long long)aoto::device_cu_count() * (p.wide ? 1 : 4);
+  // GPU blocks that the chip holds at a time: registers leave room for one with wide tiles on a CU, two narrow ones.
+  const long long full = (long long)aoto::device_cu_count() * (p.wide ? 1 : 2);
+  const long long most = (long long)max_blocks * page / 128 + 8;
+  p.units = tiles;
+  if (keys > kLeastBlocks * 128 && tiles * kv_heads < (p.wide ? 1 : 4) * full && tiles * most < (1 << 30)) {
+    p.target = (int)((full + kv_heads - 1) / kv_heads);
 #ifdef PA_TUNE
-  if (getenv("PA_T") && !p.wide) { const long long f = atoi(getenv("PA_T")); if (keys > kLeastChunk * 128) p.target = (int)((f + kv_heads - 1) / kv_heads); }
-  else
+    if (getenv("PA_T")) p.target = (atoi(getenv("PA_T")) + kv_heads - 1) / kv_heads;
 #endif
-  if (keys > kLeastChunk * 128 && blocks < full) p.target = (int)((full + kv_heads - 1) / kv_heads);
-  p.units += p.target;
-  if (p.target)
+    p.units += p.target;
     p.workspace = (size_t)tokens * 16 + (size_t)p.units * kv_heads * (p.wide ? kWideRows : p.narrow_rows) *
                                             (head_dim + 2) * sizeof(float);
+  }
   return p;
 }
 
@@ -156,6 +159,8 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention: head_dim %d (64 or 128)", head_dim);
   if (!aligned(q, 16) || q_token_stride % 8 || q_head_stride % 8 || !aligned(out, 16))
     return set_error(AOTO_ERR_ARGUMENT, "paged_attention: q and out 16-byte aligned, strides of multiples of 8");
+  if ((long long)max_blocks * page > (1 << 28))
+    return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention: block tables of more than 2^28 keys");
   if (page_stride < 0 || page_stride > 0xFFFFFFFFLL || slot_stride < 0 || slot_stride * page > 0x3FFFFFFFLL)
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention: pages of more than 2^32 elements, or rows 2^30 apart");
   if (!(scale > 0.f) || !std::isfinite(scale))
@@ -175,19 +180,19 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
   a.slot_stride = slot_stride, a.table_stride = table_stride, a.tokens = tokens, a.requests = requests;
   a.pages = pages, a.page = page, a.query_heads = query_heads, a.kv_heads = kv_heads;
   a.causal = causal != 0, a.scale = scale;
-  a.table_keys = (int)std::min<long long>((long long)max_blocks * page, 1 << 30);
+  a.table_keys = max_blocks * page;
   unsigned log2 = 0;
   while ((1u << log2) < (unsigned)page) ++log2;
   a.page_magic = (unsigned)(((1ull << (31 + log2)) + page - 1) / page), a.page_shift = log2 ? log2 - 1 : 0;
   a.narrow_tokens = plan.narrow_rows / (query_heads / kv_heads);
   a.wide_tokens = kWideRows / (query_heads / kv_heads);
-  a.target = plan.target, a.least_chunk = kLeastChunk, a.record_rows = plan.wide ? kWideRows : plan.narrow_rows;
+  a.target = plan.target, a.least_blocks = kLeastBlocks, a.record_rows = plan.wide ? kWideRows : plan.narrow_rows;
   a.joins = static_cast<int*>(workspace);
   a.records = reinterpret_cast<float*>(static_cast<char*>(workspace) + (size_t)tokens * 16);
   char name[64];
   snprintf(name, sizeof(name), "aoto_paged_attention_d%d_%s", head_dim,
            plan.wide ? "w" : plan.narrow_rows == 16 ? "n1" : "n2");
-  if (int s = launch(name, plan.units * kv_heads, 1, 256, stream, a)) return s;
+  if (int s = launch(name, (plan.target ? plan.target : plan.units) * kv_heads, 1, 256, stream, a)) return s;
   if (!plan.target) return AOTO_OK;
   return launch(head_dim == 64 ? "aoto_paged_attention_join_d64" : "aoto_paged_attention_join_d128",
                 ((long long)tokens * query_heads + 3) / 4, 1, 256, stream, a);
@@ -196,7 +201,7 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
 size_t aoto_hip_verify_draft_workspace(int requests, int drafts, int vocab) {
   if (requests <= 0 || drafts < 0 || vocab <= 0) return 0;
   const size_t chunks = ((size_t)vocab + kVerifyChunk - 1) / kVerifyChunk;
-  return (size_t)requests * chunks * ((2 * (size_t)drafts + 1) * kVerifyChunkBytes + 2 * sizeof(double));
+  return (size_t)requests * (chunks * ((2 * (size_t)drafts + 1) * kVerifyChunkBytes + 2 * sizeof(double)) + kVerifyLawBytes);
 }
 
 int aoto_hip_verify_draft(const void* logits, int logits_f32, int64_t row_stride, int rows, int vocab,
@@ -226,10 +231,11 @@ int aoto_hip_verify_draft(const void* logits, int logits_f32, int64_t row_stride
   if (int s = launch(logits_f32 ? "aoto_verify_stats_f32" : "aoto_verify_stats_bf16", a.chunks, requests * per, 256,
                      stream, a))
     return s;
-  if (temperature)
-    if (int s = launch(logits_f32 ? "aoto_verify_mass_f32" : "aoto_verify_mass_bf16", a.chunks, requests, 256, stream, a))
-      return s;
-  return launch(logits_f32 ? "aoto_verify_pick_f32" : "aoto_verify_pick_bf16", requests, 1, 256, stream, a);
+  if (!temperature)
+    return launch(logits_f32 ? "aoto_verify_greedy_f32" : "aoto_verify_greedy_bf16", requests, 1, 1024, stream, a);
+  if (int s = launch(logits_f32 ? "aoto_verify_mass_f32" : "aoto_verify_mass_bf16", a.chunks, requests, 256, stream, a))
+    return s;
+  return launch(logits_f32 ? "aoto_verify_pick_f32" : "aoto_verify_pick_bf16", requests, 1, 1024, stream, a);
 }
 
 }  // extern "C"

@@ -52,18 +52,19 @@ struct PagedAttentionArgs {
   int* joins;       // per token: where its records begin and how many there are
   long long q_token_stride, q_head_stride, page_stride, head_stride, slot_stride, table_stride;
   int tokens, requests, pages, page, query_heads, kv_heads, causal;
-  int table_keys;      // max_blocks * page, at most 2^30
+  int table_keys;      // max_blocks * page, at most 2^28
   unsigned page_magic, page_shift;  // key / page = (key * page_magic) >> 32 >> page_shift for keys below 2^31
   int narrow_tokens, wide_tokens;   // of a request, that a tile of 16 NT / 256 rows holds
-  int target;          // units a kv head that the keys are split to make; 0: not split
-  int least_chunk;     // in 128 keys
-  int record_rows;     // rows of a unit's record
+  int target;          // GPU blocks a kv head among which the key blocks (128 keys) are dealt; 0: one a tile
+  int least_blocks;    // key blocks that make a GPU block worth its while
+  int record_rows;     // rows of a record
   float scale;
 };
 
 // Tokens of a vocabulary that one block of the verification takes, and the bytes of what it leaves of a row of them.
 constexpr int kVerifyChunk = 8192;
 constexpr int kVerifyChunkBytes = 16;
+constexpr int kVerifyLawBytes = 80;  // what stands of a request's drafts, and where its token comes from
 
 struct VerifyArgs {
   const void* logits;

@@ -8,11 +8,13 @@
 // rounded to bf16 for its product (as the prefill attention does: the matrix instructions take two operands of one
 // type), its sum is not.
 //
-// Work is cut on the GPU, from the lengths as they are there: a unit is one tile of a request's rows (all query heads
-// of a kv head that share its keys, token after token) against one chunk of its keys. Every block finds its unit by
-// two sums over the requests; the chunk is the size at which the units of the whole call make about `target` blocks a
-// kv head, so that requests of very different lengths still end together. A tile whose keys make several chunks
-// leaves records (maximum, sum, unnormalized row) that aoto_paged_attention_join_* combines.
+// Work is cut on the GPU, from the lengths as they are there. An item is one tile of a request's rows (all query heads of
+// a kv head that share its keys, token after token) against all the keys they see, counted in blocks of 128 keys. With
+// `target` blocks a kv head, the items' key blocks, one item after the other, are dealt out evenly: every GPU block
+// takes the same number of them, wherever that begins and ends, so that requests of very different lengths end together
+// (an item cut among several leaves records, maximum, sum and unnormalized row, that aoto_paged_attention_join_*
+// combines). Without a target every GPU block takes one item. A GPU block finds its place by running sums over the
+// requests.
 //   narrow tiles (16 NT rows, decodes and drafted tokens): the four waves take 32 keys each of every 128; K goes
 //     straight from the pages to operand registers, V through the wave's own LDS; no barrier in the loop
 //   wide tiles (256 rows, chunks of prompts): the four waves take 64 rows each, 64-key tiles of K and V staged once
@@ -35,21 +37,27 @@ AOTO_DEVICE uint32_t paged_lds(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 
-constexpr int kPagedUnitKeys = 128;  // keys that chunks are counted in
+constexpr int kPagedUnitKeys = 128;  // keys of a key block
+// What starting on an item costs (its rows, table entries and first keys are three round trips to memory), in key
+// blocks: a GPU block that goes from one item to another takes so many fewer.
+#ifndef PA_LEAD
+#define PA_LEAD 2
+#endif
+constexpr int kPagedLead = PA_LEAD;
 constexpr int kPagedWideRows = 256;
 
 struct PagedUnit {
   int request, begin, rows;  // its first row and how many
-  int keys;                  // its keys, as far as the block table reaches
-  int first;                 // key index of the first row's own key, plus one (causal), of all rows otherwise
+  int keys;                  // that the tile's rows see, as far as the block table reaches
+  int first;                 // keys that the request's first row sees (causal; else more than there are)
   int token, tokens;         // of the request: the tile's first and count
-  int chunk, split, splits;  // in kPagedUnitKeys
-  int record;                // index of the tile's first unit
+  int from, to;              // key blocks of this part
+  int record, part, parts;   // the first part's record, which part this is of how many
   bool narrow;
 };
 
 struct PagedRequest {
-  int begin, rows, keys, tiles, tokens, blocks;  // tokens a tile; blocks of kPagedUnitKeys keys
+  int begin, rows, keys, first, tiles, tokens;  // tokens a tile
   bool narrow;
 };
 
@@ -58,86 +66,140 @@ AOTO_DEVICE PagedRequest paged_request(const PagedAttentionArgs& a, int r) {
   PagedRequest q;
   q.begin = min(max(a.query_start[r], 0), a.tokens);
   q.rows = min(max(a.query_start[r + 1], q.begin), a.tokens) - q.begin;
-  q.keys = min(max(a.kv_lens[r], 0), a.table_keys);
+  const int keys = max(a.kv_lens[r], 0);
+  q.keys = min(keys, a.table_keys);
+  q.first = a.causal ? keys - q.rows + 1 : 0x3FFFFFFF;
   q.narrow = !MIXED || q.rows <= a.narrow_tokens;
   q.tokens = max(1, q.narrow ? a.narrow_tokens : a.wide_tokens);  // more than 16 heads: only rowless ones are narrow
   q.tiles = (q.rows + q.tokens - 1) / q.tokens;
-  q.blocks = max(1, (q.keys + kPagedUnitKeys - 1) / kPagedUnitKeys);
   return q;
 }
 
-// The block's unit; false where there is none left. 256 threads, all of them.
-template <bool MIXED>
-AOTO_DEVICE bool paged_unit(const PagedAttentionArgs& a, int u, PagedUnit& unit) {
-  __shared__ double s_work[4];
-  __shared__ int s_units[4];
-  __shared__ PagedUnit s_unit;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int per = (a.requests + 255) / 256;
-  const int lo = min(tid * per, a.requests), hi = min(lo + per, a.requests);
-  int chunk = 1 << 23;  // whole: at most 2^30 keys
-  PagedRequest q{};
-  if (a.target > 0) {
-    double work = 0.0;
-    for (int r = lo; r < hi; ++r) {
-      q = paged_request<MIXED>(a, r);
-      work += (double)q.tiles * q.blocks;
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) work += __shfl_xor(work, d);
-    if (lane == 0) s_work[wave] = work;
-    __syncthreads();
-    work = s_work[0] + s_work[1] + s_work[2] + s_work[3];
-    chunk = max(a.least_chunk, (int)ceil(work / a.target));
-  }
-  int units = 0;
-  for (int r = lo; r < hi; ++r) {
-    if (per > 1 || a.target <= 0) q = paged_request<MIXED>(a, r);
-    units += q.tiles * ((q.blocks + chunk - 1) / chunk);
-  }
-  int upto = units;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int up = __shfl_up(upto, d);
-    if (lane >= d) upto += up;
-  }
-  if (lane == 63) s_units[wave] = upto;
-  if (tid == 0) s_unit.request = -1;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) upto += s_units[w];
-  if (u < upto && u >= upto - units) {
-    int before = upto - units;
-    for (int r = lo; r < hi; ++r) {
-      if (per > 1) q = paged_request<MIXED>(a, r);
-      const int splits = (q.blocks + chunk - 1) / chunk;
-      if (u < before + q.tiles * splits) {
-        const int tile = q.tiles - 1 - (u - before) / splits;  // the longest rows of a causal chunk first
-        PagedUnit one;
-        one.request = r;
-        one.begin = q.begin;
-        one.rows = q.rows;
-        one.keys = q.keys;
-        one.token = tile * q.tokens;
-        one.tokens = min(q.tokens, q.rows - one.token);
-        one.first = a.causal ? max(a.kv_lens[r], 0) - q.rows + 1 : 0x3FFFFFFF;
-        one.chunk = chunk;
-        one.split = (u - before) % splits;
-        one.record = u - one.split;
-        one.narrow = q.narrow;
-        // chunks of this tile: its last row's keys
-        const int end = a.causal ? min(q.keys, max(0, one.first + one.token + one.tokens - 1)) : q.keys;
-        one.keys = end;
-        one.splits = max(1, ((end + kPagedUnitKeys - 1) / kPagedUnitKeys + chunk - 1) / chunk);
-        s_unit = one;
-        break;
-      }
-      before += q.tiles * splits;
-    }
-  }
-  __syncthreads();
-  unit = s_unit;
-  return unit.request >= 0 && unit.split < unit.splits;
+// Keys that the rows of a tile see, and the blocks of them (one where there are none: the rows are written all the same).
+AOTO_DEVICE int paged_tile_keys(const PagedRequest& q, int tile) {
+  return min(q.keys, max(0, q.first + min(q.rows, (tile + 1) * q.tokens) - 1));
 }
+AOTO_DEVICE int paged_tile_blocks(const PagedRequest& q, int tile) {
+  return max(1, (paged_tile_keys(q, tile) + kPagedUnitKeys - 1) / kPagedUnitKeys);
+}
+
+// The parts that one GPU block goes through.
+template <bool MIXED>
+struct PagedWalk {
+  int request, tile, item, from;  // where it stands: the tile's number among all, its next place
+  int left;                       // places to go, those of whole items counted as they come (target 0: one item)
+  int block;                      // which of the `target`
+  int each, more;                 // places a GPU block takes; the first `more` take one more
+
+  // 256 threads, all of them; false where nothing is left for this one.
+  AOTO_DEVICE bool start(const PagedAttentionArgs& a, int u) {
+    __shared__ int s_sum[2][4];
+    __shared__ int s_at[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int per = (a.requests + 255) / 256;
+    const int lo = min(tid * per, a.requests), hi = min(lo + per, a.requests);
+    int items = 0, work = 0;
+    for (int r = lo; r < hi; ++r) {
+      const PagedRequest q = paged_request<MIXED>(a, r);
+      items += q.tiles;
+      if (a.target > 0)
+        for (int t = 0; t < q.tiles; ++t) work += kPagedLead + paged_tile_blocks(q, t);
+    }
+    int items_to = items, work_to = work;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int i = __shfl_up(items_to, d), w = __shfl_up(work_to, d);
+      if (lane >= d) items_to += i, work_to += w;
+    }
+    if (lane == 63) s_sum[0][wave] = items_to, s_sum[1][wave] = work_to;
+    if (tid == 0) s_at[0] = -1;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) items_to += s_sum[0][w], work_to += s_sum[1][w];
+      total += s_sum[1][w];
+    }
+    int at = u;  // of the items, or of the key blocks
+    block = u, each = 1, more = 0, left = 1;
+    if (a.target > 0) {
+      const int blocks = max(1, min(a.target, total / a.least_blocks));
+      each = __builtin_amdgcn_readfirstlane(total / blocks);
+      more = __builtin_amdgcn_readfirstlane(total - each * blocks);
+      at = u * each + min(u, more);
+      left = u < blocks ? each + (u < more ? 1 : 0) : 0;
+    }
+    const int upto = a.target > 0 ? work_to : items_to, mine = a.target > 0 ? work : items;
+    if (left > 0 && at < upto && at >= upto - mine) {
+      int before = upto - mine, item_before = items_to - items;
+      for (int r = lo; r < hi; ++r) {
+        const PagedRequest q = paged_request<MIXED>(a, r);
+        if (a.target > 0) {
+          int t = 0;
+          for (; t < q.tiles; ++t) {
+            const int n = kPagedLead + paged_tile_blocks(q, t);
+            if (at < before + n) break;
+            before += n;
+          }
+          if (t < q.tiles) {
+            s_at[0] = r, s_at[1] = t, s_at[2] = item_before + t, s_at[3] = at - before;
+            break;
+          }
+        } else if (at < item_before + q.tiles) {
+          // the longest rows of a causal chunk first
+          s_at[0] = r, s_at[1] = q.tiles - 1 - (at - item_before), s_at[2] = at, s_at[3] = 0;
+          break;
+        }
+        item_before += q.tiles;
+      }
+    }
+    __syncthreads();
+    request = __builtin_amdgcn_readfirstlane(s_at[0]), tile = __builtin_amdgcn_readfirstlane(s_at[1]);
+    item = __builtin_amdgcn_readfirstlane(s_at[2]), from = __builtin_amdgcn_readfirstlane(s_at[3]);
+    return request >= 0;
+  }
+
+  // The next part; false at the end. Uniform.
+  AOTO_DEVICE bool next(const PagedAttentionArgs& a, PagedUnit& unit) {
+    if (left <= 0) return false;
+    PagedRequest q = paged_request<MIXED>(a, request);
+    while (__builtin_amdgcn_readfirstlane(tile >= q.tiles)) {
+      if (++request >= a.requests) return false;
+      tile = 0;
+      q = paged_request<MIXED>(a, request);
+    }
+    // in scalar registers, which the loads above do not go to
+    q.begin = __builtin_amdgcn_readfirstlane(q.begin), q.rows = __builtin_amdgcn_readfirstlane(q.rows);
+    q.keys = __builtin_amdgcn_readfirstlane(q.keys), q.first = __builtin_amdgcn_readfirstlane(q.first);
+    q.narrow = !MIXED || q.rows <= a.narrow_tokens;
+    q.tokens = max(1, q.narrow ? a.narrow_tokens : a.wide_tokens);
+    const int n = paged_tile_blocks(q, tile);
+    unit.request = request, unit.begin = q.begin, unit.rows = q.rows, unit.first = q.first;
+    unit.keys = paged_tile_keys(q, tile);
+    unit.token = tile * q.tokens, unit.tokens = min(q.tokens, q.rows - unit.token);
+    unit.narrow = q.narrow;
+    unit.from = 0, unit.to = n, unit.record = unit.part = 0, unit.parts = 1;
+    if (a.target > 0) {
+      // of the item's places the first kPagedLead stand for its start
+      const int place = block * each + min(block, more) + (each + (block < more ? 1 : 0) - left) - from + kPagedLead;
+      left -= max(0, kPagedLead - from);
+      if (left <= 0) return false;
+      unit.from = max(0, from - kPagedLead), unit.to = min(n, unit.from + left);
+      left -= unit.to - unit.from;
+      // the GPU blocks that hold the item's first and last key block
+      const int head = owner(place), tail = owner(place + n - 1);
+      unit.record = head + item, unit.part = block - head, unit.parts = tail - head + 1;
+    } else {
+      left = 0;
+    }
+    from = 0, ++tile, ++item;
+    return true;
+  }
+  AOTO_DEVICE int owner(int at) const {
+    const int longer = more * (each + 1);
+    return __builtin_amdgcn_readfirstlane(at < longer ? at / (each + 1) : more + (at - longer) / each);
+  }
+};
 
 // The block table entry of a key.
 AOTO_DEVICE int paged_block(const PagedAttentionArgs& a, int key) {
@@ -175,12 +237,12 @@ AOTO_DEVICE float* paged_record(const PagedAttentionArgs& a, int unit, int kvh, 
   return a.records + (((size_t)unit * a.kv_heads + kvh) * a.record_rows + row) * (head_dim + 2);
 }
 
-// What a joined token needs: its tile's first unit, how many there are, its first row in their records.
+// What a joined token needs: its tile's first record, how many there are, its first row in them.
 AOTO_DEVICE void paged_note(const PagedAttentionArgs& a, const PagedUnit& unit, int kvh) {
-  if (a.target <= 0 || kvh != 0 || unit.split != 0) return;
+  if (a.target <= 0 || kvh != 0 || unit.part != 0) return;
   const int group = a.query_heads / a.kv_heads;
   for (int i = threadIdx.x; i < unit.tokens; i += 256)
-    reinterpret_cast<int4*>(a.joins)[unit.begin + unit.token + i] = make_int4(unit.record, unit.splits, i * group, 0);
+    reinterpret_cast<int4*>(a.joins)[unit.begin + unit.token + i] = make_int4(unit.record, unit.parts, i * group, 0);
 }
 
 // ---------------------------------------------------------------------------------------------------- narrow tiles
@@ -209,8 +271,7 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
   const uint16_t* values = a.values + kvh * a.head_stride + 8 * quad;
   uint16_t* vs = s.v[wave];
 
-  const int k0 = unit.split * unit.chunk * kPagedUnitKeys;
-  const int k1 = min(unit.keys, k0 + unit.chunk * kPagedUnitKeys);
+  const int k0 = unit.from * kPagedUnitKeys, k1 = min(unit.keys, unit.to * kPagedUnitKeys);
   // this wave's 32-key tiles: k0 + 32 wave + 128 i
   const int mine = k0 + 32 * wave;
   const int trips = k1 > mine ? (k1 - mine + 127) / 128 : 0;
@@ -237,15 +298,29 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
   }
   const float c2 = a.scale * 1.4426950408889634f;
 
-  // rows of the 32 keys at `base` that this lane loads: keys col and 16 + col (clamped into the chunk)
-  long long at[2];
-  auto rows = [&](int base, long long (&to)[2]) {
+  // This lane loads keys col and 16 + col of a tile. Their pages are looked up two tiles ahead, their offsets known one
+  // tile ahead: a lookup inside the tile that needs it is a round trip to memory in which nothing else is asked for.
+  int page[2], row[2];
+  auto look = [&](int base) {
 #pragma unroll
-    for (int g = 0; g < 2; ++g) to[g] = paged_row(a, table, min(base + 16 * g + col, k1 - 1));
+    for (int g = 0; g < 2; ++g) {
+      const int key = min(base + 16 * g + col, k1 - 1), block = paged_block(a, key);
+      page[g] = table[block];
+      row[g] = key - block * a.page;
+    }
   };
+  auto place = [&](long long (&to)[2]) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+      to[g] = (unsigned)page[g] < (unsigned)a.pages
+                  ? (long long)((unsigned long long)(unsigned)page[g] * (unsigned)a.page_stride) + row[g] * (int)a.slot_stride
+                  : -1;
+  };
+  long long at[2], next[2];
   uint4 kq[2][DC], vq[2][DC];
   if (trips > 0) {
-    rows(mine, at);
+    look(mine);
+    place(at);
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -254,11 +329,12 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int c = 0; c < DC; ++c) vq[g][c] = *reinterpret_cast<const uint4*>(values + max(at[g], 0LL) + 32 * c);
+    look(mine + 128);
+    place(next);
+    look(mine + 256);
   }
   for (int trip = 0; trip < trips; ++trip) {
     const int base = mine + 128 * trip;
-    long long next[2];
-    rows(min(base + 128, k1 - 1), next);
     f32x4_t sc[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -299,10 +375,12 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
         if (special) v = chunk_finite(v);
         *reinterpret_cast<uint4*>(vs + (16 * g + col) * STR + 32 * c + 8 * quad) = v;
       }
-    // the next tile's loads, K first
+    // the next tile's loads, K first, then the tile after it
     const long long old[2] = {at[0], at[1]};
 #pragma unroll
     for (int g = 0; g < 2; ++g) at[g] = next[g];
+    place(next);
+    look(base + 384);
     if (trip + 1 < trips) {
 #pragma unroll
       for (int g = 0; g < 2; ++g)
@@ -406,8 +484,8 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
       // a wave without keys holds zeros: 0 * 0
       v += f * *reinterpret_cast<const f32x4_t*>(&s.o[w][row][d]);
     }
-    if (unit.splits > 1) {
-      float* rec = paged_record(a, unit.record + unit.split, kvh, row, D);
+    if (unit.parts > 1) {
+      float* rec = paged_record(a, unit.record + unit.part, kvh, row, D);
       if (d == 0) rec[0] = big, rec[1] = sum;
       *reinterpret_cast<float2*>(rec + 2 + d) = make_float2(v[0], v[1]);
       *reinterpret_cast<float2*>(rec + 4 + d) = make_float2(v[2], v[3]);
@@ -483,8 +561,7 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   const int group = a.query_heads / a.kv_heads;
   const int live = unit.tokens * group;
   const int* table = a.block_tables + unit.request * a.table_stride;
-  const int k0 = unit.split * unit.chunk * kPagedUnitKeys;
-  const int k1 = min(unit.keys, k0 + unit.chunk * kPagedUnitKeys);
+  const int k0 = unit.from * kPagedUnitKeys, k1 = min(unit.keys, unit.to * kPagedUnitKeys);
   const int tiles = k1 > k0 ? (k1 - k0 + 63) / 64 : 0;
   const bool active = 64 * wave < live;  // a wave of none of the rows only stages
 
@@ -873,8 +950,8 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
     const float sum = xor32_sum(run_sum[c]);
     const int row = 64 * wave + 32 * c + col;
     if (row >= live) continue;
-    if (unit.splits > 1) {
-      float* rec = paged_record(a, unit.record + unit.split, kvh, row, D);
+    if (unit.parts > 1) {
+      float* rec = paged_record(a, unit.record + unit.part, kvh, row, D);
       if (half == 0) rec[0] = run_max[c], rec[1] = sum;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -906,11 +983,13 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
 template <int D, int NT>
 __device__ void paged_attention_narrow(const PagedAttentionArgs& a) {
   __shared__ __attribute__((aligned(16))) PagedNarrowShared<D, NT> s;
-  PagedUnit unit;
   const int kvh = blockIdx.x % a.kv_heads;
-  if (!paged_unit<false>(a, blockIdx.x / a.kv_heads, unit)) return;
-  paged_note(a, unit, kvh);
-  paged_narrow<D, NT>(a, unit, kvh, s);
+  PagedWalk<false> walk;
+  if (!walk.start(a, blockIdx.x / a.kv_heads)) return;
+  for (PagedUnit unit; walk.next(a, unit); __syncthreads()) {
+    paged_note(a, unit, kvh);
+    paged_narrow<D, NT>(a, unit, kvh, s);
+  }
 }
 
 template <int D>
@@ -919,55 +998,70 @@ __device__ void paged_attention_mixed(const PagedAttentionArgs& a) {
     PagedNarrowShared<D, 1> narrow;
     PagedWideShared<D> wide;
   } s;
-  PagedUnit unit;
   const int kvh = blockIdx.x % a.kv_heads;
-  if (!paged_unit<true>(a, blockIdx.x / a.kv_heads, unit)) return;
-  paged_note(a, unit, kvh);
-  if (unit.narrow) paged_narrow<D, 1>(a, unit, kvh, s.narrow);
-  else paged_wide<D>(a, unit, kvh, s.wide);
+  PagedWalk<true> walk;
+  if (!walk.start(a, blockIdx.x / a.kv_heads)) return;
+  for (PagedUnit unit; walk.next(a, unit); __syncthreads()) {
+    paged_note(a, unit, kvh);
+    if (unit.narrow) paged_narrow<D, 1>(a, unit, kvh, s.narrow);
+    else paged_wide<D>(a, unit, kvh, s.wide);
+  }
 }
 
-// A wave joins the chunks of one row: with m the largest maximum, out = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.
+// A wave joins the parts of one row: with m the largest maximum, out = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s. Bound
+// by latency: the note, then eight records at a time in one round trip.
 template <int D>
 __device__ void paged_attention_join(const PagedAttentionArgs& a) {
-  constexpr int PER = D / 64;
+  constexpr int PER = D / 64, SOME = 8;
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int t = row / a.query_heads, h = row % a.query_heads;
-  if (t >= min(a.tokens, a.query_start[a.requests])) return;
+  if (t >= a.tokens) return;
   const int4 note = reinterpret_cast<const int4*>(a.joins)[t];
-  if (note.y <= 1) return;
+  if (t >= a.query_start[a.requests] || note.y <= 1) return;
   const int group = a.query_heads / a.kv_heads, kvh = h / group, at = note.z + h % group;
   const size_t step = (size_t)a.kv_heads * a.record_rows * (D + 2);
   const float* rec = paged_record(a, note.x, kvh, at, D);
-  float big = -INFINITY;
-  for (int s = lane; s < note.y; s += 64) big = fmaxf(big, rec[s * step]);
-  big = wave_max(big);
-  float sum = 0.f, acc[PER] = {};
-  for (int s0 = 0; s0 < note.y; s0 += 64) {
-    const int s = s0 + lane;
-    const float m = s < note.y ? rec[s * step] : -INFINITY;
-    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - big);
-    sum += s < note.y ? f * rec[s * step + 1] : 0.f;
-    const int here = min(64, note.y - s0);
-#pragma unroll 4
-    for (int i = 0; i < here; ++i) {
-      const float w = __shfl(f, i);
-      const float* o = rec + (s0 + i) * step + 2 + PER * lane;
+  float big = -INFINITY, sum = 0.f, acc[PER] = {};
+  for (int s0 = 0; s0 < note.y; s0 += SOME) {
+    float m[SOME], l[SOME], o[SOME][PER];
 #pragma unroll
-      for (int e = 0; e < PER; ++e) acc[e] += w * o[e];
+    for (int i = 0; i < SOME; ++i) {
+      const float* from = rec + min(s0 + i, note.y - 1) * step;
+      m[i] = from[0], l[i] = from[1];
+#pragma unroll
+      for (int e = 0; e < PER; ++e) o[i][e] = from[2 + PER * lane + e];
+    }
+    float top = big;
+#pragma unroll
+    for (int i = 0; i < SOME; ++i) {
+      if (s0 + i >= note.y) m[i] = -INFINITY;
+      top = fmaxf(top, m[i]);
+    }
+    const float keep = big == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(big - top);
+    big = top;
+    sum *= keep;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] *= keep;
+#pragma unroll
+    for (int i = 0; i < SOME; ++i) {
+      const float f = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - big);
+      if (f != 0.f) {  // a part that sees no key has nothing finite to scale by 0
+        sum += f * l[i];
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] += f * o[i][e];
+      }
     }
   }
-  sum = wave_sum(sum);
   const float inv = big == -INFINITY ? 0.f : 1.f / sum;
   uint16_t* out = a.out + ((size_t)t * a.query_heads + h) * D + PER * lane;
-  if constexpr (PER == 2) *reinterpret_cast<uint32_t*>(out) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  if constexpr (PER == 2) *reinterpret_cast<uint32_t*>(out) = cvt_pk_bf16(acc[0] * inv, acc[1] * inv);
   else out[0] = (uint16_t)f32_to_bf16(acc[0] * inv);
 }
 
 }  // namespace aoto
 
 #define AOTO_PAGED_ATTENTION(D)                                                                                    \
-  extern "C" __global__ __launch_bounds__(256, 3) void aoto_paged_attention_d##D##_n1(PagedAttentionArgs a) {      \
+  extern "C" __global__ __launch_bounds__(256, PA_N1) void aoto_paged_attention_d##D##_n1(PagedAttentionArgs a) {      \
     aoto::paged_attention_narrow<D, 1>(a);                                                                         \
   }                                                                                                                \
   extern "C" __global__ __launch_bounds__(256, 2) void aoto_paged_attention_d##D##_n2(PagedAttentionArgs a) {      \

@@ -11,8 +11,9 @@
 // number, and the sums' noise in 32 bits (1e-7 of the total, against a typical weight of 1e-5 to 1e-6 of it) would
 // move it in a percent of the calls.
 //
-// Three launches over chunks of kVerifyChunk tokens: every row's maximum, its place and sum of weights by chunk; the
-// weights the following token is drawn from, summed by chunk; the token. Bound by the first one's read of the logits.
+// Three launches over chunks of kVerifyChunk tokens: every row's maximum, its place and sum of weights by chunk; what
+// stands, and the weights the following token is drawn from, summed by chunk; the token. Bound by the first one's read
+// of the logits and, where they are sampled from, about as much by its 20 f64 operations a logit.
 #pragma once
 
 #include "common.h"
@@ -28,33 +29,49 @@ struct VerifyChunk {
 };
 static_assert(sizeof(VerifyChunk) == kVerifyChunkBytes, "as the workspace is sized");
 
-// 2^x for x <= 0 (and -inf): the power series of 2^f = e^(f ln 2) to the 13th term over |f| <= 1/2, whose remainder
-// is below (ln 2 / 2)^14 / 14! = 4e-18, and the exponent's shift.
-AOTO_DEVICE double exp2_below(double x) {
-  x = fmax(x, -1100.0);
-  const double n = rint(x), y = (x - n) * 0.6931471805599453094;
-  double s = 1.0 / 6227020800.0;
-  s = fma(s, y, 1.0 / 479001600.0);
-  s = fma(s, y, 1.0 / 39916800.0);
-  s = fma(s, y, 1.0 / 3628800.0);
-  s = fma(s, y, 1.0 / 362880.0);
-  s = fma(s, y, 1.0 / 40320.0);
-  s = fma(s, y, 1.0 / 5040.0);
-  s = fma(s, y, 1.0 / 720.0);
-  s = fma(s, y, 1.0 / 120.0);
-  s = fma(s, y, 1.0 / 24.0);
-  s = fma(s, y, 1.0 / 6.0);
-  s = fma(s, y, 0.5);
-  s = fma(s, y, 1.0);
-  s = fma(s, y, 1.0);
-  return ldexp(s, (int)n);
+// 2^x for -2048 < x <= 0 (0 from 2^-1075 on): the series of 2^f = e^(f ln 2) over |f| <= 1/2 to the 12th power, whose
+// remainder is below (ln 2 / 2)^13 / 13! = 1.7e-16, and the exponent's shift. x = d * heat is rounded to the nearest
+// whole number by a sum with 1.5 * 2^52, whose low bits are that number; f = x - n in one rounding.
+AOTO_DEVICE double exp2_of(double d, double heat) {
+  constexpr double kRound = 6755399441055744.0;
+  const double t = fma(d, heat, kRound);
+  const double f = fma(d, heat, kRound - t);
+  double s = 2.5678435993488206e-11;  // ln 2 ^ 12 / 12!, and on to the 0th
+  s = fma(s, f, 4.4455382718708116e-10);
+  s = fma(s, f, 7.054911620801123e-09);
+  s = fma(s, f, 1.01780860092397e-07);
+  s = fma(s, f, 1.321548679014431e-06);
+  s = fma(s, f, 1.5252733804059841e-05);
+  s = fma(s, f, 0.0001540353039338161);
+  s = fma(s, f, 0.0013333558146428443);
+  s = fma(s, f, 0.009618129107628477);
+  s = fma(s, f, 0.05550410866482158);
+  s = fma(s, f, 0.24022650695910072);
+  s = fma(s, f, 0.6931471805599453);
+  s = fma(s, f, 1.0);
+  return ldexp(s, __double2loint(t));
 }
 
-// exp((z - top) / T) with heat = log2(e) / T; infinite values compare equal to an infinite top.
-AOTO_DEVICE double verify_weight(float z, float top, double heat) {
-  if (z == -INFINITY) return 0.0;
-  return z == top ? 1.0 : exp2_below(((double)z - (double)top) * heat);
-}
+// The weights exp((z - top) / T) of a row's tokens: heat = log2(e) / T. A NaN or -inf weighs 0; the logits equal to an
+// infinite top weigh 1 and nothing else does.
+struct VerifyScale {
+  double top, heat;
+  float floor;    // logits below it are taken as it, 2^-2000 of the top: 0
+  bool plain;     // nothing is infinite, and the floor is where it should be after its rounding to 32 bits
+  AOTO_DEVICE VerifyScale(float t, double h) : top(t), heat(h) {
+    floor = (float)((double)t - 2000.0 / h);
+    const double reach = (top - (double)floor) * h;
+    plain = fabsf(t) < INFINITY && reach >= 1100.0 && reach <= 4000.0;
+  }
+  AOTO_DEVICE double operator()(float z) const {
+    if (plain) return exp2_of((double)fmaxf(z, floor) - top, heat);  // fmaxf: a NaN gives the floor
+    if (!(z > -INFINITY)) return 0.0;
+    if ((double)z == top) return 1.0;
+    return top == INFINITY ? 0.0 : exp2_of(fmax(((double)z - top) * heat, -2000.0), 1.0);
+  }
+};
+
+AOTO_DEVICE double verify_weight(float z, float top, double heat) { return VerifyScale(top, heat)(z); }
 
 template <bool F32>
 AOTO_DEVICE float verify_logit(const void* row, int v) {
@@ -82,24 +99,40 @@ AOTO_DEVICE double wave_sum_f64(double v) {
   return v;
 }
 
-// The whole row's maximum, its first place and the sum of weights below it, from its chunks.
-AOTO_DEVICE VerifyChunk verify_join(const VerifyChunk* chunks, int count, double heat) {
-  VerifyChunk all{0.0, -INFINITY, 0};
-  for (int c = 0; c < count; ++c)
-    if (chunks[c].top > all.top) all.top = chunks[c].top, all.place = chunks[c].place;
-  for (int c = 0; c < count; ++c) all.sum += chunks[c].sum * verify_weight(chunks[c].top, all.top, heat);
-  return all;
-}
-
 template <bool F32>
 AOTO_DEVICE const void* verify_row(const void* base, long long at) {
   return F32 ? (const void*)(static_cast<const float*>(base) + at)
              : (const void*)(static_cast<const uint16_t*>(base) + at);
 }
 
+// Tokens v .. v + 7 of a row (-inf past `end`), in 16-byte loads where the row allows it.
+template <bool F32>
+AOTO_DEVICE void verify_load(const void* row, int v, int end, float (&z)[8]) {
+  if ((reinterpret_cast<uintptr_t>(row) & 15) == 0 && v + 8 <= end) {
+    if constexpr (F32) {
+      const float4* from = reinterpret_cast<const float4*>(static_cast<const float*>(row) + v);
+      const float4 a = from[0], b = from[1];
+      z[0] = a.x, z[1] = a.y, z[2] = a.z, z[3] = a.w, z[4] = b.x, z[5] = b.y, z[6] = b.z, z[7] = b.w;
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + v);
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[2 * i] = bf16_lo(w[i]), z[2 * i + 1] = bf16_hi(w[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = fmaxf(z[i], -INFINITY);  // a NaN counts as -inf
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = v + i < end ? verify_logit<F32>(row, v + i) : -INFINITY;
+  }
+}
+
 // Block (chunk, r * (2 drafts + 1) + i): target row i of request r (i <= drafts), or its draft row i - drafts - 1.
+// A thread has 32 logits in registers and weighs them against its own maximum; the threads' sums are then brought to
+// the block's. A greedy row's places are kept instead of weights.
 template <bool F32>
 __device__ void verify_stats(const VerifyArgs& a) {
+  constexpr int GROUPS = kVerifyChunk / 2048;
   __shared__ float s_top[4];
   __shared__ int s_place[4];
   __shared__ double s_sum[4];
@@ -114,36 +147,61 @@ __device__ void verify_stats(const VerifyArgs& a) {
                                                                 (i - a.drafts - 1) * a.draft_row_stride)
                           : verify_row<F32>(a.logits, (first + i) * a.row_stride);
   const int begin = blockIdx.x * kVerifyChunk, end = min(a.vocab, begin + kVerifyChunk);
-  float z[kVerifyChunk / 256], top = -INFINITY;
+  const int mine = begin + 8 * threadIdx.x;
+  float z[GROUPS][8];
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) verify_load<F32>(row, mine + 2048 * g, end, z[g]);
+  float top = -INFINITY;
   int place = begin;
-#pragma unroll
-  for (int e = 0; e < kVerifyChunk / 256; ++e) {
-    const int v = begin + 256 * e + threadIdx.x;
-    z[e] = v < end ? verify_logit<F32>(row, v) : -INFINITY;
-    if (z[e] > top) top = z[e], place = v;
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const float t = __shfl_xor(top, d);
-    const int p = __shfl_xor(place, d);
-    if (t > top || (t == top && p < place)) top = t, place = p;
-  }
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) s_top[wave] = top, s_place[wave] = place;
-  __syncthreads();
-  top = s_top[0], place = s_place[0];
-  for (int w = 1; w < 4; ++w)
-    if (s_top[w] > top || (s_top[w] == top && s_place[w] < place)) top = s_top[w], place = s_place[w];
   double sum = 0.0;
-  if (heat != kVerifyGreedy) {
+  const int wave = threadIdx.x >> 6;
+  if (heat == kVerifyGreedy) {
 #pragma unroll
-    for (int e = 0; e < kVerifyChunk / 256; ++e) sum += verify_weight(z[e], top, heat);
-    sum = wave_sum_f64(sum);
-    if ((threadIdx.x & 63) == 0) s_sum[wave] = sum;
-    __syncthreads();
-    sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+    for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (z[g][e] > top) top = z[g][e], place = mine + 2048 * g + e;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const float t = __shfl_xor(top, d);
+      const int p = __shfl_xor(place, d);
+      if (t > top || (t == top && p < place)) top = t, place = p;
+    }
+  } else {
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, z[g][e]);
+    const VerifyScale weight(top, heat);
+    if (weight.plain) {
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += exp2_of((double)fmaxf(z[g][e], weight.floor) - weight.top, heat);
+    } else {
+#pragma unroll 1
+      for (int k = 0; k < 8 * GROUPS; ++k) {
+        float x = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x = k == 8 * g + e ? z[g][e] : x;
+        sum += weight(x);
+      }
+    }
+    const float all = wave_max(top);
+    sum = wave_sum_f64(sum == 0.0 ? 0.0 : sum * verify_weight(top, all, heat));
+    top = all;
   }
+  if ((threadIdx.x & 63) == 0) s_top[wave] = top, s_place[wave] = place, s_sum[wave] = sum;
+  __syncthreads();
   if (threadIdx.x == 0) {
+    for (int w = 1; w < 4; ++w)
+      if (s_top[w] > top || (s_top[w] == top && s_place[w] < place)) top = s_top[w], place = s_place[w];
+    sum = 0.0;
+    if (heat != kVerifyGreedy)
+      for (int w = 0; w < 4; ++w)
+        if (s_sum[w] != 0.0) sum += s_sum[w] * verify_weight(s_top[w], top, heat);
     VerifyChunk* out = static_cast<VerifyChunk*>(a.workspace) + (size_t)blockIdx.y * a.chunks + blockIdx.x;
     *out = VerifyChunk{sum, top, place};
   }
@@ -151,96 +209,143 @@ __device__ void verify_stats(const VerifyArgs& a) {
 
 // How many drafts of request r stand, and the law that the following token is drawn from.
 struct VerifyLaw {
-  int accepted, place;     // place: the row's first maximum
+  int count, accepted;
+  int place;               // the row's first maximum
   int removed;             // a drafted token of point mass that the law leaves out, or -1
   const void* row;
   const void* draft_row;   // null: nothing is subtracted
   float top, draft_top;
   double sum, draft_sum, heat;
 };
+static_assert(sizeof(VerifyLaw) <= kVerifyLawBytes, "as the workspace is sized");
 
-// By one wave: lane i judges draft i (drafts <= 63), then the ballot finds the first that falls.
-template <bool F32>
+// By the whole block: 16 lanes join the chunks of a row, then lane i of the first wave judges draft i and the ballot
+// finds the first that falls.
+template <bool F32, int THREADS>
 AOTO_DEVICE VerifyLaw verify_law(const VerifyArgs& a, int r) {
+  __shared__ float s_top[126];
+  __shared__ double s_sum[126];
+  __shared__ int s_place[126];
+  __shared__ VerifyLaw s_law;
   int first, count;
   verify_rows(a, r, first, count);
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, part = threadIdx.x & 15;
   const double heat = verify_heat(a, r);
+  const bool sampled = heat != kVerifyGreedy, laws = a.draft_logits && sampled;
   const VerifyChunk* chunks = static_cast<const VerifyChunk*>(a.workspace) + (size_t)r * (2 * a.drafts + 1) * a.chunks;
-  VerifyChunk p{0.0, -INFINITY, 0}, q{0.0, -INFINITY, 0};
-  bool stands = false;
-  const bool sampled = heat != kVerifyGreedy;
-  if (lane <= count) p = verify_join(chunks + (size_t)lane * a.chunks, a.chunks, heat);
-  if (lane < count) {
-    const long long x = a.draft_tokens[(size_t)r * a.drafts + lane];
-    if (a.draft_logits && sampled) q = verify_join(chunks + (size_t)(a.drafts + 1 + lane) * a.chunks, a.chunks, heat);
-    if (x >= 0 && x < a.vocab) {
-      if (sampled) {
-        const double px = verify_weight(verify_logit<F32>(verify_row<F32>(a.logits, (first + lane) * a.row_stride), (int)x),
-                                        p.top, heat);
-        double qx = 1.0;
-        if (a.draft_logits) {
-          const float z = verify_logit<F32>(
-              verify_row<F32>(a.draft_logits, r * a.draft_request_stride + lane * a.draft_row_stride), (int)x);
-          qx = q.sum > 0.0 ? verify_weight(z, q.top, heat) / q.sum : 0.0;
+  const int rows = count + 1 + (laws && count > 0 ? count : 0);
+  for (int j0 = 0; j0 < rows; j0 += THREADS / 16) {
+    const int j = j0 + (threadIdx.x >> 4);
+    const bool live = j < rows;
+    const VerifyChunk* from = chunks + (size_t)(j <= count ? j : a.drafts + j - count) * a.chunks;
+    float top = -INFINITY;
+    int place = 0;
+    for (int c = part; live && c < a.chunks; c += 16)
+      if (from[c].top > top) top = from[c].top, place = from[c].place;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+      const float t = __shfl_xor(top, d);
+      const int p = __shfl_xor(place, d);
+      if (t > top || (t == top && p < place)) top = t, place = p;
+    }
+    double sum = 0.0;
+    if (sampled) {
+      for (int c = part; live && c < a.chunks; c += 16)
+        if (from[c].sum != 0.0) sum += from[c].sum * verify_weight(from[c].top, top, heat);
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor(sum, d);
+    }
+    if (live && part == 0) s_top[j] = top, s_sum[j] = sum, s_place[j] = top > -INFINITY ? place : 0;
+  }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    bool stands = false;
+    if (lane < count) {
+      const long long x = a.draft_tokens[(size_t)r * a.drafts + lane];
+      if (x >= 0 && x < a.vocab) {
+        if (sampled) {
+          const float z = verify_logit<F32>(verify_row<F32>(a.logits, (first + lane) * a.row_stride), (int)x);
+          const double px = s_sum[lane] > 0.0 ? verify_weight(z, s_top[lane], heat) / s_sum[lane] : 0.0;
+          double qx = 1.0;
+          if (laws) {
+            const float y = verify_logit<F32>(
+                verify_row<F32>(a.draft_logits, r * a.draft_request_stride + lane * a.draft_row_stride), (int)x);
+            const int j = count + 1 + lane;
+            qx = s_sum[j] > 0.0 ? verify_weight(y, s_top[j], heat) / s_sum[j] : 0.0;
+          }
+          stands = (double)a.uniforms[(size_t)r * (a.drafts + 1) + lane] * qx < px;
+        } else {
+          stands = s_top[lane] > -INFINITY && s_place[lane] == (int)x;
         }
-        stands = p.sum > 0.0 && (double)a.uniforms[(size_t)r * (a.drafts + 1) + lane] * qx < px / p.sum;
-      } else {
-        stands = p.top > -INFINITY && p.place == (int)x;
       }
     }
-  }
-  const unsigned long long falls = ~__ballot(stands);
-  VerifyLaw law{};
-  const int k = min(max(count, 0), __ffsll((long long)falls) - 1);
-  law.accepted = k;
-  law.heat = heat;
-  law.place = __shfl(p.place, k);
-  law.top = __shfl(p.top, k);
-  law.sum = __shfl(p.sum, k);
-  law.row = verify_row<F32>(a.logits, (long long)min(first + k, a.rows - 1) * a.row_stride);
-  law.removed = -1;
-  if (k < count && sampled) {
-    if (a.draft_logits) {
-      law.draft_row = verify_row<F32>(a.draft_logits, r * a.draft_request_stride + k * a.draft_row_stride);
-      law.draft_top = __shfl(q.top, k);
-      law.draft_sum = __shfl(q.sum, k);
-    } else {
-      const long long x = a.draft_tokens[(size_t)r * a.drafts + k];
-      law.removed = x >= 0 && x < a.vocab ? (int)x : -1;
+    const int k = min(max(count, 0), __ffsll(~__ballot(stands)) - 1);
+    if (lane == 0) {
+      VerifyLaw law{};
+      law.count = count, law.accepted = k, law.heat = heat, law.removed = -1;
+      law.row = verify_row<F32>(a.logits, (long long)min(first + k, a.rows - 1) * a.row_stride);
+      if (count >= 0) law.place = s_place[k], law.top = s_top[k], law.sum = s_sum[k];
+      if (k < count && sampled) {
+        if (laws) {
+          law.draft_row = verify_row<F32>(a.draft_logits, r * a.draft_request_stride + k * a.draft_row_stride);
+          law.draft_top = s_top[count + 1 + k], law.draft_sum = s_sum[count + 1 + k];
+        } else {
+          const long long x = a.draft_tokens[(size_t)r * a.drafts + k];
+          law.removed = x >= 0 && x < a.vocab ? (int)x : -1;
+        }
+      }
+      s_law = law;
     }
   }
-  return law;
+  __syncthreads();
+  return s_law;
 }
 
-// The weight of token v under the target's law and what is left of it.
+// The weights of tokens v .. v + 7 under the target's law and what is left of them.
 template <bool F32>
-AOTO_DEVICE void verify_left(const VerifyLaw& law, int v, double& whole, double& left) {
-  whole = law.sum > 0.0 ? verify_weight(verify_logit<F32>(law.row, v), law.top, law.heat) / law.sum : 0.0;
-  left = v == law.removed ? 0.0 : whole;
-  if (law.draft_row && law.draft_sum > 0.0)
-    left = fmax(whole - verify_weight(verify_logit<F32>(law.draft_row, v), law.draft_top, law.heat) / law.draft_sum, 0.0);
+AOTO_DEVICE void verify_left(const VerifyLaw& law, int v, int end, double (&whole)[8], double (&left)[8]) {
+  float z[8];
+  verify_load<F32>(law.row, v, end, z);
+  const VerifyScale weight(law.top, law.heat);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    whole[i] = law.sum > 0.0 && v + i < end ? weight(z[i]) : 0.0;
+    left[i] = v + i == law.removed ? 0.0 : whole[i];
+  }
+  if (law.draft_row && law.draft_sum > 0.0) {
+    // p - q, times the target's sum
+    const double ratio = law.sum / law.draft_sum;
+    const VerifyScale other(law.draft_top, law.heat);
+    verify_load<F32>(law.draft_row, v, end, z);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) left[i] = v + i < end ? fmax(whole[i] - ratio * other(z[i]), 0.0) : 0.0;
+  }
 }
 
 AOTO_DEVICE double* verify_masses(const VerifyArgs& a, int r) {
   const size_t chunks = (size_t)a.requests * (2 * a.drafts + 1) * a.chunks;
   return reinterpret_cast<double*>(static_cast<VerifyChunk*>(a.workspace) + chunks) + (size_t)r * 2 * a.chunks;
 }
+AOTO_DEVICE VerifyLaw* verify_laws(const VerifyArgs& a) {
+  return reinterpret_cast<VerifyLaw*>(verify_masses(a, a.requests));
+}
 
-// Block (chunk, r): the chunk's sums of what is left and of the whole.
+// Block (chunk, r): the chunk's sums of what is left and of the whole; the first one's law is kept.
 template <bool F32>
 __device__ void verify_mass(const VerifyArgs& a) {
   __shared__ double s_sum[4][2];
   const int r = blockIdx.y;
-  if (verify_heat(a, r) == kVerifyGreedy) return;
-  const VerifyLaw law = verify_law<F32>(a, r);
+  const VerifyLaw law = verify_law<F32, 256>(a, r);
+  if (blockIdx.x == 0 && threadIdx.x == 0) verify_laws(a)[r] = law;
+  if (law.heat == kVerifyGreedy) return;
   const int begin = blockIdx.x * kVerifyChunk, end = min(a.vocab, begin + kVerifyChunk);
   double sums[2] = {0.0, 0.0};
-  for (int v = begin + threadIdx.x; v < end; v += 256) {
-    double whole, left;
-    verify_left<F32>(law, v, whole, left);
-    sums[0] += left;
-    sums[1] += whole;
+#pragma unroll 1
+  for (int v = begin + 8 * threadIdx.x; v < end; v += 2048) {
+    double whole[8], left[8];
+    verify_left<F32>(law, v, end, whole, left);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sums[0] += left[i], sums[1] += whole[i];
   }
   for (int i = 0; i < 2; ++i) {
     sums[i] = wave_sum_f64(sums[i]);
@@ -252,83 +357,90 @@ __device__ void verify_mass(const VerifyArgs& a) {
         s_sum[0][threadIdx.x] + s_sum[1][threadIdx.x] + s_sum[2][threadIdx.x] + s_sum[3][threadIdx.x];
 }
 
-// Block r: the chunk in which the running sum passes, then the token in it.
-template <bool F32>
+// Running sums over a wave.
+AOTO_DEVICE double wave_scan_f64(double v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const double up = __shfl_up(v, d);
+    if ((int)(threadIdx.x & 63) >= d) v += up;
+  }
+  return v;
+}
+
+// Block r, 1024 threads: the chunk in which the running sum passes, then the token in it, eight a thread.
+template <bool F32, bool KEPT>
 __device__ void verify_pick(const VerifyArgs& a) {
-  __shared__ double s_sum[256];
-  __shared__ int s_last[256];
-  const int r = blockIdx.x;
-  const VerifyLaw law = verify_law<F32>(a, r);
-  int first, count;
-  verify_rows(a, r, first, count);
+  static_assert(kVerifyChunk == 8 * 1024, "a chunk is eight tokens a thread");
+  __shared__ double s_sum[16], s_before;
+  __shared__ int s_chunk, s_token, s_last;
+  const int r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  VerifyLaw law;
+  if constexpr (KEPT) law = verify_laws(a)[r];
+  else law = verify_law<F32, 1024>(a, r);
   long long token = law.place;
-  if (count >= 0 && law.heat != kVerifyGreedy) {
+  if (KEPT && law.count >= 0 && law.heat != kVerifyGreedy) {
+    const float u = a.uniforms[(size_t)r * (a.drafts + 1) + a.drafts];
     const double* masses = verify_masses(a, r);
     double total = 0.0;
-    for (int c = 0; c < a.chunks; ++c) total += masses[c];
+    for (int c = 0; c < a.chunks; c += 64) total += wave_sum_f64(c + lane < a.chunks ? masses[c + lane] : 0.0);
     const bool whole = !(total > 0.0);
     if (whole) {
       masses += a.chunks;
       total = 0.0;
-      for (int c = 0; c < a.chunks; ++c) total += masses[c];
+      for (int c = 0; c < a.chunks; c += 64) total += wave_sum_f64(c + lane < a.chunks ? masses[c + lane] : 0.0);
     }
-    const double target = (double)a.uniforms[(size_t)r * (a.drafts + 1) + a.drafts] * total;
-    // the chunk; past the total (a random number of 1, or the sums' last bits) the last one that has weight
-    double before = 0.0, run = 0.0;
-    int chunk = 0;
-    for (int c = 0; c < a.chunks; ++c) {
-      const double mass = masses[c];
-      if (mass > 0.0) {
-        chunk = c, before = run;
-        if (run + mass > target) break;
+    const double target = (double)u * total;
+    if (wave == 0) {
+      // the chunk; past the total (a random number of 1, or the sums' last bits) the last one that has weight
+      double run = 0.0, before = 0.0;
+      int chunk = 0;
+      for (int c = 0; c < a.chunks; c += 64) {
+        const double mass = c + lane < a.chunks ? masses[c + lane] : 0.0;
+        const double upto = run + wave_scan_f64(mass);
+        const unsigned long long some = __ballot(mass > 0.0), past = __ballot(mass > 0.0 && upto > target);
+        const int at = past ? __ffsll(past) - 1 : some ? 63 - __clzll((long long)some) : -1;
+        if (at >= 0) chunk = c + at, before = __shfl(upto - mass, at);
+        if (past) break;
+        run = __shfl(upto, 63);
       }
-      run += mass;
+      if (lane == 0) s_chunk = chunk, s_before = before;
     }
-    // a thread sums its run of tokens, then walks it if the sum passes there
-    const int begin = chunk * kVerifyChunk, end = min(a.vocab, begin + kVerifyChunk);
-    const int mine = begin + threadIdx.x * (kVerifyChunk / 256), stop = min(end, mine + kVerifyChunk / 256);
+    if (threadIdx.x == 0) s_token = 0x7FFFFFFF, s_last = -1;
+    __syncthreads();
+    const int begin = s_chunk * kVerifyChunk, end = min(a.vocab, begin + kVerifyChunk);
+    const int v = begin + 8 * threadIdx.x;
+    double all[8], left[8];
+    verify_left<F32>(law, v, end, all, left);
     double sum = 0.0;
     int last = -1;
-    for (int v = mine; v < stop; ++v) {
-      double all, left;
-      verify_left<F32>(law, v, all, left);
-      const double w = whole ? all : left;
-      sum += w;
-      if (w > 0.0) last = v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (whole) left[i] = all[i];
+      sum += left[i];
+      if (left[i] > 0.0) last = v + i;
     }
-    s_sum[threadIdx.x] = sum;
-    s_last[threadIdx.x] = last;
+    const double upto = wave_scan_f64(sum);
+    if (lane == 63) s_sum[wave] = upto;
     __syncthreads();
-    double at = before;
-    int owner = -1, final = -1;
-    double from = 0.0;
-    for (int i = 0; i < 256; ++i) {
-      if (s_last[i] >= 0) {
-        final = s_last[i];
-        if (owner < 0 && at + s_sum[i] > target) owner = i, from = at;
-      }
-      at += s_sum[i];
+    double run = s_before;
+    for (int w = 0; w < wave; ++w) run += s_sum[w];
+    run += upto - sum;
+    int found = 0x7FFFFFFF;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      run += left[i];
+      if (left[i] > 0.0 && run > target) found = min(found, v + i);
     }
-    token = final >= 0 ? final : law.place;
-    if (owner >= 0) {
-      token = s_last[owner];
-      int v = begin + owner * (kVerifyChunk / 256);
-      const int until = min(end, v + kVerifyChunk / 256);
-      for (; v < until; ++v) {
-        double all, left;
-        verify_left<F32>(law, v, all, left);
-        from += whole ? all : left;
-        if (from > target) {
-          token = v;
-          break;
-        }
-      }
-    }
+    if (found != 0x7FFFFFFF) atomicMin(&s_token, found);
+    if (last >= 0) atomicMax(&s_last, last);
+    __syncthreads();
+    if (s_token != 0x7FFFFFFF) token = s_token;
+    else if (s_last >= 0) token = s_last;
   }
-  for (int i = threadIdx.x; i <= a.drafts; i += 256) {
+  for (int i = threadIdx.x; i <= a.drafts; i += 1024) {
     long long out = -1;
-    if (count >= 0 && i < law.accepted) out = a.draft_tokens[(size_t)r * a.drafts + i];
-    if (count >= 0 && i == law.accepted) out = token;
+    if (law.count >= 0 && i < law.accepted) out = a.draft_tokens[(size_t)r * a.drafts + i];
+    if (law.count >= 0 && i == law.accepted) out = token;
     a.tokens_out[(size_t)r * (a.drafts + 1) + i] = out;
   }
   if (threadIdx.x == 0) a.accepted[r] = law.accepted;
@@ -336,13 +448,16 @@ __device__ void verify_pick(const VerifyArgs& a) {
 
 }  // namespace aoto
 
-#define AOTO_VERIFY_INSTANCE(NAME, F32)                                                               \
-  extern "C" __global__ __launch_bounds__(256) void aoto_verify_stats_##NAME(VerifyArgs a) {          \
-    aoto::verify_stats<F32>(a);                                                                       \
-  }                                                                                                   \
-  extern "C" __global__ __launch_bounds__(256) void aoto_verify_mass_##NAME(VerifyArgs a) {           \
-    aoto::verify_mass<F32>(a);                                                                        \
-  }                                                                                                   \
-  extern "C" __global__ __launch_bounds__(256) void aoto_verify_pick_##NAME(VerifyArgs a) {           \
-    aoto::verify_pick<F32>(a);                                                                        \
+#define AOTO_VERIFY_INSTANCE(NAME, F32)                                                                  \
+  extern "C" __global__ __launch_bounds__(256) void aoto_verify_stats_##NAME(VerifyArgs a) {             \
+    aoto::verify_stats<F32>(a);                                                                          \
+  }                                                                                                      \
+  extern "C" __global__ __launch_bounds__(256) void aoto_verify_mass_##NAME(VerifyArgs a) {              \
+    aoto::verify_mass<F32>(a);                                                                           \
+  }                                                                                                      \
+  extern "C" __global__ __launch_bounds__(1024) void aoto_verify_pick_##NAME(VerifyArgs a) {             \
+    aoto::verify_pick<F32, true>(a);                                                                     \
+  }                                                                                                      \
+  extern "C" __global__ __launch_bounds__(1024) void aoto_verify_greedy_##NAME(VerifyArgs a) {           \
+    aoto::verify_pick<F32, false>(a);                                                                    \
   }

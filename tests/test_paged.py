@@ -4,6 +4,7 @@ host and the exactness of the verification's exponential."""
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 import pytest
@@ -151,13 +152,16 @@ def test_attention_of_the_restatement_by_hand():
 
 
 def test_exponential_series_is_exact_to_the_last_bits():
-    # the series that the verification takes 2^x with: its remainder and roundings stay below 4 steps of 2^-53
-    x = -np.concatenate([np.linspace(0, 60, 20001), np.linspace(0, 1, 5001)])
-    n = np.rint(x)
-    y = (x - n) * np.log(2.0)
-    s = np.full_like(y, 1.0 / 6227020800.0)
-    for k in (479001600.0, 39916800.0, 3628800.0, 362880.0, 40320.0, 5040.0, 720.0, 120.0, 24.0, 6.0, 2.0, 1.0, 1.0):
-        s = s * y + 1.0 / k
-    got = np.ldexp(s, n.astype(int))
-    exact = np.exp2(x.astype(np.longdouble))
-    assert np.max(np.abs(got - exact) / exact) < 4 * 2.0 ** -53
+    # the series that the verification takes 2^x with, its rounding of x by a sum with 1.5 * 2^52 included: below
+    # 4 steps of 2^-53 (a remainder of 1.7e-16 over 2^f >= 0.7, and the last products' roundings)
+    x = -np.concatenate([np.linspace(0, 60, 20001), np.linspace(0, 1, 5001), [1000.0, 1999.5]])
+    whole = (x + 6755399441055744.0) - 6755399441055744.0
+    f = x - whole
+    assert np.abs(f).max() <= 0.5
+    s = np.zeros_like(f)
+    for k in range(12, -1, -1):
+        s = s * f + np.float64(np.log(np.longdouble(2)) ** k / np.longdouble(math.factorial(k)))
+    got = np.ldexp(s, whole.astype(int))
+    exact = np.exp2(x.astype(np.longdouble)).astype(np.float64)
+    assert np.all(np.abs(got - exact) <= 4 * 2.0 ** -53 * exact)
+    assert got[-1] == 0.0  # what weighs less than any number weighs nothing
