@@ -3,7 +3,6 @@
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
-#include <cstdlib>
 
 #include "aoto_hip.h"
 #include "internal.h"
@@ -64,9 +63,6 @@ AttentionPlan attention_plan(int tokens, int requests, int max_blocks, int page,
   p.units = tiles;
   if (keys > kLeastBlocks * 128 && tiles * kv_heads < (p.wide ? 1 : 4) * full && tiles * most < (1 << 30)) {
     p.target = (int)((full + kv_heads - 1) / kv_heads);
-#ifdef PA_TUNE
-    if (getenv("PA_T")) p.target = (atoi(getenv("PA_T")) + kv_heads - 1) / kv_heads;
-#endif
     p.units += p.target;
     p.workspace = (size_t)tokens * 16 + (size_t)p.units * kv_heads * (p.wide ? kWideRows : p.narrow_rows) *
                                             (head_dim + 2) * sizeof(float);
@@ -201,7 +197,7 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
 size_t aoto_hip_verify_draft_workspace(int requests, int drafts, int vocab) {
   if (requests <= 0 || drafts < 0 || vocab <= 0) return 0;
   const size_t chunks = ((size_t)vocab + kVerifyChunk - 1) / kVerifyChunk;
-  return (size_t)requests * (chunks * ((2 * (size_t)drafts + 1) * kVerifyChunkBytes + 2 * sizeof(double)) + kVerifyLawBytes);
+  return (size_t)requests * (chunks * ((2 * (size_t)drafts + 1) * kVerifyChunkBytes + sizeof(double)) + kVerifyLawBytes);
 }
 
 int aoto_hip_verify_draft(const void* logits, int logits_f32, int64_t row_stride, int rows, int vocab,
@@ -225,17 +221,18 @@ int aoto_hip_verify_draft(const void* logits, int logits_f32, int64_t row_stride
   a.accepted = accepted, a.workspace = workspace, a.row_stride = row_stride;
   a.draft_request_stride = draft_request_stride, a.draft_row_stride = draft_row_stride, a.rows = rows;
   a.requests = requests, a.drafts = drafts, a.vocab = vocab, a.chunks = (vocab - 1) / kVerifyChunk + 1;
-  const long long per = 2LL * drafts + 1;
-  if (requests * per > 65535)
+  a.judged = temperature && a.draft_logits ? 2 * drafts + 1 : drafts + 1;
+  if ((long long)requests * a.judged > 65535)
     return set_error(AOTO_ERR_UNSUPPORTED, "verify_draft: %d requests of %d drafts", requests, drafts);
-  if (int s = launch(logits_f32 ? "aoto_verify_stats_f32" : "aoto_verify_stats_bf16", a.chunks, requests * per, 256,
-                     stream, a))
+  if (int s = launch(logits_f32 ? "aoto_verify_stats_f32" : "aoto_verify_stats_bf16", (a.chunks + 3) / 4,
+                     (long long)requests * a.judged, 256, stream, a))
     return s;
-  if (!temperature)
-    return launch(logits_f32 ? "aoto_verify_greedy_f32" : "aoto_verify_greedy_bf16", requests, 1, 1024, stream, a);
+  if (!temperature || !a.draft_logits)
+    return launch(logits_f32 ? "aoto_verify_follow_f32" : "aoto_verify_follow_bf16", requests, 1, 512, stream, a);
+  if (int s = launch(logits_f32 ? "aoto_verify_law_f32" : "aoto_verify_law_bf16", requests, 1, 256, stream, a)) return s;
   if (int s = launch(logits_f32 ? "aoto_verify_mass_f32" : "aoto_verify_mass_bf16", a.chunks, requests, 256, stream, a))
     return s;
-  return launch(logits_f32 ? "aoto_verify_pick_f32" : "aoto_verify_pick_bf16", requests, 1, 1024, stream, a);
+  return launch(logits_f32 ? "aoto_verify_pick_f32" : "aoto_verify_pick_bf16", requests, 1, 512, stream, a);
 }
 
 }  // extern "C"

@@ -61,10 +61,10 @@ struct PagedAttentionArgs {
   float scale;
 };
 
-// Tokens of a vocabulary that one block of the verification takes, and the bytes of what it leaves of a row of them.
-constexpr int kVerifyChunk = 8192;
+// Tokens of a vocabulary that one wave of the verification takes, and the bytes of what it leaves of a row of them.
+constexpr int kVerifyChunk = 4096;
 constexpr int kVerifyChunkBytes = 16;
-constexpr int kVerifyLawBytes = 80;  // what stands of a request's drafts, and where its token comes from
+constexpr int kVerifyLawBytes = 96;  // what stands of a request's drafts, and where its token comes from
 
 struct VerifyArgs {
   const void* logits;
@@ -78,4 +78,5 @@ struct VerifyArgs {
   void* workspace;
   long long row_stride, draft_request_stride, draft_row_stride;
   int rows, requests, drafts, vocab, chunks;
+  int judged;  // rows of a request that have statistics: the target's drafts + 1, and the drafts' where they matter
 };

@@ -40,10 +40,7 @@ AOTO_DEVICE uint32_t paged_lds(const void* p) {
 constexpr int kPagedUnitKeys = 128;  // keys of a key block
 // What starting on an item costs (its rows, table entries and first keys are three round trips to memory), in key
 // blocks: a GPU block that goes from one item to another takes so many fewer.
-#ifndef PA_LEAD
-#define PA_LEAD 2
-#endif
-constexpr int kPagedLead = PA_LEAD;
+constexpr int kPagedLead = 2;
 constexpr int kPagedWideRows = 256;
 
 struct PagedUnit {
@@ -90,11 +87,12 @@ struct PagedWalk {
   int left;                       // places to go, those of whole items counted as they come (target 0: one item)
   int block;                      // which of the `target`
   int each, more;                 // places a GPU block takes; the first `more` take one more
+  PagedRequest q;                 // the request it stands at
 
   // 256 threads, all of them; false where nothing is left for this one.
   AOTO_DEVICE bool start(const PagedAttentionArgs& a, int u) {
     __shared__ int s_sum[2][4];
-    __shared__ int s_at[4];
+    __shared__ int s_at[8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int per = (a.requests + 255) / 256;
     const int lo = min(tid * per, a.requests), hi = min(lo + per, a.requests);
@@ -143,11 +141,13 @@ struct PagedWalk {
           }
           if (t < q.tiles) {
             s_at[0] = r, s_at[1] = t, s_at[2] = item_before + t, s_at[3] = at - before;
+            s_at[4] = q.begin, s_at[5] = q.rows, s_at[6] = q.keys, s_at[7] = q.first;
             break;
           }
         } else if (at < item_before + q.tiles) {
           // the longest rows of a causal chunk first
           s_at[0] = r, s_at[1] = q.tiles - 1 - (at - item_before), s_at[2] = at, s_at[3] = 0;
+          s_at[4] = q.begin, s_at[5] = q.rows, s_at[6] = q.keys, s_at[7] = q.first;
           break;
         }
         item_before += q.tiles;
@@ -156,23 +156,28 @@ struct PagedWalk {
     __syncthreads();
     request = __builtin_amdgcn_readfirstlane(s_at[0]), tile = __builtin_amdgcn_readfirstlane(s_at[1]);
     item = __builtin_amdgcn_readfirstlane(s_at[2]), from = __builtin_amdgcn_readfirstlane(s_at[3]);
+    q.begin = s_at[4], q.rows = s_at[5], q.keys = s_at[6], q.first = s_at[7];
+    settle(a);
     return request >= 0;
+  }
+  // The request's numbers in scalar registers, which loads do not go to, and what follows from them.
+  AOTO_DEVICE void settle(const PagedAttentionArgs& a) {
+    q.begin = __builtin_amdgcn_readfirstlane(q.begin), q.rows = __builtin_amdgcn_readfirstlane(q.rows);
+    q.keys = __builtin_amdgcn_readfirstlane(q.keys), q.first = __builtin_amdgcn_readfirstlane(q.first);
+    q.narrow = !MIXED || q.rows <= a.narrow_tokens;
+    q.tokens = max(1, q.narrow ? a.narrow_tokens : a.wide_tokens);
+    q.tiles = (q.rows + q.tokens - 1) / q.tokens;
   }
 
   // The next part; false at the end. Uniform.
   AOTO_DEVICE bool next(const PagedAttentionArgs& a, PagedUnit& unit) {
     if (left <= 0) return false;
-    PagedRequest q = paged_request<MIXED>(a, request);
-    while (__builtin_amdgcn_readfirstlane(tile >= q.tiles)) {
+    while (tile >= q.tiles) {
       if (++request >= a.requests) return false;
       tile = 0;
       q = paged_request<MIXED>(a, request);
+      settle(a);
     }
-    // in scalar registers, which the loads above do not go to
-    q.begin = __builtin_amdgcn_readfirstlane(q.begin), q.rows = __builtin_amdgcn_readfirstlane(q.rows);
-    q.keys = __builtin_amdgcn_readfirstlane(q.keys), q.first = __builtin_amdgcn_readfirstlane(q.first);
-    q.narrow = !MIXED || q.rows <= a.narrow_tokens;
-    q.tokens = max(1, q.narrow ? a.narrow_tokens : a.wide_tokens);
     const int n = paged_tile_blocks(q, tile);
     unit.request = request, unit.begin = q.begin, unit.rows = q.rows, unit.first = q.first;
     unit.keys = paged_tile_keys(q, tile);
@@ -300,27 +305,34 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
 
   // This lane loads keys col and 16 + col of a tile. Their pages are looked up two tiles ahead, their offsets known one
   // tile ahead: a lookup inside the tile that needs it is a round trip to memory in which nothing else is asked for.
-  int page[2], row[2];
+  struct Rows {
+    int page[2], row[2];
+  };
   auto look = [&](int base) {
+    Rows of;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const int key = min(base + 16 * g + col, k1 - 1), block = paged_block(a, key);
-      page[g] = table[block];
-      row[g] = key - block * a.page;
+      of.page[g] = table[block];
+      of.row[g] = key - block * a.page;
     }
+    return of;
   };
-  auto place = [&](long long (&to)[2]) {
+  auto place = [&](const Rows& of, long long (&to)[2]) {
 #pragma unroll
     for (int g = 0; g < 2; ++g)
-      to[g] = (unsigned)page[g] < (unsigned)a.pages
-                  ? (long long)((unsigned long long)(unsigned)page[g] * (unsigned)a.page_stride) + row[g] * (int)a.slot_stride
+      to[g] = (unsigned)of.page[g] < (unsigned)a.pages
+                  ? (long long)((unsigned long long)(unsigned)of.page[g] * (unsigned)a.page_stride) +
+                        of.row[g] * (int)a.slot_stride
                   : -1;
   };
   long long at[2], next[2];
   uint4 kq[2][DC], vq[2][DC];
+  Rows ahead;
   if (trips > 0) {
-    look(mine);
-    place(at);
+    const Rows now = look(mine), then = look(mine + 128);
+    ahead = look(mine + 256);
+    place(now, at);
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -329,9 +341,7 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int c = 0; c < DC; ++c) vq[g][c] = *reinterpret_cast<const uint4*>(values + max(at[g], 0LL) + 32 * c);
-    look(mine + 128);
-    place(next);
-    look(mine + 256);
+    place(then, next);
   }
   for (int trip = 0; trip < trips; ++trip) {
     const int base = mine + 128 * trip;
@@ -379,8 +389,8 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
     const long long old[2] = {at[0], at[1]};
 #pragma unroll
     for (int g = 0; g < 2; ++g) at[g] = next[g];
-    place(next);
-    look(base + 384);
+    place(ahead, next);
+    ahead = look(base + 384);
     if (trip + 1 < trips) {
 #pragma unroll
       for (int g = 0; g < 2; ++g)
@@ -588,33 +598,37 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   const int last_block = paged_block(a, max(k1 - 1, 0));
   const int page_span = a.page * (int)a.slot_stride;
   const int step_blocks = paged_block(a, 64), step_off = (64 - step_blocks * a.page) * (int)a.slot_stride;
-  // of the tile looked up next: the rows' table entries and offsets in their pages; of the one before, page and offset
-  int block[LOADS], off[LOADS], page[LOADS], off_page[LOADS];
+  // of the tile looked up next: the rows' table entries and offsets in their pages; of one looked up, pages and offsets
+  struct Rows {
+    int page[LOADS], off[LOADS];
+  };
+  int block[LOADS], off[LOADS];
+  Rows ahead;
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
     const int key = k0 + 4 * RPL * i + stage_row;
     block[i] = paged_block(a, key);
     off[i] = (key - block[i] * a.page) * (int)a.slot_stride;
   }
-  auto look_row = [&](int i) __attribute__((always_inline)) {
-    page[i] = table[min(block[i], last_block)];
-    off_page[i] = off[i];
+  auto look_row = [&](int i, Rows& to) __attribute__((always_inline)) {
+    to.page[i] = table[min(block[i], last_block)];
+    to.off[i] = off[i];
     off[i] += step_off;
     const bool over = off[i] >= page_span;
     off[i] -= over ? page_span : 0;
     block[i] += step_blocks + (over ? 1 : 0);
   };
-  auto look = [&] {
+  auto look = [&](Rows& to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) look_row(i);
+    for (int i = 0; i < LOADS; ++i) look_row(i, to);
   };
-  auto place = [&](int tile, long long (&at)[LOADS]) {
+  auto place = [&](int tile, const Rows& of, long long (&at)[LOADS]) __attribute__((always_inline)) {
     bool fine = true;
     bool there[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const bool known = (unsigned)page[i] < (unsigned)a.pages;
-      at[i] = (long long)((unsigned long long)(unsigned)(known ? page[i] : 0) * (unsigned)a.page_stride) + off_page[i];
+      const bool known = (unsigned)of.page[i] < (unsigned)a.pages;
+      at[i] = (long long)((unsigned long long)(unsigned)(known ? of.page[i] : 0) * (unsigned)a.page_stride) + of.off[i];
       there[i] = known && k0 + 64 * tile + 4 * RPL * i + stage_row < k1;
       fine = fine && there[i];
     }
@@ -851,15 +865,16 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   // tile t + 3 are looked up.
   long long at_k[LOADS], at_v[LOADS];
   if (tiles > 0) {
-    look();
-    place(0, at_v);
+    Rows now, then;
+    look(now);
+    look(then);
+    look(ahead);
+    place(0, now, at_v);
     fetch(keys, at_v, lds_k0);
     fetch(values, at_v, lds_v0);
-    look();
-    place(1, at_v);
+    place(1, then, at_v);
     fetch(keys, at_v, lds_k0 + TILEB);
-    look();
-    place(2, at_k);
+    place(2, ahead, at_k);
     paged_landed();
     __syncthreads();
     if (active) {
@@ -887,13 +902,13 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   auto stage = [&](int t, int kb) {
     fetch(keys, at_k, lds_k0 + (kb == 0 ? 2 : kb - 1) * TILEB);
     fetch(values, at_v, lds_v0 + ((t + 1) & 1) * TILEB);
-    look();
+    look(ahead);
   };
   auto staged = [&](int t) {
     paged_landed();
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) at_v[i] = at_k[i];
-    place(t + 3, at_k);
+    place(t + 3, ahead, at_k);
     __syncthreads();
   };
   // The two steps of a tile. `edge` (a compile-time bool): keys that a row may not see or that are of no page may be
@@ -904,7 +919,7 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
     step(vb, 0, lds_k + kb * TILEB, 1, kn, 0, [&](int i) __attribute__((always_inline)) {
       if (i < LOADS) fetch_row(keys, at_k, to_k, i);
       else if (i < 2 * LOADS) fetch_row(values, at_v, to_v, i - LOADS);
-      else if (i < 3 * LOADS) look_row(i - 2 * LOADS);
+      else if (i < 3 * LOADS) look_row(i - 2 * LOADS, ahead);
     });
     if constexpr (decltype(edge)::value) mask(t, 1);
     step(vb, 1, kn, 0, kn, 1, [](int) {});
@@ -1061,7 +1076,7 @@ __device__ void paged_attention_join(const PagedAttentionArgs& a) {
 }  // namespace aoto
 
 #define AOTO_PAGED_ATTENTION(D)                                                                                    \
-  extern "C" __global__ __launch_bounds__(256, PA_N1) void aoto_paged_attention_d##D##_n1(PagedAttentionArgs a) {      \
+  extern "C" __global__ __launch_bounds__(256, 2) void aoto_paged_attention_d##D##_n1(PagedAttentionArgs a) {      \
     aoto::paged_attention_narrow<D, 1>(a);                                                                         \
   }                                                                                                                \
   extern "C" __global__ __launch_bounds__(256, 2) void aoto_paged_attention_d##D##_n2(PagedAttentionArgs a) {      \

@@ -11,8 +11,8 @@
 // number, and the sums' noise in 32 bits (1e-7 of the total, against a typical weight of 1e-5 to 1e-6 of it) would
 // move it in a percent of the calls.
 //
-// Three launches over chunks of kVerifyChunk tokens: every row's maximum, its place and sum of weights by chunk; what
-// stands, and the weights the following token is drawn from, summed by chunk; the token. Bound by the first one's read
+// Launches over chunks of kVerifyChunk tokens: every row's maximum, its place and sum of weights by chunk; with a draft
+// model's logits, what stands and the weights the following token is drawn from, summed by chunk; the token. Bound by the first one's read
 // of the logits and, where they are sampled from, about as much by its 20 f64 operations a logit.
 #pragma once
 
@@ -29,61 +29,78 @@ struct VerifyChunk {
 };
 static_assert(sizeof(VerifyChunk) == kVerifyChunkBytes, "as the workspace is sized");
 
-// 2^x for -2048 < x <= 0 (0 from 2^-1075 on): the series of 2^f = e^(f ln 2) over |f| <= 1/2 to the 12th power, whose
-// remainder is below (ln 2 / 2)^13 / 13! = 1.7e-16, and the exponent's shift. x = d * heat is rounded to the nearest
-// whole number by a sum with 1.5 * 2^52, whose low bits are that number; f = x - n in one rounding.
-AOTO_DEVICE double exp2_of(double d, double heat) {
-  constexpr double kRound = 6755399441055744.0;
-  const double t = fma(d, heat, kRound);
-  const double f = fma(d, heat, kRound - t);
-  double s = 2.5678435993488206e-11;  // ln 2 ^ 12 / 12!, and on to the 0th
-  s = fma(s, f, 4.4455382718708116e-10);
-  s = fma(s, f, 7.054911620801123e-09);
-  s = fma(s, f, 1.01780860092397e-07);
-  s = fma(s, f, 1.321548679014431e-06);
-  s = fma(s, f, 1.5252733804059841e-05);
-  s = fma(s, f, 0.0001540353039338161);
-  s = fma(s, f, 0.0013333558146428443);
-  s = fma(s, f, 0.009618129107628477);
-  s = fma(s, f, 0.05550410866482158);
-  s = fma(s, f, 0.24022650695910072);
-  s = fma(s, f, 0.6931471805599453);
-  s = fma(s, f, 1.0);
-  return ldexp(s, __double2loint(t));
+// 2^(j / 32), in LDS: every kernel below fills it before its first weight. All 32 lie in banks of their own.
+struct VerifyTable {
+  double at[32];
+};
+AOTO_DEVICE void verify_table(VerifyTable& table) {
+  if (threadIdx.x < 32) {
+    // the series of e^y, 0 <= y < ln 2, to the 20th power (remainder 1e-23)
+    const double y = threadIdx.x * (0.6931471805599453094 / 32);
+    double s = 1.0;
+    for (int k = 20; k > 0; --k) s = fma(s, y / k, 1.0);
+    table.at[threadIdx.x] = s;
+  }
 }
 
-// The weights exp((z - top) / T) of a row's tokens: heat = log2(e) / T. A NaN or -inf weighs 0; the logits equal to an
-// infinite top weigh 1 and nothing else does.
+// 2^x, x = d * heat32 / 32, for -2048 < x <= 0 (0 from 2^-1075 on): 32 x is rounded to a whole number k by a sum with
+// 1.5 * 2^52, whose low bits are k; what is left, f = 32 x - k in one rounding, |f| <= 1/2, goes through the series of
+// e^(f ln 2 / 32) to the 5th power (remainder below (ln 2 / 64)^6 / 6! = 2.3e-15), k mod 32 through the table, the rest
+// of k to the exponent. NORMAL: x > -1000, and the exponent is moved by whole-number arithmetic.
+template <bool NORMAL = false>
+AOTO_DEVICE double exp2_of(double d, double heat32, const VerifyTable& table) {
+  constexpr double kRound = 6755399441055744.0;
+  const double t = fma(d, heat32, kRound);
+  const double f = fma(d, heat32, kRound - t);
+  const int k = __double2loint(t);
+  double s = 3.973709984549416e-11;  // (ln 2 / 32)^5 / 5!, and on to the 0th
+  s = fma(s, f, 9.172562701824643e-09);
+  s = fma(s, f, 1.693850972437182e-06);
+  s = fma(s, f, 0.0002345961982022468);
+  s = fma(s, f, 0.02166084939249829);
+  s = fma(s, f, 1.0);
+  s *= table.at[k & 31];
+  if constexpr (NORMAL) return __hiloint2double(__double2hiint(s) + ((k >> 5) << 20), __double2loint(s));
+  return ldexp(s, k >> 5);
+}
+
+// A request's temperature: 32 log2(e) / T and its inverse; heat32 < 0: greedy.
+struct VerifyHeat {
+  double heat32, cool;
+  AOTO_DEVICE bool greedy() const { return heat32 < 0.0; }
+};
+AOTO_DEVICE VerifyHeat verify_heat(const VerifyArgs& a, int r) {
+  const float t = a.temperature ? a.temperature[r] : 0.f;
+  if (!(t > 0.f)) return {-1.0, 0.0};
+  return {46.166241308446828384 / (double)t, (double)t / 46.166241308446828384};
+}
+
+// The weights exp((z - top) / T) of a row's tokens. A NaN or -inf weighs 0; the logits equal to an infinite top weigh 1
+// and nothing else does.
 struct VerifyScale {
-  double top, heat;
-  float floor;    // logits below it are taken as it, 2^-2000 of the top: 0
+  double top, heat32;
+  const VerifyTable& table;
+  float floor;    // logits below it are taken as it: at 2^-2000 of the top, 0
   bool plain;     // nothing is infinite, and the floor is where it should be after its rounding to 32 bits
-  AOTO_DEVICE VerifyScale(float t, double h) : top(t), heat(h) {
-    floor = (float)((double)t - 2000.0 / h);
-    const double reach = (top - (double)floor) * h;
-    plain = fabsf(t) < INFINITY && reach >= 1100.0 && reach <= 4000.0;
+  // `below`: the powers of two under the top that the floor lies
+  AOTO_DEVICE VerifyScale(float t, const VerifyHeat& h, const VerifyTable& tab, double below = 2000.0)
+      : top(t), heat32(h.heat32), table(tab) {
+    floor = (float)((double)t - 32.0 * below * h.cool);
+    const double reach = (top - (double)floor) * heat32;
+    plain = fabsf(t) < INFINITY && reach >= 0.95 * 32.0 * below && reach <= 1.02 * 32.0 * below;
   }
   AOTO_DEVICE double operator()(float z) const {
-    if (plain) return exp2_of((double)fmaxf(z, floor) - top, heat);  // fmaxf: a NaN gives the floor
+    if (plain) return exp2_of((double)fmaxf(z, floor) - top, heat32, table);  // fmaxf: a NaN gives the floor
     if (!(z > -INFINITY)) return 0.0;
     if ((double)z == top) return 1.0;
-    return top == INFINITY ? 0.0 : exp2_of(fmax(((double)z - top) * heat, -2000.0), 1.0);
+    return top == INFINITY ? 0.0 : exp2_of(fmax(((double)z - top) * heat32, -64000.0), 1.0, table);
   }
 };
-
-AOTO_DEVICE double verify_weight(float z, float top, double heat) { return VerifyScale(top, heat)(z); }
 
 template <bool F32>
 AOTO_DEVICE float verify_logit(const void* row, int v) {
   const float z = F32 ? static_cast<const float*>(row)[v] : bf16_to_f32(static_cast<const uint16_t*>(row)[v]);
   return z != z ? -INFINITY : z;
-}
-
-// log2(e) / T, or kVerifyGreedy.
-constexpr double kVerifyGreedy = -1.0;
-AOTO_DEVICE double verify_heat(const VerifyArgs& a, int r) {
-  const float t = a.temperature ? a.temperature[r] : 0.f;
-  return t > 0.f ? 1.4426950408889634074 / (double)t : kVerifyGreedy;
 }
 
 // Rows of request r: its first, and how many drafts of it there are.
@@ -93,11 +110,30 @@ AOTO_DEVICE void verify_rows(const VerifyArgs& a, int r, int& first, int& count)
   count = min(end - first - 1, a.drafts);  // -1: the request has no row
 }
 
-AOTO_DEVICE double wave_sum_f64(double v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+// A double moved across lanes as its two halves (0 where the move has no source or the row is left out).
+template <int CTRL, int ROWS>
+AOTO_DEVICE double dpp_f64(double v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xF, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xF, true);
+  return __hiloint2double(hi, lo);
+}
+// Running sums over a wave: within rows of 16 by shifts of 1, 2, 4 and 8, then the rows' last lanes on to the rows
+// behind them.
+AOTO_DEVICE double wave_scan_f64(double v) {
+  v += dpp_f64<0x111, 0xF>(v);
+  v += dpp_f64<0x112, 0xF>(v);
+  v += dpp_f64<0x114, 0xF>(v);
+  v += dpp_f64<0x118, 0xF>(v);
+  v += dpp_f64<0x142, 0xA>(v);
+  v += dpp_f64<0x143, 0xC>(v);
   return v;
 }
+AOTO_DEVICE double wave_last_f64(double v) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 63),
+                          __builtin_amdgcn_readlane(__double2loint(v), 63));
+}
+// The wave's total, in every lane.
+AOTO_DEVICE double wave_sum_f64(double v) { return wave_last_f64(wave_scan_f64(v)); }
 
 template <bool F32>
 AOTO_DEVICE const void* verify_row(const void* base, long long at) {
@@ -127,40 +163,82 @@ AOTO_DEVICE void verify_load(const void* row, int v, int end, float (&z)[8]) {
   }
 }
 
-// Block (chunk, r * (2 drafts + 1) + i): target row i of request r (i <= drafts), or its draft row i - drafts - 1.
-// A thread has 32 logits in registers and weighs them against its own maximum; the threads' sums are then brought to
-// the block's. A greedy row's places are kept instead of weights.
+// The logits of a chunk that a lane of one wave holds: 16 bytes at a time, 1 KB a wave and load.
+template <bool F32>
+struct VerifyHeld {
+  static constexpr int EACH = F32 ? 4 : 8, LOADS = kVerifyChunk / 64 / EACH;
+  uint4 raw[LOADS];
+  AOTO_DEVICE static int at(int load) { return (64 * load + (int)(threadIdx.x & 63)) * EACH; }
+  AOTO_DEVICE void get(int load, float (&z)[EACH]) const {
+    const uint32_t w[4] = {raw[load].x, raw[load].y, raw[load].z, raw[load].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (F32) z[i] = __uint_as_float(w[i]);
+      else z[2 * i] = bf16_lo(w[i]), z[2 * i + 1] = bf16_hi(w[i]);
+    }
+  }
+};
+
+// Wave (chunk, r * judged + i): target row i of request r (i <= drafts), or its draft row i - drafts - 1. All of the
+// chunk's loads go out at once and stay in registers: a lane's maximum, then its weights against that, then the lanes'
+// sums brought to the wave's maximum. Nothing is shared between waves, so none waits for another. A greedy row's first
+// place is kept instead of weights.
 template <bool F32>
 __device__ void verify_stats(const VerifyArgs& a) {
-  constexpr int GROUPS = kVerifyChunk / 2048;
-  __shared__ float s_top[4];
-  __shared__ int s_place[4];
-  __shared__ double s_sum[4];
-  const int per = 2 * a.drafts + 1;
-  const int r = blockIdx.y / per, i = blockIdx.y % per;
+  using Held = VerifyHeld<F32>;
+  __shared__ VerifyTable table;
+  const int r = blockIdx.y / a.judged, i = blockIdx.y % a.judged;
+  const int chunk = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   int first, count;
   verify_rows(a, r, first, count);
   const bool draft = i > a.drafts;
-  const double heat = verify_heat(a, r);
-  if (draft ? (a.draft_logits == nullptr || i - a.drafts - 1 >= count || heat == kVerifyGreedy) : i > count) return;
+  const VerifyHeat heat = verify_heat(a, r);
+  if (draft ? (a.draft_logits == nullptr || i - a.drafts - 1 >= count || heat.greedy()) : i > count) return;
+  verify_table(table);
+  __syncthreads();
+  if (chunk >= a.chunks) return;
   const void* row = draft ? verify_row<F32>(a.draft_logits, r * a.draft_request_stride +
                                                                 (i - a.drafts - 1) * a.draft_row_stride)
                           : verify_row<F32>(a.logits, (first + i) * a.row_stride);
-  const int begin = blockIdx.x * kVerifyChunk, end = min(a.vocab, begin + kVerifyChunk);
-  const int mine = begin + 8 * threadIdx.x;
-  float z[GROUPS][8];
+  const int begin = chunk * kVerifyChunk, end = min(a.vocab, begin + kVerifyChunk);
+  // loads past the row's end, and those of a row that is not 16-byte aligned, are put together from single logits
+  const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+  const uint4* from = reinterpret_cast<const uint4*>(verify_row<F32>(row, begin));
+  Held held;
 #pragma unroll
-  for (int g = 0; g < GROUPS; ++g) verify_load<F32>(row, mine + 2048 * g, end, z[g]);
+  for (int l = 0; l < Held::LOADS; ++l) held.raw[l] = make_uint4(0, 0, 0, 0);
+  if (aligned) {
+#pragma unroll
+    for (int l = 0; l < Held::LOADS; ++l)
+      if (begin + Held::at(l) + Held::EACH <= end) held.raw[l] = from[Held::at(l) / Held::EACH];
+  }
+  if (!aligned || begin + kVerifyChunk > end) {
+#pragma unroll
+    for (int l = 0; l < Held::LOADS; ++l)
+      if (!aligned || begin + Held::at(l) + Held::EACH > end) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int v = begin + Held::at(l) + (F32 ? k : 2 * k);
+          const float lo = v < end ? verify_logit<F32>(row, v) : -INFINITY;
+          const float hi = !F32 && v + 1 < end ? verify_logit<F32>(row, v + 1) : -INFINITY;
+          w[k] = F32 ? __float_as_uint(lo) : __float_as_uint(lo) >> 16 | (__float_as_uint(hi) & 0xFFFF0000u);
+        }
+        held.raw[l] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+  }
   float top = -INFINITY;
   int place = begin;
   double sum = 0.0;
-  const int wave = threadIdx.x >> 6;
-  if (heat == kVerifyGreedy) {
+  float z[Held::EACH];
+  if (heat.greedy()) {
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g)
+    for (int l = 0; l < Held::LOADS; ++l) {
+      held.get(l, z);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (z[g][e] > top) top = z[g][e], place = mine + 2048 * g + e;
+      for (int e = 0; e < Held::EACH; ++e)
+        if (z[e] > top) top = z[e], place = begin + Held::at(l) + e;  // a NaN is above nothing
+    }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const float t = __shfl_xor(top, d);
@@ -169,40 +247,40 @@ __device__ void verify_stats(const VerifyArgs& a) {
     }
   } else {
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g)
+    for (int l = 0; l < Held::LOADS; ++l) {
+      held.get(l, z);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, z[g][e]);
-    const VerifyScale weight(top, heat);
+      for (int e = 0; e < Held::EACH; ++e) top = fmaxf(top, z[e]);  // past a NaN
+    }
+    const VerifyScale weight(top, heat, table, 980.0);  // what lies lower adds 2^-980 instead of less
     if (weight.plain) {
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g)
+      for (int l = 0; l < Held::LOADS; ++l) {
+        held.get(l, z);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += exp2_of((double)fmaxf(z[g][e], weight.floor) - weight.top, heat);
-    } else {
+        for (int e = 0; e < Held::EACH; ++e)
+          sum += exp2_of<true>((double)fmaxf(z[e], weight.floor) - weight.top, heat.heat32, table);
+      }
+    } else if (top > -INFINITY) {
+#pragma unroll
+      for (int l = 0; l < Held::LOADS; ++l) {
+        held.get(l, z);
 #pragma unroll 1
-      for (int k = 0; k < 8 * GROUPS; ++k) {
-        float x = -INFINITY;
+        for (int e = 0; e < Held::EACH; ++e) {
+          float x = z[0];
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x = k == 8 * g + e ? z[g][e] : x;
-        sum += weight(x);
+          for (int k = 1; k < Held::EACH; ++k) x = e == k ? z[k] : x;
+          sum += weight(x);
+        }
       }
     }
     const float all = wave_max(top);
-    sum = wave_sum_f64(sum == 0.0 ? 0.0 : sum * verify_weight(top, all, heat));
+    sum = wave_sum_f64(sum == 0.0 ? 0.0 : sum * VerifyScale(all, heat, table)(top));
     top = all;
   }
-  if ((threadIdx.x & 63) == 0) s_top[wave] = top, s_place[wave] = place, s_sum[wave] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 4; ++w)
-      if (s_top[w] > top || (s_top[w] == top && s_place[w] < place)) top = s_top[w], place = s_place[w];
-    sum = 0.0;
-    if (heat != kVerifyGreedy)
-      for (int w = 0; w < 4; ++w)
-        if (s_sum[w] != 0.0) sum += s_sum[w] * verify_weight(s_top[w], top, heat);
-    VerifyChunk* out = static_cast<VerifyChunk*>(a.workspace) + (size_t)blockIdx.y * a.chunks + blockIdx.x;
+  if (lane == 0) {
+    VerifyChunk* out = static_cast<VerifyChunk*>(a.workspace) +
+                       ((size_t)r * (2 * a.drafts + 1) + i) * a.chunks + chunk;
     *out = VerifyChunk{sum, top, place};
   }
 }
@@ -215,33 +293,63 @@ struct VerifyLaw {
   const void* row;
   const void* draft_row;   // null: nothing is subtracted
   float top, draft_top;
-  double sum, draft_sum, heat;
+  double sum, draft_sum;
+  double fell;             // the removed token's weight
+  VerifyHeat heat;
 };
 static_assert(sizeof(VerifyLaw) <= kVerifyLawBytes, "as the workspace is sized");
 
 // By the whole block: 16 lanes join the chunks of a row, then lane i of the first wave judges draft i and the ballot
-// finds the first that falls.
+// finds the first that falls. Two round trips to memory: what is known of the request, then the chunks' statistics
+// beside the drafted tokens' logits.
 template <bool F32, int THREADS>
-AOTO_DEVICE VerifyLaw verify_law(const VerifyArgs& a, int r) {
+AOTO_DEVICE VerifyLaw verify_law(const VerifyArgs& a, int r, VerifyTable& table) {
   __shared__ float s_top[126];
   __shared__ double s_sum[126];
   __shared__ int s_place[126];
   __shared__ VerifyLaw s_law;
+  const int lane = threadIdx.x & 63, part = threadIdx.x & 15;
+  long long x = -1;
+  float u = 0.f;
+  if (threadIdx.x < a.drafts) {
+    x = a.draft_tokens[(size_t)r * a.drafts + threadIdx.x];
+    if (a.uniforms) u = a.uniforms[(size_t)r * (a.drafts + 1) + threadIdx.x];
+  }
   int first, count;
   verify_rows(a, r, first, count);
-  const int lane = threadIdx.x & 63, part = threadIdx.x & 15;
-  const double heat = verify_heat(a, r);
-  const bool sampled = heat != kVerifyGreedy, laws = a.draft_logits && sampled;
+  const VerifyHeat heat = verify_heat(a, r);
+  const bool sampled = !heat.greedy(), laws = a.draft_logits && sampled;
+  const bool known = (int)threadIdx.x < count && x >= 0 && x < a.vocab;
+  float zx = -INFINITY, yx = -INFINITY;
+  if (known && sampled) {
+    zx = verify_logit<F32>(verify_row<F32>(a.logits, (first + lane) * a.row_stride), (int)x);
+    if (laws)
+      yx = verify_logit<F32>(
+          verify_row<F32>(a.draft_logits, r * a.draft_request_stride + lane * a.draft_row_stride), (int)x);
+  }
   const VerifyChunk* chunks = static_cast<const VerifyChunk*>(a.workspace) + (size_t)r * (2 * a.drafts + 1) * a.chunks;
   const int rows = count + 1 + (laws && count > 0 ? count : 0);
+  verify_table(table);
+  __syncthreads();
   for (int j0 = 0; j0 < rows; j0 += THREADS / 16) {
     const int j = j0 + (threadIdx.x >> 4);
     const bool live = j < rows;
     const VerifyChunk* from = chunks + (size_t)(j <= count ? j : a.drafts + j - count) * a.chunks;
+    constexpr int SOME = 3;  // a lane's chunks that are loaded at once: 196608 tokens
+    VerifyChunk mine[SOME];
+#pragma unroll
+    for (int k = 0; k < SOME; ++k) {
+      mine[k] = VerifyChunk{0.0, -INFINITY, 0};
+      if (live && part + 16 * k < a.chunks) mine[k] = from[part + 16 * k];
+    }
     float top = -INFINITY;
     int place = 0;
-    for (int c = part; live && c < a.chunks; c += 16)
-      if (from[c].top > top) top = from[c].top, place = from[c].place;
+    auto better = [&](const VerifyChunk& one) {
+      if (one.top > top) top = one.top, place = one.place;
+    };
+#pragma unroll
+    for (int k = 0; k < SOME; ++k) better(mine[k]);
+    for (int c = part + 16 * SOME; live && c < a.chunks; c += 16) better(from[c]);
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) {
       const float t = __shfl_xor(top, d);
@@ -250,8 +358,13 @@ AOTO_DEVICE VerifyLaw verify_law(const VerifyArgs& a, int r) {
     }
     double sum = 0.0;
     if (sampled) {
-      for (int c = part; live && c < a.chunks; c += 16)
-        if (from[c].sum != 0.0) sum += from[c].sum * verify_weight(from[c].top, top, heat);
+      const VerifyScale weight(top, heat, table);
+      auto add = [&](const VerifyChunk& one) {
+        if (one.sum != 0.0) sum += one.sum * weight(one.top);
+      };
+#pragma unroll
+      for (int k = 0; k < SOME; ++k) add(mine[k]);
+      for (int c = part + 16 * SOME; live && c < a.chunks; c += 16) add(from[c]);
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor(sum, d);
     }
@@ -260,26 +373,21 @@ AOTO_DEVICE VerifyLaw verify_law(const VerifyArgs& a, int r) {
   __syncthreads();
   if (threadIdx.x < 64) {
     bool stands = false;
-    if (lane < count) {
-      const long long x = a.draft_tokens[(size_t)r * a.drafts + lane];
-      if (x >= 0 && x < a.vocab) {
-        if (sampled) {
-          const float z = verify_logit<F32>(verify_row<F32>(a.logits, (first + lane) * a.row_stride), (int)x);
-          const double px = s_sum[lane] > 0.0 ? verify_weight(z, s_top[lane], heat) / s_sum[lane] : 0.0;
-          double qx = 1.0;
-          if (laws) {
-            const float y = verify_logit<F32>(
-                verify_row<F32>(a.draft_logits, r * a.draft_request_stride + lane * a.draft_row_stride), (int)x);
-            const int j = count + 1 + lane;
-            qx = s_sum[j] > 0.0 ? verify_weight(y, s_top[j], heat) / s_sum[j] : 0.0;
-          }
-          stands = (double)a.uniforms[(size_t)r * (a.drafts + 1) + lane] * qx < px;
-        } else {
-          stands = s_top[lane] > -INFINITY && s_place[lane] == (int)x;
-        }
+    double wx = 0.0;
+    if (known) {
+      if (sampled) {
+        if (s_sum[lane] > 0.0) wx = VerifyScale(s_top[lane], heat, table)(zx);
+        const double px = s_sum[lane] > 0.0 ? wx / s_sum[lane] : 0.0;
+        const int j = count + 1 + lane;
+        const double qx = !laws ? 1.0 : s_sum[j] > 0.0 ? VerifyScale(s_top[j], heat, table)(yx) / s_sum[j] : 0.0;
+        stands = (double)u * qx < px;
+      } else {
+        stands = s_top[lane] > -INFINITY && s_place[lane] == (int)x;
       }
     }
     const int k = min(max(count, 0), __ffsll(~__ballot(stands)) - 1);
+    const long long fell = __shfl(x, k);
+    const double weighed = __shfl(wx, k);
     if (lane == 0) {
       VerifyLaw law{};
       law.count = count, law.accepted = k, law.heat = heat, law.removed = -1;
@@ -290,8 +398,8 @@ AOTO_DEVICE VerifyLaw verify_law(const VerifyArgs& a, int r) {
           law.draft_row = verify_row<F32>(a.draft_logits, r * a.draft_request_stride + k * a.draft_row_stride);
           law.draft_top = s_top[count + 1 + k], law.draft_sum = s_sum[count + 1 + k];
         } else {
-          const long long x = a.draft_tokens[(size_t)r * a.drafts + k];
-          law.removed = x >= 0 && x < a.vocab ? (int)x : -1;
+          law.removed = fell >= 0 && fell < a.vocab ? (int)fell : -1;
+          law.fell = weighed;
         }
       }
       s_law = law;
@@ -303,119 +411,141 @@ AOTO_DEVICE VerifyLaw verify_law(const VerifyArgs& a, int r) {
 
 // The weights of tokens v .. v + 7 under the target's law and what is left of them.
 template <bool F32>
-AOTO_DEVICE void verify_left(const VerifyLaw& law, int v, int end, double (&whole)[8], double (&left)[8]) {
-  float z[8];
+AOTO_DEVICE void verify_left(const VerifyLaw& law, const VerifyTable& table, int v, int end, double (&whole)[8],
+                             double (&left)[8]) {
+  const bool minus = law.draft_row && law.draft_sum > 0.0;
+  float z[8], y[8];
   verify_load<F32>(law.row, v, end, z);
-  const VerifyScale weight(law.top, law.heat);
+  if (minus) verify_load<F32>(law.draft_row, v, end, y);
+  const VerifyScale weight(law.top, law.heat, table);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     whole[i] = law.sum > 0.0 && v + i < end ? weight(z[i]) : 0.0;
     left[i] = v + i == law.removed ? 0.0 : whole[i];
   }
-  if (law.draft_row && law.draft_sum > 0.0) {
+  if (minus) {
     // p - q, times the target's sum
     const double ratio = law.sum / law.draft_sum;
-    const VerifyScale other(law.draft_top, law.heat);
-    verify_load<F32>(law.draft_row, v, end, z);
+    const VerifyScale other(law.draft_top, law.heat, table);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) left[i] = v + i < end ? fmax(whole[i] - ratio * other(z[i]), 0.0) : 0.0;
+    for (int i = 0; i < 8; ++i) left[i] = v + i < end ? fmax(whole[i] - ratio * other(y[i]), 0.0) : 0.0;
   }
 }
 
 AOTO_DEVICE double* verify_masses(const VerifyArgs& a, int r) {
   const size_t chunks = (size_t)a.requests * (2 * a.drafts + 1) * a.chunks;
-  return reinterpret_cast<double*>(static_cast<VerifyChunk*>(a.workspace) + chunks) + (size_t)r * 2 * a.chunks;
+  return reinterpret_cast<double*>(static_cast<VerifyChunk*>(a.workspace) + chunks) + (size_t)r * a.chunks;
 }
 AOTO_DEVICE VerifyLaw* verify_laws(const VerifyArgs& a) {
   return reinterpret_cast<VerifyLaw*>(verify_masses(a, a.requests));
 }
 
-// Block (chunk, r): the chunk's sums of what is left and of the whole; the first one's law is kept.
+// Block r: the request's law, for the two launches behind it (every chunk's block finding it anew cost more: 64
+// requests' sums 21 us, against 5 and 10).
+template <bool F32>
+__device__ void verify_keep(const VerifyArgs& a) {
+  __shared__ VerifyTable table;
+  const VerifyLaw law = verify_law<F32, 256>(a, blockIdx.x, table);
+  if (threadIdx.x == 0) verify_laws(a)[blockIdx.x] = law;
+}
+
+// Block (chunk, r): the chunk's sum of what a draft model's law leaves of the target's, where a draft fell. (Other
+// requests' chunk sums are those of the statistics, less a removed token's weight.)
 template <bool F32>
 __device__ void verify_mass(const VerifyArgs& a) {
-  __shared__ double s_sum[4][2];
+  __shared__ VerifyTable table;
+  __shared__ double s_sum[4];
   const int r = blockIdx.y;
-  const VerifyLaw law = verify_law<F32, 256>(a, r);
-  if (blockIdx.x == 0 && threadIdx.x == 0) verify_laws(a)[r] = law;
-  if (law.heat == kVerifyGreedy) return;
+  const VerifyLaw law = verify_laws(a)[r];
+  if (law.draft_row == nullptr) return;
+  verify_table(table);
+  __syncthreads();
   const int begin = blockIdx.x * kVerifyChunk, end = min(a.vocab, begin + kVerifyChunk);
-  double sums[2] = {0.0, 0.0};
+  double sum = 0.0;
 #pragma unroll 1
   for (int v = begin + 8 * threadIdx.x; v < end; v += 2048) {
     double whole[8], left[8];
-    verify_left<F32>(law, v, end, whole, left);
+    verify_left<F32>(law, table, v, end, whole, left);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sums[0] += left[i], sums[1] += whole[i];
+    for (int i = 0; i < 8; ++i) sum += left[i];
   }
-  for (int i = 0; i < 2; ++i) {
-    sums[i] = wave_sum_f64(sums[i]);
-    if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6][i] = sums[i];
-  }
+  sum = wave_sum_f64(sum);
+  if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum;
   __syncthreads();
-  if (threadIdx.x < 2)
-    verify_masses(a, r)[threadIdx.x * a.chunks + blockIdx.x] =
-        s_sum[0][threadIdx.x] + s_sum[1][threadIdx.x] + s_sum[2][threadIdx.x] + s_sum[3][threadIdx.x];
+  if (threadIdx.x == 0) verify_masses(a, r)[blockIdx.x] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
 }
 
-// Running sums over a wave.
-AOTO_DEVICE double wave_scan_f64(double v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double up = __shfl_up(v, d);
-    if ((int)(threadIdx.x & 63) >= d) v += up;
-  }
-  return v;
-}
-
-// Block r, 1024 threads: the chunk in which the running sum passes, then the token in it, eight a thread.
+// Block r, 512 threads: the chunk in which the running sum passes, then the token in it, eight a thread. KEPT: the law
+// and the sums of subtracted laws are there already.
 template <bool F32, bool KEPT>
 __device__ void verify_pick(const VerifyArgs& a) {
-  static_assert(kVerifyChunk == 8 * 1024, "a chunk is eight tokens a thread");
-  __shared__ double s_sum[16], s_before;
-  __shared__ int s_chunk, s_token, s_last;
+  static_assert(kVerifyChunk == 8 * 512, "a chunk is eight tokens a thread");
+  __shared__ double s_sum[8], s_before, s_target;
+  __shared__ int s_chunk, s_whole, s_token, s_last;
   const int r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ VerifyTable table;
+  const float u = a.uniforms ? a.uniforms[(size_t)r * (a.drafts + 1) + a.drafts] : 0.f;
   VerifyLaw law;
-  if constexpr (KEPT) law = verify_laws(a)[r];
-  else law = verify_law<F32, 1024>(a, r);
+  if constexpr (KEPT) {
+    law = verify_laws(a)[r];
+    verify_table(table);
+    __syncthreads();
+  } else {
+    law = verify_law<F32, 512>(a, r, table);
+  }
   long long token = law.place;
-  if (KEPT && law.count >= 0 && law.heat != kVerifyGreedy) {
-    const float u = a.uniforms[(size_t)r * (a.drafts + 1) + a.drafts];
-    const double* masses = verify_masses(a, r);
-    double total = 0.0;
-    for (int c = 0; c < a.chunks; c += 64) total += wave_sum_f64(c + lane < a.chunks ? masses[c + lane] : 0.0);
-    const bool whole = !(total > 0.0);
-    if (whole) {
-      masses += a.chunks;
-      total = 0.0;
-      for (int c = 0; c < a.chunks; c += 64) total += wave_sum_f64(c + lane < a.chunks ? masses[c + lane] : 0.0);
-    }
-    const double target = (double)u * total;
+  if (law.count >= 0 && !law.heat.greedy()) {
     if (wave == 0) {
+      const VerifyChunk* chunks = static_cast<const VerifyChunk*>(a.workspace) +
+                                  ((size_t)r * (2 * a.drafts + 1) + law.accepted) * a.chunks;
+      const VerifyScale weight(law.top, law.heat, table);
+      auto mass = [&](int c, bool whole) {
+        if (c >= a.chunks) return 0.0;
+        if (!whole && law.draft_row) return verify_masses(a, r)[c];
+        const VerifyChunk one = chunks[c];
+        double sum = one.sum != 0.0 ? one.sum * weight(one.top) : 0.0;
+        if (!whole && law.removed >= 0 && law.removed / kVerifyChunk == c) {
+          // what a removed token leaves of its chunk; of the difference's rounding nothing
+          const double left = sum - law.fell;
+          sum = left > 0x1p-50 * sum ? left : 0.0;
+        }
+        return sum;
+      };
+      bool whole = false;
+      double near = mass(lane, false), total = wave_sum_f64(near);  // the first 64 chunks stay in a register
+      for (int c = 64; c < a.chunks; c += 64) total += wave_sum_f64(mass(c + lane, false));
+      if (!(total > 0.0)) {
+        whole = true;
+        near = mass(lane, true), total = wave_sum_f64(near);
+        for (int c = 64; c < a.chunks; c += 64) total += wave_sum_f64(mass(c + lane, true));
+      }
+      const double target = (double)u * total;
       // the chunk; past the total (a random number of 1, or the sums' last bits) the last one that has weight
       double run = 0.0, before = 0.0;
       int chunk = 0;
       for (int c = 0; c < a.chunks; c += 64) {
-        const double mass = c + lane < a.chunks ? masses[c + lane] : 0.0;
-        const double upto = run + wave_scan_f64(mass);
-        const unsigned long long some = __ballot(mass > 0.0), past = __ballot(mass > 0.0 && upto > target);
+        const double m = c == 0 ? near : mass(c + lane, whole);
+        const double upto = run + wave_scan_f64(m);
+        const unsigned long long some = __ballot(m > 0.0), past = __ballot(m > 0.0 && upto > target);
         const int at = past ? __ffsll(past) - 1 : some ? 63 - __clzll((long long)some) : -1;
-        if (at >= 0) chunk = c + at, before = __shfl(upto - mass, at);
+        if (at >= 0) chunk = c + at, before = __shfl(upto - m, at);
         if (past) break;
-        run = __shfl(upto, 63);
+        run = wave_last_f64(upto);
       }
-      if (lane == 0) s_chunk = chunk, s_before = before;
+      if (lane == 0) s_chunk = chunk, s_before = before, s_whole = whole, s_target = target;
     }
     if (threadIdx.x == 0) s_token = 0x7FFFFFFF, s_last = -1;
     __syncthreads();
+    const double target = s_target;
     const int begin = s_chunk * kVerifyChunk, end = min(a.vocab, begin + kVerifyChunk);
     const int v = begin + 8 * threadIdx.x;
     double all[8], left[8];
-    verify_left<F32>(law, v, end, all, left);
+    verify_left<F32>(law, table, v, end, all, left);
     double sum = 0.0;
     int last = -1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (whole) left[i] = all[i];
+      if (s_whole) left[i] = all[i];
       sum += left[i];
       if (left[i] > 0.0) last = v + i;
     }
@@ -437,7 +567,7 @@ __device__ void verify_pick(const VerifyArgs& a) {
     if (s_token != 0x7FFFFFFF) token = s_token;
     else if (s_last >= 0) token = s_last;
   }
-  for (int i = threadIdx.x; i <= a.drafts; i += 1024) {
+  for (int i = threadIdx.x; i <= a.drafts; i += 512) {
     long long out = -1;
     if (law.count >= 0 && i < law.accepted) out = a.draft_tokens[(size_t)r * a.drafts + i];
     if (law.count >= 0 && i == law.accepted) out = token;
@@ -452,12 +582,15 @@ __device__ void verify_pick(const VerifyArgs& a) {
   extern "C" __global__ __launch_bounds__(256) void aoto_verify_stats_##NAME(VerifyArgs a) {             \
     aoto::verify_stats<F32>(a);                                                                          \
   }                                                                                                      \
+  extern "C" __global__ __launch_bounds__(256) void aoto_verify_law_##NAME(VerifyArgs a) {               \
+    aoto::verify_keep<F32>(a);                                                                           \
+  }                                                                                                      \
   extern "C" __global__ __launch_bounds__(256) void aoto_verify_mass_##NAME(VerifyArgs a) {              \
     aoto::verify_mass<F32>(a);                                                                           \
   }                                                                                                      \
-  extern "C" __global__ __launch_bounds__(1024) void aoto_verify_pick_##NAME(VerifyArgs a) {             \
+  extern "C" __global__ __launch_bounds__(512) void aoto_verify_pick_##NAME(VerifyArgs a) {             \
     aoto::verify_pick<F32, true>(a);                                                                     \
   }                                                                                                      \
-  extern "C" __global__ __launch_bounds__(1024) void aoto_verify_greedy_##NAME(VerifyArgs a) {           \
+  extern "C" __global__ __launch_bounds__(512) void aoto_verify_follow_##NAME(VerifyArgs a) {           \
     aoto::verify_pick<F32, false>(a);                                                                    \
   }

@@ -246,12 +246,18 @@ def _attend(s, *, q=None, **kwargs):
     return out
 
 
+def attention_bound(want, size):
+    return HALF * (1 + 2 * HALF) * (2 * np.abs(want) + size) + 4e-5 * size
+
+
 def _check_attention(s, got, **kwargs):
     want, size, written = oracle.attention(s["q"], s["keys"], s["values"], s["tables"], s["start"], s["kv"], **kwargs)
     got = from_gpu_bf16(got).astype(np.float64)
-    # out = sum p v / sum p: p is rounded to bf16 for the product (HALF of sum p |v|), the result once more (HALF of
-    # itself); scores of |s| < 100 in f32 add 100 * 2^-23 to log p, exponentials and sums less: 2e-5 of sum p |v|
-    bound = HALF * (np.abs(want) + (1 + HALF) * size) + 4e-5 * size
+    # out = sum p' v / sum p' with p' = p (1 + d), |d| <= HALF, the weights rounded to bf16 for the product (and, in wide
+    # tiles, for the sum): off by sum p d (v - want) / sum p' <= HALF (size + |want|) / (1 - HALF); the result is rounded
+    # once more, HALF of itself. Scores of |s| < 100 in f32 add 100 * 2^-23 to log p, exponentials and sums less: 2e-5
+    # of sum p |v| and of |want|, which is no larger
+    bound = attention_bound(want, size)
     bad = ~(np.abs(got - want) <= bound)
     assert not bad[written].any(), (np.argwhere(bad & written[:, None])[:5], np.abs(got - want)[bad & written[:, None]][:5])
     assert (got[~written] == 5.0).all()
@@ -639,7 +645,7 @@ def test_serving_steps_over_one_cache():
             want, size, _ = oracle.attention(rows[first: first + n, :hq], k, v, np.zeros((1, 1), int), [0, n],
                                              [context[r] + n])
             got = from_gpu_bf16(mixed)[first: first + n].astype(np.float64)
-            assert (np.abs(got - want) <= HALF * (np.abs(want) + (1 + HALF) * size) + 4e-5 * size).all()
+            assert (np.abs(got - want) <= attention_bound(want, size)).all()
             first += n
         assert not bool(mixed[total:].any())
         x = ops.w4_matmul(mixed, *weights["out"], 64, residual=x)
