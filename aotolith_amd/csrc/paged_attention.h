@@ -4,9 +4,9 @@
 // over the keys j of token t's request r that it may see: with n_r = query_start[r + 1] - query_start[r] rows and
 // kv_r keys, row i sees j < kv_r - n_r + i + 1 (causal) or j < kv_r, as far as the block table row goes and where its
 // entry names a page of the cache; a row that sees none gives 0. Key j of head h / (Hq / Hkv) is row j % page of page
-// block_tables[r][j / page]. Scores, maxima and sums in f32, one pass over the keys with a running maximum; P is
-// rounded to bf16 for its product (as the prefill attention does: the matrix instructions take two operands of one
-// type), its sum is not.
+// block_tables[r][j / page]. Scores, maxima and sums in f32, one pass over the keys with a running maximum. P goes
+// into its product with V as bf16, the matrix instructions' operands being of one type: as two of them in 16-row tiles,
+// rounded to one otherwise (as the prefill attention does), which is off by as much as the result's own rounding.
 //
 // Work is cut on the GPU, from the lengths as they are there. An item is one tile of a request's rows (all query heads of
 // a kv head that share its keys, token after token) against all the keys they see, counted in blocks of 128 keys. With
@@ -266,7 +266,10 @@ struct PagedNarrowShared {
 // slot 8 q + j is key 4 q + j of the first 16 (j < 4), 4 q + j - 4 of the second.
 template <int D, int NT>
 AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit, int kvh, PagedNarrowShared<D, NT>& s) {
-  constexpr int DC = D / 32, DT = D / 16, STR = PagedNarrowShared<D, NT>::STR, ROWS = 16 * NT;
+  constexpr int DC = D / 32, DT = D / 16, STR = PagedNarrowShared<D, NT>::STR;
+  // P keeps 16 bits, as its upper half cut off and the rest rounded: two products, which cost nothing here (16 rows:
+  // 78.7 us with and without for 32 requests' 88000 keys). With 32 rows they cost 7%, and P is rounded to bf16.
+  constexpr bool TWO = NT == 1;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
   const int group = a.query_heads / a.kv_heads;
@@ -401,7 +404,7 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
 #pragma unroll
         for (int c = 0; c < DC; ++c) vq[g][c] = *reinterpret_cast<const uint4*>(values + max(at[g], 0LL) + 32 * c);
     }
-    fa_bf16x8 pb[NT];
+    fa_bf16x8 pb[NT], pr[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if (!whole) {
@@ -432,12 +435,25 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
       float p[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j >> 2][j & 3], c2, -ref));
+        // not below the smallest normal number, which beside the row's weights is nothing, so that an infinite value
+        // stays one (0 * inf); the values of keys that are not there, or hidden from a row, are finite
+        p[j] = fmaxf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j >> 2][j & 3], c2, -ref)), 0x1p-126f);
         run_sum[t] += p[j];
       }
-      const uint32_t packed[4] = {cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
-                                  cvt_pk_bf16(p[6], p[7])};
-      pb[t] = __builtin_bit_cast(fa_bf16x8, packed);
+      uint32_t high[4], low[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (TWO) {
+          high[j] = __builtin_amdgcn_perm(__float_as_uint(p[2 * j + 1]), __float_as_uint(p[2 * j]), 0x07060302u);
+          low[j] = cvt_pk_bf16(fmaxf(p[2 * j] - bf16_lo(high[j]), 0x1p-126f),
+                               fmaxf(p[2 * j + 1] - bf16_hi(high[j]), 0x1p-126f));
+        } else {
+          high[j] = cvt_pk_bf16(p[2 * j], p[2 * j + 1]);
+          low[j] = 0;
+        }
+      }
+      pb[t] = __builtin_bit_cast(fa_bf16x8, high);
+      pr[t] = __builtin_bit_cast(fa_bf16x8, low);
     }
     const uint16_t* vp = vs + (4 * quad + (col >> 2)) * STR + 4 * (col & 3);
 #pragma unroll
@@ -446,8 +462,11 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
       const pa_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4*)(vp + 16 * STR + 16 * d));
       const pa_s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t) {
         o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(fa_bf16x8, both), pb[t], o[t][d], 0, 0, 0);
+        if constexpr (TWO)
+          o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(fa_bf16x8, both), pr[t], o[t][d], 0, 0, 0);
+      }
     }
     while (special) {
       const int k = __ffs(special) - 1;

@@ -357,6 +357,28 @@ def test_attention_keeps_what_it_may_not_see_out(rows):
     _check_attention(s, _attend(s))
 
 
+@pytest.mark.parametrize("rows", [1, 5, 40])
+def test_attention_of_infinite_values(rows):
+    # an infinite value reaches the rows that see its key, in its own dims, and no others
+    rng = np.random.default_rng(16)
+    s = _requests(rng, [(rows, 333), (rows, rows), (rows, 64)], 8, 2, 64, 16)
+    last = s["kv"] - 1
+    for r, (j, value) in enumerate([(200, np.inf), (last[1], -np.inf), (last[2] - rows // 2, np.nan)]):
+        s["values"][s["tables"][r, j // 16], :, j % 16, 3 * r: 3 * r + 2] = value
+    s["device"][1].copy_(to_gpu_bf16(s["values"]))
+    got = from_gpu_bf16(_attend(s)).astype(np.float64)
+    plain = {**s, "values": np.where(np.isfinite(s["values"]), s["values"], 0.0)}
+    want, size, _ = oracle.attention(plain["q"], plain["keys"], plain["values"], s["tables"], s["start"], s["kv"])
+    special = np.zeros(want.shape)
+    for r, (j, value) in enumerate([(200, np.inf), (last[1], -np.inf), (last[2] - rows // 2, np.nan)]):
+        seen = s["start"][r] + np.arange(rows)[s["kv"][r] - rows + np.arange(rows) >= j]
+        for h in range(8):
+            special[seen[:, None], 64 * h + 3 * r + np.arange(2)] = value
+    odd = special != 0
+    np.testing.assert_array_equal(got[odd], special[odd])
+    assert (np.abs(got - want) <= attention_bound(want, size))[~odd].all()
+
+
 @pytest.mark.parametrize("rows", [1, 20])
 def test_attention_of_large_scores(rows):
     # one key far above the others, scores to +-90: the running maximum moves, nothing overflows
