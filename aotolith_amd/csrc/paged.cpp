@@ -32,13 +32,12 @@ int check_pages(const char* what, const void* keys, const void* values, int64_t 
   return AOTO_OK;
 }
 
-// Rows of a wide tile of the attention, and the blocks of 128 keys that a GPU block takes at least.
-constexpr int kWideRows = 256;
-constexpr int kLeastBlocks = 2;
+// Rows of a wide tile of the attention.
+constexpr int kWideRows = 256, kHalfRows = 128;
 
 struct AttentionPlan {
-  bool wide;          // chunks of prompts may be among the requests: the instance with wide tiles
-  int narrow_rows;    // rows of a narrow tile (16 or 32)
+  int wide_rows;      // of a wide tile, 0 where no chunk of a prompt is among the requests: the narrow instances
+  int narrow_rows;    // of a narrow tile (16 or 32)
   int target;         // GPU blocks a kv head among which the keys are dealt, 0 where each takes one tile
   long long units;    // tiles and cuts of them, a kv head, at most
   size_t workspace;
@@ -47,24 +46,34 @@ struct AttentionPlan {
 // From what the host knows: shapes and the caller's bounds. The lengths are on the GPU.
 AttentionPlan attention_plan(int tokens, int requests, int max_blocks, int page, int query_heads, int kv_heads,
                              int head_dim, int max_query_len, int max_kv_len) {
-  const int group = query_heads / kv_heads;
+  const int group = query_heads / kv_heads, cus = aoto::device_cu_count();
   const long long rows = (long long)(max_query_len ? std::min(max_query_len, tokens) : tokens) * group;
-  AttentionPlan p{};
-  p.wide = rows > 32;
-  p.narrow_rows = p.wide || rows <= 16 ? 16 : 32;
-  const int tile = (p.wide ? kWideRows : p.narrow_rows) / group;
   const long long some = std::min(requests, tokens);
-  const long long tiles = some + (tokens - some) / std::max(tile, 1);
+  auto tiles = [&](int of) { return some + (tokens - some) / std::max(of / group, 1); };
+  AttentionPlan p{};
+  p.narrow_rows = rows <= 16 || rows > 32 ? 16 : 32;
+  // GPU blocks that the chip holds at a time: two narrow ones on a CU; one with wide tiles (registers; LDS at 128 dims),
+  // two with half as many rows at 64 dims.
+  long long full = 2LL * cus;
+  p.units = tiles(p.narrow_rows);
+  if (rows > 32) {
+    // Half as many rows where whole ones would leave half of the chip idle (32 / 8 heads of 128, 1024 rows: over 1024
+    // keys 40 us against 60, over 5000 126 against 129; 2048 rows over 8048 keys 346 against 292), and at 64 dims
+    // always: two blocks fit a CU there (14 / 2 heads, 4096 rows over 4097 / 10096 keys: 80 / 200 us against 105 / 243).
+    const bool half = head_dim == 64 || 2 * tiles(kWideRows) * kv_heads <= cus;
+    p.wide_rows = half ? kHalfRows : kWideRows;
+    full = head_dim == 64 ? 2LL * cus : cus;
+    p.units = tiles(p.wide_rows);
+  }
   long long keys = std::min<long long>((long long)max_blocks * page, 1 << 28);
+  const long long most = keys / 128 + 8;  // key blocks of a tile
   if (max_kv_len) keys = std::min<long long>(keys, max_kv_len);
-  // GPU blocks that the chip holds at a time: registers leave room for one with wide tiles on a CU, two narrow ones.
-  const long long full = (long long)aoto::device_cu_count() * (p.wide ? 1 : 2);
-  const long long most = (long long)max_blocks * page / 128 + 8;
-  p.units = tiles;
-  if (keys > kLeastBlocks * 128 && tiles * kv_heads < (p.wide ? 1 : 4) * full && tiles * most < (1 << 30)) {
+  // Not worth the join: narrow tiles of up to 256 keys, wide ones of up to 1024 (512 tokens over themselves: 28 us
+  // whole and 35 cut at 128 dims, 19.5 and 24 at 64).
+  if (keys > (p.wide_rows ? 1024 : 256) && p.units * kv_heads < (p.wide_rows ? 1 : 4) * full && p.units * most < (1 << 30)) {
     p.target = (int)((full + kv_heads - 1) / kv_heads);
     p.units += p.target;
-    p.workspace = (size_t)tokens * 16 + (size_t)p.units * kv_heads * (p.wide ? kWideRows : p.narrow_rows) *
+    p.workspace = (size_t)tokens * 16 + (size_t)p.units * kv_heads * (p.wide_rows ? p.wide_rows : p.narrow_rows) *
                                             (head_dim + 2) * sizeof(float);
   }
   return p;
@@ -161,9 +170,9 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention: pages of more than 2^32 elements, or rows 2^30 apart");
   if (!(scale > 0.f) || !std::isfinite(scale))
     return set_error(AOTO_ERR_ARGUMENT, "paged_attention: scale %g is not a positive number", (double)scale);
-  if (query_heads / kv_heads > kWideRows)
+  if (query_heads / kv_heads > kHalfRows)
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention: %d query heads a kv head (at most %d)",
-                     query_heads / kv_heads, kWideRows);
+                     query_heads / kv_heads, kHalfRows);
   const AttentionPlan plan = attention_plan(tokens, requests, max_blocks, page, query_heads, kv_heads, head_dim,
                                             max_query_len, max_kv_len);
   if (plan.workspace && (!workspace || !aligned(workspace, 16)))
@@ -181,13 +190,14 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
   while ((1u << log2) < (unsigned)page) ++log2;
   a.page_magic = (unsigned)(((1ull << (31 + log2)) + page - 1) / page), a.page_shift = log2 ? log2 - 1 : 0;
   a.narrow_tokens = plan.narrow_rows / (query_heads / kv_heads);
-  a.wide_tokens = kWideRows / (query_heads / kv_heads);
-  a.target = plan.target, a.least_blocks = kLeastBlocks, a.record_rows = plan.wide ? kWideRows : plan.narrow_rows;
+  a.wide_tokens = plan.wide_rows / (query_heads / kv_heads);
+  a.target = plan.target, a.least_blocks = 2;
+  a.record_rows = plan.wide_rows ? plan.wide_rows : plan.narrow_rows;
   a.joins = static_cast<int*>(workspace);
   a.records = reinterpret_cast<float*>(static_cast<char*>(workspace) + (size_t)tokens * 16);
   char name[64];
   snprintf(name, sizeof(name), "aoto_paged_attention_d%d_%s", head_dim,
-           plan.wide ? "w" : plan.narrow_rows == 16 ? "n1" : "n2");
+           plan.wide_rows == kWideRows ? "w256" : plan.wide_rows ? "w128" : plan.narrow_rows == 16 ? "n1" : "n2");
   if (int s = launch(name, (plan.target ? plan.target : plan.units) * kv_heads, 1, 256, stream, a)) return s;
   if (!plan.target) return AOTO_OK;
   return launch(head_dim == 64 ? "aoto_paged_attention_join_d64" : "aoto_paged_attention_join_d128",

@@ -17,8 +17,8 @@
 // requests.
 //   narrow tiles (16 NT rows, decodes and drafted tokens): the four waves take 32 keys each of every 128; K goes
 //     straight from the pages to operand registers, V through the wave's own LDS; no barrier in the loop
-//   wide tiles (256 rows, chunks of prompts): the four waves take 64 rows each, 64-key tiles of K and V staged once
-//     for all of them
+//   wide tiles (128 or 256 rows, chunks of prompts): the four waves take 32 or 64 rows each, 64-key tiles of K and V
+//     staged once for all of them
 #pragma once
 
 #include "common.h"
@@ -41,7 +41,6 @@ constexpr int kPagedUnitKeys = 128;  // keys of a key block
 // What starting on an item costs (its rows, table entries and first keys are three round trips to memory), in key
 // blocks: a GPU block that goes from one item to another takes so many fewer.
 constexpr int kPagedLead = 2;
-constexpr int kPagedWideRows = 256;
 
 struct PagedUnit {
   int request, begin, rows;  // its first row and how many
@@ -532,7 +531,8 @@ template <int D>
 struct PagedWideShared {
   uint16_t k[3][64 * D];
   uint16_t v[2][64 * D];
-  uint32_t exist[4][4];  // by tile (mod 4) and staging wave: which of its 16 rows exist
+  uint32_t exist[4][4];  // by tile (mod 4) and staging wave: which of its 16 rows exist (a page, and not past the end)
+  uint32_t known[4][4];  // and which have a page
   uint32_t special[4];   // which of the V tile's rows hold a value that is not finite and not seen by every row
 };
 
@@ -570,16 +570,16 @@ AOTO_DEVICE void acc_settle() {
 }
 
 // v_mfma_f32_32x32x16_bf16: S^T [32 keys x 32 rows] = K . Q^T, O^T [32 d x 32 rows] += V^T . P^T (layouts and slot
-// order as in the prefill attention). A wave has 64 rows: each K and V operand read from LDS serves two products, which
-// halves the traffic that otherwise (32 rows a wave) asks for all of the LDS's 128 bytes a cycle at the products' full
+// order as in the prefill attention). A wave has 32 C rows. With C = 2 each K and V operand read from LDS serves two
+// products, which halves the traffic that otherwise asks for all of the LDS's 128 bytes a cycle at the products' full
 // rate. One wave runs on a SIMD, with 512 registers, and what it issues between two products is free as long as it
 // takes no longer than they do; so a step holds, in this order and spread out between its products, the scores of the
-// next 32 keys (16 products; 24 of the present keys' 32 exponentials a lane) and the present keys' weights with V (16;
-// the other exponentials, the next scores out of their accumulators, their maximum). Operands are read from LDS two
+// next 32 keys (with three quarters of the present keys' exponentials) and the product of the present keys' weights with
+// V (with the other exponentials, the next scores out of their accumulators and their maximum). Operands are read from LDS two
 // products ahead. K and V go from memory to LDS without registers, K two tiles ahead and V one; the 16-byte pieces of a
 // row are permuted by a function of the row (the lanes fetch them so) that spreads each phase of the reads over all
 // banks. Rows' addresses advance by 64 keys a tile without a division or a product but the page's.
-template <int D>
+template <int D, int C>
 AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, int kvh, PagedWideShared<D>& s) {
   constexpr int DS = D / 16, DT = D / 32, LPR = D / 8;  // lanes (16-byte pieces) a row
   constexpr int RPL = 64 / LPR;                         // rows a wave's load covers
@@ -592,13 +592,13 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   const int* table = a.block_tables + unit.request * a.table_stride;
   const int k0 = unit.from * kPagedUnitKeys, k1 = min(unit.keys, unit.to * kPagedUnitKeys);
   const int tiles = k1 > k0 ? (k1 - k0 + 63) / 64 : 0;
-  const bool active = 64 * wave < live;  // a wave of none of the rows only stages
+  const bool active = 32 * C * wave < live;  // a wave of none of the rows only stages
 
-  fa_bf16x8 qf[2][DS];
-  int limit[2];
+  fa_bf16x8 qf[C][DS];
+  int limit[C];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int row = min(64 * wave + 32 * c + col, live - 1), i = unit.token + row / group, g = row % group;
+  for (int c = 0; c < C; ++c) {
+    const int row = min(32 * C * wave + 32 * c + col, live - 1), i = unit.token + row / group, g = row % group;
     const uint16_t* q = a.q + (unit.begin + i) * a.q_token_stride + (kvh * group + g) * a.q_head_stride + 8 * half;
 #pragma unroll
     for (int d = 0; d < DS; ++d) qf[c][d] = *reinterpret_cast<const fa_bf16x8*>(q + 16 * d);
@@ -643,25 +643,29 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   };
   auto place = [&](int tile, const Rows& of, long long (&at)[LOADS]) __attribute__((always_inline)) {
     bool fine = true;
-    bool there[LOADS];
+    bool there[LOADS], page[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const bool known = (unsigned)of.page[i] < (unsigned)a.pages;
       at[i] = (long long)((unsigned long long)(unsigned)(known ? of.page[i] : 0) * (unsigned)a.page_stride) + of.off[i];
       there[i] = known && k0 + 64 * tile + 4 * RPL * i + stage_row < k1;
+      page[i] = known;
       fine = fine && there[i];
     }
-    uint32_t exist = 0xFFFFu;
+    uint32_t exist = 0xFFFFu, paged = 0xFFFFu;
     if (!__all(fine)) {
-      exist = 0;
+      exist = paged = 0;
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const unsigned long long lanes = __ballot(there[i]);
+        const unsigned long long lanes = __ballot(there[i]), pages = __ballot(page[i]);
 #pragma unroll
-        for (int j = 0; j < RPL; ++j) exist |= (uint32_t)(lanes >> (j * LPR) & 1) << (i * RPL + j);
+        for (int j = 0; j < RPL; ++j) {
+          exist |= (uint32_t)(lanes >> (j * LPR) & 1) << (i * RPL + j);
+          paged |= (uint32_t)(pages >> (j * LPR) & 1) << (i * RPL + j);
+        }
       }
     }
-    if (lane == 0) s.exist[tile & 3][wave] = exist;
+    if (lane == 0) s.exist[tile & 3][wave] = exist, s.known[tile & 3][wave] = paged;
   };
   const uint32_t lds_k0 = paged_lds(s.k[0]), lds_v0 = paged_lds(s.v[0]);
   auto fetch_row = [&](const uint16_t* from, const long long (&at)[LOADS], uint32_t to, int i)
@@ -672,13 +676,6 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) fetch_row(from, at, to, i);
   };
-  // the bit of a tile's key (a constant, plus 4 in the upper half of the wave) in what the four waves staged
-  auto bit = [&](const uint32_t (&words)[4], int k) {
-    const uint32_t low = words[k / RPL % 4] >> (k / (4 * RPL) * RPL + k % RPL);
-    const uint32_t high = words[(k + 4) / RPL % 4] >> ((k + 4) / (4 * RPL) * RPL + (k + 4) % RPL);
-    return ((half ? high : low) & 1) != 0;
-  };
-
   // Operands: byte addresses in a tile, XORed with a constant per 16 (K) or 32 (V) dims.
   const uint32_t lds_k = lds_k0 + col * ROWB + ((half ^ swizzle(col)) << 4);
   const int r = lane & 15, v_row = 4 * half + (r >> 2);
@@ -694,23 +691,25 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
     return __builtin_bit_cast(fa_bf16x8, both);
   };
 
-  float run_max[2] = {-INFINITY, -INFINITY}, run_sum[2] = {0.f, 0.f}, ref[2] = {0.f, 0.f};
-  fa_f32x16 o[2][DT];
+  float run_max[C], run_sum[C], ref[C];
+  fa_f32x16 o[C][DT];
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
+  for (int c = 0; c < C; ++c) {
+    run_max[c] = -INFINITY, run_sum[c] = ref[c] = 0.f;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       o[c][d] = fa_f32x16{};
       asm("" : "+a"(o[c][d]));  // in the accumulation registers, here and wherever else than a product changes it
     }
-  fa_f32x16 sc[2];        // scores of the present 32 keys
-  float top[2];           // their maximum, over this lane's
+  }
+  fa_f32x16 sc[C];        // scores of the present 32 keys
+  float top[C];           // their maximum, over this lane's
   constexpr int AHEAD = 2;                 // products (pairs of them) that operands are read ahead; 3 measured the same
   fa_bf16x8 kf[AHEAD + 1], vf[AHEAD + 1];  // operands on their way
 
   auto top_of = [&] {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < C; ++c) {
       top[c] = sc[c][0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) top[c] = fmaxf(top[c], sc[c][e]);
@@ -721,35 +720,49 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
     const uint32_t exist = s.exist[t & 3][0] & s.exist[t & 3][1] & s.exist[t & 3][2] & s.exist[t & 3][3];
     return __builtin_amdgcn_readfirstlane(exist == 0xFFFFu && k0 + 64 * t + 64 <= least) != 0;
   };
-  // The scores that a row may not see, or that are of no key, leave; then the maximum.
+  // The scores that a row may not see, or that are of no page, leave; then the maximum.
   auto mask = [&](int t, int sub) {
     if (whole(t)) return;
-    const int j0 = k0 + 64 * t;
-    const uint32_t exist[4] = {s.exist[t & 3][0], s.exist[t & 3][1], s.exist[t & 3][2], s.exist[t & 3][3]};
+    const int j0 = k0 + 64 * t + 32 * sub + 4 * half;
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < C; ++c) {
+      const int sees = limit[c] - j0;
 #pragma unroll
+      for (int e = 0; e < 16; ++e) sc[c][e] = 8 * (e >> 2) + (e & 3) < sees ? sc[c][e] : -INFINITY;
+    }
+    const uint32_t known = s.known[t & 3][0] & s.known[t & 3][1] & s.known[t & 3][2] & s.known[t & 3][3];
+    if (__builtin_amdgcn_readfirstlane(known) != 0xFFFFu) {
+      uint32_t hidden = 0;  // of this lane's 16 keys
+#pragma unroll 1
       for (int e = 0; e < 16; ++e) {
-        const int k = 32 * sub + 8 * (e >> 2) + (e & 3);
-        if (j0 + k + 4 * half >= limit[c] || !bit(exist, k)) sc[c][e] = -INFINITY;
+        const int k = 32 * sub + 8 * (e >> 2) + 4 * half + (e & 3);
+        hidden |= (~s.known[t & 3][k / RPL % 4] >> (k / (4 * RPL) * RPL + k % RPL) & 1) << e;
       }
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[c][e] = hidden >> e & 1 ? -INFINITY : sc[c][e];
+    }
     top_of();
   };
   // the exponentials' reference moves only where a score passes it by more than 2^8; O and the sum follow
   auto move = [&] {
-    float keep[2];
+    float keep[C];
+    bool some = false;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < C; ++c) {
       const float most = xor32_max(top[c]) * c2;
       const float moved = most > run_max[c] + 8.f ? most : run_max[c];
-      keep[c] = moved == run_max[c] ? 1.f : __builtin_amdgcn_exp2f(run_max[c] - moved);
+      // (nothing to scale yet where there was no reference)
+      keep[c] = moved == run_max[c] || run_max[c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(run_max[c] - moved);
       run_max[c] = moved;
       ref[c] = moved == -INFINITY ? 0.f : moved;
+      some = some || keep[c] != 1.f;
     }
-    if (__any(keep[0] != 1.f || keep[1] != 1.f)) {
+    if (__any(some)) {
       acc_settle();
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < C; ++c) {
         run_sum[c] *= keep[c];
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -769,34 +782,37 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   auto step = [&](uint32_t v_base, int sub, uint32_t k_base, int k_sub, uint32_t kn_base, int kn_sub, auto beside)
       __attribute__((always_inline)) {
     constexpr int START = DS == 8 ? 2 : 1;           // products after which the reference is settled
-    constexpr int PER = 12 / (DS - START);           // pairs of exponentials after each of the others
-    uint32_t pk[2][2][4];
-    auto pair = [&](int u) {  // pair u of 16: k-step u / 8, rows' half u / 4 % 2
-      const int kt = u >> 3, c = u >> 2 & 1, j = u & 3, e = 8 * kt + 2 * j;
+    constexpr int PER = 6 * C / (DS - START);        // pairs of exponentials after each of the others
+    uint32_t pk[C][2][4];
+    auto pair = [&](int u) {  // pair u of 8 C: k-step u / 4 C, rows' part u / 4 % C
+      const int kt = u / (4 * C), c = u / 4 % C, j = u & 3, e = 8 * kt + 2 * j;
       const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][e], c2, -ref[c]));
       const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][e + 1], c2, -ref[c]));
       pk[c][kt][j] = cvt_pk_bf16(p0, p1);
       run_sum[c] = dot2_bf16(pk[c][kt][j], 0x3F803F80u, run_sum[c]);  // the rounded weights' sum
     };
-    fa_f32x16 next[2] = {fa_f32x16{}, fa_f32x16{}};
+    fa_f32x16 next[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) next[c] = fa_f32x16{};
 #pragma unroll
     for (int d = 0; d < DS; ++d) {
       constexpr int RING = AHEAD + 1;
       if (d + AHEAD < DS) kf[(d + AHEAD) % RING] = read_k(k_base, k_sub, d + AHEAD);
       else vf[d + AHEAD - DS] = read_v(v_base, 2 * sub + (d + AHEAD - DS) / DT, (d + AHEAD - DS) % DT);
-      next[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[d % RING], qf[0][d], next[0], 0, 0, 0);
-      if (d >= START)
 #pragma unroll
-        for (int u = 0; u < PER / 2; ++u) pair((d - START) * PER + u);
-      next[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[d % RING], qf[1][d], next[1], 0, 0, 0);
-      if (d >= START)
+      for (int c = 0; c < C; ++c) {
+        next[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[d % RING], qf[c][d], next[c], 0, 0, 0);
+        if (d >= START)
 #pragma unroll
-        for (int u = PER / 2; u < PER; ++u) pair((d - START) * PER + u);
+          for (int u = PER * c / C; u < PER * (c + 1) / C; ++u) pair((d - START) * PER + u);
+      }
       beside(d);
       if (d == START - 1) move();
       __builtin_amdgcn_sched_barrier(0);
     }
-    float most[2] = {-INFINITY, -INFINITY};
+    float most[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) most[c] = -INFINITY;
 #pragma unroll
     for (int m = 0; m < 2 * DT; ++m) {
       const int kt = m / DT, d = m % DT;
@@ -804,14 +820,14 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
       if (m + AHEAD < 2 * DT) vf[(m + AHEAD) % RING] = read_v(v_base, 2 * sub + (m + AHEAD) / DT, (m + AHEAD) % DT);
       else kf[m + AHEAD - 2 * DT] = read_k(kn_base, kn_sub, m + AHEAD - 2 * DT);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < C; ++c) {
         const uint32_t w[4] = {pk[c][kt][0], pk[c][kt][1], pk[c][kt][2], pk[c][kt][3]};
         o[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[m % RING], __builtin_bit_cast(fa_bf16x8, w), o[c][d], 0, 0, 0);
         if (kt == 0)
 #pragma unroll
-          for (int u = 12 + 4 * d / DT; u < 12 + 4 * (d + 1) / DT; ++u)
-            if (c == u % 2) pair(u);
-        // the next scores of rows' half c: 8 / DT of the first (second) eight
+          for (int u = 6 * C + 2 * C * d / DT; u < 6 * C + 2 * C * (d + 1) / DT; ++u)
+            if (c == u % C) pair(u);
+        // the next scores of rows' part c: 8 / DT of the first (second) eight
 #pragma unroll
         for (int i = 0; i < 8 / DT; ++i) {
           const int e = 8 * kt + d * (8 / DT) + i;
@@ -824,9 +840,12 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
       beside(DS + m);
       __builtin_amdgcn_sched_barrier(0);
     }
-    top[0] = most[0], top[1] = most[1];
     // what the next step needs is done in this one, among its products
-    asm volatile("" : "+v"(run_sum[0]), "+v"(run_sum[1]), "+v"(top[0]), "+v"(top[1]));
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      top[c] = most[c];
+      asm volatile("" : "+v"(run_sum[c]), "+v"(top[c]));
+    }
   };
   // V of tile t in LDS, where some of its rows do not exist or are not seen by every row: zeros for the former; for the
   // latter what is not finite goes (0 * inf) and is added at the end of the tile, row by row
@@ -866,7 +885,7 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
             const uint2 x = *reinterpret_cast<const uint2*>(v + 32 * d + 8 * g);
             const float add[4] = {special_lo(x.x), special_hi(x.x), special_lo(x.y), special_hi(x.y)};
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < C; ++c)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 float y = o[c][d][4 * g + i];
@@ -897,19 +916,20 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
     paged_landed();
     __syncthreads();
     if (active) {
-      sc[0] = fa_f32x16{}, sc[1] = fa_f32x16{};
+#pragma unroll
+      for (int c = 0; c < C; ++c) sc[c] = fa_f32x16{};
 #pragma unroll
       for (int d = 0; d < DS; ++d) {
         const fa_bf16x8 k = read_k(lds_k, 0, d);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) sc[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[c][d], sc[c], 0, 0, 0);
+        for (int c = 0; c < C; ++c) sc[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[c][d], sc[c], 0, 0, 0);
       }
       top_of();
       mask(0, 0);
 #pragma unroll
       for (int d = 0; d < AHEAD; ++d) kf[d] = read_k(lds_k, 1, d);
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           float x = sc[c][e];
@@ -980,9 +1000,9 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   }
 
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < C; ++c) {
     const float sum = xor32_sum(run_sum[c]);
-    const int row = 64 * wave + 32 * c + col;
+    const int row = 32 * C * wave + 32 * c + col;
     if (row >= live) continue;
     if (unit.parts > 1) {
       float* rec = paged_record(a, unit.record + unit.part, kvh, row, D);
@@ -1026,7 +1046,7 @@ __device__ void paged_attention_narrow(const PagedAttentionArgs& a) {
   }
 }
 
-template <int D>
+template <int D, int C>
 __device__ void paged_attention_mixed(const PagedAttentionArgs& a) {
   __shared__ __attribute__((aligned(256))) union {  // the wide form's addresses are XORed within a row
     PagedNarrowShared<D, 1> narrow;
@@ -1038,7 +1058,7 @@ __device__ void paged_attention_mixed(const PagedAttentionArgs& a) {
   for (PagedUnit unit; walk.next(a, unit); __syncthreads()) {
     paged_note(a, unit, kvh);
     if (unit.narrow) paged_narrow<D, 1>(a, unit, kvh, s.narrow);
-    else paged_wide<D>(a, unit, kvh, s.wide);
+    else paged_wide<D, C>(a, unit, kvh, s.wide);
   }
 }
 
@@ -1101,9 +1121,14 @@ __device__ void paged_attention_join(const PagedAttentionArgs& a) {
   extern "C" __global__ __launch_bounds__(256, 2) void aoto_paged_attention_d##D##_n2(PagedAttentionArgs a) {      \
     aoto::paged_attention_narrow<D, 2>(a);                                                                         \
   }                                                                                                                \
-  extern "C" __global__ __launch_bounds__(256, 1) void aoto_paged_attention_d##D##_w(PagedAttentionArgs a) {       \
-    aoto::paged_attention_mixed<D>(a);                                                                             \
+  extern "C" __global__ __launch_bounds__(256, 128 / D) void aoto_paged_attention_d##D##_w128(PagedAttentionArgs a) {            \
+    aoto::paged_attention_mixed<D, 1>(a);                                                                          \
   }                                                                                                                \
   extern "C" __global__ __launch_bounds__(256) void aoto_paged_attention_join_d##D(PagedAttentionArgs a) {         \
     aoto::paged_attention_join<D>(a);                                                                              \
+  }
+// 256-row tiles, at 128 dims (at 64 half the rows and two blocks a CU were faster throughout).
+#define AOTO_PAGED_ATTENTION_WHOLE(D)                                                                              \
+  extern "C" __global__ __launch_bounds__(256, 1) void aoto_paged_attention_d##D##_w256(PagedAttentionArgs a) {    \
+    aoto::paged_attention_mixed<D, 2>(a);                                                                          \
   }

@@ -357,26 +357,69 @@ def test_attention_keeps_what_it_may_not_see_out(rows):
     _check_attention(s, _attend(s))
 
 
+def _check_special_values(s, marks, **bounds):
+    """Place (request, key, value) in two dims of the request's own each: rows that see the key have the value there."""
+
+    hq, dim = s["q"].shape[1:]
+    page = s["keys"].shape[2]
+    for i, (r, j, value) in enumerate(marks):
+        s["values"][s["tables"][r, j // page], :, j % page, 3 * i: 3 * i + 2] = value
+    s["device"][1].copy_(to_gpu_bf16(s["values"]))
+    got = from_gpu_bf16(_attend(s, **bounds)).astype(np.float64)
+    plain = {**s, "values": np.where(np.isfinite(s["values"]), s["values"], 0.0)}
+    want, size, written = oracle.attention(plain["q"], plain["keys"], plain["values"], s["tables"], s["start"], s["kv"])
+    special = np.zeros(want.shape)
+    for i, (r, j, value) in enumerate(marks):
+        rows = s["start"][r + 1] - s["start"][r]
+        seen = s["start"][r] + np.arange(rows)[s["kv"][r] - rows + np.arange(rows) >= j]
+        for h in range(hq):
+            special[seen[:, None], dim * h + 3 * i + np.arange(2)] = value
+    odd = special != 0
+    assert odd.any()
+    np.testing.assert_array_equal(got[odd], special[odd])
+    assert (np.abs(got - want) <= attention_bound(want, size))[~odd & written[:, None]].all()
+
+
 @pytest.mark.parametrize("rows", [1, 5, 40])
 def test_attention_of_infinite_values(rows):
     # an infinite value reaches the rows that see its key, in its own dims, and no others
-    rng = np.random.default_rng(16)
-    s = _requests(rng, [(rows, 333), (rows, rows), (rows, 64)], 8, 2, 64, 16)
+    s = _requests(np.random.default_rng(16), [(rows, 333), (rows, rows), (rows, 64)], 8, 2, 64, 16)
     last = s["kv"] - 1
-    for r, (j, value) in enumerate([(200, np.inf), (last[1], -np.inf), (last[2] - rows // 2, np.nan)]):
-        s["values"][s["tables"][r, j // 16], :, j % 16, 3 * r: 3 * r + 2] = value
+    _check_special_values(s, [(0, 200, np.inf), (1, last[1], -np.inf), (2, last[2] - rows // 2, np.nan)])
+
+
+#: kernel, query heads, kv heads, head dim, most rows of a request, requests
+FORMS = [("d64_n1", 8, 4, 64, 8, 5), ("d64_n2", 8, 4, 64, 16, 5), ("d64_w128", 14, 2, 64, 150, 7),
+         ("d128_n1", 8, 2, 128, 4, 5), ("d128_n2", 8, 2, 128, 8, 5), ("d128_w128", 12, 2, 128, 150, 5),
+         ("d128_w256", 32, 8, 128, 80, 20), ("d128_w256", 128, 1, 128, 64, 9), ("d128_w128", 128, 1, 128, 7, 3)]
+
+
+@pytest.mark.parametrize("kernel,hq,hkv,dim,most,requests", FORMS)
+@pytest.mark.parametrize("keys", [700, 1500])  # within one item, over several
+def test_attention_of_every_form(kernel, hq, hkv, dim, most, requests, keys):
+    rng = np.random.default_rng(hq + most + keys)
+    rows = rng.integers(0, most + 1, requests)
+    rows[1], rows[2], rows[-1] = most, most - 1, most
+    lengths = [(int(n), int(n) + int(rng.integers(0, 400))) for n in rows]
+    lengths[2] = (most - 1, keys)
+    s = _requests(rng, lengths, hq, hkv, dim, 16, tail=3)
+    bounds = dict(max_query_len=most, max_kv_len=keys)
+    with _ops().recording_launches() as take:
+        got = _attend(s, **bounds)
+        assert "aoto_paged_attention_" + kernel in take()
+    _check_attention(s, got)
+    _check_attention(s, _attend(s, causal=False, **bounds), causal=False)
+    kv = s["kv"].copy()
+    s["kv"][1], s["kv"][-1] = most // 2, 0       # the first rows see no key; no row sees one
+    _check_attention(s, _attend(s, **bounds))
+    s["kv"] = kv
+    last = s["kv"] - 1
+    _check_special_values(s, [(1, last[1], np.inf), (2, keys - most, -np.inf), (2, last[2] - most // 2, np.nan),
+                              (2, 0, -np.inf)], **bounds)
+    s["values"] = np.where(np.isfinite(s["values"]), s["values"], 0.0)
     s["device"][1].copy_(to_gpu_bf16(s["values"]))
-    got = from_gpu_bf16(_attend(s)).astype(np.float64)
-    plain = {**s, "values": np.where(np.isfinite(s["values"]), s["values"], 0.0)}
-    want, size, _ = oracle.attention(plain["q"], plain["keys"], plain["values"], s["tables"], s["start"], s["kv"])
-    special = np.zeros(want.shape)
-    for r, (j, value) in enumerate([(200, np.inf), (last[1], -np.inf), (last[2] - rows // 2, np.nan)]):
-        seen = s["start"][r] + np.arange(rows)[s["kv"][r] - rows + np.arange(rows) >= j]
-        for h in range(8):
-            special[seen[:, None], 64 * h + 3 * r + np.arange(2)] = value
-    odd = special != 0
-    np.testing.assert_array_equal(got[odd], special[odd])
-    assert (np.abs(got - want) <= attention_bound(want, size))[~odd].all()
+    s["tables"][2, 3], s["tables"][2, -(-keys // 16) - 1], s["tables"][1, 0] = -1, 10 ** 6, -(2 ** 31)
+    _check_attention(s, _attend(s, **bounds))
 
 
 @pytest.mark.parametrize("rows", [1, 20])
