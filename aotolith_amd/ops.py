@@ -26,10 +26,12 @@ BF16 = torch.bfloat16
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
-def _stream() -> int:
+def _stream(device: int | None = None) -> int:
+    """The current device's stream (``device``: that device's number, where the caller has it)."""
+
     if _raw_stream is None:
         return torch.cuda.current_stream().cuda_stream
-    return _raw_stream(torch.cuda.current_device())
+    return _raw_stream(torch.cuda.current_device() if device is None else device)
 
 
 def _ptr(tensor: torch.Tensor | None) -> int | None:
@@ -1221,26 +1223,32 @@ class PagedStep(NamedTuple):
     free_start: torch.Tensor    # int32 [1]
 
 
-def _on_current(name: str, tensor: torch.Tensor) -> None:
-    """The launch goes to the current device's stream: a tensor of another device would be read across the link, or
-    not at all."""
+def _on_current(name: str, tensor: torch.Tensor) -> int:
+    """The device of ``tensor``, the current one: the launch goes to its stream, and a tensor of another device would
+    be read across the link, or not at all."""
 
-    if tensor.get_device() != torch.cuda.current_device():
+    device = tensor.get_device()
+    if device != torch.cuda.current_device():
         raise ValueError(f"{name} is on {tensor.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return device
 
 
 def _expect_all(device: int, tensors) -> None:
     """:func:`_expect` for ``(tensor, name, dtype, shape)`` of one call, all of them on ``device``."""
 
     for tensor, name, dtype, shape in tensors:
-        _expect(tensor, name, dtype, shape)
-        if tensor.get_device() != device:
+        if not (isinstance(tensor, torch.Tensor) and tensor.get_device() == device and tensor.dtype is dtype
+                and tensor.is_contiguous() and (shape is None or tensor.shape == shape)):
+            _expect(tensor, name, dtype, shape)
             raise ValueError(f"{name} is on {tensor.device}, the call's other tensors on cuda:{device}")
 
 
 def _expect_rows(tensor: torch.Tensor, name: str, dtype: torch.dtype, dims: int, device: int) -> None:
     """A ``dims``-dimensional operand whose rows (last dimension) are contiguous, at any other strides."""
 
+    if (isinstance(tensor, torch.Tensor) and tensor.is_cuda and tensor.get_device() == device
+            and tensor.dtype is dtype and tensor.dim() == dims and tensor.stride(-1) == 1):
+        return
     if not isinstance(tensor, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(tensor).__name__}")
     if tensor.device.type != "cuda":
@@ -1255,14 +1263,15 @@ def _expect_rows(tensor: torch.Tensor, name: str, dtype: torch.dtype, dims: int,
         raise ValueError(f"{name}'s rows must be contiguous")
 
 
-def _expect_pages(keys: torch.Tensor, values: torch.Tensor, device: int) -> tuple[int, int, int, int]:
-    """``(pages, Hkv, page, D)`` of a layer's cache."""
+def _expect_pages(keys: torch.Tensor, values: torch.Tensor, device: int) -> tuple[tuple, tuple]:
+    """``(pages, Hkv, page, D)`` of a layer's cache, and its strides."""
 
     _expect_rows(keys, "keys", BF16, 4, device)
     _expect_rows(values, "values", BF16, 4, device)
-    if keys.shape != values.shape or keys.stride() != values.stride():
+    shape, strides = keys.shape, keys.stride()
+    if shape != values.shape or strides != values.stride():
         raise ValueError("keys and values must have one shape and the same strides")
-    return tuple(keys.shape)
+    return shape, strides
 
 
 def paged_tables(
@@ -1295,14 +1304,14 @@ def paged_tables(
     """
 
     _expect(context_lens, "context_lens", torch.int32)
-    device = context_lens.get_device()
-    _on_current("context_lens", context_lens)
+    device = _on_current("context_lens", context_lens)
     requests = context_lens.numel()
     max_tokens = int(max_tokens)
+    if context_lens.dim() != 1:
+        raise ValueError(f"context_lens must be [R], got {tuple(context_lens.shape)}")
     _expect_all(device, (
-        (context_lens, "context_lens", torch.int32, (requests,)), (new_lens, "new_lens", torch.int32, (requests,)),
-        (page_counts, "page_counts", torch.int32, (requests,)), (free_pages, "free_pages", torch.int32, None),
-        (free_start, "free_start", torch.int32, (1,)),
+        (new_lens, "new_lens", torch.int32, (requests,)), (page_counts, "page_counts", torch.int32, (requests,)),
+        (free_pages, "free_pages", torch.int32, None), (free_start, "free_start", torch.int32, (1,)),
     ))
     _expect_rows(block_tables, "block_tables", torch.int32, 2, device)
     if block_tables.shape[0] != requests:
@@ -1312,11 +1321,10 @@ def paged_tables(
     if max_tokens < 0:
         raise ValueError(f"max_tokens must not be negative, got {max_tokens}")
     if step is None:
-        where = context_lens.device
-        lens = torch.empty((3 * requests + 2,), dtype=torch.int32, device=where)
-        maps = torch.empty((2, max_tokens), dtype=torch.int64, device=where)
-        start, kv, counts, first = lens.split((requests + 1, requests, requests, 1))
-        step = PagedStep(start, kv, maps[0], maps[1], counts, first)
+        lens = context_lens.new_empty((3 * requests + 2,))
+        start, kv, counts, first = lens.split_with_sizes((requests + 1, requests, requests, 1))
+        maps = torch.empty((2, max_tokens), dtype=torch.int64, device=context_lens.device)
+        step = PagedStep(start, kv, *maps.unbind(), counts, first)
     else:
         _expect_all(device, (
             (step.query_start, "step.query_start", torch.int32, (requests + 1,)),
@@ -1332,7 +1340,7 @@ def paged_tables(
             _ptr(context_lens), _ptr(new_lens), _ptr(block_tables), block_tables.stride(0), _ptr(page_counts),
             _ptr(free_pages), _ptr(free_start), requests, block_tables.shape[1], free_pages.numel(), int(page_size),
             max_tokens, _ptr(step.query_start), _ptr(step.kv_lens), _ptr(step.positions), _ptr(step.slots),
-            _ptr(step.page_counts), _ptr(step.free_start), _ptr(error), _stream(),
+            _ptr(step.page_counts), _ptr(step.free_start), _ptr(error), _stream(device),
         )
     )
     return step
@@ -1359,34 +1367,30 @@ def paged_rope_append(
     or ``PAGED_BAD_POSITION`` in ``error`` (int32 ``[1]``). Slots other than -1 must not repeat within a call.
     """
 
-    _expect(positions, "positions", torch.int64)
-    _on_current("positions", positions)
-    device = positions.get_device()
-    _expect_rows(qkv, "qkv", BF16, 2, device)
-    pages, kv_heads, page, dim = _expect_pages(keys, values, device)
+    _expect_rows(qkv, "qkv", BF16, 2, qkv.get_device() if isinstance(qkv, torch.Tensor) else 0)
+    device = _on_current("qkv", qkv)
+    (pages, kv_heads, page, dim), (page_stride, head_stride, slot_stride, _) = _expect_pages(keys, values, device)
     tokens, width = qkv.shape
     query_heads = int(query_heads)
     if query_heads <= 0 or width != (query_heads + 2 * kv_heads) * dim:
         raise ValueError(f"qkv rows of {width} do not hold {query_heads} + 2 x {kv_heads} heads of {dim}")
-    _expect(cos_table, "cos_table", BF16)
+    _expect_all(device, ((positions, "positions", torch.int64, (tokens,)), (slots, "slots", torch.int64, (tokens,)),
+                         (cos_table, "cos_table", BF16, None)))
     if cos_table.dim() != 2 or cos_table.shape[1] != dim:
         raise ValueError(f"cos_table must be [P, {dim}], got {tuple(cos_table.shape)}")
-    _expect_all(device, (
-        (positions, "positions", torch.int64, (tokens,)), (slots, "slots", torch.int64, (tokens,)),
-        (cos_table, "cos_table", BF16, None), (sin_table, "sin_table", BF16, tuple(cos_table.shape)),
-    ))
+    _expect_all(device, ((sin_table, "sin_table", BF16, cos_table.shape),))
     if error is not None:
         _expect_all(device, ((error, "error", torch.int32, (1,)),))
     if q_out is None:
-        q_out = torch.empty((tokens, query_heads, dim), dtype=BF16, device=qkv.device)
+        q_out = qkv.new_empty((tokens, query_heads, dim))
     else:
         _expect_all(device, ((q_out, "q_out", BF16, (tokens, query_heads, dim)),))
     _ready(qkv)
     _lib.check(
         _lib.library().aoto_hip_paged_rope_append(
             _ptr(qkv), qkv.stride(0), _ptr(positions), _ptr(slots), _ptr(cos_table), _ptr(sin_table),
-            cos_table.shape[0], _ptr(keys), _ptr(values), keys.stride(0), keys.stride(1), keys.stride(2), pages, page,
-            tokens, query_heads, kv_heads, dim, _ptr(q_out), _ptr(error), _stream(),
+            cos_table.shape[0], _ptr(keys), _ptr(values), page_stride, head_stride, slot_stride, pages, page, tokens,
+            query_heads, kv_heads, dim, _ptr(q_out), _ptr(error), _stream(device),
         )
     )
     return q_out
@@ -1431,10 +1435,9 @@ def paged_attention(
     """
 
     _expect_rows(q, "q", BF16, 3, q.get_device() if isinstance(q, torch.Tensor) else 0)
-    _on_current("q", q)
-    device = q.get_device()
+    device = _on_current("q", q)
     tokens, query_heads, dim = q.shape
-    pages, kv_heads, page, key_dim = _expect_pages(keys, values, device)
+    (pages, kv_heads, page, key_dim), (page_stride, head_stride, slot_stride, _) = _expect_pages(keys, values, device)
     if key_dim != dim:
         raise ValueError(f"q heads have {dim} elements, the cache's {key_dim}")
     _expect_rows(block_tables, "block_tables", torch.int32, 2, device)
@@ -1444,7 +1447,7 @@ def paged_attention(
     if scale is None:
         scale = ctypes.c_float(dim ** -0.5).value
     if out is None:
-        out = torch.empty((tokens, query_heads * dim), dtype=BF16, device=q.device)
+        out = q.new_empty((tokens, query_heads * dim))
     else:
         _expect_all(device, ((out, "out", BF16, (tokens, query_heads * dim)),))
     _ready(q)
@@ -1462,10 +1465,10 @@ def paged_attention(
         workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
     _lib.check(
         lib.aoto_hip_paged_attention(
-            _ptr(q), q.stride(0), q.stride(1), _ptr(keys), _ptr(values), keys.stride(0), keys.stride(1),
-            keys.stride(2), pages, page, _ptr(block_tables), block_tables.stride(0), max_blocks, _ptr(query_start),
+            _ptr(q), q.stride(0), q.stride(1), _ptr(keys), _ptr(values), page_stride, head_stride,
+            slot_stride, pages, page, _ptr(block_tables), block_tables.stride(0), max_blocks, _ptr(query_start),
             _ptr(kv_lens), tokens, requests, query_heads, kv_heads, dim, int(bool(causal)), float(scale),
-            max_query_len, max_kv_len, _ptr(workspace if need else None), _ptr(out), _stream(),
+            max_query_len, max_kv_len, _ptr(workspace if need else None), _ptr(out), _stream(device),
         )
     )
     return out
@@ -1501,15 +1504,13 @@ def verify_draft(
     if dtype not in (BF16, torch.float32):
         raise TypeError(f"logits must be bf16 or f32, got {dtype}")
     _expect_rows(logits, "logits", dtype, 2, logits.get_device() if isinstance(logits, torch.Tensor) else 0)
-    _on_current("logits", logits)
-    device = logits.get_device()
+    device = _on_current("logits", logits)
     rows, vocab = logits.shape
-    _expect(draft_tokens, "draft_tokens", torch.int64)
+    _expect_all(device, ((draft_tokens, "draft_tokens", torch.int64, None),))
     if draft_tokens.dim() != 2:
         raise ValueError(f"draft_tokens must be [R, K], got {tuple(draft_tokens.shape)}")
     requests, drafts = draft_tokens.shape
-    _expect_all(device, ((draft_tokens, "draft_tokens", torch.int64, (requests, drafts)),
-                         (query_start, "query_start", torch.int32, (requests + 1,)),
+    _expect_all(device, ((query_start, "query_start", torch.int32, (requests + 1,)),
                          (uniforms, "uniforms", torch.float32, (requests, drafts + 1))))
     if temperature is not None:
         _expect_all(device, ((temperature, "temperature", torch.float32, (requests,)),))
@@ -1518,11 +1519,11 @@ def verify_draft(
         if tuple(draft_logits.shape) != (requests, drafts, vocab):
             raise ValueError(f"draft_logits must be {(requests, drafts, vocab)}, got {tuple(draft_logits.shape)}")
     if tokens is None:
-        tokens = torch.empty((requests, drafts + 1), dtype=torch.int64, device=logits.device)
+        tokens = draft_tokens.new_empty((requests, drafts + 1))
     else:
         _expect_all(device, ((tokens, "tokens", torch.int64, (requests, drafts + 1)),))
     if accepted is None:
-        accepted = torch.empty((requests,), dtype=torch.int32, device=logits.device)
+        accepted = query_start.new_empty((requests,))
     else:
         _expect_all(device, ((accepted, "accepted", torch.int32, (requests,)),))
     _ready(logits)
@@ -1541,7 +1542,7 @@ def verify_draft(
             _ptr(logits), int(dtype is torch.float32), logits.stride(0), rows, vocab, _ptr(draft_tokens),
             _ptr(draft_logits), 0 if draft_logits is None else draft_logits.stride(0),
             0 if draft_logits is None else draft_logits.stride(1), _ptr(query_start), _ptr(uniforms),
-            _ptr(temperature), requests, drafts, _ptr(workspace), _ptr(tokens), _ptr(accepted), _stream(),
+            _ptr(temperature), requests, drafts, _ptr(workspace), _ptr(tokens), _ptr(accepted), _stream(device),
         )
     )
     return tokens, accepted
