@@ -221,6 +221,7 @@ int aoto_hip_verify_draft(const void* logits, int logits_f32, int64_t row_stride
   if (rows <= 0 || vocab <= 0 || requests <= 0 || drafts < 0)
     return set_error(AOTO_ERR_ARGUMENT, "verify_draft: bad shape");
   if (drafts > 62) return set_error(AOTO_ERR_UNSUPPORTED, "verify_draft: %d drafts a request (at most 62)", drafts);
+  if (vocab > 1 << 30) return set_error(AOTO_ERR_UNSUPPORTED, "verify_draft: %d tokens (at most 2^30)", vocab);
   const size_t size = logits_f32 ? 4 : 2;
   if (!aligned(logits, size) || (draft_logits && !aligned(draft_logits, size)) || !aligned(workspace, 8))
     return set_error(AOTO_ERR_ARGUMENT, "verify_draft: logits aligned to their type, workspace to 8 bytes");
@@ -238,11 +239,11 @@ int aoto_hip_verify_draft(const void* logits, int logits_f32, int64_t row_stride
                      (long long)requests * a.judged, 256, stream, a))
     return s;
   if (!temperature || !a.draft_logits)
-    return launch(logits_f32 ? "aoto_verify_follow_f32" : "aoto_verify_follow_bf16", requests, 1, 512, stream, a);
+    return launch(logits_f32 ? "aoto_verify_follow_f32" : "aoto_verify_follow_bf16", requests, 1, kVerifyChunk / 8, stream, a);
   if (int s = launch(logits_f32 ? "aoto_verify_law_f32" : "aoto_verify_law_bf16", requests, 1, 256, stream, a)) return s;
   if (int s = launch(logits_f32 ? "aoto_verify_mass_f32" : "aoto_verify_mass_bf16", a.chunks, requests, 256, stream, a))
     return s;
-  return launch(logits_f32 ? "aoto_verify_pick_f32" : "aoto_verify_pick_bf16", requests, 1, 512, stream, a);
+  return launch(logits_f32 ? "aoto_verify_pick_f32" : "aoto_verify_pick_bf16", requests, 1, kVerifyChunk / 8, stream, a);
 }
 
 }  // extern "C"

@@ -54,7 +54,7 @@ struct PagedAttentionArgs {
   int tokens, requests, pages, page, query_heads, kv_heads, causal;
   int table_keys;      // max_blocks * page, at most 2^28
   unsigned page_magic, page_shift;  // key / page = (key * page_magic) >> 32 >> page_shift for keys below 2^31
-  int narrow_tokens, wide_tokens;   // of a request, that a tile of 16 NT / 256 rows holds
+  int narrow_tokens, wide_tokens;   // of a request, that a narrow / wide tile holds
   int target;          // GPU blocks a kv head among which the key blocks (128 keys) are dealt; 0: one a tile
   int least_blocks;    // key blocks that make a GPU block worth its while
   int record_rows;     // rows of a record
@@ -62,7 +62,7 @@ struct PagedAttentionArgs {
 };
 
 // Tokens of a vocabulary that one wave of the verification takes, and the bytes of what it leaves of a row of them.
-constexpr int kVerifyChunk = 4096;
+constexpr int kVerifyChunk = 2048;
 constexpr int kVerifyChunkBytes = 16;
 constexpr int kVerifyLawBytes = 96;  // what stands of a request's drafts, and where its token comes from
 

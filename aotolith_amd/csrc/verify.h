@@ -12,14 +12,21 @@
 // move it in a percent of the calls.
 //
 // Launches over chunks of kVerifyChunk tokens: every row's maximum, its place and sum of weights by chunk; with a draft
-// model's logits, what stands and the weights the following token is drawn from, summed by chunk; the token. Bound by the first one's read
-// of the logits and, where they are sampled from, about as much by its 20 f64 operations a logit.
+// model's logits, what stands and the weights the following token is drawn from, summed by chunk; the token.
+//
+// The first is bound by its instructions, 20 a logit of which 11 in 64 bits (64 requests, up to five drafts with their
+// logits, 151936 bf16 tokens: 33 us of 57), after it by the chain request -> statistics -> law -> chunk -> token, each
+// a round trip to memory: 6 + 10 + 10 us there, 13 of 25 us without a draft model. Chunks of 2048 tokens deal the work
+// out evenly (57 us; 4096: 63, 1024: 64 us) and leave the joins short. A loop over the chunk's loads, for less code,
+// cost more than the instructions it fetched (1 to 2 us).
 #pragma once
 
 #include "common.h"
 #include "paged_args.h"
 
 namespace aoto {
+
+constexpr int kVerifyPick = kVerifyChunk / 8;  // threads of the last launch: a chunk is eight tokens each
 
 // What the first launch leaves of a chunk of a row: the sum of exp((z - max) / T), the maximum and its first place.
 struct VerifyChunk {
@@ -38,7 +45,8 @@ AOTO_DEVICE void verify_table(VerifyTable& table) {
     // the series of e^y, 0 <= y < ln 2, to the 20th power (remainder 1e-23)
     const double y = threadIdx.x * (0.6931471805599453094 / 32);
     double s = 1.0;
-    for (int k = 20; k > 0; --k) s = fma(s, y / k, 1.0);
+#pragma unroll
+    for (int k = 20; k > 0; --k) s = fma(s, y * (1.0 / k), 1.0);
     table.at[threadIdx.x] = s;
   }
 }
@@ -46,22 +54,31 @@ AOTO_DEVICE void verify_table(VerifyTable& table) {
 // 2^x, x = d * heat32 / 32, for -2048 < x <= 0 (0 from 2^-1075 on): 32 x is rounded to a whole number k by a sum with
 // 1.5 * 2^52, whose low bits are k; what is left, f = 32 x - k in one rounding, |f| <= 1/2, goes through the series of
 // e^(f ln 2 / 32) to the 5th power (remainder below (ln 2 / 64)^6 / 6! = 2.3e-15), k mod 32 through the table, the rest
-// of k to the exponent. NORMAL: x > -1000, and the exponent is moved by whole-number arithmetic.
-template <bool NORMAL = false>
-AOTO_DEVICE double exp2_of(double d, double heat32, const VerifyTable& table) {
+// of k to the exponent.
+struct VerifyPower {
+  double series;
+  int k;
+};
+AOTO_DEVICE VerifyPower exp2_parts(double d, double heat32) {
   constexpr double kRound = 6755399441055744.0;
   const double t = fma(d, heat32, kRound);
   const double f = fma(d, heat32, kRound - t);
-  const int k = __double2loint(t);
   double s = 3.973709984549416e-11;  // (ln 2 / 32)^5 / 5!, and on to the 0th
   s = fma(s, f, 9.172562701824643e-09);
   s = fma(s, f, 1.693850972437182e-06);
   s = fma(s, f, 0.0002345961982022468);
   s = fma(s, f, 0.02166084939249829);
-  s = fma(s, f, 1.0);
-  s *= table.at[k & 31];
-  if constexpr (NORMAL) return __hiloint2double(__double2hiint(s) + ((k >> 5) << 20), __double2loint(s));
-  return ldexp(s, k >> 5);
+  return {fma(s, f, 1.0), __double2loint(t)};
+}
+AOTO_DEVICE double exp2_of(double d, double heat32, const VerifyTable& table) {
+  const VerifyPower p = exp2_parts(d, heat32);
+  return ldexp(p.series * table.at[p.k & 31], p.k >> 5);
+}
+// sum + 2^x for x > -1000: the exponent goes into the table's number by whole-number arithmetic.
+AOTO_DEVICE double exp2_added(double d, double heat32, const VerifyTable& table, double sum) {
+  const VerifyPower p = exp2_parts(d, heat32);
+  const double scale = table.at[p.k & 31];
+  return fma(p.series, __hiloint2double(__double2hiint(scale) + ((p.k >> 5) << 20), __double2loint(scale)), sum);
 }
 
 // A request's temperature: 32 log2(e) / T and its inverse; heat32 < 0: greedy.
@@ -69,10 +86,10 @@ struct VerifyHeat {
   double heat32, cool;
   AOTO_DEVICE bool greedy() const { return heat32 < 0.0; }
 };
-AOTO_DEVICE VerifyHeat verify_heat(const VerifyArgs& a, int r) {
-  const float t = a.temperature ? a.temperature[r] : 0.f;
+AOTO_DEVICE float verify_temperature(const VerifyArgs& a, int r) { return a.temperature ? a.temperature[r] : 0.f; }
+AOTO_DEVICE VerifyHeat verify_heat(float t) {
   if (!(t > 0.f)) return {-1.0, 0.0};
-  return {46.166241308446828384 / (double)t, (double)t / 46.166241308446828384};
+  return {46.166241308446828384 / (double)t, (double)t * (1.0 / 46.166241308446828384)};
 }
 
 // The weights exp((z - top) / T) of a row's tokens. A NaN or -inf weighs 0; the logits equal to an infinite top weigh 1
@@ -89,8 +106,11 @@ struct VerifyScale {
     const double reach = (top - (double)floor) * heat32;
     plain = fabsf(t) < INFINITY && reach >= 0.95 * 32.0 * below && reach <= 1.02 * 32.0 * below;
   }
-  AOTO_DEVICE double operator()(float z) const {
-    if (plain) return exp2_of((double)fmaxf(z, floor) - top, heat32, table);  // fmaxf: a NaN gives the floor
+  AOTO_DEVICE double operator()(float z) const { return plain ? quick(z) : careful(z); }
+  AOTO_DEVICE double quick(float z) const {
+    return exp2_of((double)fmaxf(z, floor) - top, heat32, table);  // fmaxf: a NaN gives the floor
+  }
+  AOTO_DEVICE double careful(float z) const {
     if (!(z > -INFINITY)) return 0.0;
     if ((double)z == top) return 1.0;
     return top == INFINITY ? 0.0 : exp2_of(fmax(((double)z - top) * heat32, -64000.0), 1.0, table);
@@ -192,11 +212,8 @@ __device__ void verify_stats(const VerifyArgs& a) {
   int first, count;
   verify_rows(a, r, first, count);
   const bool draft = i > a.drafts;
-  const VerifyHeat heat = verify_heat(a, r);
-  if (draft ? (a.draft_logits == nullptr || i - a.drafts - 1 >= count || heat.greedy()) : i > count) return;
-  verify_table(table);
-  __syncthreads();
-  if (chunk >= a.chunks) return;
+  const float temperature = verify_temperature(a, r);
+  if (draft ? (a.draft_logits == nullptr || i - a.drafts - 1 >= count || !(temperature > 0.f)) : i > count) return;
   const void* row = draft ? verify_row<F32>(a.draft_logits, r * a.draft_request_stride +
                                                                 (i - a.drafts - 1) * a.draft_row_stride)
                           : verify_row<F32>(a.logits, (first + i) * a.row_stride);
@@ -227,6 +244,13 @@ __device__ void verify_stats(const VerifyArgs& a) {
         held.raw[l] = make_uint4(w[0], w[1], w[2], w[3]);
       }
   }
+  // while the loads are on their way
+  const VerifyHeat heat = verify_heat(temperature);
+  if (!heat.greedy()) {
+    verify_table(table);
+    __syncthreads();
+  }
+  if (chunk >= a.chunks) return;  // it held nothing
   float top = -INFINITY;
   int place = begin;
   double sum = 0.0;
@@ -259,7 +283,7 @@ __device__ void verify_stats(const VerifyArgs& a) {
         held.get(l, z);
 #pragma unroll
         for (int e = 0; e < Held::EACH; ++e)
-          sum += exp2_of<true>((double)fmaxf(z[e], weight.floor) - weight.top, heat.heat32, table);
+          sum = exp2_added((double)fmaxf(z[e], weight.floor) - weight.top, heat.heat32, table, sum);
       }
     } else if (top > -INFINITY) {
 #pragma unroll
@@ -317,7 +341,7 @@ AOTO_DEVICE VerifyLaw verify_law(const VerifyArgs& a, int r, VerifyTable& table)
   }
   int first, count;
   verify_rows(a, r, first, count);
-  const VerifyHeat heat = verify_heat(a, r);
+  const VerifyHeat heat = verify_heat(verify_temperature(a, r));
   const bool sampled = !heat.greedy(), laws = a.draft_logits && sampled;
   const bool known = (int)threadIdx.x < count && x >= 0 && x < a.vocab;
   float zx = -INFINITY, yx = -INFINITY;
@@ -335,7 +359,7 @@ AOTO_DEVICE VerifyLaw verify_law(const VerifyArgs& a, int r, VerifyTable& table)
     const int j = j0 + (threadIdx.x >> 4);
     const bool live = j < rows;
     const VerifyChunk* from = chunks + (size_t)(j <= count ? j : a.drafts + j - count) * a.chunks;
-    constexpr int SOME = 3;  // a lane's chunks that are loaded at once: 196608 tokens
+    constexpr int SOME = 5;  // a lane's chunks that are loaded at once: 163840 tokens
     VerifyChunk mine[SOME];
 #pragma unroll
     for (int k = 0; k < SOME; ++k) {
@@ -409,6 +433,26 @@ AOTO_DEVICE VerifyLaw verify_law(const VerifyArgs& a, int r, VerifyTable& table)
   return s_law;
 }
 
+// The weights of eight logits, 0 from the `count`th on. (What is not plain is rare and kept out of the way.)
+AOTO_DEVICE void verify_weights(const VerifyScale& weight, const float (&z)[8], int count, double (&w)[8]) {
+  if (weight.plain) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = weight.quick(z[i]);
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      float x = z[0];
+#pragma unroll
+      for (int k = 1; k < 8; ++k) x = i == k ? z[k] : x;
+      const double one = weight.careful(x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = i == k ? one : w[k];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = i < count ? w[i] : 0.0;
+}
+
 // The weights of tokens v .. v + 7 under the target's law and what is left of them.
 template <bool F32>
 AOTO_DEVICE void verify_left(const VerifyLaw& law, const VerifyTable& table, int v, int end, double (&whole)[8],
@@ -417,18 +461,16 @@ AOTO_DEVICE void verify_left(const VerifyLaw& law, const VerifyTable& table, int
   float z[8], y[8];
   verify_load<F32>(law.row, v, end, z);
   if (minus) verify_load<F32>(law.draft_row, v, end, y);
-  const VerifyScale weight(law.top, law.heat, table);
+  verify_weights(VerifyScale(law.top, law.heat, table), z, law.sum > 0.0 ? end - v : 0, whole);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    whole[i] = law.sum > 0.0 && v + i < end ? weight(z[i]) : 0.0;
-    left[i] = v + i == law.removed ? 0.0 : whole[i];
-  }
+  for (int i = 0; i < 8; ++i) left[i] = v + i == law.removed ? 0.0 : whole[i];
   if (minus) {
     // p - q, times the target's sum
     const double ratio = law.sum / law.draft_sum;
-    const VerifyScale other(law.draft_top, law.heat, table);
+    double other[8];
+    verify_weights(VerifyScale(law.draft_top, law.heat, table), y, end - v, other);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) left[i] = v + i < end ? fmax(whole[i] - ratio * other(y[i]), 0.0) : 0.0;
+    for (int i = 0; i < 8; ++i) left[i] = fmax(whole[i] - ratio * other[i], 0.0);
   }
 }
 
@@ -440,8 +482,8 @@ AOTO_DEVICE VerifyLaw* verify_laws(const VerifyArgs& a) {
   return reinterpret_cast<VerifyLaw*>(verify_masses(a, a.requests));
 }
 
-// Block r: the request's law, for the two launches behind it (every chunk's block finding it anew cost more: 64
-// requests' sums 21 us, against 5 and 10).
+// Block r: the request's law, for the two launches behind it (every chunk's block finding it anew cost more: the sums
+// of 64 requests took 21 us, against 5 for this launch and 10).
 template <bool F32>
 __device__ void verify_keep(const VerifyArgs& a) {
   __shared__ VerifyTable table;
@@ -475,12 +517,12 @@ __device__ void verify_mass(const VerifyArgs& a) {
   if (threadIdx.x == 0) verify_masses(a, r)[blockIdx.x] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
 }
 
-// Block r, 512 threads: the chunk in which the running sum passes, then the token in it, eight a thread. KEPT: the law
+// Block r: the chunk in which the running sum passes, then the token in it, eight a thread. KEPT: the law
 // and the sums of subtracted laws are there already.
 template <bool F32, bool KEPT>
 __device__ void verify_pick(const VerifyArgs& a) {
-  static_assert(kVerifyChunk == 8 * 512, "a chunk is eight tokens a thread");
-  __shared__ double s_sum[8], s_before, s_target;
+  static_assert(kVerifyChunk == 8 * kVerifyPick, "a chunk is eight tokens a thread");
+  __shared__ double s_sum[kVerifyPick / 64], s_before, s_target;
   __shared__ int s_chunk, s_whole, s_token, s_last;
   const int r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   __shared__ VerifyTable table;
@@ -491,7 +533,7 @@ __device__ void verify_pick(const VerifyArgs& a) {
     verify_table(table);
     __syncthreads();
   } else {
-    law = verify_law<F32, 512>(a, r, table);
+    law = verify_law<F32, kVerifyPick>(a, r, table);
   }
   long long token = law.place;
   if (law.count >= 0 && !law.heat.greedy()) {
@@ -567,7 +609,7 @@ __device__ void verify_pick(const VerifyArgs& a) {
     if (s_token != 0x7FFFFFFF) token = s_token;
     else if (s_last >= 0) token = s_last;
   }
-  for (int i = threadIdx.x; i <= a.drafts; i += 512) {
+  for (int i = threadIdx.x; i <= a.drafts; i += kVerifyPick) {
     long long out = -1;
     if (law.count >= 0 && i < law.accepted) out = a.draft_tokens[(size_t)r * a.drafts + i];
     if (law.count >= 0 && i == law.accepted) out = token;
@@ -578,19 +620,19 @@ __device__ void verify_pick(const VerifyArgs& a) {
 
 }  // namespace aoto
 
-#define AOTO_VERIFY_INSTANCE(NAME, F32)                                                                  \
-  extern "C" __global__ __launch_bounds__(256) void aoto_verify_stats_##NAME(VerifyArgs a) {             \
-    aoto::verify_stats<F32>(a);                                                                          \
-  }                                                                                                      \
-  extern "C" __global__ __launch_bounds__(256) void aoto_verify_law_##NAME(VerifyArgs a) {               \
-    aoto::verify_keep<F32>(a);                                                                           \
-  }                                                                                                      \
-  extern "C" __global__ __launch_bounds__(256) void aoto_verify_mass_##NAME(VerifyArgs a) {              \
-    aoto::verify_mass<F32>(a);                                                                           \
-  }                                                                                                      \
-  extern "C" __global__ __launch_bounds__(512) void aoto_verify_pick_##NAME(VerifyArgs a) {             \
-    aoto::verify_pick<F32, true>(a);                                                                     \
-  }                                                                                                      \
-  extern "C" __global__ __launch_bounds__(512) void aoto_verify_follow_##NAME(VerifyArgs a) {           \
-    aoto::verify_pick<F32, false>(a);                                                                    \
+#define AOTO_VERIFY_INSTANCE(NAME, F32)                                                                    \
+  extern "C" __global__ __launch_bounds__(256) void aoto_verify_stats_##NAME(VerifyArgs a) {               \
+    aoto::verify_stats<F32>(a);                                                                            \
+  }                                                                                                        \
+  extern "C" __global__ __launch_bounds__(256) void aoto_verify_law_##NAME(VerifyArgs a) {                 \
+    aoto::verify_keep<F32>(a);                                                                             \
+  }                                                                                                        \
+  extern "C" __global__ __launch_bounds__(256) void aoto_verify_mass_##NAME(VerifyArgs a) {                \
+    aoto::verify_mass<F32>(a);                                                                             \
+  }                                                                                                        \
+  extern "C" __global__ __launch_bounds__(aoto::kVerifyPick) void aoto_verify_pick_##NAME(VerifyArgs a) {  \
+    aoto::verify_pick<F32, true>(a);                                                                       \
+  }                                                                                                        \
+  extern "C" __global__ __launch_bounds__(aoto::kVerifyPick) void aoto_verify_follow_##NAME(VerifyArgs a) {\
+    aoto::verify_pick<F32, false>(a);                                                                      \
   }

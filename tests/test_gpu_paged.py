@@ -536,7 +536,7 @@ def _check_verify(start, logits, host, tokens, law, law_host, uniforms, temperat
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("vocab", [1, 2, 255, 1000, 8191, 8192, 8193, 50001])
+@pytest.mark.parametrize("vocab", [1, 2, 255, 1000, 2047, 2049, 8191, 8192, 8193, 50001, 200003])
 @pytest.mark.parametrize("with_law", [False, True])
 def test_verify_of_ragged_drafts(dtype, vocab, with_law):
     rng = np.random.default_rng(vocab)
