@@ -192,7 +192,7 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
   a.narrow_tokens = plan.narrow_rows / (query_heads / kv_heads);
   a.wide_tokens = plan.wide_rows / (query_heads / kv_heads);
   a.target = plan.target, a.least_blocks = 2;
-  a.record_rows = plan.wide_rows ? plan.wide_rows : plan.narrow_rows;
+  a.record_rows = plan.wide_rows ? plan.wide_rows : plan.narrow_rows, a.units = (int)std::min(plan.units, 0x3FFFFFFFLL);
   a.joins = static_cast<int*>(workspace);
   a.records = reinterpret_cast<float*>(static_cast<char*>(workspace) + (size_t)tokens * 16);
   char name[64];

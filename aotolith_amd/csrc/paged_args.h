@@ -58,6 +58,7 @@ struct PagedAttentionArgs {
   int target;          // GPU blocks a kv head among which the key blocks (128 keys) are dealt; 0: one a tile
   int least_blocks;    // key blocks that make a GPU block worth its while
   int record_rows;     // rows of a record
+  int units;           // records a kv head that the workspace holds
   float scale;
 };
 

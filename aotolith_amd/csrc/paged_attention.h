@@ -193,6 +193,8 @@ struct PagedWalk {
       // the GPU blocks that hold the item's first and last key block
       const int head = owner(place), tail = owner(place + n - 1);
       unit.record = head + item, unit.part = block - head, unit.parts = tail - head + 1;
+      // only where query_start decreases and requests share rows: more tiles than rows make
+      if (unit.record < 0 || unit.part < 0 || unit.record > a.units - unit.parts) return false;
     } else {
       left = 0;
     }
@@ -1071,7 +1073,9 @@ __device__ void paged_attention_join(const PagedAttentionArgs& a) {
   const int t = row / a.query_heads, h = row % a.query_heads;
   if (t >= a.tokens) return;
   const int4 note = reinterpret_cast<const int4*>(a.joins)[t];
-  if (t >= a.query_start[a.requests] || note.y <= 1) return;
+  if (t < a.query_start[0] || t >= a.query_start[a.requests] || note.y <= 1) return;
+  // no note where query_start decreases
+  if (note.x < 0 || note.y > a.units || note.x > a.units - note.y || (unsigned)note.z >= (unsigned)a.record_rows) return;
   const int group = a.query_heads / a.kv_heads, kvh = h / group, at = note.z + h % group;
   const size_t step = (size_t)a.kv_heads * a.record_rows * (D + 2);
   const float* rec = paged_record(a, note.x, kvh, at, D);
@@ -1121,7 +1125,8 @@ __device__ void paged_attention_join(const PagedAttentionArgs& a) {
   extern "C" __global__ __launch_bounds__(256, 2) void aoto_paged_attention_d##D##_n2(PagedAttentionArgs a) {      \
     aoto::paged_attention_narrow<D, 2>(a);                                                                         \
   }                                                                                                                \
-  extern "C" __global__ __launch_bounds__(256, 128 / D) void aoto_paged_attention_d##D##_w128(PagedAttentionArgs a) {            \
+  extern "C" __global__ __launch_bounds__(256, 128 / D)                                                            \
+  void aoto_paged_attention_d##D##_w128(PagedAttentionArgs a) {                                                    \
     aoto::paged_attention_mixed<D, 1>(a);                                                                          \
   }                                                                                                                \
   extern "C" __global__ __launch_bounds__(256) void aoto_paged_attention_join_d##D(PagedAttentionArgs a) {         \

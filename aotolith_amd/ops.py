@@ -1429,9 +1429,11 @@ def paged_attention(
     (int32 ``[R]``), its own new ones among them, in the pages that ``block_tables[r]`` (int32 ``[R, max_blocks]``)
     names: one token, a few drafted ones or a chunk of a prompt, side by side. Row ``i`` of ``n`` sees the keys up to
     its own, ``j <= kv_lens[r] - n + i`` (all of them with ``causal=False``); keys past the block table row or in
-    entries that name no page are not there, and a row that sees none gives 0. Rows from ``query_start[R]`` on keep
-    what ``out`` held. The lengths are read on the GPU; ``max_query_len`` and ``max_kv_len`` (0: not known) are the
-    caller's bounds on a request's rows and keys, which choose the launch and never the result.
+    entries that name no page are not there, and a row that sees none gives 0. Rows before ``query_start[0]`` and from
+    ``query_start[R]`` on keep what ``out`` held. The lengths are read on the GPU; ``max_query_len`` and ``max_kv_len``
+    (0: not known) are the caller's bounds on a request's rows and keys, which choose the launch and never the result.
+    ``workspace`` (:func:`paged_attention_workspace`; allocated where it is missing or too small) is written by the
+    call: calls that share one are ordered on one stream.
     """
 
     _expect_rows(q, "q", BF16, 3, q.get_device() if isinstance(q, torch.Tensor) else 0)

@@ -614,7 +614,8 @@ int aoto_hip_generic_attention(const aoto_tensor* out, const aoto_tensor* q, con
  *   free_start_out   free_start + the pages taken
  *   positions, slots int64 [max_tokens]: token i of request r has position context_lens[r] + i and the slot
  *                    block_tables[r][position / page] * page + position % page; 0 and -1 behind the last token
- * page_counts_out and free_start_out may be the arrays they are computed from. */
+ * page_counts_out and free_start_out may be the arrays they are computed from. At most 2^20 blocks a request, 2^20
+ * tokens a page, 2^30 - 1 rows. */
 int aoto_hip_paged_tables(const int32_t* context_lens, const int32_t* new_lens, int32_t* block_tables,
                           int64_t table_stride, const int32_t* page_counts, const int32_t* free_pages,
                           const int32_t* free_start, int requests, int max_blocks, int free_count, int page,
@@ -633,11 +634,13 @@ int aoto_hip_paged_rope_append(const void* qkv, int64_t row_stride, const int64_
                                void* stream);
 
 /* Attention of the requests' new tokens over their pages: request r's rows are query_start[r] .. query_start[r + 1]
- * of q (strides in elements, multiples of 8) and of out [tokens, Hq * head_dim]; row i of n sees the keys
- * j < kv_lens[r] - n + i + 1 (causal) or j < kv_lens[r], as far as its block table reaches and names pages of the
- * cache. A row that sees none gives 0; rows from query_start[requests] on keep what they held. head_dim 64 or 128.
- * max_query_len and max_kv_len (0: not known) are the caller's bounds on a request's rows and keys; they choose the
- * launch and never the result. workspace: aoto_hip_paged_attention_workspace() bytes for the same arguments. */
+ * of q (strides in elements, multiples of 8) and of out [tokens, Hq * head_dim], query_start not decreasing; row i of
+ * n sees the keys j < kv_lens[r] - n + i + 1 (causal) or j < kv_lens[r], as far as its block table reaches and names
+ * pages of the cache. A row that sees none gives 0; rows before query_start[0] and from query_start[requests] on keep
+ * what they held. max_query_len and max_kv_len (0: not known) are the caller's bounds on a request's rows and keys;
+ * they choose the launch and never the result. workspace: aoto_hip_paged_attention_workspace() bytes for the same
+ * arguments (0: none needed). head_dim 64 or 128, at most 128 query heads a kv head, block tables of at most 2^28
+ * keys (max_blocks * page), page_stride below 2^32, slot_stride * page below 2^30, scale positive and finite. */
 size_t aoto_hip_paged_attention_workspace(int tokens, int requests, int max_blocks, int page, int query_heads,
                                           int kv_heads, int head_dim, int max_query_len, int max_kv_len);
 int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* keys,
@@ -657,9 +660,12 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
  * from the last row's p: the first token whose running sum of weights is above u times their total. T =
  * temperature[r]; where it is not above 0, and everywhere with temperature NULL, a draft stands where it is the row's
  * first maximum, which is also the token that follows. NaN logits count as -inf; a row of nothing else judges no
- * draft true and is followed by token 0; the logits equal to an infinite maximum share its law. Sums and exponentials in f64.
+ * draft true and is followed by token 0; the logits equal to an infinite maximum share its law. Sums and
+ * exponentials in f64.
  * tokens_out int64 [requests, drafts + 1]: the drafts that stand, the token that follows, -1 behind it (-1 throughout
- * for a request without rows); accepted int32 [requests]: how many stand. */
+ * for a request without rows); accepted int32 [requests]: how many stand. vocab at most 2^30; requests * (drafts + 1),
+ * with temperature and draft_logits requests * (2 * drafts + 1), at most 65535. workspace:
+ * aoto_hip_verify_draft_workspace() bytes, 8-byte aligned. */
 size_t aoto_hip_verify_draft_workspace(int requests, int drafts, int vocab);
 int aoto_hip_verify_draft(const void* logits, int logits_f32, int64_t row_stride, int rows, int vocab,
                           const int64_t* draft_tokens, const void* draft_logits, int64_t draft_request_stride,

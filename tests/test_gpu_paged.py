@@ -332,6 +332,18 @@ def test_attention_without_keys_gives_zero(rows):
 
 
 @pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("keys", [60, 3000])  # whole items, items that are cut and joined
+def test_attention_leaves_rows_before_the_first_request(rows, keys):
+    rng = np.random.default_rng(17)
+    s = _requests(rng, [(rows, keys), (rows, 40)], 8, 2, 64, 16)
+    s["q"] = np.concatenate([bf16_normal(rng, (5, 8, 64)), s["q"]])
+    s["start"] = s["start"] + 5
+    got = _attend(s, max_query_len=rows, max_kv_len=keys)
+    assert bool((got[:5] == 5.0).all())
+    _check_attention(s, got)
+
+
+@pytest.mark.parametrize("rows", [1, 20])
 def test_attention_leaves_out_entries_that_name_no_page(rows):
     rng = np.random.default_rng(9)
     s = _requests(rng, [(rows, 400), (rows, 300)], 8, 2, 128, 16)

@@ -87,7 +87,7 @@ def _verify(**changes):
 @pytest.mark.parametrize("changes,code", [
     (dict(logits=None), 1), (dict(drafts_in=None), 1), (dict(start=None), 1), (dict(uniforms=None), 1),
     (dict(workspace=None), 1), (dict(out=None), 1), (dict(accepted=None), 1), (dict(rows=0), 1), (dict(vocab=0), 1),
-    (dict(requests=0), 1), (dict(drafts=-1), 1), (dict(drafts=63), 4), (dict(logits=ctypes.c_void_p(4097)), 1),
+    (dict(requests=0), 1), (dict(drafts=-1), 1), (dict(drafts=63), 4), (dict(vocab=2 ** 30 + 1), 4), (dict(logits=ctypes.c_void_p(4097)), 1),
     (dict(f32=1, logits=ctypes.c_void_p(4098)), 1), (dict(law=ctypes.c_void_p(4097)), 1)])
 def test_verify_refuses(changes, code):
     _refused(_verify(**changes), code, "verify_draft")
