@@ -229,7 +229,6 @@ AOTO_GENERIC_ATTENTION(f32, true, 128, a, false)
 // Attention over a paged cache: head dim x {narrow tiles of 16 and 32 rows, wide tiles beside narrow ones, join}.
 AOTO_PAGED_ATTENTION(64)
 AOTO_PAGED_ATTENTION(128)
-AOTO_PAGED_ATTENTION_WHOLE(128)
 
 // Verification of drafted tokens: {logits' type} x {statistics, masses, pick}.
 AOTO_VERIFY_INSTANCE(bf16, false)

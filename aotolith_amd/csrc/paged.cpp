@@ -33,7 +33,7 @@ int check_pages(const char* what, const void* keys, const void* values, int64_t 
 }
 
 // Rows of a wide tile of the attention.
-constexpr int kWideRows = 256, kHalfRows = 128;
+constexpr int kWideRows = 128;
 
 struct AttentionPlan {
   int wide_rows;      // of a wide tile, 0 where no chunk of a prompt is among the requests: the narrow instances
@@ -52,25 +52,17 @@ AttentionPlan attention_plan(int tokens, int requests, int max_blocks, int page,
   auto tiles = [&](int of) { return some + (tokens - some) / std::max(of / group, 1); };
   AttentionPlan p{};
   p.narrow_rows = rows <= 16 || rows > 32 ? 16 : 32;
-  // GPU blocks that the chip holds at a time: two narrow ones on a CU; one with wide tiles (registers; LDS at 128 dims),
-  // two with half as many rows at 64 dims.
-  long long full = 2LL * cus;
-  p.units = tiles(p.narrow_rows);
-  if (rows > 32) {
-    // Half as many rows where whole ones would leave half of the chip idle (32 / 8 heads of 128, 1024 rows: over 1024
-    // keys 40 us against 60, over 5000 126 against 129; 2048 rows over 8048 keys 346 against 292), and at 64 dims
-    // always: two blocks fit a CU there (14 / 2 heads, 4096 rows over 4097 / 10096 keys: 80 / 200 us against 105 / 243).
-    const bool half = head_dim == 64 || 2 * tiles(kWideRows) * kv_heads <= cus;
-    p.wide_rows = half ? kHalfRows : kWideRows;
-    full = head_dim == 64 ? 2LL * cus : cus;
-    p.units = tiles(p.wide_rows);
-  }
+  p.wide_rows = rows > 32 ? kWideRows : 0;
+  p.units = tiles(p.wide_rows ? p.wide_rows : p.narrow_rows);
+  const long long full = 2LL * cus;  // GPU blocks that the chip holds at a time
   long long keys = std::min<long long>((long long)max_blocks * page, 1 << 28);
   const long long most = keys / 128 + 8;  // key blocks of a tile
   if (max_kv_len) keys = std::min<long long>(keys, max_kv_len);
   // Not worth the join: narrow tiles of up to 256 keys, wide ones of up to 1024 (512 tokens over themselves: 28 us
-  // whole and 35 cut at 128 dims, 19.5 and 24 at 64).
-  if (keys > (p.wide_rows ? 1024 : 256) && p.units * kv_heads < (p.wide_rows ? 1 : 4) * full && p.units * most < (1 << 30)) {
+  // whole and 35 cut at 128 dims, 19.5 and 24 at 64), wide ones that give every CU a block (32 / 8 heads of 128, 1024
+  // tokens over 1 / 1000 / 4000 keys before them: 41 / 62 / 127 us whole, 56 / 76 / 128 cut).
+  if (keys > (p.wide_rows ? 1024 : 256) && 2 * p.units * kv_heads < (p.wide_rows ? 1 : 8) * full &&
+      p.units * most < (1 << 30)) {
     p.target = (int)((full + kv_heads - 1) / kv_heads);
     p.units += p.target;
     p.workspace = (size_t)tokens * 16 + (size_t)p.units * kv_heads * (p.wide_rows ? p.wide_rows : p.narrow_rows) *
@@ -170,9 +162,9 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention: pages of more than 2^32 elements, or rows 2^30 apart");
   if (!(scale > 0.f) || !std::isfinite(scale))
     return set_error(AOTO_ERR_ARGUMENT, "paged_attention: scale %g is not a positive number", (double)scale);
-  if (query_heads / kv_heads > kHalfRows)
+  if (query_heads / kv_heads > kWideRows)
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention: %d query heads a kv head (at most %d)",
-                     query_heads / kv_heads, kHalfRows);
+                     query_heads / kv_heads, kWideRows);
   const AttentionPlan plan = attention_plan(tokens, requests, max_blocks, page, query_heads, kv_heads, head_dim,
                                             max_query_len, max_kv_len);
   if (plan.workspace && (!workspace || !aligned(workspace, 16)))
@@ -197,7 +189,7 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
   a.records = reinterpret_cast<float*>(static_cast<char*>(workspace) + (size_t)tokens * 16);
   char name[64];
   snprintf(name, sizeof(name), "aoto_paged_attention_d%d_%s", head_dim,
-           plan.wide_rows == kWideRows ? "w256" : plan.wide_rows ? "w128" : plan.narrow_rows == 16 ? "n1" : "n2");
+           plan.wide_rows ? "w" : plan.narrow_rows == 16 ? "n1" : "n2");
   if (int s = launch(name, (plan.target ? plan.target : plan.units) * kv_heads, 1, 256, stream, a)) return s;
   if (!plan.target) return AOTO_OK;
   return launch(head_dim == 64 ? "aoto_paged_attention_join_d64" : "aoto_paged_attention_join_d128",

@@ -17,8 +17,8 @@
 // requests.
 //   narrow tiles (16 NT rows, decodes and drafted tokens): the four waves take 32 keys each of every 128; K goes
 //     straight from the pages to operand registers, V through the wave's own LDS; no barrier in the loop
-//   wide tiles (128 or 256 rows, chunks of prompts): the four waves take 32 or 64 rows each, 64-key tiles of K and V
-//     staged once for all of them
+//   wide tiles (128 rows, chunks of prompts): the four waves take 32 rows each, 64-key tiles of K and V staged once for
+//     all of them
 #pragma once
 
 #include "common.h"
@@ -531,7 +531,7 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
 // ------------------------------------------------------------------------------------------------------ wide tiles
 template <int D>
 struct PagedWideShared {
-  uint16_t k[3][64 * D];
+  uint16_t k[5][32 * D];  // halves of tiles: tile t's are slots 2 t and 2 t + 1, mod 5
   uint16_t v[2][64 * D];
   uint32_t exist[4][4];  // by tile (mod 4) and staging wave: which of its 16 rows exist (a page, and not past the end)
   uint32_t known[4][4];  // and which have a page
@@ -572,21 +572,25 @@ AOTO_DEVICE void acc_settle() {
 }
 
 // v_mfma_f32_32x32x16_bf16: S^T [32 keys x 32 rows] = K . Q^T, O^T [32 d x 32 rows] += V^T . P^T (layouts and slot
-// order as in the prefill attention). A wave has 32 C rows. With C = 2 each K and V operand read from LDS serves two
-// products, which halves the traffic that otherwise asks for all of the LDS's 128 bytes a cycle at the products' full
-// rate. One wave runs on a SIMD, with 512 registers, and what it issues between two products is free as long as it
-// takes no longer than they do; so a step holds, in this order and spread out between its products, the scores of the
-// next 32 keys (with three quarters of the present keys' exponentials) and the product of the present keys' weights with
-// V (with the other exponentials, the next scores out of their accumulators and their maximum). Operands are read from LDS two
-// products ahead. K and V go from memory to LDS without registers, K two tiles ahead and V one; the 16-byte pieces of a
-// row are permuted by a function of the row (the lanes fetch them so) that spreads each phase of the reads over all
-// banks. Rows' addresses advance by 64 keys a tile without a division or a product but the page's.
-template <int D, int C>
+// order as in the prefill attention). A wave has 32 rows; two waves, of two blocks, share a SIMD and its 512 registers.
+// A step holds, in this order and spread out between its products, the scores of the next 32 keys (with three quarters
+// of the present keys' exponentials) and the product of the present keys' weights with V (with the other exponentials,
+// the next scores out of their accumulators and their maximum). Operands are read from LDS two products ahead. K and V
+// go from memory to LDS without registers, K up to two tiles ahead and V one; K in five slots of half a tile, so that
+// two blocks' tiles fit the LDS. The 16-byte pieces of a row are permuted by a function of the row (the lanes fetch
+// them so) that spreads each phase of the reads over all banks. Rows' addresses advance by 64 keys a tile without a
+// division or a product but the page's.
+//
+// Bound by what a wave issues and waits for between its products: 2048 rows over 8048 keys, 32 / 8 heads of 128, run at
+// 0.83 PFLOP/s in 283 us, the matrix units busy for 37% of it and the vector units for 60%. One wave a SIMD with 64
+// rows, half the reads from LDS and 512 registers took 297 us there, and from 96 us (77 here) to 61 (41) for 2048 and
+// 1024 rows over themselves, where its tiles are too few for the chip.
+template <int D>
 AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, int kvh, PagedWideShared<D>& s) {
   constexpr int DS = D / 16, DT = D / 32, LPR = D / 8;  // lanes (16-byte pieces) a row
   constexpr int RPL = 64 / LPR;                         // rows a wave's load covers
   constexpr int LOADS = 16 / RPL;                       // loads of K (and V) a thread does for a 64-key tile
-  constexpr int ROWB = 2 * D, TILEB = 64 * ROWB;
+  constexpr int ROWB = 2 * D, HALFB = 32 * ROWB, TILEB = 64 * ROWB;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int group = a.query_heads / a.kv_heads;
@@ -594,18 +598,15 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   const int* table = a.block_tables + unit.request * a.table_stride;
   const int k0 = unit.from * kPagedUnitKeys, k1 = min(unit.keys, unit.to * kPagedUnitKeys);
   const int tiles = k1 > k0 ? (k1 - k0 + 63) / 64 : 0;
-  const bool active = 32 * C * wave < live;  // a wave of none of the rows only stages
+  const bool active = 32 * wave < live;  // a wave of none of the rows only stages
 
-  fa_bf16x8 qf[C][DS];
-  int limit[C];
+  // this lane's row: its token of the request and head of the group, and the keys it sees
+  const int row = 32 * wave + col, token = unit.token + min(row, live - 1) / group, head = min(row, live - 1) % group;
+  const uint16_t* q = a.q + (unit.begin + token) * a.q_token_stride + (kvh * group + head) * a.q_head_stride + 8 * half;
+  fa_bf16x8 qf[DS];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int row = min(32 * C * wave + 32 * c + col, live - 1), i = unit.token + row / group, g = row % group;
-    const uint16_t* q = a.q + (unit.begin + i) * a.q_token_stride + (kvh * group + g) * a.q_head_stride + 8 * half;
-#pragma unroll
-    for (int d = 0; d < DS; ++d) qf[c][d] = *reinterpret_cast<const fa_bf16x8*>(q + 16 * d);
-    limit[c] = min(k1, unit.first + i);
-  }
+  for (int d = 0; d < DS; ++d) qf[d] = *reinterpret_cast<const fa_bf16x8*>(q + 16 * d);
+  const int limit = min(k1, unit.first + token);
   const int least = min(k1, unit.first + unit.token);  // keys that every row of the block sees
   const float c2 = a.scale * 1.4426950408889634f;
 
@@ -616,50 +617,58 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   const int piece = 8 * ((lane % LPR) ^ swizzle(stage_row));
   const uint16_t* keys = a.keys + kvh * a.head_stride + piece;
   const uint16_t* values = a.values + kvh * a.head_stride + piece;
-  const int last_block = paged_block(a, max(k1 - 1, 0));
-  const int page_span = a.page * (int)a.slot_stride;
-  const int step_blocks = paged_block(a, 64), step_off = (64 - step_blocks * a.page) * (int)a.slot_stride;
-  // of the tile looked up next: the rows' table entries and offsets in their pages; of one looked up, pages and offsets
-  struct Rows {
-    int page[LOADS], off[LOADS];
-  };
-  int block[LOADS], off[LOADS];
-  Rows ahead;
+  const uint32_t last_entry = 4 * paged_block(a, max(k1 - 1, 0));
+  const uint32_t page_span = a.page * (uint32_t)a.slot_stride;
+  const int step_blocks = paged_block(a, 64);
+  const uint32_t step_off = (64 - step_blocks * a.page) * (uint32_t)a.slot_stride;
+  // of the tile looked up last: the rows' table entries (bytes in the table), their offsets in their pages, the pages
+  uint32_t entry[LOADS], off[LOADS];
+  int ahead[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
-    const int key = k0 + 4 * RPL * i + stage_row;
-    block[i] = paged_block(a, key);
-    off[i] = (key - block[i] * a.page) * (int)a.slot_stride;
+    const int key = k0 + 4 * RPL * i + stage_row, block = paged_block(a, key);
+    entry[i] = 4 * block;
+    off[i] = (key - block * a.page) * (uint32_t)a.slot_stride;
   }
-  auto look_row = [&](int i, Rows& to) __attribute__((always_inline)) {
-    to.page[i] = table[min(block[i], last_block)];
-    to.off[i] = off[i];
-    off[i] += step_off;
-    const bool over = off[i] >= page_span;
-    off[i] -= over ? page_span : 0;
-    block[i] += step_blocks + (over ? 1 : 0);
+  auto look_row = [&](int i, int (&page)[LOADS]) __attribute__((always_inline)) {
+    page[i] = *reinterpret_cast<const int*>(reinterpret_cast<const char*>(table) + min(entry[i], last_entry));
   };
-  auto look = [&](Rows& to) __attribute__((always_inline)) {
+  auto look = [&](int (&page)[LOADS]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) look_row(i, to);
+    for (int i = 0; i < LOADS; ++i) look_row(i, page);
   };
-  auto place = [&](int tile, const Rows& of, long long (&at)[LOADS]) __attribute__((always_inline)) {
-    bool fine = true;
-    bool there[LOADS], page[LOADS];
+  // to the next tile's entries and offsets
+  auto advance = [&] {
+    if (step_off == 0) {  // whole pages a tile
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) entry[i] += 4 * step_blocks;
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const bool known = (unsigned)of.page[i] < (unsigned)a.pages;
-      at[i] = (long long)((unsigned long long)(unsigned)(known ? of.page[i] : 0) * (unsigned)a.page_stride) + of.off[i];
-      there[i] = known && k0 + 64 * tile + 4 * RPL * i + stage_row < k1;
-      page[i] = known;
-      fine = fine && there[i];
+      off[i] += step_off;
+      const bool over = off[i] >= page_span;
+      off[i] -= over ? page_span : 0;
+      entry[i] += 4 * (step_blocks + (over ? 1 : 0));
+    }
+  };
+  auto place = [&](int tile, const int (&page)[LOADS], const uint32_t (&row)[LOADS], long long (&at)[LOADS])
+      __attribute__((always_inline)) {
+    uint32_t most = page[0];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      most = max(most, (uint32_t)page[i]);
+      at[i] = (long long)((unsigned long long)(unsigned)page[i] * (unsigned)a.page_stride + row[i]);
     }
     uint32_t exist = 0xFFFFu, paged = 0xFFFFu;
-    if (!__all(fine)) {
+    if (k0 + 64 * tile + 64 > k1 || __any(most >= (unsigned)a.pages)) {
       exist = paged = 0;
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const unsigned long long lanes = __ballot(there[i]), pages = __ballot(page[i]);
+        const bool known = (unsigned)page[i] < (unsigned)a.pages;
+        if (!known) at[i] = row[i];  // of page 0, and not looked at
+        const unsigned long long pages = __ballot(known);
+        const unsigned long long lanes = __ballot(known && k0 + 64 * tile + 4 * RPL * i + stage_row < k1);
 #pragma unroll
         for (int j = 0; j < RPL; ++j) {
           exist |= (uint32_t)(lanes >> (j * LPR) & 1) << (i * RPL + j);
@@ -670,21 +679,27 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
     if (lane == 0) s.exist[tile & 3][wave] = exist, s.known[tile & 3][wave] = paged;
   };
   const uint32_t lds_k0 = paged_lds(s.k[0]), lds_v0 = paged_lds(s.v[0]);
-  auto fetch_row = [&](const uint16_t* from, const long long (&at)[LOADS], uint32_t to, int i)
-      __attribute__((always_inline)) {
-    paged_dma(from + at[i], __builtin_amdgcn_readfirstlane(to + (4 * i + wave) * 1024));
+  auto slot = [](int n) { return n >= 5 ? n - 5 : n; };
+  auto fetch_k_row = [&](const long long (&at)[LOADS], int kb, int i) __attribute__((always_inline)) {
+    const uint32_t to = lds_k0 + (i < LOADS / 2 ? kb : slot(kb + 1)) * HALFB;
+    paged_dma(keys + at[i], __builtin_amdgcn_readfirstlane(to + (4 * (i % (LOADS / 2)) + wave) * 1024));
   };
-  auto fetch = [&](const uint16_t* from, const long long (&at)[LOADS], uint32_t to) {
+  auto fetch_v_row = [&](const long long (&at)[LOADS], uint32_t to, int i) __attribute__((always_inline)) {
+    paged_dma(values + at[i], __builtin_amdgcn_readfirstlane(to + (4 * i + wave) * 1024));
+  };
+  auto fetch_k = [&](const long long (&at)[LOADS], int kb) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) fetch_row(from, at, to, i);
+    for (int i = 0; i < LOADS; ++i) fetch_k_row(at, kb, i);
+  };
+  auto fetch_v = [&](const long long (&at)[LOADS], uint32_t to) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) fetch_v_row(at, to, i);
   };
   // Operands: byte addresses in a tile, XORed with a constant per 16 (K) or 32 (V) dims.
   const uint32_t lds_k = lds_k0 + col * ROWB + ((half ^ swizzle(col)) << 4);
   const int r = lane & 15, v_row = 4 * half + (r >> 2);
   const uint32_t lds_v = lds_v0 + v_row * ROWB + (((2 * (lane >> 4 & 1) + (r & 3) / 2) ^ swizzle(v_row)) << 4) + (r & 1) * 8;
-  auto read_k = [&](uint32_t base, int sub, int d) {
-    return *(const paged_lds_bf16x8*)((base ^ (d << 5)) + sub * (32 * ROWB));
-  };
+  auto read_k = [&](uint32_t base, int d) { return *(const paged_lds_bf16x8*)(uintptr_t)(base ^ (d << 5)); };
   auto read_v = [&](uint32_t base, int kt, int d) {  // keys 16 kt .. of the tile
     const pa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4*)((base ^ (d << 6)) + kt * (16 * ROWB)));
     const pa_s16x4 hi =
@@ -693,29 +708,22 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
     return __builtin_bit_cast(fa_bf16x8, both);
   };
 
-  float run_max[C], run_sum[C], ref[C];
-  fa_f32x16 o[C][DT];
+  float run_max = -INFINITY, run_sum = 0.f, ref = 0.f;
+  fa_f32x16 o[DT];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    run_max[c] = -INFINITY, run_sum[c] = ref[c] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      o[c][d] = fa_f32x16{};
-      asm("" : "+a"(o[c][d]));  // in the accumulation registers, here and wherever else than a product changes it
-    }
+  for (int d = 0; d < DT; ++d) {
+    o[d] = fa_f32x16{};
+    asm("" : "+a"(o[d]));  // in the accumulation registers, here and wherever else than a product changes it
   }
-  fa_f32x16 sc[C];        // scores of the present 32 keys
-  float top[C];           // their maximum, over this lane's
-  constexpr int AHEAD = 2;                 // products (pairs of them) that operands are read ahead; 3 measured the same
+  fa_f32x16 sc;                            // scores of the present 32 keys
+  float top;                               // their maximum, over this lane's
+  constexpr int AHEAD = 2;                 // products that operands are read ahead; 3 measured the same
   fa_bf16x8 kf[AHEAD + 1], vf[AHEAD + 1];  // operands on their way
 
   auto top_of = [&] {
+    top = sc[0];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      top[c] = sc[c][0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) top[c] = fmaxf(top[c], sc[c][e]);
-    }
+    for (int e = 1; e < 16; ++e) top = fmaxf(top, sc[e]);
   };
   // Whether every row sees every key of tile t.
   auto whole = [&](int t) {
@@ -726,12 +734,9 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   auto mask = [&](int t, int sub) {
     if (whole(t)) return;
     const int j0 = k0 + 64 * t + 32 * sub + 4 * half;
+    const int sees = limit - j0;
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int sees = limit[c] - j0;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sc[c][e] = 8 * (e >> 2) + (e & 3) < sees ? sc[c][e] : -INFINITY;
-    }
+    for (int e = 0; e < 16; ++e) sc[e] = 8 * (e >> 2) + (e & 3) < sees ? sc[e] : -INFINITY;
     const uint32_t known = s.known[t & 3][0] & s.known[t & 3][1] & s.known[t & 3][2] & s.known[t & 3][3];
     if (__builtin_amdgcn_readfirstlane(known) != 0xFFFFu) {
       uint32_t hidden = 0;  // of this lane's 16 keys
@@ -741,113 +746,88 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
         hidden |= (~s.known[t & 3][k / RPL % 4] >> (k / (4 * RPL) * RPL + k % RPL) & 1) << e;
       }
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sc[c][e] = hidden >> e & 1 ? -INFINITY : sc[c][e];
+      for (int e = 0; e < 16; ++e) sc[e] = hidden >> e & 1 ? -INFINITY : sc[e];
     }
     top_of();
   };
   // the exponentials' reference moves only where a score passes it by more than 2^8; O and the sum follow
   auto move = [&] {
-    float keep[C];
-    bool some = false;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const float most = xor32_max(top[c]) * c2;
-      const float moved = most > run_max[c] + 8.f ? most : run_max[c];
-      // (nothing to scale yet where there was no reference)
-      keep[c] = moved == run_max[c] || run_max[c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(run_max[c] - moved);
-      run_max[c] = moved;
-      ref[c] = moved == -INFINITY ? 0.f : moved;
-      some = some || keep[c] != 1.f;
-    }
-    if (__any(some)) {
+    const float most = xor32_max(top) * c2;
+    const float moved = most > run_max + 8.f ? most : run_max;
+    // (nothing to scale yet where there was no reference)
+    const float keep = moved == run_max || run_max == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(run_max - moved);
+    run_max = moved;
+    ref = moved == -INFINITY ? 0.f : moved;
+    if (__any(keep != 1.f)) {
       acc_settle();
+      run_sum *= keep;
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        run_sum[c] *= keep[c];
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float x = o[c][d][e];
-            acc_scale(x, keep[c]);
-            o[c][d][e] = x;
-          }
-      }
+        for (int e = 0; e < 16; ++e) {
+          float x = o[d][e];
+          acc_scale(x, keep);
+          o[d][e] = x;
+        }
       acc_settle();
     }
   };
   // Keys 32 sub .. of tile t (their scores in sc); then, with K of 32 keys at k_base (operands 0 and 1 in kf), the
   // scores of those; the first operands at kn_base follow into kf.
   // `beside(i)`: what else goes among the products, i of DS + 2 DT times.
-  auto step = [&](uint32_t v_base, int sub, uint32_t k_base, int k_sub, uint32_t kn_base, int kn_sub, auto beside)
+  auto step = [&](uint32_t v_base, int sub, uint32_t k_base, uint32_t kn_base, auto beside)
       __attribute__((always_inline)) {
     constexpr int START = DS == 8 ? 2 : 1;           // products after which the reference is settled
-    constexpr int PER = 6 * C / (DS - START);        // pairs of exponentials after each of the others
-    uint32_t pk[C][2][4];
-    auto pair = [&](int u) {  // pair u of 8 C: k-step u / 4 C, rows' part u / 4 % C
-      const int kt = u / (4 * C), c = u / 4 % C, j = u & 3, e = 8 * kt + 2 * j;
-      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][e], c2, -ref[c]));
-      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][e + 1], c2, -ref[c]));
-      pk[c][kt][j] = cvt_pk_bf16(p0, p1);
-      run_sum[c] = dot2_bf16(pk[c][kt][j], 0x3F803F80u, run_sum[c]);  // the rounded weights' sum
+    constexpr int PER = 6 / (DS - START);            // pairs of exponentials after each of the others
+    uint32_t pk[2][4];
+    auto pair = [&](int u) {  // pair u of 8: k-step u / 4
+      const int e = 8 * (u >> 2) + 2 * (u & 3);
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], c2, -ref));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e + 1], c2, -ref));
+      pk[u >> 2][u & 3] = cvt_pk_bf16(p0, p1);
+      run_sum = dot2_bf16(pk[u >> 2][u & 3], 0x3F803F80u, run_sum);  // the rounded weights' sum
     };
-    fa_f32x16 next[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) next[c] = fa_f32x16{};
+    fa_f32x16 next = fa_f32x16{};
 #pragma unroll
     for (int d = 0; d < DS; ++d) {
       constexpr int RING = AHEAD + 1;
-      if (d + AHEAD < DS) kf[(d + AHEAD) % RING] = read_k(k_base, k_sub, d + AHEAD);
+      if (d + AHEAD < DS) kf[(d + AHEAD) % RING] = read_k(k_base, d + AHEAD);
       else vf[d + AHEAD - DS] = read_v(v_base, 2 * sub + (d + AHEAD - DS) / DT, (d + AHEAD - DS) % DT);
+      next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[d % RING], qf[d], next, 0, 0, 0);
+      if (d >= START)
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        next[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[d % RING], qf[c][d], next[c], 0, 0, 0);
-        if (d >= START)
-#pragma unroll
-          for (int u = PER * c / C; u < PER * (c + 1) / C; ++u) pair((d - START) * PER + u);
-      }
+        for (int u = (d - START) * PER; u < (d - START + 1) * PER; ++u) pair(u);
       beside(d);
       if (d == START - 1) move();
       __builtin_amdgcn_sched_barrier(0);
     }
-    float most[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) most[c] = -INFINITY;
+    float most = -INFINITY;
 #pragma unroll
     for (int m = 0; m < 2 * DT; ++m) {
       const int kt = m / DT, d = m % DT;
       constexpr int RING = AHEAD + 1;
       if (m + AHEAD < 2 * DT) vf[(m + AHEAD) % RING] = read_v(v_base, 2 * sub + (m + AHEAD) / DT, (m + AHEAD) % DT);
-      else kf[m + AHEAD - 2 * DT] = read_k(kn_base, kn_sub, m + AHEAD - 2 * DT);
+      else kf[m + AHEAD - 2 * DT] = read_k(kn_base, m + AHEAD - 2 * DT);
+      const uint32_t w[4] = {pk[kt][0], pk[kt][1], pk[kt][2], pk[kt][3]};
+      o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[m % RING], __builtin_bit_cast(fa_bf16x8, w), o[d], 0, 0, 0);
+      if (kt == 0)
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const uint32_t w[4] = {pk[c][kt][0], pk[c][kt][1], pk[c][kt][2], pk[c][kt][3]};
-        o[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[m % RING], __builtin_bit_cast(fa_bf16x8, w), o[c][d], 0, 0, 0);
-        if (kt == 0)
+        for (int u = 6 + 2 * d / DT; u < 6 + 2 * (d + 1) / DT; ++u) pair(u);
+      // 8 / DT of the first (second) eight of the next scores
 #pragma unroll
-          for (int u = 6 * C + 2 * C * d / DT; u < 6 * C + 2 * C * (d + 1) / DT; ++u)
-            if (c == u % C) pair(u);
-        // the next scores of rows' part c: 8 / DT of the first (second) eight
-#pragma unroll
-        for (int i = 0; i < 8 / DT; ++i) {
-          const int e = 8 * kt + d * (8 / DT) + i;
-          float x = next[c][e];
-          asm("" : "+v"(x));  // out of its accumulator once, here
-          sc[c][e] = x;
-          most[c] = fmaxf(most[c], x);
-        }
+      for (int i = 0; i < 8 / DT; ++i) {
+        const int e = 8 * kt + d * (8 / DT) + i;
+        float x = next[e];
+        asm("" : "+v"(x));  // out of its accumulator once, here
+        sc[e] = x;
+        most = fmaxf(most, x);
       }
       beside(DS + m);
       __builtin_amdgcn_sched_barrier(0);
     }
     // what the next step needs is done in this one, among its products
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      top[c] = most[c];
-      asm volatile("" : "+v"(run_sum[c]), "+v"(top[c]));
-    }
+    top = most;
+    asm volatile("" : "+v"(run_sum), "+v"(top));
   };
   // V of tile t in LDS, where some of its rows do not exist or are not seen by every row: zeros for the former; for the
   // latter what is not finite goes (0 * inf) and is added at the end of the tile, row by row
@@ -887,89 +867,93 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
             const uint2 x = *reinterpret_cast<const uint2*>(v + 32 * d + 8 * g);
             const float add[4] = {special_lo(x.x), special_hi(x.x), special_lo(x.y), special_hi(x.y)};
 #pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                float y = o[c][d][4 * g + i];
-                acc_add(y, k < limit[c] ? add[i] : 0.f);
-                o[c][d][4 * g + i] = y;
-              }
+            for (int i = 0; i < 4; ++i) {
+              float y = o[d][4 * g + i];
+              acc_add(y, k < limit ? add[i] : 0.f);
+              o[d][4 * g + i] = y;
+            }
           }
       }
     }
     acc_settle();
   };
 
-  // At tile t: K of tiles t and t + 1 and V of tile t are in LDS, the scores of tile t's first 32 keys in sc; K of tile
-  // t + 2 goes to the buffer of tile t - 1 and V of tile t + 1 to that of tile t - 1 while it runs, and the rows of
-  // tile t + 3 are looked up.
+  // At tile t: K of tile t's second half and of tile t + 1 and V of tile t are in LDS, the scores of tile t's first 32
+  // keys in sc; K of tile t + 2 goes to the two free slots and V of tile t + 1 to the buffer of tile t - 1 while it runs,
+  // and the rows of tile t + 3 are looked up.
   long long at_k[LOADS], at_v[LOADS];
   if (tiles > 0) {
-    Rows now, then;
+    int now[LOADS], then[LOADS];
+    uint32_t row_now[LOADS], row_then[LOADS];
     look(now);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) row_now[i] = off[i];
+    advance();
     look(then);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) row_then[i] = off[i];
+    advance();
     look(ahead);
-    place(0, now, at_v);
-    fetch(keys, at_v, lds_k0);
-    fetch(values, at_v, lds_v0);
-    place(1, then, at_v);
-    fetch(keys, at_v, lds_k0 + TILEB);
-    place(2, ahead, at_k);
+    place(0, now, row_now, at_v);
+    fetch_k(at_v, 0);
+    fetch_v(at_v, lds_v0);
+    place(1, then, row_then, at_v);
+    fetch_k(at_v, 2);
+    place(2, ahead, off, at_k);
+    advance();
     paged_landed();
     __syncthreads();
     if (active) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) sc[c] = fa_f32x16{};
+      sc = fa_f32x16{};
 #pragma unroll
       for (int d = 0; d < DS; ++d) {
-        const fa_bf16x8 k = read_k(lds_k, 0, d);
-#pragma unroll
-        for (int c = 0; c < C; ++c) sc[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[c][d], sc[c], 0, 0, 0);
+        const fa_bf16x8 k = read_k(lds_k, d);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[d], sc, 0, 0, 0);
       }
       top_of();
       mask(0, 0);
 #pragma unroll
-      for (int d = 0; d < AHEAD; ++d) kf[d] = read_k(lds_k, 1, d);
+      for (int d = 0; d < AHEAD; ++d) kf[d] = read_k(lds_k + HALFB, d);
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float x = sc[c][e];
-          asm("" : "+v"(x));
-          sc[c][e] = x;
-        }
+      for (int e = 0; e < 16; ++e) {
+        float x = sc[e];
+        asm("" : "+v"(x));
+        sc[e] = x;
+      }
     }
+    __syncthreads();  // the first half has been read by all: tile 2 goes there
   }
   auto stage = [&](int t, int kb) {
-    fetch(keys, at_k, lds_k0 + (kb == 0 ? 2 : kb - 1) * TILEB);
-    fetch(values, at_v, lds_v0 + ((t + 1) & 1) * TILEB);
+    fetch_k(at_k, slot(kb + 4));
+    fetch_v(at_v, lds_v0 + ((t + 1) & 1) * TILEB);
     look(ahead);
   };
   auto staged = [&](int t) {
     paged_landed();
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) at_v[i] = at_k[i];
-    place(t + 3, ahead, at_k);
+    place(t + 3, ahead, off, at_k);
+    advance();
     __syncthreads();
   };
   // The two steps of a tile. `edge` (a compile-time bool): keys that a row may not see or that are of no page may be
   // among those of this tile and the next one's; without it there is no branch but the reference's move.
   auto tile = [&](int t, int kb, auto edge) __attribute__((always_inline)) {
-    const uint32_t vb = lds_v + (t & 1) * TILEB, kn = lds_k + (kb == 2 ? 0 : kb + 1) * TILEB;
-    const uint32_t to_k = lds_k0 + (kb == 0 ? 2 : kb - 1) * TILEB, to_v = lds_v0 + ((t + 1) & 1) * TILEB;
-    step(vb, 0, lds_k + kb * TILEB, 1, kn, 0, [&](int i) __attribute__((always_inline)) {
-      if (i < LOADS) fetch_row(keys, at_k, to_k, i);
-      else if (i < 2 * LOADS) fetch_row(values, at_v, to_v, i - LOADS);
+    const uint32_t vb = lds_v + (t & 1) * TILEB, to_v = lds_v0 + ((t + 1) & 1) * TILEB;
+    const uint32_t kn = lds_k + slot(kb + 2) * HALFB;
+    step(vb, 0, lds_k + slot(kb + 1) * HALFB, kn, [&](int i) __attribute__((always_inline)) {
+      if (i < LOADS) fetch_k_row(at_k, slot(kb + 4), i);
+      else if (i < 2 * LOADS) fetch_v_row(at_v, to_v, i - LOADS);
       else if (i < 3 * LOADS) look_row(i - 2 * LOADS, ahead);
     });
     if constexpr (decltype(edge)::value) mask(t, 1);
-    step(vb, 1, kn, 0, kn, 1, [](int) {});
+    step(vb, 1, kn, lds_k + slot(kb + 3) * HALFB, [](int) {});
     if constexpr (decltype(edge)::value)
       if (t + 1 < tiles) mask(t + 1, 0);
   };
-  auto after = [](int kb) { return kb == 2 ? 0 : kb + 1; };
+  auto after = [&](int kb) { return slot(kb + 2); };
   paged_landed();     // on the way past the block above too
-  int t = 0, kb = 0;  // kb = t % 3
+  int t = 0, kb = 0;  // kb = 2 t % 5
   if (!active) {
     for (; t < tiles; ++t, kb = after(kb)) {
       stage(t, kb);
@@ -1001,37 +985,32 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
     staged(t);
   }
 
+  const float sum = xor32_sum(run_sum);
+  if (row >= live) return;
+  if (unit.parts > 1) {
+    float* rec = paged_record(a, unit.record + unit.part, kvh, row, D);
+    if (half == 0) rec[0] = run_max, rec[1] = sum;
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const float sum = xor32_sum(run_sum[c]);
-    const int row = 32 * C * wave + 32 * c + col;
-    if (row >= live) continue;
-    if (unit.parts > 1) {
-      float* rec = paged_record(a, unit.record + unit.part, kvh, row, D);
-      if (half == 0) rec[0] = run_max[c], rec[1] = sum;
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int g = 0; g < 4; ++g) {
+        float2* to = reinterpret_cast<float2*>(rec + 2 + 32 * d + 8 * g + 4 * half);
+        to[0] = make_float2(o[d][4 * g], o[d][4 * g + 1]);
+        to[1] = make_float2(o[d][4 * g + 2], o[d][4 * g + 3]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  } else {
+    const float inv = run_max == -INFINITY ? 0.f : 1.f / sum;
+    uint16_t* to = a.out + ((size_t)(unit.begin + token) * a.query_heads + kvh * group + head) * D + 4 * half;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float2* to = reinterpret_cast<float2*>(rec + 2 + 32 * d + 8 * g + 4 * half);
-          to[0] = make_float2(o[c][d][4 * g], o[c][d][4 * g + 1]);
-          to[1] = make_float2(o[c][d][4 * g + 2], o[c][d][4 * g + 3]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-    } else {
-      const float inv = run_max[c] == -INFINITY ? 0.f : 1.f / sum;
-      const size_t token = unit.begin + unit.token + row / group;
-      uint16_t* to = a.out + (token * a.query_heads + kvh * group + row % group) * D + 4 * half;
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          *reinterpret_cast<uint2*>(to + 32 * d + 8 * g) =
-              make_uint2(cvt_pk_bf16(o[c][d][4 * g] * inv, o[c][d][4 * g + 1] * inv),
-                         cvt_pk_bf16(o[c][d][4 * g + 2] * inv, o[c][d][4 * g + 3] * inv));
-          __builtin_amdgcn_sched_barrier(0);
-        }
-    }
+      for (int g = 0; g < 4; ++g) {
+        *reinterpret_cast<uint2*>(to + 32 * d + 8 * g) =
+            make_uint2(cvt_pk_bf16(o[d][4 * g] * inv, o[d][4 * g + 1] * inv),
+                       cvt_pk_bf16(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
+        __builtin_amdgcn_sched_barrier(0);
+      }
   }
 }
 
@@ -1048,7 +1027,7 @@ __device__ void paged_attention_narrow(const PagedAttentionArgs& a) {
   }
 }
 
-template <int D, int C>
+template <int D>
 __device__ void paged_attention_mixed(const PagedAttentionArgs& a) {
   __shared__ __attribute__((aligned(256))) union {  // the wide form's addresses are XORed within a row
     PagedNarrowShared<D, 1> narrow;
@@ -1060,7 +1039,7 @@ __device__ void paged_attention_mixed(const PagedAttentionArgs& a) {
   for (PagedUnit unit; walk.next(a, unit); __syncthreads()) {
     paged_note(a, unit, kvh);
     if (unit.narrow) paged_narrow<D, 1>(a, unit, kvh, s.narrow);
-    else paged_wide<D, C>(a, unit, kvh, s.wide);
+    else paged_wide<D>(a, unit, kvh, s.wide);
   }
 }
 
@@ -1125,15 +1104,9 @@ __device__ void paged_attention_join(const PagedAttentionArgs& a) {
   extern "C" __global__ __launch_bounds__(256, 2) void aoto_paged_attention_d##D##_n2(PagedAttentionArgs a) {      \
     aoto::paged_attention_narrow<D, 2>(a);                                                                         \
   }                                                                                                                \
-  extern "C" __global__ __launch_bounds__(256, 128 / D)                                                            \
-  void aoto_paged_attention_d##D##_w128(PagedAttentionArgs a) {                                                    \
-    aoto::paged_attention_mixed<D, 1>(a);                                                                          \
+  extern "C" __global__ __launch_bounds__(256, 2) void aoto_paged_attention_d##D##_w(PagedAttentionArgs a) {       \
+    aoto::paged_attention_mixed<D>(a);                                                                             \
   }                                                                                                                \
   extern "C" __global__ __launch_bounds__(256) void aoto_paged_attention_join_d##D(PagedAttentionArgs a) {         \
     aoto::paged_attention_join<D>(a);                                                                              \
-  }
-// 256-row tiles, at 128 dims (at 64 half the rows and two blocks a CU were faster throughout).
-#define AOTO_PAGED_ATTENTION_WHOLE(D)                                                                              \
-  extern "C" __global__ __launch_bounds__(256, 1) void aoto_paged_attention_d##D##_w256(PagedAttentionArgs a) {    \
-    aoto::paged_attention_mixed<D, 2>(a);                                                                          \
   }
