@@ -60,7 +60,8 @@ AttentionPlan attention_plan(int tokens, int requests, int max_blocks, int page,
   if (max_kv_len) keys = std::min<long long>(keys, max_kv_len);
   // Not worth the join: narrow tiles of up to 256 keys, wide ones of up to 1024 (512 tokens over themselves: 28 us
   // whole and 35 cut at 128 dims, 19.5 and 24 at 64), wide ones that give every CU a block (32 / 8 heads of 128, 1024
-  // tokens over 1 / 1000 / 4000 keys before them: 41 / 62 / 127 us whole, 56 / 76 / 128 cut).
+  // tokens over 1 / 1000 / 4000 keys before them: 41 / 62 / 127 us whole, 56 / 76 / 128 cut; 14 / 2 heads of 64, 4096
+  // over 2000 / 6000: 113 / 191 and 153 / 231).
   if (keys > (p.wide_rows ? 1024 : 256) && 2 * p.units * kv_heads < (p.wide_rows ? 1 : 8) * full &&
       p.units * most < (1 << 30)) {
     p.target = (int)((full + kv_heads - 1) / kv_heads);

@@ -15,7 +15,7 @@
 // model's logits, what stands and the weights the following token is drawn from, summed by chunk; the token.
 //
 // The first is bound by its instructions, 20 a logit of which 11 in 64 bits (64 requests, up to five drafts with their
-// logits, 151936 bf16 tokens: 33 us of 57), after it by the chain request -> statistics -> law -> chunk -> token, each
+// logits, 128256 bf16 tokens: 33 us of 57), after it by the chain request -> statistics -> law -> chunk -> token, each
 // a round trip to memory: 6 + 10 + 10 us there, 13 of 25 us without a draft model. Chunks of 2048 tokens deal the work
 // out evenly (57 us; 4096: 63, 1024: 64 us) and leave the joins short. A loop over the chunk's loads, for less code,
 // cost more than the instructions it fetched (1 to 2 us).
