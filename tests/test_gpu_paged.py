@@ -276,7 +276,7 @@ def test_attention_of_single_tokens(hq, hkv, dim, page):
 
 
 @pytest.mark.parametrize("hq,hkv,dim", HEADS)
-@pytest.mark.parametrize("page", [8, 48])
+@pytest.mark.parametrize("page", [1, 8, 48, 256])
 def test_attention_of_chunks(hq, hkv, dim, page):
     rng = np.random.default_rng(hq * dim + page)
     s = _requests(rng, [(5, 5), (1, 200), (70, 133), (2, 31), (0, 0), (131, 131), (9, 300)], hq, hkv, dim, page, tail=2)
