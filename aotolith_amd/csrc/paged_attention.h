@@ -584,10 +584,12 @@ AOTO_DEVICE void acc_settle() {
 // them so) that spreads each phase of the reads over all banks. Rows' addresses advance by 64 keys a tile without a
 // division or a product but the page's.
 //
-// Bound by what a wave issues and waits for between its products: 2048 rows over 8048 keys, 32 / 8 heads of 128, run at
-// 0.83 PFLOP/s in 283 us, the matrix units busy for 37% of it and the vector units for 60%. One wave a SIMD with 64
-// rows, half the reads from LDS and 512 registers took 297 us there, and from 96 us (77 here) to 61 (41) for 2048 and
-// 1024 rows over themselves, where its tiles are too few for the chip.
+// Bound by issue, every part with its share: 2048 rows over 8048 keys, 32 / 8 heads of 128, run at 0.85 PFLOP/s in
+// 277 us, the matrix units busy for 37% of it and the vector units for 64%; without its loads to LDS it would take 35 us
+// less, without the reads of K 34, of V 11, without half of the products 32, without the exponentials 17. Reading
+// operands one or three products ahead, no fences between the products, and the packing of weights one product later
+// changed it by less than 1%. One wave a SIMD with 64 rows, half the reads from LDS and 512 registers took 297 us
+// there, 96 us (73 here) for 2048 rows over themselves and 61 us (41) for 1024, its tiles being too few for the chip.
 template <int D>
 AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, int kvh, PagedWideShared<D>& s) {
   constexpr int DS = D / 16, DT = D / 32, LPR = D / 8;  // lanes (16-byte pieces) a row
@@ -801,7 +803,10 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
 #pragma unroll
         for (int u = (d - START) * PER; u < (d - START + 1) * PER; ++u) pair(u);
       beside(d);
-      if (d == START - 1) move();
+      if (d == START - 1) {
+        move();
+        __builtin_amdgcn_s_setprio(1);  // ahead of the SIMD's other wave where that stages or waits (284 -> 277 us)
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     float most = -INFINITY;
@@ -828,6 +833,7 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
       beside(DS + m);
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     // what the next step needs is done in this one, among its products
     top = most;
     asm volatile("" : "+v"(run_sum), "+v"(top));
