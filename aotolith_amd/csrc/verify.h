@@ -541,32 +541,42 @@ __device__ void verify_pick(const VerifyArgs& a) {
       const VerifyChunk* chunks = static_cast<const VerifyChunk*>(a.workspace) +
                                   ((size_t)r * (2 * a.drafts + 1) + law.accepted) * a.chunks;
       const VerifyScale weight(law.top, law.heat, table);
-      auto mass = [&](int c, bool whole) {
-        if (c >= a.chunks) return 0.0;
-        if (!whole && law.draft_row) return verify_masses(a, r)[c];
-        const VerifyChunk one = chunks[c];
-        double sum = one.sum != 0.0 ? one.sum * weight(one.top) : 0.0;
-        if (!whole && law.removed >= 0 && law.removed / kVerifyChunk == c) {
-          // what a removed token leaves of its chunk; of the difference's rounding nothing
-          const double left = sum - law.fell;
-          sum = left > 0x1p-50 * sum ? left : 0.0;
-        }
-        return sum;
-      };
       bool whole = false;
-      double near = mass(lane, false), total = wave_sum_f64(near);  // the first 64 chunks stay in a register
-      for (int c = 64; c < a.chunks; c += 64) total += wave_sum_f64(mass(c + lane, false));
-      if (!(total > 0.0)) {
-        whole = true;
-        near = mass(lane, true), total = wave_sum_f64(near);
-        for (int c = 64; c < a.chunks; c += 64) total += wave_sum_f64(mass(c + lane, true));
-      }
+      // a chunk's weight: as a subtracted law left it, or of its statistics
+      auto load = [&](int c) {
+        const int at = min(c, a.chunks - 1);
+        if (!whole && law.draft_row) return VerifyChunk{verify_masses(a, r)[at], law.top, 0};
+        return chunks[at];
+      };
+      auto mass = [&](int c, const VerifyChunk& of) {
+        if (c >= a.chunks || !(of.sum > 0.0)) return 0.0;
+        if (!whole && law.draft_row) return of.sum;
+        const double sum = of.sum * weight(of.top);
+        if (whole || law.removed < 0 || law.removed / kVerifyChunk != c) return sum;
+        // what a removed token leaves of its chunk; of the difference's rounding nothing
+        const double left = sum - law.fell;
+        return left > 0x1p-50 * sum ? left : 0.0;
+      };
+      constexpr int NEAR = 2;  // chunks a lane that are loaded once and stay in registers: 262144 tokens
+      double near[NEAR];
+      auto sum_up = [&] {
+        VerifyChunk of[NEAR];
+#pragma unroll
+        for (int n = 0; n < NEAR; ++n) of[n] = load(64 * n + lane);
+        double total = 0.0;
+#pragma unroll
+        for (int n = 0; n < NEAR; ++n) near[n] = mass(64 * n + lane, of[n]), total += near[n];
+        for (int c = 64 * NEAR + lane; c < a.chunks; c += 64) total += mass(c, load(c));
+        return wave_sum_f64(total);
+      };
+      double total = sum_up();
+      if (!(total > 0.0)) whole = true, total = sum_up();
       const double target = (double)u * total;
       // the chunk; past the total (a random number of 1, or the sums' last bits) the last one that has weight
       double run = 0.0, before = 0.0;
       int chunk = 0;
       for (int c = 0; c < a.chunks; c += 64) {
-        const double m = c == 0 ? near : mass(c + lane, whole);
+        const double m = c == 0 ? near[0] : c == 64 ? near[1] : mass(c + lane, load(c + lane));
         const double upto = run + wave_scan_f64(m);
         const unsigned long long some = __ballot(m > 0.0), past = __ballot(m > 0.0 && upto > target);
         const int at = past ? __ffsll(past) - 1 : some ? 63 - __clzll((long long)some) : -1;
