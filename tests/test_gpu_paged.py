@@ -504,6 +504,24 @@ def test_attention_on_another_stream_and_with_a_small_workspace():
     _check_attention(s, got)
 
 
+def test_attention_on_two_streams_at_once():
+    # each call has a workspace of its own
+    rng = np.random.default_rng(18)
+    ops, streams, runs = _ops(), [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for lengths in ([(1, 3000), (1, 50), (1, 4100)], [(150, 2000), (1, 900), (7, 7)]):
+        s = _requests(rng, lengths, 8, 2, 64, 16)
+        runs.append((s, [to_gpu_bf16(s["q"]), *s["device"], _i32(s["tables"]), _i32(s["start"]), _i32(s["kv"])], []))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for (_, inputs, outs), stream in zip(runs, streams):
+            with torch.cuda.stream(stream):
+                outs.append(ops.paged_attention(*inputs))
+    torch.cuda.synchronize()
+    for s, _, outs in runs:
+        _check_attention(s, outs[0])
+        assert all(bool((o == outs[0]).all()) for o in outs)
+
+
 def test_attention_is_the_same_every_time():
     rng = np.random.default_rng(15)
     s = _requests(rng, [(1, 3000), (40, 2500), (3, 50)], 8, 2, 64, 16)
@@ -760,3 +778,74 @@ def test_serving_steps_over_one_cache():
                 context[r] += 1 + stood
                 texts[r] += [int(t) for t in expected[r, : stood + 1]]
     assert int(counts.sum()) == int(start) and len(set(_np(tables)[_np(tables) >= 0])) == int(start)
+
+
+def test_a_captured_step_of_every_operator_replays():
+    """Decodes and drafted tokens of six requests: the step captured once against the same steps called one by one."""
+
+    ops = _ops()
+    hq, hkv, dim, vocab, page, requests, room, drafts = 8, 2, 64, 5000, 16, 6, 24, 3
+    device = dict(device="cuda")
+
+    def state():
+        rng = np.random.default_rng(19)
+        (keys, values), _ = _cache(rng, 400, hkv, page, dim, "dense")
+        context = np.array([0, 15, 16, 700, 3, 250])
+        counts = -(-context // page)
+        tables, order, at = np.full((requests, 64), -1, np.int32), rng.permutation(400), 0
+        for r, count in enumerate(counts):
+            tables[r, :count], at = order[at: at + count], at + count
+        angle = rng.random((1024, dim)) * 6
+        cos, sin = (torch.tensor(f(angle), **device).to(torch.bfloat16) for f in (np.cos, np.sin))
+        return dict(context=_i32(context), new=_i32([1] * requests), tables=_i32(tables), counts=_i32(counts),
+                    free=_i32(order[at:]), start=_i32([0]), keys=keys, values=values, cos=cos, sin=sin,
+                    qkv=torch.zeros((room, (hq + 2 * hkv) * dim), dtype=torch.bfloat16, **device),
+                    logits=torch.zeros((room, vocab), **device), drafts=_i64(np.zeros((requests, drafts))),
+                    uniforms=torch.zeros((requests, drafts + 1), **device),
+                    heat=torch.tensor([0.0, 1.0, 0.7, 0.0, 2.0, 1.0], **device),
+                    error=torch.zeros(1, dtype=torch.int32, **device),
+                    out=torch.zeros((room, hq * dim), dtype=torch.bfloat16, **device),
+                    q=torch.zeros((room, hq, dim), dtype=torch.bfloat16, **device))
+
+    def run(d):
+        step = d.get("step")
+        step = ops.paged_tables(d["context"], d["new"], d["tables"], d["counts"], d["free"], d["start"],
+                                page_size=page, max_tokens=room, step=step, error=d["error"])
+        ops.paged_rope_append(d["qkv"], step.positions, step.slots, d["cos"], d["sin"], d["keys"], d["values"],
+                              query_heads=hq, q_out=d["q"], error=d["error"])
+        ops.paged_attention(d["q"], d["keys"], d["values"], d["tables"], step.query_start, step.kv_lens, out=d["out"],
+                            max_query_len=drafts + 1)
+        tokens, accepted = ops.verify_draft(d["logits"], d["drafts"], step.query_start, d["uniforms"],
+                                            temperature=d["heat"])
+        return step, tokens, accepted
+
+    one, two = state(), state()
+    spare = state()
+    spare["step"] = run(spare)[0]._replace(page_counts=spare["counts"], free_start=spare["start"])
+    two["step"] = ops.PagedStep(*(torch.zeros_like(t) for t in spare["step"][:4]), two["counts"], two["start"])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run(two)
+    rng = np.random.default_rng(20)
+    for _ in range(12):
+        new = rng.integers(0, drafts + 2, requests)
+        qkv, logits = bf16_normal(rng, tuple(one["qkv"].shape)), rng.standard_normal((room, vocab)) * 3
+        guesses, uniforms = rng.integers(0, vocab, (requests, drafts)), rng.random((requests, drafts + 1))
+        for d in (one, two):
+            d["new"].copy_(_i32(new))
+            d["qkv"].copy_(to_gpu_bf16(qkv))
+            d["logits"].copy_(torch.tensor(logits, **device))
+            d["drafts"].copy_(_i64(guesses))
+            d["uniforms"].copy_(torch.tensor(uniforms, **device))
+        step, tokens, accepted = run(one)
+        one["counts"], one["start"] = step.page_counts, step.free_start
+        graph.replay()
+        for a, b in zip((*step, tokens, accepted), (*captured[0], *captured[1:])):
+            assert bool((a == b).all())
+        for name in ("tables", "keys", "values", "q", "out", "error"):
+            assert bool((one[name] == two[name]).all()), name
+        # what stood of each request is kept
+        context = torch.where(one["new"] > 0, step.kv_lens - one["new"] + accepted + 1, step.kv_lens)
+        for d in (one, two):
+            d["context"].copy_(context)
+    assert int(one["error"]) == 0
