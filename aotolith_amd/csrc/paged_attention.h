@@ -230,6 +230,14 @@ AOTO_DEVICE long long paged_row(const PagedAttentionArgs& a, const int* __restri
   return (unsigned)page < (unsigned)a.pages ? page * a.page_stride + row * a.slot_stride : -1;
 }
 
+// Of a weight that is not negative: the smallest normal number where it is below that. By the bits as a whole number,
+// where a NaN is above all others and stays one.
+AOTO_DEVICE float paged_floor(float p) { return __uint_as_float(max(__float_as_uint(p), 0x00800000u)); }
+
+// 1 / sum of a row's weights, whose maximum is `big`: 0 where no key was seen (a row whose scores are all NaN has no
+// maximum either, but a sum of NaN).
+AOTO_DEVICE float paged_inverse(float big, float sum) { return big == -INFINITY && sum == 0.f ? 0.f : 1.f / sum; }
+
 AOTO_DEVICE bool bf16_pair_special(uint32_t w) {
   return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
 }
@@ -451,7 +459,7 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
       for (int j = 0; j < 8; ++j) {
         // not below the smallest normal number, which beside the row's weights is nothing, so that an infinite value
         // stays one (0 * inf); the values of keys that are not there, or hidden from a row, are finite
-        p[j] = fmaxf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j >> 2][j & 3], c2, -ref)), 0x1p-126f);
+        p[j] = paged_floor(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j >> 2][j & 3], c2, -ref)));
         run_sum[t] += p[j];
       }
       uint32_t high[4], low[4];
@@ -459,8 +467,7 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
       for (int j = 0; j < 4; ++j) {
         if constexpr (TWO) {
           high[j] = __builtin_amdgcn_perm(__float_as_uint(p[2 * j + 1]), __float_as_uint(p[2 * j]), 0x07060302u);
-          low[j] = cvt_pk_bf16(fmaxf(p[2 * j] - bf16_lo(high[j]), 0x1p-126f),
-                               fmaxf(p[2 * j + 1] - bf16_hi(high[j]), 0x1p-126f));
+          low[j] = cvt_pk_bf16(paged_floor(p[2 * j] - bf16_lo(high[j])), paged_floor(p[2 * j + 1] - bf16_hi(high[j])));
         } else {
           high[j] = cvt_pk_bf16(p[2 * j], p[2 * j + 1]);
           low[j] = 0;
@@ -533,7 +540,7 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
       *reinterpret_cast<float2*>(rec + 2 + d) = make_float2(v[0], v[1]);
       *reinterpret_cast<float2*>(rec + 4 + d) = make_float2(v[2], v[3]);
     } else {
-      const float inv = big == -INFINITY ? 0.f : 1.f / sum;
+      const float inv = paged_inverse(big, sum);
       const size_t token = unit.begin + unit.token + row / group;
       *reinterpret_cast<uint2*>(a.out + (token * a.query_heads + kvh * group + row % group) * D + d) =
           make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
@@ -1019,7 +1026,7 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
         __builtin_amdgcn_sched_barrier(0);
       }
   } else {
-    const float inv = run_max == -INFINITY ? 0.f : 1.f / sum;
+    const float inv = paged_inverse(run_max, sum);
     uint16_t* to = a.out + ((size_t)(unit.begin + token) * a.query_heads + kvh * group + head) * D + 4 * half;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -1090,7 +1097,7 @@ __device__ void paged_attention_join(const PagedAttentionArgs& a) {
     float top = big;
 #pragma unroll
     for (int i = 0; i < SOME; ++i) {
-      if (s0 + i >= note.y) m[i] = -INFINITY;
+      if (s0 + i >= note.y) m[i] = -INFINITY, l[i] = 0.f;
       top = fmaxf(top, m[i]);
     }
     const float keep = big == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(big - top);
@@ -1101,14 +1108,14 @@ __device__ void paged_attention_join(const PagedAttentionArgs& a) {
 #pragma unroll
     for (int i = 0; i < SOME; ++i) {
       const float f = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - big);
-      if (f != 0.f) {  // a part that sees no key has nothing finite to scale by 0
-        sum += f * l[i];
+      sum += f * l[i];  // NaN of a part whose scores are all NaN, too
+      if (f != 0.f) {
 #pragma unroll
         for (int e = 0; e < PER; ++e) acc[e] += f * o[i][e];
       }
     }
   }
-  const float inv = big == -INFINITY ? 0.f : 1.f / sum;
+  const float inv = paged_inverse(big, sum);
   uint16_t* out = a.out + ((size_t)t * a.query_heads + h) * D + PER * lane;
   if constexpr (PER == 2) *reinterpret_cast<uint32_t*>(out) = cvt_pk_bf16(acc[0] * inv, acc[1] * inv);
   else out[0] = (uint16_t)f32_to_bf16(acc[0] * inv);

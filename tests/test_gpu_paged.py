@@ -434,6 +434,63 @@ def test_attention_of_every_form(kernel, hq, hkv, dim, most, requests, keys):
     _check_attention(s, _attend(s, **bounds))
 
 
+def _form_requests(rng, hq, hkv, dim, most, requests, keys):
+    """Requests of a form of ``FORMS``: the second and the last of ``most`` rows, the third over ``keys`` keys."""
+
+    rows = rng.integers(0, most + 1, requests)
+    rows[1], rows[2], rows[-1] = most, most - 1, most
+    lengths = [(int(n), int(n) + int(rng.integers(0, 400))) for n in rows]
+    lengths[2] = (most - 1, keys)
+    return _requests(rng, lengths, hq, hkv, dim, 16, tail=3)
+
+
+def _form_attend(s, kernel, most, keys, cut):
+    """The call with that kernel, its items whole or cut and joined."""
+
+    with _ops().recording_launches() as take:
+        # a bound that is not true keeps the items whole
+        got = _attend(s, max_query_len=most, max_kv_len=keys if cut else 64)
+        launches = take()
+    assert "aoto_paged_attention_" + kernel in launches
+    return got, any("join" in name for name in launches)
+
+
+def _check_attention_pattern(s, got):
+    """NaN where the definition has it, everything else within the bound."""
+
+    with np.errstate(invalid="ignore"):
+        want, size, written = oracle.attention(s["q"], s["keys"], s["values"], s["tables"], s["start"], s["kv"])
+    got = from_gpu_bf16(got).astype(np.float64)
+    odd = np.isnan(want)
+    assert odd.any() and not odd[written].all()
+    np.testing.assert_array_equal(np.isnan(got), odd)
+    assert (np.abs(got - want) <= attention_bound(want, size))[~odd & written[:, None]].all()
+    assert (got[~written] == 5.0).all()
+
+
+@pytest.mark.parametrize("kernel,hq,hkv,dim,most,requests", FORMS)
+@pytest.mark.parametrize("cut", [False, True])
+def test_attention_of_nan_and_infinite_scores(kernel, hq, hkv, dim, most, requests, cut):
+    # a query that is NaN makes its row NaN, a key that is NaN the rows that see it; a score of +inf the row it is in
+    # (inf - inf), one of -inf weighs nothing
+    rng = np.random.default_rng(hq + most)
+    s = _form_requests(rng, hq, hkv, dim, most, requests, 1500)
+    first, rows, kv = s["start"][:-1], np.diff(s["start"]), s["kv"]
+
+    def key(r, j):
+        return s["keys"][s["tables"][r, j // 16], :, j % 16]
+
+    s["q"][first[2] + 1, 0, 5] = np.nan                  # all scores of one head's row
+    key(1, kv[1] - 1 - rows[1] // 2)[hkv - 1, 7] = np.nan  # a key that the later rows of one kv head see
+    key(2, 700)[0, 3] = np.nan if hkv > 1 else np.inf    # inside the long request, in one part of it
+    key(requests - 1, kv[-1] - 1)[0, 0] = np.inf         # +inf or -inf, as the last row's query has it
+    s["device"][0].copy_(to_gpu_bf16(s["keys"]))
+    got, joined = _form_attend(s, kernel, most, 1500, cut)
+    if not cut:
+        assert not joined
+    _check_attention_pattern(s, got)
+
+
 @pytest.mark.parametrize("rows", [1, 20])
 def test_attention_of_large_scores(rows):
     # one key far above the others, scores to +-90: the running maximum moves, nothing overflows
