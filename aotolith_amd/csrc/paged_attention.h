@@ -230,10 +230,6 @@ AOTO_DEVICE long long paged_row(const PagedAttentionArgs& a, const int* __restri
   return (unsigned)page < (unsigned)a.pages ? page * a.page_stride + row * a.slot_stride : -1;
 }
 
-// Of a weight that is not negative: the smallest normal number where it is below that. By the bits as a whole number,
-// where a NaN is above all others and stays one.
-AOTO_DEVICE float paged_floor(float p) { return __uint_as_float(max(__float_as_uint(p), 0x00800000u)); }
-
 // 1 / sum of a row's weights, whose maximum is `big`: 0 where no key was seen (a row whose scores are all NaN has no
 // maximum either, but a sum of NaN).
 AOTO_DEVICE float paged_inverse(float big, float sum) { return big == -INFINITY && sum == 0.f ? 0.f : 1.f / sum; }
@@ -256,6 +252,32 @@ AOTO_DEVICE uint4 chunk_finite(const uint4& v) {
 // The infinity or NaN in the upper or lower half of w, else 0.
 AOTO_DEVICE float special_lo(uint32_t w) { return (w & 0x7F80u) == 0x7F80u ? bf16_lo(w) : 0.f; }
 AOTO_DEVICE float special_hi(uint32_t w) { return (w & 0x7F800000u) == 0x7F800000u ? bf16_hi(w) : 0.f; }
+
+
+// The sum of the infinities and NaN among four dims of keys k0 .. limit - 1 that have a page, 0 where there are none.
+// A weight of 0 (2^-126 of the row's largest and less, and every second term of one that bf16 holds) makes a NaN of an
+// infinite value, which the result should be: a row that has one, though none of its scores is, takes this sum there.
+// Seldom called, so kept short: one round trip to memory for four keys.
+AOTO_DEVICE f32x4_t paged_special(const PagedAttentionArgs& a, const int* __restrict__ table,
+                                  const uint16_t* __restrict__ values, int k0, int limit) {
+  f32x4_t sum{};
+#pragma unroll 4
+  for (int k = k0; k < limit; ++k) {
+    const long long row = paged_row(a, table, k);
+    const uint2 w = *reinterpret_cast<const uint2*>(values + max(row, 0LL));
+    const bool there = row >= 0;
+    sum[0] += there ? special_lo(w.x) : 0.f, sum[1] += there ? special_hi(w.x) : 0.f;
+    sum[2] += there ? special_lo(w.y) : 0.f, sum[3] += there ? special_hi(w.y) : 0.f;
+  }
+  return sum;
+}
+AOTO_DEVICE bool paged_any_nan(const f32x4_t& v) { return v[0] != v[0] || v[1] != v[1] || v[2] != v[2] || v[3] != v[3]; }
+// v with the sums of special values (not 0 where there are some) in the place of its NaN.
+AOTO_DEVICE f32x4_t paged_with_special(f32x4_t v, const f32x4_t& special) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = v[i] != v[i] && special[i] != 0.f ? special[i] : v[i];
+  return v;
+}
 
 AOTO_DEVICE float* paged_record(const PagedAttentionArgs& a, int unit, int kvh, int row, int head_dim) {
   return a.records + (((size_t)unit * a.kv_heads + kvh) * a.record_rows + row) * (head_dim + 2);
@@ -457,9 +479,8 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
       float p[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        // not below the smallest normal number, which beside the row's weights is nothing, so that an infinite value
-        // stays one (0 * inf); the values of keys that are not there, or hidden from a row, are finite
-        p[j] = paged_floor(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j >> 2][j & 3], c2, -ref)));
+        // 0 for a key that is not there or hidden from the row, whose value here is finite
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j >> 2][j & 3], c2, -ref));
         run_sum[t] += p[j];
       }
       uint32_t high[4], low[4];
@@ -467,7 +488,7 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
       for (int j = 0; j < 4; ++j) {
         if constexpr (TWO) {
           high[j] = __builtin_amdgcn_perm(__float_as_uint(p[2 * j + 1]), __float_as_uint(p[2 * j]), 0x07060302u);
-          low[j] = cvt_pk_bf16(paged_floor(p[2 * j] - bf16_lo(high[j])), paged_floor(p[2 * j + 1] - bf16_hi(high[j])));
+          low[j] = cvt_pk_bf16(p[2 * j] - bf16_lo(high[j]), p[2 * j + 1] - bf16_hi(high[j]));
         } else {
           high[j] = cvt_pk_bf16(p[2 * j], p[2 * j + 1]);
           low[j] = 0;
@@ -534,6 +555,10 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
       // a wave without keys holds zeros: 0 * 0
       v += f * *reinterpret_cast<const f32x4_t*>(&s.o[w][row][d]);
     }
+    // kept out of the way: fetched with the code around it, it took 0.2 of a small call's 7.2 us
+    if (__builtin_expect(__any(paged_any_nan(v) && sum == sum), 0))
+      v = paged_with_special(v, paged_special(a, table, a.values + kvh * a.head_stride + d, k0,
+                                              min(k1, unit.first + unit.token + row / group)));
     if (unit.parts > 1) {
       float* rec = paged_record(a, unit.record + unit.part, kvh, row, D);
       if (d == 0) rec[0] = big, rec[1] = sum;

@@ -491,6 +491,37 @@ def test_attention_of_nan_and_infinite_scores(kernel, hq, hkv, dim, most, reques
     _check_attention_pattern(s, got)
 
 
+def _vanishing(rng, s, r, keys):
+    """Keys of request r whose weights are below 2^-150 of their rows' largest: queries near 1, these keys -16."""
+
+    first, last = s["start"][r], s["start"][r + 1]
+    s["q"][first:last] = from_gpu_bf16(to_gpu_bf16(1 + 0.1 * bf16_normal(rng, s["q"][first:last].shape)))
+    for j in keys:
+        s["keys"][s["tables"][r, j // 16], :, j % 16] = -16.0
+    s["device"][0].copy_(to_gpu_bf16(s["keys"]))
+
+
+@pytest.mark.parametrize("kernel,hq,hkv,dim,most,requests", FORMS)
+@pytest.mark.parametrize("cut", [False, True])
+def test_attention_of_large_values_that_weigh_nothing(kernel, hq, hkv, dim, most, requests, cut):
+    # values near the largest number, hidden from a row or next to it of no weight, leave the row as it is
+    rng = np.random.default_rng(hq + most + 1)
+    s = _form_requests(rng, hq, hkv, dim, most, requests, 1500)
+    low = [*range(600), 700, 1023, 1024, 1490 - most]
+    _vanishing(rng, s, 2, low)
+    for i, j in enumerate((0, 300, *low[600:])):
+        s["values"][s["tables"][2, j // 16], :, j % 16, 4 * i: 4 * i + 2] = -3e38 if i % 2 else 3e38
+    last = s["kv"][1] - 1   # the key of the second request's last row
+    s["values"][s["tables"][1, last // 16], :, last % 16, 40: 50] = 3e38
+    s["device"][1].copy_(to_gpu_bf16(s["values"]))
+    s["values"] = from_gpu_bf16(s["device"][1]).copy()
+    got = from_gpu_bf16(_form_attend(s, kernel, most, 1500, cut)[0]).astype(np.float64)
+    want, size, written = oracle.attention(s["q"], s["keys"], s["values"], s["tables"], s["start"], s["kv"])
+    written[s["start"][2] - 1] = False
+    # scores of up to 16 * 128^(1/2) = 181 in f32 add 181 * 2^-23 = 2.2e-5 to log p, of the few that matter 2e-6
+    assert (np.abs(got - want) <= attention_bound(want, size))[written].all()
+
+
 @pytest.mark.parametrize("rows", [1, 20])
 def test_attention_of_large_scores(rows):
     # one key far above the others, scores to +-90: the running maximum moves, nothing overflows
