@@ -278,6 +278,8 @@ AOTO_DEVICE f32x4_t paged_with_special(f32x4_t v, const f32x4_t& special) {
   for (int i = 0; i < 4; ++i) v[i] = v[i] != v[i] && special[i] != 0.f ? special[i] : v[i];
   return v;
 }
+// An infinite value of a part stays one under any factor, 0 too.
+AOTO_DEVICE float paged_scaled(float x, float by) { return fabsf(x) < INFINITY ? x * by : x; }
 
 AOTO_DEVICE float* paged_record(const PagedAttentionArgs& a, int unit, int kvh, int row, int head_dim) {
   return a.records + (((size_t)unit * a.kv_heads + kvh) * a.record_rows + row) * (head_dim + 2);
@@ -1038,21 +1040,26 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
 
   const float sum = xor32_sum(run_sum);
   if (row >= live) return;
+  float probe = 0.f;  // NaN where an element of O is not finite
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) probe = __builtin_fmaf(o[d][e], 0.f, probe);
+  float* rec = unit.parts > 1 ? paged_record(a, unit.record + unit.part, kvh, row, D) : nullptr;
+  uint16_t* to = a.out + ((size_t)(unit.begin + token) * a.query_heads + kvh * group + head) * D + 4 * half;
   if (unit.parts > 1) {
-    float* rec = paged_record(a, unit.record + unit.part, kvh, row, D);
     if (half == 0) rec[0] = run_max, rec[1] = sum;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        float2* to = reinterpret_cast<float2*>(rec + 2 + 32 * d + 8 * g + 4 * half);
-        to[0] = make_float2(o[d][4 * g], o[d][4 * g + 1]);
-        to[1] = make_float2(o[d][4 * g + 2], o[d][4 * g + 3]);
+        float2* at = reinterpret_cast<float2*>(rec + 2 + 32 * d + 8 * g + 4 * half);
+        at[0] = make_float2(o[d][4 * g], o[d][4 * g + 1]);
+        at[1] = make_float2(o[d][4 * g + 2], o[d][4 * g + 3]);
         __builtin_amdgcn_sched_barrier(0);
       }
   } else {
     const float inv = paged_inverse(run_max, sum);
-    uint16_t* to = a.out + ((size_t)(unit.begin + token) * a.query_heads + kvh * group + head) * D + 4 * half;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -1062,6 +1069,21 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
                        cvt_pk_bf16(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
         __builtin_amdgcn_sched_barrier(0);
       }
+  }
+  if (__builtin_expect(__any(probe != probe && sum == sum), 0)) {
+    // special values in the place of NaN, in what this lane has just written
+#pragma unroll 1
+    for (int c = 0; c < D / 8; ++c) {
+      float2* at = reinterpret_cast<float2*>(rec + 2 + 8 * c + 4 * half);
+      uint2* out = reinterpret_cast<uint2*>(to + 8 * c);
+      f32x4_t v;
+      if (unit.parts > 1) v = f32x4_t{at[0].x, at[0].y, at[1].x, at[1].y};
+      else v = f32x4_t{bf16_lo(out->x), bf16_hi(out->x), bf16_lo(out->y), bf16_hi(out->y)};
+      if (!paged_any_nan(v) || sum != sum) continue;
+      v = paged_with_special(v, paged_special(a, table, a.values + kvh * a.head_stride + 8 * c + 4 * half, k0, limit));
+      if (unit.parts > 1) at[0] = make_float2(v[0], v[1]), at[1] = make_float2(v[2], v[3]);
+      else *out = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    }
   }
 }
 
@@ -1122,22 +1144,24 @@ __device__ void paged_attention_join(const PagedAttentionArgs& a) {
     float top = big;
 #pragma unroll
     for (int i = 0; i < SOME; ++i) {
-      if (s0 + i >= note.y) m[i] = -INFINITY, l[i] = 0.f;
+      if (s0 + i >= note.y) {
+        m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) o[i][e] = 0.f;
+      }
       top = fmaxf(top, m[i]);
     }
     const float keep = big == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(big - top);
     big = top;
     sum *= keep;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] *= keep;
+    for (int e = 0; e < PER; ++e) acc[e] = paged_scaled(acc[e], keep);
 #pragma unroll
     for (int i = 0; i < SOME; ++i) {
       const float f = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - big);
       sum += f * l[i];  // NaN of a part whose scores are all NaN, too
-      if (f != 0.f) {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) acc[e] += f * o[i][e];
-      }
+      for (int e = 0; e < PER; ++e) acc[e] += paged_scaled(o[i][e], f);
     }
   }
   const float inv = paged_inverse(big, sum);

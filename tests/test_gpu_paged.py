@@ -522,6 +522,19 @@ def test_attention_of_large_values_that_weigh_nothing(kernel, hq, hkv, dim, most
     assert (np.abs(got - want) <= attention_bound(want, size))[written].all()
 
 
+@pytest.mark.parametrize("kernel,hq,hkv,dim,most,requests", FORMS)
+@pytest.mark.parametrize("cut", [False, True])
+def test_attention_of_infinite_values_that_weigh_nothing(kernel, hq, hkv, dim, most, requests, cut):
+    # a weight is above 0 however small, and infinite with an infinite value: in whole tiles, in parts whose keys all
+    # weigh nothing beside the others', before and after the running maximum
+    rng = np.random.default_rng(hq + most + 2)
+    s = _form_requests(rng, hq, hkv, dim, most, requests, 1500)
+    _vanishing(rng, s, 2, [*range(600), 700, 1023, 1024, 1490 - most])
+    bounds = dict(max_query_len=most, max_kv_len=1500 if cut else 64)
+    _check_special_values(s, [(2, 0, np.inf), (2, 300, -np.inf), (2, 700, np.inf), (2, 1024, np.nan), (2, 1023, -np.inf),
+                              (1, s["kv"][1] - 1, np.inf)], **bounds)
+
+
 @pytest.mark.parametrize("rows", [1, 20])
 def test_attention_of_large_scores(rows):
     # one key far above the others, scores to +-90: the running maximum moves, nothing overflows
