@@ -230,9 +230,14 @@ AOTO_DEVICE long long paged_row(const PagedAttentionArgs& a, const int* __restri
   return (unsigned)page < (unsigned)a.pages ? page * a.page_stride + row * a.slot_stride : -1;
 }
 
-// 1 / sum of a row's weights, whose maximum is `big`: 0 where no key was seen (a row whose scores are all NaN has no
-// maximum either, but a sum of NaN).
-AOTO_DEVICE float paged_inverse(float big, float sum) { return big == -INFINITY && sum == 0.f ? 0.f : 1.f / sum; }
+// 1 / sum of a row's weights, whose maximum is `big`: 0 where no key was seen, NaN where every score is one (they have
+// no maximum, but a sum of NaN) or is -inf (kPagedNoWeight).
+AOTO_DEVICE float paged_inverse(float big, float sum) {
+  return sum == 0.f ? (big == -INFINITY ? 0.f : NAN) : 1.f / sum;
+}
+// The maximum of a row that sees keys, their scores all -inf: beside other keys it weighs nothing, but it is not that of
+// a row without keys.
+constexpr float kPagedNoWeight = -0x1.fffffep127f;
 
 AOTO_DEVICE bool bf16_pair_special(uint32_t w) {
   return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
@@ -253,6 +258,14 @@ AOTO_DEVICE uint4 chunk_finite(const uint4& v) {
 AOTO_DEVICE float special_lo(uint32_t w) { return (w & 0x7F80u) == 0x7F80u ? bf16_lo(w) : 0.f; }
 AOTO_DEVICE float special_hi(uint32_t w) { return (w & 0x7F800000u) == 0x7F800000u ? bf16_hi(w) : 0.f; }
 
+
+// Whether one of keys k0 .. limit - 1 (k0 < limit) has a page.
+AOTO_DEVICE bool paged_sees(const PagedAttentionArgs& a, const int* __restrict__ table, int k0, int limit) {
+  bool sees = false;
+#pragma unroll 1
+  for (int b = paged_block(a, k0); !sees && b * a.page < limit; ++b) sees = (unsigned)table[b] < (unsigned)a.pages;
+  return sees;
+}
 
 // The sum of the infinities and NaN among four dims of keys k0 .. limit - 1 that have a page, 0 where there are none.
 // A weight of 0 (2^-126 of the row's largest and less, and every second term of one that bf16 holds) makes a NaN of an
@@ -557,10 +570,13 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
       // a wave without keys holds zeros: 0 * 0
       v += f * *reinterpret_cast<const f32x4_t*>(&s.o[w][row][d]);
     }
-    // kept out of the way: fetched with the code around it, it took 0.2 of a small call's 7.2 us
-    if (__builtin_expect(__any(paged_any_nan(v) && sum == sum), 0))
-      v = paged_with_special(v, paged_special(a, table, a.values + kvh * a.head_stride + d, k0,
-                                              min(k1, unit.first + unit.token + row / group)));
+    // what is rare, out of the way: fetched with the code around it, it took 0.2 of a small call's 7.2 us
+    if (__builtin_expect(__any(!(fabsf(v[0] + v[1] + v[2] + v[3]) < INFINITY && sum > 0.f)), 0)) {
+      const int sees = min(k1, unit.first + unit.token + row / group);
+      if (paged_any_nan(v) && sum == sum)
+        v = paged_with_special(v, paged_special(a, table, a.values + kvh * a.head_stride + d, k0, sees));
+      if (big == -INFINITY && sum == 0.f && k0 < sees && paged_sees(a, table, k0, sees)) big = kPagedNoWeight;
+    }
     if (unit.parts > 1) {
       float* rec = paged_record(a, unit.record + unit.part, kvh, row, D);
       if (d == 0) rec[0] = big, rec[1] = sum;
@@ -1040,6 +1056,9 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
 
   const float sum = xor32_sum(run_sum);
   if (row >= live) return;
+  const bool none = run_max == -INFINITY && sum == 0.f && k0 < limit;
+  if (__builtin_expect(__any(none), 0))
+    if (none && paged_sees(a, table, k0, limit)) run_max = kPagedNoWeight;
   float probe = 0.f;  // NaN where an element of O is not finite
 #pragma unroll
   for (int d = 0; d < DT; ++d)

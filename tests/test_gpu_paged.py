@@ -535,6 +535,23 @@ def test_attention_of_infinite_values_that_weigh_nothing(kernel, hq, hkv, dim, m
                               (1, s["kv"][1] - 1, np.inf)], **bounds)
 
 
+@pytest.mark.parametrize("kernel,hq,hkv,dim,most,requests", FORMS)
+@pytest.mark.parametrize("cut", [False, True])
+def test_attention_of_scores_that_are_all_minus_infinity(kernel, hq, hkv, dim, most, requests, cut):
+    # 0 / 0 is NaN for rows that see such keys alone; beside others they weigh nothing; rows without keys are 0
+    rng = np.random.default_rng(hq + most + 3)
+    s = _form_requests(rng, hq, hkv, dim, most, requests, 1500)
+    s["q"][s["start"][1]: s["start"][3], :, 0] = -1.0
+    for r, keys in ((1, range(s["kv"][1])), (2, range(640))):
+        for j in keys:
+            s["keys"][s["tables"][r, j // 16], :, j % 16, 0] = np.inf
+    s["device"][0].copy_(to_gpu_bf16(s["keys"]))
+    s["kv"][-1] = 0
+    _check_attention_pattern(s, _form_attend(s, kernel, most, 1500, cut)[0])
+    s["tables"][1] = -1     # without pages it sees none of them
+    _check_attention(s, _form_attend(s, kernel, most, 1500, cut)[0])
+
+
 @pytest.mark.parametrize("rows", [1, 20])
 def test_attention_of_large_scores(rows):
     # one key far above the others, scores to +-90: the running maximum moves, nothing overflows
