@@ -552,6 +552,23 @@ def test_attention_of_scores_that_are_all_minus_infinity(kernel, hq, hkv, dim, m
     _check_attention(s, _form_attend(s, kernel, most, 1500, cut)[0])
 
 
+@pytest.mark.parametrize("requests", [8, 32, 33, 128, 129, 256, 257, 600])
+@pytest.mark.parametrize("most", [1, 40])        # narrow tiles; wide ones beside them
+@pytest.mark.parametrize("cut", [False, True])
+def test_attention_of_many_requests(requests, most, cut):
+    # a thread of the dealing takes a share of a request's tiles, a request, or several of them
+    rng = np.random.default_rng(requests + most)
+    rows = rng.choice([0, 1, 1, 3, most], requests)
+    rows = np.minimum(rows, most)
+    rows[-1] = most
+    kv = rows + rng.integers(0, 60, requests)
+    kv[::9] += rng.integers(0, 1300, len(kv[::9]))
+    s = _requests(rng, list(zip(rows.tolist(), kv.tolist())), 4, 1, 64, 16, tail=1, blocks=90)
+    got, joined = _form_attend(s, "d64_w" if most > 1 else "d64_n1", most, 1440, cut)
+    assert joined == (cut and (most == 1 or requests < 256))
+    _check_attention(s, got)
+
+
 @pytest.mark.parametrize("rows", [1, 20])
 def test_attention_of_large_scores(rows):
     # one key far above the others, scores to +-90: the running maximum moves, nothing overflows
