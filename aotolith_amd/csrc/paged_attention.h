@@ -5,8 +5,8 @@
 // kv_r keys, row i sees j < kv_r - n_r + i + 1 (causal) or j < kv_r, as far as the block table row goes and where its
 // entry names a page of the cache; a row that sees none gives 0. Key j of head h / (Hq / Hkv) is row j % page of page
 // block_tables[r][j / page]. Scores, maxima and sums in f32, one pass over the keys with a running maximum. P goes
-// into its product with V as bf16, the matrix instructions' operands being of one type: as two of them in 16-row tiles,
-// rounded to one otherwise (as the prefill attention does), which is off by as much as the result's own rounding.
+// into its product with V as bf16, the matrix instructions' operands being of one type: as two of them in narrow tiles,
+// rounded to one in wide tiles (as the prefill attention does), which is off by as much as the result's own rounding.
 //
 // Work is cut on the GPU, from the lengths as they are there. An item is one tile of a request's rows (all query heads of
 // a kv head that share its keys, token after token) against all the keys they see, counted in blocks of 128 keys. With
@@ -326,9 +326,9 @@ struct PagedNarrowShared {
 template <int D, int NT>
 AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit, int kvh, PagedNarrowShared<D, NT>& s) {
   constexpr int DC = D / 32, DT = D / 16, STR = PagedNarrowShared<D, NT>::STR;
-  // P keeps 16 bits, as its upper half cut off and the rest rounded: two products, which cost nothing here (16 rows:
-  // 78.7 us with and without for 32 requests' 88000 keys). With 32 rows they cost 7%, and P is rounded to bf16.
-  constexpr bool TWO = NT == 1;
+  // P keeps 16 bits, as its upper half cut off and the rest rounded: two products, which cost nothing with 16 rows (78.7
+  // us with and without for 32 requests' 88000 keys) and 4% with 32 (16 requests' five rows 44.5 us, 42.7 rounded to bf16:
+  // a single token may run in either tile, by the bound its caller gives).
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
   const int group = a.query_heads / a.kv_heads;
@@ -501,13 +501,8 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
       uint32_t high[4], low[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if constexpr (TWO) {
-          high[j] = __builtin_amdgcn_perm(__float_as_uint(p[2 * j + 1]), __float_as_uint(p[2 * j]), 0x07060302u);
-          low[j] = cvt_pk_bf16(p[2 * j] - bf16_lo(high[j]), p[2 * j + 1] - bf16_hi(high[j]));
-        } else {
-          high[j] = cvt_pk_bf16(p[2 * j], p[2 * j + 1]);
-          low[j] = 0;
-        }
+        high[j] = __builtin_amdgcn_perm(__float_as_uint(p[2 * j + 1]), __float_as_uint(p[2 * j]), 0x07060302u);
+        low[j] = cvt_pk_bf16(p[2 * j] - bf16_lo(high[j]), p[2 * j + 1] - bf16_hi(high[j]));
       }
       pb[t] = __builtin_bit_cast(fa_bf16x8, high);
       pr[t] = __builtin_bit_cast(fa_bf16x8, low);
@@ -521,8 +516,7 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(fa_bf16x8, both), pb[t], o[t][d], 0, 0, 0);
-        if constexpr (TWO)
-          o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(fa_bf16x8, both), pr[t], o[t][d], 0, 0, 0);
+        o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(fa_bf16x8, both), pr[t], o[t][d], 0, 0, 0);
       }
     }
     while (special) {

@@ -569,6 +569,32 @@ def test_attention_of_many_requests(requests, most, cut):
     _check_attention(s, got)
 
 
+def narrow_bound(want, size):
+    # a weight is its upper 8 bits and what they leave, less than 2^-7 of it, rounded to bf16: off by 2^-7 HALF, and by
+    # as much of sum p |v|; the sum is of the weights as they were, the result is rounded once, and f32 adds what it
+    # does in _check_attention
+    return HALF * (1 + HALF) * np.abs(want) + (1 + HALF) * (2.0 ** -7 * HALF + 4e-5) * size
+
+
+@pytest.mark.parametrize("hq,hkv,dim", [h for h in HEADS if h[0] // h[1] <= 16])
+@pytest.mark.parametrize("most", [1, 200])       # narrow tiles alone, and beside wide ones
+def test_attention_of_single_tokens_keeps_16_bits_of_the_weights(hq, hkv, dim, most):
+    rng = np.random.default_rng(hq * dim + most)
+    s = _requests(rng, [(1, 1), (1, 2), (0, 9), (1, 16), (1, 129), (1, 700), (1, 1500)], hq, hkv, dim, 16, tail=2)
+    got = from_gpu_bf16(_attend(s, max_query_len=most)).astype(np.float64)
+    want, size, written = oracle.attention(s["q"], s["keys"], s["values"], s["tables"], s["start"], s["kv"])
+    assert (np.abs(got - want) <= narrow_bound(want, size))[written].all()
+
+
+@pytest.mark.parametrize("hq,hkv,dim", [(8, 2, 64), (8, 2, 128), (16, 4, 128)])
+def test_attention_of_drafted_rows_keeps_16_bits_of_the_weights(hq, hkv, dim):
+    rng = np.random.default_rng(hq * dim)
+    s = _requests(rng, [(5, 5), (8, 40), (0, 9), (1, 16), (7, 129), (8, 700), (3, 1500)], hq, hkv, dim, 16, tail=2)
+    got = from_gpu_bf16(_attend(s, max_query_len=8)).astype(np.float64)
+    want, size, written = oracle.attention(s["q"], s["keys"], s["values"], s["tables"], s["start"], s["kv"])
+    assert (np.abs(got - want) <= narrow_bound(want, size))[written].all()
+
+
 @pytest.mark.parametrize("rows", [1, 20])
 def test_attention_of_large_scores(rows):
     # one key far above the others, scores to +-90: the running maximum moves, nothing overflows
