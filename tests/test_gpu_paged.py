@@ -737,6 +737,27 @@ def test_verify_of_ragged_drafts(dtype, vocab, with_law):
     _check_verify(*drafts, np.linspace(0.05, 4, 8))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [262143, 262144, 262145, 300001, 600000])
+@pytest.mark.parametrize("with_law", [False, True])
+def test_verify_of_large_vocabularies(dtype, vocab, with_law):
+    # more chunks than a wave keeps in registers; laws whose weight is all behind them, a drafted token among it
+    rng = np.random.default_rng(vocab)
+    start, logits, host, tokens, law, law_host, uniforms = _drafted(rng, [2, 0, 1, 2], 2, vocab, dtype, with_law)
+    behind = min(262144, vocab - 1)
+    for t in (logits[1], logits[3], logits[4:6], *(() if law is None else (law[0], law[2]))):
+        t[..., :behind] -= 40.0
+    tokens[0, 0], tokens[2, 0] = vocab - 1, behind
+    if with_law:                    # both fall: the draft is all but sure of them
+        law[0, 0, vocab - 1], law[2, 0, behind] = 60.0, 60.0
+        law_host = _np(law.float())
+    host = _np(logits.float())
+    for row in (uniforms, np.full_like(uniforms, 1 - 2.0 ** -24), np.full_like(uniforms, 0.5)):
+        state = start, logits, host, tokens, law, law_host, row
+        _check_verify(*state, [1.0, 0.7, 1.3, 0.0])
+    _check_verify(*state, None)
+
+
 @pytest.mark.parametrize("drafts", [0, 1, 5, 62])
 @pytest.mark.parametrize("with_law", [False, True])
 def test_verify_of_any_number_of_drafts(drafts, with_law):
