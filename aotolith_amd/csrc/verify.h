@@ -7,9 +7,9 @@
 // at which the running sum of weights passes u_last times their total. T <= 0: a draft stands where it is the row's
 // first maximum, which is also the token that follows.
 //
-// All of it is held in 64 bits, the exponentials too: a token is where a sum over the vocabulary passes a random
-// number, and the sums' noise in 32 bits (1e-7 of the total, against a typical weight of 1e-5 to 1e-6 of it) would
-// move it in a percent of the calls.
+// All of it is held in 64 bits, the exponentials too (right to 3e-15 of themselves, exp2.h): a token is where a sum over
+// the vocabulary passes a random number, and the sums' noise in 32 bits (1e-7 of the total, against a typical weight of
+// 1e-5 to 1e-6 of it) would move it in a percent of the calls.
 //
 // Launches over chunks of kVerifyChunk tokens: every row's maximum, its place and sum of weights by chunk; with a draft
 // model's logits, what stands and the weights the following token is drawn from, summed by chunk; the token.
@@ -22,6 +22,7 @@
 #pragma once
 
 #include "common.h"
+#include "exp2.h"
 #include "paged_args.h"
 
 namespace aoto {
@@ -41,44 +42,7 @@ struct VerifyTable {
   double at[32];
 };
 AOTO_DEVICE void verify_table(VerifyTable& table) {
-  if (threadIdx.x < 32) {
-    // the series of e^y, 0 <= y < ln 2, to the 20th power (remainder 1e-23)
-    const double y = threadIdx.x * (0.6931471805599453094 / 32);
-    double s = 1.0;
-#pragma unroll
-    for (int k = 20; k > 0; --k) s = fma(s, y * (1.0 / k), 1.0);
-    table.at[threadIdx.x] = s;
-  }
-}
-
-// 2^x, x = d * heat32 / 32, for -2048 < x <= 0 (0 from 2^-1075 on): 32 x is rounded to a whole number k by a sum with
-// 1.5 * 2^52, whose low bits are k; what is left, f = 32 x - k in one rounding, |f| <= 1/2, goes through the series of
-// e^(f ln 2 / 32) to the 5th power (remainder below (ln 2 / 64)^6 / 6! = 2.3e-15), k mod 32 through the table, the rest
-// of k to the exponent.
-struct VerifyPower {
-  double series;
-  int k;
-};
-AOTO_DEVICE VerifyPower exp2_parts(double d, double heat32) {
-  constexpr double kRound = 6755399441055744.0;
-  const double t = fma(d, heat32, kRound);
-  const double f = fma(d, heat32, kRound - t);
-  double s = 3.973709984549416e-11;  // (ln 2 / 32)^5 / 5!, and on to the 0th
-  s = fma(s, f, 9.172562701824643e-09);
-  s = fma(s, f, 1.693850972437182e-06);
-  s = fma(s, f, 0.0002345961982022468);
-  s = fma(s, f, 0.02166084939249829);
-  return {fma(s, f, 1.0), __double2loint(t)};
-}
-AOTO_DEVICE double exp2_of(double d, double heat32, const VerifyTable& table) {
-  const VerifyPower p = exp2_parts(d, heat32);
-  return ldexp(p.series * table.at[p.k & 31], p.k >> 5);
-}
-// sum + 2^x for x > -1000: the exponent goes into the table's number by whole-number arithmetic.
-AOTO_DEVICE double exp2_added(double d, double heat32, const VerifyTable& table, double sum) {
-  const VerifyPower p = exp2_parts(d, heat32);
-  const double scale = table.at[p.k & 31];
-  return fma(p.series, __hiloint2double(__double2hiint(scale) + ((p.k >> 5) << 20), __double2loint(scale)), sum);
+  if (threadIdx.x < 32) table.at[threadIdx.x] = exp2_32nds(threadIdx.x);
 }
 
 // A request's temperature: 32 log2(e) / T and its inverse; heat32 < 0: greedy.
@@ -108,12 +72,12 @@ struct VerifyScale {
   }
   AOTO_DEVICE double operator()(float z) const { return plain ? quick(z) : careful(z); }
   AOTO_DEVICE double quick(float z) const {
-    return exp2_of((double)fmaxf(z, floor) - top, heat32, table);  // fmaxf: a NaN gives the floor
+    return exp2_of((double)fmaxf(z, floor) - top, heat32, table.at);  // fmaxf: a NaN gives the floor
   }
   AOTO_DEVICE double careful(float z) const {
     if (!(z > -INFINITY)) return 0.0;
     if ((double)z == top) return 1.0;
-    return top == INFINITY ? 0.0 : exp2_of(fmax(((double)z - top) * heat32, -64000.0), 1.0, table);
+    return top == INFINITY ? 0.0 : exp2_of(fmax(((double)z - top) * heat32, -64000.0), 1.0, table.at);
   }
 };
 
@@ -283,7 +247,7 @@ __device__ void verify_stats(const VerifyArgs& a) {
         held.get(l, z);
 #pragma unroll
         for (int e = 0; e < Held::EACH; ++e)
-          sum = exp2_added((double)fmaxf(z[e], weight.floor) - weight.top, heat.heat32, table, sum);
+          sum = exp2_added((double)fmaxf(z[e], weight.floor) - weight.top, heat.heat32, table.at, sum);
       }
     } else if (top > -INFINITY) {
 #pragma unroll

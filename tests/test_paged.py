@@ -5,6 +5,9 @@ from __future__ import annotations
 
 import ctypes
 import math
+import os
+import shutil
+import subprocess
 
 import numpy as np
 import pytest
@@ -165,3 +168,64 @@ def test_exponential_series_is_exact_to_the_last_bits():
     exact = np.exp2(x.astype(np.longdouble)).astype(np.float64)
     assert np.all(np.abs(got - exact) <= 4 * 2.0 ** -53 * exact)
     assert got[-1] == 0.0  # what weighs less than any number weighs nothing
+
+
+# ---------------------------------------------------------------- the verification's exponential, as the kernels have it
+_EXP2 = r"""
+#include <cmath>
+#include <cstdint>
+#include <cstring>
+using std::fma; using std::ldexp;
+#define AOTO_DEVICE static inline
+static inline uint64_t bits(double v) { uint64_t b; std::memcpy(&b, &v, 8); return b; }
+static inline int __double2loint(double v) { return (int)(uint32_t)bits(v); }
+static inline int __double2hiint(double v) { return (int)(uint32_t)(bits(v) >> 32); }
+static inline double __hiloint2double(int hi, int lo) {
+  const uint64_t b = (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo;
+  double v;
+  std::memcpy(&v, &b, 8);
+  return v;
+}
+#include "exp2.h"
+extern "C" void powers(const double* d, double heat32, int n, double* of, double* added, double* table) {
+  for (int j = 0; j < 32; ++j) table[j] = aoto::exp2_32nds(j);
+  for (int i = 0; i < n; ++i) of[i] = aoto::exp2_of(d[i], heat32, table);
+  for (int i = 0; i < n; ++i) added[i] = aoto::exp2_added(d[i], heat32, table, 0.0);
+}
+"""
+
+
+@pytest.mark.parametrize("heat32", [32.0, 32 * math.log2(math.e), 32 * math.log2(math.e) / 0.7, 1e-3, 3e5])
+def test_exponentials_of_the_verification(tmp_path, heat32):
+    """``csrc/exp2.h`` compiled for the host: 2^(d heat32 / 32) within 27 steps of 2^-53.
+
+    The series' remainder is (ln 2 / 64)^6 / 6! = 2.24e-15 = 20.2 steps, over e^f >= 0.989 20.4. A table entry is off by
+    3: its y by 2 roundings of up to 0.69, its last two products and sums by 1 + 0.4, the others by less than 0.2. The
+    series' last sum and the product of the two are a rounding each; its other terms, of a factor of 0.011, 0.1; f, once
+    rounded at 1/2, 0.02. The exact value's own rounding here adds half a step: 20.4 + 3 + 2 + 0.12 + 0.5 < 27.
+    """
+
+    compiler = shutil.which("g++") or shutil.which("c++")
+    if compiler is None:
+        pytest.skip("no host compiler")
+    (tmp_path / "powers.cpp").write_text(_EXP2)
+    include = os.path.join(os.path.dirname(ops.__file__), "csrc")
+    subprocess.run([compiler, "-O1", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared", "-I" + include,
+                    str(tmp_path / "powers.cpp"), "-o", str(tmp_path / "powers.so")], check=True)
+    rng = np.random.default_rng(0)
+    x = -np.concatenate([np.linspace(0, 60, 40001), np.linspace(0, 2, 20001), rng.random(40000) * 999, [0.0, 1.0, 999.9]])
+    d = x * 32 / heat32
+    of, added, table = np.empty_like(d), np.empty_like(d), np.empty(32)
+    pointer = ctypes.POINTER(ctypes.c_double)
+    powers = ctypes.CDLL(str(tmp_path / "powers.so")).powers
+    powers.argtypes = [pointer, ctypes.c_double, ctypes.c_int, pointer, pointer, pointer]
+    powers(*(v.ctypes.data_as(pointer) if isinstance(v, np.ndarray) else v for v in (d, heat32, len(d), of, added, table)))
+    exact = np.exp2(d.astype(np.longdouble) * np.longdouble(heat32) / 32).astype(np.float64)
+    step = 2.0 ** -53
+    assert (np.abs(of - exact) <= 27 * step * exact).all()
+    assert (np.abs(added - exact) <= 27 * step * exact).all()
+    entries = np.exp2(np.arange(32, dtype=np.longdouble) / 32).astype(np.float64)
+    assert (np.abs(table - entries) <= 3.5 * step * entries).all()
+    low = np.array([-1100.0, -2000.0]) * 32 / heat32      # where the floors of the weights lie: nothing
+    powers(*(v.ctypes.data_as(pointer) if isinstance(v, np.ndarray) else v for v in (low, heat32, 2, of, added, table)))
+    assert (of[:2] == 0.0).all()
