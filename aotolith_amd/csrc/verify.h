@@ -459,6 +459,7 @@ __device__ void verify_keep(const VerifyArgs& a) {
 // requests' chunk sums are those of the statistics, less a removed token's weight.)
 template <bool F32>
 __device__ void verify_mass(const VerifyArgs& a) {
+  static_assert(kVerifyChunk == 8 * 256, "a chunk is eight tokens a thread");
   __shared__ VerifyTable table;
   __shared__ double s_sum[4];
   const int r = blockIdx.y;
@@ -467,9 +468,9 @@ __device__ void verify_mass(const VerifyArgs& a) {
   verify_table(table);
   __syncthreads();
   const int begin = blockIdx.x * kVerifyChunk, end = min(a.vocab, begin + kVerifyChunk);
+  const int v = begin + 8 * threadIdx.x;
   double sum = 0.0;
-#pragma unroll 1
-  for (int v = begin + 8 * threadIdx.x; v < end; v += 2048) {
+  if (v < end) {
     double whole[8], left[8];
     verify_left<F32>(law, table, v, end, whole, left);
 #pragma unroll
