@@ -159,7 +159,7 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
     return set_error(AOTO_ERR_ARGUMENT, "paged_attention: q and out 16-byte aligned, strides of multiples of 8");
   if ((long long)max_blocks * page > (1 << 28))
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention: block tables of more than 2^28 keys");
-  if (page_stride < 0 || page_stride > 0xFFFFFFFFLL || slot_stride < 0 || slot_stride * page > 0x3FFFFFFFLL)
+  if (page_stride < 0 || page_stride > 0xFFFFFFFFLL || slot_stride < 0 || slot_stride > 0x3FFFFFFFLL / page)
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention: pages of more than 2^32 elements, or rows 2^30 apart");
   if (!(scale > 0.f) || !std::isfinite(scale))
     return set_error(AOTO_ERR_ARGUMENT, "paged_attention: scale %g is not a positive number", (double)scale);

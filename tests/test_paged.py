@@ -80,6 +80,22 @@ def test_attention_refuses(changes, code):
     _refused(_attention(**changes), code, "paged_attention")
 
 
+@pytest.mark.parametrize("changes,code", [
+    *[(dict(scale=v), 1) for v in (0.0, -0.125, math.inf, math.nan)],
+    (dict(page_stride=2 ** 32), 4), (dict(page_stride=-2048), 4), (dict(slot_stride=2 ** 26), 4),
+    (dict(slot_stride=-64), 4), (dict(slot_stride=2 ** 60), 4), (dict(slot_stride=2 ** 62), 4),  # page times it wraps
+    (dict(blocks=2 ** 24 + 1, stride=2 ** 25), 4), (dict(heads=129, kv_heads=1), 4)])
+def test_attention_refuses_what_its_addresses_do_not_reach(changes, code):
+    _refused(_attention(**changes), code, "paged_attention")
+
+
+@pytest.mark.parametrize("changes", [
+    dict(requests=21846), dict(requests=13108, law=GOOD), dict(requests=65536, drafts=0)])
+def test_verify_refuses_more_rows_than_a_launch_has(changes):
+    # requests * (drafts + 1), with a draft model's logits requests * (2 drafts + 1): 65536 and more
+    _refused(_verify(**changes), _lib.AOTO_ERR_UNSUPPORTED, "requests of")
+
+
 def _verify(**changes):
     a = dict(logits=GOOD, f32=0, row=1000, rows=9, vocab=1000, drafts_in=GOOD, law=None, law_request=0, law_row=0,
              start=GOOD, uniforms=GOOD, temperature=GOOD, requests=3, drafts=2, workspace=GOOD, out=GOOD,
