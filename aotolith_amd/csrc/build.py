@@ -61,8 +61,8 @@ def build(verbose: bool = False) -> tuple[str, str]:
     _run([HIPCC, *DEVICE_FLAGS, "--genco", "--no-gpu-bundle-output", os.path.join(CSRC, "kernels.hip"), "-o", tmp_obj], verbose)
     os.replace(tmp_obj, CODE_OBJECT)
     tmp_lib = LIBRARY + ".tmp"
-    # The host library: the C-ABI launchers (paged.cpp: those over the paged cache), plus noalloc.hip, whose device part is
-    # only the static scratch buffer of the allocation-free GEMM entry point.
+    # The host library: the C-ABI launchers (paged.cpp: those over the paged cache), plus noalloc.hip, whose device
+    # part is only the static scratch buffer of the allocation-free GEMM entry point.
     _run(
         [
             HIPCC,

@@ -61,7 +61,8 @@ AttentionPlan attention_plan(int tokens, int requests, int max_blocks, int page,
   // Not worth the join: narrow tiles of up to 256 keys, wide ones of up to 1024 (512 tokens over themselves: 28 us
   // whole and 35 cut at 128 dims, 19.5 and 24 at 64), wide ones that give every CU a block (32 / 8 heads of 128, 1024
   // tokens over 1 / 1000 / 4000 keys before them: 41 / 62 / 127 us whole, 56 / 76 / 128 cut; 14 / 2 heads of 64, 4096
-  // over 2000 / 6000: 113 / 191 and 153 / 231).
+  // over 2000 / 6000: 113 / 191 and 153 / 231). Those are tiles of equal length; the count says nothing of lengths, so
+  // where it ends the cutting (256 single tokens of 8 kv heads, say) one request far longer than the rest ends late.
   if (keys > (p.wide_rows ? 1024 : 256) && 2 * p.units * kv_heads < (p.wide_rows ? 1 : 8) * full &&
       p.units * most < (1 << 30)) {
     p.target = (int)((full + kv_heads - 1) / kv_heads);
@@ -90,7 +91,8 @@ int aoto_hip_paged_tables(const int32_t* context_lens, const int32_t* new_lens, 
   if (requests <= 0 || max_blocks <= 0 || free_count < 0 || page <= 0 || max_tokens < 0 || table_stride < max_blocks)
     return set_error(AOTO_ERR_ARGUMENT, "paged_tables: bad shape");
   if (max_blocks > (1 << 20) || page > (1 << 20) || max_tokens >= (1 << 30))
-    return set_error(AOTO_ERR_UNSUPPORTED, "paged_tables: at most 2^20 blocks a request and tokens a page, 2^30 - 1 rows");
+    return set_error(AOTO_ERR_UNSUPPORTED,
+                     "paged_tables: at most 2^20 blocks a request and tokens a page, 2^30 - 1 rows");
   PagedTablesArgs a{};
   a.context_lens = context_lens, a.new_lens = new_lens, a.block_tables = block_tables, a.page_counts = page_counts;
   a.free_pages = free_pages, a.free_start = free_start, a.query_start = query_start, a.kv_lens = kv_lens;
@@ -112,7 +114,8 @@ int aoto_hip_paged_rope_append(const void* qkv, int64_t row_stride, const int64_
                                void* stream) {
   if (!qkv || !positions || !slots || !cos_table || !sin_table || !q_out)
     return set_error(AOTO_ERR_ARGUMENT, "paged_rope_append: null pointer");
-  if (int s = check_pages("paged_rope_append", keys, values, page_stride, head_stride, slot_stride, pages, page)) return s;
+  if (int s = check_pages("paged_rope_append", keys, values, page_stride, head_stride, slot_stride, pages, page))
+    return s;
   if (tokens <= 0 || query_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || table_rows <= 0)
     return set_error(AOTO_ERR_ARGUMENT, "paged_rope_append: bad shape");
   if (head_dim % 16)
@@ -149,7 +152,8 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
                              int max_kv_len, void* workspace, void* out, void* stream) {
   if (!q || !block_tables || !query_start || !kv_lens || !out)
     return set_error(AOTO_ERR_ARGUMENT, "paged_attention: null pointer");
-  if (int s = check_pages("paged_attention", keys, values, page_stride, head_stride, slot_stride, pages, page)) return s;
+  if (int s = check_pages("paged_attention", keys, values, page_stride, head_stride, slot_stride, pages, page))
+    return s;
   if (tokens <= 0 || requests <= 0 || max_blocks <= 0 || query_heads <= 0 || kv_heads <= 0 ||
       query_heads % kv_heads || table_stride < max_blocks || max_query_len < 0 || max_kv_len < 0)
     return set_error(AOTO_ERR_ARGUMENT, "paged_attention: bad shape");
@@ -169,7 +173,8 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
   const AttentionPlan plan = attention_plan(tokens, requests, max_blocks, page, query_heads, kv_heads, head_dim,
                                             max_query_len, max_kv_len);
   if (plan.workspace && (!workspace || !aligned(workspace, 16)))
-    return set_error(AOTO_ERR_ARGUMENT, "paged_attention: needs a 16-byte aligned workspace of %zu bytes", plan.workspace);
+    return set_error(AOTO_ERR_ARGUMENT, "paged_attention: needs a 16-byte aligned workspace of %zu bytes",
+                     plan.workspace);
   PagedAttentionArgs a{};
   a.q = static_cast<const uint16_t*>(q), a.keys = static_cast<const uint16_t*>(keys);
   a.values = static_cast<const uint16_t*>(values), a.block_tables = block_tables, a.query_start = query_start;
@@ -200,7 +205,8 @@ int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_he
 size_t aoto_hip_verify_draft_workspace(int requests, int drafts, int vocab) {
   if (requests <= 0 || drafts < 0 || vocab <= 0) return 0;
   const size_t chunks = ((size_t)vocab + kVerifyChunk - 1) / kVerifyChunk;
-  return (size_t)requests * (chunks * ((2 * (size_t)drafts + 1) * kVerifyChunkBytes + sizeof(double)) + kVerifyLawBytes);
+  return (size_t)requests *
+         (chunks * ((2 * (size_t)drafts + 1) * kVerifyChunkBytes + sizeof(double)) + kVerifyLawBytes);
 }
 
 int aoto_hip_verify_draft(const void* logits, int logits_f32, int64_t row_stride, int rows, int vocab,
@@ -232,11 +238,14 @@ int aoto_hip_verify_draft(const void* logits, int logits_f32, int64_t row_stride
                      (long long)requests * a.judged, 256, stream, a))
     return s;
   if (!temperature || !a.draft_logits)
-    return launch(logits_f32 ? "aoto_verify_follow_f32" : "aoto_verify_follow_bf16", requests, 1, kVerifyChunk / 8, stream, a);
-  if (int s = launch(logits_f32 ? "aoto_verify_law_f32" : "aoto_verify_law_bf16", requests, 1, 256, stream, a)) return s;
+    return launch(logits_f32 ? "aoto_verify_follow_f32" : "aoto_verify_follow_bf16", requests, 1, kVerifyChunk / 8,
+                  stream, a);
+  if (int s = launch(logits_f32 ? "aoto_verify_law_f32" : "aoto_verify_law_bf16", requests, 1, 256, stream, a))
+    return s;
   if (int s = launch(logits_f32 ? "aoto_verify_mass_f32" : "aoto_verify_mass_bf16", a.chunks, requests, 256, stream, a))
     return s;
-  return launch(logits_f32 ? "aoto_verify_pick_f32" : "aoto_verify_pick_bf16", requests, 1, kVerifyChunk / 8, stream, a);
+  return launch(logits_f32 ? "aoto_verify_pick_f32" : "aoto_verify_pick_bf16", requests, 1, kVerifyChunk / 8, stream,
+                a);
 }
 
 }  // extern "C"

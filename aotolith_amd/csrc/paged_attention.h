@@ -8,13 +8,18 @@
 // into its product with V as bf16, the matrix instructions' operands being of one type: as two of them in narrow tiles,
 // rounded to one in wide tiles (as the prefill attention does), which is off by as much as the result's own rounding.
 //
-// Work is cut on the GPU, from the lengths as they are there. An item is one tile of a request's rows (all query heads of
-// a kv head that share its keys, token after token) against all the keys they see, counted in blocks of 128 keys. With
-// `target` blocks a kv head, the items' key blocks, one item after the other, are dealt out evenly: every GPU block
-// takes the same number of them, wherever that begins and ends, so that requests of very different lengths end together
-// (an item cut among several leaves records, maximum, sum and unnormalized row, that aoto_paged_attention_join_*
-// combines). Without a target every GPU block takes one item. A GPU block finds its place by running sums over the
-// requests.
+// NaN and infinities are the softmax's, in every tile and however an item is cut: a NaN score or one of +inf makes its
+// row NaN, scores of -inf weigh nothing beside others and give NaN alone, a NaN or infinite value that a row sees is in
+// its dim of the row however small its weight (one that f32 or a score of -inf makes 0, too), and what a row does not
+// see weighs exactly 0 and leaves nothing.
+//
+// Work is cut on the GPU, from the lengths as they are there. An item is one tile of a request's rows (all query heads
+// of a kv head that share its keys, token after token) against all the keys they see, counted in blocks of 128 keys.
+// With `target` blocks a kv head, the items' key blocks, one item after the other, are dealt out evenly: every GPU
+// block takes the same number of them, wherever that begins and ends, so that requests of very different lengths end
+// together (an item cut among several leaves records, maximum, sum and unnormalized row, that
+// aoto_paged_attention_join_* combines). Without a target, where the host counts tiles enough for the chip, every GPU
+// block takes one item, and the longest ends last. A GPU block finds its place by running sums over the requests.
 //   narrow tiles (16 NT rows, decodes and drafted tokens): the four waves take 32 keys each of every 128; K goes
 //     straight from the pages to operand registers, V through the wave's own LDS; no barrier in the loop
 //   wide tiles (128 rows, chunks of prompts): the four waves take 32 rows each, 64-key tiles of K and V staged once for
@@ -72,7 +77,8 @@ AOTO_DEVICE PagedRequest paged_request(const PagedAttentionArgs& a, int r) {
   return q;
 }
 
-// Keys that the rows of a tile see, and the blocks of them (one where there are none: the rows are written all the same).
+// Keys that the rows of a tile see, and the blocks of them (one where there are none: the rows are written all the
+// same).
 AOTO_DEVICE int paged_tile_keys(const PagedRequest& q, int tile) {
   return min(q.keys, max(0, q.first + min(q.rows, (tile + 1) * q.tokens) - 1));
 }
@@ -235,8 +241,8 @@ AOTO_DEVICE long long paged_row(const PagedAttentionArgs& a, const int* __restri
 AOTO_DEVICE float paged_inverse(float big, float sum) {
   return sum == 0.f ? (big == -INFINITY ? 0.f : NAN) : 1.f / sum;
 }
-// The maximum of a row that sees keys, their scores all -inf: beside other keys it weighs nothing, but it is not that of
-// a row without keys.
+// The maximum of a row that sees keys, their scores all -inf: beside other keys it weighs nothing, but it is not that
+// of a row without keys.
 constexpr float kPagedNoWeight = -0x1.fffffep127f;
 
 AOTO_DEVICE bool bf16_pair_special(uint32_t w) {
@@ -284,7 +290,9 @@ AOTO_DEVICE f32x4_t paged_special(const PagedAttentionArgs& a, const int* __rest
   }
   return sum;
 }
-AOTO_DEVICE bool paged_any_nan(const f32x4_t& v) { return v[0] != v[0] || v[1] != v[1] || v[2] != v[2] || v[3] != v[3]; }
+AOTO_DEVICE bool paged_any_nan(const f32x4_t& v) {
+  return v[0] != v[0] || v[1] != v[1] || v[2] != v[2] || v[3] != v[3];
+}
 // v with the sums of special values (not 0 where there are some) in the place of its NaN.
 AOTO_DEVICE f32x4_t paged_with_special(f32x4_t v, const f32x4_t& special) {
 #pragma unroll
@@ -324,11 +332,12 @@ struct PagedNarrowShared {
 // Bound by the read of K and V: 88000 keys of 32 requests, 8 kv heads of 128, in 72 us, 5.0 TB/s. Each wave keeps a
 // tile's K and V on their way while it works on the one before, and waits for nobody.
 template <int D, int NT>
-AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit, int kvh, PagedNarrowShared<D, NT>& s) {
+AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit, int kvh,
+                              PagedNarrowShared<D, NT>& s) {
   constexpr int DC = D / 32, DT = D / 16, STR = PagedNarrowShared<D, NT>::STR;
-  // P keeps 16 bits, as its upper half cut off and the rest rounded: two products, which cost nothing with 16 rows (78.7
-  // us with and without for 32 requests' 88000 keys) and 4% with 32 (16 requests' five rows 44.5 us, 42.7 rounded to bf16:
-  // a single token may run in either tile, by the bound its caller gives).
+  // P keeps 16 bits, as its upper half cut off and the rest rounded: two products, which cost nothing with 16 rows
+  // (78.7 us with and without for 32 requests' 88000 keys) and 4% with 32 (16 requests' five rows 44.5 us, 42.7 rounded
+  // to bf16: a single token may run in either tile, by the bound its caller gives).
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
   const int group = a.query_heads / a.kv_heads;
@@ -608,8 +617,8 @@ AOTO_DEVICE void paged_landed() {
   asm volatile("" ::: "memory");
 }
 
-// Changes of an accumulator that the tile loop makes seldom, in place: as plain arithmetic they make the compiler hold O
-// in the ordinary registers and move all of it (128 registers) to the accumulation registers and back in every tile.
+// Changes of an accumulator that the tile loop makes seldom, in place: as plain arithmetic they make the compiler hold
+// O in the ordinary registers and move all of it (128 registers) to the accumulation registers and back in every tile.
 // It does not see that these read what products wrote, so acc_settle() stands before the first and after the last: the
 // 64 cycles that a product's result takes, with room.
 AOTO_DEVICE void acc_scale(float& x, float by) {
@@ -757,7 +766,8 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   // Operands: byte addresses in a tile, XORed with a constant per 16 (K) or 32 (V) dims.
   const uint32_t lds_k = lds_k0 + col * ROWB + ((half ^ swizzle(col)) << 4);
   const int r = lane & 15, v_row = 4 * half + (r >> 2);
-  const uint32_t lds_v = lds_v0 + v_row * ROWB + (((2 * (lane >> 4 & 1) + (r & 3) / 2) ^ swizzle(v_row)) << 4) + (r & 1) * 8;
+  const uint32_t lds_v =
+      lds_v0 + v_row * ROWB + (((2 * (lane >> 4 & 1) + (r & 3) / 2) ^ swizzle(v_row)) << 4) + (r & 1) * 8;
   auto read_k = [&](uint32_t base, int d) { return *(const paged_lds_bf16x8*)(uintptr_t)(base ^ (d << 5)); };
   auto read_v = [&](uint32_t base, int kt, int d) {  // keys 16 kt .. of the tile
     const pa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4*)((base ^ (d << 6)) + kt * (16 * ROWB)));
@@ -942,8 +952,8 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
   };
 
   // At tile t: K of tile t's second half and of tile t + 1 and V of tile t are in LDS, the scores of tile t's first 32
-  // keys in sc; K of tile t + 2 goes to the two free slots and V of tile t + 1 to the buffer of tile t - 1 while it runs,
-  // and the rows of tile t + 3 are looked up.
+  // keys in sc; K of tile t + 2 goes to the two free slots and V of tile t + 1 to the buffer of tile t - 1 while it
+  // runs, and the rows of tile t + 3 are looked up.
   long long at_k[LOADS], at_v[LOADS];
   if (tiles > 0) {
     int now[LOADS], then[LOADS];
@@ -1129,8 +1139,9 @@ __device__ void paged_attention_mixed(const PagedAttentionArgs& a) {
   }
 }
 
-// A wave joins the parts of one row (32 to 80 tokens of 32 heads: 5 us with its launch): with m the largest maximum, out = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s. Bound
-// by latency: the note, then eight records at a time in one round trip.
+// A wave joins the parts of one row (32 to 80 tokens of 32 heads: 5 us with its launch): with m the largest maximum,
+// out = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s. Bound by latency: the note, then eight records at a time in one
+// round trip.
 template <int D>
 __device__ void paged_attention_join(const PagedAttentionArgs& a) {
   constexpr int PER = D / 64, SOME = 8;
@@ -1140,7 +1151,8 @@ __device__ void paged_attention_join(const PagedAttentionArgs& a) {
   const int4 note = reinterpret_cast<const int4*>(a.joins)[t];
   if (t < a.query_start[0] || t >= a.query_start[a.requests] || note.y <= 1) return;
   // no note where query_start decreases
-  if (note.x < 0 || note.y > a.units || note.x > a.units - note.y || (unsigned)note.z >= (unsigned)a.record_rows) return;
+  if (note.x < 0 || note.y > a.units || note.x > a.units - note.y || (unsigned)note.z >= (unsigned)a.record_rows)
+    return;
   const int group = a.query_heads / a.kv_heads, kvh = h / group, at = note.z + h % group;
   const size_t step = (size_t)a.kv_heads * a.record_rows * (D + 2);
   const float* rec = paged_record(a, note.x, kvh, at, D);

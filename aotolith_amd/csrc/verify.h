@@ -7,9 +7,9 @@
 // at which the running sum of weights passes u_last times their total. T <= 0: a draft stands where it is the row's
 // first maximum, which is also the token that follows.
 //
-// All of it is held in 64 bits, the exponentials too (right to 3e-15 of themselves, exp2.h): a token is where a sum over
-// the vocabulary passes a random number, and the sums' noise in 32 bits (1e-7 of the total, against a typical weight of
-// 1e-5 to 1e-6 of it) would move it in a percent of the calls.
+// All of it is held in 64 bits, the exponentials too (right to 3e-15 of themselves, exp2.h): a token is where a sum
+// over the vocabulary passes a random number, and the sums' noise in 32 bits (1e-7 of the total, against a typical
+// weight of 1e-5 to 1e-6 of it) would move it in a percent of the calls.
 //
 // Launches over chunks of kVerifyChunk tokens: every row's maximum, its place and sum of weights by chunk; with a draft
 // model's logits, what stands and the weights the following token is drawn from, summed by chunk; the token.

@@ -55,7 +55,7 @@ def rope(x, cos, sin):
 
 
 def attention(q, keys, values, block_tables, query_start, kv_lens, causal=True, scale=None):
-    """``(out [T, Hq * D], sum_j p_j |v_j| of the same shape, rows written [T])``; keys, values ``[P, Hkv, page, D]``."""
+    """``(out [T, Hq * D], sum_j p_j |v_j|, rows written [T])``; keys, values ``[P, Hkv, page, D]``."""
 
     tokens, heads, dim = q.shape
     pages, kv_heads, page, _ = keys.shape
