@@ -274,9 +274,10 @@ AOTO_DEVICE bool paged_sees(const PagedAttentionArgs& a, const int* __restrict__
 }
 
 // The sum of the infinities and NaN among four dims of keys k0 .. limit - 1 that have a page, 0 where there are none.
-// A weight of 0 (2^-126 of the row's largest and less, and every second term of one that bf16 holds) makes a NaN of an
+// A weight of 0 (2^-126 of the row's largest and less; 2^-110 for the second term of narrow tiles) makes a NaN of an
 // infinite value, which the result should be: a row that has one, though none of its scores is, takes this sum there.
-// Seldom called, so kept short: one round trip to memory for four keys.
+// Seldom called, so kept short: one round trip to memory for four keys (2048 rows over 32000 keys, a value infinite in
+// one dim and without weight: 13 ms instead of 1.2; 32 tokens over 8000 each: 2.9 instead of 0.2).
 AOTO_DEVICE f32x4_t paged_special(const PagedAttentionArgs& a, const int* __restrict__ table,
                                   const uint16_t* __restrict__ values, int k0, int limit) {
   f32x4_t sum{};
@@ -511,7 +512,11 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         high[j] = __builtin_amdgcn_perm(__float_as_uint(p[2 * j + 1]), __float_as_uint(p[2 * j]), 0x07060302u);
-        low[j] = cvt_pk_bf16(p[2 * j] - bf16_lo(high[j]), p[2 * j + 1] - bf16_hi(high[j]));
+        // the rest, and 2^-23 of the weight, which is lost beside it but keeps the term from 0 where nothing is left: 0
+        // would make a NaN of every infinite value
+        constexpr float kMore = 1.f + 0x1p-23f;
+        low[j] = cvt_pk_bf16(__builtin_fmaf(p[2 * j], kMore, -bf16_lo(high[j])),
+                             __builtin_fmaf(p[2 * j + 1], kMore, -bf16_hi(high[j])));
       }
       pb[t] = __builtin_bit_cast(fa_bf16x8, high);
       pr[t] = __builtin_bit_cast(fa_bf16x8, low);
@@ -648,11 +653,12 @@ AOTO_DEVICE void acc_settle() {
 // division or a product but the page's.
 //
 // Bound by issue, every part with its share: 2048 rows over 8048 keys, 32 / 8 heads of 128, run at 0.85 PFLOP/s in
-// 277 us, the matrix units busy for 37% of it and the vector units for 64%; without its loads to LDS it would take 35 us
-// less, without the reads of K 34, of V 11, without half of the products 32, without the exponentials 17. Reading
-// operands one or three products ahead, no fences between the products, and the packing of weights one product later
-// changed it by less than 1%. One wave a SIMD with 64 rows, half the reads from LDS and 512 registers took 297 us
-// there, 96 us (73 here) for 2048 rows over themselves and 61 us (41) for 1024, its tiles being too few for the chip.
+// 276 us (268 to 283, by the card), the matrix units busy for 37% of it and the vector units for 64%; without its loads
+// to LDS it would take 35 us less, without the reads of K 34, of V 11, without half of the products 32, without the
+// exponentials 17. Reading operands one or three products ahead, no fences between the products, and the packing of
+// weights one product later changed it by less than 1%. One wave a SIMD with 64 rows, half the reads from LDS and 512
+// registers took 297 us there, 96 us (73 here) for 2048 rows over themselves and 61 us (41) for 1024, its tiles being
+// too few for the chip.
 template <int D>
 AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, int kvh, PagedWideShared<D>& s) {
   constexpr int DS = D / 16, DT = D / 32, LPR = D / 8;  // lanes (16-byte pieces) a row
