@@ -1429,11 +1429,13 @@ def paged_attention(
     (int32 ``[R]``), its own new ones among them, in the pages that ``block_tables[r]`` (int32 ``[R, max_blocks]``)
     names: one token, a few drafted ones or a chunk of a prompt, side by side. Row ``i`` of ``n`` sees the keys up to
     its own, ``j <= kv_lens[r] - n + i`` (all of them with ``causal=False``); keys past the block table row or in
-    entries that name no page are not there, and a row that sees none gives 0. Rows before ``query_start[0]`` and from
-    ``query_start[R]`` on keep what ``out`` held. The lengths are read on the GPU; ``max_query_len`` and ``max_kv_len``
-    (0: not known) are the caller's bounds on a request's rows and keys, which choose the launch and never the result.
-    ``workspace`` (:func:`paged_attention_workspace`; allocated where it is missing or too small) is written by the
-    call: calls that share one are ordered on one stream.
+    entries that name no page are not there, and a row that sees none gives 0. NaN and infinities in what a row sees
+    are the softmax's: a NaN or +inf among its scores, or none but -inf, makes it NaN, a value is in its dim however
+    small the weight. Rows before ``query_start[0]`` and from ``query_start[R]`` on keep what ``out`` held. The lengths
+    are read on the GPU; ``max_query_len`` and ``max_kv_len`` (0: not known) are the caller's bounds on a request's
+    rows and keys, which choose the launch, and with it the order of sums and whether weights are rounded to bf16 or
+    kept to 16 bits; what is computed goes by the lengths. ``workspace`` (:func:`paged_attention_workspace`; allocated
+    where it is missing or too small) is written by the call: calls that share one are ordered on one stream.
     """
 
     _expect_rows(q, "q", BF16, 3, q.get_device() if isinstance(q, torch.Tensor) else 0)
@@ -1499,7 +1501,8 @@ def verify_draft(
     at which the running sum of weights is above ``u[K]`` times their total. At a temperature of 0 (and everywhere
     with ``temperature=None``) a draft stands where it is the row's first maximum, which is also the token that
     follows. ``tokens`` holds the drafts that stand, the token that follows them and -1 behind it; ``accepted`` counts
-    the former. A request without rows gets -1 throughout. Everything is summed in 64 bits.
+    the former. A request without rows gets -1 throughout. Weights and sums are held in 64 bits (the exponentials right
+    to 3e-15 of themselves).
     """
 
     dtype = logits.dtype if isinstance(logits, torch.Tensor) else BF16

@@ -633,14 +633,17 @@ int aoto_hip_paged_rope_append(const void* qkv, int64_t row_stride, const int64_
                                int tokens, int query_heads, int kv_heads, int head_dim, void* q_out, int32_t* error,
                                void* stream);
 
-/* Attention of the requests' new tokens over their pages: request r's rows are query_start[r] .. query_start[r + 1]
- * of q (strides in elements, multiples of 8) and of out [tokens, Hq * head_dim], query_start not decreasing; row i of
- * n sees the keys j < kv_lens[r] - n + i + 1 (causal) or j < kv_lens[r], as far as its block table reaches and names
- * pages of the cache. A row that sees none gives 0; rows before query_start[0] and from query_start[requests] on keep
- * what they held. max_query_len and max_kv_len (0: not known) are the caller's bounds on a request's rows and keys;
- * they choose the launch and never the result. workspace: aoto_hip_paged_attention_workspace() bytes for the same
- * arguments (0: none needed). head_dim 64 or 128, at most 128 query heads a kv head, block tables of at most 2^28
- * keys (max_blocks * page), page_stride below 2^32, slot_stride * page below 2^30, scale positive and finite. */
+/* Attention of the requests' new tokens over their pages: request r's rows are query_start[r] .. query_start[r + 1] of
+ * q (strides in elements, multiples of 8) and of out [tokens, Hq * head_dim], query_start not decreasing; row i of n
+ * sees the keys j < kv_lens[r] - n + i + 1 (causal) or j < kv_lens[r], as far as its block table reaches and names
+ * pages of the cache. A row that sees none gives 0; NaN and infinities in what it sees are the softmax's (a NaN or +inf
+ * among its scores, or none but -inf: NaN; in a value: in that dim, however small the weight); rows before
+ * query_start[0] and from query_start[requests] on keep what they held. max_query_len and max_kv_len (0: not known) are
+ * the caller's bounds on a request's rows and keys; they choose the launch, with it the order of sums and whether
+ * weights are rounded to bf16 or kept to 16 bits, and need not be true: what is computed goes by the lengths.
+ * workspace: aoto_hip_paged_attention_workspace() bytes for the same arguments (0: none needed). head_dim 64 or 128, at
+ * most 128 query heads a kv head, block tables of at most 2^28 keys (max_blocks * page), page_stride below 2^32,
+ * slot_stride * page below 2^30, scale positive and finite. */
 size_t aoto_hip_paged_attention_workspace(int tokens, int requests, int max_blocks, int page, int query_heads,
                                           int kv_heads, int head_dim, int max_query_len, int max_kv_len);
 int aoto_hip_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* keys,
