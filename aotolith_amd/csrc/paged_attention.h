@@ -274,7 +274,7 @@ AOTO_DEVICE bool paged_sees(const PagedAttentionArgs& a, const int* __restrict__
 }
 
 // The sum of the infinities and NaN among four dims of keys k0 .. limit - 1 that have a page, 0 where there are none.
-// A weight of 0 (2^-126 of the row's largest and less; 2^-110 for the second term of narrow tiles) makes a NaN of an
+// A weight of 0 (2^-118 of the row's largest and less; 2^-95 for the second term of narrow tiles) makes a NaN of an
 // infinite value, which the result should be: a row that has one, though none of its scores is, takes this sum there.
 // Seldom called, so kept short: one round trip to memory for four keys (2048 rows over 32000 keys, a value infinite in
 // one dim and without weight: 13 ms instead of 1.2; 32 tokens over 8000 each: 2.9 instead of 0.2).
@@ -491,8 +491,9 @@ AOTO_DEVICE void paged_narrow(const PagedAttentionArgs& a, const PagedUnit& unit
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[t][g][e]);
       top = xor32_max(xor16_max(top)) * c2;
-      // the exponentials' reference moves only where a score passes it by more than 2^8
-      const float moved = top > run_max[t] + 8.f ? top : run_max[t];
+      // the exponentials' reference moves only where a score passes it, and then 2^8 ahead: no weight is above 1, which
+      // a value near the largest number would not bear
+      const float moved = top > run_max[t] ? top + 8.f : run_max[t];
       const float keep = moved == run_max[t] ? 1.f : __builtin_amdgcn_exp2f(run_max[t] - moved);
       run_max[t] = moved;
       const float ref = moved == -INFINITY ? 0.f : moved;
@@ -653,7 +654,7 @@ AOTO_DEVICE void acc_settle() {
 // division or a product but the page's.
 //
 // Bound by issue, every part with its share: 2048 rows over 8048 keys, 32 / 8 heads of 128, run at 0.85 PFLOP/s in
-// 276 us (268 to 283, by the card), the matrix units busy for 37% of it and the vector units for 64%; without its loads
+// 276 us (263 to 283, by the card), the matrix units busy for 37% of it and the vector units for 64%; without its loads
 // to LDS it would take 35 us less, without the reads of K 34, of V 11, without half of the products 32, without the
 // exponentials 17. Reading operands one or three products ahead, no fences between the products, and the packing of
 // weights one product later changed it by less than 1%. One wave a SIMD with 64 rows, half the reads from LDS and 512
@@ -825,10 +826,10 @@ AOTO_DEVICE void paged_wide(const PagedAttentionArgs& a, const PagedUnit& unit, 
     }
     top_of();
   };
-  // the exponentials' reference moves only where a score passes it by more than 2^8; O and the sum follow
+  // the exponentials' reference moves only where a score passes it, and then 2^8 ahead; O and the sum follow
   auto move = [&] {
     const float most = xor32_max(top) * c2;
-    const float moved = most > run_max + 8.f ? most : run_max;
+    const float moved = most > run_max ? most + 8.f : run_max;
     // (nothing to scale yet where there was no reference)
     const float keep = moved == run_max || run_max == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(run_max - moved);
     run_max = moved;

@@ -595,6 +595,22 @@ def test_attention_of_drafted_rows_keeps_16_bits_of_the_weights(hq, hkv, dim):
     assert (np.abs(got - want) <= narrow_bound(want, size))[written].all()
 
 
+@pytest.mark.parametrize("kernel,hq,hkv,dim,most,requests", FORMS)
+@pytest.mark.parametrize("cut", [False, True])
+def test_attention_of_large_values_as_scores_rise(kernel, hq, hkv, dim, most, requests, cut):
+    # a value near the largest number, its weight 200 times that of the keys before it and a tenth of the row's
+    rng = np.random.default_rng(hq + most + 4)
+    s = _form_requests(rng, hq, hkv, dim, most, requests, 1500)
+    s["q"][s["start"][2]: s["start"][3]] = 1.0
+    for j in range(1500):
+        s["keys"][s["tables"][2, j // 16], :, j % 16] = 5.3 / dim ** 0.5 if j == 700 else 0.0
+    s["values"][s["tables"][2, 700 // 16], :, 700 % 16, :9] = -3e38
+    for host, device in zip((s["keys"], s["values"]), s["device"]):
+        device.copy_(to_gpu_bf16(host))
+    s["keys"], s["values"] = (from_gpu_bf16(device).copy() for device in s["device"])
+    _check_attention(s, _form_attend(s, kernel, most, 1500, cut)[0])
+
+
 @pytest.mark.parametrize("rows", [1, 20])
 def test_attention_of_large_scores(rows):
     # one key far above the others, scores to +-90: the running maximum moves, nothing overflows
