@@ -61,7 +61,7 @@ def build(verbose: bool = False) -> tuple[str, str]:
     _run([HIPCC, *DEVICE_FLAGS, "--genco", "--no-gpu-bundle-output", os.path.join(CSRC, "kernels.hip"), "-o", tmp_obj], verbose)
     os.replace(tmp_obj, CODE_OBJECT)
     tmp_lib = LIBRARY + ".tmp"
-    # The host library: the C-ABI launchers (paged.cpp: those over the paged cache), plus noalloc.hip, whose device
+    # The host library: the C-ABI launchers (paged.cpp and serving.cpp: those of serving), plus noalloc.hip, whose device
     # part is only the static scratch buffer of the allocation-free GEMM entry point.
     _run(
         [
@@ -79,6 +79,7 @@ def build(verbose: bool = False) -> tuple[str, str]:
             "-I" + CSRC,
             os.path.join(CSRC, "aoto_hip.cpp"),
             os.path.join(CSRC, "paged.cpp"),
+            os.path.join(CSRC, "serving.cpp"),
             os.path.join(CSRC, "noalloc.hip"),
             "-o",
             tmp_lib,

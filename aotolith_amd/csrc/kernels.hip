@@ -19,6 +19,10 @@
 #include "paged_cache.h"
 #include "paged_attention.h"
 #include "verify.h"
+#include "paged_mx4.h"
+#include "paged_mx4_attention.h"
+#include "paged_pages.h"
+#include "adjust.h"
 
 // Marks the code objects whose build chose plans by the present rules (present_rules in aoto_hip.cpp).
 extern "C" __global__ void aoto_plan_rules_3() {}
@@ -233,3 +237,11 @@ AOTO_PAGED_ATTENTION(128)
 // Verification of drafted tokens: {logits' type} x {statistics, masses, pick}.
 AOTO_VERIFY_INSTANCE(bf16, false)
 AOTO_VERIFY_INSTANCE(f32, true)
+
+// Attention over a paged cache in 4 bits: head dim x {narrow tiles of 16 and 32 rows, wide tiles beside narrow ones}.
+AOTO_PAGED_MX4_ATTENTION(64)
+AOTO_PAGED_MX4_ATTENTION(128)
+
+// Penalties, biases and masks of logits, by the logits' type.
+AOTO_ADJUST_INSTANCE(bf16, false)
+AOTO_ADJUST_INSTANCE(f32, true)

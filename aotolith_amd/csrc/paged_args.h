@@ -81,3 +81,129 @@ struct VerifyArgs {
   int rows, requests, drafts, vocab, chunks;
   int judged;  // rows of a request that have statistics: the target's drafts + 1, and the drafts' where they matter
 };
+
+// A layer's cache in 4 bits: codes and scale bytes, each with strides (bytes) of its own.
+struct PagedMx4Cache {
+  uint8_t* keys;
+  uint8_t* values;
+  uint8_t* key_scales;
+  uint8_t* value_scales;
+  long long page_stride, head_stride, slot_stride;
+  long long scale_page_stride, scale_head_stride, scale_slot_stride;
+};
+
+struct PagedMx4AppendArgs {
+  PagedMx4Cache cache;
+  const uint16_t* qkv;
+  const long long* positions;
+  const long long* slots;
+  const uint16_t* cos_table;
+  const uint16_t* sin_table;
+  uint16_t* q_out;
+  int* error;
+  long long row_stride, slot_count;
+  int tokens, query_heads, kv_heads, head_dim, page, table_rows;
+};
+
+struct PagedMx4UnpackArgs {
+  PagedMx4Cache cache;
+  uint16_t* keys_out;
+  uint16_t* values_out;
+  int page, kv_heads, head_dim;
+};
+
+struct PagedMx4AttentionArgs {
+  PagedAttentionArgs base;  // its pages' addresses and strides are not used
+  PagedMx4Cache cache;
+};
+
+struct PagedForkArgs {
+  const int* parents;
+  const int* context_lens;
+  int* block_tables;
+  const int* page_counts;
+  int* shares;
+  const int* free_pages;
+  const int* free_start;
+  int* context_lens_out;
+  int* page_counts_out;
+  int* free_start_out;
+  int* source;
+  int* target;
+  int* plan;   // two entries a request: full pages taken over (-1: none is asked for), its length
+  int* error;
+  long long table_stride;
+  int requests, max_blocks, free_count, pages, page;
+};
+
+struct PagedReleaseArgs {
+  const int* keep_lens;
+  const int* block_tables;
+  const int* page_counts;
+  int* shares;
+  int* free_pages;
+  const int* free_start;
+  int* page_counts_out;
+  int* free_start_out;
+  int* error;
+  long long table_stride;
+  int requests, max_blocks, free_count, pages, page;
+};
+
+struct PagedCompactArgs {
+  int* block_tables;
+  const int* page_counts;
+  int* shares;
+  int* free_pages;
+  const int* free_start;
+  int* source;
+  int* target;
+  int* count;
+  int* state;  // of each page: what it is, then its new number
+  int* error;
+  long long table_stride;
+  int requests, max_blocks, free_count, pages;
+};
+
+// What a copy of pages moves: planes of pages of one size.
+constexpr int kPagedCopyTensors = 64;
+constexpr int kPagedCopyChunk = 16384;  // bytes that a block moves at a time
+
+struct PagedCopyTensor {
+  uint8_t* base;
+  long long page_stride, plane_stride;  // bytes
+  long long bytes;                      // of a page
+  int first;                            // planes of the tensors before it
+  int chunks;                           // of a page
+};
+
+struct PagedCopyArgs {
+  const int* source;
+  const int* target;
+  const int* count;  // pairs in use, or NULL: all
+  int* error;
+  int pairs, pages, tensors, planes, chunks;  // planes of all tensors, chunks of the longest page
+  int wide;                                   // everything a multiple of 16 bytes
+  PagedCopyTensor at[kPagedCopyTensors];
+};
+
+// Tokens of a vocabulary that a block of adjust_logits takes: eight a thread.
+constexpr int kAdjustChunk = 2048;
+
+struct AdjustArgs {
+  const void* logits;
+  void* out;
+  const int* query_start;   // NULL: a row a request
+  const long long* history;
+  const int* history_lens;
+  const int* prompt_lens;
+  const long long* draft_tokens;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const long long* bias_tokens;
+  const float* bias_values;
+  const uint8_t* allowed;
+  long long row_stride, out_stride, history_stride, draft_stride, bias_stride, value_stride, allowed_stride;
+  int rows, requests, vocab, history_len, drafts, biases;
+};

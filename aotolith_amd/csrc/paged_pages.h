@@ -1,0 +1,335 @@
+// The pages of a paged cache beyond a step's own: requests that go on in several ways, pages given back, pages moved
+// together, and the copy of what is in them.
+//
+// A page's holders are the block table rows that name it: shares[page] + 1 of them, 0 where it is free or has one.
+// Pages that nobody holds are free_pages[free_start ..). Everything here is decided by integers in a fixed order,
+// whatever order the threads run in.
+#pragma once
+
+#include "common.h"
+#include "paged_args.h"
+#include "paged_cache.h"
+
+namespace aoto {
+
+constexpr int kPageSteps = 8, kPageBatch = 1024 * kPageSteps;  // pages that a block looks at in one round trip
+
+// Of a batch of flags in the order of their pages (thread tid has those of pages 1024 i + tid, bit i of `bits`): how
+// many lie before each. before[i] for this thread's, `total` for the block. `scratch`: kPageRanks values.
+constexpr int kPageRanks = 16 * kPageSteps + 2;
+AOTO_DEVICE void page_ranks(uint32_t bits, int (&before)[kPageSteps], int& total, int* scratch) {
+  constexpr int ALL = 16 * kPageSteps;  // waves of flags: two waves sum them
+  static_assert(ALL == 128, "two waves");
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+  for (int i = 0; i < kPageSteps; ++i) {
+    const unsigned long long lanes = __ballot(bits >> i & 1);
+    before[i] = __popcll(lanes & ((1ull << lane) - 1));
+    if (lane == 0) scratch[16 * i + wave] = __popcll(lanes);
+  }
+  __syncthreads();
+  int own = 0, sum = 0;
+  if (tid < ALL) {
+    own = sum = scratch[tid];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(sum, d);
+      if (lane >= d) sum += up;
+    }
+    if (lane == 63) scratch[ALL + wave] = sum;
+  }
+  __syncthreads();
+  if (tid < ALL) scratch[tid] = sum - own + (wave ? scratch[ALL] : 0);
+  total = scratch[ALL] + scratch[ALL + 1];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPageSteps; ++i) before[i] += scratch[16 * i + wave];
+  __syncthreads();
+}
+
+}  // namespace aoto
+
+// Which rows go on from which, the pages taken for them and what is to be copied (formulas at the entry point's
+// declaration). One block: everything hangs on a running sum over the requests.
+extern "C" __global__ __launch_bounds__(1024) void aoto_paged_fork(PagedForkArgs a) {
+  using namespace aoto;
+  __shared__ long long s_scan[16];
+  __shared__ int s_error;
+  const int tid = threadIdx.x;
+  if (tid == 0) s_error = 0;
+  const int start = a.free_start[0];
+  const long long first_free = max(start, 0);
+  long long taken = 0;
+  int error = 0;
+  __syncthreads();
+  for (int base = 0; base < a.requests; base += 1024) {
+    const int r = base + tid;
+    int parent = -1, full = -1, length = 0;
+    if (r < a.requests) {
+      parent = a.parents[r];
+      const bool empty = a.page_counts[r] <= 0;
+      if (parent >= a.requests) error |= AOTO_PAGED_BAD_ROW, parent = -1;
+      if (parent >= 0 && !empty) error |= AOTO_PAGED_ROW_HELD, parent = -1;
+      if (parent >= 0) {
+        const int count = min(max(a.page_counts[parent], 0), a.max_blocks);
+        length = (int)min((long long)max(a.context_lens[parent], 0), (long long)count * a.page);
+        full = length / a.page;
+      }
+    }
+    const bool part = full >= 0 && length > full * a.page;
+    long long total = 0;
+    const long long at = first_free + taken + block_scan_1024(part ? 1 : 0, s_scan, total) - 1;
+    if (r < a.requests) {
+      int source = -1, target = -1;
+      if (part) {
+        if (at < a.free_count) {
+          source = a.block_tables[(size_t)parent * a.table_stride + full];
+          target = a.free_pages[at];
+          a.block_tables[(size_t)r * a.table_stride + full] = target;
+        } else {
+          error |= AOTO_PAGED_NO_PAGES;
+          length = full * a.page;
+        }
+      }
+      a.source[r] = source, a.target[r] = target;
+      a.plan[2 * r] = full, a.plan[2 * r + 1] = length;
+    }
+    taken += total;
+  }
+  if (error) atomicOr(&s_error, error);
+  __syncthreads();
+  // only now: a row may be the parent of another, and the outputs may be the inputs
+  for (int r = tid; r < a.requests; r += 1024) {
+    const int full = a.plan[2 * r], length = a.plan[2 * r + 1];
+    a.context_lens_out[r] = full >= 0 ? length : a.context_lens[r];
+    a.page_counts_out[r] = full >= 0 ? full + (length > full * a.page ? 1 : 0) : a.page_counts[r];
+  }
+  if (tid == 0) {
+    const long long available = max(0LL, a.free_count - first_free);
+    a.free_start_out[0] = taken ? (int)(first_free + min(taken, available)) : start;
+    if (s_error && a.error) atomicOr(a.error, s_error);
+  }
+}
+
+// The full pages of the rows that go on: entered in their own rows, one holder more each.
+extern "C" __global__ __launch_bounds__(256) void aoto_paged_share(PagedForkArgs a) {
+  const int r = blockIdx.x, full = a.plan[2 * r];
+  if (full <= 0) return;
+  const int* from = a.block_tables + (size_t)a.parents[r] * a.table_stride;
+  int* to = a.block_tables + (size_t)r * a.table_stride;
+  for (int j = threadIdx.x; j < full; j += 256) {
+    const int page = from[j];
+    to[j] = page;
+    if ((unsigned)page < (unsigned)a.pages) atomicAdd(a.shares + page, 1);
+  }
+}
+
+// Requests' pages past what they keep lose a holder each; a page without one stands at -1 until aoto_paged_reclaim.
+extern "C" __global__ __launch_bounds__(256) void aoto_paged_drop(PagedReleaseArgs a) {
+  const int r = blockIdx.x, held = a.page_counts[r], keep = a.keep_lens[r];
+  const int count = min(max(held, 0), a.max_blocks);
+  const int stays = keep < 0 ? count : min(count, (int)(((unsigned)keep + (unsigned)a.page - 1) / (unsigned)a.page));
+  __syncthreads();  // the counts written may be the counts read
+  if (threadIdx.x == 0) a.page_counts_out[r] = keep < 0 ? held : stays;
+  const int* table = a.block_tables + (size_t)r * a.table_stride;
+  for (int j = stays + threadIdx.x; j < count; j += 256) {
+    const int page = table[j];
+    if ((unsigned)page < (unsigned)a.pages) atomicSub(a.shares + page, 1);
+  }
+}
+
+// The pages left without a holder, in the order of their numbers, to the places before the free list's first. One
+// block: 8192 pages a round trip.
+extern "C" __global__ __launch_bounds__(1024) void aoto_paged_reclaim(PagedReleaseArgs a) {
+  using namespace aoto;
+  __shared__ int s_scratch[kPageRanks];
+  const int tid = threadIdx.x;
+  const int start = a.free_start[0], first = min(max(start, 0), a.free_count);
+  int freed = 0, error = 0;
+  for (int base = 0; base < a.pages; base += kPageBatch) {
+    int share[kPageSteps];
+#pragma unroll
+    for (int i = 0; i < kPageSteps; ++i) {
+      const int page = base + 1024 * i + tid;
+      share[i] = page < a.pages ? a.shares[page] : 0;
+    }
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < kPageSteps; ++i) bits |= (uint32_t)(share[i] < 0) << i;
+    int before[kPageSteps], total;
+    page_ranks(bits, before, total, s_scratch);
+#pragma unroll
+    for (int i = 0; i < kPageSteps; ++i)
+      if (share[i] < 0) {
+        const int page = base + 1024 * i + tid, at = first - 1 - freed - before[i];
+        if (share[i] < -1) error |= AOTO_PAGED_BAD_SHARE;
+        a.shares[page] = 0;
+        if (at >= 0) a.free_pages[at] = page;
+        else error |= AOTO_PAGED_LIST_FULL;
+      }
+    freed += total;
+  }
+  if (error && a.error) atomicOr(a.error, error);
+  __syncthreads();  // the start written may be the start read
+  if (tid == 0) a.free_start_out[0] = freed ? max(0, first - freed) : start;
+}
+
+// What each page is: 0, and then (aoto_paged_mark) 1 where a request holds it, 2 where it is in the free list.
+extern "C" __global__ __launch_bounds__(256) void aoto_paged_clear(PagedCompactArgs a) {
+  const int page = blockIdx.x * 256 + threadIdx.x;
+  if (page < a.pages) a.state[page] = 0;
+}
+
+// Blocks 0 .. requests - 1: a row of the tables each; the others: the free list.
+extern "C" __global__ __launch_bounds__(256) void aoto_paged_mark(PagedCompactArgs a) {
+  const int r = blockIdx.x;
+  if (r < a.requests) {
+    const int count = min(max(a.page_counts[r], 0), a.max_blocks);
+    for (int j = threadIdx.x; j < count; j += 256) {
+      const int page = a.block_tables[(size_t)r * a.table_stride + j];
+      if ((unsigned)page < (unsigned)a.pages) atomicOr(a.state + page, 1);
+    }
+    return;
+  }
+  const int first = max(a.free_start[0], 0), others = gridDim.x - a.requests;
+  for (long long j = first + (long long)(r - a.requests) * 256 + threadIdx.x; j < a.free_count; j += others * 256LL) {
+    const int page = a.free_pages[j];
+    if ((unsigned)page < (unsigned)a.pages) atomicOr(a.state + page, 2);
+  }
+}
+
+// The moves. With m pages held, and the pages held or free in the order of their numbers: held ones past the first m
+// go, in order, to the free ones among the first m, and the rest is the free list. One block: 8192 pages a round trip,
+// once for m and once for the places.
+extern "C" __global__ __launch_bounds__(1024) void aoto_paged_moves(PagedCompactArgs a) {
+  using namespace aoto;
+  __shared__ int s_scratch[kPageRanks];
+  __shared__ int s_low;
+  const int tid = threadIdx.x;
+  const int first = min(max(a.free_start[0], 0), a.free_count);
+  int own = 0, both = 0;
+  for (int base = 0; base < a.pages; base += kPageBatch) {
+    int state[kPageSteps];
+#pragma unroll
+    for (int i = 0; i < kPageSteps; ++i) {
+      const int page = base + 1024 * i + tid;
+      state[i] = page < a.pages ? a.state[page] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kPageSteps; ++i) own += state[i] & 1, both += state[i] == 3;
+  }
+  int error = both ? AOTO_PAGED_BAD_SHARE : 0;
+  __shared__ long long s_scan[16];
+  long long total_held;
+  block_scan_1024(own, s_scan, total_held);
+  const int m = (int)total_held;
+  if (tid == 0) s_low = 0;
+  __syncthreads();
+  int places = 0, held = 0;  // of the pages before
+  for (int base = 0; base < a.pages; base += kPageBatch) {
+    int state[kPageSteps], share[kPageSteps];
+#pragma unroll
+    for (int i = 0; i < kPageSteps; ++i) {
+      const int page = base + 1024 * i + tid;
+      state[i] = page < a.pages ? a.state[page] : 0;
+      share[i] = page < a.pages ? a.shares[page] : 0;
+    }
+    uint32_t any = 0, is_held = 0;
+#pragma unroll
+    for (int i = 0; i < kPageSteps; ++i) {
+      any |= (uint32_t)(state[i] != 0) << i;
+      is_held |= (uint32_t)(state[i] & 1) << i;
+    }
+    int place[kPageSteps], held_before[kPageSteps], some, some_held;
+    page_ranks(any, place, some, s_scratch);
+    page_ranks(is_held, held_before, some_held, s_scratch);
+#pragma unroll
+    for (int i = 0; i < kPageSteps; ++i) {
+      place[i] += places, held_before[i] += held;
+      const int page = base + 1024 * i + tid;
+      if (any >> i & 1 && place[i] < m) {
+        if (!(is_held >> i & 1)) a.target[place[i] - held_before[i]] = page;
+        if (place[i] == m - 1) s_low = held_before[i] + (is_held >> i & 1);  // held pages that stay
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPageSteps; ++i) {
+      const int page = base + 1024 * i + tid;
+      if (page >= a.pages) continue;
+      int now = page;
+      if (any >> i & 1 && place[i] >= m) {
+        if (is_held >> i & 1) {
+          const int k = held_before[i] - s_low;
+          a.source[k] = page;
+          now = a.target[k];
+          a.shares[now] = share[i];
+          a.shares[page] = 0;
+        }
+        const int at = first + place[i] - m;
+        if (at < a.free_count) a.free_pages[at] = page;
+      }
+      a.state[page] = now;
+    }
+    places += some, held += some_held;
+    __syncthreads();
+  }
+  const int moved = m - s_low;
+  for (int k = moved + tid; k < a.pages; k += 1024) a.source[k] = a.target[k] = -1;
+  // entries of the list that named no page, or one twice
+  const int rest = first + places - m;
+  if (rest < a.free_count) error |= AOTO_PAGED_BAD_SHARE;
+  for (int j = rest + tid; j < a.free_count; j += 1024) a.free_pages[j] = -1;
+  if (error && a.error) atomicOr(a.error, error);
+  if (tid == 0) a.count[0] = moved;
+}
+
+extern "C" __global__ __launch_bounds__(256) void aoto_paged_remap(PagedCompactArgs a) {
+  const int r = blockIdx.x, count = min(max(a.page_counts[r], 0), a.max_blocks);
+  for (int j = threadIdx.x; j < count; j += 256) {
+    int* entry = a.block_tables + (size_t)r * a.table_stride + j;
+    const int page = *entry;
+    if ((unsigned)page < (unsigned)a.pages) *entry = a.state[page];
+  }
+}
+
+// Pages' contents from source[i] to target[i], in every plane of every tensor. A block takes chunks of 16 KB of a page
+// of a plane, those of one pair after the other's; every block passes over all pairs, so that pairs without a copy cost
+// no more than a look.
+extern "C" __global__ __launch_bounds__(256) void aoto_paged_copy(PagedCopyArgs a) {
+  const int pairs = a.count ? min(max(a.count[0], 0), a.pairs) : a.pairs;
+  const int each = a.planes * a.chunks;  // chunks of a pair
+  const long long items = (long long)pairs * each;
+  for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+    const int pair = (int)(item / each), within = (int)(item - (long long)pair * each);
+    const int source = a.source[pair], target = a.target[pair];
+    if ((unsigned)source >= (unsigned)a.pages || (unsigned)target >= (unsigned)a.pages) {
+      const bool bad = source < -1 || source >= a.pages || target < -1 || target >= a.pages;
+      if (bad && a.error && within == 0 && threadIdx.x == 0)
+        atomicOr(a.error, AOTO_PAGED_BAD_SLOT);
+      continue;
+    }
+    if (source == target) continue;
+    const int plane = within / a.chunks, chunk = within - plane * a.chunks;
+    int t = 0;
+    while (t + 1 < a.tensors && a.at[t + 1].first <= plane) ++t;
+    const PagedCopyTensor& at = a.at[t];
+    if (chunk >= at.chunks) continue;
+    uint8_t* base = at.base + (plane - at.first) * at.plane_stride + (long long)chunk * kPagedCopyChunk;
+    const uint8_t* from = base + source * at.page_stride;
+    uint8_t* to = base + target * at.page_stride;
+    const int bytes = (int)min(at.bytes - (long long)chunk * kPagedCopyChunk, (long long)kPagedCopyChunk);
+    if (a.wide && bytes == kPagedCopyChunk) {
+      uint4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = reinterpret_cast<const uint4*>(from)[256 * i + threadIdx.x];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(to)[256 * i + threadIdx.x] = v[i];
+    } else if (a.wide) {
+      for (int b = threadIdx.x; b < bytes / 16; b += 256)
+        reinterpret_cast<uint4*>(to)[b] = reinterpret_cast<const uint4*>(from)[b];
+    } else {
+      for (int b = threadIdx.x; b < bytes; b += 256) to[b] = from[b];
+    }
+  }
+}

@@ -1,0 +1,253 @@
+// Host side of the C ABI's entry points over a 4-bit paged cache, for its pages' upkeep and for logits
+// (include/aoto_hip.h): checks, launch choices, launches.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <cstdio>
+
+#include "aoto_hip.h"
+#include "internal.h"
+#include "paged_args.h"
+#include "paged_host.h"
+
+namespace {
+
+using aoto::aligned;
+using aoto::attention_plan;
+using aoto::AttentionPlan;
+using aoto::kWideRows;
+using aoto::launch;
+using aoto::set_error;
+
+int check_cache(const char* what, const aoto_mx4_cache* c, int page, int kv_heads, int head_dim, PagedMx4Cache& to) {
+  if (!c || !c->keys || !c->values || !c->key_scales || !c->value_scales)
+    return set_error(AOTO_ERR_ARGUMENT, "%s: null pointer", what);
+  if (c->pages <= 0 || page <= 0 || page > (1 << 20) || kv_heads <= 0 || head_dim <= 0)
+    return set_error(AOTO_ERR_ARGUMENT, "%s: bad cache shape", what);
+  if (head_dim % 64)
+    return set_error(AOTO_ERR_UNSUPPORTED, "%s: head_dim %d is not a multiple of 64", what, head_dim);
+  if (!aligned(c->keys, 16) || !aligned(c->values, 16) || c->page_stride % 16 || c->head_stride % 16 ||
+      c->slot_stride % 16)
+    return set_error(AOTO_ERR_ARGUMENT, "%s: codes 16-byte aligned with strides of multiples of 16", what);
+  to.keys = static_cast<uint8_t*>(c->keys), to.values = static_cast<uint8_t*>(c->values);
+  to.key_scales = static_cast<uint8_t*>(c->key_scales), to.value_scales = static_cast<uint8_t*>(c->value_scales);
+  to.page_stride = c->page_stride, to.head_stride = c->head_stride, to.slot_stride = c->slot_stride;
+  to.scale_page_stride = c->scale_page_stride, to.scale_head_stride = c->scale_head_stride;
+  to.scale_slot_stride = c->scale_slot_stride;
+  return AOTO_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int aoto_hip_paged_rope_append_mx4(const void* qkv, int64_t row_stride, const int64_t* positions, const int64_t* slots,
+                                   const void* cos_table, const void* sin_table, int table_rows,
+                                   const aoto_mx4_cache* cache, int page, int tokens, int query_heads, int kv_heads,
+                                   int head_dim, void* q_out, int32_t* error, void* stream) {
+  if (!qkv || !positions || !slots || !cos_table || !sin_table || !q_out)
+    return set_error(AOTO_ERR_ARGUMENT, "paged_rope_append_mx4: null pointer");
+  PagedMx4AppendArgs a{};
+  if (int s = check_cache("paged_rope_append_mx4", cache, page, kv_heads, head_dim, a.cache)) return s;
+  if (tokens <= 0 || query_heads <= 0 || table_rows <= 0)
+    return set_error(AOTO_ERR_ARGUMENT, "paged_rope_append_mx4: bad shape");
+  if (!aligned(qkv, 16) || row_stride % 8 || !aligned(cos_table, 16) || !aligned(sin_table, 16) || !aligned(q_out, 16))
+    return set_error(AOTO_ERR_ARGUMENT, "paged_rope_append_mx4: rows, tables and q_out 16-byte aligned");
+  const long long per_token = (query_heads + 2LL * kv_heads) * (head_dim / 16);
+  if (per_token > (1 << 24)) return set_error(AOTO_ERR_UNSUPPORTED, "paged_rope_append_mx4: rows too long");
+  a.qkv = static_cast<const uint16_t*>(qkv), a.row_stride = row_stride;
+  a.positions = reinterpret_cast<const long long*>(positions), a.slots = reinterpret_cast<const long long*>(slots);
+  a.cos_table = static_cast<const uint16_t*>(cos_table), a.sin_table = static_cast<const uint16_t*>(sin_table);
+  a.q_out = static_cast<uint16_t*>(q_out), a.error = error;
+  a.slot_count = (long long)cache->pages * page, a.tokens = tokens, a.query_heads = query_heads;
+  a.kv_heads = kv_heads, a.head_dim = head_dim, a.page = page, a.table_rows = table_rows;
+  return launch("aoto_paged_rope_append_mx4", (tokens * per_token + 255) / 256, 1, 256, stream, a);
+}
+
+int aoto_hip_paged_unpack_mx4(const aoto_mx4_cache* cache, int page, int kv_heads, int head_dim, void* keys_out,
+                              void* values_out, void* stream) {
+  if (!keys_out || !values_out) return set_error(AOTO_ERR_ARGUMENT, "paged_unpack_mx4: null pointer");
+  PagedMx4UnpackArgs a{};
+  if (int s = check_cache("paged_unpack_mx4", cache, page, kv_heads, head_dim, a.cache)) return s;
+  if (!aligned(keys_out, 16) || !aligned(values_out, 16))
+    return set_error(AOTO_ERR_ARGUMENT, "paged_unpack_mx4: outputs 16-byte aligned");
+  a.keys_out = static_cast<uint16_t*>(keys_out), a.values_out = static_cast<uint16_t*>(values_out);
+  a.page = page, a.kv_heads = kv_heads, a.head_dim = head_dim;
+  const long long rows = (long long)kv_heads * page;
+  if (rows >= (1 << 24) || head_dim > (1 << 10))
+    return set_error(AOTO_ERR_UNSUPPORTED, "paged_unpack_mx4: pages too large");
+  return launch("aoto_paged_unpack_mx4", cache->pages, (rows * (head_dim / 16) + 255) / 256, 256, stream, a);
+}
+
+int aoto_hip_paged_attention_mx4(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                 const aoto_mx4_cache* cache, int page, const int32_t* block_tables,
+                                 int64_t table_stride, int max_blocks, const int32_t* query_start,
+                                 const int32_t* kv_lens, int tokens, int requests, int query_heads, int kv_heads,
+                                 int head_dim, int causal, float scale, int max_query_len, int max_kv_len,
+                                 void* workspace, void* out, void* stream) {
+  if (!q || !block_tables || !query_start || !kv_lens || !out)
+    return set_error(AOTO_ERR_ARGUMENT, "paged_attention_mx4: null pointer");
+  PagedMx4AttentionArgs args{};
+  if (int s = check_cache("paged_attention_mx4", cache, page, kv_heads, head_dim, args.cache)) return s;
+  if (tokens <= 0 || requests <= 0 || max_blocks <= 0 || query_heads <= 0 || query_heads % kv_heads ||
+      table_stride < max_blocks || max_query_len < 0 || max_kv_len < 0)
+    return set_error(AOTO_ERR_ARGUMENT, "paged_attention_mx4: bad shape");
+  if (head_dim != 64 && head_dim != 128)
+    return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention_mx4: head_dim %d (64 or 128)", head_dim);
+  if (!aligned(q, 16) || q_token_stride % 8 || q_head_stride % 8 || !aligned(out, 16))
+    return set_error(AOTO_ERR_ARGUMENT, "paged_attention_mx4: q and out 16-byte aligned, strides of multiples of 8");
+  if ((long long)max_blocks * page > (1 << 28))
+    return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention_mx4: block tables of more than 2^28 keys");
+  if (!(scale > 0.f) || !std::isfinite(scale))
+    return set_error(AOTO_ERR_ARGUMENT, "paged_attention_mx4: scale %g is not a positive number", (double)scale);
+  if (query_heads / kv_heads > kWideRows)
+    return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention_mx4: %d query heads a kv head (at most %d)",
+                     query_heads / kv_heads, kWideRows);
+  const AttentionPlan plan = attention_plan(tokens, requests, max_blocks, page, query_heads, kv_heads, head_dim,
+                                            max_query_len, max_kv_len);
+  if (plan.workspace && (!workspace || !aligned(workspace, 16)))
+    return set_error(AOTO_ERR_ARGUMENT, "paged_attention_mx4: needs a 16-byte aligned workspace of %zu bytes",
+                     plan.workspace);
+  PagedAttentionArgs& a = args.base;
+  a.q = static_cast<const uint16_t*>(q), a.block_tables = block_tables, a.query_start = query_start;
+  a.kv_lens = kv_lens, a.out = static_cast<uint16_t*>(out), a.q_token_stride = q_token_stride;
+  a.q_head_stride = q_head_stride, a.table_stride = table_stride, a.tokens = tokens, a.requests = requests;
+  a.pages = cache->pages, a.page = page, a.query_heads = query_heads, a.kv_heads = kv_heads;
+  a.causal = causal != 0, a.scale = scale;
+  aoto::attention_launch(plan, max_blocks, workspace, a);
+  char name[64];
+  snprintf(name, sizeof(name), "aoto_paged_attention_mx4_d%d_%s", head_dim,
+           plan.wide_rows ? "w" : plan.narrow_rows == 16 ? "n1" : "n2");
+  if (int s = launch(name, (plan.target ? plan.target : plan.units) * kv_heads, 1, 256, stream, args)) return s;
+  if (!plan.target) return AOTO_OK;
+  return launch(head_dim == 64 ? "aoto_paged_attention_join_d64" : "aoto_paged_attention_join_d128",
+                ((long long)tokens * query_heads + 3) / 4, 1, 256, stream, a);
+}
+
+int aoto_hip_paged_fork(const int32_t* parents, const int32_t* context_lens, int32_t* block_tables,
+                        int64_t table_stride, const int32_t* page_counts, int32_t* shares, const int32_t* free_pages,
+                        const int32_t* free_start, int requests, int max_blocks, int free_count, int pages, int page,
+                        int32_t* context_lens_out, int32_t* page_counts_out, int32_t* free_start_out, int32_t* source,
+                        int32_t* target, int32_t* plan, int32_t* error, void* stream) {
+  if (!parents || !context_lens || !block_tables || !page_counts || !shares || (!free_pages && free_count) ||
+      !free_start || !context_lens_out || !page_counts_out || !free_start_out || !source || !target || !plan)
+    return set_error(AOTO_ERR_ARGUMENT, "paged_fork: null pointer");
+  if (requests <= 0 || max_blocks <= 0 || free_count < 0 || pages <= 0 || page <= 0 || table_stride < max_blocks)
+    return set_error(AOTO_ERR_ARGUMENT, "paged_fork: bad shape");
+  if (max_blocks > (1 << 20) || page > (1 << 20) || requests > (1 << 28))
+    return set_error(AOTO_ERR_UNSUPPORTED, "paged_fork: at most 2^20 blocks a request and tokens a page");
+  PagedForkArgs a{};
+  a.parents = parents, a.context_lens = context_lens, a.block_tables = block_tables, a.page_counts = page_counts;
+  a.shares = shares, a.free_pages = free_pages, a.free_start = free_start, a.context_lens_out = context_lens_out;
+  a.page_counts_out = page_counts_out, a.free_start_out = free_start_out, a.source = source, a.target = target;
+  a.plan = plan, a.error = error, a.table_stride = table_stride, a.requests = requests, a.max_blocks = max_blocks;
+  a.free_count = free_count, a.pages = pages, a.page = page;
+  if (int s = launch("aoto_paged_fork", 1, 1, 1024, stream, a)) return s;
+  return launch("aoto_paged_share", requests, 1, 256, stream, a);
+}
+
+int aoto_hip_paged_release(const int32_t* keep_lens, const int32_t* block_tables, int64_t table_stride,
+                           const int32_t* page_counts, int32_t* shares, int32_t* free_pages,
+                           const int32_t* free_start, int requests, int max_blocks, int free_count, int pages,
+                           int page, int32_t* page_counts_out, int32_t* free_start_out, int32_t* error, void* stream) {
+  if (!keep_lens || !block_tables || !page_counts || !shares || (!free_pages && free_count) || !free_start ||
+      !page_counts_out || !free_start_out)
+    return set_error(AOTO_ERR_ARGUMENT, "paged_release: null pointer");
+  if (requests <= 0 || max_blocks <= 0 || free_count < 0 || pages <= 0 || page <= 0 || table_stride < max_blocks)
+    return set_error(AOTO_ERR_ARGUMENT, "paged_release: bad shape");
+  if (max_blocks > (1 << 20) || page > (1 << 20) || pages > (1 << 30))
+    return set_error(AOTO_ERR_UNSUPPORTED,
+                     "paged_release: at most 2^20 blocks a request and tokens a page, 2^30 pages");
+  PagedReleaseArgs a{};
+  a.keep_lens = keep_lens, a.block_tables = block_tables, a.page_counts = page_counts, a.shares = shares;
+  a.free_pages = free_pages, a.free_start = free_start, a.page_counts_out = page_counts_out;
+  a.free_start_out = free_start_out, a.error = error, a.table_stride = table_stride, a.requests = requests;
+  a.max_blocks = max_blocks, a.free_count = free_count, a.pages = pages, a.page = page;
+  if (int s = launch("aoto_paged_drop", requests, 1, 256, stream, a)) return s;
+  return launch("aoto_paged_reclaim", 1, 1, 1024, stream, a);
+}
+
+int aoto_hip_paged_compact(int32_t* block_tables, int64_t table_stride, const int32_t* page_counts, int32_t* shares,
+                           int32_t* free_pages, const int32_t* free_start, int requests, int max_blocks,
+                           int free_count, int pages, int32_t* source, int32_t* target, int32_t* count,
+                           int32_t* state, int32_t* error, void* stream) {
+  if (!block_tables || !page_counts || !shares || (!free_pages && free_count) || !free_start || !source || !target ||
+      !count || !state)
+    return set_error(AOTO_ERR_ARGUMENT, "paged_compact: null pointer");
+  if (requests <= 0 || max_blocks <= 0 || free_count < 0 || pages <= 0 || table_stride < max_blocks)
+    return set_error(AOTO_ERR_ARGUMENT, "paged_compact: bad shape");
+  if (max_blocks > (1 << 20) || pages > (1 << 30) || requests > (1 << 28))
+    return set_error(AOTO_ERR_UNSUPPORTED, "paged_compact: at most 2^20 blocks a request, 2^30 pages");
+  PagedCompactArgs a{};
+  a.block_tables = block_tables, a.page_counts = page_counts, a.shares = shares, a.free_pages = free_pages;
+  a.free_start = free_start, a.source = source, a.target = target, a.count = count, a.state = state, a.error = error;
+  a.table_stride = table_stride, a.requests = requests, a.max_blocks = max_blocks, a.free_count = free_count;
+  a.pages = pages;
+  if (int s = launch("aoto_paged_clear", (pages + 255LL) / 256, 1, 256, stream, a)) return s;
+  const long long lists = std::min(256LL, std::max(1LL, (free_count + 255LL) / 256));
+  if (int s = launch("aoto_paged_mark", requests + lists, 1, 256, stream, a)) return s;
+  if (int s = launch("aoto_paged_moves", 1, 1, 1024, stream, a)) return s;
+  return launch("aoto_paged_remap", requests, 1, 256, stream, a);
+}
+
+int aoto_hip_paged_copy(const aoto_page_tensor* tensors, int tensor_count, int pages, const int32_t* source,
+                        const int32_t* target, int pairs, const int32_t* count, int32_t* error, void* stream) {
+  if (!tensors || !source || !target) return set_error(AOTO_ERR_ARGUMENT, "paged_copy: null pointer");
+  if (tensor_count <= 0 || pages <= 0 || pairs <= 0) return set_error(AOTO_ERR_ARGUMENT, "paged_copy: bad shape");
+  for (int from = 0; from < tensor_count; from += kPagedCopyTensors) {
+    PagedCopyArgs a{};
+    a.source = source, a.target = target, a.count = count, a.error = from ? nullptr : error;
+    a.pairs = pairs, a.pages = pages, a.tensors = std::min(kPagedCopyTensors, tensor_count - from), a.wide = 1;
+    long long planes = 0;
+    for (int i = 0; i < a.tensors; ++i) {
+      const aoto_page_tensor& t = tensors[from + i];
+      if (!t.data || t.planes <= 0 || t.page_bytes <= 0)
+        return set_error(AOTO_ERR_ARGUMENT, "paged_copy: tensor %d: bad shape", from + i);
+      const long long chunks = (t.page_bytes - 1) / kPagedCopyChunk + 1;
+      if (chunks > (1 << 20)) return set_error(AOTO_ERR_UNSUPPORTED, "paged_copy: pages of more than 16 GB");
+      a.at[i].base = static_cast<uint8_t*>(t.data), a.at[i].page_stride = t.page_stride;
+      a.at[i].plane_stride = t.plane_stride, a.at[i].bytes = t.page_bytes, a.at[i].first = (int)planes;
+      a.at[i].chunks = (int)chunks, a.chunks = std::max(a.chunks, (int)chunks);
+      if (!aligned(t.data, 16) || t.page_stride % 16 || t.plane_stride % 16 || t.page_bytes % 16) a.wide = 0;
+      planes += t.planes;
+      if (planes > (1 << 20)) return set_error(AOTO_ERR_UNSUPPORTED, "paged_copy: more than 2^20 planes");
+    }
+    a.planes = (int)planes;
+    if (planes * a.chunks > 0x7FFFFFFFLL) return set_error(AOTO_ERR_UNSUPPORTED, "paged_copy: pages too large");
+    const long long items = planes * a.chunks * (long long)pairs;
+    // eight blocks a CU at most: one that ends takes the next of its chunks
+    if (int s = launch("aoto_paged_copy", std::min(items, 8LL * aoto::device_cu_count()), 1, 256, stream, a)) return s;
+  }
+  return AOTO_OK;
+}
+
+int aoto_hip_adjust_logits(const void* logits, int logits_f32, int64_t row_stride, int rows, int vocab, int requests,
+                           const aoto_adjustments* adjust, void* out, int64_t out_stride, void* stream) {
+  if (!logits || !adjust || !out) return set_error(AOTO_ERR_ARGUMENT, "adjust_logits: null pointer");
+  if (rows <= 0 || vocab <= 0 || requests <= 0) return set_error(AOTO_ERR_ARGUMENT, "adjust_logits: bad shape");
+  const aoto_adjustments& j = *adjust;
+  if (j.history_len < 0 || j.drafts < 0 || j.biases < 0 || (j.history_len && !j.history) ||
+      (j.drafts && !j.draft_tokens) || (j.biases && (!j.bias_tokens || !j.bias_values)))
+    return set_error(AOTO_ERR_ARGUMENT, "adjust_logits: null pointer");
+  if (vocab > 1 << 30) return set_error(AOTO_ERR_UNSUPPORTED, "adjust_logits: %d tokens (at most 2^30)", vocab);
+  if (j.history_len >= 1 << 30) return set_error(AOTO_ERR_UNSUPPORTED, "adjust_logits: texts of 2^30 tokens");
+  if (requests > 65535) return set_error(AOTO_ERR_UNSUPPORTED, "adjust_logits: %d requests (at most 65535)", requests);
+  const size_t size = logits_f32 ? 4 : 2;
+  if (!aligned(logits, size) || !aligned(out, size))
+    return set_error(AOTO_ERR_ARGUMENT, "adjust_logits: logits aligned to their type");
+  AdjustArgs a{};
+  a.logits = logits, a.out = out, a.query_start = j.query_start;
+  a.history = reinterpret_cast<const long long*>(j.history), a.history_lens = j.history_lens;
+  a.prompt_lens = j.prompt_lens, a.draft_tokens = reinterpret_cast<const long long*>(j.draft_tokens);
+  a.repetition = j.repetition, a.presence = j.presence, a.frequency = j.frequency;
+  a.bias_tokens = reinterpret_cast<const long long*>(j.bias_tokens), a.bias_values = j.bias_values;
+  a.allowed = reinterpret_cast<const uint8_t*>(j.allowed), a.row_stride = row_stride, a.out_stride = out_stride;
+  a.history_stride = j.history_stride, a.draft_stride = j.draft_stride, a.bias_stride = j.bias_stride;
+  a.value_stride = j.value_stride, a.allowed_stride = 4 * j.allowed_stride;
+  a.rows = rows, a.requests = requests, a.vocab = vocab, a.history_len = j.history_len, a.drafts = j.drafts;
+  a.biases = j.biases;
+  return launch(logits_f32 ? "aoto_adjust_logits_f32" : "aoto_adjust_logits_bf16", (vocab - 1) / kAdjustChunk + 1,
+                requests, 256, stream, a);
+}
+
+}  // extern "C"

@@ -1551,3 +1551,539 @@ def verify_draft(
         )
     )
     return tokens, accepted
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# The paged cache in 4 bits. A row of D dims is D / 2 bytes of codes and D / 32 scale bytes: a code is a sign and one of
+# 0, 0.5, 1, 1.5, 2, 3, 4, 6 (dim 2i in the low half of byte i), its group of 32 dims shares the scale 2^(byte - 127),
+# and a byte above 252 makes the group NaN. 68 bytes for 128 dims, 256 in bf16.
+
+
+class PagedMx4(NamedTuple):
+    """A layer's cache in 4 bits: uint8 codes ``[pages, Hkv, page, D / 2]`` and scale bytes ``[pages, Hkv, page,
+    D / 32]`` (views with contiguous rows will do; the codes' other strides and bases are multiples of 16 bytes)."""
+
+    keys: torch.Tensor
+    values: torch.Tensor
+    key_scales: torch.Tensor
+    value_scales: torch.Tensor
+
+
+def paged_mx4_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, *, device=None) -> PagedMx4:
+    """A layer's cache in 4 bits, all zeros."""
+
+    pages, kv_heads, page_size, head_dim = int(pages), int(kv_heads), int(page_size), int(head_dim)
+    if min(pages, kv_heads, page_size, head_dim) <= 0 or head_dim % 64:
+        raise ValueError("a 4-bit cache has heads of multiples of 64 dims, got "
+                         f"{pages} pages of {kv_heads} x {page_size} rows of {head_dim}")
+    device = torch.device("cuda") if device is None else device
+    codes, scales = (torch.zeros((2, pages, kv_heads, page_size, head_dim // n), dtype=torch.uint8, device=device)
+                     for n in (2, 32))
+    return PagedMx4(*codes.unbind(), *scales.unbind())
+
+
+def _expect_mx4(cache: PagedMx4, device: int) -> tuple[tuple, _lib.Mx4CacheArg]:
+    """``(pages, Hkv, page, D)`` of a cache, and its descriptor for the C ABI."""
+
+    if not isinstance(cache, PagedMx4):
+        raise TypeError(f"cache must be a PagedMx4, got {type(cache).__name__}")
+    keys, values, key_scales, value_scales = cache
+    for name, tensor in zip(cache._fields, cache):
+        _expect_rows(tensor, name, torch.uint8, 4, device)
+    shape, strides, scale_strides = keys.shape, keys.stride(), key_scales.stride()
+    if shape != values.shape or strides != values.stride():
+        raise ValueError("keys and values must have one shape and the same strides")
+    dim = 2 * shape[3]
+    if dim % 64:
+        raise ValueError(f"heads of a 4-bit cache have a multiple of 64 dims, got {dim}")
+    if tuple(key_scales.shape) != (*shape[:3], dim // 32) or key_scales.shape != value_scales.shape:
+        raise ValueError(f"key_scales and value_scales must be {(*shape[:3], dim // 32)}, got "
+                         f"{tuple(key_scales.shape)} and {tuple(value_scales.shape)}")
+    if scale_strides != value_scales.stride():
+        raise ValueError("key_scales and value_scales must have the same strides")
+    return (shape[0], shape[1], shape[2], dim), _lib.Mx4CacheArg(
+        keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), *strides[:3],
+        *scale_strides[:3], shape[0])
+
+
+def paged_rope_append_mx4(
+    qkv: torch.Tensor,
+    positions: torch.Tensor,
+    slots: torch.Tensor,
+    cos_table: torch.Tensor,
+    sin_table: torch.Tensor,
+    cache: PagedMx4,
+    *,
+    query_heads: int,
+    q_out: torch.Tensor | None = None,
+    error: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`paged_rope_append` into a 4-bit cache: returns ``q [T, Hq, D]``.
+
+    Keys go from f32 to their codes without a rounding to bf16 between. A group's scale is the least power of two of
+    which its largest magnitude is at most 7 (bytes 1 to 252), a code the nearest value, ties to the even code,
+    magnitudes above 6 to 6; a group that holds an infinity or a NaN stands for NaN.
+    """
+
+    _expect_rows(qkv, "qkv", BF16, 2, qkv.get_device() if isinstance(qkv, torch.Tensor) else 0)
+    device = _on_current("qkv", qkv)
+    (_, kv_heads, page, dim), arg = _expect_mx4(cache, device)
+    tokens, width = qkv.shape
+    query_heads = int(query_heads)
+    if query_heads <= 0 or width != (query_heads + 2 * kv_heads) * dim:
+        raise ValueError(f"qkv rows of {width} do not hold {query_heads} + 2 x {kv_heads} heads of {dim}")
+    _expect_all(device, ((positions, "positions", torch.int64, (tokens,)), (slots, "slots", torch.int64, (tokens,)),
+                         (cos_table, "cos_table", BF16, None)))
+    if cos_table.dim() != 2 or cos_table.shape[1] != dim:
+        raise ValueError(f"cos_table must be [P, {dim}], got {tuple(cos_table.shape)}")
+    _expect_all(device, ((sin_table, "sin_table", BF16, cos_table.shape),))
+    if error is not None:
+        _expect_all(device, ((error, "error", torch.int32, (1,)),))
+    if q_out is None:
+        q_out = qkv.new_empty((tokens, query_heads, dim))
+    else:
+        _expect_all(device, ((q_out, "q_out", BF16, (tokens, query_heads, dim)),))
+    _ready(qkv)
+    _lib.check(
+        _lib.library().aoto_hip_paged_rope_append_mx4(
+            _ptr(qkv), qkv.stride(0), _ptr(positions), _ptr(slots), _ptr(cos_table), _ptr(sin_table),
+            cos_table.shape[0], ctypes.byref(arg), page, tokens, query_heads, kv_heads, dim, _ptr(q_out), _ptr(error),
+            _stream(device),
+        )
+    )
+    return q_out
+
+
+def paged_unpack_mx4(cache: PagedMx4, *, out: tuple[torch.Tensor, torch.Tensor] | None = None
+                     ) -> tuple[torch.Tensor, torch.Tensor]:
+    """What a 4-bit cache stands for: ``(keys, values)`` bf16 ``[pages, Hkv, page, D]`` (exact: bf16 holds every value
+    that an append writes)."""
+
+    if not isinstance(cache, PagedMx4):
+        raise TypeError(f"cache must be a PagedMx4, got {type(cache).__name__}")
+    _expect_rows(cache.keys, "keys", torch.uint8, 4, cache.keys.get_device()
+                 if isinstance(cache.keys, torch.Tensor) else 0)
+    device = _on_current("keys", cache.keys)
+    shape, arg = _expect_mx4(cache, device)
+    if out is None:
+        out = tuple(torch.empty(shape, dtype=BF16, device=cache.keys.device) for _ in range(2))
+    else:
+        keys_out, values_out = out
+        _expect_all(device, ((keys_out, "out[0]", BF16, shape), (values_out, "out[1]", BF16, shape)))
+    _ready(cache.keys)
+    _lib.check(_lib.library().aoto_hip_paged_unpack_mx4(ctypes.byref(arg), shape[2], shape[1], shape[3], _ptr(out[0]),
+                                                        _ptr(out[1]), _stream(device)))
+    return out
+
+
+def paged_attention_mx4(
+    q: torch.Tensor,
+    cache: PagedMx4,
+    block_tables: torch.Tensor,
+    query_start: torch.Tensor,
+    kv_lens: torch.Tensor,
+    *,
+    causal: bool = True,
+    scale: float | None = None,
+    max_query_len: int = 0,
+    max_kv_len: int = 0,
+    workspace: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`paged_attention` over a 4-bit cache: the requests' new tokens ``q [T, Hq, D]`` (D 64 or 128) over the
+    values that the codes of their pages stand for -> ``[T, Hq * D]``.
+
+    Everything else is :func:`paged_attention`'s, the workspace (:func:`paged_attention_workspace`) and what a row sees
+    among it. A NaN group of a key that a row sees, a NaN or an infinity in its q make the row NaN; a NaN group of a
+    value makes those 32 dims NaN, however small its weight. Requests of more than 32 rows a kv head multiply K as it is
+    in the cache by q as two 8-bit numbers (exactly q to 2^-22 of the largest of each 32 dims).
+    """
+
+    _expect_rows(q, "q", BF16, 3, q.get_device() if isinstance(q, torch.Tensor) else 0)
+    device = _on_current("q", q)
+    tokens, query_heads, dim = q.shape
+    (_, kv_heads, page, key_dim), arg = _expect_mx4(cache, device)
+    if key_dim != dim:
+        raise ValueError(f"q heads have {dim} elements, the cache's {key_dim}")
+    _expect_rows(block_tables, "block_tables", torch.int32, 2, device)
+    requests, max_blocks = block_tables.shape
+    _expect_all(device, ((query_start, "query_start", torch.int32, (requests + 1,)),
+                         (kv_lens, "kv_lens", torch.int32, (requests,))))
+    if scale is None:
+        scale = ctypes.c_float(dim ** -0.5).value
+    if out is None:
+        out = q.new_empty((tokens, query_heads * dim))
+    else:
+        _expect_all(device, ((out, "out", BF16, (tokens, query_heads * dim)),))
+    _ready(q)
+    lib = _lib.library()
+    max_query_len, max_kv_len = int(max_query_len), int(max_kv_len)
+    need = lib.aoto_hip_paged_attention_workspace(tokens, requests, max_blocks, page, query_heads, kv_heads, dim,
+                                                  max_query_len, max_kv_len)
+    if workspace is not None:
+        _on_device(workspace)
+        if workspace.get_device() != device:
+            raise ValueError(f"the workspace is on {workspace.device}, the call's other tensors on cuda:{device}")
+        if not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+            workspace = None
+    if need and workspace is None:
+        workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
+    _lib.check(
+        lib.aoto_hip_paged_attention_mx4(
+            _ptr(q), q.stride(0), q.stride(1), ctypes.byref(arg), page, _ptr(block_tables), block_tables.stride(0),
+            max_blocks, _ptr(query_start), _ptr(kv_lens), tokens, requests, query_heads, kv_heads, dim,
+            int(bool(causal)), float(scale), max_query_len, max_kv_len, _ptr(workspace if need else None), _ptr(out),
+            _stream(device),
+        )
+    )
+    return out
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# The pages of a cache beyond a step's own. ``shares`` (int32 ``[pages]``) counts a page's holders beyond the first: the
+# block table rows that name it within their page counts. :func:`paged_tables` takes pages that nobody shares.
+
+#: More bits of the ``error`` tensor, raised by the functions below (``AOTO_PAGED_*`` in ``include/aoto_hip.h``).
+PAGED_ROW_HELD, PAGED_BAD_ROW, PAGED_BAD_SHARE, PAGED_LIST_FULL = 32, 64, 128, 256
+
+
+class PagedFork(NamedTuple):
+    """What :func:`paged_fork` says of the requests, and the pages to copy."""
+
+    context_lens: torch.Tensor  # int32 [R]
+    page_counts: torch.Tensor   # int32 [R]
+    free_start: torch.Tensor    # int32 [1]
+    source: torch.Tensor        # int32 [R]: the page to copy for each row, -1 without
+    target: torch.Tensor        # int32 [R]: where to
+
+
+class PagedMoves(NamedTuple):
+    """What :func:`paged_compact` moved: page ``source[i]`` to ``target[i]``, ``i < count``; -1 behind them."""
+
+    source: torch.Tensor  # int32 [pages]
+    target: torch.Tensor  # int32 [pages]
+    count: torch.Tensor   # int32 [1]
+
+
+def _expect_pool(block_tables, page_counts, shares, free_pages, free_start, error) -> tuple[int, int]:
+    """The pool's tensors, as every function on pages takes them: ``(device, requests)``."""
+
+    _expect(shares, "shares", torch.int32)
+    device = _on_current("shares", shares)
+    if shares.dim() != 1 or not shares.numel():
+        raise ValueError(f"shares must be [pages], got {tuple(shares.shape)}")
+    _expect_rows(block_tables, "block_tables", torch.int32, 2, device)
+    requests = block_tables.shape[0]
+    _expect_all(device, (
+        (page_counts, "page_counts", torch.int32, (requests,)), (free_pages, "free_pages", torch.int32, None),
+        (free_start, "free_start", torch.int32, (1,)),
+    ))
+    if error is not None:
+        _expect_all(device, ((error, "error", torch.int32, (1,)),))
+    return device, requests
+
+
+def paged_fork(
+    parents: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_tables: torch.Tensor,
+    page_counts: torch.Tensor,
+    shares: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_start: torch.Tensor,
+    *,
+    page_size: int,
+    step: PagedFork | None = None,
+    error: torch.Tensor | None = None,
+) -> PagedFork:
+    """Requests that go on from another: samples of one prompt, beams.
+
+    Row ``r`` with ``parents[r] >= 0`` (int32 ``[R]``) must hold no pages; it gets the cached tokens of row
+    ``parents[r]`` as that was before the call. Full pages are shared: entered in its row of ``block_tables``, one more
+    in ``shares``. A page in progress becomes the next one of ``free_pages[free_start:]``, rows in order, and its
+    content is to be copied: ``source``, ``target`` for :func:`paged_copy` on every layer's cache. Other rows stay.
+    ``block_tables`` and ``shares`` are changed in place; lengths, counts and the list's start are in the result, whose
+    tensors ``step`` may give, also as the ones passed in. ``error`` (int32 ``[1]``) collects ``PAGED_ROW_HELD`` (the
+    row holds pages: left as it is), ``PAGED_BAD_ROW`` (no such parent: the same) and ``PAGED_NO_PAGES`` (the free list
+    ran out: the row ends with its last full page).
+    """
+
+    device, requests = _expect_pool(block_tables, page_counts, shares, free_pages, free_start, error)
+    _expect_all(device, ((parents, "parents", torch.int32, (requests,)),
+                         (context_lens, "context_lens", torch.int32, (requests,))))
+    shapes = ((requests,), (requests,), (1,), (requests,), (requests,))
+    if step is None:
+        all_of = shares.new_empty((6 * requests + 1,))
+        lens, counts, source, target, plan, first = all_of.split_with_sizes(
+            (requests, requests, requests, requests, 2 * requests, 1))
+        step = PagedFork(lens, counts, first, source, target)
+    else:
+        _expect_all(device, ((x, f"step.{name}", torch.int32, shape)
+                             for x, name, shape in zip(step, PagedFork._fields, shapes)))
+        plan = shares.new_empty((2 * requests,))
+    _ready(shares)
+    _lib.check(
+        _lib.library().aoto_hip_paged_fork(
+            _ptr(parents), _ptr(context_lens), _ptr(block_tables), block_tables.stride(0), _ptr(page_counts),
+            _ptr(shares), _ptr(free_pages), _ptr(free_start), requests, block_tables.shape[1], free_pages.numel(),
+            shares.numel(), int(page_size), _ptr(step.context_lens), _ptr(step.page_counts), _ptr(step.free_start),
+            _ptr(step.source), _ptr(step.target), _ptr(plan), _ptr(error), _stream(device),
+        )
+    )
+    return step
+
+
+def paged_release(
+    keep_lens: torch.Tensor,
+    block_tables: torch.Tensor,
+    page_counts: torch.Tensor,
+    shares: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_start: torch.Tensor,
+    *,
+    page_size: int,
+    out: tuple[torch.Tensor, torch.Tensor] | None = None,
+    error: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Pages given back, of requests that ended or whose drafted tokens did not stand: ``(page_counts, free_start)``.
+
+    Row ``r`` keeps the pages of its first ``keep_lens[r]`` tokens (int32 ``[R]``; 0: none, negative: all that it has).
+    The others lose a holder each, and those left without one go to the places of ``free_pages`` before ``free_start``,
+    downwards from it in ascending order of their numbers. ``shares`` and ``free_pages`` are changed in place, entries
+    of ``block_tables`` past the new counts stay what they were; ``out`` gives the tensors of the result, which may be
+    the ones passed in. ``error`` (int32 ``[1]``) collects ``PAGED_BAD_SHARE`` (a page given back more often than held)
+    and ``PAGED_LIST_FULL`` (no place before the list's first: the page is lost).
+    """
+
+    device, requests = _expect_pool(block_tables, page_counts, shares, free_pages, free_start, error)
+    _expect_all(device, ((keep_lens, "keep_lens", torch.int32, (requests,)),))
+    if out is None:
+        out = shares.new_empty((requests + 1,)).split_with_sizes((requests, 1))
+    else:
+        counts_out, start_out = out
+        _expect_all(device, ((counts_out, "out[0]", torch.int32, (requests,)),
+                             (start_out, "out[1]", torch.int32, (1,))))
+    _ready(shares)
+    _lib.check(
+        _lib.library().aoto_hip_paged_release(
+            _ptr(keep_lens), _ptr(block_tables), block_tables.stride(0), _ptr(page_counts), _ptr(shares),
+            _ptr(free_pages), _ptr(free_start), requests, block_tables.shape[1], free_pages.numel(), shares.numel(),
+            int(page_size), _ptr(out[0]), _ptr(out[1]), _ptr(error), _stream(device),
+        )
+    )
+    return tuple(out)
+
+
+def paged_compact(
+    block_tables: torch.Tensor,
+    page_counts: torch.Tensor,
+    shares: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_start: torch.Tensor,
+    *,
+    moves: PagedMoves | None = None,
+    error: torch.Tensor | None = None,
+) -> PagedMoves:
+    """A pool's pages moved together, so that what is behind them can be given up.
+
+    With ``m`` pages held by the rows of ``block_tables`` and the pages held or in ``free_pages[free_start:]`` in
+    ascending order, held pages past the first ``m`` of them go, in order, to free ones among the first ``m``. The
+    tables and ``shares`` are changed to the new numbers in place; the free list keeps its place and holds the rest,
+    ascending (so the pool's highest numbers are free ones). Pages neither held nor free stay what they are. The
+    contents are :func:`paged_copy`'s, on every layer's cache, with the result's ``source``, ``target`` and ``count``.
+    ``error`` (int32 ``[1]``) collects ``PAGED_BAD_SHARE``: a page both held and free, or a list that names a page twice
+    or none.
+    """
+
+    device, requests = _expect_pool(block_tables, page_counts, shares, free_pages, free_start, error)
+    pages = shares.numel()
+    if moves is None:
+        source, target, state, count = shares.new_empty((3 * pages + 1,)).split_with_sizes((pages, pages, pages, 1))
+        moves = PagedMoves(source, target, count)
+    else:
+        _expect_all(device, ((x, f"moves.{name}", torch.int32, shape)
+                             for x, name, shape in zip(moves, PagedMoves._fields, ((pages,), (pages,), (1,)))))
+        state = shares.new_empty((pages,))
+    _ready(shares)
+    _lib.check(
+        _lib.library().aoto_hip_paged_compact(
+            _ptr(block_tables), block_tables.stride(0), _ptr(page_counts), _ptr(shares), _ptr(free_pages),
+            _ptr(free_start), requests, block_tables.shape[1], free_pages.numel(), pages, _ptr(moves.source),
+            _ptr(moves.target), _ptr(moves.count), _ptr(state), _ptr(error), _stream(device),
+        )
+    )
+    return moves
+
+
+def _page_tensor(tensor: torch.Tensor, name: str, dim: int, pages: int | None, device: int) -> _lib.PageTensorArg:
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(tensor).__name__}")
+    if tensor.device.type != "cuda":
+        raise ValueError(f"{name} must be on the GPU, got {tensor.device}")
+    if tensor.get_device() != device:
+        raise ValueError(f"{name} is on {tensor.device}, the call's other tensors on cuda:{device}")
+    shape, strides, size = tensor.shape, tensor.stride(), tensor.element_size()
+    if not 0 <= dim < len(shape) or not tensor.numel():
+        raise ValueError(f"{name} {tuple(shape)} has no pages in dim {dim}")
+    if pages is not None and shape[dim] != pages:
+        raise ValueError(f"{name} has {shape[dim]} pages, the first tensor {pages}")
+    # a page: its dims in some order one dense block
+    dense = 1
+    for stride, length in sorted((s, n) for s, n in zip(strides[dim + 1:], shape[dim + 1:]) if n > 1):
+        if stride != dense:
+            raise ValueError(f"{name}'s pages must be dense in memory, got strides {strides}")
+        dense *= length
+    planes, plane_stride = 1, 0
+    for stride, length in zip(strides[:dim][::-1], shape[:dim][::-1]):
+        if length == 1:
+            continue
+        if planes > 1 and stride != planes * plane_stride:
+            raise ValueError(f"{name}'s dims before its pages must be evenly spaced, got strides {strides}")
+        plane_stride = plane_stride if planes > 1 else stride
+        planes *= length
+    page_stride = strides[dim] if shape[dim] > 1 else dense
+    # of two strides the smaller one is past a page, the other past all that it spans
+    low, high = sorted(((page_stride, shape[dim]), (plane_stride if planes > 1 else page_stride * shape[dim], planes)))
+    if low[0] < dense or high[0] < low[0] * (low[1] - 1) + dense:
+        raise ValueError(f"{name}'s pages overlap, got strides {strides}")
+    return _lib.PageTensorArg(tensor.data_ptr(), planes, plane_stride * size, page_stride * size, dense * size)
+
+
+def paged_copy(
+    caches: torch.Tensor | list[torch.Tensor] | tuple[torch.Tensor, ...],
+    source: torch.Tensor,
+    target: torch.Tensor,
+    *,
+    count: torch.Tensor | None = None,
+    dim: int = 0,
+    error: torch.Tensor | None = None,
+) -> None:
+    """Pages' contents from ``source[i]`` to ``target[i]`` (int32 ``[N]``) in every tensor of ``caches``, in place.
+
+    The pages are in dim ``dim`` of each tensor, of any type: ``[pages, Hkv, page, D]`` for one layer's keys, with
+    ``dim=2`` ``[layers, 2, pages, ...]`` for all layers at once. What follows that dim is dense in memory (in any
+    order), what precedes it evenly spaced. ``count`` (int32 ``[1]``, on the GPU) takes only the first pairs. Pairs with
+    a -1 are left out, and others that name no page too, which raises ``PAGED_BAD_SLOT`` in ``error`` (int32 ``[1]``).
+    No target may be the source or the target of another pair, as none of :func:`paged_fork` and :func:`paged_compact`
+    is.
+    """
+
+    _expect(source, "source", torch.int32)
+    device = _on_current("source", source)
+    if source.dim() != 1:
+        raise ValueError(f"source must be [N], got {tuple(source.shape)}")
+    _expect_all(device, ((target, "target", torch.int32, source.shape),))
+    for x, name in ((count, "count"), (error, "error")):
+        if x is not None:
+            _expect_all(device, ((x, name, torch.int32, (1,)),))
+    if isinstance(caches, torch.Tensor):
+        caches = (caches,)
+    if not caches:
+        raise ValueError("no caches")
+    dim = int(dim)
+    args = (_lib.PageTensorArg * len(caches))()
+    pages = None
+    for i, tensor in enumerate(caches):
+        args[i] = _page_tensor(tensor, f"caches[{i}]", dim, pages, device)
+        pages = tensor.shape[dim]
+    if not source.numel():
+        return
+    _ready(source)
+    _lib.check(_lib.library().aoto_hip_paged_copy(args, len(caches), pages, _ptr(source), _ptr(target), source.numel(),
+                                                  _ptr(count), _ptr(error), _stream(device)))
+
+
+def adjust_logits(
+    logits: torch.Tensor,
+    query_start: torch.Tensor | None = None,
+    *,
+    history: torch.Tensor | None = None,
+    history_lens: torch.Tensor | None = None,
+    prompt_lens: torch.Tensor | None = None,
+    draft_tokens: torch.Tensor | None = None,
+    repetition: torch.Tensor | None = None,
+    presence: torch.Tensor | None = None,
+    frequency: torch.Tensor | None = None,
+    bias_tokens: torch.Tensor | None = None,
+    bias_values: torch.Tensor | None = None,
+    allowed: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Penalties, biases and masks on ``logits [T, V]`` (bf16 or f32), before :func:`verify_draft` judges or draws.
+
+    Request ``r`` has the rows ``query_start[r] .. query_start[r + 1]`` (int32 ``[R + 1]``; None: one row each), row
+    ``i`` of them behind its first ``i`` drafts (``draft_tokens`` int64 ``[R, K]``). Its text is ``history[r]`` (int64
+    ``[R, L]``) up to ``history_lens[r]`` (int32 ``[R]``; None: L), from ``prompt_lens[r]`` on (None: 0) its own answer,
+    and those drafts, which belong to the answer. In this order, in f32, with one rounding:
+
+    * a logit ``z`` of a token in the text becomes ``z / repetition[r]`` if positive, else ``z * repetition[r]``,
+    * that of a token ``c > 0`` times in the answer loses ``frequency[r] * c + presence[r]``,
+    * ``bias_values[r, j]`` is added to that of ``bias_tokens[r, j]`` (f32 and int64 ``[R, B]``, the last entry of a
+      token counts, tokens outside the vocabulary, -1 say, are none),
+    * one whose bit ``v % 32`` of ``allowed[t, v // 32]`` (int32 ``[T, ceil(V / 32)]``) is 0 becomes -inf.
+
+    ``repetition``, ``presence``, ``frequency`` are f32 ``[R]``; what is None is left out. ``out`` may be ``logits``;
+    its rows of no request are left as they are (in a new tensor: not set).
+    """
+
+    dtype = logits.dtype if isinstance(logits, torch.Tensor) else BF16
+    if dtype not in (BF16, torch.float32):
+        raise TypeError(f"logits must be bf16 or f32, got {dtype}")
+    _expect_rows(logits, "logits", dtype, 2, logits.get_device() if isinstance(logits, torch.Tensor) else 0)
+    device = _on_current("logits", logits)
+    rows, vocab = logits.shape
+    requests = rows
+    if query_start is not None:
+        _expect_all(device, ((query_start, "query_start", torch.int32, None),))
+        requests = query_start.numel() - 1
+        if query_start.dim() != 1 or requests < 1:
+            raise ValueError(f"query_start must be [R + 1], got {tuple(query_start.shape)}")
+    arg = _lib.AdjustmentsArg()
+    arg.query_start = _ptr(query_start)
+
+    def lists(tensor, name, kind, dims=(None, None)):
+        _expect_rows(tensor, name, kind, 2, device)
+        want = (dims[0] or requests, tensor.shape[1] if dims[1] is None else dims[1])
+        if tuple(tensor.shape) != want:
+            raise ValueError(f"{name} must be {want}, got {tuple(tensor.shape)}")
+        return tensor.data_ptr(), tensor.stride(0)
+
+    if history is not None:
+        arg.history, arg.history_stride = lists(history, "history", torch.int64)
+        arg.history_len = history.shape[1]
+    elif history_lens is not None or prompt_lens is not None:
+        raise ValueError("history_lens and prompt_lens need a history")
+    if draft_tokens is not None:
+        arg.draft_tokens, arg.draft_stride = lists(draft_tokens, "draft_tokens", torch.int64)
+        arg.drafts = draft_tokens.shape[1]
+    if (bias_tokens is None) != (bias_values is None):
+        raise ValueError("bias_tokens and bias_values come together")
+    if bias_tokens is not None:
+        arg.bias_tokens, arg.bias_stride = lists(bias_tokens, "bias_tokens", torch.int64)
+        arg.biases = bias_tokens.shape[1]
+        arg.bias_values, arg.value_stride = lists(bias_values, "bias_values", torch.float32, (None, arg.biases))
+    if allowed is not None:
+        arg.allowed, arg.allowed_stride = lists(allowed, "allowed", torch.int32, (rows, (vocab + 31) // 32))
+    for name, tensor, kind in (("history_lens", history_lens, torch.int32), ("prompt_lens", prompt_lens, torch.int32),
+                               ("repetition", repetition, torch.float32), ("presence", presence, torch.float32),
+                               ("frequency", frequency, torch.float32)):
+        if tensor is not None:
+            _expect_all(device, ((tensor, name, kind, (requests,)),))
+            setattr(arg, name, tensor.data_ptr())
+    if out is None:
+        out = logits.new_empty((rows, vocab))
+    else:
+        _expect_rows(out, "out", dtype, 2, device)
+        if out.shape != logits.shape:
+            raise ValueError(f"out must be {(rows, vocab)}, got {tuple(out.shape)}")
+        if (out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr()
+                and (out.data_ptr() != logits.data_ptr() or out.stride() != logits.stride())):
+            raise ValueError("out must be logits itself or in memory of its own")
+    _ready(logits)
+    _lib.check(
+        _lib.library().aoto_hip_adjust_logits(
+            _ptr(logits), int(dtype is torch.float32), logits.stride(0), rows, vocab, requests, ctypes.byref(arg),
+            _ptr(out), out.stride(0), _stream(device),
+        )
+    )
+    return out

@@ -603,6 +603,10 @@ int aoto_hip_generic_attention(const aoto_tensor* out, const aoto_tensor* q, con
 #define AOTO_PAGED_TABLE_FULL 4   /* a request longer than its block table row: slots of -1 past it */
 #define AOTO_PAGED_BAD_SLOT 8     /* a slot outside the cache and not -1: nothing written for that row */
 #define AOTO_PAGED_BAD_POSITION 16 /* a position outside the RoPE tables: nothing written for that row */
+#define AOTO_PAGED_ROW_HELD 32    /* a request that holds pages was to go on from another: left as it was */
+#define AOTO_PAGED_BAD_ROW 64     /* a parent past the last request: left as it was */
+#define AOTO_PAGED_BAD_SHARE 128  /* a page given back more often than held, or both held and free, or listed twice */
+#define AOTO_PAGED_LIST_FULL 256  /* no place before the free list's first: the page is lost */
 
 /* A step's pages, block tables and token maps from the requests' lengths. Request r has context_lens[r] cached tokens
  * (negative ones count as 0, ones past 2^30 as 2^30) and gets new_lens[r] more (negative: 0); its row of block_tables
@@ -675,6 +679,125 @@ int aoto_hip_verify_draft(const void* logits, int logits_f32, int64_t row_stride
                           int64_t draft_row_stride, const int32_t* query_start, const float* uniforms,
                           const float* temperature, int requests, int drafts, void* workspace, int64_t* tokens_out,
                           int32_t* accepted, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * The same cache in 4 bits. No counterpart in the reference, whose cache is bf16.
+ *
+ * A row of head_dim dims (a multiple of 64) is head_dim / 2 bytes of codes and head_dim / 32 scale bytes. Dim 2 i is
+ * the low half of code byte i: a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (E2M1), times 2^(b - 127) with b the scale
+ * byte of the dim's group of 32. b above 252: the group stands for NaN. Codes of page p, head h, slot s begin at p *
+ * page_stride + h * head_stride + s * slot_stride (bytes; multiples of 16, the bases 16-byte aligned), its scale bytes
+ * at the same with the scale strides (any). */
+typedef struct aoto_mx4_cache {
+  void* keys;
+  void* values;
+  void* key_scales;
+  void* value_scales;
+  int64_t page_stride, head_stride, slot_stride;
+  int64_t scale_page_stride, scale_head_stride, scale_slot_stride;
+  int32_t pages;
+} aoto_mx4_cache;
+
+/* aoto_hip_paged_rope_append into a 4-bit cache. q_out is rounded to bf16; a group of a key (rotated, f32) or value
+ * gets the least scale 2^(b - 127), 1 <= b <= 252, of which its largest magnitude is at most 7, and each dim the
+ * nearest code, ties to the even one, magnitudes above 6 to 6. A group with an infinity or NaN: b = 255, codes 0. */
+int aoto_hip_paged_rope_append_mx4(const void* qkv, int64_t row_stride, const int64_t* positions, const int64_t* slots,
+                                   const void* cos_table, const void* sin_table, int table_rows,
+                                   const aoto_mx4_cache* cache, int page, int tokens, int query_heads, int kv_heads,
+                                   int head_dim, void* q_out, int32_t* error, void* stream);
+
+/* What a whole cache stands for, bf16 [pages][kv_heads][page][head_dim] twice (exact but below 2^-133). */
+int aoto_hip_paged_unpack_mx4(const aoto_mx4_cache* cache, int page, int kv_heads, int head_dim, void* keys_out,
+                              void* values_out, void* stream);
+
+/* aoto_hip_paged_attention over a 4-bit cache, with the same rules, limits of shapes and workspace
+ * (aoto_hip_paged_attention_workspace()). A NaN that a row sees, in a key's group or in q, makes the row NaN, in a
+ * value's group those 32 dims, however small the weight. */
+int aoto_hip_paged_attention_mx4(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                 const aoto_mx4_cache* cache, int page, const int32_t* block_tables,
+                                 int64_t table_stride, int max_blocks, const int32_t* query_start,
+                                 const int32_t* kv_lens, int tokens, int requests, int query_heads, int kv_heads,
+                                 int head_dim, int causal, float scale, int max_query_len, int max_kv_len,
+                                 void* workspace, void* out, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * A paged cache's pages beyond a step's own. No counterpart in the reference.
+ *
+ * shares[page] (int32 [pages]) is a page's holders beyond the first: block table rows that name it within their
+ * page_counts. aoto_hip_paged_tables takes pages of 0 from the free list free_pages[free_start .. free_count). Outputs
+ * named *_out may be the arrays they are computed from. Everything is the same at every run, whatever the threads'
+ * order. */
+
+/* Requests that go on from another: row r with parents[r] >= 0, which must hold no pages, gets the first
+ * ceil(n / page) pages of row parents[r], n = min(context_lens, page_counts * page) of that row as it was before the
+ * call: full pages themselves (shares + 1), one in progress as the next page of the free list, rows in order, with
+ * (source[r], target[r]) the pages to copy, -1 without. context_lens_out, page_counts_out and free_start_out follow;
+ * without a free page (AOTO_PAGED_NO_PAGES) the row ends with its last full page. Rows with parents[r] < 0 stay. plan:
+ * scratch of 2 * requests entries. */
+int aoto_hip_paged_fork(const int32_t* parents, const int32_t* context_lens, int32_t* block_tables,
+                        int64_t table_stride, const int32_t* page_counts, int32_t* shares, const int32_t* free_pages,
+                        const int32_t* free_start, int requests, int max_blocks, int free_count, int pages, int page,
+                        int32_t* context_lens_out, int32_t* page_counts_out, int32_t* free_start_out, int32_t* source,
+                        int32_t* target, int32_t* plan, int32_t* error, void* stream);
+
+/* Pages given back: row r keeps the first ceil(keep_lens[r] / page) of its page_counts[r] pages (all with
+ * keep_lens[r] < 0); the others lose a holder each, entries of block_tables stay as they are. Pages left without one go
+ * to free_pages[free_start - 1], [free_start - 2], ... in ascending order of their numbers. */
+int aoto_hip_paged_release(const int32_t* keep_lens, const int32_t* block_tables, int64_t table_stride,
+                           const int32_t* page_counts, int32_t* shares, int32_t* free_pages,
+                           const int32_t* free_start, int requests, int max_blocks, int free_count, int pages,
+                           int page, int32_t* page_counts_out, int32_t* free_start_out, int32_t* error, void* stream);
+
+/* Pages moved together: with m pages held by the rows and S the pages held or free in ascending order, the held pages
+ * past the first m of S go, in ascending order, to the free ones among the first m of S. source, target (int32
+ * [pages]): the moves, -1 behind the last; count: how many. block_tables and shares are changed to the new numbers; the
+ * free list keeps its place and becomes the rest of S in ascending order. Pages neither held nor free stay what they
+ * are. state: scratch of `pages` entries. The pages' contents are aoto_hip_paged_copy's. */
+int aoto_hip_paged_compact(int32_t* block_tables, int64_t table_stride, const int32_t* page_counts, int32_t* shares,
+                           int32_t* free_pages, const int32_t* free_start, int requests, int max_blocks,
+                           int free_count, int pages, int32_t* source, int32_t* target, int32_t* count,
+                           int32_t* state, int32_t* error, void* stream);
+
+/* `planes` times the pages of a cache, plane_stride bytes apart; page p's page_bytes lie together at p * page_stride.
+ * */
+typedef struct aoto_page_tensor {
+  void* data;
+  int64_t planes, plane_stride, page_stride, page_bytes;
+} aoto_page_tensor;
+
+/* The contents of pages source[i] to target[i], i < pairs, in every plane of every tensor; *count (device memory, or
+ * NULL) may make the pairs fewer. Pairs with a -1 are left out, other numbers outside the cache too
+ * (AOTO_PAGED_BAD_SLOT). No target may be the source or the target of another pair. */
+int aoto_hip_paged_copy(const aoto_page_tensor* tensors, int tensor_count, int pages, const int32_t* source,
+                        const int32_t* target, int pairs, const int32_t* count, int32_t* error, void* stream);
+
+/* What is done to logits before a token is chosen. Request r's rows are query_start[r] .. query_start[r + 1] (NULL: row
+ * r), row i of them behind its first i drafts. With T its text, the first history_lens[r] (NULL: history_len) tokens of
+ * history[r] and those drafts, and A the part of T from prompt_lens[r] (NULL: 0) on:
+ *   z = logits; where v is in T: z > 0 ? z / repetition[r] : z * repetition[r]
+ *   where v is c > 0 times in A: z - (frequency[r] * c + presence[r])
+ *   z + bias_values[r][j] for the last j with bias_tokens[r][j] = v
+ *   -inf where bit v % 32 of allowed[row][v / 32] is 0
+ * in f32, rounded once to the logits' type. NULL repetition, presence, frequency, allowed: left out. Tokens outside the
+ * vocabulary are no tokens. Strides in elements. Rows of no request keep what out held; out may be logits. */
+typedef struct aoto_adjustments {
+  const int32_t* query_start;
+  const int64_t* history;
+  const int32_t* history_lens;
+  const int32_t* prompt_lens;
+  const int64_t* draft_tokens;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const int64_t* bias_tokens;
+  const float* bias_values;
+  const int32_t* allowed;
+  int64_t history_stride, draft_stride, bias_stride, value_stride, allowed_stride;
+  int32_t history_len, drafts, biases;
+} aoto_adjustments;
+
+int aoto_hip_adjust_logits(const void* logits, int logits_f32, int64_t row_stride, int rows, int vocab, int requests,
+                           const aoto_adjustments* adjust, void* out, int64_t out_stride, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,248 @@
+"""The operators over a 4-bit paged cache, on pages and on logits without a GPU: their plain restatements' own cases and
+what the entry points refuse on the host."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from aotolith_amd import _lib, ops
+from oracle import serving as oracle
+
+GOOD = ctypes.c_void_p(4096)  # an address that no entry point may read: each refuses first
+
+
+def _refused(status, code, word):
+    assert status == code
+    assert word in _lib.last_error()
+
+
+def _cache(**changes):
+    a = dict(keys=4096, values=4096, key_scales=4097, value_scales=4099, page_stride=2048, head_stride=1024,
+             slot_stride=64, scale_page_stride=7, scale_head_stride=5, scale_slot_stride=3, pages=4) | changes
+    return ctypes.byref(_lib.Mx4CacheArg(*a.values()))
+
+
+CACHE_REFUSALS = [
+    (dict(keys=None), 1), (dict(values=None), 1), (dict(key_scales=None), 1), (dict(value_scales=None), 1),
+    (dict(pages=0), 1), (dict(keys=4104), 1), (dict(values=4097), 1), (dict(page_stride=2056), 1),
+    (dict(head_stride=8), 1), (dict(slot_stride=65), 1)]
+
+
+def _append(changed=None, **changes):
+    a = dict(qkv=GOOD, row=2048, positions=GOOD, slots=GOOD, cos=GOOD, sin=GOOD, rows=100,
+             cache=_cache(**(changed or {})), page=16, tokens=3, heads=12, kv_heads=2, dim=128, q=GOOD) | changes
+    return _lib.library().aoto_hip_paged_rope_append_mx4(*a.values(), None, None)
+
+
+@pytest.mark.parametrize("changes,code", [
+    (dict(qkv=None), 1), (dict(positions=None), 1), (dict(slots=None), 1), (dict(cos=None), 1), (dict(sin=None), 1),
+    (dict(q=None), 1), (dict(rows=0), 1), (dict(page=0), 1), (dict(page=2 ** 20 + 1), 1), (dict(tokens=0), 1),
+    (dict(heads=0), 1), (dict(kv_heads=0), 1), (dict(dim=96), 4), (dict(dim=0), 1), (dict(row=2049), 1),
+    (dict(qkv=ctypes.c_void_p(4098)), 1), (dict(q=ctypes.c_void_p(4104)), 1), (dict(heads=2 ** 30), 4)])
+def test_append_refuses(changes, code):
+    _refused(_append(**changes), code, "paged_rope_append_mx4")
+
+
+@pytest.mark.parametrize("changes,code", CACHE_REFUSALS)
+def test_every_entry_point_refuses_a_bad_cache(changes, code):
+    _refused(_append(changes), code, "paged_rope_append_mx4")
+    _refused(_unpack(changes), code, "paged_unpack_mx4")
+    _refused(_attention(changes), code, "paged_attention_mx4")
+
+
+def _unpack(changed=None, **changes):
+    a = dict(cache=_cache(**(changed or {})), page=16, kv_heads=2, dim=128, keys=GOOD, values=GOOD) | changes
+    return _lib.library().aoto_hip_paged_unpack_mx4(*a.values(), None)
+
+
+@pytest.mark.parametrize("changes,code", [
+    (dict(keys=None), 1), (dict(values=None), 1), (dict(keys=ctypes.c_void_p(4100)), 1), (dict(dim=32), 4),
+    (dict(page=2 ** 20, kv_heads=16), 4), (dict(cache=None), 1)])
+def test_unpack_refuses(changes, code):
+    _refused(_unpack(**changes), code, "paged_unpack_mx4")
+
+
+def _attention(changed=None, **changes):
+    a = dict(q=GOOD, q_token=1536, q_head=128, cache=_cache(**(changed or {})), page=16, tables=GOOD, stride=8,
+             blocks=8, start=GOOD, kv=GOOD, tokens=3, requests=2, heads=12, kv_heads=2, dim=128, causal=1, scale=0.125,
+             rows=0, length=0, workspace=GOOD, out=GOOD) | changes
+    return _lib.library().aoto_hip_paged_attention_mx4(*a.values(), None)
+
+
+@pytest.mark.parametrize("changes,code", [
+    (dict(q=None), 1), (dict(tables=None), 1), (dict(start=None), 1), (dict(kv=None), 1), (dict(out=None), 1),
+    (dict(cache=None), 1), (dict(tokens=0), 1), (dict(requests=0), 1), (dict(blocks=0), 1), (dict(stride=7), 1),
+    (dict(heads=13), 1), (dict(kv_heads=0), 1), (dict(dim=192), 4), (dict(q_head=68), 1),
+    (dict(q=ctypes.c_void_p(4104)), 1), (dict(out=ctypes.c_void_p(4104)), 1), (dict(rows=-1), 1), (dict(length=-1), 1),
+    *[(dict(scale=v), 1) for v in (0.0, -0.125, math.inf, math.nan)],
+    (dict(blocks=2 ** 24 + 1, stride=2 ** 25), 4), (dict(heads=129, kv_heads=1), 4)])
+def test_attention_refuses(changes, code):
+    _refused(_attention(**changes), code, "paged_attention_mx4")
+
+
+def _fork(**changes):
+    a = dict(parents=GOOD, lens=GOOD, tables=GOOD, stride=8, counts=GOOD, shares=GOOD, free=GOOD, start=GOOD,
+             requests=4, blocks=8, count=100, pages=50, page=16, lens_out=GOOD, counts_out=GOOD, start_out=GOOD,
+             source=GOOD, target=GOOD, plan=GOOD) | changes
+    return _lib.library().aoto_hip_paged_fork(*a.values(), None, None)
+
+
+@pytest.mark.parametrize("changes,code", [
+    *[({name: None}, 1) for name in ("parents", "lens", "tables", "counts", "shares", "free", "start", "lens_out",
+                                     "counts_out", "start_out", "source", "target", "plan")],
+    (dict(requests=0), 1), (dict(blocks=0), 1), (dict(count=-1), 1), (dict(pages=0), 1), (dict(page=0), 1),
+    (dict(stride=7), 1), (dict(blocks=2 ** 20 + 1, stride=2 ** 21), 4), (dict(page=2 ** 20 + 1), 4)])
+def test_fork_refuses(changes, code):
+    _refused(_fork(**changes), code, "paged_fork")
+
+
+def _release(**changes):
+    a = dict(keep=GOOD, tables=GOOD, stride=8, counts=GOOD, shares=GOOD, free=GOOD, start=GOOD, requests=4, blocks=8,
+             count=100, pages=50, page=16, counts_out=GOOD, start_out=GOOD) | changes
+    return _lib.library().aoto_hip_paged_release(*a.values(), None, None)
+
+
+@pytest.mark.parametrize("changes,code", [
+    *[({name: None}, 1) for name in ("keep", "tables", "counts", "shares", "free", "start", "counts_out", "start_out")],
+    (dict(requests=0), 1), (dict(blocks=0), 1), (dict(count=-1), 1), (dict(pages=0), 1), (dict(page=0), 1),
+    (dict(stride=7), 1), (dict(blocks=2 ** 20 + 1, stride=2 ** 21), 4), (dict(page=2 ** 20 + 1), 4)])
+def test_release_refuses(changes, code):
+    _refused(_release(**changes), code, "paged_release")
+
+
+def _compact(**changes):
+    a = dict(tables=GOOD, stride=8, counts=GOOD, shares=GOOD, free=GOOD, start=GOOD, requests=4, blocks=8, count=100,
+             pages=50, source=GOOD, target=GOOD, moved=GOOD, state=GOOD) | changes
+    return _lib.library().aoto_hip_paged_compact(*a.values(), None, None)
+
+
+@pytest.mark.parametrize("changes,code", [
+    *[({name: None}, 1) for name in ("tables", "counts", "shares", "free", "start", "source", "target", "moved",
+                                     "state")],
+    (dict(requests=0), 1), (dict(blocks=0), 1), (dict(count=-1), 1), (dict(pages=0), 1), (dict(stride=7), 1),
+    (dict(blocks=2 ** 20 + 1, stride=2 ** 21), 4)])
+def test_compact_refuses(changes, code):
+    _refused(_compact(**changes), code, "paged_compact")
+
+
+def _copy(tensor=None, **changes):
+    t = dict(data=4096, planes=2, plane_stride=4096, page_stride=64, page_bytes=64) | (tensor or {})
+    a = dict(tensors=ctypes.byref(_lib.PageTensorArg(*t.values())), count=1, pages=4, source=GOOD, target=GOOD,
+             pairs=3) | changes
+    return _lib.library().aoto_hip_paged_copy(*a.values(), None, None, None)
+
+
+@pytest.mark.parametrize("tensor,changes,code", [
+    ({}, dict(tensors=None), 1), ({}, dict(source=None), 1), ({}, dict(target=None), 1), ({}, dict(count=0), 1),
+    ({}, dict(pages=0), 1), ({}, dict(pairs=0), 1), (dict(data=None), {}, 1), (dict(planes=0), {}, 1),
+    (dict(page_bytes=0), {}, 1), (dict(planes=2 ** 20 + 1), {}, 4), (dict(page_bytes=2 ** 35), {}, 4),
+    (dict(planes=2 ** 19, page_bytes=2 ** 33), {}, 4)])
+def test_copy_refuses(tensor, changes, code):
+    _refused(_copy(tensor, **changes), code, "paged_copy")
+
+
+def _adjust(fields=None, **changes):
+    arg = _lib.AdjustmentsArg()
+    for name, value in (fields or {}).items():
+        setattr(arg, name, value)
+    a = dict(logits=GOOD, f32=0, row=1000, rows=9, vocab=1000, requests=3, adjust=ctypes.byref(arg), out=GOOD,
+             out_row=1000) | changes
+    return _lib.library().aoto_hip_adjust_logits(*a.values(), None)
+
+
+@pytest.mark.parametrize("adjust,changes,code", [
+    ({}, dict(logits=None), 1), ({}, dict(out=None), 1), ({}, dict(adjust=None), 1), ({}, dict(rows=0), 1),
+    ({}, dict(vocab=0), 1), ({}, dict(requests=0), 1), ({}, dict(vocab=2 ** 30 + 1), 4), ({}, dict(requests=65536), 4),
+    ({}, dict(logits=ctypes.c_void_p(4097)), 1), ({}, dict(f32=1, out=ctypes.c_void_p(4098)), 1),
+    (dict(history_len=5), {}, 1), (dict(drafts=2), {}, 1), (dict(biases=2), {}, 1),
+    (dict(biases=2, bias_tokens=4096), {}, 1), (dict(history_len=-1), {}, 1), (dict(drafts=-1), {}, 1),
+    (dict(history_len=2 ** 30, history=4096), {}, 4)])
+def test_adjust_refuses(adjust, changes, code):
+    _refused(_adjust(adjust, **changes), code, "adjust_logits")
+
+
+def _host_cache():
+    return ops.PagedMx4(*(torch.zeros((1, 1, 1, n), dtype=torch.uint8) for n in (32, 32, 2, 2)))
+
+
+@pytest.mark.parametrize("call", [
+    lambda i, b, l: ops.paged_rope_append_mx4(l, i.long(), i.long(), l, l, _host_cache(), query_heads=1),
+    lambda i, b, l: ops.paged_unpack_mx4(_host_cache()),
+    lambda i, b, l: ops.paged_attention_mx4(l, _host_cache(), b, i, i),
+    lambda i, b, l: ops.paged_fork(i, i, b, i, i, i, i, page_size=16),
+    lambda i, b, l: ops.paged_release(i, b, i, i, i, i, page_size=16),
+    lambda i, b, l: ops.paged_compact(b, i, i, i, i),
+    lambda i, b, l: ops.paged_copy(l, i, i),
+    lambda i, b, l: ops.adjust_logits(l)])
+def test_host_tensors_are_refused(call):
+    with pytest.raises(ValueError, match="on the GPU"):
+        call(torch.zeros(1, dtype=torch.int32), torch.zeros((1, 1), dtype=torch.int32),
+             torch.zeros((1, 1), dtype=torch.bfloat16))
+
+
+def test_other_types_are_refused():
+    with pytest.raises(TypeError, match="bf16 or f32"):
+        ops.adjust_logits(torch.zeros((1, 8), dtype=torch.float16))
+    with pytest.raises(TypeError, match="PagedMx4"):
+        ops.paged_unpack_mx4(torch.zeros(1))
+    with pytest.raises(ValueError, match="multiples of 64"):
+        ops.paged_mx4_cache(4, 2, 16, 96, device="cpu")
+
+
+def test_a_new_cache_is_zero():
+    cache = ops.paged_mx4_cache(3, 2, 5, 128, device="cpu")
+    assert [tuple(t.shape) for t in cache] == [(3, 2, 5, 64)] * 2 + [(3, 2, 5, 4)] * 2
+    assert all(t.dtype == torch.uint8 and not t.any() for t in cache)
+    assert all(t.data_ptr() % 16 == 0 for t in cache[:2]) and cache.keys.stride() == cache.values.stride()
+
+
+# ---------------------------------------------------------------- the restatements
+def test_codes_of_the_restatement():
+    x = np.zeros((1, 32))
+    x[0, :16] = [7.0, 6.0, 5.0, 5.01, 3.5, 2.5, 1.75, 1.25, 0.75, 0.25, 0.26, -0.25, -0.75, -7.0, -3.49, 2.0]
+    codes, scales = oracle.mx4_pack(x)
+    assert scales.tolist() == [[127]]
+    np.testing.assert_array_equal(oracle.mx4_unpack(codes, scales)[0, :16],
+                                  [6, 6, 4, 6, 4, 2, 2, 1, 1, 0, 0.5, -0.0, -1, -6, -3, 2])
+    x[0, 0] = 7.001  # the next power of two
+    assert oracle.mx4_pack(x)[1].tolist() == [[128]]
+    for value, byte in ((0.0, 1), (1e-44, 1), (3e38, 252), (np.inf, 255), (np.nan, 255)):
+        x[:] = 0
+        x[0, 5] = value
+        codes, scales = oracle.mx4_pack(x)
+        assert scales.tolist() == [[byte]]
+        assert np.isnan(oracle.mx4_unpack(codes, scales)).all() == (byte == 255)
+
+
+def test_pages_of_the_restatement():
+    tables = np.array([[4, 7, 2], [-1, -1, -1], [-1, -1, -1], [5, -1, -1]], np.int32)
+    shares, free = np.zeros(8, np.int32), np.array([9, 0, 6, 1, 3], np.int32)
+    lens, counts, start, source, target, tables, shares, error = oracle.fork(
+        [-1, 0, 0, -1], [40, 0, 0, 16], tables, [3, 0, 0, 1], shares, free, 1, 16)
+    assert (lens.tolist(), counts.tolist(), int(start[0]), error) == ([40, 40, 40, 16], [3, 3, 3, 1], 3, 0)
+    assert (source.tolist(), target.tolist()) == ([-1, 2, 2, -1], [-1, 0, 6, -1])
+    assert tables[1].tolist() == [4, 7, 0] and tables[2].tolist() == [4, 7, 6]
+    assert shares.tolist() == [0, 0, 0, 0, 2, 0, 0, 2]
+    counts, start, free, shares, error = oracle.release([0, 17, -1, 0], tables, counts, shares, free, start[0], 16)
+    assert (counts.tolist(), int(start[0]), error) == ([0, 2, 3, 0], 0, 0)
+    assert free.tolist() == [5, 2, 0, 1, 3] and shares.tolist() == [0, 0, 0, 0, 1, 0, 0, 1]
+    # held: 4, 7, 6; free: 0, 1, 2, 3, 5
+    source, target, count, tables, shares, free, error = oracle.compact(tables, counts, shares, free, 0)
+    assert (source[:3].tolist(), target[:3].tolist(), int(count[0]), error) == ([4, 6, 7], [0, 1, 2], 3, 0)
+    assert tables[1, :2].tolist() == [0, 2] and tables[2].tolist() == [0, 2, 1]
+    assert shares.tolist() == [1, 0, 1, 0, 0, 0, 0, 0] and free.tolist() == [3, 4, 5, 6, 7]
+
+
+def test_adjustments_of_the_restatement():
+    z = np.array([[2.0, -2.0, 1.0, 0.5, 0.0, 3.0]] * 2)
+    out, _, written = oracle.adjust(
+        z, [0, 2], np.array([[0, 1, 1, 5]]), [3], [1], np.array([[2]]), [2.0], [0.5], [0.25], np.array([[3, 3, -1, 9]]),
+        np.array([[7.0, 1.0, 5.0, 5.0]]), np.array([[0b101111], [-1]], np.int32))
+    np.testing.assert_array_equal(out[0], [1.0, -5.0, 1.0, 1.5, -np.inf, 3.0])
+    np.testing.assert_array_equal(out[1], [1.0, -5.0, -0.25, 1.5, 0.0, 3.0])
+    assert written.all()
