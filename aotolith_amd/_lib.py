@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import hashlib
 import os
+import struct
 import threading
 import weakref
 
@@ -149,7 +150,7 @@ SIGNATURES: dict[str, tuple] = {
         _p, _p, _p, _i64, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _c_int, _p, _p, _p, _p, _p, _p, _p, _p,
     ),
     "aoto_hip_paged_release": (
-        _p, _p, _i64, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _c_int, _p, _p, _p, _p,
+        _p, _p, _i64, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _c_int, _p, _p, _p, _p, _p,
     ),
     "aoto_hip_paged_compact": (
         _p, _i64, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _p, _p, _p, _p, _p, _p,
@@ -159,29 +160,11 @@ SIGNATURES: dict[str, tuple] = {
 }
 
 
-class Mx4CacheArg(ctypes.Structure):
-    """``aoto_mx4_cache``."""
-
-    _fields_ = [(name, _p) for name in ("keys", "values", "key_scales", "value_scales")] + [
-        (name, _i64) for name in ("page_stride", "head_stride", "slot_stride", "scale_page_stride",
-                                  "scale_head_stride", "scale_slot_stride")] + [("pages", ctypes.c_int32)]
-
-
-class PageTensorArg(ctypes.Structure):
-    """``aoto_page_tensor``."""
-
-    _fields_ = [("data", _p)] + [(name, _i64) for name in ("planes", "plane_stride", "page_stride", "page_bytes")]
-
-
-class AdjustmentsArg(ctypes.Structure):
-    """``aoto_adjustments``."""
-
-    _fields_ = [(name, _p) for name in (
-        "query_start", "history", "history_lens", "prompt_lens", "draft_tokens", "repetition", "presence", "frequency",
-        "bias_tokens", "bias_values", "allowed")] + [(name, _i64) for name in (
-            "history_stride", "draft_stride", "bias_stride", "value_stride", "allowed_stride")] + [
-        (name, ctypes.c_int32) for name in ("history_len", "drafts", "biases")]
-
+#: The structs of the C ABI as the bytes an entry point reads (packing them takes a third of filling a
+#: ``ctypes.Structure``): ``aoto_mx4_cache``, ``aoto_page_tensor``, ``aoto_adjustments``.
+MX4_CACHE = struct.Struct("4P6qi4x")
+PAGE_TENSOR = struct.Struct("P4q")
+ADJUSTMENTS = struct.Struct("11P5q3i4x")
 
 #: Entry points returning a size rather than a status.
 SIZE_RETURNING = {"aoto_hip_last_error", "aoto_hip_take_launches", "aoto_hip_decode_attention_workspace",

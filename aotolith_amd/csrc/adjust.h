@@ -8,7 +8,9 @@
 //
 // A block takes 2048 tokens of the vocabulary, eight a thread, for all rows of a request. The text is counted by
 // passing over it once in every block: counters of the block's own tokens in LDS, then in registers, where the drafts
-// are added row by row. Nothing of the size of the vocabulary is kept between launches.
+// are added row by row. Nothing of the size of the vocabulary is kept between launches. Four rows are on their way at a
+// time, the first four while the text is counted. With out = logits, threads whose tokens nothing changes neither read
+// nor write.
 #pragma once
 
 #include "common.h"
@@ -16,9 +18,16 @@
 
 namespace aoto {
 
+// Eight logits at an address of their type's alignment: global memory takes wide loads and stores at any.
+template <bool F32>
+struct __attribute__((packed, aligned(F32 ? 4 : 2))) AdjustEight {
+  uint32_t w[F32 ? 8 : 4];
+};
+
 template <bool F32>
 __device__ void adjust_logits(const AdjustArgs& a) {
-  constexpr int SIZE = F32 ? 4 : 2;
+  using Eight = AdjustEight<F32>;
+  constexpr int SIZE = F32 ? 4 : 2, ROWS = 4;
   constexpr uint32_t SEEN = 0x80000000u;
   __shared__ uint32_t s_text[kAdjustChunk];  // bit 31: in the text; below it: how often in the answer
   __shared__ int s_bias[kAdjustChunk];       // the last entry of the list that names the token, and one
@@ -27,27 +36,70 @@ __device__ void adjust_logits(const AdjustArgs& a) {
   const int end = a.query_start ? min(max(a.query_start[r + 1], first), a.rows) : min(r + 1, a.rows);
   if (first >= end) return;
   const int v0 = blockIdx.x * kAdjustChunk, own = v0 + 8 * tid;
+  const int count = min(8, a.vocab - own);  // tokens of this thread, none where not above 0
+  const bool same = a.logits == a.out;
+  const char* in = static_cast<const char*>(a.logits) + ((long long)first * a.row_stride + own) * SIZE;
+  char* out = static_cast<char*>(a.out) + ((long long)first * a.out_stride + own) * SIZE;
+  const uint8_t* allowed = a.allowed ? a.allowed + first * a.allowed_stride + (own >> 3) : nullptr;
+  Eight raw[ROWS];
+  uint32_t mask[ROWS];
+  // rows row .. row + 3, as far as there are; `all`: their logits too
+  auto load = [&](int row, bool all) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      mask[i] = 0xFFu;
+      if (row + i >= end || count <= 0) continue;
+      if (allowed) mask[i] = allowed[(long long)(row + i - first) * a.allowed_stride];
+      if (!all) continue;
+      const char* at = in + (long long)(row + i - first) * a.row_stride * SIZE;
+      if (count == 8) {
+        raw[i] = *reinterpret_cast<const Eight*>(at);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if constexpr (F32) {
+            raw[i].w[k] = k < count ? reinterpret_cast<const uint32_t*>(at)[k] : 0u;
+          } else {
+            const uint32_t half = k < count ? reinterpret_cast<const uint16_t*>(at)[k] : 0u;
+            raw[i].w[k >> 1] = k & 1 ? raw[i].w[k >> 1] | half << 16 : half;
+          }
+        }
+      }
+    }
+  };
+  if (!same) load(first, true);
+  const float repetition = a.repetition ? a.repetition[r] : 1.f;
+  const float presence = a.presence ? a.presence[r] : 0.f, frequency = a.frequency ? a.frequency[r] : 0.f;
   uint32_t text[8] = {};
   float bias[8] = {};
   bool touched = false;
   if (a.history_len > 0 || a.biases > 0) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) s_text[256 * i + tid] = 0, s_bias[256 * i + tid] = 0;
-    __syncthreads();
     const int told = a.history_lens ? a.history_lens[r] : a.history_len;
     const int len = min(max(told, 0), a.history_len);
     const int prompt = a.prompt_lens ? a.prompt_lens[r] : 0;
     const long long* history = a.history + r * a.history_stride;
-#pragma unroll 8
-    for (int j = tid; j < len; j += 256) {
-      const unsigned long long at = (unsigned long long)(history[j] - v0);
-      if (at < kAdjustChunk) {
-        atomicOr(&s_text[at], SEEN);
-        if (j >= prompt) atomicAdd(&s_text[at], 1u);
+    __syncthreads();
+    constexpr int SOME = 8;  // tokens of the text that a thread asks for at a time
+    for (int base = 0; base < len; base += 256 * SOME) {
+      long long token[SOME];
+#pragma unroll
+      for (int i = 0; i < SOME; ++i) {
+        const int j = base + 256 * i + tid;
+        token[i] = j < len ? history[j] : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < SOME; ++i) {
+        const unsigned long long at = (unsigned long long)token[i] - v0;
+        if (at < kAdjustChunk) {
+          atomicOr(&s_text[at], SEEN);
+          if (base + 256 * i + tid >= prompt) atomicAdd(&s_text[at], 1u);
+        }
       }
     }
     for (int j = tid; j < a.biases; j += 256) {
-      const unsigned long long at = (unsigned long long)(a.bias_tokens[r * a.bias_stride + j] - v0);
+      const unsigned long long at = (unsigned long long)a.bias_tokens[r * a.bias_stride + j] - v0;
       if (at < kAdjustChunk) atomicMax(&s_bias[at], j + 1);
     }
     __syncthreads();
@@ -59,73 +111,66 @@ __device__ void adjust_logits(const AdjustArgs& a) {
       touched |= text[i] != 0 || entry != 0;
     }
   }
-  if (own >= a.vocab) return;
-  const int count = min(8, a.vocab - own);
-  const float repetition = a.repetition ? a.repetition[r] : 1.f;
-  const float presence = a.presence ? a.presence[r] : 0.f, frequency = a.frequency ? a.frequency[r] : 0.f;
-  const char* in = static_cast<const char*>(a.logits) + ((long long)first * a.row_stride + own) * SIZE;
-  char* out = static_cast<char*>(a.out) + ((long long)first * a.out_stride + own) * SIZE;
-  const uint8_t* allowed = a.allowed ? a.allowed + first * a.allowed_stride + (own >> 3) : nullptr;
-  for (int row = first; row < end; ++row) {
-    const uint32_t mask = allowed ? *allowed : 0xFFu;
-    float z[8];
-    uint4 raw[F32 ? 2 : 1];
-    const bool whole = count == 8 && ((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-    if (whole) {
-#pragma unroll
-      for (int i = 0; i < (F32 ? 2 : 1); ++i) raw[i] = reinterpret_cast<const uint4*>(in)[i];
-      if constexpr (F32) {
-        z[0] = __uint_as_float(raw[0].x), z[1] = __uint_as_float(raw[0].y);
-        z[2] = __uint_as_float(raw[0].z), z[3] = __uint_as_float(raw[0].w);
-        z[4] = __uint_as_float(raw[1].x), z[5] = __uint_as_float(raw[1].y);
-        z[6] = __uint_as_float(raw[1].z), z[7] = __uint_as_float(raw[1].w);
-      } else {
-        z[0] = bf16_lo(raw[0].x), z[1] = bf16_hi(raw[0].x), z[2] = bf16_lo(raw[0].y), z[3] = bf16_hi(raw[0].y);
-        z[4] = bf16_lo(raw[0].z), z[5] = bf16_hi(raw[0].z), z[6] = bf16_lo(raw[0].w), z[7] = bf16_hi(raw[0].w);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < count)
-          z[i] = F32 ? reinterpret_cast<const float*>(in)[i] : bf16_to_f32(reinterpret_cast<const uint16_t*>(in)[i]);
-    }
-    if (touched) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (text[i]) z[i] = z[i] > 0.f ? z[i] / repetition : z[i] * repetition;
-        const uint32_t said = text[i] & ~SEEN;
-        if (said) z[i] -= frequency * (float)said + presence;
-        z[i] += bias[i];
-      }
+  if (count <= 0) return;
+  for (int row = first; row < end; row += ROWS) {
+    if (row > first || same) {
+      // which of the next drafts are this thread's tokens is known before their rows are
+      bool later = touched;
+      for (int i = row - first; i < min(row - first + ROWS - 1, a.drafts); ++i)
+        later |= (unsigned long long)a.draft_tokens[r * a.draft_stride + i] - own < 8;
+      load(row, !same || later || allowed);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (!(mask >> i & 1)) z[i] = -INFINITY;
-    if (whole) {
-      if constexpr (F32) {
-        reinterpret_cast<float4*>(out)[0] = make_float4(z[0], z[1], z[2], z[3]);
-        reinterpret_cast<float4*>(out)[1] = make_float4(z[4], z[5], z[6], z[7]);
-      } else {
-        *reinterpret_cast<uint4*>(out) = make_uint4(pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3]),
-                                                    pack_bf16x2(z[4], z[5]), pack_bf16x2(z[6], z[7]));
-      }
-    } else {
+    for (int i = 0; i < ROWS; ++i) {
+      if (row + i >= end) break;
+      if (!same || touched || mask[i] != 0xFFu) {
+        char* to = out + (long long)(row + i - first) * a.out_stride * SIZE;
+        Eight made = raw[i];
+        if (touched || mask[i] != 0xFFu) {
+          float z[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < count) {
-          if constexpr (F32) reinterpret_cast<float*>(out)[i] = z[i];
-          else reinterpret_cast<uint16_t*>(out)[i] = (uint16_t)f32_to_bf16(z[i]);
+          for (int k = 0; k < 8; ++k)
+            z[k] = F32 ? __uint_as_float(raw[i].w[k]) : k & 1 ? bf16_hi(raw[i].w[k >> 1]) : bf16_lo(raw[i].w[k >> 1]);
+          if (touched) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              if (text[k]) z[k] = z[k] > 0.f ? z[k] / repetition : z[k] * repetition;
+              const uint32_t said = text[k] & ~SEEN;
+              if (said) z[k] -= frequency * (float)said + presence;
+              z[k] += bias[k];
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (!(mask[i] >> k & 1)) z[k] = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            if constexpr (F32) made.w[k] = __float_as_uint(z[k]);
+            else if (k & 1) made.w[k >> 1] = cvt_pk_bf16(z[k - 1], z[k]);
+          }
         }
-    }
-    in += a.row_stride * SIZE, out += a.out_stride * SIZE;
-    if (allowed) allowed += a.allowed_stride;
-    // the draft that this row judges is in the text of the rows behind it
-    const int i = row - first;
-    if (i < a.drafts) {
-      const unsigned long long at = (unsigned long long)(a.draft_tokens[r * a.draft_stride + i] - own);
+        if (count == 8) {
+          *reinterpret_cast<Eight*>(to) = made;
+        } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (at == (unsigned long long)k) text[k] = (text[k] + 1) | SEEN, touched = true;
+          for (int k = 0; k < 8; ++k)
+            if (k < count) {
+              if constexpr (F32) reinterpret_cast<uint32_t*>(to)[k] = made.w[k];
+              else reinterpret_cast<uint16_t*>(to)[k] = (uint16_t)(made.w[k >> 1] >> (16 * (k & 1)));
+            }
+        }
+      }
+      // the draft that this row judges is in the text of the rows behind it
+      const int draft = row + i - first;
+      if (draft < a.drafts) {
+        const unsigned long long at = (unsigned long long)a.draft_tokens[r * a.draft_stride + draft] - own;
+        if (at < 8) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (at == (unsigned long long)k) text[k] = (text[k] + 1) | SEEN;
+          touched = true;
+        }
+      }
     }
   }
 }

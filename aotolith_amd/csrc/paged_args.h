@@ -136,6 +136,9 @@ struct PagedForkArgs {
   int requests, max_blocks, free_count, pages, page;
 };
 
+// Pages that a block of paged_release looks at.
+constexpr int kPageChunk = 1024;
+
 struct PagedReleaseArgs {
   const int* keep_lens;
   const int* block_tables;
@@ -145,6 +148,7 @@ struct PagedReleaseArgs {
   const int* free_start;
   int* page_counts_out;
   int* free_start_out;
+  int* scratch;  // the list's start as it was, then the pages given back in each kPageChunk
   int* error;
   long long table_stride;
   int requests, max_blocks, free_count, pages, page;
@@ -163,6 +167,7 @@ struct PagedCompactArgs {
   int* error;
   long long table_stride;
   int requests, max_blocks, free_count, pages;
+  int list_blocks;  // of aoto_paged_mark, that go over the free list
 };
 
 // What a copy of pages moves: planes of pages of one size.
@@ -183,6 +188,7 @@ struct PagedCopyArgs {
   const int* count;  // pairs in use, or NULL: all
   int* error;
   int pairs, pages, tensors, planes, chunks;  // planes of all tensors, chunks of the longest page
+  int blocks;                                 // of the launch
   int wide;                                   // everything a multiple of 16 bytes
   PagedCopyTensor at[kPagedCopyTensors];
 };

@@ -47,6 +47,18 @@ AOTO_DEVICE void page_ranks(uint32_t bits, int (&before)[kPageSteps], int& total
   __syncthreads();
 }
 
+// Four neighbours of a list, 0 past its end.
+struct __attribute__((packed, aligned(4))) PageFour {
+  int v[4];
+};
+AOTO_DEVICE PageFour page_four(const int* values, int from, int count) {
+  if (from + 4 <= count) return *reinterpret_cast<const PageFour*>(values + from);
+  PageFour four;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) four.v[e] = from + e < count ? values[from + e] : 0;
+  return four;
+}
+
 }  // namespace aoto
 
 // Which rows go on from which, the pages taken for them and what is to be copied (formulas at the entry point's
@@ -138,40 +150,60 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_drop(PagedReleaseAr
   }
 }
 
-// The pages left without a holder, in the order of their numbers, to the places before the free list's first. One
-// block: 8192 pages a round trip.
-extern "C" __global__ __launch_bounds__(1024) void aoto_paged_reclaim(PagedReleaseArgs a) {
+// The pages left without a holder, in the order of their numbers, to the places before the free list's first: their
+// number in each 1024 pages, then their places. (In one launch a block would have to read the whole pool for its own
+// place, at a single CU's 20 GB/s: 15 us for 41000 pages instead of RECLAIM_FIGURE.)
+extern "C" __global__ __launch_bounds__(256) void aoto_paged_gone(PagedReleaseArgs a) {
   using namespace aoto;
-  __shared__ int s_scratch[kPageRanks];
-  const int tid = threadIdx.x;
-  const int start = a.free_start[0], first = min(max(start, 0), a.free_count);
-  int freed = 0, error = 0;
-  for (int base = 0; base < a.pages; base += kPageBatch) {
-    int share[kPageSteps];
+  __shared__ int s_count[4];
+  const int wave = threadIdx.x >> 6, chunk = blockIdx.x;
+  const PageFour share = page_four(a.shares, kPageChunk * chunk + 4 * threadIdx.x, a.pages);
+  int count = 0;
 #pragma unroll
-    for (int i = 0; i < kPageSteps; ++i) {
-      const int page = base + 1024 * i + tid;
-      share[i] = page < a.pages ? a.shares[page] : 0;
-    }
-    uint32_t bits = 0;
+  for (int e = 0; e < 4; ++e) count += __popcll(__ballot(share.v[e] < 0));
+  if ((threadIdx.x & 63) == 0) s_count[wave] = count;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  a.scratch[1 + chunk] = s_count[0] + s_count[1] + s_count[2] + s_count[3];
+  if (chunk == 0) a.scratch[0] = a.free_start[0];  // the start written may be the start read
+}
+
+extern "C" __global__ __launch_bounds__(256) void aoto_paged_reclaim(PagedReleaseArgs a) {
+  using namespace aoto;
+  __shared__ int s_count[4], s_before[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, chunk = blockIdx.x;
+  const int from = kPageChunk * chunk + 4 * tid;
+  const PageFour share = page_four(a.shares, from, a.pages);
+  int before = 0;
+  for (int i = tid; i < chunk; i += 256) before += a.scratch[1 + i];
+  const int start = a.scratch[0], first = min(max(start, 0), a.free_count);
 #pragma unroll
-    for (int i = 0; i < kPageSteps; ++i) bits |= (uint32_t)(share[i] < 0) << i;
-    int before[kPageSteps], total;
-    page_ranks(bits, before, total, s_scratch);
+  for (int d = 1; d < 64; d <<= 1) before += __shfl_xor(before, d);
+  int count = 0, rank = 0;
+  const unsigned long long below = (1ull << lane) - 1;
 #pragma unroll
-    for (int i = 0; i < kPageSteps; ++i)
-      if (share[i] < 0) {
-        const int page = base + 1024 * i + tid, at = first - 1 - freed - before[i];
-        if (share[i] < -1) error |= AOTO_PAGED_BAD_SHARE;
-        a.shares[page] = 0;
-        if (at >= 0) a.free_pages[at] = page;
-        else error |= AOTO_PAGED_LIST_FULL;
-      }
-    freed += total;
+  for (int e = 0; e < 4; ++e) {
+    const unsigned long long lanes = __ballot(share.v[e] < 0);
+    count += __popcll(lanes), rank += __popcll(lanes & below);
   }
+  if (lane == 0) s_count[wave] = count, s_before[wave] = before;
+  __syncthreads();
+  before = s_before[0] + s_before[1] + s_before[2] + s_before[3];
+  int total = before;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) rank += w < wave ? s_count[w] : 0, total += s_count[w];
+  int error = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (share.v[e] < 0) {
+      const int at = first - 1 - before - rank++;
+      if (share.v[e] < -1) error |= AOTO_PAGED_BAD_SHARE;
+      a.shares[from + e] = 0;
+      if (at >= 0) a.free_pages[at] = from + e;
+      else error |= AOTO_PAGED_LIST_FULL;
+    }
   if (error && a.error) atomicOr(a.error, error);
-  __syncthreads();  // the start written may be the start read
-  if (tid == 0) a.free_start_out[0] = freed ? max(0, first - freed) : start;
+  if (tid == 0 && chunk == (a.pages - 1) / kPageChunk) a.free_start_out[0] = total ? max(0, first - total) : start;
 }
 
 // What each page is: 0, and then (aoto_paged_mark) 1 where a request holds it, 2 where it is in the free list.
@@ -191,7 +223,7 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_mark(PagedCompactAr
     }
     return;
   }
-  const int first = max(a.free_start[0], 0), others = gridDim.x - a.requests;
+  const int first = max(a.free_start[0], 0), others = a.list_blocks;
   for (long long j = first + (long long)(r - a.requests) * 256 + threadIdx.x; j < a.free_count; j += others * 256LL) {
     const int page = a.free_pages[j];
     if ((unsigned)page < (unsigned)a.pages) atomicOr(a.state + page, 2);
@@ -227,12 +259,11 @@ extern "C" __global__ __launch_bounds__(1024) void aoto_paged_moves(PagedCompact
   __syncthreads();
   int places = 0, held = 0;  // of the pages before
   for (int base = 0; base < a.pages; base += kPageBatch) {
-    int state[kPageSteps], share[kPageSteps];
+    int state[kPageSteps];
 #pragma unroll
     for (int i = 0; i < kPageSteps; ++i) {
       const int page = base + 1024 * i + tid;
       state[i] = page < a.pages ? a.state[page] : 0;
-      share[i] = page < a.pages ? a.shares[page] : 0;
     }
     uint32_t any = 0, is_held = 0;
 #pragma unroll
@@ -263,7 +294,7 @@ extern "C" __global__ __launch_bounds__(1024) void aoto_paged_moves(PagedCompact
           const int k = held_before[i] - s_low;
           a.source[k] = page;
           now = a.target[k];
-          a.shares[now] = share[i];
+          a.shares[now] = a.shares[page];
           a.shares[page] = 0;
         }
         const int at = first + place[i] - m;
@@ -293,43 +324,54 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_remap(PagedCompactA
   }
 }
 
-// Pages' contents from source[i] to target[i], in every plane of every tensor. A block takes chunks of 16 KB of a page
-// of a plane, those of one pair after the other's; every block passes over all pairs, so that pairs without a copy cost
-// no more than a look.
+// Pages' contents from source[i] to target[i], in every plane of every tensor. Every wave looks at 64 pairs at a time,
+// a lane each, and the block takes its share of the chunks (16 KB of a page of a plane) of those that are to be copied:
+// pairs without a copy cost a 64th of a look. The grid's size comes as an argument, and a thread's 64 bytes have names
+// of their own: what makes the compiler ask for the dispatch packet (gridDim, an array that it moves to LDS) is a read of
+// host memory by every block, 40 ns each one after the other (384 blocks without a page to copy: 15.6 us).
 extern "C" __global__ __launch_bounds__(256) void aoto_paged_copy(PagedCopyArgs a) {
+  const int lane = threadIdx.x & 63;
   const int pairs = a.count ? min(max(a.count[0], 0), a.pairs) : a.pairs;
-  const int each = a.planes * a.chunks;  // chunks of a pair
-  const long long items = (long long)pairs * each;
-  for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-    const int pair = (int)(item / each), within = (int)(item - (long long)pair * each);
-    const int source = a.source[pair], target = a.target[pair];
-    if ((unsigned)source >= (unsigned)a.pages || (unsigned)target >= (unsigned)a.pages) {
-      const bool bad = source < -1 || source >= a.pages || target < -1 || target >= a.pages;
-      if (bad && a.error && within == 0 && threadIdx.x == 0)
-        atomicOr(a.error, AOTO_PAGED_BAD_SLOT);
-      continue;
+  const unsigned each = (unsigned)a.planes * a.chunks;  // chunks of a pair
+  int error = 0;
+  unsigned next = blockIdx.x;  // this block's next chunk, counted from the present pairs' first
+  for (int base = 0; base < pairs; base += 64) {
+    const int mine = min(base + lane, pairs - 1);
+    const int source = a.source[mine], target = a.target[mine];
+    const bool inside = (unsigned)source < (unsigned)a.pages && (unsigned)target < (unsigned)a.pages;
+    const unsigned long long some = __ballot(inside && source != target && base + lane < pairs);
+    if (source < -1 || source >= a.pages || target < -1 || target >= a.pages) error = AOTO_PAGED_BAD_SLOT;
+    const unsigned long long chunks = (unsigned long long)__popcll(some) * each;
+    const int rank = __popcll(some & ((1ull << lane) - 1));
+    unsigned long long item = next;
+    for (; item < chunks; item += a.blocks) {
+      const int pair = (int)(item < 0x80000000ull ? (unsigned)item / each : item / each);
+      const unsigned within = (unsigned)(item - (unsigned long long)pair * each);
+      const int at_lane = __ffsll(__ballot(some >> lane & 1 && rank == pair)) - 1;
+      const int from_page = __builtin_amdgcn_readlane(source, at_lane);
+      const int to_page = __builtin_amdgcn_readlane(target, at_lane);
+      const int plane = a.chunks == 1 ? within : within / a.chunks, chunk = within - plane * a.chunks;
+      int t = 0;
+      while (t + 1 < a.tensors && a.at[t + 1].first <= plane) ++t;
+      const PagedCopyTensor& at = a.at[t];
+      if (chunk >= at.chunks) continue;
+      uint8_t* first = at.base + (plane - at.first) * at.plane_stride + (long long)chunk * kPagedCopyChunk;
+      const uint8_t* from = first + from_page * at.page_stride;
+      uint8_t* to = first + to_page * at.page_stride;
+      const int bytes = (int)min(at.bytes - (long long)chunk * kPagedCopyChunk, (long long)kPagedCopyChunk);
+      if (a.wide && bytes == kPagedCopyChunk) {
+        const uint4* f = reinterpret_cast<const uint4*>(from) + threadIdx.x;
+        uint4* t4 = reinterpret_cast<uint4*>(to) + threadIdx.x;
+        const uint4 v0 = f[0], v1 = f[256], v2 = f[512], v3 = f[768];
+        t4[0] = v0, t4[256] = v1, t4[512] = v2, t4[768] = v3;
+      } else if (a.wide) {
+        for (int b = threadIdx.x; b < bytes / 16; b += 256)
+          reinterpret_cast<uint4*>(to)[b] = reinterpret_cast<const uint4*>(from)[b];
+      } else {
+        for (int b = threadIdx.x; b < bytes; b += 256) to[b] = from[b];
+      }
     }
-    if (source == target) continue;
-    const int plane = within / a.chunks, chunk = within - plane * a.chunks;
-    int t = 0;
-    while (t + 1 < a.tensors && a.at[t + 1].first <= plane) ++t;
-    const PagedCopyTensor& at = a.at[t];
-    if (chunk >= at.chunks) continue;
-    uint8_t* base = at.base + (plane - at.first) * at.plane_stride + (long long)chunk * kPagedCopyChunk;
-    const uint8_t* from = base + source * at.page_stride;
-    uint8_t* to = base + target * at.page_stride;
-    const int bytes = (int)min(at.bytes - (long long)chunk * kPagedCopyChunk, (long long)kPagedCopyChunk);
-    if (a.wide && bytes == kPagedCopyChunk) {
-      uint4 v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = reinterpret_cast<const uint4*>(from)[256 * i + threadIdx.x];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(to)[256 * i + threadIdx.x] = v[i];
-    } else if (a.wide) {
-      for (int b = threadIdx.x; b < bytes / 16; b += 256)
-        reinterpret_cast<uint4*>(to)[b] = reinterpret_cast<const uint4*>(from)[b];
-    } else {
-      for (int b = threadIdx.x; b < bytes; b += 256) to[b] = from[b];
-    }
+    next = (unsigned)(item - chunks);
   }
+  if (error && a.error && blockIdx.x == 0) atomicOr(a.error, error);
 }

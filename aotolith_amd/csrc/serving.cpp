@@ -149,9 +149,10 @@ int aoto_hip_paged_fork(const int32_t* parents, const int32_t* context_lens, int
 int aoto_hip_paged_release(const int32_t* keep_lens, const int32_t* block_tables, int64_t table_stride,
                            const int32_t* page_counts, int32_t* shares, int32_t* free_pages,
                            const int32_t* free_start, int requests, int max_blocks, int free_count, int pages,
-                           int page, int32_t* page_counts_out, int32_t* free_start_out, int32_t* error, void* stream) {
+                           int page, int32_t* page_counts_out, int32_t* free_start_out, int32_t* scratch,
+                           int32_t* error, void* stream) {
   if (!keep_lens || !block_tables || !page_counts || !shares || (!free_pages && free_count) || !free_start ||
-      !page_counts_out || !free_start_out)
+      !page_counts_out || !free_start_out || !scratch)
     return set_error(AOTO_ERR_ARGUMENT, "paged_release: null pointer");
   if (requests <= 0 || max_blocks <= 0 || free_count < 0 || pages <= 0 || page <= 0 || table_stride < max_blocks)
     return set_error(AOTO_ERR_ARGUMENT, "paged_release: bad shape");
@@ -162,9 +163,11 @@ int aoto_hip_paged_release(const int32_t* keep_lens, const int32_t* block_tables
   a.keep_lens = keep_lens, a.block_tables = block_tables, a.page_counts = page_counts, a.shares = shares;
   a.free_pages = free_pages, a.free_start = free_start, a.page_counts_out = page_counts_out;
   a.free_start_out = free_start_out, a.error = error, a.table_stride = table_stride, a.requests = requests;
-  a.max_blocks = max_blocks, a.free_count = free_count, a.pages = pages, a.page = page;
+  a.max_blocks = max_blocks, a.free_count = free_count, a.pages = pages, a.page = page, a.scratch = scratch;
+  const int chunks = (pages - 1) / kPageChunk + 1;
   if (int s = launch("aoto_paged_drop", requests, 1, 256, stream, a)) return s;
-  return launch("aoto_paged_reclaim", 1, 1, 1024, stream, a);
+  if (int s = launch("aoto_paged_gone", chunks, 1, 256, stream, a)) return s;
+  return launch("aoto_paged_reclaim", chunks, 1, 256, stream, a);
 }
 
 int aoto_hip_paged_compact(int32_t* block_tables, int64_t table_stride, const int32_t* page_counts, int32_t* shares,
@@ -184,8 +187,8 @@ int aoto_hip_paged_compact(int32_t* block_tables, int64_t table_stride, const in
   a.table_stride = table_stride, a.requests = requests, a.max_blocks = max_blocks, a.free_count = free_count;
   a.pages = pages;
   if (int s = launch("aoto_paged_clear", (pages + 255LL) / 256, 1, 256, stream, a)) return s;
-  const long long lists = std::min(256LL, std::max(1LL, (free_count + 255LL) / 256));
-  if (int s = launch("aoto_paged_mark", requests + lists, 1, 256, stream, a)) return s;
+  a.list_blocks = (int)std::min(256LL, std::max(1LL, (free_count + 255LL) / 256));
+  if (int s = launch("aoto_paged_mark", (long long)requests + a.list_blocks, 1, 256, stream, a)) return s;
   if (int s = launch("aoto_paged_moves", 1, 1, 1024, stream, a)) return s;
   return launch("aoto_paged_remap", requests, 1, 256, stream, a);
 }
@@ -215,8 +218,8 @@ int aoto_hip_paged_copy(const aoto_page_tensor* tensors, int tensor_count, int p
     a.planes = (int)planes;
     if (planes * a.chunks > 0x7FFFFFFFLL) return set_error(AOTO_ERR_UNSUPPORTED, "paged_copy: pages too large");
     const long long items = planes * a.chunks * (long long)pairs;
-    // eight blocks a CU at most: one that ends takes the next of its chunks
-    if (int s = launch("aoto_paged_copy", std::min(items, 8LL * aoto::device_cu_count()), 1, 256, stream, a)) return s;
+    a.blocks = (int)std::min(items, 8LL * aoto::device_cu_count());  // what the chip holds at a time
+    if (int s = launch("aoto_paged_copy", a.blocks, 1, 256, stream, a)) return s;
   }
   return AOTO_OK;
 }

@@ -1582,28 +1582,42 @@ def paged_mx4_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, *,
     return PagedMx4(*codes.unbind(), *scales.unbind())
 
 
-def _expect_mx4(cache: PagedMx4, device: int) -> tuple[tuple, _lib.Mx4CacheArg]:
+def _expect_mx4(cache: PagedMx4, device: int) -> tuple[tuple, bytes]:
     """``(pages, Hkv, page, D)`` of a cache, and its descriptor for the C ABI."""
 
     if not isinstance(cache, PagedMx4):
         raise TypeError(f"cache must be a PagedMx4, got {type(cache).__name__}")
     keys, values, key_scales, value_scales = cache
-    for name, tensor in zip(cache._fields, cache):
-        _expect_rows(tensor, name, torch.uint8, 4, device)
-    shape, strides, scale_strides = keys.shape, keys.stride(), key_scales.stride()
-    if shape != values.shape or strides != values.stride():
-        raise ValueError("keys and values must have one shape and the same strides")
-    dim = 2 * shape[3]
-    if dim % 64:
-        raise ValueError(f"heads of a 4-bit cache have a multiple of 64 dims, got {dim}")
-    if tuple(key_scales.shape) != (*shape[:3], dim // 32) or key_scales.shape != value_scales.shape:
-        raise ValueError(f"key_scales and value_scales must be {(*shape[:3], dim // 32)}, got "
-                         f"{tuple(key_scales.shape)} and {tuple(value_scales.shape)}")
-    if scale_strides != value_scales.stride():
-        raise ValueError("key_scales and value_scales must have the same strides")
-    return (shape[0], shape[1], shape[2], dim), _lib.Mx4CacheArg(
+    u8 = torch.uint8
+    try:  # one pass over the attributes, the reasons only for a cache that fails
+        shape, strides, small, scale_strides = keys.shape, keys.stride(), key_scales.shape, key_scales.stride()
+        pages, kv_heads, page, half = shape
+        good = (keys.dtype is u8 and values.dtype is u8 and key_scales.dtype is u8 and value_scales.dtype is u8
+                and keys.get_device() == device and values.get_device() == device
+                and key_scales.get_device() == device and value_scales.get_device() == device
+                and values.shape == shape and values.stride() == strides and strides[3] == 1
+                and small == (pages, kv_heads, page, half // 16) and half % 32 == 0
+                and value_scales.shape == small and value_scales.stride() == scale_strides and scale_strides[3] == 1)
+    except (AttributeError, ValueError):
+        good = False
+    if not good:
+        for name, tensor in zip(cache._fields, cache):
+            _expect_rows(tensor, name, u8, 4, device)
+        shape, strides, scale_strides = keys.shape, keys.stride(), key_scales.stride()
+        if shape != values.shape or strides != values.stride():
+            raise ValueError("keys and values must have one shape and the same strides")
+        pages, kv_heads, page, half = shape
+        if half % 32:
+            raise ValueError(f"heads of a 4-bit cache have a multiple of 64 dims, got {2 * half}")
+        want = (pages, kv_heads, page, half // 16)
+        if tuple(key_scales.shape) != want or tuple(value_scales.shape) != want:
+            raise ValueError(f"key_scales and value_scales must be {want}, got {tuple(key_scales.shape)} and "
+                             f"{tuple(value_scales.shape)}")
+        if scale_strides != value_scales.stride():
+            raise ValueError("key_scales and value_scales must have the same strides")
+    return (pages, kv_heads, page, 2 * half), _lib.MX4_CACHE.pack(
         keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), *strides[:3],
-        *scale_strides[:3], shape[0])
+        *scale_strides[:3], pages)
 
 
 def paged_rope_append_mx4(
@@ -1647,7 +1661,7 @@ def paged_rope_append_mx4(
     _lib.check(
         _lib.library().aoto_hip_paged_rope_append_mx4(
             _ptr(qkv), qkv.stride(0), _ptr(positions), _ptr(slots), _ptr(cos_table), _ptr(sin_table),
-            cos_table.shape[0], ctypes.byref(arg), page, tokens, query_heads, kv_heads, dim, _ptr(q_out), _ptr(error),
+            cos_table.shape[0], arg, page, tokens, query_heads, kv_heads, dim, _ptr(q_out), _ptr(error),
             _stream(device),
         )
     )
@@ -1666,12 +1680,12 @@ def paged_unpack_mx4(cache: PagedMx4, *, out: tuple[torch.Tensor, torch.Tensor] 
     device = _on_current("keys", cache.keys)
     shape, arg = _expect_mx4(cache, device)
     if out is None:
-        out = tuple(torch.empty(shape, dtype=BF16, device=cache.keys.device) for _ in range(2))
+        out = torch.empty((2, *shape), dtype=BF16, device=cache.keys.device).unbind()
     else:
         keys_out, values_out = out
         _expect_all(device, ((keys_out, "out[0]", BF16, shape), (values_out, "out[1]", BF16, shape)))
     _ready(cache.keys)
-    _lib.check(_lib.library().aoto_hip_paged_unpack_mx4(ctypes.byref(arg), shape[2], shape[1], shape[3], _ptr(out[0]),
+    _lib.check(_lib.library().aoto_hip_paged_unpack_mx4(arg, shape[2], shape[1], shape[3], _ptr(out[0]),
                                                         _ptr(out[1]), _stream(device)))
     return out
 
@@ -1730,7 +1744,7 @@ def paged_attention_mx4(
         workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
     _lib.check(
         lib.aoto_hip_paged_attention_mx4(
-            _ptr(q), q.stride(0), q.stride(1), ctypes.byref(arg), page, _ptr(block_tables), block_tables.stride(0),
+            _ptr(q), q.stride(0), q.stride(1), arg, page, _ptr(block_tables), block_tables.stride(0),
             max_blocks, _ptr(query_start), _ptr(kv_lens), tokens, requests, query_heads, kv_heads, dim,
             int(bool(causal)), float(scale), max_query_len, max_kv_len, _ptr(workspace if need else None), _ptr(out),
             _stream(device),
@@ -1857,10 +1871,12 @@ def paged_release(
 
     device, requests = _expect_pool(block_tables, page_counts, shares, free_pages, free_start, error)
     _expect_all(device, ((keep_lens, "keep_lens", torch.int32, (requests,)),))
+    room = shares.numel() // 1024 + 2
     if out is None:
-        out = shares.new_empty((requests + 1,)).split_with_sizes((requests, 1))
+        counts_out, start_out, scratch = shares.new_empty((requests + 1 + room,)).split_with_sizes((requests, 1, room))
     else:
         counts_out, start_out = out
+        scratch = shares.new_empty((room,))
         _expect_all(device, ((counts_out, "out[0]", torch.int32, (requests,)),
                              (start_out, "out[1]", torch.int32, (1,))))
     _ready(shares)
@@ -1868,10 +1884,10 @@ def paged_release(
         _lib.library().aoto_hip_paged_release(
             _ptr(keep_lens), _ptr(block_tables), block_tables.stride(0), _ptr(page_counts), _ptr(shares),
             _ptr(free_pages), _ptr(free_start), requests, block_tables.shape[1], free_pages.numel(), shares.numel(),
-            int(page_size), _ptr(out[0]), _ptr(out[1]), _ptr(error), _stream(device),
+            int(page_size), _ptr(counts_out), _ptr(start_out), _ptr(scratch), _ptr(error), _stream(device),
         )
     )
-    return tuple(out)
+    return counts_out, start_out
 
 
 def paged_compact(
@@ -1915,7 +1931,8 @@ def paged_compact(
     return moves
 
 
-def _page_tensor(tensor: torch.Tensor, name: str, dim: int, pages: int | None, device: int) -> _lib.PageTensorArg:
+def _page_tensor(tensor: torch.Tensor, index: int, dim: int, pages: int | None, device: int) -> bytes:
+    name = f"caches[{index}]"
     if not isinstance(tensor, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(tensor).__name__}")
     if tensor.device.type != "cuda":
@@ -1946,7 +1963,7 @@ def _page_tensor(tensor: torch.Tensor, name: str, dim: int, pages: int | None, d
     low, high = sorted(((page_stride, shape[dim]), (plane_stride if planes > 1 else page_stride * shape[dim], planes)))
     if low[0] < dense or high[0] < low[0] * (low[1] - 1) + dense:
         raise ValueError(f"{name}'s pages overlap, got strides {strides}")
-    return _lib.PageTensorArg(tensor.data_ptr(), planes, plane_stride * size, page_stride * size, dense * size)
+    return _lib.PAGE_TENSOR.pack(tensor.data_ptr(), planes, plane_stride * size, page_stride * size, dense * size)
 
 
 def paged_copy(
@@ -1981,16 +1998,19 @@ def paged_copy(
     if not caches:
         raise ValueError("no caches")
     dim = int(dim)
-    args = (_lib.PageTensorArg * len(caches))()
-    pages = None
+    args, pages = [], None
     for i, tensor in enumerate(caches):
-        args[i] = _page_tensor(tensor, f"caches[{i}]", dim, pages, device)
+        args.append(_page_tensor(tensor, i, dim, pages, device))
         pages = tensor.shape[dim]
     if not source.numel():
         return
     _ready(source)
-    _lib.check(_lib.library().aoto_hip_paged_copy(args, len(caches), pages, _ptr(source), _ptr(target), source.numel(),
-                                                  _ptr(count), _ptr(error), _stream(device)))
+    _lib.check(
+        _lib.library().aoto_hip_paged_copy(
+            b"".join(args), len(args), pages, _ptr(source), _ptr(target), source.numel(), _ptr(count), _ptr(error),
+            _stream(device),
+        )
+    )
 
 
 def adjust_logits(
@@ -2038,38 +2058,38 @@ def adjust_logits(
         requests = query_start.numel() - 1
         if query_start.dim() != 1 or requests < 1:
             raise ValueError(f"query_start must be [R + 1], got {tuple(query_start.shape)}")
-    arg = _lib.AdjustmentsArg()
-    arg.query_start = _ptr(query_start)
+    def lists(tensor, name, kind, rows_, columns=None):
+        """A ``[rows_, columns]`` operand's address, row stride and columns."""
 
-    def lists(tensor, name, kind, dims=(None, None)):
         _expect_rows(tensor, name, kind, 2, device)
-        want = (dims[0] or requests, tensor.shape[1] if dims[1] is None else dims[1])
-        if tuple(tensor.shape) != want:
-            raise ValueError(f"{name} must be {want}, got {tuple(tensor.shape)}")
-        return tensor.data_ptr(), tensor.stride(0)
+        shape = tensor.shape
+        if shape[0] != rows_ or columns is not None and shape[1] != columns:
+            raise ValueError(f"{name} must be {(rows_, shape[1] if columns is None else columns)}, got {tuple(shape)}")
+        return tensor.data_ptr(), tensor.stride(0), shape[1]
 
-    if history is not None:
-        arg.history, arg.history_stride = lists(history, "history", torch.int64)
-        arg.history_len = history.shape[1]
-    elif history_lens is not None or prompt_lens is not None:
+    def each(tensor, name, kind):
+        """A ``[R]`` operand's address."""
+
+        if tensor is None:
+            return 0
+        _expect_all(device, ((tensor, name, kind, (requests,)),))
+        return tensor.data_ptr()
+
+    none = (0, 0, 0)
+    if history is None and (history_lens is not None or prompt_lens is not None):
         raise ValueError("history_lens and prompt_lens need a history")
-    if draft_tokens is not None:
-        arg.draft_tokens, arg.draft_stride = lists(draft_tokens, "draft_tokens", torch.int64)
-        arg.drafts = draft_tokens.shape[1]
     if (bias_tokens is None) != (bias_values is None):
         raise ValueError("bias_tokens and bias_values come together")
-    if bias_tokens is not None:
-        arg.bias_tokens, arg.bias_stride = lists(bias_tokens, "bias_tokens", torch.int64)
-        arg.biases = bias_tokens.shape[1]
-        arg.bias_values, arg.value_stride = lists(bias_values, "bias_values", torch.float32, (None, arg.biases))
-    if allowed is not None:
-        arg.allowed, arg.allowed_stride = lists(allowed, "allowed", torch.int32, (rows, (vocab + 31) // 32))
-    for name, tensor, kind in (("history_lens", history_lens, torch.int32), ("prompt_lens", prompt_lens, torch.int32),
-                               ("repetition", repetition, torch.float32), ("presence", presence, torch.float32),
-                               ("frequency", frequency, torch.float32)):
-        if tensor is not None:
-            _expect_all(device, ((tensor, name, kind, (requests,)),))
-            setattr(arg, name, tensor.data_ptr())
+    text = none if history is None else lists(history, "history", torch.int64, requests)
+    drafts = none if draft_tokens is None else lists(draft_tokens, "draft_tokens", torch.int64, requests)
+    biases = none if bias_tokens is None else lists(bias_tokens, "bias_tokens", torch.int64, requests)
+    values = none if bias_values is None else lists(bias_values, "bias_values", torch.float32, requests, biases[2])
+    masks = none if allowed is None else lists(allowed, "allowed", torch.int32, rows, (vocab + 31) // 32)
+    arg = _lib.ADJUSTMENTS.pack(
+        0 if query_start is None else query_start.data_ptr(), text[0], each(history_lens, "history_lens", torch.int32),
+        each(prompt_lens, "prompt_lens", torch.int32), drafts[0], each(repetition, "repetition", torch.float32),
+        each(presence, "presence", torch.float32), each(frequency, "frequency", torch.float32), biases[0], values[0],
+        masks[0], text[1], drafts[1], biases[1], values[1], masks[1], text[2], drafts[2], biases[2])
     if out is None:
         out = logits.new_empty((rows, vocab))
     else:
@@ -2082,7 +2102,7 @@ def adjust_logits(
     _ready(logits)
     _lib.check(
         _lib.library().aoto_hip_adjust_logits(
-            _ptr(logits), int(dtype is torch.float32), logits.stride(0), rows, vocab, requests, ctypes.byref(arg),
+            _ptr(logits), int(dtype is torch.float32), logits.stride(0), rows, vocab, requests, arg,
             _ptr(out), out.stride(0), _stream(device),
         )
     )

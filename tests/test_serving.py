@@ -24,7 +24,7 @@ def _refused(status, code, word):
 def _cache(**changes):
     a = dict(keys=4096, values=4096, key_scales=4097, value_scales=4099, page_stride=2048, head_stride=1024,
              slot_stride=64, scale_page_stride=7, scale_head_stride=5, scale_slot_stride=3, pages=4) | changes
-    return ctypes.byref(_lib.Mx4CacheArg(*a.values()))
+    return _lib.MX4_CACHE.pack(*(0 if x is None else x for x in a.values()))
 
 
 CACHE_REFUSALS = [
@@ -103,12 +103,13 @@ def test_fork_refuses(changes, code):
 
 def _release(**changes):
     a = dict(keep=GOOD, tables=GOOD, stride=8, counts=GOOD, shares=GOOD, free=GOOD, start=GOOD, requests=4, blocks=8,
-             count=100, pages=50, page=16, counts_out=GOOD, start_out=GOOD) | changes
+             count=100, pages=50, page=16, counts_out=GOOD, start_out=GOOD, scratch=GOOD) | changes
     return _lib.library().aoto_hip_paged_release(*a.values(), None, None)
 
 
 @pytest.mark.parametrize("changes,code", [
-    *[({name: None}, 1) for name in ("keep", "tables", "counts", "shares", "free", "start", "counts_out", "start_out")],
+    *[({name: None}, 1) for name in ("keep", "tables", "counts", "shares", "free", "start", "counts_out", "start_out",
+                                     "scratch")],
     (dict(requests=0), 1), (dict(blocks=0), 1), (dict(count=-1), 1), (dict(pages=0), 1), (dict(page=0), 1),
     (dict(stride=7), 1), (dict(blocks=2 ** 20 + 1, stride=2 ** 21), 4), (dict(page=2 ** 20 + 1), 4)])
 def test_release_refuses(changes, code):
@@ -132,8 +133,8 @@ def test_compact_refuses(changes, code):
 
 def _copy(tensor=None, **changes):
     t = dict(data=4096, planes=2, plane_stride=4096, page_stride=64, page_bytes=64) | (tensor or {})
-    a = dict(tensors=ctypes.byref(_lib.PageTensorArg(*t.values())), count=1, pages=4, source=GOOD, target=GOOD,
-             pairs=3) | changes
+    a = dict(tensors=_lib.PAGE_TENSOR.pack(*(0 if x is None else x for x in t.values())), count=1, pages=4,
+             source=GOOD, target=GOOD, pairs=3) | changes
     return _lib.library().aoto_hip_paged_copy(*a.values(), None, None, None)
 
 
@@ -147,10 +148,12 @@ def test_copy_refuses(tensor, changes, code):
 
 
 def _adjust(fields=None, **changes):
-    arg = _lib.AdjustmentsArg()
-    for name, value in (fields or {}).items():
-        setattr(arg, name, value)
-    a = dict(logits=GOOD, f32=0, row=1000, rows=9, vocab=1000, requests=3, adjust=ctypes.byref(arg), out=GOOD,
+    names = ("query_start", "history", "history_lens", "prompt_lens", "draft_tokens", "repetition", "presence",
+             "frequency", "bias_tokens", "bias_values", "allowed", "history_stride", "draft_stride", "bias_stride",
+             "value_stride", "allowed_stride", "history_len", "drafts", "biases")
+    assert set(fields or {}) <= set(names)
+    arg = _lib.ADJUSTMENTS.pack(*((fields or {}).get(name, 0) for name in names))
+    a = dict(logits=GOOD, f32=0, row=1000, rows=9, vocab=1000, requests=3, adjust=arg, out=GOOD,
              out_row=1000) | changes
     return _lib.library().aoto_hip_adjust_logits(*a.values(), None)
 
@@ -246,3 +249,8 @@ def test_adjustments_of_the_restatement():
     np.testing.assert_array_equal(out[0], [1.0, -5.0, 1.0, 1.5, -np.inf, 3.0])
     np.testing.assert_array_equal(out[1], [1.0, -5.0, -0.25, 1.5, 0.0, 3.0])
     assert written.all()
+
+
+def test_structs_are_the_headers():
+    # pointers, 64-bit strides, 32-bit counts and the room behind them, as the C ABI lays them out
+    assert [x.size for x in (_lib.MX4_CACHE, _lib.PAGE_TENSOR, _lib.ADJUSTMENTS)] == [88, 40, 144]
