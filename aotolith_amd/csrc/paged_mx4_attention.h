@@ -16,6 +16,11 @@ namespace aoto {
 
 typedef int mx4_i32x8 __attribute__((ext_vector_type(8)));
 
+// Where a page's row begins. The host sees to page strides below 2^32 and pages that span less than 2^30 bytes.
+AOTO_DEVICE long long mx4_at(unsigned page, long long page_stride, int row, long long slot_stride) {
+  return (long long)((unsigned long long)page * (unsigned)page_stride + (unsigned)(row * (int)slot_stride));
+}
+
 // ---------------------------------------------------------------------------------------------------- narrow tiles
 // As paged_narrow, whose layouts and softmax these are. A lane has D / 4 neighbouring dims of the keys it loads, 16 (8)
 // bytes and one scale byte: the k slots of the first product hold the dims in that order, in K and in Q.
@@ -98,9 +103,9 @@ AOTO_DEVICE void paged_mx4_narrow(const PagedMx4AttentionArgs& args, const Paged
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       to.paged[g] = (unsigned)of.page[g] < (unsigned)a.pages;
-      const long long page = to.paged[g] ? of.page[g] : 0, row = to.paged[g] ? of.row[g] : 0;
-      at[g] = page * cache.page_stride + row * cache.slot_stride;
-      scale_at[g] = page * cache.scale_page_stride + row * cache.scale_slot_stride;
+      const unsigned page = to.paged[g] ? of.page[g] : 0;
+      at[g] = mx4_at(page, cache.page_stride, of.row[g], cache.slot_stride);
+      scale_at[g] = mx4_at(page, cache.scale_page_stride, of.row[g], cache.scale_slot_stride);
     }
 #pragma unroll
     for (int g = 0; g < 2; ++g) words(keys + at[g], to.k[g]), to.ks[g] = key_scales[scale_at[g]];
@@ -277,9 +282,9 @@ AOTO_DEVICE void paged_mx4_narrow(const PagedMx4AttentionArgs& args, const Paged
 template <int D>
 struct PagedMx4WideShared {
   uint16_t v[2][64 * D];       // pieces of 16 bytes of a row in the order of paged_wide
-  uint8_t k[2][64 * D / 2];    // codes
-  uint8_t ks[2][64 * D / 32];  // scale bytes
-  uint32_t exist[2][4];        // by staging wave: which of its 16 rows exist (a page, and not past the end)
+  uint8_t k[3][64 * D / 2];    // codes
+  uint8_t ks[3][64 * D / 32];  // scale bytes
+  uint32_t exist[4][4];        // by tile and staging wave: which of its 16 rows exist (a page, and not past the end)
   unsigned long long special[2][4];  // groups, not seen by every row, that stand for NaN, by lane of the staging wave
 };
 
@@ -303,13 +308,18 @@ AOTO_DEVICE void mx4_split(const uint32_t (&w)[8], uint32_t byte, int* high, int
   }
 }
 
-// The scores of 32 keys over 64 dims, the small terms first. BYTE: of the keys' scales.
-template <int BYTE>
-AOTO_DEVICE fa_f32x16 mx4_scores(const mx4_i32x8& k, uint32_t ks, const mx4_i32x8& high, const mx4_i32x8& low, int qs,
-                                 fa_f32x16 sum) {
+// 32 keys' scores over 64 dims of one of q's parts. KEY, Q: which byte of a lane's scales is the product's.
+template <int KEY, int Q>
+AOTO_DEVICE fa_f32x16 mx4_product(const uint4& k, uint32_t ks, const mx4_i32x8& q, int qs, const fa_f32x16& sum) {
   constexpr int FP4 = 4, FP8 = 0;
-  sum = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, low, sum, FP4, FP8, BYTE, (int)ks, 1, qs);
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, high, sum, FP4, FP8, BYTE, (int)ks, 0, qs);
+  const mx4_i32x8 codes = {(int)k.x, (int)k.y, (int)k.z, (int)k.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes, q, sum, FP4, FP8, KEY, (int)ks, Q, qs);
+}
+
+// The larger of two pairs of positive bf16: their bits are in the order of their values.
+AOTO_DEVICE uint32_t mx4_larger(uint32_t a, uint32_t b) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
 
 template <int D>
@@ -376,55 +386,66 @@ AOTO_DEVICE void paged_mx4_wide(const PagedMx4AttentionArgs& args, const PagedUn
   const uint8_t* key_scales = cache.key_scales + kvh * cache.scale_head_stride + scale_of;
   const uint8_t* value_scales = cache.value_scales + kvh * cache.scale_head_stride + scale_of;
   constexpr int W = D / 32;  // words of codes
-  struct Staged {
-    uint32_t k[W], v[W];
-    uint32_t ks, vs;
+  struct Row {               // of a tile: where it is
+    long long at, scale_at;
     bool paged;
-  } staged;
+  };
+  struct Codes {
+    uint32_t w[W];
+    uint32_t scale;
+  };
   int ahead_page, ahead_row;
   auto look = [&](int t) {
     const int key = min(k0 + 64 * t + srow, k1 - 1), block = paged_block(a, key);
     ahead_page = table[block];
     ahead_row = key - block * a.page;
   };
-  auto fetch = [&] {
-    staged.paged = (unsigned)ahead_page < (unsigned)a.pages;
-    const long long page = staged.paged ? ahead_page : 0, r = staged.paged ? ahead_row : 0;
-    const long long at = page * cache.page_stride + r * cache.slot_stride;
-    const long long scale_at = page * cache.scale_page_stride + r * cache.scale_slot_stride;
-    if constexpr (D == 128) {
-      const uint4 k = *reinterpret_cast<const uint4*>(keys + at), v = *reinterpret_cast<const uint4*>(values + at);
-      staged.k[0] = k.x, staged.k[1] = k.y, staged.k[2] = k.z, staged.k[3] = k.w;
-      staged.v[0] = v.x, staged.v[1] = v.y, staged.v[2] = v.z, staged.v[3] = v.w;
-    } else {
-      const uint2 k = *reinterpret_cast<const uint2*>(keys + at), v = *reinterpret_cast<const uint2*>(values + at);
-      staged.k[0] = k.x, staged.k[1] = k.y, staged.v[0] = v.x, staged.v[1] = v.y;
-    }
-    staged.ks = key_scales[scale_at], staged.vs = value_scales[scale_at];
+  auto place = [&](Row& to) {
+    to.paged = (unsigned)ahead_page < (unsigned)a.pages;
+    const unsigned page = to.paged ? ahead_page : 0;
+    to.at = mx4_at(page, cache.page_stride, ahead_row, cache.slot_stride);
+    to.scale_at = mx4_at(page, cache.scale_page_stride, ahead_row, cache.scale_slot_stride);
   };
-  auto store = [&](int t) {
-    const int b = t & 1;
-    const bool there = staged.paged && k0 + 64 * t + srow < k1;
-    const uint32_t exist = (uint32_t)(__ballot(there) & 0xFFFFu);
-    unsigned long long special = 0;
-    if (least < k1 && k0 + 64 * t + 64 > least) special = __ballot(there && staged.vs > 252);
-    const bool none = !there || (special && staged.vs > 252);
-    const float scale = mx4_scale(none ? 0 : staged.vs);
-    if constexpr (D == 128)
-      *reinterpret_cast<uint4*>(s.k[b] + srow * 64 + ((part ^ (srow >> 2 & 3)) << 4)) =
-          make_uint4(staged.k[0], staged.k[1], staged.k[2], staged.k[3]);
-    else
-      *reinterpret_cast<uint2*>(s.k[b] + srow * 32 + 8 * part) = make_uint2(staged.k[0], staged.k[1]);
-    if (D == 128 || (part & 1) == 0) s.ks[b][srow * (D / 32) + scale_of] = (uint8_t)(staged.ks > 252 ? 255 : staged.ks);
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      char* to = reinterpret_cast<char*>(s.v[b]) + srow * ROWB + (((W * part + i) ^ swizzle(srow)) << 4);
-      *reinterpret_cast<uint4*>(to) = mx4_unpack(none ? 0u : staged.v[i], scale);
+  auto fetch = [&](const uint8_t* codes, const uint8_t* scales, const Row& of, Codes& to) {
+    if constexpr (D == 128) {
+      const uint4 w = *reinterpret_cast<const uint4*>(codes + of.at);
+      to.w[0] = w.x, to.w[1] = w.y, to.w[2] = w.z, to.w[3] = w.w;
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2*>(codes + of.at);
+      to.w[0] = w.x, to.w[1] = w.y;
     }
-    if (lane == 0) s.exist[b][wave] = exist, s.special[b][wave] = special;
+    to.scale = scales[of.scale_at];
+  };
+  auto store_k = [&](int t, int slot, const Row& of, const Codes& k) {
+    const uint32_t exist = (uint32_t)(__ballot(of.paged && k0 + 64 * t + srow < k1) & 0xFFFFu);
+    if constexpr (D == 128)
+      *reinterpret_cast<uint4*>(s.k[slot] + srow * 64 + ((part ^ (srow >> 2 & 3)) << 4)) =
+          make_uint4(k.w[0], k.w[1], k.w[2], k.w[3]);
+    else
+      *reinterpret_cast<uint2*>(s.k[slot] + srow * 32 + 8 * part) = make_uint2(k.w[0], k.w[1]);
+    if (D == 128 || (part & 1) == 0)
+      s.ks[slot][srow * (D / 32) + scale_of] = (uint8_t)(k.scale > 252 ? 255 : k.scale);
+    if (lane == 0) s.exist[t & 3][wave] = exist;
+  };
+  // V in four (two) pieces; what stands in for its codes and scale where the row is not there, or stands for NaN and is
+  // not seen by every row.
+  bool v_none;
+  float v_scale;
+  auto store_v = [&](int t, const Row& of, const Codes& v, int i) __attribute__((always_inline)) {
+    const int b = t & 1;
+    if (i == 0) {
+      const bool there = of.paged && k0 + 64 * t + srow < k1, partial = least < k1 && k0 + 64 * t + 64 > least;
+      const unsigned long long special = __ballot(partial && there && v.scale > 252);
+      v_none = !there || (partial && v.scale > 252);
+      v_scale = mx4_scale(v_none ? 0 : v.scale);
+      if (lane == 0) s.special[b][wave] = special;
+    }
+    char* to = reinterpret_cast<char*>(s.v[b]) + srow * ROWB + (((W * part + i) ^ swizzle(srow)) << 4);
+    *reinterpret_cast<uint4*>(to) = mx4_unpack(v_none ? 0u : v.w[i], v_scale);
   };
 
-  float run_max = -INFINITY, run_sum = 0.f, ref = 0.f;
+  float run_max = -INFINITY, run_sum = 0.f, ref = -INFINITY;
+  fa_f32x16 sc;  // scores of the present 32 keys
   fa_f32x16 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = fa_f32x16{};
@@ -439,105 +460,183 @@ AOTO_DEVICE void paged_mx4_wide(const PagedMx4AttentionArgs& args, const PagedUn
     const pa_s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(fa_bf16x8, both);
   };
-
-  if (tiles > 0) {
-    look(0);
-    fetch();
-    look(1);
-    store(0);
-    fetch();
-    look(2);
-  }
-  __syncthreads();
-  for (int t = 0; t < tiles; ++t) {
-    const int b = t & 1;
-    if (active) {
-      // the scores of 64 keys
-      fa_f32x16 sc[2];
+  // Operands of the scores of keys 32 sub .. of the tile in slot `slot`, and the i-th of their 2 KS products.
+  struct Keys {
+    uint4 codes[KS];
+    uint32_t scales;
+  };
+  auto read_keys = [&](int slot, int sub, Keys& to) __attribute__((always_inline)) {
+    const int key = 32 * sub + col;
+    if constexpr (D == 128) to.scales = *reinterpret_cast<const uint32_t*>(s.ks[slot] + 4 * key) >> (8 * half);
+    else to.scales = s.ks[slot][2 * key + half];
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        const int key = 32 * sub + col;
-        sc[sub] = fa_f32x16{};
-        uint32_t ks;
-        if constexpr (D == 128) ks = *reinterpret_cast<const uint32_t*>(s.ks[b] + 4 * key) >> (8 * half);
-        else ks = s.ks[b][2 * key + half];
+    for (int st = 0; st < KS; ++st)
+      to.codes[st] = D == 128 ? *reinterpret_cast<const uint4*>(s.k[slot] + key * 64 +
+                                                                (((2 * st + half) ^ (key >> 2 & 3)) << 4))
+                              : *reinterpret_cast<const uint4*>(s.k[slot] + key * 32 + 16 * half);
+  };
+  auto product = [&](int i, const Keys& k, const fa_f32x16& sum) __attribute__((always_inline)) {
+    return i == 0   ? mx4_product<0, 1>(k.codes[0], k.scales, ql[0], q_scale[0], sum)
+           : i == 1 ? mx4_product<0, 0>(k.codes[0], k.scales, qh[0], q_scale[0], sum)
+           : i == 2 ? mx4_product<2, 1>(k.codes[KS - 1], k.scales, ql[KS - 1], q_scale[KS - 1], sum)
+                    : mx4_product<2, 0>(k.codes[KS - 1], k.scales, qh[KS - 1], q_scale[KS - 1], sum);
+  };
+  // Whether every row sees every key of tile t: uniform, and told so.
+  auto whole = [&](int t) {
+    const uint32_t exist = s.exist[t & 3][0] & s.exist[t & 3][1] & s.exist[t & 3][2] & s.exist[t & 3][3];
+    return __builtin_amdgcn_readfirstlane(exist == 0xFFFFu && k0 + 64 * t + 64 <= least) != 0;
+  };
+  // The scores of keys 32 sub .. of tile t that a row may not see, or that are of no page, leave.
+  auto mask = [&](int t, int sub) {
+    if (whole(t)) return;
+    const int sees = limit - (k0 + 64 * t + 32 * sub + 4 * half);
+    const uint32_t exist = (s.exist[t & 3][2 * sub] | s.exist[t & 3][2 * sub + 1] << 16) >> (4 * half);
 #pragma unroll
-        for (int st = 0; st < KS; ++st) {
-          uint4 w;
-          if constexpr (D == 128)
-            w = *reinterpret_cast<const uint4*>(s.k[b] + key * 64 + (((2 * st + half) ^ (key >> 2 & 3)) << 4));
-          else
-            w = *reinterpret_cast<const uint4*>(s.k[b] + key * 32 + 16 * half);
-          const mx4_i32x8 k = {(int)w.x, (int)w.y, (int)w.z, (int)w.w, 0, 0, 0, 0};
-          sc[sub] = st == 0 ? mx4_scores<0>(k, ks, qh[st], ql[st], q_scale[st], sc[sub])
-                            : mx4_scores<2>(k, ks, qh[st], ql[st], q_scale[st], sc[sub]);
-        }
-      }
-      const bool whole = (s.exist[b][0] & s.exist[b][1] & s.exist[b][2] & s.exist[b][3]) == 0xFFFFu &&
-                         k0 + 64 * t + 64 <= least;
-      if (!whole) {
+    for (int e = 0; e < 16; ++e) {
+      const int k = 8 * (e >> 2) + (e & 3);
+      sc[e] = (exist >> k & 1) && k < sees ? sc[e] : -INFINITY;
+    }
+  };
+  // Two of the weights of the present scores. A row without a reference (-inf) gets infinities or NaN, which lead to one.
+  auto pair = [&](int u) __attribute__((always_inline)) {
+    return cvt_pk_bf16(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * u], c2, -ref)),
+                       __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * u + 1], c2, -ref)));
+  };
+  // Scores sc of keys 32 sub .. of tile t: their weights go among the products of the scores behind them (operands in
+  // `keys`), then their product with V; the keys of the step after it are read at the end. `beside(i)`: what else goes
+  // among the products with V, i of 2 DT.
+  Keys keys_next;
+  auto step = [&](int t, int sub, int later_slot, int later_sub, auto beside) __attribute__((always_inline)) {
+    const uint32_t v_base = lds_v + (t & 1) * TILEB;
+    uint32_t w[8];
+    fa_bf16x8 vf[3];
+    fa_f32x16 next = fa_f32x16{};
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
+    for (int i = 0; i < 2 * KS; ++i) {
+      next = product(i, keys_next, next);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int k = 32 * sub + 8 * (e >> 2) + 4 * half + (e & 3);
-            if (!(s.exist[b][k >> 4] >> (k & 15) & 1) || k0 + 64 * t + k >= limit) sc[sub][e] = -INFINITY;
-          }
-      }
+      for (int u = 0; u < 4 / KS; ++u) w[4 / KS * i + u] = pair(4 / KS * i + u);
+      if (i == 2 * KS - 1) vf[0] = read_v(v_base, 2 * sub, 0), vf[1] = read_v(v_base, 2 * sub, 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) asm volatile("" : "+v"(w[u]));
+    uint32_t most = w[0];
+#pragma unroll
+    for (int u = 1; u < 8; ++u) most = mx4_larger(most, w[u]);
+    // The reference moves only where a weight is above 1, and then 2^8 ahead of the largest score; O and the sum follow.
+    if (__any((most & 0xFFFFu) > 0x3F80u || most > 0x3F80FFFFu)) {
+      // a use on this way too: else the products move behind the branch, where the exponentials are not beside them
+      asm volatile("" : "+v"(next));
       float top = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, fmaxf(sc[0][e], sc[1][e]));
-      // the exponentials' reference moves only where a score passes it, and then 2^8 ahead
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[e]);
       top = xor32_max(top) * c2;
       const float moved = top > run_max ? top + 8.f : run_max;
       const float keep = moved == run_max || run_max == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(run_max - moved);
       run_max = moved;
       ref = moved == -INFINITY ? 0.f : moved;
-      if (__any(keep != 1.f)) {
-        run_sum *= keep;
+      run_sum *= keep;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] *= keep;
-      }
+      for (int d = 0; d < DT; ++d) o[d] *= keep;
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        uint32_t w[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int e = 8 * (kt & 1) + 2 * u;
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt >> 1][e], c2, -ref));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt >> 1][e + 1], c2, -ref));
-          w[u] = cvt_pk_bf16(p0, p1);
-          run_sum = dot2_bf16(w[u], 0x3F803F80u, run_sum);  // the rounded weights' sum
-        }
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_v(lds_v + b * TILEB, kt, d),
-                                                         __builtin_bit_cast(fa_bf16x8, w), o[d], 0, 0, 0);
-      }
-      if (!whole) {
-        for (int w = 0; w < 4; ++w) {
-          unsigned long long special = s.special[b][w];
-          while (special) {
-            const int from = __ffsll(special) - 1;
-            special &= special - 1;
-            const int k = k0 + 64 * t + 16 * w + (from & 15), of = (from >> 4) * (D / 4) / 32;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-              if (d == of && k < limit) o[d] += NAN;
-          }
-        }
-      }
+      for (int u = 0; u < 8; ++u) w[u] = pair(u);
+      ref = run_max;  // none yet: the next scores look for one
     }
-    if (t + 1 < tiles) {
-      store(t + 1);
-      if (t + 2 < tiles) {
-        fetch();
-        look(t + 3);
+#pragma unroll
+    for (int m = 0; m < 2 * DT; ++m) {
+      const int kt = m / DT, d = m % DT;
+      if (m + 2 < 2 * DT) vf[(m + 2) % 3] = read_v(v_base, 2 * sub + (m + 2) / DT, (m + 2) % DT);
+      else if (m + 2 == 2 * DT) read_keys(later_slot, later_sub, keys_next);
+      const uint32_t x[4] = {w[4 * kt], w[4 * kt + 1], w[4 * kt + 2], w[4 * kt + 3]};
+      o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[m % 3], __builtin_bit_cast(fa_bf16x8, x), o[d], 0, 0, 0);
+#pragma unroll
+      for (int u = 4 / DT * m; u < 4 / DT * (m + 1); ++u)
+        run_sum = dot2_bf16(w[u], 0x3F803F80u, run_sum);  // the rounded weights' sum
+      beside(m);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    sc = next;
+  };
+
+  // At tile t: K of tiles t and t + 1 and V of tile t are in LDS, K of tile t + 2 and V of tile t + 1 in registers or on
+  // their way; they go to LDS while the tile is worked on, and those behind them are asked for.
+  Row row_k, row_v;
+  Codes code_k, code_v;
+  if (tiles > 0) {
+    Row first;
+    look(0);
+    place(first);
+    look(1);
+    fetch(keys, key_scales, first, code_k);
+    fetch(values, value_scales, first, code_v);
+    place(row_v);
+    look(2);
+    store_k(0, 0, first, code_k);
+#pragma unroll
+    for (int i = 0; i < W; ++i) store_v(0, first, code_v, i);
+    fetch(keys, key_scales, row_v, code_k);
+    place(row_k);
+    look(3);
+    store_k(1, 1, row_v, code_k);
+    fetch(keys, key_scales, row_k, code_k);
+    fetch(values, value_scales, row_v, code_v);
+    __syncthreads();
+    if (active) {
+      sc = fa_f32x16{};
+      read_keys(0, 0, keys_next);
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) sc = product(i, keys_next, sc);
+      mask(0, 0);
+      read_keys(0, 1, keys_next);
+    }
+  }
+  int slot = 0;  // t mod 3
+  auto after = [](int n) { return n == 2 ? 0 : n + 1; };
+  // V's words of tile t + 1, K of tile t + 2, then what comes after them.
+  auto stage = [&](int t, int i) __attribute__((always_inline)) {
+    if (i < W) store_v(t + 1, row_v, code_v, i);
+    if (i == W) store_k(t + 2, slot == 0 ? 2 : slot - 1, row_k, code_k);
+    if (i == W + 1) {
+      row_v = row_k;
+      place(row_k);
+      fetch(keys, key_scales, row_k, code_k);
+      fetch(values, value_scales, row_v, code_v);
+      look(t + 4);
+    }
+  };
+  if (!active) {
+    for (int t = 0; t < tiles; ++t, slot = after(slot)) {
+#pragma unroll
+      for (int i = 0; i < W + 2; ++i) stage(t, i);
+      __syncthreads();
+    }
+    return;
+  }
+  for (int t = 0; t < tiles; ++t, slot = after(slot)) {
+    step(t, 0, after(slot), 0, [&](int m) __attribute__((always_inline)) {
+      if (D == 128) stage(t, m);
+      else if (m < 2) stage(t, 2 * m), stage(t, 2 * m + 1);
+    });
+    mask(t, 1);
+    step(t, 1, after(slot), 1, [](int) {});
+    mask(t + 1, 0);
+    if (!whole(t)) {
+#pragma unroll 1
+      for (int w = 0; w < 4; ++w) {
+        unsigned long long special = s.special[t & 1][w];
+        while (special) {
+          const int from = __ffsll(special) - 1;
+          special &= special - 1;
+          const int k = k0 + 64 * t + 16 * w + (from & 15), of = (from >> 4) * (D / 4) / 32;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+            if (d == of && k < limit) o[d] += NAN;
+        }
       }
     }
     __syncthreads();
   }
-  if (!active) return;
   const float sum = xor32_sum(run_sum);
   if (row >= live) return;
   const bool none = run_max == -INFINITY && sum == 0.f && k0 < limit;

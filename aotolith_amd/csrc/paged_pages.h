@@ -47,6 +47,13 @@ AOTO_DEVICE void page_ranks(uint32_t bits, int (&before)[kPageSteps], int& total
   __syncthreads();
 }
 
+// Entry j of request r is its parent's, whose page has one holder more.
+AOTO_DEVICE void share_page(const PagedForkArgs& a, int r, int j) {
+  const int page = a.block_tables[(size_t)a.parents[r] * a.table_stride + j];
+  a.block_tables[(size_t)r * a.table_stride + j] = page;
+  if ((unsigned)page < (unsigned)a.pages) atomicAdd(a.shares + page, 1);
+}
+
 // Four neighbours of a list, 0 past its end.
 struct __attribute__((packed, aligned(4))) PageFour {
   int v[4];
@@ -62,8 +69,9 @@ AOTO_DEVICE PageFour page_four(const int* values, int from, int count) {
 }  // namespace aoto
 
 // Which rows go on from which, the pages taken for them and what is to be copied (formulas at the entry point's
-// declaration). One block: everything hangs on a running sum over the requests.
-extern "C" __global__ __launch_bounds__(1024) void aoto_paged_fork(PagedForkArgs a) {
+// declaration). One block: everything hangs on a running sum over the requests. Where `fill` is set it also enters the
+// full pages, which aoto_paged_share does otherwise.
+extern "C" __global__ __launch_bounds__(1024) void aoto_paged_fork(PagedForkArgs a, int fill) {
   using namespace aoto;
   __shared__ long long s_scan[16];
   __shared__ int s_error;
@@ -116,6 +124,11 @@ extern "C" __global__ __launch_bounds__(1024) void aoto_paged_fork(PagedForkArgs
     a.context_lens_out[r] = full >= 0 ? length : a.context_lens[r];
     a.page_counts_out[r] = full >= 0 ? full + (length > full * a.page ? 1 : 0) : a.page_counts[r];
   }
+  if (fill)
+    for (int k = tid; k < a.requests * a.max_blocks; k += 1024) {
+      const int r = k / a.max_blocks, j = k - r * a.max_blocks;
+      if (j < a.plan[2 * r]) share_page(a, r, j);
+    }
   if (tid == 0) {
     const long long available = max(0LL, a.free_count - first_free);
     a.free_start_out[0] = taken ? (int)(first_free + min(taken, available)) : start;
@@ -126,14 +139,7 @@ extern "C" __global__ __launch_bounds__(1024) void aoto_paged_fork(PagedForkArgs
 // The full pages of the rows that go on: entered in their own rows, one holder more each.
 extern "C" __global__ __launch_bounds__(256) void aoto_paged_share(PagedForkArgs a) {
   const int r = blockIdx.x, full = a.plan[2 * r];
-  if (full <= 0) return;
-  const int* from = a.block_tables + (size_t)a.parents[r] * a.table_stride;
-  int* to = a.block_tables + (size_t)r * a.table_stride;
-  for (int j = threadIdx.x; j < full; j += 256) {
-    const int page = from[j];
-    to[j] = page;
-    if ((unsigned)page < (unsigned)a.pages) atomicAdd(a.shares + page, 1);
-  }
+  for (int j = threadIdx.x; j < full; j += 256) aoto::share_page(a, r, j);
 }
 
 // Requests' pages past what they keep lose a holder each; a page without one stands at -1 until aoto_paged_reclaim.

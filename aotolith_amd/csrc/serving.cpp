@@ -37,6 +37,10 @@ int check_cache(const char* what, const aoto_mx4_cache* c, int page, int kv_head
   return AOTO_OK;
 }
 
+// Entries of all block tables up to which the fork's one block enters the pages itself: a second launch costs more than
+// it saves.
+constexpr long long kForkFill = 16384;
+
 }  // namespace
 
 extern "C" {
@@ -98,6 +102,9 @@ int aoto_hip_paged_attention_mx4(const void* q, int64_t q_token_stride, int64_t 
     return set_error(AOTO_ERR_ARGUMENT, "paged_attention_mx4: q and out 16-byte aligned, strides of multiples of 8");
   if ((long long)max_blocks * page > (1 << 28))
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention_mx4: block tables of more than 2^28 keys");
+  for (const int64_t* stride : {&cache->page_stride, &cache->scale_page_stride})
+    if (stride[0] < 0 || stride[0] > 0xFFFFFFFFLL || stride[2] < 0 || stride[2] > 0x3FFFFFFFLL / page)
+      return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention_mx4: pages 2^32 bytes apart, or rows 2^30");
   if (!(scale > 0.f) || !std::isfinite(scale))
     return set_error(AOTO_ERR_ARGUMENT, "paged_attention_mx4: scale %g is not a positive number", (double)scale);
   if (query_heads / kv_heads > kWideRows)
@@ -142,7 +149,9 @@ int aoto_hip_paged_fork(const int32_t* parents, const int32_t* context_lens, int
   a.page_counts_out = page_counts_out, a.free_start_out = free_start_out, a.source = source, a.target = target;
   a.plan = plan, a.error = error, a.table_stride = table_stride, a.requests = requests, a.max_blocks = max_blocks;
   a.free_count = free_count, a.pages = pages, a.page = page;
-  if (int s = launch("aoto_paged_fork", 1, 1, 1024, stream, a)) return s;
+  const int fill = (long long)requests * max_blocks <= kForkFill;
+  if (int s = launch("aoto_paged_fork", 1, 1, 1024, stream, a, fill)) return s;
+  if (fill) return AOTO_OK;
   return launch("aoto_paged_share", requests, 1, 256, stream, a);
 }
 
