@@ -142,6 +142,9 @@ SIGNATURES: dict[str, tuple] = {
         _p, _i64, _p, _p, _p, _p, _c_int, _p, _c_int, _c_int, _c_int, _c_int, _c_int, _p, _p, _p,
     ),
     "aoto_hip_paged_unpack_mx4": (_p, _c_int, _c_int, _c_int, _p, _p, _p),
+    "aoto_hip_paged_attention_mx4_workspace": (
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+    ),
     "aoto_hip_paged_attention_mx4": (
         _p, _i64, _i64, _p, _c_int, _p, _i64, _c_int, _p, _p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float,
         _c_int, _c_int, _p, _p, _p,
@@ -170,7 +173,8 @@ ADJUSTMENTS = struct.Struct("11P5q3i4x")
 SIZE_RETURNING = {"aoto_hip_last_error", "aoto_hip_take_launches", "aoto_hip_decode_attention_workspace",
                   "aoto_hip_w4_gemm_workspace", "aoto_hip_w4_gemm_gate_up_workspace", "aoto_hip_w4_gemm_qkv_rope_workspace",
                   "aoto_hip_w4_gemv_argmax_keys", "aoto_hip_w4_gemv_finish_max_keys",
-                  "aoto_hip_paged_attention_workspace", "aoto_hip_verify_draft_workspace"}
+                  "aoto_hip_paged_attention_workspace", "aoto_hip_verify_draft_workspace",
+                  "aoto_hip_paged_attention_mx4_workspace"}
 
 
 class HipBackendUnavailable(RuntimeError):

@@ -31,9 +31,10 @@ struct AttentionPlan {
   size_t workspace;
 };
 
-// From what the host knows: shapes and the caller's bounds. The lengths are on the GPU.
+// From what the host knows: shapes and the caller's bounds. The lengths are on the GPU. narrow_blocks: GPU blocks of the
+// narrow tiles of 16 rows that a CU holds.
 inline AttentionPlan attention_plan(int tokens, int requests, int max_blocks, int page, int query_heads, int kv_heads,
-                                    int head_dim, int max_query_len, int max_kv_len) {
+                                    int head_dim, int max_query_len, int max_kv_len, int narrow_blocks = 2) {
   const int group = query_heads / kv_heads, cus = device_cu_count();
   const long long rows = (long long)(max_query_len ? std::min(max_query_len, tokens) : tokens) * group;
   const long long some = std::min(requests, tokens);
@@ -42,7 +43,8 @@ inline AttentionPlan attention_plan(int tokens, int requests, int max_blocks, in
   p.narrow_rows = rows <= 16 || rows > 32 ? 16 : 32;
   p.wide_rows = rows > 32 ? kWideRows : 0;
   p.units = tiles(p.wide_rows ? p.wide_rows : p.narrow_rows);
-  const long long full = 2LL * cus;  // GPU blocks that the chip holds at a time
+  // GPU blocks that the chip holds at a time
+  const long long full = (p.wide_rows || p.narrow_rows > 16 ? 2LL : narrow_blocks) * cus;
   long long keys = std::min<long long>((long long)max_blocks * page, 1 << 28);
   const long long most = keys / 128 + 8;  // key blocks of a tile
   if (max_kv_len) keys = std::min<long long>(keys, max_kv_len);

@@ -175,28 +175,33 @@ AOTO_DEVICE void paged_mx4_narrow(const PagedMx4AttentionArgs& args, const Paged
             if (!(exist >> k & 1) || base + k >= limit[t]) sc[t][g][e] = -INFINITY;
           }
       }
-      float top = -INFINITY;
+      // The exponentials' reference moves only where a weight is above 1 (or NaN, as a row's without a reference are), and
+      // then 2^8 ahead of the largest score: in most tiles no maximum stands before the exponentials.
+      float p[8];
+      uint32_t most = 0;
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
+      for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j >> 2][j & 3], c2, -run_max[t]));
+        most = max(most, __float_as_uint(p[j]));
+      }
+      if (__any(most > 0x3F800000u)) {
+        float top = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[t][g][e]);
-      top = xor32_max(xor16_max(top)) * c2;
-      // the exponentials' reference moves only where a score passes it, and then 2^8 ahead
-      const float moved = top > run_max[t] ? top + 8.f : run_max[t];
-      const float keep = moved == run_max[t] ? 1.f : __builtin_amdgcn_exp2f(run_max[t] - moved);
-      run_max[t] = moved;
-      const float ref = moved == -INFINITY ? 0.f : moved;
-      if (__any(keep != 1.f)) {
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, sc[t][j >> 2][j & 3]);
+        top = xor32_max(xor16_max(top)) * c2;
+        const float moved = top > run_max[t] ? top + 8.f : run_max[t];
+        const float keep = moved == run_max[t] || run_max[t] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(run_max[t] - moved);
+        run_max[t] = moved;
         run_sum[t] *= keep;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[t][d] *= keep;
-      }
-      float p[8];
+        const float by = moved == -INFINITY ? 0.f : moved;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j >> 2][j & 3], c2, -ref));
-        run_sum[t] += p[j];
+        for (int j = 0; j < 8; ++j)
+          p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j >> 2][j & 3], c2, -by));
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) run_sum[t] += p[j];
       // 16 bits of a weight: its upper half cut off and the rest rounded, in two products
       uint32_t high[4], low[4];
 #pragma unroll
@@ -698,7 +703,7 @@ __device__ void paged_mx4_attention_mixed(const PagedMx4AttentionArgs& a) {
 }  // namespace aoto
 
 #define AOTO_PAGED_MX4_ATTENTION(D)                                                                                  \
-  extern "C" __global__ __launch_bounds__(256, 2) void aoto_paged_attention_mx4_d##D##_n1(PagedMx4AttentionArgs a) { \
+  extern "C" __global__ __launch_bounds__(256, 3) void aoto_paged_attention_mx4_d##D##_n1(PagedMx4AttentionArgs a) { \
     aoto::paged_mx4_attention_narrow<D, 1>(a);                                                                       \
   }                                                                                                                  \
   extern "C" __global__ __launch_bounds__(256, 2) void aoto_paged_attention_mx4_d##D##_n2(PagedMx4AttentionArgs a) { \

@@ -37,6 +37,11 @@ int check_cache(const char* what, const aoto_mx4_cache* c, int page, int kv_head
   return AOTO_OK;
 }
 
+// GPU blocks of the attention's narrow tiles of 16 rows that a CU holds. A tile's rows are a quarter of what they are in
+// bf16, so that two do not ask for enough at a time (345000 keys of 64 requests, 8 kv heads of 128: 88 us with two, 84
+// with three, 93 with four, whose registers are too few).
+constexpr int kMx4NarrowBlocks = 3;
+
 // Entries of all block tables up to which the fork's one block enters the pages itself: a second launch costs more than
 // it saves.
 constexpr long long kForkFill = 16384;
@@ -83,6 +88,16 @@ int aoto_hip_paged_unpack_mx4(const aoto_mx4_cache* cache, int page, int kv_head
   return launch("aoto_paged_unpack_mx4", cache->pages, (rows * (head_dim / 16) + 255) / 256, 256, stream, a);
 }
 
+size_t aoto_hip_paged_attention_mx4_workspace(int tokens, int requests, int max_blocks, int page, int query_heads,
+                                              int kv_heads, int head_dim, int max_query_len, int max_kv_len) {
+  if (tokens <= 0 || requests <= 0 || max_blocks <= 0 || page <= 0 || query_heads <= 0 || kv_heads <= 0 ||
+      query_heads % kv_heads || head_dim <= 0 || max_query_len < 0 || max_kv_len < 0)
+    return 0;
+  return attention_plan(tokens, requests, max_blocks, page, query_heads, kv_heads, head_dim, max_query_len, max_kv_len,
+                        kMx4NarrowBlocks)
+      .workspace;
+}
+
 int aoto_hip_paged_attention_mx4(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                                  const aoto_mx4_cache* cache, int page, const int32_t* block_tables,
                                  int64_t table_stride, int max_blocks, const int32_t* query_start,
@@ -111,7 +126,7 @@ int aoto_hip_paged_attention_mx4(const void* q, int64_t q_token_stride, int64_t 
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_attention_mx4: %d query heads a kv head (at most %d)",
                      query_heads / kv_heads, kWideRows);
   const AttentionPlan plan = attention_plan(tokens, requests, max_blocks, page, query_heads, kv_heads, head_dim,
-                                            max_query_len, max_kv_len);
+                                            max_query_len, max_kv_len, kMx4NarrowBlocks);
   if (plan.workspace && (!workspace || !aligned(workspace, 16)))
     return set_error(AOTO_ERR_ARGUMENT, "paged_attention_mx4: needs a 16-byte aligned workspace of %zu bytes",
                      plan.workspace);

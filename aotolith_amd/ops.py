@@ -1690,6 +1690,18 @@ def paged_unpack_mx4(cache: PagedMx4, *, out: tuple[torch.Tensor, torch.Tensor] 
     return out
 
 
+def paged_attention_mx4_workspace(tokens: int, requests: int, max_blocks: int, page_size: int, query_heads: int,
+                                  kv_heads: int, head_dim: int, *, max_query_len: int = 0, max_kv_len: int = 0,
+                                  device=None) -> torch.Tensor:
+    """A workspace for :func:`paged_attention_mx4` with these shapes and bounds, as
+    :func:`paged_attention_workspace`'s."""
+
+    size = _lib.library().aoto_hip_paged_attention_mx4_workspace(
+        int(tokens), int(requests), int(max_blocks), int(page_size), int(query_heads), int(kv_heads), int(head_dim),
+        int(max_query_len), int(max_kv_len))
+    return torch.empty((max(size, 16),), dtype=torch.uint8, device=device)
+
+
 def paged_attention_mx4(
     q: torch.Tensor,
     cache: PagedMx4,
@@ -1707,10 +1719,11 @@ def paged_attention_mx4(
     """:func:`paged_attention` over a 4-bit cache: the requests' new tokens ``q [T, Hq, D]`` (D 64 or 128) over the
     values that the codes of their pages stand for -> ``[T, Hq * D]``.
 
-    Everything else is :func:`paged_attention`'s, the workspace (:func:`paged_attention_workspace`) and what a row sees
-    among it. A NaN group of a key that a row sees, a NaN or an infinity in its q make the row NaN; a NaN group of a
-    value makes those 32 dims NaN, however small its weight. Requests of more than 32 rows a kv head multiply K as it is
-    in the cache by q as two 8-bit numbers (exactly q to 2^-22 of the largest of each 32 dims).
+    Everything else is :func:`paged_attention`'s, what a row sees among it (the workspace:
+    :func:`paged_attention_mx4_workspace`). A NaN group of a key that a row sees, a NaN or an infinity in its q make
+    the row NaN; a NaN group of a value makes those 32 dims NaN, however small its weight. Requests of more than 32 rows
+    a kv head multiply K as it is in the cache by q as two 8-bit numbers (exactly q to 2^-22 of the largest of each 32
+    dims), in sums that keep 13 bits below the largest of each eight products.
     """
 
     _expect_rows(q, "q", BF16, 3, q.get_device() if isinstance(q, torch.Tensor) else 0)
@@ -1732,8 +1745,8 @@ def paged_attention_mx4(
     _ready(q)
     lib = _lib.library()
     max_query_len, max_kv_len = int(max_query_len), int(max_kv_len)
-    need = lib.aoto_hip_paged_attention_workspace(tokens, requests, max_blocks, page, query_heads, kv_heads, dim,
-                                                  max_query_len, max_kv_len)
+    need = lib.aoto_hip_paged_attention_mx4_workspace(tokens, requests, max_blocks, page, query_heads, kv_heads, dim,
+                                                      max_query_len, max_kv_len)
     if workspace is not None:
         _on_device(workspace)
         if workspace.get_device() != device:

@@ -710,9 +710,12 @@ int aoto_hip_paged_rope_append_mx4(const void* qkv, int64_t row_stride, const in
 int aoto_hip_paged_unpack_mx4(const aoto_mx4_cache* cache, int page, int kv_heads, int head_dim, void* keys_out,
                               void* values_out, void* stream);
 
-/* aoto_hip_paged_attention over a 4-bit cache, with the same rules, limits of shapes and workspace
- * (aoto_hip_paged_attention_workspace()). A NaN that a row sees, in a key's group or in q, makes the row NaN, in a
- * value's group those 32 dims, however small the weight. */
+/* aoto_hip_paged_attention over a 4-bit cache, with the same rules and limits of shapes; page strides below 2^32, a
+ * page's rows within 2^30 bytes, codes and scales alike. A NaN that a row sees, in a key's group or in q, makes the row
+ * NaN, in a value's group those 32 dims, however small the weight. workspace:
+ * aoto_hip_paged_attention_mx4_workspace() bytes for the same arguments (0: none needed). */
+size_t aoto_hip_paged_attention_mx4_workspace(int tokens, int requests, int max_blocks, int page, int query_heads,
+                                              int kv_heads, int head_dim, int max_query_len, int max_kv_len);
 int aoto_hip_paged_attention_mx4(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                                  const aoto_mx4_cache* cache, int page, const int32_t* block_tables,
                                  int64_t table_stride, int max_blocks, const int32_t* query_start,

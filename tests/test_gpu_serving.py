@@ -472,7 +472,7 @@ def test_attention_replays_in_graphs_that_share_a_workspace():
     ops = _ops()
     graphs = []
     shapes = [[(1, 900), (1, 40), (1, 2000)], [(20, 900), (1, 40), (4, 1500)]]
-    sizes = [ops.paged_attention_workspace(sum(n for n, _ in x), 3, 125, 16, 8, 2, 64, device="cuda").numel()
+    sizes = [ops.paged_attention_mx4_workspace(sum(n for n, _ in x), 3, 125, 16, 8, 2, 64, device="cuda").numel()
              for x in shapes]
     workspace = torch.empty(max(sizes), dtype=torch.uint8, device="cuda")
     for lengths in shapes:

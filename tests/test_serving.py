@@ -85,6 +85,21 @@ def test_attention_refuses(changes, code):
     _refused(_attention(**changes), code, "paged_attention_mx4")
 
 
+@pytest.mark.parametrize("changes", [
+    dict(page_stride=2 ** 32), dict(page_stride=-2048), dict(slot_stride=2 ** 26), dict(slot_stride=-64),
+    dict(slot_stride=2 ** 60), dict(slot_stride=2 ** 62), dict(scale_page_stride=2 ** 32), dict(scale_page_stride=-1),
+    dict(scale_slot_stride=2 ** 26 + 1), dict(scale_slot_stride=-1), dict(scale_slot_stride=2 ** 62)])
+def test_attention_refuses_what_its_addresses_do_not_reach(changes):
+    _refused(_attention(changes), 4, "paged_attention_mx4")
+
+
+def test_workspaces_of_empty_calls_are_empty():
+    lib = _lib.library()
+    assert lib.aoto_hip_paged_attention_mx4_workspace(0, 1, 8, 16, 14, 2, 64, 0, 0) == 0
+    assert lib.aoto_hip_paged_attention_mx4_workspace(1, 1, 8, 16, 15, 2, 64, 0, 0) == 0
+    assert lib.aoto_hip_paged_attention_mx4_workspace(1, 1, 800, 16, 14, 2, 64, 1, 0) > 0
+
+
 def _fork(**changes):
     a = dict(parents=GOOD, lens=GOOD, tables=GOOD, stride=8, counts=GOOD, shares=GOOD, free=GOOD, start=GOOD,
              requests=4, blocks=8, count=100, pages=50, page=16, lens_out=GOOD, counts_out=GOOD, start_out=GOOD,
