@@ -4,16 +4,21 @@ Outputs (next to the package, so they travel with the source tree):
 
 * ``aotolith_amd/aoto_gfx950.hsaco`` - every kernel, ``hipcc --genco`` for gfx950;
 * ``aotolith_amd/libaoto_hip.so``     - the ``extern "C"`` launchers of
-  ``include/aoto_hip.h``.
+  ``include/aoto_hip.h``;
+* ``aotolith_amd/_calls.so``          - the serving operators' calls from Python
+  (``calls.cpp``: host code against torch's headers; ``ops.py`` makes the same
+  calls without it, at 5 to 8 us more each).
 
 Run ``python -m aotolith_amd.csrc.build`` or call :func:`build`.
 """
 
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import subprocess
 import sys
+import sysconfig
 
 CSRC = os.path.dirname(os.path.abspath(__file__))
 PACKAGE = os.path.dirname(CSRC)
@@ -24,6 +29,7 @@ ROCM = os.path.dirname(os.path.dirname(HIPCC))
 
 CODE_OBJECT = os.path.join(PACKAGE, "aoto_gfx950.hsaco")
 LIBRARY = os.path.join(PACKAGE, "libaoto_hip.so")
+CALLS = os.path.join(PACKAGE, "_calls.so")
 
 # Device flags: gfx950 only; packed-FP32 VALU forms disabled (they are not used
 # by hand and the compiler is told not to form them); kernel arguments preloaded
@@ -54,16 +60,25 @@ def _run(command: list[str], verbose: bool) -> None:
         raise RuntimeError(f"build step failed ({result.returncode}): {' '.join(command)}")
 
 
-def build(verbose: bool = False) -> tuple[str, str]:
-    """Compile the code object and the host library; return their paths."""
+def _calls_command(output: str) -> list[str]:
+    import torch
+    from torch.utils import cpp_extension
 
-    tmp_obj = CODE_OBJECT + ".tmp"
-    _run([HIPCC, *DEVICE_FLAGS, "--genco", "--no-gpu-bundle-output", os.path.join(CSRC, "kernels.hip"), "-o", tmp_obj], verbose)
-    os.replace(tmp_obj, CODE_OBJECT)
-    tmp_lib = LIBRARY + ".tmp"
-    # The host library: the C-ABI launchers (paged.cpp and serving.cpp: those of serving), plus noalloc.hip, whose device
-    # part is only the static scratch buffer of the allocation-free GEMM entry point.
-    _run(
+    libraries = os.path.join(os.path.dirname(torch.__file__), "lib")
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-I" + INCLUDE,
+            "-I" + sysconfig.get_paths()["include"], *("-I" + path for path in cpp_extension.include_paths()),
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", os.path.join(CSRC, "calls.cpp"), "-o",
+            output, "-L" + libraries, "-ltorch_python", "-ltorch_cpu", "-lc10"]
+
+
+def build(verbose: bool = False) -> tuple[str, str]:
+    """Compile the code object, the host library and the Python calls; return the first two's paths."""
+
+    tmp_obj, tmp_lib, tmp_calls = CODE_OBJECT + ".tmp", LIBRARY + ".tmp", CALLS + ".tmp"
+    commands = (
+        [HIPCC, *DEVICE_FLAGS, "--genco", "--no-gpu-bundle-output", os.path.join(CSRC, "kernels.hip"), "-o", tmp_obj],
+        # The host library: the C-ABI launchers (paged.cpp and serving.cpp: those of serving), plus noalloc.hip, whose
+        # device part is only the static scratch buffer of the allocation-free GEMM entry point.
         [
             HIPCC,
             "-O2",
@@ -84,9 +99,14 @@ def build(verbose: bool = False) -> tuple[str, str]:
             "-o",
             tmp_lib,
         ],
-        verbose,
+        _calls_command(tmp_calls),
     )
+    with concurrent.futures.ThreadPoolExecutor() as pool:
+        for step in [pool.submit(_run, command, verbose) for command in commands]:
+            step.result()
+    os.replace(tmp_obj, CODE_OBJECT)
     os.replace(tmp_lib, LIBRARY)
+    os.replace(tmp_calls, CALLS)
     return CODE_OBJECT, LIBRARY
 
 

@@ -1554,6 +1554,44 @@ def verify_draft(
 
 
 # ------------------------------------------------------------------------------------------------------------------
+# The functions from here on make their call through ``_calls`` (csrc/calls.cpp) where that is built: the checks, the
+# outputs' allocation and the C ABI's call in one step, 3 us instead of the 8 to 11 that the same takes below. It gives
+# None where an argument is not as it should be or the call was refused; the checks below then say why, or make a call
+# that it does not (outputs given as a tuple, numbers of other types).
+
+
+class _Unbound:
+    """``_calls`` before it is bound, and where it is not built: makes no call."""
+
+    def __getattr__(self, name: str):
+        return lambda *args: None
+
+
+_calls = _Unbound()
+
+#: The entry points ``_calls`` is given, in its order.
+_CALLED = ("code_object_loaded", "paged_rope_append_mx4", "paged_unpack_mx4", "paged_attention_mx4",
+           "paged_attention_mx4_workspace", "paged_fork", "paged_release", "paged_compact", "paged_copy",
+           "adjust_logits")
+
+
+def _bind_calls() -> None:
+    """Bind ``_calls``, once, on the way of a first call that was made without it."""
+
+    global _calls
+    if type(_calls) is not _Unbound or _raw_stream is None:
+        return
+    try:
+        from . import _calls as module
+    except ImportError:
+        return
+    lib = _lib.library()
+    entries = (ctypes.cast(getattr(lib, "aoto_hip_" + name), ctypes.c_void_p).value for name in _CALLED)
+    module.bind(*entries, _raw_stream, PagedMx4)
+    _calls = module
+
+
+# ------------------------------------------------------------------------------------------------------------------
 # The paged cache in 4 bits. A row of D dims is D / 2 bytes of codes and D / 32 scale bytes: a code is a sign and one of
 # 0, 0.5, 1, 1.5, 2, 3, 4, 6 (dim 2i in the low half of byte i), its group of 32 dims shares the scale 2^(byte - 127),
 # and a byte above 252 makes the group NaN. 68 bytes for 128 dims, 256 in bf16.
@@ -1639,6 +1677,10 @@ def paged_rope_append_mx4(
     magnitudes above 6 to 6; a group that holds an infinity or a NaN stands for NaN.
     """
 
+    made = _calls.paged_rope_append_mx4(qkv, positions, slots, cos_table, sin_table, cache, query_heads, q_out, error)
+    if made is not None:
+        return made
+
     _expect_rows(qkv, "qkv", BF16, 2, qkv.get_device() if isinstance(qkv, torch.Tensor) else 0)
     device = _on_current("qkv", qkv)
     (_, kv_heads, page, dim), arg = _expect_mx4(cache, device)
@@ -1658,6 +1700,7 @@ def paged_rope_append_mx4(
     else:
         _expect_all(device, ((q_out, "q_out", BF16, (tokens, query_heads, dim)),))
     _ready(qkv)
+    _bind_calls()
     _lib.check(
         _lib.library().aoto_hip_paged_rope_append_mx4(
             _ptr(qkv), qkv.stride(0), _ptr(positions), _ptr(slots), _ptr(cos_table), _ptr(sin_table),
@@ -1673,6 +1716,11 @@ def paged_unpack_mx4(cache: PagedMx4, *, out: tuple[torch.Tensor, torch.Tensor] 
     """What a 4-bit cache stands for: ``(keys, values)`` bf16 ``[pages, Hkv, page, D]`` (exact: bf16 holds every value
     that an append writes)."""
 
+    if out is None:
+        made = _calls.paged_unpack_mx4(cache)
+        if made is not None:
+            return made
+
     if not isinstance(cache, PagedMx4):
         raise TypeError(f"cache must be a PagedMx4, got {type(cache).__name__}")
     _expect_rows(cache.keys, "keys", torch.uint8, 4, cache.keys.get_device()
@@ -1685,6 +1733,7 @@ def paged_unpack_mx4(cache: PagedMx4, *, out: tuple[torch.Tensor, torch.Tensor] 
         keys_out, values_out = out
         _expect_all(device, ((keys_out, "out[0]", BF16, shape), (values_out, "out[1]", BF16, shape)))
     _ready(cache.keys)
+    _bind_calls()
     _lib.check(_lib.library().aoto_hip_paged_unpack_mx4(arg, shape[2], shape[1], shape[3], _ptr(out[0]),
                                                         _ptr(out[1]), _stream(device)))
     return out
@@ -1726,6 +1775,11 @@ def paged_attention_mx4(
     dims), in sums that keep 13 bits below the largest of each eight products.
     """
 
+    made = _calls.paged_attention_mx4(q, cache, block_tables, query_start, kv_lens, causal, scale, max_query_len,
+                                      max_kv_len, workspace, out)
+    if made is not None:
+        return made
+
     _expect_rows(q, "q", BF16, 3, q.get_device() if isinstance(q, torch.Tensor) else 0)
     device = _on_current("q", q)
     tokens, query_heads, dim = q.shape
@@ -1743,8 +1797,11 @@ def paged_attention_mx4(
     else:
         _expect_all(device, ((out, "out", BF16, (tokens, query_heads * dim)),))
     _ready(q)
+    _bind_calls()
     lib = _lib.library()
     max_query_len, max_kv_len = int(max_query_len), int(max_kv_len)
+    if not (0 <= max_query_len < 2 ** 31 and 0 <= max_kv_len < 2 ** 31):
+        raise ValueError(f"max_query_len and max_kv_len are of 31 bits, got {max_query_len} and {max_kv_len}")
     need = lib.aoto_hip_paged_attention_mx4_workspace(tokens, requests, max_blocks, page, query_heads, kv_heads, dim,
                                                       max_query_len, max_kv_len)
     if workspace is not None:
@@ -1835,6 +1892,12 @@ def paged_fork(
     ran out: the row ends with its last full page).
     """
 
+    if step is None:
+        made = _calls.paged_fork(parents, context_lens, block_tables, page_counts, shares, free_pages, free_start,
+                                 page_size, error)
+        if made is not None:
+            return PagedFork(*made)
+
     device, requests = _expect_pool(block_tables, page_counts, shares, free_pages, free_start, error)
     _expect_all(device, ((parents, "parents", torch.int32, (requests,)),
                          (context_lens, "context_lens", torch.int32, (requests,))))
@@ -1849,6 +1912,7 @@ def paged_fork(
                              for x, name, shape in zip(step, PagedFork._fields, shapes)))
         plan = shares.new_empty((2 * requests,))
     _ready(shares)
+    _bind_calls()
     _lib.check(
         _lib.library().aoto_hip_paged_fork(
             _ptr(parents), _ptr(context_lens), _ptr(block_tables), block_tables.stride(0), _ptr(page_counts),
@@ -1882,6 +1946,12 @@ def paged_release(
     and ``PAGED_LIST_FULL`` (no place before the list's first: the page is lost).
     """
 
+    if out is None:
+        made = _calls.paged_release(keep_lens, block_tables, page_counts, shares, free_pages, free_start, page_size,
+                                    error)
+        if made is not None:
+            return made
+
     device, requests = _expect_pool(block_tables, page_counts, shares, free_pages, free_start, error)
     _expect_all(device, ((keep_lens, "keep_lens", torch.int32, (requests,)),))
     room = shares.numel() // 1024 + 2
@@ -1893,6 +1963,7 @@ def paged_release(
         _expect_all(device, ((counts_out, "out[0]", torch.int32, (requests,)),
                              (start_out, "out[1]", torch.int32, (1,))))
     _ready(shares)
+    _bind_calls()
     _lib.check(
         _lib.library().aoto_hip_paged_release(
             _ptr(keep_lens), _ptr(block_tables), block_tables.stride(0), _ptr(page_counts), _ptr(shares),
@@ -1924,6 +1995,11 @@ def paged_compact(
     or none.
     """
 
+    if moves is None:
+        made = _calls.paged_compact(block_tables, page_counts, shares, free_pages, free_start, error)
+        if made is not None:
+            return PagedMoves(*made)
+
     device, requests = _expect_pool(block_tables, page_counts, shares, free_pages, free_start, error)
     pages = shares.numel()
     if moves is None:
@@ -1934,6 +2010,7 @@ def paged_compact(
                              for x, name, shape in zip(moves, PagedMoves._fields, ((pages,), (pages,), (1,)))))
         state = shares.new_empty((pages,))
     _ready(shares)
+    _bind_calls()
     _lib.check(
         _lib.library().aoto_hip_paged_compact(
             _ptr(block_tables), block_tables.stride(0), _ptr(page_counts), _ptr(shares), _ptr(free_pages),
@@ -1998,6 +2075,9 @@ def paged_copy(
     is.
     """
 
+    if _calls.paged_copy(caches, source, target, count, dim, error) is not None:
+        return
+
     _expect(source, "source", torch.int32)
     device = _on_current("source", source)
     if source.dim() != 1:
@@ -2018,6 +2098,7 @@ def paged_copy(
     if not source.numel():
         return
     _ready(source)
+    _bind_calls()
     _lib.check(
         _lib.library().aoto_hip_paged_copy(
             b"".join(args), len(args), pages, _ptr(source), _ptr(target), source.numel(), _ptr(count), _ptr(error),
@@ -2058,6 +2139,11 @@ def adjust_logits(
     ``repetition``, ``presence``, ``frequency`` are f32 ``[R]``; what is None is left out. ``out`` may be ``logits``;
     its rows of no request are left as they are (in a new tensor: not set).
     """
+
+    made = _calls.adjust_logits(logits, query_start, history, history_lens, prompt_lens, draft_tokens, repetition,
+                                presence, frequency, bias_tokens, bias_values, allowed, out)
+    if made is not None:
+        return made
 
     dtype = logits.dtype if isinstance(logits, torch.Tensor) else BF16
     if dtype not in (BF16, torch.float32):
@@ -2113,6 +2199,7 @@ def adjust_logits(
                 and (out.data_ptr() != logits.data_ptr() or out.stride() != logits.stride())):
             raise ValueError("out must be logits itself or in memory of its own")
     _ready(logits)
+    _bind_calls()
     _lib.check(
         _lib.library().aoto_hip_adjust_logits(
             _ptr(logits), int(dtype is torch.float32), logits.stride(0), rows, vocab, requests, arg,

@@ -1164,3 +1164,71 @@ def test_a_captured_step_over_a_4_bit_cache_replays():
             assert torch.equal(a, b)
         torch.cuda.synchronize()
     assert int(one["error"]) == 0
+
+
+# ---------------------------------------------------------------- the calls with and without the compiled ones
+def _every_call(ops):
+    """One call of each operator with outputs of its own, the same at every run; what comes back and what is changed."""
+
+    rng = np.random.default_rng(40)
+    cache, _, _ = _cache(rng, 12, 2, 16, 64)
+    qkv, table = to_gpu_bf16(bf16_normal(rng, (5, 8 * 64))), to_gpu_bf16(bf16_normal(rng, (50, 64)))
+    q = ops.paged_rope_append_mx4(qkv, _i64(range(5)), _i64(range(3, 8)), table, table, cache, query_heads=4)
+    yield q, *ops.paged_unpack_mx4(cache)
+    tables = _i32(rng.permutation(12).reshape(2, 6))
+    yield (ops.paged_attention_mx4(q, cache, tables, _i32([0, 2, 5]), _i32([60, 90])),
+           ops.paged_attention_mx4(q, cache, tables, _i32([0, 2, 5]), _i32([60, 90]), causal=False, scale=0.3,
+                                   max_query_len=3, max_kv_len=90))
+    pool = [_i32(x) for x in _pool(rng, [40, 0, 0, 33], 16)]
+    fork = ops.paged_fork(_i32([-1, 0, 3, -1]), _i32([40, 0, 0, 33]), *pool, page_size=16)
+    pages = torch.arange(pool[2].numel() * 10, device="cuda").view(-1, 10).clone()
+    ops.paged_copy(pages, fork.source, fork.target)
+    ops.paged_copy([pages, pages.clone()], fork.source, fork.target, count=_i32([2]))
+    yield *fork, *pool, pages
+    pool[1], pool[4] = fork.page_counts, fork.free_start
+    yield *ops.paged_release(_i32([0, 17, -1, 0]), *pool, page_size=16), *pool
+    yield *ops.paged_compact(*pool), *pool
+    logits, s = _adjustments(rng, [1, 3, 2], 3001, torch.bfloat16)
+    s = {k: torch.tensor(v, device="cuda") for k, v in s.items()}
+    yield (ops.adjust_logits(logits, **s), ops.adjust_logits(logits.float()),
+           ops.adjust_logits(logits, out=logits.clone()))
+
+
+def test_compiled_calls_are_the_calls_that_python_makes(monkeypatch):
+    ops = _ops()
+    ops.paged_unpack_mx4(ops.paged_mx4_cache(1, 1, 1, 64))   # binds them
+    assert ops._calls is not None and type(ops._calls) is not ops._Unbound, "_calls.so is not built"
+    made = [[t.clone() for t in step] for step in _every_call(ops)]
+    with monkeypatch.context() as patch:
+        patch.setattr(ops, "_ready", None)                   # Python's own way ends here
+        for _ in _every_call(ops):
+            pass
+    monkeypatch.setattr(ops, "_calls", ops._Unbound())
+    monkeypatch.setattr(ops, "_bind_calls", lambda: None)
+    for one, two in zip(made, _every_call(ops), strict=True):
+        for a, b in zip(one, two, strict=True):
+            assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
+
+
+def test_compiled_calls_leave_other_arguments_to_python():
+    # numbers of other types, a subclass, sizes that the C ABI refuses: as without them
+    ops = _ops()
+    cache = ops.paged_mx4_cache(4, 2, 16, 64)
+    q = torch.ones((1, 2, 64), dtype=torch.bfloat16, device="cuda")
+    args = (cache, _i32([[0, 1]]), _i32([0, 1]), _i32([20]))
+    want = ops.paged_attention_mx4(q, *args)
+    for kwargs in (dict(scale=np.float32(0.125)), dict(max_query_len=np.int64(1)), dict(max_kv_len=np.int32(20)),
+                   dict(causal=np.bool_(True)), dict(scale=0.125), dict(workspace=torch.empty(3, device="cuda"))):
+        assert torch.equal(ops.paged_attention_mx4(q, *args, **kwargs), want)
+
+    class Other(torch.Tensor):
+        pass
+
+    assert torch.equal(ops.paged_attention_mx4(q.as_subclass(Other), *args).as_subclass(torch.Tensor), want)
+    assert torch.equal(ops.paged_attention_mx4(q.clone().requires_grad_(), *args), want)
+    for kwargs, error in ((dict(scale=-1.0), Exception), (dict(max_query_len=-1), Exception),
+                          (dict(max_kv_len=2 ** 40), Exception), (dict(out=torch.empty(3, device="cuda")), Exception),
+                          (dict(workspace=torch.empty(3)), ValueError), (dict(scale="x"), Exception)):
+        with pytest.raises(error):
+            ops.paged_attention_mx4(q, *args, **kwargs)
+    assert torch.equal(ops.paged_attention_mx4(q, *args), want)
