@@ -3,8 +3,9 @@
 // us a call.
 //
 // Every function gives None where it does not make the call, for an argument that is not what the kernels assume or a
-// status that is not AOTO_OK: ops.py goes through its own checks then, which give the reason, and makes or refuses the
-// call. So nothing is refused here, and nothing is accepted that ops.py would refuse.
+// call that the C ABI refuses: ops.py goes through its own checks then, which give the reason, and makes or refuses the
+// call. So nothing is refused here, and nothing is accepted that ops.py would refuse. A call that fails on its way to
+// the GPU is an exception and not made a second time: some of its kernels may run.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -43,10 +44,13 @@ struct Library {
   decltype(&aoto_hip_adjust_logits) adjust = nullptr;
   PyObject* raw_stream = nullptr;   // device -> address of its current stream
   PyObject* mx4 = nullptr;          // ops.PagedMx4
+  PyObject* check = nullptr;        // status -> its exception
 } lib;
 
 // An argument that is not as it should be.
 struct Unfit {};
+// A Python exception is set.
+struct Raised {};
 
 void need(bool fits) {
   if (!fits) throw Unfit();
@@ -159,7 +163,16 @@ PyObject* wrapped(std::initializer_list<Tensor> tensors) {
   return all;
 }
 
-void ok(int status) { need(status == AOTO_OK); }
+void ok(int status) {
+  if (status == AOTO_OK) return;
+  need(status != AOTO_ERR_ARGUMENT && status != AOTO_ERR_UNSUPPORTED);
+  if (PyObject* number = PyLong_FromLong(status)) {
+    Py_XDECREF(PyObject_CallOneArg(lib.check, number));
+    Py_DECREF(number);
+  }
+  need(PyErr_Occurred());
+  throw Raised();
+}
 
 PyObject* append(PyObject* const* a) {
   Call call;
@@ -412,22 +425,23 @@ PyObject* adjust(PyObject* const* a) {
   return wrapped(out);
 }
 
-// Any way out but a made call is None, with no Python error left behind.
+// None, with no Python error left behind, where the call was not made.
 template <PyObject* (*F)(PyObject* const*), Py_ssize_t N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t count) {
   try {
-    if (count == N)
-      if (PyObject* made = F(args)) return made;
+    if (count == N) return F(args);
+  } catch (const Raised&) {
+    return nullptr;
   } catch (...) {
   }
   PyErr_Clear();
   Py_RETURN_NONE;
 }
 
-// bind(addresses of the entry points in the order of Library, raw_stream, PagedMx4)
+// bind(addresses of the entry points in the order of Library, raw_stream, PagedMx4, check)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t count) {
-  if (count != 12) {
-    PyErr_SetString(PyExc_TypeError, "bind takes ten addresses, a function and a type");
+  if (count != 13) {
+    PyErr_SetString(PyExc_TypeError, "bind takes ten addresses, a function, a type and a function");
     return nullptr;
   }
   void* at[10];
@@ -438,9 +452,9 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t count) {
   auto set = [&](auto& to, int i) { to = reinterpret_cast<std::decay_t<decltype(to)>>(at[i]); };
   set(lib.loaded, 0), set(lib.append, 1), set(lib.unpack, 2), set(lib.attention, 3), set(lib.attention_workspace, 4);
   set(lib.fork, 5), set(lib.release, 6), set(lib.compact, 7), set(lib.copy, 8), set(lib.adjust, 9);
-  Py_INCREF(args[10]), Py_INCREF(args[11]);
-  Py_XDECREF(lib.raw_stream), Py_XDECREF(lib.mx4);
-  lib.raw_stream = args[10], lib.mx4 = args[11];
+  for (int i = 10; i < 13; ++i) Py_INCREF(args[i]);
+  Py_XDECREF(lib.raw_stream), Py_XDECREF(lib.mx4), Py_XDECREF(lib.check);
+  lib.raw_stream = args[10], lib.mx4 = args[11], lib.check = args[12];
   Py_RETURN_NONE;
 }
 

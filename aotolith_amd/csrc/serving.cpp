@@ -37,9 +37,9 @@ int check_cache(const char* what, const aoto_mx4_cache* c, int page, int kv_head
   return AOTO_OK;
 }
 
-// GPU blocks of the attention's narrow tiles of 16 rows that a CU holds. A tile's rows are a quarter of what they are in
-// bf16, so that two do not ask for enough at a time (345000 keys of 64 requests, 8 kv heads of 128: 88 us with two, 84
-// with three, 93 with four, whose registers are too few).
+// GPU blocks of the attention's narrow tiles of 16 rows that a CU holds. A tile's rows are a quarter of what they are
+// in bf16, so that two do not ask for enough at a time (345000 keys of 64 requests, 8 kv heads of 128: 88 us with two,
+// 84 with three, 93 with four, whose registers are too few).
 constexpr int kMx4NarrowBlocks = 3;
 
 // Entries of all block tables up to which the fork's one block enters the pages itself: a second launch costs more than
@@ -221,30 +221,33 @@ int aoto_hip_paged_copy(const aoto_page_tensor* tensors, int tensor_count, int p
                         const int32_t* target, int pairs, const int32_t* count, int32_t* error, void* stream) {
   if (!tensors || !source || !target) return set_error(AOTO_ERR_ARGUMENT, "paged_copy: null pointer");
   if (tensor_count <= 0 || pages <= 0 || pairs <= 0) return set_error(AOTO_ERR_ARGUMENT, "paged_copy: bad shape");
-  for (int from = 0; from < tensor_count; from += kPagedCopyTensors) {
-    PagedCopyArgs a{};
-    a.source = source, a.target = target, a.count = count, a.error = from ? nullptr : error;
-    a.pairs = pairs, a.pages = pages, a.tensors = std::min(kPagedCopyTensors, tensor_count - from), a.wide = 1;
-    long long planes = 0;
-    for (int i = 0; i < a.tensors; ++i) {
-      const aoto_page_tensor& t = tensors[from + i];
-      if (!t.data || t.planes <= 0 || t.page_bytes <= 0)
-        return set_error(AOTO_ERR_ARGUMENT, "paged_copy: tensor %d: bad shape", from + i);
-      const long long chunks = (t.page_bytes - 1) / kPagedCopyChunk + 1;
-      if (chunks > (1 << 20)) return set_error(AOTO_ERR_UNSUPPORTED, "paged_copy: pages of more than 16 GB");
-      a.at[i].base = static_cast<uint8_t*>(t.data), a.at[i].page_stride = t.page_stride;
-      a.at[i].plane_stride = t.plane_stride, a.at[i].bytes = t.page_bytes, a.at[i].first = (int)planes;
-      a.at[i].chunks = (int)chunks, a.chunks = std::max(a.chunks, (int)chunks);
-      if (!aligned(t.data, 16) || t.page_stride % 16 || t.plane_stride % 16 || t.page_bytes % 16) a.wide = 0;
-      planes += t.planes;
-      if (planes > (1 << 20)) return set_error(AOTO_ERR_UNSUPPORTED, "paged_copy: more than 2^20 planes");
+  // all of them looked at before the first launch: a refused call has copied nothing
+  for (const bool run : {false, true})
+    for (int from = 0; from < tensor_count; from += kPagedCopyTensors) {
+      PagedCopyArgs a{};
+      a.source = source, a.target = target, a.count = count, a.error = from ? nullptr : error;
+      a.pairs = pairs, a.pages = pages, a.tensors = std::min(kPagedCopyTensors, tensor_count - from), a.wide = 1;
+      long long planes = 0;
+      for (int i = 0; i < a.tensors; ++i) {
+        const aoto_page_tensor& t = tensors[from + i];
+        if (!t.data || t.planes <= 0 || t.page_bytes <= 0)
+          return set_error(AOTO_ERR_ARGUMENT, "paged_copy: tensor %d: bad shape", from + i);
+        const long long chunks = (t.page_bytes - 1) / kPagedCopyChunk + 1;
+        if (chunks > (1 << 20)) return set_error(AOTO_ERR_UNSUPPORTED, "paged_copy: pages of more than 16 GB");
+        a.at[i].base = static_cast<uint8_t*>(t.data), a.at[i].page_stride = t.page_stride;
+        a.at[i].plane_stride = t.plane_stride, a.at[i].bytes = t.page_bytes, a.at[i].first = (int)planes;
+        a.at[i].chunks = (int)chunks, a.chunks = std::max(a.chunks, (int)chunks);
+        if (!aligned(t.data, 16) || t.page_stride % 16 || t.plane_stride % 16 || t.page_bytes % 16) a.wide = 0;
+        planes += t.planes;
+        if (planes > (1 << 20)) return set_error(AOTO_ERR_UNSUPPORTED, "paged_copy: more than 2^20 planes");
+      }
+      a.planes = (int)planes;
+      if (planes * a.chunks > 0x7FFFFFFFLL) return set_error(AOTO_ERR_UNSUPPORTED, "paged_copy: pages too large");
+      const long long items = planes * a.chunks * (long long)pairs;
+      a.blocks = (int)std::min(items, 8LL * aoto::device_cu_count());  // what the chip holds at a time
+      if (run)
+        if (int s = launch("aoto_paged_copy", a.blocks, 1, 256, stream, a)) return s;
     }
-    a.planes = (int)planes;
-    if (planes * a.chunks > 0x7FFFFFFFLL) return set_error(AOTO_ERR_UNSUPPORTED, "paged_copy: pages too large");
-    const long long items = planes * a.chunks * (long long)pairs;
-    a.blocks = (int)std::min(items, 8LL * aoto::device_cu_count());  // what the chip holds at a time
-    if (int s = launch("aoto_paged_copy", a.blocks, 1, 256, stream, a)) return s;
-  }
   return AOTO_OK;
 }
 
@@ -262,6 +265,7 @@ int aoto_hip_adjust_logits(const void* logits, int logits_f32, int64_t row_strid
   const size_t size = logits_f32 ? 4 : 2;
   if (!aligned(logits, size) || !aligned(out, size))
     return set_error(AOTO_ERR_ARGUMENT, "adjust_logits: logits aligned to their type");
+  if (rows > 1 && out_stride < vocab) return set_error(AOTO_ERR_ARGUMENT, "adjust_logits: rows of out overlap");
   AdjustArgs a{};
   a.logits = logits, a.out = out, a.query_start = j.query_start;
   a.history = reinterpret_cast<const long long*>(j.history), a.history_lens = j.history_lens;
@@ -274,7 +278,7 @@ int aoto_hip_adjust_logits(const void* logits, int logits_f32, int64_t row_strid
   a.rows = rows, a.requests = requests, a.vocab = vocab, a.history_len = j.history_len, a.drafts = j.drafts;
   a.biases = j.biases;
   return launch(logits_f32 ? "aoto_adjust_logits_f32" : "aoto_adjust_logits_bf16", (vocab - 1) / kAdjustChunk + 1,
-                requests, 256, stream, a);
+                requests, kAdjustThreads, stream, a);
 }
 
 }  // extern "C"

@@ -1587,7 +1587,7 @@ def _bind_calls() -> None:
         return
     lib = _lib.library()
     entries = (ctypes.cast(getattr(lib, "aoto_hip_" + name), ctypes.c_void_p).value for name in _CALLED)
-    module.bind(*entries, _raw_stream, PagedMx4)
+    module.bind(*entries, _raw_stream, PagedMx4, _lib.check)
     _calls = module
 
 
@@ -2195,6 +2195,8 @@ def adjust_logits(
         _expect_rows(out, "out", dtype, 2, device)
         if out.shape != logits.shape:
             raise ValueError(f"out must be {(rows, vocab)}, got {tuple(out.shape)}")
+        if rows > 1 and out.stride(0) < vocab:
+            raise ValueError(f"out's rows overlap, got strides {out.stride()}")
         if (out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr()
                 and (out.data_ptr() != logits.data_ptr() or out.stride() != logits.stride())):
             raise ValueError("out must be logits itself or in memory of its own")

@@ -2,6 +2,7 @@
 (``oracle/serving.py``, ``oracle/paged.py``)."""
 
 from __future__ import annotations
+import ctypes
 
 import numpy as np
 import pytest
@@ -1232,3 +1233,56 @@ def test_compiled_calls_leave_other_arguments_to_python():
         with pytest.raises(error):
             ops.paged_attention_mx4(q, *args, **kwargs)
     assert torch.equal(ops.paged_attention_mx4(q, *args), want)
+
+
+def test_calls_that_fail_on_their_way_to_the_gpu_are_made_once(monkeypatch):
+    ops = _ops()
+    _lib = ops._lib
+    ops.paged_unpack_mx4(ops.paged_mx4_cache(1, 1, 1, 64))
+    lib, made = _lib.library(), []
+
+    def entries(status):
+        def failing(*args):
+            made.append(status)
+            return status
+
+        fail = ctypes.CFUNCTYPE(ctypes.c_int, *lib.aoto_hip_paged_fork.argtypes)(failing)
+        at = [ctypes.cast(fail if name == "paged_fork" else getattr(lib, "aoto_hip_" + name), ctypes.c_void_p).value
+              for name in ops._CALLED]
+        return fail, at
+
+    args = (_i32([-1, 0]), _i32([20, 0]), _i32([[1, 2], [0, 0]]), _i32([2, 0]), _i32([0] * 4), _i32([0, 3]), _i32([0]))
+    want = [t.tolist() for t in ops.paged_fork(*(t.clone() for t in args), page_size=16)]
+    rest = (ops._raw_stream, ops.PagedMx4, _lib.check)
+    try:
+        for status in (_lib.AOTO_ERR_HIP, _lib.AOTO_ERR_UNSUPPORTED):
+            held, at = entries(status)
+            ops._calls.bind(*at, *rest)
+            if status == _lib.AOTO_ERR_HIP:
+                with pytest.raises(_lib.HipKernelError):
+                    ops.paged_fork(*args, page_size=16)
+            else:   # nothing was launched: Python makes the call
+                assert [t.tolist() for t in ops.paged_fork(*args, page_size=16)] == want
+        assert made == [_lib.AOTO_ERR_HIP, _lib.AOTO_ERR_UNSUPPORTED]
+    finally:
+        _, at = entries(0)
+        at[ops._CALLED.index("paged_fork")] = ctypes.cast(lib.aoto_hip_paged_fork, ctypes.c_void_p).value
+        ops._calls.bind(*at, *rest)
+    assert args[4].tolist() == [0, 1, 0, 0]   # shared once
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_adjusted_rows_that_overlap_are_refused(monkeypatch, compiled):
+    ops = _ops()
+    ops.paged_unpack_mx4(ops.paged_mx4_cache(1, 1, 1, 64))
+    if not compiled:
+        monkeypatch.setattr(ops, "_calls", ops._Unbound())
+        monkeypatch.setattr(ops, "_bind_calls", lambda: None)
+    one = torch.zeros((1, 50), device="cuda")
+    for out in (one.expand(3, 50), torch.zeros(200, device="cuda").as_strided((3, 50), (49, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.adjust_logits(torch.zeros((3, 50), device="cuda"), out=out)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.adjust_logits(one.expand(3, 50), out=one.expand(3, 50))
+    assert torch.equal(ops.adjust_logits(one.expand(3, 50)), torch.zeros((3, 50), device="cuda"))
+    assert torch.equal(ops.adjust_logits(one, out=one.expand(1, 50)), one)

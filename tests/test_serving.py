@@ -162,6 +162,15 @@ def test_copy_refuses(tensor, changes, code):
     _refused(_copy(tensor, **changes), code, "paged_copy")
 
 
+def test_copy_looks_at_all_tensors_before_it_copies():
+    # the launch for the first ones would answer that no code object is loaded
+    tensor = [4096, 1, 4096, 4096, 1024]
+    for bad, code in ((tensor[:4] + [0], 1), (tensor[:1] + [1 << 21] + tensor[2:], 4)):
+        tensors = b"".join(_lib.PAGE_TENSOR.pack(*t) for t in [tensor] * 40 + [bad])
+        _refused(_lib.library().aoto_hip_paged_copy(tensors, 41, 4, GOOD, GOOD, 2, None, None, None), code,
+                 "paged_copy")
+
+
 def _adjust(fields=None, **changes):
     names = ("query_start", "history", "history_lens", "prompt_lens", "draft_tokens", "repetition", "presence",
              "frequency", "bias_tokens", "bias_values", "allowed", "history_stride", "draft_stride", "bias_stride",
@@ -174,7 +183,8 @@ def _adjust(fields=None, **changes):
 
 
 @pytest.mark.parametrize("adjust,changes,code", [
-    ({}, dict(logits=None), 1), ({}, dict(out=None), 1), ({}, dict(adjust=None), 1), ({}, dict(rows=0), 1),
+    ({}, dict(logits=None), 1), ({}, dict(out=None), 1), ({}, dict(out_row=999), 1), ({}, dict(adjust=None), 1),
+    ({}, dict(rows=0), 1),
     ({}, dict(vocab=0), 1), ({}, dict(requests=0), 1), ({}, dict(vocab=2 ** 30 + 1), 4), ({}, dict(requests=65536), 4),
     ({}, dict(logits=ctypes.c_void_p(4097)), 1), ({}, dict(f32=1, out=ctypes.c_void_p(4098)), 1),
     (dict(history_len=5), {}, 1), (dict(drafts=2), {}, 1), (dict(biases=2), {}, 1),
