@@ -115,6 +115,7 @@ struct PagedMx4UnpackArgs {
 struct PagedMx4AttentionArgs {
   PagedAttentionArgs base;  // its pages' addresses and strides are not used
   PagedMx4Cache cache;
+  int turn_from, turn_to;  // items taken in the opposite order
 };
 
 struct PagedForkArgs {

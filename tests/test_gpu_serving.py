@@ -280,6 +280,15 @@ def test_attention_over_long_requests_is_split_and_joined(rows, dim):
     _check(s, _attend(s, max_query_len=rows, max_kv_len=9000))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_of_more_tiles_than_compute_units(causal):
+    # 18 tiles of 32 kv heads: whole, those from the ninth to the sixteenth in the opposite order
+    rng = np.random.default_rng(18)
+    s = _requests(rng, [(700, 900), (1, 50), (900, 900), (0, 4), (300, 1400)], 32, 32, 64, 16, tail=2)
+    assert _ops().paged_attention_mx4_workspace(1903, 5, s["tables"].shape[1], 16, 32, 32, 64).numel() == 16
+    _check(s, _attend(s, causal=causal), causal=causal)
+
+
 @pytest.mark.parametrize("rows", [1, 20])
 def test_attention_without_keys_gives_zero(rows):
     rng = np.random.default_rng(8)
