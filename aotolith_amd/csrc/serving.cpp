@@ -42,9 +42,9 @@ int check_cache(const char* what, const aoto_mx4_cache* c, int page, int kv_head
 // 84 with three, 93 with four, whose registers are too few).
 constexpr int kMx4NarrowBlocks = 3;
 
-// Entries of all block tables up to which the fork's one block enters the pages itself: a second launch costs more than
-// it saves.
-constexpr long long kForkFill = 16384;
+// Entries of all block tables up to which the fork's one block enters the pages itself instead of a second launch (8 x
+// 64 entries 3.9 us and 5.5 with two launches, 32 x 64 4.8 and 5.6, 64 x 64 6.5 and 5.5, 64 x 256 17.1 and 5.7).
+constexpr long long kForkFill = 2048;
 
 }  // namespace
 
