@@ -806,6 +806,15 @@ def test_copy_refusals():
         ops.paged_copy(x, pair[0].long(), pair[1].long())
 
 
+def test_copy_past_32_bits():
+    x = torch.zeros((5, 2 ** 30 + 48), dtype=torch.uint8, device="cuda")
+    x[1].fill_(7)
+    x[1, -1] = 9
+    _ops().paged_copy(x, _i32([1, -1]), _i32([4, 2]))
+    assert torch.equal(x[4], x[1])
+    assert not x[0].any() and not x[2:4].any()
+
+
 # ---------------------------------------------------------------- logits
 def _adjustments(rng, counts, vocab, dtype, *, length=200, drafts=3, biases=5, masked=True):
     requests, rows = len(counts), int(np.sum(counts))
@@ -946,6 +955,17 @@ def test_adjust_of_infinite_and_missing_logits(dtype):
     lowest = torch.full_like(logits, torch.finfo(dtype).min)
     _check_adjusted(lowest, s, repetition=np.ones(2, np.float32), presence=None, frequency=None, bias_tokens=None,
                     bias_values=None)
+
+
+def test_adjust_past_32_bits():
+    rows, vocab = 17000, 131101   # 2.2e9 logits, two bytes each
+    logits = torch.ones((rows, vocab), dtype=torch.bfloat16, device="cuda")
+    history = _i64([[vocab - 1, 5, 40000]])
+    kwargs = dict(history=history, frequency=torch.full((1,), 0.5, device="cuda"))
+    want = _ops().adjust_logits(torch.ones((3, vocab), dtype=torch.bfloat16, device="cuda"), _i32([0, 3]), **kwargs)
+    assert want[:, [vocab - 1, 5, 40000]].eq(0.5).all() and want.eq(1).sum() == 3 * (vocab - 3)
+    assert _ops().adjust_logits(logits, _i32([rows - 3, rows]), **kwargs, out=logits) is logits
+    assert torch.equal(logits[-3:], want) and logits[:-3].eq(1).all()
 
 
 def test_adjust_refusals():
