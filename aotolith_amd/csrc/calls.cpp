@@ -174,6 +174,16 @@ void ok(int status) {
   throw Raised();
 }
 
+// The C ABI's call without the interpreter's lock: a launch may wait for room in its queue.
+template <typename F>
+int unlocked(F call) {
+  struct Unlocked {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Unlocked() { PyEval_RestoreThread(state); }
+  } here;
+  return call();
+}
+
 PyObject* append(PyObject* const* a) {
   Call call;
   const Tensor& qkv = call.rows(a[0], kBFloat16, 2);
@@ -193,9 +203,12 @@ PyObject* append(PyObject* const* a) {
   }
   int32_t* error = call.one<int32_t>(a[8]);
   if (!q.defined()) q = call.empty({tokens, heads, cache.dim}, kBFloat16);
-  ok(lib.append(qkv.data_ptr(), qkv.stride(0), data<int64_t>(positions), data<int64_t>(slots), cos.data_ptr(),
-                sin.data_ptr(), small(cos.size(0)), &cache.c, small(cache.page), small(tokens), (int)heads,
-                small(cache.kv_heads), small(cache.dim), q.data_ptr(), error, call.stream()));
+  void* const stream = call.stream();
+  ok(unlocked([&] {
+    return lib.append(qkv.data_ptr(), qkv.stride(0), data<int64_t>(positions), data<int64_t>(slots), cos.data_ptr(),
+                      sin.data_ptr(), small(cos.size(0)), &cache.c, small(cache.page), small(tokens), (int)heads,
+                      small(cache.kv_heads), small(cache.dim), q.data_ptr(), error, stream);
+  }));
   return wrapped(q);
 }
 
@@ -204,8 +217,11 @@ PyObject* unpack(PyObject* const* a) {
   const Cache cache = cache_of(call, a[0]);
   const std::array<int64_t, 4> shape = {cache.c.pages, cache.kv_heads, cache.page, cache.dim};
   const Tensor keys = call.empty(shape, kBFloat16), values = call.empty(shape, kBFloat16);
-  ok(lib.unpack(&cache.c, small(cache.page), small(cache.kv_heads), small(cache.dim), keys.data_ptr(),
-                values.data_ptr(), call.stream()));
+  void* const stream = call.stream();
+  ok(unlocked([&] {
+    return lib.unpack(&cache.c, small(cache.page), small(cache.kv_heads), small(cache.dim), keys.data_ptr(),
+                      values.data_ptr(), stream);
+  }));
   return wrapped({keys, values});
 }
 
@@ -246,10 +262,13 @@ PyObject* attention(PyObject* const* a) {
   }
   if (size && !workspace.defined()) workspace = call.empty({(int64_t)size}, kByte);
   if (!out.defined()) out = call.empty({tokens, heads * dim}, kBFloat16);
-  ok(lib.attention(q.data_ptr(), q.stride(0), q.stride(1), &cache.c, small(cache.page), data<int32_t>(tables),
-                   tables.stride(0), small(blocks), data<int32_t>(start), data<int32_t>(kv), small(tokens),
-                   small(requests), small(heads), small(cache.kv_heads), small(dim), causal, (float)scale, rows, keys,
-                   size ? workspace.data_ptr() : nullptr, out.data_ptr(), call.stream()));
+  void* const stream = call.stream();
+  ok(unlocked([&] {
+    return lib.attention(q.data_ptr(), q.stride(0), q.stride(1), &cache.c, small(cache.page), data<int32_t>(tables),
+                         tables.stride(0), small(blocks), data<int32_t>(start), data<int32_t>(kv), small(tokens),
+                         small(requests), small(heads), small(cache.kv_heads), small(dim), causal, (float)scale, rows,
+                         keys, size ? workspace.data_ptr() : nullptr, out.data_ptr(), stream);
+  }));
   return wrapped(out);
 }
 
@@ -274,11 +293,14 @@ PyObject* fork(PyObject* const* a) {
   const int page = number(a[7]);
   const int64_t n = p.requests;
   const std::vector<Tensor> out = call.lists({n, n, 1, n, n, 2 * n});
-  ok(lib.fork(data<int32_t>(parents), data<int32_t>(lens), data<int32_t>(p.tables), p.tables.stride(0),
-              data<int32_t>(p.counts), data<int32_t>(p.shares), data<int32_t>(p.free), data<int32_t>(p.start),
-              small(n), small(p.tables.size(1)), small(p.free.size(0)), small(p.shares.size(0)), page,
-              data<int32_t>(out[0]), data<int32_t>(out[1]), data<int32_t>(out[2]), data<int32_t>(out[3]),
-              data<int32_t>(out[4]), data<int32_t>(out[5]), p.error, call.stream()));
+  void* const stream = call.stream();
+  ok(unlocked([&] {
+    return lib.fork(data<int32_t>(parents), data<int32_t>(lens), data<int32_t>(p.tables), p.tables.stride(0),
+                    data<int32_t>(p.counts), data<int32_t>(p.shares), data<int32_t>(p.free), data<int32_t>(p.start),
+                    small(n), small(p.tables.size(1)), small(p.free.size(0)), small(p.shares.size(0)), page,
+                    data<int32_t>(out[0]), data<int32_t>(out[1]), data<int32_t>(out[2]), data<int32_t>(out[3]),
+                    data<int32_t>(out[4]), data<int32_t>(out[5]), p.error, stream);
+  }));
   return wrapped({out[0], out[1], out[2], out[3], out[4]});
 }
 
@@ -288,10 +310,13 @@ PyObject* release(PyObject* const* a) {
   const Tensor& keep = call.list(a[0], kInt, p.requests);
   const int page = number(a[6]);
   const std::vector<Tensor> out = call.lists({p.requests, 1, p.shares.size(0) / 1024 + 2});
-  ok(lib.release(data<int32_t>(keep), data<int32_t>(p.tables), p.tables.stride(0), data<int32_t>(p.counts),
-                 data<int32_t>(p.shares), data<int32_t>(p.free), data<int32_t>(p.start), small(p.requests),
-                 small(p.tables.size(1)), small(p.free.size(0)), small(p.shares.size(0)), page, data<int32_t>(out[0]),
-                 data<int32_t>(out[1]), data<int32_t>(out[2]), p.error, call.stream()));
+  void* const stream = call.stream();
+  ok(unlocked([&] {
+    return lib.release(data<int32_t>(keep), data<int32_t>(p.tables), p.tables.stride(0), data<int32_t>(p.counts),
+                       data<int32_t>(p.shares), data<int32_t>(p.free), data<int32_t>(p.start), small(p.requests),
+                       small(p.tables.size(1)), small(p.free.size(0)), small(p.shares.size(0)), page,
+                       data<int32_t>(out[0]), data<int32_t>(out[1]), data<int32_t>(out[2]), p.error, stream);
+  }));
   return wrapped({out[0], out[1]});
 }
 
@@ -300,10 +325,13 @@ PyObject* compact(PyObject* const* a) {
   const Pool p(call, a, a[5]);
   const int64_t n = p.shares.size(0);
   const std::vector<Tensor> out = call.lists({n, n, 1, n});
-  ok(lib.compact(data<int32_t>(p.tables), p.tables.stride(0), data<int32_t>(p.counts), data<int32_t>(p.shares),
-                 data<int32_t>(p.free), data<int32_t>(p.start), small(p.requests), small(p.tables.size(1)),
-                 small(p.free.size(0)), small(n), data<int32_t>(out[0]), data<int32_t>(out[1]), data<int32_t>(out[2]),
-                 data<int32_t>(out[3]), p.error, call.stream()));
+  void* const stream = call.stream();
+  ok(unlocked([&] {
+    return lib.compact(data<int32_t>(p.tables), p.tables.stride(0), data<int32_t>(p.counts), data<int32_t>(p.shares),
+                       data<int32_t>(p.free), data<int32_t>(p.start), small(p.requests), small(p.tables.size(1)),
+                       small(p.free.size(0)), small(n), data<int32_t>(out[0]), data<int32_t>(out[1]),
+                       data<int32_t>(out[2]), data<int32_t>(out[3]), p.error, stream);
+  }));
   return wrapped({out[0], out[1], out[2]});
 }
 
@@ -359,8 +387,11 @@ PyObject* copy(PyObject* const* a) {
     if (pages < 0) pages = t.size(dim);
     tensors.push_back(pages_of(t, dim, pages));
   }
-  ok(lib.copy(tensors.data(), small(n), small(pages), data<int32_t>(source), data<int32_t>(target),
-              small(source.size(0)), count, error, call.stream()));
+  void* const stream = call.stream();
+  ok(unlocked([&] {
+    return lib.copy(tensors.data(), small(n), small(pages), data<int32_t>(source), data<int32_t>(target),
+                    small(source.size(0)), count, error, stream);
+  }));
   Py_RETURN_TRUE;
 }
 
@@ -420,8 +451,11 @@ PyObject* adjust(PyObject* const* a) {
   } else {
     out = call.empty({rows, vocab}, type);
   }
-  ok(lib.adjust(logits.data_ptr(), type == kFloat, logits.stride(0), small(rows), small(vocab), small(requests), &j,
-                out.data_ptr(), out.stride(0), call.stream()));
+  void* const stream = call.stream();
+  ok(unlocked([&] {
+    return lib.adjust(logits.data_ptr(), type == kFloat, logits.stride(0), small(rows), small(vocab), small(requests),
+                      &j, out.data_ptr(), out.stride(0), stream);
+  }));
   return wrapped(out);
 }
 
