@@ -243,5 +243,8 @@ AOTO_PAGED_MX4_ATTENTION(64)
 AOTO_PAGED_MX4_ATTENTION(128)
 
 // Penalties, biases and masks of logits, by the logits' type.
-AOTO_ADJUST_INSTANCE(bf16, false)
-AOTO_ADJUST_INSTANCE(f32, true)
+AOTO_ADJUST_INSTANCE(bf16_2, false, 2, 512)
+AOTO_ADJUST_INSTANCE(bf16_4, false, 4, 256)
+AOTO_ADJUST_INSTANCE(bf16_8, false, 8, 256)
+AOTO_ADJUST_INSTANCE(f32_2, true, 2, 512)
+AOTO_ADJUST_INSTANCE(f32_4, true, 4, 256)

@@ -194,10 +194,6 @@ struct PagedCopyArgs {
   PagedCopyTensor at[kPagedCopyTensors];
 };
 
-// Tokens of a vocabulary that a block of adjust_logits takes: eight a thread.
-constexpr int kAdjustChunk = 2048, kAdjustThreads = kAdjustChunk / 8;
-constexpr int kAdjustSome = 8;
-
 struct AdjustArgs {
   const void* logits;
   void* out;

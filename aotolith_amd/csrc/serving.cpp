@@ -285,8 +285,12 @@ int aoto_hip_adjust_logits(const void* logits, int logits_f32, int64_t row_strid
   a.value_stride = j.value_stride, a.allowed_stride = 4 * j.allowed_stride;
   a.rows = rows, a.requests = requests, a.vocab = vocab, a.history_len = j.history_len, a.drafts = j.drafts;
   a.biases = j.biases;
-  return launch(logits_f32 ? "aoto_adjust_logits_f32" : "aoto_adjust_logits_bf16", (vocab - 1) / kAdjustChunk + 1,
-                requests, kAdjustThreads, stream, a);
+  // tokens a thread, by the logits that there are room for (adjust.h)
+  const long long most = (long long)rows * vocab;
+  const int per = most <= 1 << 21 ? 2 : logits_f32 || most <= 1 << 23 ? 4 : 8, threads = per == 2 ? 512 : 256;
+  char name[64];
+  snprintf(name, sizeof(name), "aoto_adjust_logits_%s_%d", logits_f32 ? "f32" : "bf16", per);
+  return launch(name, (vocab - 1) / (per * threads) + 1, requests, threads, stream, a);
 }
 
 }  // extern "C"

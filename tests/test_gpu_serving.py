@@ -886,6 +886,26 @@ def test_adjust_without_some_of_it(without, dtype):
     _check_adjusted(logits, {k: v for k, v in s.items() if k not in without})
 
 
+@pytest.mark.parametrize("kernel,counts,vocab", [
+    ("bf16_2", [5, 0, 9], 4099), ("bf16_4", [5, 1, 9, 0], 150001), ("bf16_8", [5, 4, 8] * 4, 140003),
+    ("bf16_8", [61], 140006), ("f32_2", [5, 0, 9], 4098), ("f32_4", [5, 1, 9, 0], 150003)])
+def test_adjust_of_every_form(kernel, counts, vocab):
+    rng = np.random.default_rng(vocab)
+    dtype = torch.bfloat16 if kernel.startswith("bf16") else torch.float32
+    logits, s = _adjustments(rng, counts, vocab, dtype, drafts=8)
+    rows = len(logits)
+    s["history"][:, :40] = vocab - 1 - np.arange(40)     # the last block's too
+    wide = torch.full((rows, vocab + 5), 7.0, dtype=dtype, device="cuda")
+    wide[:, 1: vocab + 1] = logits
+    same = logits.clone()
+    with _ops().recording_launches() as take:
+        _check_adjusted(logits, s)
+        _check_adjusted(same, s, out=same, allowed=None)
+        _check_adjusted(wide[:, 1: vocab + 1], s, out=wide[:, 1: vocab + 1])
+        assert set(take()) == {"aoto_adjust_logits_" + kernel}
+    assert bool((wide[:, 0] == 7.0).all()) and bool((wide[:, vocab + 1:] == 7.0).all())
+
+
 def test_adjust_of_a_row_each():
     logits, s = _adjustments(np.random.default_rng(2), [1] * 5, 3001, torch.bfloat16)
     del s["query_start"]
