@@ -137,8 +137,8 @@ struct PagedForkArgs {
   int requests, max_blocks, free_count, pages, page;
 };
 
-// Pages that a block of paged_release looks at.
-constexpr int kPageChunk = 1024;
+// Pages that a block of paged_release looks at, and pages of a pool that one block does all of it for.
+constexpr int kPageChunk = 1024, kPagesFew = 4096;
 
 struct PagedReleaseArgs {
   const int* keep_lens;

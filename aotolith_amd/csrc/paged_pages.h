@@ -66,6 +66,26 @@ AOTO_DEVICE PageFour page_four(const int* values, int from, int count) {
   return four;
 }
 
+// f(row, place, page) for the table entries of all rows (those past a row's count too), by one block: eight entries a
+// thread on their way at a time.
+template <typename F>
+AOTO_DEVICE void each_entry(const int* tables, long long stride, int requests, int max_blocks, F f) {
+  const int all = requests * max_blocks, tid = threadIdx.x;
+  for (int base = 0; base < all; base += kPageBatch) {
+    int page[kPageSteps];
+#pragma unroll
+    for (int i = 0; i < kPageSteps; ++i) {
+      const int k = min(base + 1024 * i + tid, all - 1), r = k / max_blocks;
+      page[i] = tables[(size_t)r * stride + (k - r * max_blocks)];
+    }
+#pragma unroll
+    for (int i = 0; i < kPageSteps; ++i) {
+      const int k = base + 1024 * i + tid, r = k / max_blocks;
+      if (k < all) f(r, k - r * max_blocks, page[i]);
+    }
+  }
+}
+
 }  // namespace aoto
 
 // Which rows go on from which, the pages taken for them and what is to be copied (formulas at the entry point's
@@ -142,11 +162,18 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_share(PagedForkArgs
   for (int j = threadIdx.x; j < full; j += 256) aoto::share_page(a, r, j);
 }
 
+namespace aoto {
+// The pages that a request holds, and those of them that it keeps.
+AOTO_DEVICE int pages_held(const PagedReleaseArgs& a, int held) { return min(max(held, 0), a.max_blocks); }
+AOTO_DEVICE int pages_kept(const PagedReleaseArgs& a, int count, int keep) {
+  return keep < 0 ? count : min(count, (int)(((unsigned)keep + (unsigned)a.page - 1) / (unsigned)a.page));
+}
+}  // namespace aoto
+
 // Requests' pages past what they keep lose a holder each; a page without one stands at -1 until aoto_paged_reclaim.
 extern "C" __global__ __launch_bounds__(256) void aoto_paged_drop(PagedReleaseArgs a) {
   const int r = blockIdx.x, held = a.page_counts[r], keep = a.keep_lens[r];
-  const int count = min(max(held, 0), a.max_blocks);
-  const int stays = keep < 0 ? count : min(count, (int)(((unsigned)keep + (unsigned)a.page - 1) / (unsigned)a.page));
+  const int count = aoto::pages_held(a, held), stays = aoto::pages_kept(a, count, keep);
   __syncthreads();  // the counts written may be the counts read
   if (threadIdx.x == 0) a.page_counts_out[r] = keep < 0 ? held : stays;
   const int* table = a.block_tables + (size_t)r * a.table_stride;
@@ -210,6 +237,56 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_reclaim(PagedReleas
     }
   if (error && a.error) atomicOr(a.error, error);
   if (tid == 0 && chunk == (a.pages - 1) / kPageChunk) a.free_start_out[0] = total ? max(0, first - total) : start;
+}
+
+// All of it by one block, which counts the holders that go in LDS: pools of up to kPagesFew pages. What bounds it is
+// one CU's reading, so it gains by its two launches fewer (2 to 3 us each where they are not captured) and only as long
+// as the GPU is hardly slower: 512 entries of tables and 600 pages 5.6 us and 5.7 in three launches, 2048 and 2500 6.6
+// and 6.5, 4096 and 5000 7.6 and 6.3, 8192 and 10000 11.0 and 6.6.
+extern "C" __global__ __launch_bounds__(1024) void aoto_paged_release_few(PagedReleaseArgs a) {
+  using namespace aoto;
+  __shared__ int s_gone[kPagesFew];
+  __shared__ int s_scratch[kPageRanks];
+  const int tid = threadIdx.x;
+  const int start = a.free_start[0], first = min(max(start, 0), a.free_count);
+  for (int page = tid; page < a.pages; page += 1024) s_gone[page] = 0;
+  __syncthreads();
+  each_entry(a.block_tables, a.table_stride, a.requests, a.max_blocks, [&](int r, int j, int page) {
+    const int count = pages_held(a, a.page_counts[r]);
+    if (j < count && j >= pages_kept(a, count, a.keep_lens[r]) && (unsigned)page < (unsigned)a.pages)
+      atomicAdd(&s_gone[page], 1);
+  });
+  __syncthreads();  // also: the counts written may be the counts read
+  for (int r = tid; r < a.requests; r += 1024) {
+    const int held = a.page_counts[r], keep = a.keep_lens[r];
+    a.page_counts_out[r] = keep < 0 ? held : pages_kept(a, pages_held(a, held), keep);
+  }
+  static_assert(kPagesFew <= kPageBatch, "one look at each page");
+  int left[kPageSteps], rank[kPageSteps], total, error = 0;
+  uint32_t none = 0;
+#pragma unroll
+  for (int i = 0; i < kPageSteps; ++i) {
+    const int page = 1024 * i + tid;
+    left[i] = page < a.pages ? a.shares[page] : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < kPageSteps; ++i) {
+    const int page = 1024 * i + tid, gone = page < a.pages ? s_gone[page] : 0;
+    left[i] -= gone;
+    none |= (uint32_t)(left[i] < 0) << i;
+    if (gone || left[i] < 0) a.shares[page] = max(left[i], 0);
+    if (left[i] < -1) error |= AOTO_PAGED_BAD_SHARE;
+  }
+  page_ranks(none, rank, total, s_scratch);
+#pragma unroll
+  for (int i = 0; i < kPageSteps; ++i)
+    if (none >> i & 1) {
+      const int at = first - 1 - rank[i];
+      if (at >= 0) a.free_pages[at] = 1024 * i + tid;
+      else error |= AOTO_PAGED_LIST_FULL;
+    }
+  if (error && a.error) atomicOr(a.error, error);
+  if (tid == 0) a.free_start_out[0] = total ? max(0, first - total) : start;
 }
 
 // What each page is: 0, and then (aoto_paged_mark) 1 where a request holds it, 2 where it is in the free list.

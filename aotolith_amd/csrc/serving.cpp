@@ -46,6 +46,9 @@ constexpr int kMx4NarrowBlocks = 3;
 // 64 entries 3.9 us and 5.5 with two launches, 32 x 64 4.8 and 5.6, 64 x 64 6.5 and 5.5, 64 x 256 17.1 and 5.7).
 constexpr long long kForkFill = 2048;
 
+// Entries of all block tables up to which one block releases the pages of a pool of up to kPagesFew (paged_pages.h).
+constexpr long long kReleaseFew = 4096;
+
 }  // namespace
 
 extern "C" {
@@ -196,6 +199,8 @@ int aoto_hip_paged_release(const int32_t* keep_lens, const int32_t* block_tables
   a.free_pages = free_pages, a.free_start = free_start, a.page_counts_out = page_counts_out;
   a.free_start_out = free_start_out, a.error = error, a.table_stride = table_stride, a.requests = requests;
   a.max_blocks = max_blocks, a.free_count = free_count, a.pages = pages, a.page = page, a.scratch = scratch;
+  if (pages <= kPagesFew && (long long)requests * max_blocks <= kReleaseFew)
+    return launch("aoto_paged_release_few", 1, 1, 1024, stream, a);
   const int chunks = (pages - 1) / kPageChunk + 1;
   if (int s = launch("aoto_paged_drop", requests, 1, 256, stream, a)) return s;
   if (int s = launch("aoto_paged_gone", chunks, 1, 256, stream, a)) return s;

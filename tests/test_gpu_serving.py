@@ -677,13 +677,25 @@ def test_release_of_large_pools(pages):
     _check_release(np.full(100, -1), *state, 1)      # nothing is given back
 
 
-def test_release_of_what_is_not_held():
+@pytest.mark.parametrize("pages", [1, 4095, 4096, 4097])
+def test_release_in_one_launch_and_in_three(pages):
+    rng = np.random.default_rng(pages)
+    for requests, most in ((1, pages), (40, pages // 60), (4, pages // 5)):
+        lens = rng.integers(0, most + 1, requests)
+        state = _pool(rng, lens, 1, spare=pages - int(lens.sum()), share=0.4, blocks=max(1, 4096 // requests))
+        with _ops().recording_launches() as take:
+            _check_release(np.where(rng.random(requests) < 0.5, 0, lens // 2), *state, 1, in_place=requests == 4)
+            assert take()[0] == "aoto_paged_" + ("release_few" if pages <= 4096 else "drop")
+
+
+@pytest.mark.parametrize("spare", [20, 5000])   # one launch, three
+def test_release_of_what_is_not_held(spare):
     rng = np.random.default_rng(8)
-    tables, counts, shares, free, start = _pool(rng, [60, 60, 30], 16)
+    tables, counts, shares, free, start = _pool(rng, [60, 60, 30], 16, spare=spare)
     tables[1, 1] = tables[0, 1]                       # held twice, said to be held once
     tables[1, 2], tables[2, 1] = -1, 10 ** 6
     assert _check_release([0, 0, 0], tables, counts, shares, free, start, 16)[4] == 128
-    tables, counts, shares, free, start = _pool(rng, [60, 60, 30], 16)
+    tables, counts, shares, free, start = _pool(rng, [60, 60, 30], 16, spare=spare)
     assert _check_release([0, 0, 0], tables, counts, shares, free, np.array([3], np.int32), 16)[4] == 256
     counts[0], counts[1] = 1000, -4                   # counts past the table, below it
     _check_release([20, 0, -7], tables, counts, shares, free, start, 16)
