@@ -279,6 +279,8 @@ int aoto_hip_adjust_logits(const void* logits, int logits_f32, int64_t row_strid
   if (!aligned(logits, size) || !aligned(out, size))
     return set_error(AOTO_ERR_ARGUMENT, "adjust_logits: logits aligned to their type");
   if (rows > 1 && out_stride < vocab) return set_error(AOTO_ERR_ARGUMENT, "adjust_logits: rows of out overlap");
+  if (rows > 1 && out == logits && out_stride != row_stride)
+    return set_error(AOTO_ERR_ARGUMENT, "adjust_logits: out is logits at another stride");
   AdjustArgs a{};
   a.logits = logits, a.out = out, a.query_start = j.query_start;
   a.history = reinterpret_cast<const long long*>(j.history), a.history_lens = j.history_lens;

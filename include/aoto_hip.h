@@ -784,7 +784,8 @@ int aoto_hip_paged_copy(const aoto_page_tensor* tensors, int tensor_count, int p
  *   z + bias_values[r][j] for the last j with bias_tokens[r][j] = v
  *   -inf where bit v % 32 of allowed[row][v / 32] is 0
  * in f32, rounded once to the logits' type. NULL repetition, presence, frequency, allowed: left out. Tokens outside the
- * vocabulary are no tokens. Strides in elements. Rows of no request keep what out held; out may be logits. */
+ * vocabulary are no tokens. Strides in elements. Rows of no request keep what out held. out may be logits, at the same
+ * stride; else it overlaps neither them nor itself. */
 typedef struct aoto_adjustments {
   const int32_t* query_start;
   const int64_t* history;

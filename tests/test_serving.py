@@ -184,7 +184,7 @@ def _adjust(fields=None, **changes):
 
 @pytest.mark.parametrize("adjust,changes,code", [
     ({}, dict(logits=None), 1), ({}, dict(out=None), 1), ({}, dict(out_row=999), 1), ({}, dict(adjust=None), 1),
-    ({}, dict(rows=0), 1),
+    ({}, dict(rows=0), 1), ({}, dict(out_row=1008), 1),
     ({}, dict(vocab=0), 1), ({}, dict(requests=0), 1), ({}, dict(vocab=2 ** 30 + 1), 4), ({}, dict(requests=65536), 4),
     ({}, dict(logits=ctypes.c_void_p(4097)), 1), ({}, dict(f32=1, out=ctypes.c_void_p(4098)), 1),
     (dict(history_len=5), {}, 1), (dict(drafts=2), {}, 1), (dict(biases=2), {}, 1),
