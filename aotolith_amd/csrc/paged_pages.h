@@ -315,9 +315,9 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_mark(PagedCompactAr
 
 // The moves. With m pages held, and the pages held or free in the order of their numbers: held ones past the first m
 // go, in order, to the free ones among the first m, and the rest is the free list. One block: 8192 pages a round trip,
-// once for m and once for the places.
-extern "C" __global__ __launch_bounds__(1024) void aoto_paged_moves(PagedCompactArgs a) {
-  using namespace aoto;
+// once for m and once for the places. `state_of`: what each page is, then its new number.
+namespace aoto {
+AOTO_DEVICE void page_moves(const PagedCompactArgs& a, int* state_of) {
   __shared__ int s_scratch[kPageRanks];
   __shared__ int s_low;
   const int tid = threadIdx.x;
@@ -328,7 +328,7 @@ extern "C" __global__ __launch_bounds__(1024) void aoto_paged_moves(PagedCompact
 #pragma unroll
     for (int i = 0; i < kPageSteps; ++i) {
       const int page = base + 1024 * i + tid;
-      state[i] = page < a.pages ? a.state[page] : 0;
+      state[i] = page < a.pages ? state_of[page] : 0;
     }
 #pragma unroll
     for (int i = 0; i < kPageSteps; ++i) own += state[i] & 1, both += state[i] == 3;
@@ -346,7 +346,7 @@ extern "C" __global__ __launch_bounds__(1024) void aoto_paged_moves(PagedCompact
 #pragma unroll
     for (int i = 0; i < kPageSteps; ++i) {
       const int page = base + 1024 * i + tid;
-      state[i] = page < a.pages ? a.state[page] : 0;
+      state[i] = page < a.pages ? state_of[page] : 0;
     }
     uint32_t any = 0, is_held = 0;
 #pragma unroll
@@ -383,7 +383,7 @@ extern "C" __global__ __launch_bounds__(1024) void aoto_paged_moves(PagedCompact
         const int at = first + place[i] - m;
         if (at < a.free_count) a.free_pages[at] = page;
       }
-      a.state[page] = now;
+      state_of[page] = now;
     }
     places += some, held += some_held;
     __syncthreads();
@@ -397,6 +397,11 @@ extern "C" __global__ __launch_bounds__(1024) void aoto_paged_moves(PagedCompact
   if (error && a.error) atomicOr(a.error, error);
   if (tid == 0) a.count[0] = moved;
 }
+}  // namespace aoto
+
+extern "C" __global__ __launch_bounds__(1024) void aoto_paged_moves(PagedCompactArgs a) {
+  aoto::page_moves(a, a.state);
+}
 
 extern "C" __global__ __launch_bounds__(256) void aoto_paged_remap(PagedCompactArgs a) {
   const int r = blockIdx.x, count = min(max(a.page_counts[r], 0), a.max_blocks);
@@ -405,6 +410,31 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_remap(PagedCompactA
     const int page = *entry;
     if ((unsigned)page < (unsigned)a.pages) *entry = a.state[page];
   }
+}
+
+// All of it by one block, with the pages' states in LDS: pools of up to kPagesFew pages. As in aoto_paged_release_few,
+// the gain is three launches: 512 entries of tables and 600 pages 9.8 us and 11.5 in four, 2048 and 2500 11.4 and 11.7,
+// 4096 and 5000 12.9 and 12.4, 8192 and 10000 19.3 and 16.8.
+extern "C" __global__ __launch_bounds__(1024) void aoto_paged_compact_few(PagedCompactArgs a) {
+  using namespace aoto;
+  __shared__ int s_state[kPagesFew];
+  const int tid = threadIdx.x;
+  for (int page = tid; page < a.pages; page += 1024) s_state[page] = 0;
+  __syncthreads();
+  auto mark = [&](int page, int as) {
+    if ((unsigned)page < (unsigned)a.pages) atomicOr(&s_state[page], as);
+  };
+  each_entry(a.block_tables, a.table_stride, a.requests, a.max_blocks, [&](int r, int j, int page) {
+    if (j < a.page_counts[r]) mark(page, 1);
+  });
+  for (long long j = max(a.free_start[0], 0) + tid; j < a.free_count; j += 1024) mark(a.free_pages[j], 2);
+  __syncthreads();
+  page_moves(a, s_state);
+  __syncthreads();
+  each_entry(a.block_tables, a.table_stride, a.requests, a.max_blocks, [&](int r, int j, int page) {
+    if (j < a.page_counts[r] && (unsigned)page < (unsigned)a.pages)
+      a.block_tables[(size_t)r * a.table_stride + j] = s_state[page];
+  });
 }
 
 // Pages' contents from source[i] to target[i], in every plane of every tensor. Every wave looks at 64 pairs at a time,

@@ -46,8 +46,9 @@ constexpr int kMx4NarrowBlocks = 3;
 // 64 entries 3.9 us and 5.5 with two launches, 32 x 64 4.8 and 5.6, 64 x 64 6.5 and 5.5, 64 x 256 17.1 and 5.7).
 constexpr long long kForkFill = 2048;
 
-// Entries of all block tables up to which one block releases the pages of a pool of up to kPagesFew (paged_pages.h).
-constexpr long long kReleaseFew = 4096;
+// Entries of all block tables (and of the free list) up to which one block releases the pages of a pool of up to
+// kPagesFew, or compacts it (paged_pages.h).
+constexpr long long kEntriesFew = 4096;
 
 }  // namespace
 
@@ -199,7 +200,7 @@ int aoto_hip_paged_release(const int32_t* keep_lens, const int32_t* block_tables
   a.free_pages = free_pages, a.free_start = free_start, a.page_counts_out = page_counts_out;
   a.free_start_out = free_start_out, a.error = error, a.table_stride = table_stride, a.requests = requests;
   a.max_blocks = max_blocks, a.free_count = free_count, a.pages = pages, a.page = page, a.scratch = scratch;
-  if (pages <= kPagesFew && (long long)requests * max_blocks <= kReleaseFew)
+  if (pages <= kPagesFew && (long long)requests * max_blocks <= kEntriesFew)
     return launch("aoto_paged_release_few", 1, 1, 1024, stream, a);
   const int chunks = (pages - 1) / kPageChunk + 1;
   if (int s = launch("aoto_paged_drop", requests, 1, 256, stream, a)) return s;
@@ -223,6 +224,8 @@ int aoto_hip_paged_compact(int32_t* block_tables, int64_t table_stride, const in
   a.free_start = free_start, a.source = source, a.target = target, a.count = count, a.state = state, a.error = error;
   a.table_stride = table_stride, a.requests = requests, a.max_blocks = max_blocks, a.free_count = free_count;
   a.pages = pages;
+  if (pages <= kPagesFew && (long long)requests * max_blocks <= kEntriesFew && free_count <= kEntriesFew)
+    return launch("aoto_paged_compact_few", 1, 1, 1024, stream, a);
   if (int s = launch("aoto_paged_clear", (pages + 255LL) / 256, 1, 256, stream, a)) return s;
   a.list_blocks = (int)std::min(256LL, std::max(1LL, (free_count + 255LL) / 256));
   if (int s = launch("aoto_paged_mark", (long long)requests + a.list_blocks, 1, 256, stream, a)) return s;

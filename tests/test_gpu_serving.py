@@ -735,9 +735,25 @@ def test_compact_of_large_pools(pages):
     _check_compact(*_pool(rng, lens, 1, spare=pages - int(lens.sum()), share=0.3))
 
 
-def test_compact_of_lists_that_are_wrong():
+@pytest.mark.parametrize("pages", [1, 4095, 4096, 4097])
+def test_compact_in_one_launch_and_in_four(pages):
+    rng = np.random.default_rng(pages)
+    for requests, most in ((1, pages), (40, pages // 60), (4, pages // 5)):
+        lens = rng.integers(0, most + 1, requests)
+        state = _pool(rng, lens, 1, spare=pages - int(lens.sum()), share=0.4, blocks=max(1, 4096 // requests))
+        with _ops().recording_launches() as take:
+            _check_compact(*state, given=requests == 4)
+            assert take()[0] == "aoto_paged_" + ("compact_few" if pages <= 4096 else "clear")
+    tables, counts, shares, free, start = state
+    with _ops().recording_launches() as take:     # a list longer than the pool
+        _check_compact(tables, counts, shares, np.concatenate([np.full(5000, -1, np.int32), free]), start + 5000)
+        assert take()[0] == "aoto_paged_clear"
+
+
+@pytest.mark.parametrize("spare", [20, 5000])     # one launch, four
+def test_compact_of_lists_that_are_wrong(spare):
     rng = np.random.default_rng(9)
-    tables, counts, shares, free, start = _pool(rng, [60, 60, 30], 16)
+    tables, counts, shares, free, start = _pool(rng, [60, 60, 30], 16, spare=spare)
     free[-1], free[-2], free[-3] = free[-4], -1, tables[0, 0]  # twice, none, held
     tables[1, 1] = 10 ** 6
     assert _check_compact(tables, counts, shares, free, start)[6] == 128
