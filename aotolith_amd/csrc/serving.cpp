@@ -37,6 +37,31 @@ int check_cache(const char* what, const aoto_mx4_cache* c, int page, int kv_head
   return AOTO_OK;
 }
 
+// An array of an entry point on pages. Those that are written have the one input that they may be, at the same address.
+struct Array {
+  const void* at;
+  long long bytes;
+  const void* with = nullptr;
+};
+template <size_t N, size_t M>
+bool overlap(const Array (&written)[N], const Array (&read)[M]) {
+  auto meet = [](const Array& a, const Array& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    return a.at && b.at && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+  };
+  for (size_t i = 0; i < N; ++i) {
+    for (const Array& b : read)
+      if (meet(written[i], b) && !(written[i].at == b.at && b.at == written[i].with)) return true;
+    for (size_t j = 0; j < i; ++j)
+      if (meet(written[i], written[j])) return true;
+  }
+  return false;
+}
+// The bytes of block tables from the first entry to the last.
+long long table_bytes(int requests, int max_blocks, int64_t stride) {
+  return 4 * ((requests - 1LL) * stride + max_blocks);
+}
+
 // GPU blocks of the attention's narrow tiles of 16 rows that a CU holds. A tile's rows are a quarter of what they are
 // in bf16, so that two do not ask for enough at a time (345000 keys of 64 requests, 8 kv heads of 128: 88 us with two,
 // 84 with three, 93 with four, whose registers are too few).
@@ -170,6 +195,14 @@ int aoto_hip_paged_fork(const int32_t* parents, const int32_t* context_lens, int
     return set_error(AOTO_ERR_ARGUMENT, "paged_fork: bad shape");
   if (max_blocks > (1 << 20) || page > (1 << 20) || requests > (1 << 28))
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_fork: at most 2^20 blocks a request and tokens a page");
+  // what is written is read by other threads than those that read the inputs
+  const long long row = 4LL * requests;
+  const Array written[] = {{context_lens_out, row, context_lens}, {page_counts_out, row, page_counts},
+                           {free_start_out, 4, free_start}, {source, row}, {target, row}, {plan, 2 * row}};
+  const Array read[] = {{parents, row}, {context_lens, row}, {page_counts, row}, {free_start, 4}, {error, 4},
+                        {block_tables, table_bytes(requests, max_blocks, table_stride)}, {shares, 4LL * pages},
+                        {free_pages, 4LL * free_count}};
+  if (overlap(written, read)) return set_error(AOTO_ERR_ARGUMENT, "paged_fork: its outputs overlap other arrays");
   PagedForkArgs a{};
   a.parents = parents, a.context_lens = context_lens, a.block_tables = block_tables, a.page_counts = page_counts;
   a.shares = shares, a.free_pages = free_pages, a.free_start = free_start, a.context_lens_out = context_lens_out;
@@ -219,6 +252,11 @@ int aoto_hip_paged_compact(int32_t* block_tables, int64_t table_stride, const in
     return set_error(AOTO_ERR_ARGUMENT, "paged_compact: bad shape");
   if (max_blocks > (1 << 20) || pages > (1 << 30) || requests > (1 << 28))
     return set_error(AOTO_ERR_UNSUPPORTED, "paged_compact: at most 2^20 blocks a request, 2^30 pages");
+  const long long all = 4LL * pages;
+  const Array written[] = {{source, all}, {target, all}, {count, 4}, {state, all}};
+  const Array read[] = {{page_counts, 4LL * requests}, {free_start, 4}, {error, 4}, {shares, all},
+                        {block_tables, table_bytes(requests, max_blocks, table_stride)}, {free_pages, 4LL * free_count}};
+  if (overlap(written, read)) return set_error(AOTO_ERR_ARGUMENT, "paged_compact: its outputs overlap other arrays");
   PagedCompactArgs a{};
   a.block_tables = block_tables, a.page_counts = page_counts, a.shares = shares, a.free_pages = free_pages;
   a.free_start = free_start, a.source = source, a.target = target, a.count = count, a.state = state, a.error = error;

@@ -1887,7 +1887,7 @@ def paged_fork(
     in ``shares``. A page in progress becomes the next one of ``free_pages[free_start:]``, rows in order, and its
     content is to be copied: ``source``, ``target`` for :func:`paged_copy` on every layer's cache. Other rows stay.
     ``block_tables`` and ``shares`` are changed in place; lengths, counts and the list's start are in the result, whose
-    tensors ``step`` may give, also as the ones passed in. ``error`` (int32 ``[1]``) collects ``PAGED_ROW_HELD`` (the
+    tensors ``step`` may give: these three also as the ones passed in, else in memory of their own. ``error`` (int32 ``[1]``) collects ``PAGED_ROW_HELD`` (the
     row holds pages: left as it is), ``PAGED_BAD_ROW`` (no such parent: the same) and ``PAGED_NO_PAGES`` (the free list
     ran out: the row ends with its last full page).
     """
@@ -1990,7 +1990,8 @@ def paged_compact(
     ascending order, held pages past the first ``m`` of them go, in order, to free ones among the first ``m``. The
     tables and ``shares`` are changed to the new numbers in place; the free list keeps its place and holds the rest,
     ascending (so the pool's highest numbers are free ones). Pages neither held nor free stay what they are. The
-    contents are :func:`paged_copy`'s, on every layer's cache, with the result's ``source``, ``target`` and ``count``.
+    contents are :func:`paged_copy`'s, on every layer's cache, with the result's ``source``, ``target`` and ``count``
+    (tensors that ``moves`` may give, in memory of their own).
     ``error`` (int32 ``[1]``) collects ``PAGED_BAD_SHARE``: a page both held and free, or a list that names a page twice
     or none.
     """

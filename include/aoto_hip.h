@@ -728,8 +728,8 @@ int aoto_hip_paged_attention_mx4(const void* q, int64_t q_token_stride, int64_t 
  *
  * shares[page] (int32 [pages]) is a page's holders beyond the first: block table rows that name it within their
  * page_counts. aoto_hip_paged_tables takes pages of 0 from the free list free_pages[free_start .. free_count). Outputs
- * named *_out may be the arrays they are computed from. Everything is the same at every run, whatever the threads'
- * order. */
+ * named *_out may be the arrays they are computed from; else outputs overlap no other array (aoto_hip_paged_fork and
+ * _compact refuse it). Everything is the same at every run, whatever the threads' order. */
 
 /* Requests that go on from another: row r with parents[r] >= 0, which must hold no pages, gets the first
  * ceil(n / page) pages of row parents[r], n = min(context_lens, page_counts * page) of that row as it was before the

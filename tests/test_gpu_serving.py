@@ -1363,3 +1363,26 @@ def test_adjusted_rows_that_overlap_are_refused(monkeypatch, compiled):
         ops.adjust_logits(one.expand(3, 50), out=one.expand(3, 50))
     assert torch.equal(ops.adjust_logits(one.expand(3, 50)), torch.zeros((3, 50), device="cuda"))
     assert torch.equal(ops.adjust_logits(one, out=one.expand(1, 50)), one)
+
+
+# ---------------------------------------------------------------- arrays given twice
+def test_outputs_on_pages_that_overlap_other_arrays_are_refused():
+    ops = _ops()
+    parents, lens, tables, counts = _i32([-1, 0]), _i32([20, 0]), _i32([[1, 2], [0, 0]]), _i32([2, 0])
+    shares, free, start = _i32([0] * 4), _i32([0, 3]), _i32([0])
+    pages = (tables, counts, shares, free, start)
+    new = lambda n=2: _i32([0] * n)  # noqa: E731
+    for step in (ops.PagedFork(lens, counts, start, parents, new()), ops.PagedFork(parents, counts, start, new(), new()),
+                 ops.PagedFork(counts, lens, start, new(), new()), ops.PagedFork(lens, counts, start, free, new()),
+                 ops.PagedFork(lens, (x := new(3))[:2], start, x[1:], new())):
+        with pytest.raises(ops._lib.HipKernelError, match="overlap"):
+            ops.paged_fork(parents, lens, *pages, page_size=16, step=step)
+    whole = new(9)   # neighbours do not overlap
+    step = ops.PagedFork(whole[:2], whole[2:4], whole[4:5], whole[5:7], whole[7:])
+    assert ops.paged_fork(parents, lens, *pages, page_size=16, step=step) is step
+    assert whole.tolist() == [20, 20, 2, 2, 1, -1, 2, -1, 0] and shares.tolist() == [0, 1, 0, 0]
+    for moves in (ops.PagedMoves(x := new(4), x, new(1)), ops.PagedMoves(shares, new(4), new(1)),
+                  ops.PagedMoves(new(4), shares, new(1)), ops.PagedMoves(new(4), new(4), start)):
+        with pytest.raises(ops._lib.HipKernelError, match="overlap"):
+            ops.paged_compact(*pages, moves=moves)
+    assert shares.tolist() == [0, 1, 0, 0] and start.tolist() == [0]

@@ -146,6 +146,42 @@ def test_compact_refuses(changes, code):
     _refused(_compact(**changes), code, "paged_compact")
 
 
+def _apart(call, names, **changes):
+    """`call` with arrays of 64 KB each, apart from each other."""
+
+    at = {name: 2 ** 20 + 2 ** 16 * i for i, name in enumerate(names)}
+    at |= {name: at[x] if x in at else x for name, x in changes.items()}
+    return call(**{name: ctypes.c_void_p(x) if name in names else x for name, x in at.items()})
+
+
+FORK_IN = ("parents", "lens", "tables", "counts", "shares", "free", "start")
+FORK_OUT = ("lens_out", "counts_out", "start_out", "source", "target", "plan")
+
+
+@pytest.mark.parametrize("out,other", [(a, b) for a in FORK_OUT for b in FORK_IN + FORK_OUT
+                                       if a not in (b, b + "_out")])
+def test_fork_refuses_outputs_that_overlap_other_arrays(out, other):
+    # a parent's number read after a page's was written there would be a row of no table
+    _refused(_apart(_fork, FORK_IN + FORK_OUT, **{out: other}), 1, "overlap")
+
+
+@pytest.mark.parametrize("changes", [
+    dict(source=2 ** 20 + 2 * 2 ** 16 + 4 * 31), dict(target=2 ** 20 + 4 * 2 ** 16 + 4 * 49),
+    dict(lens_out=2 ** 20 + 2 ** 16 - 12), dict(counts_out=2 ** 20 + 12 * 2 ** 16 + 28)])
+def test_fork_refuses_outputs_that_overlap_other_arrays_in_part(changes):
+    # the last table entry, the last share, all but the first length, the last entry of the plan
+    _refused(_apart(_fork, FORK_IN + FORK_OUT, **changes), 1, "overlap")
+
+
+COMPACT_IN = ("tables", "counts", "shares", "free", "start")
+COMPACT_OUT = ("source", "target", "moved", "state")
+
+
+@pytest.mark.parametrize("out,other", [(a, b) for a in COMPACT_OUT for b in COMPACT_IN + COMPACT_OUT if a != b])
+def test_compact_refuses_outputs_that_overlap_other_arrays(out, other):
+    _refused(_apart(_compact, COMPACT_IN + COMPACT_OUT, **{out: other}), 1, "overlap")
+
+
 def _copy(tensor=None, **changes):
     t = dict(data=4096, planes=2, plane_stride=4096, page_stride=64, page_bytes=64) | (tensor or {})
     a = dict(tensors=_lib.PAGE_TENSOR.pack(*(0 if x is None else x for x in t.values())), count=1, pages=4,
