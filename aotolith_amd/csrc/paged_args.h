@@ -153,6 +153,7 @@ struct PagedReleaseArgs {
   int* error;
   long long table_stride;
   int requests, max_blocks, free_count, pages, page;
+  int list_blocks;  // of aoto_paged_drop, that go over the free list
 };
 
 struct PagedCompactArgs {

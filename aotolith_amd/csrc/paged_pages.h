@@ -168,11 +168,29 @@ AOTO_DEVICE int pages_held(const PagedReleaseArgs& a, int held) { return min(max
 AOTO_DEVICE int pages_kept(const PagedReleaseArgs& a, int count, int keep) {
   return keep < 0 ? count : min(count, (int)(((unsigned)keep + (unsigned)a.page - 1) / (unsigned)a.page));
 }
+// While a pool's pages are given back, what stands in `shares` of a page of the free list has kPageMark added, once for
+// each of its entries. A page's shares and the holders that go are below 2^27, so that the upper four bits tell the
+// mark; the lower ones are the shares that are left, -1 where nobody holds the page.
+constexpr int kPageMark = 1 << 28;
+AOTO_DEVICE int page_mark(int v) { return ((unsigned)v + kPageMark / 2) >> 28; }
+AOTO_DEVICE int page_share(int v) { return (int)((unsigned)v << 4) >> 4; }
+AOTO_DEVICE bool page_gone(int v) { return page_share(v) < 0 && !page_mark(v); }
 }  // namespace aoto
 
-// Requests' pages past what they keep lose a holder each; a page without one stands at -1 until aoto_paged_reclaim.
+// Requests' pages past what they keep lose a holder each, and pages of the free list are marked: additions, in any
+// order, from which aoto::page_mark and page_share tell both. Blocks 0 .. requests - 1: a row of the tables each; the
+// others: the free list.
 extern "C" __global__ __launch_bounds__(256) void aoto_paged_drop(PagedReleaseArgs a) {
-  const int r = blockIdx.x, held = a.page_counts[r], keep = a.keep_lens[r];
+  const int r = blockIdx.x;
+  if (r >= a.requests) {
+    const int first = min(max(a.free_start[0], 0), a.free_count);
+    for (long long j = first + (r - a.requests) * 256LL + threadIdx.x; j < a.free_count; j += a.list_blocks * 256LL) {
+      const int page = a.free_pages[j];
+      if ((unsigned)page < (unsigned)a.pages) atomicAdd(a.shares + page, aoto::kPageMark);
+    }
+    return;
+  }
+  const int held = a.page_counts[r], keep = a.keep_lens[r];
   const int count = aoto::pages_held(a, held), stays = aoto::pages_kept(a, count, keep);
   __syncthreads();  // the counts written may be the counts read
   if (threadIdx.x == 0) a.page_counts_out[r] = keep < 0 ? held : stays;
@@ -185,7 +203,8 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_drop(PagedReleaseAr
 
 // The pages left without a holder, in the order of their numbers, to the places before the free list's first: their
 // number in each 1024 pages, then their places. (In one launch a block would have to read the whole pool for its own
-// place, at a single CU's 20 GB/s: 15 us for 41000 pages instead of 2.2 + 2.8 us.)
+// place, at a single CU's 20 GB/s: 15 us for 41000 pages instead of 2.2 + 2.8 us.) A page that the list holds already
+// was given back more often than held and is not entered again.
 extern "C" __global__ __launch_bounds__(256) void aoto_paged_gone(PagedReleaseArgs a) {
   using namespace aoto;
   __shared__ int s_count[4];
@@ -193,7 +212,7 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_gone(PagedReleaseAr
   const PageFour share = page_four(a.shares, kPageChunk * chunk + 4 * threadIdx.x, a.pages);
   int count = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) count += __popcll(__ballot(share.v[e] < 0));
+  for (int e = 0; e < 4; ++e) count += __popcll(__ballot(page_gone(share.v[e])));
   if ((threadIdx.x & 63) == 0) s_count[wave] = count;
   __syncthreads();
   if (threadIdx.x != 0) return;
@@ -216,7 +235,7 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_reclaim(PagedReleas
   const unsigned long long below = (1ull << lane) - 1;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const unsigned long long lanes = __ballot(share.v[e] < 0);
+    const unsigned long long lanes = __ballot(page_gone(share.v[e]));
     count += __popcll(lanes), rank += __popcll(lanes & below);
   }
   if (lane == 0) s_count[wave] = count, s_before[wave] = before;
@@ -227,14 +246,16 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_reclaim(PagedReleas
   for (int w = 0; w < 4; ++w) rank += w < wave ? s_count[w] : 0, total += s_count[w];
   int error = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (share.v[e] < 0) {
+  for (int e = 0; e < 4; ++e) {
+    const int left = page_share(share.v[e]), now = max(left, 0);
+    if (now != share.v[e]) a.shares[from + e] = now;
+    if (left < -1 || (left < 0 && page_mark(share.v[e]))) error |= AOTO_PAGED_BAD_SHARE;
+    if (page_gone(share.v[e])) {
       const int at = first - 1 - before - rank++;
-      if (share.v[e] < -1) error |= AOTO_PAGED_BAD_SHARE;
-      a.shares[from + e] = 0;
       if (at >= 0) a.free_pages[at] = from + e;
       else error |= AOTO_PAGED_LIST_FULL;
     }
+  }
   if (error && a.error) atomicOr(a.error, error);
   if (tid == 0 && chunk == (a.pages - 1) / kPageChunk) a.free_start_out[0] = total ? max(0, first - total) : start;
 }
@@ -245,7 +266,8 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_reclaim(PagedReleas
 // and 6.5, 4096 and 5000 7.6 and 6.3, 8192 and 10000 11.0 and 6.6.
 extern "C" __global__ __launch_bounds__(1024) void aoto_paged_release_few(PagedReleaseArgs a) {
   using namespace aoto;
-  __shared__ int s_gone[kPagesFew];
+  constexpr uint32_t LISTED = 0x80000000u;
+  __shared__ uint32_t s_gone[kPagesFew];  // of each page: the holders that go, and whether the free list holds it
   __shared__ int s_scratch[kPageRanks];
   const int tid = threadIdx.x;
   const int start = a.free_start[0], first = min(max(start, 0), a.free_count);
@@ -254,8 +276,12 @@ extern "C" __global__ __launch_bounds__(1024) void aoto_paged_release_few(PagedR
   each_entry(a.block_tables, a.table_stride, a.requests, a.max_blocks, [&](int r, int j, int page) {
     const int count = pages_held(a, a.page_counts[r]);
     if (j < count && j >= pages_kept(a, count, a.keep_lens[r]) && (unsigned)page < (unsigned)a.pages)
-      atomicAdd(&s_gone[page], 1);
+      atomicAdd(&s_gone[page], 1u);
   });
+  for (int j = first + tid; j < a.free_count; j += 1024) {
+    const int page = a.free_pages[j];
+    if ((unsigned)page < (unsigned)a.pages) atomicOr(&s_gone[page], LISTED);
+  }
   __syncthreads();  // also: the counts written may be the counts read
   for (int r = tid; r < a.requests; r += 1024) {
     const int held = a.page_counts[r], keep = a.keep_lens[r];
@@ -271,11 +297,13 @@ extern "C" __global__ __launch_bounds__(1024) void aoto_paged_release_few(PagedR
   }
 #pragma unroll
   for (int i = 0; i < kPageSteps; ++i) {
-    const int page = 1024 * i + tid, gone = page < a.pages ? s_gone[page] : 0;
+    const int page = 1024 * i + tid;
+    const uint32_t of = page < a.pages ? s_gone[page] : 0;
+    const int gone = (int)(of & ~LISTED);
     left[i] -= gone;
-    none |= (uint32_t)(left[i] < 0) << i;
+    none |= (uint32_t)(left[i] < 0 && !(of & LISTED)) << i;
     if (gone || left[i] < 0) a.shares[page] = max(left[i], 0);
-    if (left[i] < -1) error |= AOTO_PAGED_BAD_SHARE;
+    if (left[i] < -1 || (left[i] < 0 && of & LISTED)) error |= AOTO_PAGED_BAD_SHARE;
   }
   page_ranks(none, rank, total, s_scratch);
 #pragma unroll

@@ -233,10 +233,11 @@ int aoto_hip_paged_release(const int32_t* keep_lens, const int32_t* block_tables
   a.free_pages = free_pages, a.free_start = free_start, a.page_counts_out = page_counts_out;
   a.free_start_out = free_start_out, a.error = error, a.table_stride = table_stride, a.requests = requests;
   a.max_blocks = max_blocks, a.free_count = free_count, a.pages = pages, a.page = page, a.scratch = scratch;
-  if (pages <= kPagesFew && (long long)requests * max_blocks <= kEntriesFew)
+  if (pages <= kPagesFew && (long long)requests * max_blocks <= kEntriesFew && free_count <= kEntriesFew)
     return launch("aoto_paged_release_few", 1, 1, 1024, stream, a);
   const int chunks = (pages - 1) / kPageChunk + 1;
-  if (int s = launch("aoto_paged_drop", requests, 1, 256, stream, a)) return s;
+  a.list_blocks = (int)std::min(256LL, std::max(1LL, (free_count + 255LL) / 256));
+  if (int s = launch("aoto_paged_drop", (long long)requests + a.list_blocks, 1, 256, stream, a)) return s;
   if (int s = launch("aoto_paged_gone", chunks, 1, 256, stream, a)) return s;
   return launch("aoto_paged_reclaim", chunks, 1, 256, stream, a);
 }

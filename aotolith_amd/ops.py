@@ -1942,8 +1942,9 @@ def paged_release(
     The others lose a holder each, and those left without one go to the places of ``free_pages`` before ``free_start``,
     downwards from it in ascending order of their numbers. ``shares`` and ``free_pages`` are changed in place, entries
     of ``block_tables`` past the new counts stay what they were; ``out`` gives the tensors of the result, which may be
-    the ones passed in. ``error`` (int32 ``[1]``) collects ``PAGED_BAD_SHARE`` (a page given back more often than held)
-    and ``PAGED_LIST_FULL`` (no place before the list's first: the page is lost).
+    the ones passed in. ``error`` (int32 ``[1]``) collects ``PAGED_BAD_SHARE`` (a page given back more often than held, in
+    this call or by one before: what ``free_pages[free_start:]`` holds already is not entered again) and
+    ``PAGED_LIST_FULL`` (no place before the list's first: the page is lost).
     """
 
     if out is None:

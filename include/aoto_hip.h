@@ -745,8 +745,9 @@ int aoto_hip_paged_fork(const int32_t* parents, const int32_t* context_lens, int
 
 /* Pages given back: row r keeps the first ceil(keep_lens[r] / page) of its page_counts[r] pages (all with
  * keep_lens[r] < 0); the others lose a holder each, entries of block_tables stay as they are. Pages left without one go
- * to free_pages[free_start - 1], [free_start - 2], ... in ascending order of their numbers. scratch: pages / 1024 + 2
- * entries. */
+ * to free_pages[free_start - 1], [free_start - 2], ... in ascending order of their numbers, but for those that
+ * free_pages[free_start .. free_count) holds (given back before: AOTO_PAGED_BAD_SHARE). shares are below 2^27. scratch:
+ * pages / 1024 + 2 entries. */
 int aoto_hip_paged_release(const int32_t* keep_lens, const int32_t* block_tables, int64_t table_stride,
                            const int32_t* page_counts, int32_t* shares, int32_t* free_pages,
                            const int32_t* free_start, int requests, int max_blocks, int free_count, int pages,

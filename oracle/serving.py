@@ -99,6 +99,10 @@ def release(keep, tables, counts, shares, free, start, page):
                 holders[entry] -= 1
         counts_out[r] = stays
     at, error = min(max(int(start), 0), len(free)), 0
+    listed = np.isin(np.arange(len(holders)), free[at:])
+    if (listed & (holders <= 0)).any():               # given back before
+        error |= 128
+        holders[listed & (holders <= 0)] = 1
     gone = np.nonzero(holders <= 0)[0]
     for p in gone:
         error |= 128 if holders[p] < 0 else 0

@@ -1365,6 +1365,50 @@ def test_adjusted_rows_that_overlap_are_refused(monkeypatch, compiled):
     assert torch.equal(ops.adjust_logits(one, out=one.expand(1, 50)), one)
 
 
+# ---------------------------------------------------------------- pages given back again
+@pytest.mark.parametrize("spare", [20, 5000, 60000])   # one launch, three
+@pytest.mark.parametrize("share", [0.0, 0.6])
+def test_release_of_what_was_given_back_before(spare, share):
+    """A second call with the counts of before the first: nothing is entered twice, and the error says so."""
+
+    rng = np.random.default_rng(spare + int(share))
+    tables, counts, shares, free, start = _pool(rng, [60, 200, 30, 111, 64], 16, spare=spare, share=share)
+    keep = np.array([0, 40, 0, -1, 16])
+    first = _check_release(keep, tables, counts, shares, free, start, 16)
+    assert first[4] == 0 and len(set(first[2][first[1][0]:])) == len(first[2]) - first[1][0]
+    again = _check_release(keep, tables, counts, first[3], first[2], first[1], 16, in_place=share > 0)
+    assert again[4] == 128
+    assert len(set(again[2][again[1][0]:])) == len(again[2]) - again[1][0]
+    # beside pages that do go
+    keep = np.array([0, 40, 0, 0, 16])
+    again = _check_release(keep, tables, counts, first[3], first[2], first[1], 16)
+    assert again[4] == 128 and (again[1] < first[1]).all()
+    # without room before the list
+    _check_release(keep, tables, counts, first[3], first[2][first[1][0]:], np.array([0], np.int32), 16)
+
+
+@pytest.mark.parametrize("spare", [20, 5000])
+def test_release_beside_lists_that_are_wrong(spare):
+    rng = np.random.default_rng(10)
+    tables, counts, shares, free, start = _pool(rng, [60, 60, 30], 16, spare=spare)
+    free[-1], free[-2], free[-3], free[-4], free[-5] = free[-6], -1, tables[0, 0], 10 ** 6, tables[2, 0]  # twice, none, held
+    assert _check_release([17, 0, -1], tables, counts, shares, free, start, 16)[4] == 0     # those that go are not there
+    assert _check_release([0, 0, -1], tables, counts, shares, free, start, 16)[4] == 128
+    shares[tables[1, 2]] = -3                          # too few holders, before
+    assert _check_release([-1, -1, -1], tables, counts, shares, free, start, 16)[4] == 128
+    free = np.concatenate([free, np.full(14, tables[0, 1], np.int32)])   # a held page many times
+    assert _check_release([0, 0, -1], tables, counts, shares, free, start, 16)[4] == 128
+
+
+def test_release_with_a_list_longer_than_the_pool():
+    rng = np.random.default_rng(11)
+    tables, counts, shares, free, start = _pool(rng, [60, 60, 30], 16)
+    free = np.concatenate([free, np.full(5000, -1, np.int32)])
+    with _ops().recording_launches() as take:
+        _check_release([0, 20, -1], tables, counts, shares, free, start, 16)
+        assert take()[0] == "aoto_paged_drop"
+
+
 # ---------------------------------------------------------------- arrays given twice
 def test_outputs_on_pages_that_overlap_other_arrays_are_refused():
     ops = _ops()

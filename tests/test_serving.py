@@ -302,6 +302,16 @@ def test_pages_of_the_restatement():
     assert shares.tolist() == [1, 0, 1, 0, 0, 0, 0, 0] and free.tolist() == [3, 4, 5, 6, 7]
 
 
+def test_pages_of_the_restatement_are_given_back_once():
+    tables, shares, free = np.array([[4, 2], [4, 1]], np.int32), np.array([0, 0, 0, 0, 1], np.int32), np.zeros(4, np.int32)
+    free[3] = 3
+    first = oracle.release([0, 0], tables, [2, 2], shares, free, 3, 16)
+    assert first[2].tolist() == [4, 2, 1, 3] and first[1].tolist() == [0] and first[4] == 0
+    again = oracle.release([0, -1], tables, [2, 2], first[3], first[2], 0, 16)   # the counts of before
+    assert again[2].tolist() == [4, 2, 1, 3] and again[1].tolist() == [0] and again[4] == 128
+    assert again[3].tolist() == [0] * 5
+
+
 def test_adjustments_of_the_restatement():
     z = np.array([[2.0, -2.0, 1.0, 0.5, 0.0, 3.0]] * 2)
     out, _, written = oracle.adjust(
