@@ -131,7 +131,9 @@ struct PagedForkArgs {
   int* free_start_out;
   int* source;
   int* target;
-  int* plan;   // two entries a request: full pages taken over (-1: none is asked for), its length
+  // Two entries a request: the full pages that it takes over, -1 where it stays as it is, -2 - j where it gets entry j
+  // of its own; its length.
+  int* plan;
   int* error;
   long long table_stride;
   int requests, max_blocks, free_count, pages, page;

@@ -88,12 +88,14 @@ AOTO_DEVICE void each_entry(const int* tables, long long stride, int requests, i
 
 }  // namespace aoto
 
-// Which rows go on from which, the pages taken for them and what is to be copied (formulas at the entry point's
-// declaration). One block: everything hangs on a running sum over the requests. Where `fill` is set it also enters the
-// full pages, which aoto_paged_share does otherwise.
+// Which rows go on from which, which of the others end inside a page that is not theirs alone, the pages taken for them
+// and what is to be copied (formulas at the entry point's declaration). One block: everything hangs on a running sum
+// over the requests. Where `fill` is set it also enters the full pages, which aoto_paged_share does otherwise.
 extern "C" __global__ __launch_bounds__(1024) void aoto_paged_fork(PagedForkArgs a, int fill) {
   using namespace aoto;
   __shared__ long long s_scan[16];
+  __shared__ int s_ends[1024];   // the shared page that a row of this pass ends in, -1 without
+  __shared__ int s_spare[1024];  // the free list's next
   __shared__ int s_error;
   const int tid = threadIdx.x;
   if (tid == 0) s_error = 0;
@@ -103,46 +105,62 @@ extern "C" __global__ __launch_bounds__(1024) void aoto_paged_fork(PagedForkArgs
   int error = 0;
   __syncthreads();
   for (int base = 0; base < a.requests; base += 1024) {
-    const int r = base + tid;
-    int parent = -1, full = -1, length = 0;
-    if (r < a.requests) {
-      parent = a.parents[r];
-      const bool empty = a.page_counts[r] <= 0;
-      if (parent >= a.requests) error |= AOTO_PAGED_BAD_ROW, parent = -1;
-      if (parent >= 0 && !empty) error |= AOTO_PAGED_ROW_HELD, parent = -1;
-      if (parent >= 0) {
-        const int count = min(max(a.page_counts[parent], 0), a.max_blocks);
-        length = (int)min((long long)max(a.context_lens[parent], 0), (long long)count * a.page);
-        full = length / a.page;
-      }
-    }
-    const bool part = full >= 0 && length > full * a.page;
+    const int r = base + tid, mine = min(r, a.requests - 1);
+    // asked for together: the row as one that stays, and the pages that this pass may take
+    int parent = a.parents[mine], count = a.page_counts[mine], length = a.context_lens[mine];
+    const long long next = first_free + taken + tid;
+    const int spare = next < a.free_count ? a.free_pages[next] : -1;
+    if (r >= a.requests) parent = -1, count = 0;
+    if (parent >= a.requests) error |= AOTO_PAGED_BAD_ROW, parent = -1;
+    if (parent >= 0 && count > 0) error |= AOTO_PAGED_ROW_HELD, parent = -1;
+    const int of = parent >= 0 ? parent : mine;
+    if (parent >= 0) count = a.page_counts[parent], length = a.context_lens[parent];
+    count = min(max(count, 0), a.max_blocks);
+    length = (int)min((long long)max(length, 0), (long long)count * a.page);
+    const int full = length / a.page;
+    const int page = length > full * a.page ? a.block_tables[(size_t)of * a.table_stride + full] : -1;
+    // Holders of the page that a row which stays ends in, beside it. What the passes before took from them is not in the
+    // first cache (whose load is 1 us sooner).
+    int others = 0;
+    if (parent < 0 && (unsigned)page < (unsigned)a.pages)
+      others = base ? __hip_atomic_load(a.shares + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : a.shares[page];
+    s_spare[tid] = spare, s_ends[tid] = others > 0 ? page : -1;
+    __syncthreads();
+    if (others > 0)
+      for (int i = 0; i < tid; ++i) others -= s_ends[i] == page;  // those of rows before are gone
+    const bool leaves = others > 0, part = leaves || (parent >= 0 && length > full * a.page);
     long long total = 0;
-    const long long at = first_free + taken + block_scan_1024(part ? 1 : 0, s_scan, total) - 1;
+    const int at = (int)block_scan_1024(part ? 1 : 0, s_scan, total) - 1;
     if (r < a.requests) {
-      int source = -1, target = -1;
+      int source = -1, target = -1, plan = parent >= 0 ? full : -1;
       if (part) {
-        if (at < a.free_count) {
-          source = a.block_tables[(size_t)parent * a.table_stride + full];
-          target = a.free_pages[at];
-          a.block_tables[(size_t)r * a.table_stride + full] = target;
-        } else {
-          error |= AOTO_PAGED_NO_PAGES;
-          length = full * a.page;
+        const bool some = first_free + taken + at < a.free_count;
+        if (some) source = page, target = s_spare[at];
+        if (!some) error |= AOTO_PAGED_NO_PAGES, length = full * a.page;
+        if (leaves) {
+          if ((unsigned)target < (unsigned)a.pages) {
+            plan = -2 - full;
+            if (atomicSub(a.shares + page, 1) <= 0) error |= AOTO_PAGED_BAD_SHARE;
+          } else {
+            source = target = -1, error |= AOTO_PAGED_NO_PAGES | AOTO_PAGED_ROW_SHARED;
+          }
         }
       }
       a.source[r] = source, a.target[r] = target;
-      a.plan[2 * r] = full, a.plan[2 * r + 1] = length;
+      a.plan[2 * r] = plan, a.plan[2 * r + 1] = length;
     }
     taken += total;
+    if (base + 1024 < a.requests) __syncthreads();  // s_spare and s_ends are read
   }
   if (error) atomicOr(&s_error, error);
   __syncthreads();
   // only now: a row may be the parent of another, and the outputs may be the inputs
   for (int r = tid; r < a.requests; r += 1024) {
     const int full = a.plan[2 * r], length = a.plan[2 * r + 1];
+    const bool part = full >= 0 && length > full * a.page;
+    if (part || full < -1) a.block_tables[(size_t)r * a.table_stride + (part ? full : -2 - full)] = a.target[r];
     a.context_lens_out[r] = full >= 0 ? length : a.context_lens[r];
-    a.page_counts_out[r] = full >= 0 ? full + (length > full * a.page ? 1 : 0) : a.page_counts[r];
+    a.page_counts_out[r] = full >= 0 ? full + (part ? 1 : 0) : a.page_counts[r];
   }
   if (fill)
     for (int k = tid; k < a.requests * a.max_blocks; k += 1024) {

@@ -1828,7 +1828,7 @@ def paged_attention_mx4(
 # block table rows that name it within their page counts. :func:`paged_tables` takes pages that nobody shares.
 
 #: More bits of the ``error`` tensor, raised by the functions below (``AOTO_PAGED_*`` in ``include/aoto_hip.h``).
-PAGED_ROW_HELD, PAGED_BAD_ROW, PAGED_BAD_SHARE, PAGED_LIST_FULL = 32, 64, 128, 256
+PAGED_ROW_HELD, PAGED_BAD_ROW, PAGED_BAD_SHARE, PAGED_LIST_FULL, PAGED_ROW_SHARED = 32, 64, 128, 256, 512
 
 
 class PagedFork(NamedTuple):
@@ -1885,11 +1885,15 @@ def paged_fork(
     Row ``r`` with ``parents[r] >= 0`` (int32 ``[R]``) must hold no pages; it gets the cached tokens of row
     ``parents[r]`` as that was before the call. Full pages are shared: entered in its row of ``block_tables``, one more
     in ``shares``. A page in progress becomes the next one of ``free_pages[free_start:]``, rows in order, and its
-    content is to be copied: ``source``, ``target`` for :func:`paged_copy` on every layer's cache. Other rows stay.
+    content is to be copied: ``source``, ``target`` for :func:`paged_copy` on every layer's cache. Other rows stay, but
+    for the page that one of ``context_lens[r]`` tokens has in progress: where others hold it too (:func:`paged_release`
+    cut the row there), the row gets a page of its own in its place, with the copy in ``source`` and ``target``, before
+    tokens that are appended would become the others'. (The last holder that ends there keeps the page.)
     ``block_tables`` and ``shares`` are changed in place; lengths, counts and the list's start are in the result, whose
     tensors ``step`` may give: these three also as the ones passed in, else in memory of their own. ``error`` (int32 ``[1]``) collects ``PAGED_ROW_HELD`` (the
-    row holds pages: left as it is), ``PAGED_BAD_ROW`` (no such parent: the same) and ``PAGED_NO_PAGES`` (the free list
-    ran out: the row ends with its last full page).
+    row holds pages: left as it is), ``PAGED_BAD_ROW`` (no such parent: the same), ``PAGED_NO_PAGES`` (the free list
+    ran out: the row ends with its last full page) and ``PAGED_ROW_SHARED`` (nor was there a page for a row that ends
+    inside another's: it is as it was and must not be appended to).
     """
 
     if step is None:
@@ -1945,6 +1949,10 @@ def paged_release(
     the ones passed in. ``error`` (int32 ``[1]``) collects ``PAGED_BAD_SHARE`` (a page given back more often than held, in
     this call or by one before: what ``free_pages[free_start:]`` holds already is not entered again) and
     ``PAGED_LIST_FULL`` (no place before the list's first: the page is lost).
+
+    A row that went on from another may be cut inside a page that it still shares. The next token's slot is in that
+    page, over the others' tokens: :func:`paged_fork` (with ``parents`` of -1 where no row goes on) and its copy come
+    before the step's :func:`paged_tables`, and give the row a page of its own.
     """
 
     if out is None:

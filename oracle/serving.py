@@ -55,18 +55,30 @@ def fork(parents, lens, tables, counts, shares, free, start, page):
     """``(lens, counts, start, source, target, tables, shares, error)``."""
 
     requests, blocks = tables.shape
-    before, tables, shares = tables, tables.copy(), shares.copy()
+    before, tables, left, shares = tables, tables.copy(), shares.copy(), shares.copy()
     lens_out, counts_out = np.array(lens, np.int32), np.array(counts, np.int32)
     source, target = np.full(requests, -1, np.int32), np.full(requests, -1, np.int32)
     at, taken, error = max(int(start), 0), False, 0
     for r, p in enumerate(parents):
-        if p < 0:
-            continue
-        if p >= requests or counts[r] > 0:
+        if p >= requests or (p >= 0 and counts[r] > 0):
             error |= 64 if p >= requests else 32
-            continue
-        n = min(max(int(lens[p]), 0), min(max(int(counts[p]), 0), blocks) * page)
+            p = -1
+        of = r if p < 0 else p
+        n = min(max(int(lens[of]), 0), min(max(int(counts[of]), 0), blocks) * page)
         full = n // page
+        if p < 0:
+            # a row that stays: its page in progress is to be its own
+            own = int(before[r, full]) if n % page else -1
+            if 0 <= own < len(shares) and left[own] > 0:
+                taken = True
+                if at < len(free) and 0 <= free[at] < len(shares):
+                    source[r], target[r], tables[r, full] = own, free[at], free[at]
+                    shares[own] -= 1
+                else:
+                    error |= 2 | 512
+                left[own] -= 1
+                at = min(at + 1, max(len(free), at))
+            continue
         tables[r, :full] = before[p, :full]
         for entry in before[p, :full]:
             if 0 <= entry < len(shares):

@@ -1409,6 +1409,115 @@ def test_release_with_a_list_longer_than_the_pool():
         assert take()[0] == "aoto_paged_drop"
 
 
+# ---------------------------------------------------------------- rows cut inside a page of others
+@pytest.mark.parametrize("page", [4, 16])
+@pytest.mark.parametrize("requests", [3, 70, 1024, 1025, 2500])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_fork_of_rows_that_end_inside_a_page_of_others(page, requests, in_place):
+    rng = np.random.default_rng(page + requests)
+    lens = rng.integers(page, 90, requests)
+    lens[rng.random(requests) < 0.3] = 0
+    lens[:3] = 70, 70, 0
+    tables, counts, shares, free, start = _pool(rng, lens, page, spare=2 * requests, share=0.7, blocks=40)
+    cut = np.where(rng.random(requests) < 0.6, rng.integers(0, lens + 1), lens)
+    cut[0], cut[1] = page + 1, page + 2
+    counts, start, free, shares, error = oracle.release(cut, tables, counts, shares, free, start[0], page)
+    assert error == 0
+    # rows of nothing go on from any, also from one that gets a page of its own
+    parents = np.where(counts == 0, rng.integers(-1, requests, requests), -1)
+    parents[rng.integers(3, requests + 1, 2) - 1] = requests
+    parents[2] = 1
+    want = _check_fork(parents, cut, tables, counts, shares, free, start, page, in_place)
+    own = (want[3] >= 0) & (parents < 0)
+    assert want[7] & ~(64 | 32) == 0 and (own.any() or requests == 3)
+    # nothing is left to do
+    again = _check_fork(np.full(requests, -1), want[0], want[5], want[1], want[6], free, want[2], page)
+    assert (again[3] == -1).all() and again[2] == want[2]
+
+
+@pytest.mark.parametrize("requests", [5, 1500])
+@pytest.mark.parametrize("others", [0, 1])
+def test_fork_of_many_rows_that_end_inside_one_page(requests, others):
+    """One of them keeps the page if nobody else holds it."""
+
+    tables = np.full((requests + 1, 3), -1, np.int32)
+    tables[:, :2] = [5, 3]
+    counts = np.full(requests + 1, 2, np.int32)
+    lens = np.full(requests + 1, 17 + 3)
+    lens[0], counts[0] = (32, 2) if others else (0, 0)
+    holders = requests + others
+    shares = np.zeros(requests + 20, np.int32)
+    shares[[5, 3]] = holders - 1
+    free = np.setdiff1d(np.arange(requests + 20), [5, 3]).astype(np.int32)
+    want = _check_fork(np.full(requests + 1, -1), lens, tables, counts, shares, free, np.array([0], np.int32), 16)
+    assert (want[3] == 3).sum() == requests - (not others) and want[6][3] == 0 and want[6][5] == holders - 1
+    assert want[7] == 0
+    # without pages for all of them
+    want = _check_fork(np.full(requests + 1, -1), lens, tables, counts, shares, free[:3], np.array([1], np.int32), 16)
+    assert want[7] == 2 | 512 and (want[3] == 3).sum() == 2
+
+
+def test_a_row_cut_inside_a_shared_page_leaves_the_others_tokens():
+    ops, rng = _ops(), np.random.default_rng(33)
+    page, dim, hkv, pool, rows = 16, 64, 2, 40, 3
+    cache = ops.paged_mx4_cache(pool, hkv, page, dim)
+    bf16 = [torch.zeros((pool, hkv, page, dim), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    error = torch.zeros(1, dtype=torch.int32, device="cuda")
+    tables, counts = torch.full((rows, 8), -1, dtype=torch.int32, device="cuda"), _i32([0] * rows)
+    shares, free, start = _i32([0] * pool), _i32(rng.permutation(pool)), _i32([0])
+    ones = torch.ones((128, dim), dtype=torch.bfloat16, device="cuda")
+    texts = [[] for _ in range(rows)]
+    context = [0] * rows
+
+    def step(new):
+        nonlocal counts, start
+        s = ops.paged_tables(_i32(context), _i32(new), tables, counts, free, start, page_size=page,
+                             max_tokens=sum(new), error=error)
+        counts, start = s.page_counts, s.free_start
+        x = bf16_normal(rng, (sum(new), 3 * hkv * dim))
+        args = (to_gpu_bf16(x), s.positions, s.slots, ones, torch.zeros_like(ones))
+        ops.paged_rope_append_mx4(*args, cache, query_heads=hkv, error=error)
+        ops.paged_rope_append(*args, *bf16, query_heads=hkv, error=error)
+        at = 0
+        for r in range(rows):
+            texts[r] += list(x[at: at + new[r]])
+            at, context[r] = at + new[r], context[r] + new[r]
+
+    def own_pages(parents):
+        nonlocal counts, start
+        fork = ops.paged_fork(_i32(parents), _i32(context), tables, counts, shares, free, start, page_size=page,
+                              error=error)
+        ops.paged_copy([*cache, *bf16], fork.source, fork.target, error=error)
+        counts, start, context[:] = fork.page_counts, fork.free_start, fork.context_lens.tolist()
+
+    def read_back():
+        values, table = _values([_np(t) for t in cache]), _np(tables)
+        for r in range(rows):
+            for j, x in enumerate(texts[r]):
+                k, v = x.astype(np.float64).reshape(-1, dim)[hkv:].reshape(2, hkv, dim)
+                at = (table[r, j // page], slice(None), j % page)
+                np.testing.assert_array_equal(values[0][at], oracle.mx4_unpack(*oracle.mx4_pack(k)))
+                np.testing.assert_array_equal(values[1][at], oracle.mx4_unpack(*oracle.mx4_pack(v)))
+                np.testing.assert_array_equal(from_gpu_bf16(bf16[0][at]), k)
+                np.testing.assert_array_equal(from_gpu_bf16(bf16[1][at]), v)
+        holders = np.bincount([p for r in range(rows) for p in table[r, : _np(counts)[r]]], minlength=pool)
+        np.testing.assert_array_equal(_np(shares), np.maximum(holders - 1, 0))
+
+    step([70, 3, 0])
+    own_pages([-1, -1, 0])
+    texts[2] = list(texts[0])
+    step([2, 1, 9])
+    context[2] = 20                                    # inside the second page, which row 0 has whole
+    del texts[2][20:]
+    counts, start = ops.paged_release(_i32([-1, -1, 20]), tables, counts, shares, free, start, page_size=page,
+                                      error=error)
+    own_pages([-1] * rows)
+    for new in ([1, 1, 1], [0, 2, 30], [3, 0, 1]):
+        step(new)
+        read_back()
+    assert int(error) == 0
+
+
 # ---------------------------------------------------------------- arrays given twice
 def test_outputs_on_pages_that_overlap_other_arrays_are_refused():
     ops = _ops()
