@@ -1391,8 +1391,8 @@ def test_release_of_what_was_given_back_before(spare, share):
 def test_release_beside_lists_that_are_wrong(spare):
     rng = np.random.default_rng(10)
     tables, counts, shares, free, start = _pool(rng, [60, 60, 30], 16, spare=spare)
-    free[-1], free[-2], free[-3], free[-4], free[-5] = free[-6], -1, tables[0, 0], 10 ** 6, tables[2, 0]  # twice, none, held
-    assert _check_release([17, 0, -1], tables, counts, shares, free, start, 16)[4] == 0     # those that go are not there
+    free[-5:] = tables[2, 0], 10 ** 6, tables[0, 0], -1, free[-6]                          # held, none, twice
+    assert _check_release([17, 0, -1], tables, counts, shares, free, start, 16)[4] == 0    # those that go are not there
     assert _check_release([0, 0, -1], tables, counts, shares, free, start, 16)[4] == 128
     shares[tables[1, 2]] = -3                          # too few holders, before
     assert _check_release([-1, -1, -1], tables, counts, shares, free, start, 16)[4] == 128
@@ -1518,6 +1518,102 @@ def test_a_row_cut_inside_a_shared_page_leaves_the_others_tokens():
     assert int(error) == 0
 
 
+@pytest.mark.parametrize("pages_before_the_pool_moves", [60, 5000])   # upkeep in one launch, in several
+def test_a_captured_step_keeps_every_rows_text(pages_before_the_pool_moves):
+    """Ends, cuts, forks, moves, appends and attention of a captured step, plan after plan: what a row reads through its
+    table is the text it was given, whoever shares its pages; the pages' holders and the free list add up."""
+
+    ops, rng = _ops(), np.random.default_rng(34)
+    hq, hkv, dim, page, rows, blocks, pool = 4, 2, 64, 16, 6, 12, pages_before_the_pool_moves
+    cache = ops.paged_mx4_cache(pool, hkv, page, dim)
+    d = dict(tables=torch.full((rows, blocks), -1, dtype=torch.int32, device="cuda"), free=_i32(rng.permutation(pool)),
+             shares=_i32([0] * pool),
+             qkv=torch.zeros((rows, (hq + 2 * hkv) * dim), dtype=torch.bfloat16, device="cuda"),
+             **{k: _i32([0] * rows) for k in ("counts", "lens", "new", "parents", "keep", "source", "target")},
+             **{k: _i32([0]) for k in ("start", "error")})
+    pages = [d[k] for k in ("tables", "counts", "shares", "free", "start")]
+    ones, zeros = (torch.full((blocks * page, dim), x, dtype=torch.bfloat16, device="cuda") for x in (1.0, 0.0))
+
+    def run():
+        e = d["error"]
+        ops.paged_release(d["keep"], *pages, page_size=page, out=(d["counts"], d["start"]), error=e)
+        fork = ops.paged_fork(d["parents"], d["lens"], *pages, page_size=page, error=e,
+                              step=ops.PagedFork(*(d[k] for k in ("lens", "counts", "start", "source", "target"))))
+        ops.paged_copy(cache, fork.source, fork.target, error=e)
+        moves = ops.paged_compact(*pages, error=e)
+        ops.paged_copy(cache, moves.source, moves.target, count=moves.count, error=e)
+        step = ops.paged_tables(d["lens"], d["new"], d["tables"], d["counts"], d["free"], d["start"], page_size=page,
+                                max_tokens=rows, error=e)
+        d["counts"].copy_(step.page_counts)
+        d["start"].copy_(step.free_start)
+        q = ops.paged_rope_append_mx4(d["qkv"], step.positions, step.slots, ones, zeros, cache, query_heads=hq, error=e)
+        out = ops.paged_attention_mx4(q, cache, d["tables"], step.query_start, step.kv_lens, max_query_len=1)
+        d["lens"].copy_(step.kv_lens)
+        return q, out, step.query_start, step.kv_lens
+
+    run()                                              # of no requests
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q, out, start, kv = run()
+    texts = [[] for _ in range(rows)]
+    for r, n in ((0, 70), (3, 33)):                     # prompts
+        x = bf16_normal(rng, (n, (hq + 2 * hkv) * dim))
+        s = ops.paged_tables(_i32([0] * rows), _i32([n if i == r else 0 for i in range(rows)]), d["tables"], d["counts"],
+                             d["free"], d["start"], page_size=page, max_tokens=n, error=d["error"])
+        ops.paged_rope_append_mx4(to_gpu_bf16(x), s.positions, s.slots, ones, zeros, cache, query_heads=hq)
+        d["counts"].copy_(s.page_counts)
+        d["start"].copy_(s.free_start)
+        texts[r] = list(x)
+    cuts = 0
+    for plan in range(24):
+        keep, parents = [-1] * rows, [-1] * rows
+        for r in range(rows):
+            if texts[r] and (rng.random() < 0.35 or len(texts[r]) > 120):
+                keep[r] = 0 if rng.random() < 0.4 and sum(map(bool, texts)) > 2 else int(rng.integers(1, len(texts[r])))
+                del texts[r][keep[r]:]
+        for r in range(rows):
+            if not texts[r] and rng.random() < 0.6:
+                parents[r] = int(rng.choice([p for p in range(rows) if texts[p] and parents[p] < 0]))
+                # from here on the parent's text, as it is before this step's token
+        given = {r: list(texts[p]) for r, p in enumerate(parents) if p >= 0}
+        lens = [len(t) for t in texts]
+        for r, text in given.items():
+            texts[r] = text
+        new = [int(bool(t)) for t in texts]
+        x = bf16_normal(rng, (rows, (hq + 2 * hkv) * dim))
+        for name, value in (("keep", keep), ("parents", parents), ("lens", lens), ("new", new)):
+            d[name].copy_(_i32(value))
+        d["qkv"].copy_(to_gpu_bf16(x))
+        graph.replay()
+        at = 0
+        for r in range(rows):
+            if new[r]:
+                texts[r].append(x[at])
+                at += 1
+        own = _np(d["source"])
+        cuts += sum(own[r] >= 0 and parents[r] < 0 for r in range(rows))
+        values, table, counts = _values([_np(t) for t in cache]), _np(d["tables"]), _np(d["counts"])
+        assert int(d["error"]) == 0 and _np(d["lens"]).tolist() == [len(t) for t in texts]
+        for r in range(rows):
+            if not texts[r]:
+                continue
+            heads = np.stack(texts[r]).astype(np.float64).reshape(len(texts[r]), -1, dim)
+            j = np.arange(len(texts[r]))
+            for got, part in ((values[0], heads[:, hq: hq + hkv]), (values[1], heads[:, hq + hkv:])):
+                want = oracle.mx4_unpack(*oracle.mx4_pack(part))
+                np.testing.assert_array_equal(got[table[r, j // page], :, j % page], want)
+        holders = np.bincount([p for r in range(rows) for p in table[r, : counts[r]]], minlength=pool)
+        np.testing.assert_array_equal(_np(d["shares"]), np.maximum(holders - 1, 0))
+        spare = _np(d["free"])[int(d["start"]):]
+        assert sorted([*spare, *np.nonzero(holders)[0]]) == list(range(pool))
+        state = dict(q=from_gpu_bf16(q)[:at], keys=values[0], values=values[1], tables=table, start=_np(start),
+                     kv=_np(kv))
+        want, size, written = paged_oracle.attention(*state.values())
+        got = from_gpu_bf16(out).astype(np.float64)[:at]
+        assert (np.abs(got - want) <= _bound(state, want, size))[written].all()
+    assert cuts > 0
+
+
 # ---------------------------------------------------------------- arrays given twice
 def test_outputs_on_pages_that_overlap_other_arrays_are_refused():
     ops = _ops()
@@ -1525,7 +1621,8 @@ def test_outputs_on_pages_that_overlap_other_arrays_are_refused():
     shares, free, start = _i32([0] * 4), _i32([0, 3]), _i32([0])
     pages = (tables, counts, shares, free, start)
     new = lambda n=2: _i32([0] * n)  # noqa: E731
-    for step in (ops.PagedFork(lens, counts, start, parents, new()), ops.PagedFork(parents, counts, start, new(), new()),
+    for step in (ops.PagedFork(lens, counts, start, parents, new()),
+                 ops.PagedFork(parents, counts, start, new(), new()),
                  ops.PagedFork(counts, lens, start, new(), new()), ops.PagedFork(lens, counts, start, free, new()),
                  ops.PagedFork(lens, (x := new(3))[:2], start, x[1:], new())):
         with pytest.raises(ops._lib.HipKernelError, match="overlap"):

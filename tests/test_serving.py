@@ -303,8 +303,8 @@ def test_pages_of_the_restatement():
 
 
 def test_pages_of_the_restatement_are_given_back_once():
-    tables, shares, free = np.array([[4, 2], [4, 1]], np.int32), np.array([0, 0, 0, 0, 1], np.int32), np.zeros(4, np.int32)
-    free[3] = 3
+    tables, shares = np.array([[4, 2], [4, 1]], np.int32), np.array([0, 0, 0, 0, 1], np.int32)
+    free = np.array([0, 0, 0, 3], np.int32)
     first = oracle.release([0, 0], tables, [2, 2], shares, free, 3, 16)
     assert first[2].tolist() == [4, 2, 1, 3] and first[1].tolist() == [0] and first[4] == 0
     again = oracle.release([0, -1], tables, [2, 2], first[3], first[2], 0, 16)   # the counts of before
@@ -316,16 +316,18 @@ def test_rows_of_the_restatement_that_end_inside_a_page_of_others():
     # rows 0, 1, 2 hold pages 4 and 7, row 0 also 2; 1 and 2 are cut inside 7
     tables, shares = np.array([[4, 7, 2], [4, 7, -1], [4, 7, -1]], np.int32), np.array([0] * 8, np.int32)
     shares[[4, 7]] = 2
-    counts, start, free, shares, error = oracle.release([-1, 20, 18], tables, [3, 2, 2], shares, np.array([1, 3, 5]), 0, 16)
+    free = np.array([1, 3, 5])
+    counts, start, free, shares, error = oracle.release([-1, 20, 18], tables, [3, 2, 2], shares, free, 0, 16)
     assert counts.tolist() == [3, 2, 2] and error == 0
     lens, counts, start, source, target, one, left, error = oracle.fork(
-        [-1] * 3, [40, 20, 18], tables, counts, shares, np.array([1, 3, 5]), 0, 16)
+        [-1] * 3, [40, 20, 18], tables, counts, shares, free, 0, 16)
     assert (source.tolist(), target.tolist(), start.tolist(), error) == ([-1, 7, 7], [-1, 1, 3], [2], 0)
     assert one.tolist() == [[4, 7, 2], [4, 1, -1], [4, 3, -1]] and left[[4, 7]].tolist() == [2, 0]
     # row 0 ends there too: the last of the three keeps the page; without free pages all stay as they are
     *_, source, target, one, left, error = oracle.fork([-1] * 3, [20, 20, 18], tables, counts, shares, free, 0, 16)
     assert (source.tolist(), one[:, 1].tolist(), left[7], error) == ([7, 7, -1], [1, 3, 7], 0, 0)
-    lens, _, start, source, _, one, left, error = oracle.fork([-1] * 3, [20, 20, 18], tables, counts, shares, free, 2, 16)
+    lens, _, start, source, _, one, left, error = oracle.fork(
+        [-1] * 3, [20, 20, 18], tables, counts, shares, free, 2, 16)
     assert (source.tolist(), one[:, 1].tolist(), left[7], error) == ([7, -1, -1], [5, 7, 7], 1, 512 + 2)
     assert lens.tolist() == [20, 20, 18] and start.tolist() == [3]
 
