@@ -1849,6 +1849,15 @@ class PagedMoves(NamedTuple):
     count: torch.Tensor   # int32 [1]
 
 
+def _page_size(page_size: int) -> int:
+    """For the C ABI's 32 bits, which ctypes cuts an integer to without a word."""
+
+    page_size = int(page_size)
+    if not -(2 ** 31) <= page_size < 2 ** 31:
+        raise ValueError(f"page_size is a number of 32 bits, got {page_size}")
+    return page_size
+
+
 def _expect_pool(block_tables, page_counts, shares, free_pages, free_start, error) -> tuple[int, int]:
     """The pool's tensors, as every function on pages takes them: ``(device, requests)``."""
 
@@ -1921,8 +1930,8 @@ def paged_fork(
         _lib.library().aoto_hip_paged_fork(
             _ptr(parents), _ptr(context_lens), _ptr(block_tables), block_tables.stride(0), _ptr(page_counts),
             _ptr(shares), _ptr(free_pages), _ptr(free_start), requests, block_tables.shape[1], free_pages.numel(),
-            shares.numel(), int(page_size), _ptr(step.context_lens), _ptr(step.page_counts), _ptr(step.free_start),
-            _ptr(step.source), _ptr(step.target), _ptr(plan), _ptr(error), _stream(device),
+            shares.numel(), _page_size(page_size), _ptr(step.context_lens), _ptr(step.page_counts),
+            _ptr(step.free_start), _ptr(step.source), _ptr(step.target), _ptr(plan), _ptr(error), _stream(device),
         )
     )
     return step
@@ -1977,7 +1986,7 @@ def paged_release(
         _lib.library().aoto_hip_paged_release(
             _ptr(keep_lens), _ptr(block_tables), block_tables.stride(0), _ptr(page_counts), _ptr(shares),
             _ptr(free_pages), _ptr(free_start), requests, block_tables.shape[1], free_pages.numel(), shares.numel(),
-            int(page_size), _ptr(counts_out), _ptr(start_out), _ptr(scratch), _ptr(error), _stream(device),
+            _page_size(page_size), _ptr(counts_out), _ptr(start_out), _ptr(scratch), _ptr(error), _stream(device),
         )
     )
     return counts_out, start_out

@@ -1636,3 +1636,15 @@ def test_outputs_on_pages_that_overlap_other_arrays_are_refused():
         with pytest.raises(ops._lib.HipKernelError, match="overlap"):
             ops.paged_compact(*pages, moves=moves)
     assert shares.tolist() == [0, 1, 0, 0] and start.tolist() == [0]
+
+
+@pytest.mark.parametrize("page_size", [2 ** 32 + 16, 2 ** 31, -(2 ** 32) + 16, 0, -16])
+def test_page_sizes_that_are_no_number_of_tokens_are_refused(page_size):
+    ops = _ops()
+    pages = _i32([[1, 2], [0, 0]]), _i32([2, 0]), _i32([0] * 4), _i32([-1, -1, 0, 3]), _i32([2])
+    want = [t.tolist() for t in pages]
+    for call in (lambda: ops.paged_fork(_i32([-1, 0]), _i32([20, 0]), *pages, page_size=page_size),
+                 lambda: ops.paged_release(_i32([0, 0]), *pages, page_size=page_size)):
+        with pytest.raises((ValueError, ops._lib.HipKernelError), match="page_size|bad shape"):
+            call()
+    assert [t.tolist() for t in pages] == want
