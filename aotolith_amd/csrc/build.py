@@ -19,6 +19,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+import warnings
 
 CSRC = os.path.dirname(os.path.abspath(__file__))
 PACKAGE = os.path.dirname(CSRC)
@@ -71,8 +72,16 @@ def _calls_command(output: str) -> list[str]:
             output, "-L" + libraries, "-ltorch_python", "-ltorch_cpu", "-lc10"]
 
 
+def _build_calls(output: str, verbose: bool) -> None:
+    _run(_calls_command(output), verbose)
+
+
 def build(verbose: bool = False) -> tuple[str, str]:
-    """Compile the code object, the host library and the Python calls; return the first two's paths."""
+    """Compile the code object, the host library and the Python calls; return the first two's paths.
+
+    The calls need a host compiler, Python's headers and torch's. Where those are missing the others are built all the
+    same, with a warning, and no calls of an earlier build stay.
+    """
 
     tmp_obj, tmp_lib, tmp_calls = CODE_OBJECT + ".tmp", LIBRARY + ".tmp", CALLS + ".tmp"
     commands = (
@@ -99,14 +108,20 @@ def build(verbose: bool = False) -> tuple[str, str]:
             "-o",
             tmp_lib,
         ],
-        _calls_command(tmp_calls),
     )
     with concurrent.futures.ThreadPoolExecutor() as pool:
+        calls = pool.submit(_build_calls, tmp_calls, verbose)
         for step in [pool.submit(_run, command, verbose) for command in commands]:
             step.result()
     os.replace(tmp_obj, CODE_OBJECT)
     os.replace(tmp_lib, LIBRARY)
-    os.replace(tmp_calls, CALLS)
+    try:
+        calls.result()
+        os.replace(tmp_calls, CALLS)
+    except (RuntimeError, OSError, ImportError) as error:
+        if os.path.exists(CALLS):
+            os.remove(CALLS)
+        warnings.warn(f"_calls.so is not built, ops.py makes the serving operators' calls itself: {error}")
     return CODE_OBJECT, LIBRARY
 
 

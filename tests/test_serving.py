@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from aotolith_amd import _lib, ops
+from aotolith_amd.csrc import build
 from oracle import serving as oracle
 
 GOOD = ctypes.c_void_p(4096)  # an address that no entry point may read: each refuses first
@@ -345,3 +346,43 @@ def test_adjustments_of_the_restatement():
 def test_structs_are_the_headers():
     # pointers, 64-bit strides, 32-bit counts and the room behind them, as the C ABI lays them out
     assert [x.size for x in (_lib.MX4_CACHE, _lib.PAGE_TENSOR, _lib.ADJUSTMENTS)] == [88, 40, 144]
+
+
+# ---------------------------------------------------------------- the compiled calls
+@pytest.mark.parametrize("failure", [RuntimeError("no Python.h"), FileNotFoundError("g++"), ImportError("torch"), None])
+def test_a_build_without_the_calls_keeps_the_rest(monkeypatch, tmp_path, failure):
+    paths = {name: tmp_path / name for name in ("CODE_OBJECT", "LIBRARY", "CALLS")}
+    for name, path in paths.items():
+        monkeypatch.setattr(build, name, str(path))
+        path.write_text("old")
+
+    def run(command, verbose):
+        if failure is not None and any("calls.cpp" in word for word in command):
+            raise failure
+        with open(command[command.index("-o") + 1], "w") as made:
+            made.write("new")
+
+    monkeypatch.setattr(build, "_run", run)
+    if failure is None:
+        build.build()
+    else:
+        with pytest.warns(UserWarning, match="_calls.so is not built"):
+            build.build()
+    assert {name: path.read_text() for name, path in paths.items() if path.exists()} == (
+        {name: "new" for name in paths if failure is None or name != "CALLS"})
+
+
+def test_a_build_that_fails_changes_nothing(monkeypatch, tmp_path):
+    paths = [tmp_path / name for name in ("CODE_OBJECT", "LIBRARY", "CALLS")]
+    for path in paths:
+        monkeypatch.setattr(build, path.name, str(path))
+        path.write_text("old")
+
+    def run(command, verbose):
+        if any("kernels.hip" in word for word in command):
+            raise RuntimeError("build step failed")
+
+    monkeypatch.setattr(build, "_run", run)
+    with pytest.raises(RuntimeError, match="build step failed"):
+        build.build()
+    assert [path.read_text() for path in paths] == ["old"] * 3
