@@ -61,6 +61,14 @@ def _run(command: list[str], verbose: bool) -> None:
         raise RuntimeError(f"build step failed ({result.returncode}): {' '.join(command)}")
 
 
+def calls_built_for() -> str:
+    """The torch and Python whose objects ``calls.cpp`` reaches into: a build for others is not to be used."""
+
+    import torch
+
+    return f"torch {torch.__version__} {torch.version.git_version}, {sys.implementation.cache_tag}"
+
+
 def _calls_command(output: str) -> list[str]:
     import torch
     from torch.utils import cpp_extension
@@ -68,8 +76,9 @@ def _calls_command(output: str) -> list[str]:
     libraries = os.path.join(os.path.dirname(torch.__file__), "lib")
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-I" + INCLUDE,
             "-I" + sysconfig.get_paths()["include"], *("-I" + path for path in cpp_extension.include_paths()),
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", os.path.join(CSRC, "calls.cpp"), "-o",
-            output, "-L" + libraries, "-ltorch_python", "-ltorch_cpu", "-lc10"]
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            f'-DAOTO_BUILT_FOR="{calls_built_for()}"', os.path.join(CSRC, "calls.cpp"), "-o", output,
+            "-L" + libraries, "-ltorch_python", "-ltorch_cpu", "-lc10"]
 
 
 def _build_calls(output: str, verbose: bool) -> None:

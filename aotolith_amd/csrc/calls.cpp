@@ -523,4 +523,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nul
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls() { return PyModule_Create(&module); }
+// built_for: the torch and Python of the headers; with others nothing here but this may be called.
+PyMODINIT_FUNC PyInit__calls() {
+  PyObject* calls = PyModule_Create(&module);
+  if (calls && PyModule_AddStringConstant(calls, "built_for", AOTO_BUILT_FOR) < 0) Py_CLEAR(calls);
+  return calls;
+}

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import warnings
 from typing import NamedTuple
 
 import torch
@@ -1567,6 +1568,10 @@ class _Unbound:
         return lambda *args: None
 
 
+class _Refused(_Unbound):
+    """The same in place of a build that is not to be bound."""
+
+
 _calls = _Unbound()
 
 #: The entry points ``_calls`` is given, in its order.
@@ -1584,6 +1589,13 @@ def _bind_calls() -> None:
     try:
         from . import _calls as module
     except ImportError:
+        return
+    from .csrc.build import calls_built_for
+
+    if getattr(module, "built_for", None) != calls_built_for():  # the layout of its tensors may be another
+        warnings.warn("_calls.so is of another build of torch or Python, the calls are made without it: build it with "
+                      "`python -m aotolith_amd.csrc.build`")
+        _calls = _Refused()
         return
     lib = _lib.library()
     entries = (ctypes.cast(getattr(lib, "aoto_hip_" + name), ctypes.c_void_p).value for name in _CALLED)

@@ -5,11 +5,14 @@ from __future__ import annotations
 
 import ctypes
 import math
+import sys
+import warnings
 
 import numpy as np
 import pytest
 import torch
 
+import aotolith_amd
 from aotolith_amd import _lib, ops
 from aotolith_amd.csrc import build
 from oracle import serving as oracle
@@ -386,3 +389,40 @@ def test_a_build_that_fails_changes_nothing(monkeypatch, tmp_path):
     with pytest.raises(RuntimeError, match="build step failed"):
         build.build()
     assert [path.read_text() for path in paths] == ["old"] * 3
+
+
+class _Calls:
+    def __init__(self, built_for):
+        if built_for is not None:
+            self.built_for = built_for
+
+    def bind(self, *args):
+        raise AssertionError("bound")
+
+
+@pytest.mark.parametrize("built_for", [None, "", "torch 2.9.1 0123456, cpython-310"])
+def test_calls_that_were_built_for_another_torch_are_not_bound(monkeypatch, built_for):
+    monkeypatch.setattr(aotolith_amd, "_calls", _Calls(built_for), raising=False)
+    monkeypatch.setitem(sys.modules, "aotolith_amd._calls", aotolith_amd._calls)
+    monkeypatch.setattr(ops, "_calls", ops._Unbound())
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: 0)
+    with pytest.warns(UserWarning, match="another build of torch"):
+        ops._bind_calls()
+    assert ops._calls.paged_unpack_mx4(None) is None
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")   # once
+        ops._bind_calls()
+
+
+def test_calls_that_were_built_for_this_torch_are_bound(monkeypatch):
+    monkeypatch.setattr(aotolith_amd, "_calls", _Calls(build.calls_built_for()), raising=False)
+    monkeypatch.setitem(sys.modules, "aotolith_amd._calls", aotolith_amd._calls)
+    monkeypatch.setattr(ops, "_calls", ops._Unbound())
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: 0)
+    with pytest.raises(AssertionError, match="bound"):
+        ops._bind_calls()
+
+
+def test_the_built_calls_say_what_they_were_built_for():
+    calls = pytest.importorskip("aotolith_amd._calls")
+    assert calls.built_for == build.calls_built_for()
