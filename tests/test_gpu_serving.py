@@ -450,6 +450,55 @@ def test_attention_of_q_of_every_size(rows):
     _check(s, _attend(s, scale=2.0 ** 100), scale=2.0 ** 100)
 
 
+def _nearer_bound(s, want, size):
+    """As :func:`_bound`, from each key's own products: scores off by up to e_j change weights p_j by up to m_j =
+    exp(e_j) - 1 of themselves, their sum by M = sum p_j m_j, the result by sum p_j m_j (|v_j| + |want|) / (1 - M)."""
+
+    tokens, heads, dim = s["q"].shape
+    hkv, page = s["keys"].shape[1:3]
+    want = want.reshape(tokens, heads, dim)
+    more = np.zeros_like(want)
+    for r, length in enumerate(s["kv"]):
+        first, last = s["start"][r], s["start"][r + 1]
+        at = (s["tables"][r, np.arange(length) // page], slice(None), np.arange(length) % page)
+        k, v = s["keys"][at], s["values"][at]
+        for t in range(first, last):
+            n = length - (last - first) + (t - first) + 1
+            for h in range(heads):
+                products = s["q"][t, h].astype(np.float64) * k[:n, h * hkv // heads]
+                score = dim ** -0.5 * products.sum(-1)
+                p = np.exp(score - score.max())
+                p /= p.sum()
+                off = dim ** -0.5 * 8 * 2.0 ** -13 * (1 + 2.0 ** -5) * np.abs(products).reshape(n, -1, 8).max(-1).sum(-1)
+                pm = p * np.expm1(off)
+                assert pm.sum() < 0.5
+                more[t, h] = (pm @ np.abs(v[:n, h * hkv // heads]) + pm.sum() * np.abs(want[t, h])) / (1 - pm.sum())
+    want = want.reshape(tokens, -1)
+    return attention_bound(want, size) + more.reshape(tokens, -1)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [2, 40])               # narrow tiles, wide ones
+@pytest.mark.parametrize("sharp,large", [(4.0, 0), (16.0, 0), (1.0, 30), (4.0, 30)])
+def test_attention_of_sharp_heads_and_of_large_dims(dim, rows, sharp, large):
+    """Heads whose weight is a few keys', and a dim that is large in every key and row, as some models have it."""
+
+    rng = np.random.default_rng(int(sharp) + large)
+    s = _requests(rng, [(rows, 500), (rows, 90)], 8, 2, dim, 16)
+    keys = rng.standard_normal(s["keys"].shape)
+    s["q"] *= sharp
+    if large:
+        keys[..., 5], s["q"][..., 5] = large, large
+    s["q"] = from_gpu_bf16(to_gpu_bf16(s["q"]))
+    s["host"][0], s["host"][2] = oracle.mx4_pack(keys)
+    _put(s)
+    want, size, _ = paged_oracle.attention(s["q"], s["keys"], s["values"], s["tables"], s["start"], s["kv"])
+    got = from_gpu_bf16(_attend(s, max_query_len=rows)).astype(np.float64)
+    # scores of up to 1000 in f32: 1000 * 2^-23 of their weights each way
+    bound = _nearer_bound(s, want, size) + 3e-4 * (size + np.abs(want))
+    assert (np.abs(got - want) <= bound).all()
+
+
 @pytest.mark.parametrize("rows", [1, 20])
 def test_attention_past_32_bits_of_cache(rows):
     # 2^32 bytes of codes and more before the pages in use
