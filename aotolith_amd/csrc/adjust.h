@@ -26,10 +26,11 @@
 //   f32, 72 rows x 128256                        24.2      19.9      23.6
 //   f32, 203 rows x 128256, masks                59.1      54.5
 //   f32, 256 requests' one row, texts of 4000    91.3     100.0
-// 108 MB of the sixth at 3.9 TB/s, of three times as many requests at 4.7. Blocks of 4096 and more tokens gain for
-// texts as long as a quarter of the vocabulary only (bf16, 8 rows x 128256, texts of 32000: 17.2 us with 2048, 12.2
-// with 4096), 16 tokens of a text on their way instead of 8 for none (30.5 us for the sixth: registers, and with them
-// waves).
+// 108 MB of the sixth at 3.9 TB/s, of three times as many requests at 4.7. The rule goes by rows and vocabulary, which
+// the host knows; history_len is only the room for texts, so the last line, whose time is its texts', loses by the rule.
+// Blocks of 4096 and more tokens gain for texts as long as a quarter of the vocabulary only (bf16, 8 rows x 128256,
+// texts of 32000: 17.2 us with 2048, 12.2 with 4096), 16 tokens of a text on their way instead of 8 for none (30.5 us
+// for the sixth: registers, and with them waves).
 #pragma once
 
 #include "common.h"

@@ -30,8 +30,8 @@ AOTO_DEVICE uint32_t mx4_pack(const float (&x)[8], float scale) {
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], scale, 3);
 }
 
-// Eight codes as bf16, which holds every value but those below its least (scale bytes below 4): exact. NaN for a scale
-// byte of 255.
+// Eight codes as bf16, exactly: the least of them but 0, 2^-127 / 2, is a subnormal number of bf16 (2^-133 and its
+// multiples). NaN for a scale byte of 255.
 AOTO_DEVICE uint4 mx4_unpack(uint32_t codes, float scale) {
   uint4 v;
   v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));

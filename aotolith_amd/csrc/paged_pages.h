@@ -90,7 +90,9 @@ AOTO_DEVICE void each_entry(const int* tables, long long stride, int requests, i
 
 // Which rows go on from which, which of the others end inside a page that is not theirs alone, the pages taken for them
 // and what is to be copied (formulas at the entry point's declaration). One block: everything hangs on a running sum
-// over the requests. Where `fill` is set it also enters the full pages, which aoto_paged_share does otherwise.
+// over the requests. Where `fill` is set it also enters the full pages, which aoto_paged_share does otherwise. Bound by
+// round trips: a row, the row that it goes on from, the page in progress, its holders, the writes (8 rows 4.3 us, 900
+// and the second launch 8.2).
 extern "C" __global__ __launch_bounds__(1024) void aoto_paged_fork(PagedForkArgs a, int fill) {
   using namespace aoto;
   __shared__ long long s_scan[16];
@@ -119,11 +121,12 @@ extern "C" __global__ __launch_bounds__(1024) void aoto_paged_fork(PagedForkArgs
     length = (int)min((long long)max(length, 0), (long long)count * a.page);
     const int full = length / a.page;
     const int page = length > full * a.page ? a.block_tables[(size_t)of * a.table_stride + full] : -1;
-    // Holders of the page that a row which stays ends in, beside it. What the passes before took from them is not in the
-    // first cache (whose load is 1 us sooner).
+    // Holders of the page that a row which stays ends in, beside it. What the passes before took from them is past the
+    // first cache.
     int others = 0;
     if (parent < 0 && (unsigned)page < (unsigned)a.pages)
-      others = base ? __hip_atomic_load(a.shares + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : a.shares[page];
+      others = base ? __hip_atomic_load(a.shares + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                    : a.shares[page];
     s_spare[tid] = spare, s_ends[tid] = others > 0 ? page : -1;
     __syncthreads();
     if (others > 0)
@@ -221,7 +224,7 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_drop(PagedReleaseAr
 
 // The pages left without a holder, in the order of their numbers, to the places before the free list's first: their
 // number in each 1024 pages, then their places. (In one launch a block would have to read the whole pool for its own
-// place, at a single CU's 20 GB/s: 15 us for 41000 pages instead of 2.2 + 2.8 us.) A page that the list holds already
+// place, at a single CU's 20 GB/s: 15 us for 41000 pages instead of 2.2 + 2.8.) A page that the list holds already
 // was given back more often than held and is not entered again.
 extern "C" __global__ __launch_bounds__(256) void aoto_paged_gone(PagedReleaseArgs a) {
   using namespace aoto;
@@ -280,8 +283,9 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_reclaim(PagedReleas
 
 // All of it by one block, which counts the holders that go in LDS: pools of up to kPagesFew pages. What bounds it is
 // one CU's reading, so it gains by its two launches fewer (2 to 3 us each where they are not captured) and only as long
-// as the GPU is hardly slower: 512 entries of tables and 600 pages 5.6 us and 5.7 in three launches, 2048 and 2500 6.6
-// and 6.5, 4096 and 5000 7.6 and 6.3, 8192 and 10000 11.0 and 6.6.
+// as the GPU is hardly slower. In a graph, for entries of tables and pages of the pool: 512 and 600 5.5 us, 5.7 in three
+// launches, 2048 and 2500 6.7 and 6.3, 4096 and 4000 7.7 and 6.1; in an instance for 8192 pages 8192 and 8000 9.8 and
+// 6.6.
 extern "C" __global__ __launch_bounds__(1024) void aoto_paged_release_few(PagedReleaseArgs a) {
   using namespace aoto;
   constexpr uint32_t LISTED = 0x80000000u;
@@ -459,8 +463,8 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_remap(PagedCompactA
 }
 
 // All of it by one block, with the pages' states in LDS: pools of up to kPagesFew pages. As in aoto_paged_release_few,
-// the gain is three launches: 512 entries of tables and 600 pages 9.8 us and 11.5 in four, 2048 and 2500 11.4 and 11.7,
-// 4096 and 5000 12.9 and 12.4, 8192 and 10000 19.3 and 16.8.
+// the gain is three launches: 512 entries of tables and 600 pages 9.5 us and 11.0 in four, 2048 and 2500 11.1 and 11.4,
+// 4096 and 4000 12.5 and 11.9; in an instance for 8192 pages 8192 and 8000 15.8 and 12.9.
 extern "C" __global__ __launch_bounds__(1024) void aoto_paged_compact_few(PagedCompactArgs a) {
   using namespace aoto;
   __shared__ int s_state[kPagesFew];

@@ -37,18 +37,30 @@ int check_cache(const char* what, const aoto_mx4_cache* c, int page, int kv_head
   return AOTO_OK;
 }
 
-// An array of an entry point on pages. Those that are written have the one input that they may be, at the same address.
+// An array of an entry point on pages: `rows` of `bytes` each, `stride` bytes apart. Those that are written are one row
+// and have the one input that they may be, at the same address.
 struct Array {
   const void* at;
   long long bytes;
   const void* with = nullptr;
+  long long rows = 1, stride = 1;
 };
+Array table_array(const int32_t* tables, int requests, int max_blocks, int64_t stride) {
+  return {tables, 4LL * max_blocks, nullptr, requests, 4 * stride};
+}
+// Whether one row meets any of another array's.
+bool meet(const Array& one, const Array& other) {
+  if (!one.at || !other.at) return false;
+  long long from = (long long)(reinterpret_cast<uintptr_t>(one.at) - reinterpret_cast<uintptr_t>(other.at));
+  const long long to = from + one.bytes;
+  from = std::max(from, 0LL);
+  // the last row that begins before `from` ends behind it, or the next one begins before `to`
+  const long long row = std::min(from / other.stride, other.rows - 1);
+  return from < to && (from < row * other.stride + other.bytes ||
+                       (row + 1 < other.rows && (row + 1) * other.stride < to));
+}
 template <size_t N, size_t M>
 bool overlap(const Array (&written)[N], const Array (&read)[M]) {
-  auto meet = [](const Array& a, const Array& b) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
-    return a.at && b.at && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
-  };
   for (size_t i = 0; i < N; ++i) {
     for (const Array& b : read)
       if (meet(written[i], b) && !(written[i].at == b.at && b.at == written[i].with)) return true;
@@ -57,10 +69,6 @@ bool overlap(const Array (&written)[N], const Array (&read)[M]) {
   }
   return false;
 }
-// The bytes of block tables from the first entry to the last.
-long long table_bytes(int requests, int max_blocks, int64_t stride) {
-  return 4 * ((requests - 1LL) * stride + max_blocks);
-}
 
 // GPU blocks of the attention's narrow tiles of 16 rows that a CU holds. A tile's rows are a quarter of what they are
 // in bf16, so that two do not ask for enough at a time (345000 keys of 64 requests, 8 kv heads of 128: 88 us with two,
@@ -68,7 +76,7 @@ long long table_bytes(int requests, int max_blocks, int64_t stride) {
 constexpr int kMx4NarrowBlocks = 3;
 
 // Entries of all block tables up to which the fork's one block enters the pages itself instead of a second launch (8 x
-// 64 entries 3.9 us and 5.5 with two launches, 32 x 64 4.8 and 5.6, 64 x 64 6.5 and 5.5, 64 x 256 17.1 and 5.7).
+// 64 entries 4.2 us and 6.1 with two launches, 32 x 64 5.5 and 6.0, 64 x 64 7.7 and 6.4, 64 x 256 16.4 and 6.7).
 constexpr long long kForkFill = 2048;
 
 // Entries of all block tables (and of the free list) up to which one block releases the pages of a pool of up to
@@ -168,8 +176,9 @@ int aoto_hip_paged_attention_mx4(const void* q, int64_t q_token_stride, int64_t 
   aoto::attention_launch(plan, max_blocks, workspace, a);
   // Tiles not cut, a chunk's longest first, two GPU blocks a CU: the second ones shortest first, so that a CU's two are
   // as long together as another's (one request of 32 / 8 heads of 128: 2048 tokens over 6000 keys 236 -> 229 us, 4096
-  // over themselves 160 -> 149; 14 / 2 of 64, 4096 over 2000: 120 -> 121). What comes after them goes to whoever ends
-  // first.
+  // over themselves 160 -> 149; 14 / 2 of 64, both sides in turn, five calls after a pause: 4096 over 2000 134.9 ->
+  // 134.3, 8192 over themselves 228.0 -> 219.9, three of 2000 62.7 -> 61.6; 32 / 8 of 64, 2048 over 6000: 207 -> 202).
+  // What comes after them goes to whoever ends first.
   if (!plan.target && plan.wide_rows) {
     args.turn_from = std::max(1, aoto::device_cu_count() / kv_heads);
     args.turn_to = (int)std::min(plan.units, 2LL * args.turn_from);
@@ -200,8 +209,8 @@ int aoto_hip_paged_fork(const int32_t* parents, const int32_t* context_lens, int
   const Array written[] = {{context_lens_out, row, context_lens}, {page_counts_out, row, page_counts},
                            {free_start_out, 4, free_start}, {source, row}, {target, row}, {plan, 2 * row}};
   const Array read[] = {{parents, row}, {context_lens, row}, {page_counts, row}, {free_start, 4}, {error, 4},
-                        {block_tables, table_bytes(requests, max_blocks, table_stride)}, {shares, 4LL * pages},
-                        {free_pages, 4LL * free_count}};
+                        {shares, 4LL * pages}, {free_pages, 4LL * free_count},
+                        table_array(block_tables, requests, max_blocks, table_stride)};
   if (overlap(written, read)) return set_error(AOTO_ERR_ARGUMENT, "paged_fork: its outputs overlap other arrays");
   PagedForkArgs a{};
   a.parents = parents, a.context_lens = context_lens, a.block_tables = block_tables, a.page_counts = page_counts;
@@ -256,7 +265,7 @@ int aoto_hip_paged_compact(int32_t* block_tables, int64_t table_stride, const in
   const long long all = 4LL * pages;
   const Array written[] = {{source, all}, {target, all}, {count, 4}, {state, all}};
   const Array read[] = {{page_counts, 4LL * requests}, {free_start, 4}, {error, 4}, {shares, all},
-                        {block_tables, table_bytes(requests, max_blocks, table_stride)}, {free_pages, 4LL * free_count}};
+                        {free_pages, 4LL * free_count}, table_array(block_tables, requests, max_blocks, table_stride)};
   if (overlap(written, read)) return set_error(AOTO_ERR_ARGUMENT, "paged_compact: its outputs overlap other arrays");
   PagedCompactArgs a{};
   a.block_tables = block_tables, a.page_counts = page_counts, a.shares = shares, a.free_pages = free_pages;
@@ -334,7 +343,7 @@ int aoto_hip_adjust_logits(const void* logits, int logits_f32, int64_t row_strid
   a.value_stride = j.value_stride, a.allowed_stride = 4 * j.allowed_stride;
   a.rows = rows, a.requests = requests, a.vocab = vocab, a.history_len = j.history_len, a.drafts = j.drafts;
   a.biases = j.biases;
-  // tokens a thread, by the logits that there are room for (adjust.h)
+  // tokens a thread, by the logits that there are room for; how long the texts are is known on the GPU alone (adjust.h)
   const long long most = (long long)rows * vocab;
   const int per = most <= 1 << 21 ? 2 : logits_f32 || most <= 1 << 23 ? 4 : 8, threads = per == 2 ? 512 : 256;
   char name[64];

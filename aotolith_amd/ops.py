@@ -1784,7 +1784,8 @@ def paged_attention_mx4(
     :func:`paged_attention_mx4_workspace`). A NaN group of a key that a row sees, a NaN or an infinity in its q make
     the row NaN; a NaN group of a value makes those 32 dims NaN, however small its weight. Requests of more than 32 rows
     a kv head multiply K as it is in the cache by q as two 8-bit numbers (exactly q to 2^-22 of the largest of each 32
-    dims), in sums that keep 13 bits below the largest of each eight products.
+    dims), in sums that keep 13 bits below the largest of each eight products. Scores are of magnitudes below 2^29: past
+    it the exponentials lose their reference, which is held in f32.
     """
 
     made = _calls.paged_attention_mx4(q, cache, block_tables, query_start, kv_lens, causal, scale, max_query_len,

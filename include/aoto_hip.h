@@ -707,7 +707,7 @@ int aoto_hip_paged_rope_append_mx4(const void* qkv, int64_t row_stride, const in
                                    const aoto_mx4_cache* cache, int page, int tokens, int query_heads, int kv_heads,
                                    int head_dim, void* q_out, int32_t* error, void* stream);
 
-/* What a whole cache stands for, bf16 [pages][kv_heads][page][head_dim] twice (exact but below 2^-133). */
+/* What a whole cache stands for, bf16 [pages][kv_heads][page][head_dim] twice, exactly. */
 int aoto_hip_paged_unpack_mx4(const aoto_mx4_cache* cache, int page, int kv_heads, int head_dim, void* keys_out,
                               void* values_out, void* stream);
 
@@ -736,11 +736,11 @@ int aoto_hip_paged_attention_mx4(const void* q, int64_t q_token_stride, int64_t 
  * ceil(n / page) pages of row parents[r], n = min(context_lens, page_counts * page) of that row as it was before the
  * call: full pages themselves (shares + 1), one in progress as the next page of the free list, rows in order, with
  * (source[r], target[r]) the pages to copy, -1 without. context_lens_out, page_counts_out and free_start_out follow;
- * without a free page (AOTO_PAGED_NO_PAGES) the row ends with its last full page. Rows with parents[r] < 0 stay, but for
- * the page that such a row, of n tokens as above, has in progress (n % page != 0): while others hold it, rows in order,
- * the row gets the next page of the free list in its place, with the copy in source and target too, and shares - 1 (the
- * last holder that ends there keeps it). Where no page is left for that the row stays as it is (AOTO_PAGED_NO_PAGES and
- * AOTO_PAGED_ROW_SHARED). plan: scratch of 2 * requests entries. */
+ * without a free page (AOTO_PAGED_NO_PAGES) the row ends with its last full page. Rows with parents[r] < 0 stay, but
+ * for the page that such a row, of n tokens as above, has in progress (n % page != 0): while others hold it, rows in
+ * order, the row gets the next page of the free list in its place, with the copy in source and target too, and
+ * shares - 1 (the last holder that ends there keeps it). Where no page is left for that the row stays as it is
+ * (AOTO_PAGED_NO_PAGES and AOTO_PAGED_ROW_SHARED). plan: scratch of 2 * requests entries. */
 int aoto_hip_paged_fork(const int32_t* parents, const int32_t* context_lens, int32_t* block_tables,
                         int64_t table_stride, const int32_t* page_counts, int32_t* shares, const int32_t* free_pages,
                         const int32_t* free_start, int requests, int max_blocks, int free_count, int pages, int page,
@@ -750,8 +750,8 @@ int aoto_hip_paged_fork(const int32_t* parents, const int32_t* context_lens, int
 /* Pages given back: row r keeps the first ceil(keep_lens[r] / page) of its page_counts[r] pages (all with
  * keep_lens[r] < 0); the others lose a holder each, entries of block_tables stay as they are. Pages left without one go
  * to free_pages[free_start - 1], [free_start - 2], ... in ascending order of their numbers, but for those that
- * free_pages[free_start .. free_count) holds (given back before: AOTO_PAGED_BAD_SHARE). A row may end inside a page that
- * others hold too, where the next token's slot would be theirs: aoto_hip_paged_fork, called before that token's
+ * free_pages[free_start .. free_count) holds (given back before: AOTO_PAGED_BAD_SHARE). A row may end inside a page
+ * that others hold too, where the next token's slot would be theirs: aoto_hip_paged_fork, called before that token's
  * aoto_hip_paged_tables, gives the row a page of its own. shares are below 2^27. scratch: pages / 1024 + 2 entries. */
 int aoto_hip_paged_release(const int32_t* keep_lens, const int32_t* block_tables, int64_t table_stride,
                            const int32_t* page_counts, int32_t* shares, int32_t* free_pages,

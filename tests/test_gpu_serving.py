@@ -427,6 +427,19 @@ def test_attention_of_nan_values_that_weigh_nothing(kernel, hq, hkv, dim, most, 
 
 @pytest.mark.parametrize("kernel,hq,hkv,dim,most,requests", FORMS)
 @pytest.mark.parametrize("cut", [False, True])
+def test_attention_of_scores_as_large_as_they_may_be(kernel, hq, hkv, dim, most, requests, cut):
+    # one key of up to 2^28 and the others far below: its value alone, weights of one key cancelling in the division
+    s, at = _peaked(np.random.default_rng(hq), kernel, hq, hkv, dim, most, requests)
+    s["q"] *= 2.0 ** 23
+    _put(s)
+    got = from_gpu_bf16(_form_attend(s, kernel, most, 1500, cut)).reshape(-1, hq, dim).astype(np.float64)
+    want = np.repeat(s["values"][at], hq // hkv, 0)
+    bad = ~(np.abs(got[s["start"][2]: s["start"][3]] - want) <= (HALF + 1e-4) * np.abs(want))
+    assert not bad.any()
+
+
+@pytest.mark.parametrize("kernel,hq,hkv,dim,most,requests", FORMS)
+@pytest.mark.parametrize("cut", [False, True])
 def test_attention_of_the_largest_values(kernel, hq, hkv, dim, most, requests, cut):
     # 6 * 2^113 in every value: a mean of such values is one, whatever the scores; 2^12 of them do not pass the range
     s = _form_requests(np.random.default_rng(hq), hq, hkv, dim, most, requests, 1500)
@@ -1680,6 +1693,13 @@ def test_outputs_on_pages_that_overlap_other_arrays_are_refused():
     step = ops.PagedFork(whole[:2], whole[2:4], whole[4:5], whole[5:7], whole[7:])
     assert ops.paged_fork(parents, lens, *pages, page_size=16, step=step) is step
     assert whole.tolist() == [20, 20, 2, 2, 1, -1, 2, -1, 0] and shares.tolist() == [0, 1, 0, 0]
+    # nor do other columns of the tables' rows
+    wide = torch.full((3, 12), -1, dtype=torch.int32, device="cuda")
+    wide[:2, :2], wide[:2, 2:] = _i32([[1, 2], [0, 0]]), 7
+    part = wide.view(-1)
+    step = ops.PagedFork(part[2:4], part[4:6], part[6:7], part[7:9], part[26:28])
+    ops.paged_fork(parents, lens, wide[:2, :2], counts, new(4), free, start, page_size=16, step=step)
+    assert wide.tolist() == [[1, 2, 20, 20, 2, 2, 1, -1, 2, 7, 7, 7], [1, 0] + [7] * 10, [-1, -1, -1, 0] + [-1] * 8]
     for moves in (ops.PagedMoves(x := new(4), x, new(1)), ops.PagedMoves(shares, new(4), new(1)),
                   ops.PagedMoves(new(4), shares, new(1)), ops.PagedMoves(new(4), new(4), start)):
         with pytest.raises(ops._lib.HipKernelError, match="overlap"):

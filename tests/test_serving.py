@@ -171,9 +171,12 @@ def test_fork_refuses_outputs_that_overlap_other_arrays(out, other):
 
 @pytest.mark.parametrize("changes", [
     dict(source=2 ** 20 + 2 * 2 ** 16 + 4 * 31), dict(target=2 ** 20 + 4 * 2 ** 16 + 4 * 49),
-    dict(lens_out=2 ** 20 + 2 ** 16 - 12), dict(counts_out=2 ** 20 + 12 * 2 ** 16 + 28)])
+    dict(lens_out=2 ** 20 + 2 ** 16 - 12), dict(counts_out=2 ** 20 + 12 * 2 ** 16 + 28),
+    dict(stride=20, source=2 ** 20 + 2 * 2 ** 16 + 4 * 17), dict(stride=12, source=2 ** 20 + 2 * 2 ** 16 + 4 * 9),
+    dict(stride=20, source=2 ** 20 + 2 * 2 ** 16 - 12), dict(stride=20, source=2 ** 20 + 2 * 2 ** 16 + 4 * 67)])
 def test_fork_refuses_outputs_that_overlap_other_arrays_in_part(changes):
-    # the last table entry, the last share, all but the first length, the last entry of the plan
+    # the last table entry, the last share, all but the first length, the last entry of the plan; of tables with other
+    # columns: the first entry of the second row behind those, and with too few, the first entry, the last
     _refused(_apart(_fork, FORK_IN + FORK_OUT, **changes), 1, "overlap")
 
 
