@@ -1912,10 +1912,10 @@ def paged_fork(
     cut the row there), the row gets a page of its own in its place, with the copy in ``source`` and ``target``, before
     tokens that are appended would become the others'. (The last holder that ends there keeps the page.)
     ``block_tables`` and ``shares`` are changed in place; lengths, counts and the list's start are in the result, whose
-    tensors ``step`` may give: these three also as the ones passed in, else in memory of their own. ``error`` (int32 ``[1]``) collects ``PAGED_ROW_HELD`` (the
-    row holds pages: left as it is), ``PAGED_BAD_ROW`` (no such parent: the same), ``PAGED_NO_PAGES`` (the free list
-    ran out: the row ends with its last full page) and ``PAGED_ROW_SHARED`` (nor was there a page for a row that ends
-    inside another's: it is as it was and must not be appended to).
+    tensors ``step`` may give: these three also as the ones passed in, else in memory of their own. ``error`` (int32
+    ``[1]``) collects ``PAGED_ROW_HELD`` (the row holds pages: left as it is), ``PAGED_BAD_ROW`` (no such parent: the
+    same), ``PAGED_NO_PAGES`` (the free list ran out: the row ends with its last full page) and ``PAGED_ROW_SHARED``
+    (nor was there a page for a row that ends inside another's: it is as it was and must not be appended to).
     """
 
     if step is None:
@@ -1968,8 +1968,8 @@ def paged_release(
     The others lose a holder each, and those left without one go to the places of ``free_pages`` before ``free_start``,
     downwards from it in ascending order of their numbers. ``shares`` and ``free_pages`` are changed in place, entries
     of ``block_tables`` past the new counts stay what they were; ``out`` gives the tensors of the result, which may be
-    the ones passed in. ``error`` (int32 ``[1]``) collects ``PAGED_BAD_SHARE`` (a page given back more often than held, in
-    this call or by one before: what ``free_pages[free_start:]`` holds already is not entered again) and
+    the ones passed in. ``error`` (int32 ``[1]``) collects ``PAGED_BAD_SHARE`` (a page given back more often than held,
+    in this call or by one before: what ``free_pages[free_start:]`` holds already is not entered again) and
     ``PAGED_LIST_FULL`` (no place before the list's first: the page is lost).
 
     A row that went on from another may be cut inside a page that it still shares. The next token's slot is in that
