@@ -123,6 +123,10 @@ SIGNATURES: dict[str, tuple] = {
     "aoto_hip_paged_tables": (
         _p, _p, _p, _i64, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _c_int, _p, _p, _p, _p, _p, _p, _p, _p,
     ),
+    "aoto_hip_paged_tables_shared": (
+        _p, _p, _p, _i64, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _p, _p, _p, _p, _p, _p, _p,
+        _p,
+    ),
     "aoto_hip_paged_rope_append": (
         _p, _i64, _p, _p, _p, _p, _c_int, _p, _p, _i64, _i64, _i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
         _p, _p, _p,

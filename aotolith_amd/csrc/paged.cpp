@@ -40,10 +40,23 @@ int aoto_hip_paged_tables(const int32_t* context_lens, const int32_t* new_lens, 
                           const int32_t* free_start, int requests, int max_blocks, int free_count, int page,
                           int max_tokens, int32_t* query_start, int32_t* kv_lens, int64_t* positions, int64_t* slots,
                           int32_t* page_counts_out, int32_t* free_start_out, int32_t* error, void* stream) {
+  return aoto_hip_paged_tables_shared(context_lens, new_lens, block_tables, table_stride, page_counts, free_pages,
+                                      free_start, nullptr, requests, max_blocks, free_count, 0, page, max_tokens,
+                                      query_start, kv_lens, positions, slots, page_counts_out, free_start_out, error,
+                                      stream);
+}
+
+int aoto_hip_paged_tables_shared(const int32_t* context_lens, const int32_t* new_lens, int32_t* block_tables,
+                                 int64_t table_stride, const int32_t* page_counts, const int32_t* free_pages,
+                                 const int32_t* free_start, const int32_t* shares, int requests, int max_blocks,
+                                 int free_count, int pages, int page, int max_tokens, int32_t* query_start,
+                                 int32_t* kv_lens, int64_t* positions, int64_t* slots, int32_t* page_counts_out,
+                                 int32_t* free_start_out, int32_t* error, void* stream) {
   if (!context_lens || !new_lens || !block_tables || !page_counts || (!free_pages && free_count) || !free_start ||
       !query_start || !kv_lens || ((!positions || !slots) && max_tokens) || !page_counts_out || !free_start_out)
     return set_error(AOTO_ERR_ARGUMENT, "paged_tables: null pointer");
-  if (requests <= 0 || max_blocks <= 0 || free_count < 0 || page <= 0 || max_tokens < 0 || table_stride < max_blocks)
+  if (requests <= 0 || max_blocks <= 0 || free_count < 0 || page <= 0 || max_tokens < 0 || table_stride < max_blocks ||
+      pages < (shares ? 1 : 0))
     return set_error(AOTO_ERR_ARGUMENT, "paged_tables: bad shape");
   if (max_blocks > (1 << 20) || page > (1 << 20) || max_tokens >= (1 << 30))
     return set_error(AOTO_ERR_UNSUPPORTED,
@@ -54,7 +67,7 @@ int aoto_hip_paged_tables(const int32_t* context_lens, const int32_t* new_lens, 
   a.positions = reinterpret_cast<long long*>(positions), a.slots = reinterpret_cast<long long*>(slots);
   a.page_counts_out = page_counts_out, a.free_start_out = free_start_out, a.error = error;
   a.table_stride = table_stride, a.requests = requests, a.max_blocks = max_blocks, a.free_count = free_count;
-  a.page = page, a.max_tokens = max_tokens;
+  a.page = page, a.max_tokens = max_tokens, a.shares = shares, a.pages = pages;
   const int fill = max_tokens <= kTablesFill;
   if (int s = launch("aoto_paged_tables", 1, 1, 1024, stream, a, fill)) return s;
   if (fill) return AOTO_OK;

@@ -24,6 +24,8 @@ struct PagedTablesArgs {
   int* error;
   long long table_stride;
   int requests, max_blocks, free_count, page, max_tokens;
+  const int* shares;  // of each of `pages` pages, holders beyond the first, or NULL: not looked at
+  int pages;
 };
 
 struct PagedAppendArgs {

@@ -42,6 +42,11 @@ AOTO_DEVICE int first_above(const int* sums, int n, int k) {
   return lo;
 }
 
+// Whether a token may not be written to a page because others read it there.
+AOTO_DEVICE bool page_of_others(const PagedTablesArgs& a, int page) {
+  return a.shares && (unsigned)page < (unsigned)a.pages && a.shares[page] > 0;
+}
+
 }  // namespace aoto
 
 // A step's pages, block tables and token maps from the requests' lengths (formulas at the entry point's declaration).
@@ -117,6 +122,7 @@ extern "C" __global__ __launch_bounds__(1024) void aoto_paged_tables(PagedTables
         int page = -1;
         if (block < s_count[i] + s_taken[i] - begin_taken)
           page = a.block_tables[(size_t)(base + i) * a.table_stride + block];
+        if (page_of_others(a, page)) page = -1, error |= AOTO_PAGED_ROW_SHARED;
         a.positions[offset + k] = position;
         a.slots[offset + k] = page < 0 ? -1 : (long long)page * a.page + (position - block * a.page);
       }
@@ -155,7 +161,11 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_slots(PagedTablesAr
       position = context + t - begin;
       const int block = position / a.page;
       const int page = block < count ? a.block_tables[(size_t)r * a.table_stride + block] : -1;
-      if (page >= 0) slot = (long long)page * a.page + (position - block * a.page);
+      if (aoto::page_of_others(a, page)) {
+        if (a.error) atomicOr(a.error, AOTO_PAGED_ROW_SHARED);
+      } else if (page >= 0) {
+        slot = (long long)page * a.page + (position - block * a.page);
+      }
     }
     a.positions[t] = position;
     a.slots[t] = slot;

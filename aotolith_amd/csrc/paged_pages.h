@@ -283,9 +283,9 @@ extern "C" __global__ __launch_bounds__(256) void aoto_paged_reclaim(PagedReleas
 
 // All of it by one block, which counts the holders that go in LDS: pools of up to kPagesFew pages. What bounds it is
 // one CU's reading, so it gains by its two launches fewer (2 to 3 us each where they are not captured) and only as long
-// as the GPU is hardly slower. In a graph, for entries of tables and pages of the pool: 512 and 600 5.5 us, 5.7 in three
-// launches, 2048 and 2500 6.7 and 6.3, 4096 and 4000 7.7 and 6.1; in an instance for 8192 pages 8192 and 8000 9.8 and
-// 6.6.
+// as the GPU is hardly slower. In a graph, for entries of tables and pages of the pool: 512 and 600 5.5 us and 5.7 in
+// three launches, 2048 and 2500 6.7 and 6.3, 4096 and 4000 7.7 and 6.1; in an instance for 8192 pages 8192 and 8000 9.8
+// and 6.6.
 extern "C" __global__ __launch_bounds__(1024) void aoto_paged_release_few(PagedReleaseArgs a) {
   using namespace aoto;
   constexpr uint32_t LISTED = 0x80000000u;

@@ -1285,6 +1285,7 @@ def paged_tables(
     *,
     page_size: int,
     max_tokens: int,
+    shares: torch.Tensor | None = None,
     step: PagedStep | None = None,
     error: torch.Tensor | None = None,
 ) -> PagedStep:
@@ -1301,7 +1302,9 @@ def paged_tables(
     ``step`` gives the tensors to write (a captured step replays into them); its ``page_counts`` and ``free_start``
     may be the ones passed in. ``error`` (int32 ``[1]``) collects ``PAGED_TOKENS_CUT`` (more tokens than
     ``max_tokens``: the last are left out), ``PAGED_NO_PAGES`` (the free list ran out: table entries and slots of -1)
-    and ``PAGED_TABLE_FULL`` (a request longer than its row: slots of -1).
+    and ``PAGED_TABLE_FULL`` (a request longer than its row: slots of -1). With ``shares`` (int32 ``[pages]``, where
+    rows go on from others by :func:`paged_fork`) also ``PAGED_ROW_SHARED``: a token's page is held by others too, whom
+    it would be written over (slots of -1).
     """
 
     _expect(context_lens, "context_lens", torch.int32)
@@ -1319,6 +1322,10 @@ def paged_tables(
         raise ValueError(f"block_tables must have {requests} rows, got {block_tables.shape[0]}")
     if error is not None:
         _expect_all(device, ((error, "error", torch.int32, (1,)),))
+    if shares is not None:
+        _expect_all(device, ((shares, "shares", torch.int32, None),))
+        if shares.dim() != 1 or not shares.numel():
+            raise ValueError(f"shares must be [pages], got {tuple(shares.shape)}")
     if max_tokens < 0:
         raise ValueError(f"max_tokens must not be negative, got {max_tokens}")
     if step is None:
@@ -1337,11 +1344,12 @@ def paged_tables(
         ))
     _ready(context_lens)
     _lib.check(
-        _lib.library().aoto_hip_paged_tables(
+        _lib.library().aoto_hip_paged_tables_shared(
             _ptr(context_lens), _ptr(new_lens), _ptr(block_tables), block_tables.stride(0), _ptr(page_counts),
-            _ptr(free_pages), _ptr(free_start), requests, block_tables.shape[1], free_pages.numel(), int(page_size),
-            max_tokens, _ptr(step.query_start), _ptr(step.kv_lens), _ptr(step.positions), _ptr(step.slots),
-            _ptr(step.page_counts), _ptr(step.free_start), _ptr(error), _stream(device),
+            _ptr(free_pages), _ptr(free_start), _ptr(shares), requests, block_tables.shape[1], free_pages.numel(),
+            0 if shares is None else shares.numel(), int(page_size), max_tokens, _ptr(step.query_start),
+            _ptr(step.kv_lens), _ptr(step.positions), _ptr(step.slots), _ptr(step.page_counts), _ptr(step.free_start),
+            _ptr(error), _stream(device),
         )
     )
     return step
@@ -1974,7 +1982,8 @@ def paged_release(
 
     A row that went on from another may be cut inside a page that it still shares. The next token's slot is in that
     page, over the others' tokens: :func:`paged_fork` (with ``parents`` of -1 where no row goes on) and its copy come
-    before the step's :func:`paged_tables`, and give the row a page of its own.
+    before the step's :func:`paged_tables`, and give the row a page of its own. (With ``shares``, that call leaves such
+    tokens out and says so.)
     """
 
     if out is None:

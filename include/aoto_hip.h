@@ -607,7 +607,7 @@ int aoto_hip_generic_attention(const aoto_tensor* out, const aoto_tensor* q, con
 #define AOTO_PAGED_BAD_ROW 64     /* a parent past the last request: left as it was */
 #define AOTO_PAGED_BAD_SHARE 128  /* a page given back more often than held, or both held and free, or listed twice */
 #define AOTO_PAGED_LIST_FULL 256  /* no place before the free list's first: the page is lost */
-#define AOTO_PAGED_ROW_SHARED 512 /* no page for a row that ends inside one that others hold: not to be appended to */
+#define AOTO_PAGED_ROW_SHARED 512 /* a token whose page others hold, left out; or no page of its own for such a row */
 
 /* A step's pages, block tables and token maps from the requests' lengths. Request r has context_lens[r] cached tokens
  * (negative ones count as 0, ones past 2^30 as 2^30) and gets new_lens[r] more (negative: 0); its row of block_tables
@@ -732,6 +732,16 @@ int aoto_hip_paged_attention_mx4(const void* q, int64_t q_token_stride, int64_t 
  * named *_out may be the arrays they are computed from; else outputs overlap no other array (aoto_hip_paged_fork and
  * _compact refuse it). Everything is the same at every run, whatever the threads' order. */
 
+/* aoto_hip_paged_tables where rows share pages (shares of `pages` pages; NULL: not looked at): a token whose page
+ * others hold too has slot -1, and raises AOTO_PAGED_ROW_SHARED. Its row was cut there and needs aoto_hip_paged_fork
+ * first. */
+int aoto_hip_paged_tables_shared(const int32_t* context_lens, const int32_t* new_lens, int32_t* block_tables,
+                                 int64_t table_stride, const int32_t* page_counts, const int32_t* free_pages,
+                                 const int32_t* free_start, const int32_t* shares, int requests, int max_blocks,
+                                 int free_count, int pages, int page, int max_tokens, int32_t* query_start,
+                                 int32_t* kv_lens, int64_t* positions, int64_t* slots, int32_t* page_counts_out,
+                                 int32_t* free_start_out, int32_t* error, void* stream);
+
 /* Requests that go on from another: row r with parents[r] >= 0, which must hold no pages, gets the first
  * ceil(n / page) pages of row parents[r], n = min(context_lens, page_counts * page) of that row as it was before the
  * call: full pages themselves (shares + 1), one in progress as the next page of the free list, rows in order, with
@@ -752,7 +762,8 @@ int aoto_hip_paged_fork(const int32_t* parents, const int32_t* context_lens, int
  * to free_pages[free_start - 1], [free_start - 2], ... in ascending order of their numbers, but for those that
  * free_pages[free_start .. free_count) holds (given back before: AOTO_PAGED_BAD_SHARE). A row may end inside a page
  * that others hold too, where the next token's slot would be theirs: aoto_hip_paged_fork, called before that token's
- * aoto_hip_paged_tables, gives the row a page of its own. shares are below 2^27. scratch: pages / 1024 + 2 entries. */
+ * aoto_hip_paged_tables, gives the row a page of its own, and aoto_hip_paged_tables_shared leaves out what is not asked
+ * for so. shares are below 2^27. scratch: pages / 1024 + 2 entries. */
 int aoto_hip_paged_release(const int32_t* keep_lens, const int32_t* block_tables, int64_t table_stride,
                            const int32_t* page_counts, int32_t* shares, int32_t* free_pages,
                            const int32_t* free_start, int requests, int max_blocks, int free_count, int pages,

@@ -482,7 +482,8 @@ def _nearer_bound(s, want, size):
                 score = dim ** -0.5 * products.sum(-1)
                 p = np.exp(score - score.max())
                 p /= p.sum()
-                off = dim ** -0.5 * 8 * 2.0 ** -13 * (1 + 2.0 ** -5) * np.abs(products).reshape(n, -1, 8).max(-1).sum(-1)
+                most = np.abs(products).reshape(n, -1, 8).max(-1).sum(-1)
+                off = dim ** -0.5 * 8 * 2.0 ** -13 * (1 + 2.0 ** -5) * most
                 pm = p * np.expm1(off)
                 assert pm.sum() < 0.5
                 more[t, h] = (pm @ np.abs(v[:n, h * hkv // heads]) + pm.sum() * np.abs(want[t, h])) / (1 - pm.sum())
@@ -1534,7 +1535,7 @@ def test_a_row_cut_inside_a_shared_page_leaves_the_others_tokens():
     def step(new):
         nonlocal counts, start
         s = ops.paged_tables(_i32(context), _i32(new), tables, counts, free, start, page_size=page,
-                             max_tokens=sum(new), error=error)
+                             max_tokens=sum(new), shares=shares, error=error)
         counts, start = s.page_counts, s.free_start
         x = bf16_normal(rng, (sum(new), 3 * hkv * dim))
         args = (to_gpu_bf16(x), s.positions, s.slots, ones, torch.zeros_like(ones))
@@ -1573,6 +1574,11 @@ def test_a_row_cut_inside_a_shared_page_leaves_the_others_tokens():
     del texts[2][20:]
     counts, start = ops.paged_release(_i32([-1, -1, 20]), tables, counts, shares, free, start, page_size=page,
                                       error=error)
+    # a step that asks before the row has a page of its own is told so
+    told = torch.zeros(1, dtype=torch.int32, device="cuda")
+    s = ops.paged_tables(_i32(context), _i32([1, 0, 1]), tables.clone(), counts, free, start, page_size=page,
+                         max_tokens=2, shares=shares, error=told)
+    assert int(told) == ops.PAGED_ROW_SHARED and s.slots[1] == -1 and s.slots[0] >= 0
     own_pages([-1] * rows)
     for new in ([1, 1, 1], [0, 2, 30], [3, 0, 1]):
         step(new)
@@ -1620,8 +1626,9 @@ def test_a_captured_step_keeps_every_rows_text(pages_before_the_pool_moves):
     texts = [[] for _ in range(rows)]
     for r, n in ((0, 70), (3, 33)):                     # prompts
         x = bf16_normal(rng, (n, (hq + 2 * hkv) * dim))
-        s = ops.paged_tables(_i32([0] * rows), _i32([n if i == r else 0 for i in range(rows)]), d["tables"], d["counts"],
-                             d["free"], d["start"], page_size=page, max_tokens=n, error=d["error"])
+        new = _i32([n if i == r else 0 for i in range(rows)])
+        s = ops.paged_tables(_i32([0] * rows), new, d["tables"], d["counts"], d["free"], d["start"], page_size=page,
+                             max_tokens=n, error=d["error"])
         ops.paged_rope_append_mx4(to_gpu_bf16(x), s.positions, s.slots, ones, zeros, cache, query_heads=hq)
         d["counts"].copy_(s.page_counts)
         d["start"].copy_(s.free_start)
@@ -1674,6 +1681,47 @@ def test_a_captured_step_keeps_every_rows_text(pages_before_the_pool_moves):
         got = from_gpu_bf16(out).astype(np.float64)[:at]
         assert (np.abs(got - want) <= _bound(state, want, size))[written].all()
     assert cuts > 0
+
+
+@pytest.mark.parametrize("tokens", [1, 9, 700])         # the maps in one launch, in a second
+@pytest.mark.parametrize("requests", [4, 40, 1100])
+def test_tables_leave_out_tokens_of_pages_that_others_hold(requests, tokens):
+    rng = np.random.default_rng(requests + tokens)
+    page, lens = 16, rng.integers(0, 200, requests)
+    tables, counts, shares, free, start = _pool(rng, lens, page, spare=requests * 50, share=0.7, blocks=60)
+    cut = np.where(rng.random(requests) < 0.5, rng.integers(0, lens + 1), lens)
+    new = rng.integers(0, tokens + 1, requests)
+    most = int(new.sum()) + 3
+    want = paged_oracle.tables(cut, new, tables, counts, free, start[0], page, most)
+    slots = want[3].copy()
+    theirs = (slots >= 0) & (shares[np.maximum(slots, 0) // page] > 0)
+    assert theirs.any() or requests == 4
+    slots[theirs] = -1
+    ops = _ops()
+    for given in (shares, None, shares[:5]):
+        device, error = _strided(tables), torch.zeros(1, dtype=torch.int32, device="cuda")
+        got = ops.paged_tables(_i32(cut), _i32(new), device, _i32(counts), _i32(free), _i32(start), page_size=page,
+                               max_tokens=most, shares=None if given is None else _i32(given), error=error)
+        if given is shares:
+            np.testing.assert_array_equal(_np(got.slots), slots)
+            assert int(error) == (want[7] | (512 if theirs.any() else 0))
+        elif given is None:
+            np.testing.assert_array_equal(_np(got.slots), want[3])
+            assert int(error) == want[7]
+        else:                                             # pages past the shares are not looked at
+            few = theirs & (want[3] // page < 5)
+            np.testing.assert_array_equal(_np(got.slots), np.where(few, -1, want[3]))
+        for a, b in zip((got.query_start, got.kv_lens, got.positions, device, got.page_counts, got.free_start),
+                        (*want[:3], *want[4:7])):
+            np.testing.assert_array_equal(_np(a), b)
+
+
+def test_tables_refuse_shares_that_are_none():
+    ops, one = _ops(), _i32([1])
+    for shares, error in ((_i32([]), ValueError), (_i32([[0, 0]]), ValueError),
+                          (torch.zeros(3, device="cuda"), TypeError), (torch.zeros(3, dtype=torch.int32), ValueError)):
+        with pytest.raises(error):
+            ops.paged_tables(one, one, _i32([[0]]), one, one, _i32([0]), page_size=16, max_tokens=1, shares=shares)
 
 
 # ---------------------------------------------------------------- arrays given twice

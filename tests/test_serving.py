@@ -120,6 +120,23 @@ def test_fork_refuses(changes, code):
     _refused(_fork(**changes), code, "paged_fork")
 
 
+def _tables(**changes):
+    a = dict(lens=GOOD, new=GOOD, tables=GOOD, stride=8, counts=GOOD, free=GOOD, start=GOOD, shares=GOOD, requests=2,
+             blocks=8, count=10, pages=10, page=16, most=4, query=GOOD, kv=GOOD, positions=GOOD, slots=GOOD,
+             counts_out=GOOD, start_out=GOOD) | changes
+    return _lib.library().aoto_hip_paged_tables_shared(*a.values(), None, None)
+
+
+@pytest.mark.parametrize("changes,code", [
+    *[({name: None}, 1) for name in ("lens", "new", "tables", "counts", "free", "start", "query", "kv", "positions",
+                                     "slots", "counts_out", "start_out")],
+    (dict(pages=0), 1), (dict(shares=None, pages=-1), 1), (dict(requests=0), 1), (dict(blocks=0), 1),
+    (dict(count=-1), 1), (dict(page=0), 1), (dict(most=-1), 1), (dict(stride=7), 1),
+    (dict(blocks=2 ** 20 + 1, stride=2 ** 21), 4), (dict(page=2 ** 20 + 1), 4), (dict(most=2 ** 30), 4)])
+def test_tables_of_shared_pages_refuse(changes, code):
+    _refused(_tables(**changes), code, "paged_tables")
+
+
 def _release(**changes):
     a = dict(keep=GOOD, tables=GOOD, stride=8, counts=GOOD, shares=GOOD, free=GOOD, start=GOOD, requests=4, blocks=8,
              count=100, pages=50, page=16, counts_out=GOOD, start_out=GOOD, scratch=GOOD) | changes
